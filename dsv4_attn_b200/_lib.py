@@ -68,7 +68,9 @@ EXPORTS = ("dsv4_attn_version", "dsv4_debug_set_wait", "dsv4_debug_set_flags", "
            "dsv4_noalloc_scratch_bytes", "dsv4_attn_last_error", "dsv4_csa_compress_reduce_fwd",
            "dsv4_hca_dense_decode_fwd", "dsv4_hca_dense_decode_simt", "dsv4_attn_combine", "dsv4_attn_plan_splits",
            "dsv4_attn_workspace_bytes", "hca_decode_fwd", "dsv4_hca_compress_fwd", "dsv4_kv_quantize_insert",
-           "dsv4_hca_packed_decode_fwd", "dsv4_rope_norm_fwd", "dsv4_indexer_topk_fwd")
+           "dsv4_hca_packed_decode_fwd", "dsv4_rope_norm_fwd", "dsv4_indexer_topk_fwd",
+           "dsv4_hca_tree_decode_fwd", "dsv4_kv_pages_copy", "dsv4_kv_pages_fork", "dsv4_kv_pages_free", "dsv4_kv_pages_compact", "dsv4_kv_entries_move",
+           "dsv4_sample_fwd")
 
 
 class CsaCompressReduceParams(C.Structure):
@@ -132,6 +134,37 @@ class KvQuantizeInsertParams(C.Structure):
     ]
 
 
+# include/dsv4_speculative.h
+class HcaTreeDecodeParams(C.Structure):
+    _fields_ = [
+        ("B", C.c_int32), ("T", C.c_int32), ("H", C.c_int32), ("max_pages", C.c_int32), ("win_cap", C.c_int32),
+        ("mask_words", C.c_int32), ("num_splits", C.c_int32), ("sm_scale", C.c_float), ("make_plan", C.c_int32),
+        ("reserved0", C.c_int32), ("num_pages", C.c_int64),
+        ("q", C.c_void_p), ("kv_pool", C.c_void_p), ("block_table", C.c_void_p), ("kv_len", C.c_void_p),
+        ("win_pool", C.c_void_p), ("win_len", C.c_void_p), ("tree_mask", C.c_void_p), ("attn_sink", C.c_void_p),
+        ("out", C.c_void_p), ("lse", C.c_void_p), ("partial_o", C.c_void_p), ("partial_lse", C.c_void_p),
+        ("status", C.c_void_p), ("sched", C.c_void_p), ("sched_bytes", C.c_int64),
+    ]
+
+
+class KvPagesParams(C.Structure):
+    _fields_ = [
+        ("pool", C.c_void_p), ("num_pages", C.c_int64), ("layers", C.c_int64), ("entries", C.c_int64),
+        ("B", C.c_int32), ("max_pages", C.c_int32), ("n", C.c_int32), ("reserved0", C.c_int32),
+        ("src", C.c_void_p), ("dst", C.c_void_p), ("block_table", C.c_void_p), ("kv_len", C.c_void_p),
+        ("refs", C.c_void_p), ("new_table", C.c_void_p), ("new_refs", C.c_void_p), ("count", C.c_void_p),
+        ("scratch", C.c_void_p), ("status", C.c_void_p),
+    ]
+
+
+class SampleParams(C.Structure):
+    _fields_ = [
+        ("N", C.c_int32), ("V", C.c_int32), ("dtype", C.c_int32), ("reserved0", C.c_int32), ("stride_n", C.c_int64),
+        ("logits", C.c_void_p), ("u", C.c_void_p), ("temperature", C.c_void_p), ("top_k", C.c_void_p),
+        ("top_p", C.c_void_p), ("min_p", C.c_void_p), ("token", C.c_void_p), ("logprob", C.c_void_p),
+    ]
+
+
 def _load() -> C.CDLL:
     path = library_path()
     if not path.exists():
@@ -157,7 +190,14 @@ def _load() -> C.CDLL:
                      ("dsv4_hca_packed_decode_fwd", HcaPackedDecodeParams),
                      ("dsv4_kv_quantize_insert", KvQuantizeInsertParams),
                      ("dsv4_attn_plan", PlanParams),
-                     ("dsv4_attn_combine", CombineParams)):
+                     ("dsv4_attn_combine", CombineParams),
+                     ("dsv4_hca_tree_decode_fwd", HcaTreeDecodeParams),
+                     ("dsv4_kv_pages_copy", KvPagesParams),
+                     ("dsv4_kv_pages_fork", KvPagesParams),
+                     ("dsv4_kv_pages_free", KvPagesParams),
+                     ("dsv4_kv_pages_compact", KvPagesParams),
+                     ("dsv4_kv_entries_move", KvPagesParams),
+                     ("dsv4_sample_fwd", SampleParams)):
         fn = getattr(lib, name)
         fn.restype = C.c_int
         fn.argtypes = [P(st), C.c_void_p]

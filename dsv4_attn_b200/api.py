@@ -60,7 +60,9 @@ def _rc(rc: int, what: str) -> None:
 ENTRY_POINTS = (
     "dsv4_csa_sparse_decode_fwd", "dsv4_hca_dense_decode_fwd", "dsv4_hca_packed_decode_fwd", "hca_decode_fwd", "dsv4_rope_norm_fwd",
     "dsv4_kv_quantize_insert", "dsv4_csa_compress_reduce_fwd", "dsv4_hca_compress_fwd", "dsv4_indexer_topk_fwd", "dsv4_attn_combine",
-    "dsv4_attn_plan", "dsv4_attn_plan_splits")
+    "dsv4_attn_plan", "dsv4_attn_plan_splits",
+    "dsv4_hca_tree_decode_fwd", "dsv4_attn_sched_bytes", "dsv4_kv_pages_copy", "dsv4_kv_pages_fork", "dsv4_kv_pages_free", "dsv4_kv_pages_compact",
+    "dsv4_kv_entries_move", "dsv4_sample_fwd")
 _host.bind(*(C.cast(getattr(_lib.LIB, name), C.c_void_p).value for name in ENTRY_POINTS))
 
 
@@ -585,3 +587,185 @@ def indexer_topk(q_fp8, q_weight, key_pages, block_table, n_vis, k, *, scores=No
                                status=_ptr(status))
     _rc(_lib.LIB.dsv4_indexer_topk_fwd(C.byref(p), _stream(q_fp8.device)), "dsv4_indexer_topk_fwd")
     return out, scores
+
+
+# ── a speculative step (include/dsv4_speculative.h) ──
+def hca_tree_decode(q, kv_pool, block_table, kv_len, win_pool, win_len, tree_mask, sm_scale, *, attn_sink=None, num_splits=None,
+                    out=None, lse=None, workspace=None, status=None, max_len=None, plan=None):
+    """HCA decode of the T drafted nodes of a tree per request, in one call: every node attends to the request's
+    compressed entries [0, kv_len[b]) and to the rows of its window buffer that the node's mask names.
+    q bf16 [B, T, H, 576]; kv_pool uint8 [P, 64, 656]; block_table int32 [B, max_pages]; kv_len / win_len int32 [B];
+    win_pool uint8 [B, W, 656] (committed tokens and drafts); tree_mask int32 [B, T, words], bit w % 32 of word w // 32:
+    the node sees window row w (`layout.pack_tree_mask`).  Returns (out bf16 [B, T, H, 512], lse f32 [B, T, H]).
+
+    `num_splits` None: where the nodes fill the device more than once the call plans the work on the device
+    (as `plan_hca(B, 1, T * H, kv_len[:, None], win_len[:, None])` does, which can be passed as `plan` to all layers
+    of a step instead); otherwise rows are split so that it is full."""
+    r = _host.tree(q, kv_pool, block_table, kv_len, win_pool, win_len, tree_mask, sm_scale, attn_sink, num_splits, out, lse, workspace, status, max_len,
+                   None if plan is None else plan.fast)
+    if r is not None:
+        return r if type(r) is tuple else _rc(r, "dsv4_hca_tree_decode_fwd")
+    _cuda_contig(q, "q", torch.bfloat16, 4)
+    B, T, H, dq = q.shape
+    _check(dq == D_QK, f"q last dim must be {D_QK}")
+    _cuda_contig(kv_pool, "kv_pool", torch.uint8, 3)
+    _check(kv_pool.shape[1] == PAGE_ENTRIES and kv_pool.shape[2] == ENTRY_BYTES, f"kv_pool must be [num_pages, {PAGE_ENTRIES}, {ENTRY_BYTES}]")
+    _cuda_contig(block_table, "block_table", torch.int32, 2)
+    _check(block_table.shape[0] == B, "block_table must be [B, max_pages]")
+    for name, t in (("kv_len", kv_len), ("win_len", win_len)):
+        _cuda_contig(t, name, torch.int32, 1)
+        _check(t.shape[0] == B, f"{name} must be [B]")
+    _cuda_contig(win_pool, "win_pool", torch.uint8, 3)
+    _check(win_pool.shape[0] == B and win_pool.shape[2] == ENTRY_BYTES, f"win_pool must be [B, W, {ENTRY_BYTES}]")
+    _cuda_contig(tree_mask, "tree_mask", torch.int32, 3)
+    _check(tuple(tree_mask.shape[:2]) == (B, T), "tree_mask must be [B, T, words]")
+    if attn_sink is not None:
+        _cuda_contig(attn_sink, "attn_sink", torch.float32, 1)
+        _check(attn_sink.shape[0] == H, "attn_sink must be [H]")
+    if out is not None:
+        _cuda_contig(out, "out", torch.bfloat16, 4)
+        _check(tuple(out.shape) == (B, T, H, D_LATENT), "out must be [B, T, H, 512]")
+    if lse is not None:
+        _cuda_contig(lse, "lse", torch.float32, 3)
+        _check(tuple(lse.shape) == (B, T, H), "lse must be [B, T, H]")
+    _check(num_splits is None or 1 <= num_splits <= MAX_SPLITS, f"num_splits must be in [1, {MAX_SPLITS}]")
+    if plan is not None:
+        _check((plan.kind, plan.B, plan.s_q, plan.H) == (1, B, 1, T * H), "plan was made for another batch shape")
+    _check(B > 0 and T > 0 and H > 0 and block_table.shape[1] > 0 and kv_pool.shape[0] > 0, "empty batch, table or pool")
+    if workspace is not None:
+        po, pl = workspace
+        _cuda_contig(po, "partial_o", torch.float32)
+        _cuda_contig(pl, "partial_lse", torch.float32)
+        _check(num_splits is not None and po.numel() >= num_splits * B * T * H * D_LATENT and pl.numel() >= num_splits * B * T * H,
+               "workspace needs num_splits, and room for that many")
+    raise Dsv4Error("dsv4_hca_tree_decode_fwd refused the call (sizes out of range, or no device memory)")
+
+
+def sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None, out=None, logprob=None):
+    """Tokens drawn from logits [N, V] (f32, bf16 or f16; rows may be any distance apart) with the random numbers u f32 [N] in [0, 1):
+    temperature f32 [N], top_k int32 [N], top_p f32 [N] and min_p f32 [N], each optional, filter in this order (see
+    Dsv4SampleParams).  Returns (token int32 [N], logprob f32 [N] of the token under what it was drawn from).  A token depends on
+    its row alone, not on the batch; a row without a finite logit gives -1."""
+    r = _host.sample(logits, u, temperature, top_k, top_p, min_p, out, logprob)
+    if r is not None:
+        return r if type(r) is tuple else _rc(r, "dsv4_sample_fwd")
+    _check(isinstance(logits, torch.Tensor) and logits.is_cuda and logits.dim() == 2, "logits must be a cuda tensor [N, V]")
+    _check(logits.dtype in (torch.float32, torch.bfloat16, torch.float16), f"logits must be f32, bf16 or f16, got {logits.dtype}")
+    N, V = logits.shape
+    _check(0 < V <= 1 << 22, "V must be in [1, 2^22]")
+    _check(V == 1 or logits.stride(1) == 1, "the logits of a row must be contiguous")
+    _check(N <= 1 or logits.stride(0) >= V, "the rows of logits must not overlap")
+    for name, t, dtype in (("u", u, torch.float32), ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32),
+                           ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32), ("out", out, torch.int32), ("logprob", logprob, torch.float32)):
+        if t is None and name != "u":
+            continue
+        _cuda_contig(t, name, dtype, 1)
+        _check(t.shape[0] == N, f"{name} must be [N]")
+    raise Dsv4Error("dsv4_sample_fwd refused the call (sizes out of range, or no device memory)")
+
+
+def _pages_pool(kv_pool):
+    _check(isinstance(kv_pool, torch.Tensor) and kv_pool.dim() in (3, 4), f"kv_pool must be [pages, {PAGE_ENTRIES}, {ENTRY_BYTES}] or [layers, pages, {PAGE_ENTRIES}, {ENTRY_BYTES}]")
+    _cuda_contig(kv_pool, "kv_pool", torch.uint8)
+    _check(kv_pool.shape[-2] == PAGE_ENTRIES and kv_pool.shape[-1] == ENTRY_BYTES and kv_pool.numel() > 0,
+           f"kv_pool must be [pages, {PAGE_ENTRIES}, {ENTRY_BYTES}] or [layers, pages, {PAGE_ENTRIES}, {ENTRY_BYTES}]")
+
+
+def _pages_tables(block_table, kv_len, page_refs, num_pages=None):
+    _cuda_contig(block_table, "block_table", torch.int32, 2)
+    _check(block_table.numel() > 0, "block_table must not be empty")
+    if kv_len is not None:
+        _cuda_contig(kv_len, "kv_len", torch.int32, 1)
+        _check(kv_len.shape[0] == block_table.shape[0], "kv_len must have one value per row of block_table")
+    _cuda_contig(page_refs, "page_refs", torch.int32, 1)
+    _check(page_refs.shape[0] == num_pages if num_pages is not None else page_refs.shape[0] > 0, "page_refs must have one value per page")
+
+
+def _pages_items(**lists):
+    for name, t in lists.items():
+        _cuda_contig(t, name, torch.int32, 1)
+    _check(len({t.shape[0] for t in lists.values()}) == 1, f"{' and '.join(lists)} must have the same length")
+
+
+def _pages_status(status):
+    if status is not None:
+        _cuda_contig(status, "status", torch.int32, 1)
+        _check(status.numel() >= 4, "status must hold 4 int32")
+
+
+def _pages_done(r, what):
+    _check(r is not None, f"{what}: sizes out of range, or no device memory")
+    if r != 0:
+        _rc(r, what)
+
+
+def kv_pages_copy(kv_pool, src, dst, *, status=None) -> None:
+    """Page src[i] to page dst[i] (int32, negative: left out) in every layer of kv_pool uint8 [pages, 64, 656] or
+    [layers, pages, 64, 656].  No page is named twice among dst, nor in both lists."""
+    r = _host.pages_copy(kv_pool, src, dst, status)
+    if r is None:
+        _pages_pool(kv_pool)
+        _pages_items(src=src, dst=dst)
+        _pages_status(status)
+    _pages_done(r, "dsv4_kv_pages_copy")
+
+
+def kv_entries_move(pool, src, dst, *, status=None) -> None:
+    """Entry src[i] to entry dst[i] (int32, negative: left out) in every layer.  pool uint8 [layers, rows, n, 656] or [rows, n, 656]
+    (a window buffer, or a cache by pages); entry numbers count through a layer: row * n + place.  Accepted drafts to their places.
+    No entry is named twice among dst, nor in both lists."""
+    r = _host.entries_move(pool, src, dst, status)
+    if r is None:
+        _check(isinstance(pool, torch.Tensor) and pool.dim() in (3, 4), f"pool must be [rows, n, {ENTRY_BYTES}] or [layers, rows, n, {ENTRY_BYTES}]")
+        _cuda_contig(pool, "pool", torch.uint8)
+        _check(pool.shape[-1] == ENTRY_BYTES and pool.numel() > 0, f"pool must be [rows, n, {ENTRY_BYTES}] or [layers, rows, n, {ENTRY_BYTES}]")
+        _pages_items(src=src, dst=dst)
+        _pages_status(status)
+    _pages_done(r, "dsv4_kv_entries_move")
+
+
+def kv_pages_free(block_table, kv_len, page_refs, requests, *, status=None) -> None:
+    """The pages of `requests` (int32, distinct rows of block_table, negative: left out) are given back, in place: one reference
+    less each in page_refs int32 [pages], table rows -1, lengths 0.  A page whose count is 0 is free."""
+    r = _host.pages_free(block_table, kv_len, page_refs, requests, status)
+    if r is None:
+        _pages_tables(block_table, kv_len, page_refs)
+        _pages_items(requests=requests)
+        _pages_status(status)
+    _pages_done(r, "dsv4_kv_pages_free")
+
+
+def kv_pages_fork(kv_pool, block_table, kv_len, page_refs, parent, child, *, status=None) -> None:
+    """Request child[i] becomes a copy of request parent[i], in place: it shares the parent's full pages and gets a page of its own (free pages in
+    ascending order) with a copy of the entries of a partly filled last one, in every layer of kv_pool.  What a child held must
+    have been freed (`kv_pages_free`).  Children are distinct and no child is a parent.  Without a free page left the child
+    has the full pages only, and status says 10."""
+    r = _host.pages_fork(kv_pool, block_table, kv_len, page_refs, parent, child, status)
+    if r is None:
+        _pages_pool(kv_pool)
+        _pages_tables(block_table, kv_len, page_refs, kv_pool.shape[-3])
+        _pages_items(parent=parent, child=child)
+        _pages_status(status)
+    _pages_done(r, "dsv4_kv_pages_fork")
+
+
+def kv_pages_compact(kv_pool, block_table, page_refs, *, new_table=None, new_refs=None, count=None, workspace=None, status=None):
+    """Live pages move to the front of the pool (every layer), as few as possible: with `count` of them the k-th live page from number `count` on
+    goes to the k-th free page below it.  Returns (block_table, page_refs, count int32 [1]) as they are afterwards; the tensors passed in are left as
+    they were unless they are passed as new_table / new_refs too.  workspace: int32 [3 * pages + 1]."""
+    r = _host.pages_compact(kv_pool, block_table, page_refs, new_table, new_refs, count, workspace, status)
+    if r is None:
+        _pages_pool(kv_pool)
+        pages = kv_pool.shape[-3]
+        _pages_tables(block_table, None, page_refs, pages)
+        for name, t, shape in (("new_table", new_table, block_table.shape), ("new_refs", new_refs, page_refs.shape), ("count", count, (1,))):
+            if t is not None:
+                _cuda_contig(t, name, torch.int32, len(shape))
+                _check(tuple(t.shape) == tuple(shape), f"{name} must be {list(shape)}")
+        if workspace is not None:
+            _cuda_contig(workspace, "workspace", torch.int32, 1)
+            _check(workspace.numel() >= 3 * pages + 1, "workspace must hold 3 * pages + 1 int32")
+        _pages_status(status)
+    if type(r) is tuple:
+        return r
+    _pages_done(r, "dsv4_kv_pages_compact")

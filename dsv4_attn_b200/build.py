@@ -23,8 +23,9 @@ HERE = Path(__file__).resolve().parent
 SOURCE = HERE / "csrc" / "api.cu"
 OUT = HERE / "libdsv4_attn.so"
 HEADER = HERE.parent / "include" / "dsv4_attn.h"
+HEADERS = (HEADER, HEADER.with_name("dsv4_speculative.h"))
 HOST_SOURCE = HERE / "csrc" / "host.cpp"
-DEPS = [p for p in sorted((HERE / "csrc").glob("*")) if p != HOST_SOURCE] + [HEADER]
+DEPS = [p for p in sorted((HERE / "csrc").glob("*")) if p != HOST_SOURCE] + list(HEADERS)
 
 
 def needs_build(out: Path = OUT, deps=tuple(DEPS)) -> bool:
@@ -42,7 +43,7 @@ def host_path() -> Path:
 
 def build_host(force: bool = False, quiet: bool = False) -> Path:
     out = host_path()
-    if not force and not needs_build(out, (HOST_SOURCE, HEADER)):
+    if not force and not needs_build(out, (HOST_SOURCE, *HEADERS)):
         return out
     import sysconfig
 

@@ -4,6 +4,7 @@
 // the entry point that allocates nothing (all written once, atomically), each thread's RoPE frequencies of the theta it used
 // last, and the test switches of dsv4_debug_set_flags / dsv4_debug_set_wait, which are read once per call.
 #include "../../include/dsv4_attn.h"
+#include "../../include/dsv4_speculative.h"
 
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -19,6 +20,8 @@
 #include "decode_kernel.cuh"
 #include "sched.cuh"
 #include "decode_simt.cuh"
+#include "kv_pages.cuh"
+#include "sample.cuh"
 
 namespace dsv4 {
 namespace {
@@ -180,18 +183,29 @@ int64_t sched_slot_cap(int n_units, int num_splits, int num_pairs) {
 // wait before they touch memory, see ptx.cuh): in a chain of small kernels the launch and set-up of each - 2 to 3 us when a
 // kernel takes 4 to 10 - then lie under the tail of the one before.  A preceding kernel that never triggers makes it an
 // ordinary launch.
+// `cluster`: blocks per cluster where the launch decides on them.
 template <class Args>
-cudaError_t launch(void (*kernel)(Args), dim3 grid, int threads, size_t smem, cudaStream_t stream, const Args& args) {
+cudaError_t launch(void (*kernel)(Args), dim3 grid, int threads, size_t smem, cudaStream_t stream, const Args& args, int cluster = 0) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = (g_dbg.load(std::memory_order_relaxed) & 64) ? 0 : 1;
+    cudaLaunchAttribute attr[2] = {};
+    unsigned used = 0;
+    if (cluster > 0) {
+        attr[used].id = cudaLaunchAttributeClusterDimension;
+        attr[used].val.clusterDim.x = unsigned(cluster);
+        attr[used].val.clusterDim.y = attr[used].val.clusterDim.z = 1;
+        ++used;
+    }
+    if (!(g_dbg.load(std::memory_order_relaxed) & 64)) {
+        attr[used].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[used].val.programmaticStreamSerializationAllowed = 1;
+        ++used;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = used;
     return cudaLaunchKernelEx(&cfg, kernel, args);
 }
 
@@ -242,9 +256,9 @@ cudaError_t launch_combine(const CombineArgs& c, cudaStream_t stream) {
     // plan cut.  Below that a warp looks its unit up and is done sooner than a block has gathered the cut units.
     const int64_t resident = int64_t(device_sms()) * 4;
     if (c.unit_nsplits != nullptr && int64_t(c.N) * c.H > resident * kCombineWarps)
-        return launch(combine_sched_kernel, dim3(unsigned(resident)), kCombineWarps * 32, 0, stream, c);
+        return launch(c.half ? combine_sched_kernel<true> : combine_sched_kernel<false>, dim3(unsigned(resident)), kCombineWarps * 32, 0, stream, c);
     const int64_t units = int64_t(c.N) * c.H;
-    return launch(combine_kernel, dim3(unsigned((units + kCombineWarps - 1) / kCombineWarps)), kCombineWarps * 32, 0, stream, c);
+    return launch(c.half ? combine_kernel<true> : combine_kernel<false>, dim3(unsigned((units + kCombineWarps - 1) / kCombineWarps)), kCombineWarps * 32, 0, stream, c);
 }
 
 CombineArgs contiguous_combine(int rows, int H, int S, const float* po, const float* pl, void* out, float* lse,
@@ -365,10 +379,14 @@ int decode_fwd(DecodeArgs& a, const void* sched, cudaStream_t stream) {
         c.unit_nsplits = static_cast<const int32_t*>(sched) + l.unit_nsplits;
         c.unit_slot = static_cast<const int32_t*>(sched) + l.unit_slot;
         c.hgs = hgs;
+        c.sink_heads = a.tree_heads;
+        c.half = half_partials(SRC);
         e = launch_combine(c, stream);
     } else if (a.num_splits > 1) {
         CombineArgs c = contiguous_combine(rows, a.H, a.num_splits, a.partial_o, a.partial_lse, a.out, a.lse, a.attn_sink,
                                            true);
+        c.sink_heads = a.tree_heads;
+        c.half = half_partials(SRC);
         e = launch_combine(c, stream);
     }
     return e == cudaSuccess ? 0 : launch_failed(e);
@@ -890,4 +908,147 @@ extern "C" int dsv4_indexer_topk_fwd(const Dsv4IndexerTopkParams* p, void* strea
     if (e != cudaSuccess) return int(e);
     return int(launch(pair ? topk_select_pair_kernel : topk_select_kernel, dim3(pair ? t.rows * 2 : t.rows), kTopkThreads,
                       t.row_in_smem ? row_bytes : 0, s, t));
+}
+
+
+// ── a speculative step: tree decode, pages, sampling (dsv4_speculative.h) ──
+
+extern "C" int dsv4_hca_tree_decode_fwd(const Dsv4HcaTreeDecodeParams* p, void* stream) {
+    t_last_error = "invalid argument";
+    if (p == nullptr || p->T <= 0 || p->H <= 0 || p->num_splits < 0 || p->mask_words < 0) return int(cudaErrorInvalidValue);
+    const int64_t rows = int64_t(p->T) * p->H;
+    if (p->B <= 0 || rows * p->B > 0x7FFFFFFF - kHeadsPerCta) return int(cudaErrorInvalidValue);      // TMA coordinates are 32-bit
+    const bool scheduled = p->num_splits == 0;
+    if (!common_ok(p->B, 1, int(rows), scheduled ? 2 : p->num_splits, p->sm_scale, p->q, p->out, p->partial_o, p->partial_lse)) return int(cudaErrorInvalidValue);
+    if (p->max_pages <= 0 || p->win_cap < 0 || p->num_pages <= 0 || (scheduled && (p->sched == nullptr || !aligned(p->sched, 16)))) return int(cudaErrorInvalidValue);
+    if (p->kv_pool == nullptr || p->block_table == nullptr || p->kv_len == nullptr || p->win_len == nullptr) return int(cudaErrorInvalidValue);
+    if ((p->win_cap > 0 && p->win_pool == nullptr) || (p->mask_words > 0 && p->tree_mask == nullptr)) return int(cudaErrorInvalidValue);
+    if (!aligned(p->kv_pool, 16) || !aligned(p->win_pool, 16)) return int(cudaErrorInvalidValue);
+    t_last_error = "";
+    DecodeArgs a{};
+    a.B = p->B;  a.s_q = 1;  a.H = int(rows);  a.max_pages = p->max_pages;  a.win_cap = p->win_cap;
+    a.num_pages = p->num_pages;
+    a.num_splits = scheduled ? 1 : p->num_splits;
+    a.scale_log2 = p->sm_scale * 1.4426950408889634f;
+    a.q = static_cast<const __nv_bfloat16*>(p->q);
+    a.kv_pool = static_cast<const uint8_t*>(p->kv_pool);
+    a.block_table = p->block_table;  a.kv_len = p->kv_len;
+    a.win_pool = static_cast<const uint8_t*>(p->win_pool);  a.win_len = p->win_len;
+    a.tree_mask = p->tree_mask;  a.tree_words = p->mask_words;  a.tree_heads = p->H;
+    a.attn_sink = p->attn_sink;
+    a.out = static_cast<__nv_bfloat16*>(p->out);  a.lse = p->lse;
+    a.partial_o = p->partial_o;  a.partial_lse = p->partial_lse;  a.status = p->status;
+    if (scheduled && p->make_plan) {
+        Dsv4PlanParams q{};
+        q.kind = DSV4_PLAN_HCA;
+        q.B = p->B;  q.s_q = 1;  q.H = int(rows);
+        q.kv_len = p->kv_len;  q.win_len = p->win_len;
+        q.sched = p->sched;  q.sched_bytes = p->sched_bytes;
+        const int rc = dsv4_attn_plan(&q, stream);
+        if (rc != 0) return rc;
+    }
+    return decode_fwd<kSrcTree>(a, scheduled ? p->sched : nullptr, static_cast<cudaStream_t>(stream));
+}
+
+namespace {
+KvPagesArgs pages_args(const Dsv4KvPagesParams* p) {
+    KvPagesArgs a{};
+    a.pool = static_cast<uint4*>(p->pool);
+    a.num_pages = p->num_pages;  a.layers = p->layers;  a.entries = p->entries;
+    a.B = p->B;  a.max_pages = p->max_pages;  a.n = p->n;
+    a.src = p->src;  a.dst = p->dst;
+    a.block_table = p->block_table;  a.kv_len = p->kv_len;  a.refs = p->refs;
+    a.new_table = p->new_table;  a.new_refs = p->new_refs;  a.count = p->count;
+    a.status = p->status;
+    return a;
+}
+bool pages_pool_ok(const Dsv4KvPagesParams* p) {
+    return p->pool != nullptr && aligned(p->pool, 16) && p->layers > 0 && p->layers <= 0x7FFFFFFF / kCopyBatches && p->num_pages > 0 && p->num_pages <= 0x7FFFFFFF;
+}
+bool pages_table_ok(const Dsv4KvPagesParams* p) {
+    return p->block_table != nullptr && p->refs != nullptr && p->B > 0 && p->max_pages > 0 && p->num_pages > 0 && p->num_pages <= 0x7FFFFFFF;
+}
+// Blocks of eight warps for `units` warps' worth of copying: at most eight an SM, which then loop.
+dim3 copy_grid(int64_t units) {
+    const int64_t want = (units + kPagesThreads / 32 - 1) / (kPagesThreads / 32), cap = int64_t(device_sms()) * 8;
+    return dim3(unsigned(want < cap ? (want > 0 ? want : 1) : cap));
+}
+}  // namespace
+
+extern "C" int dsv4_kv_pages_copy(const Dsv4KvPagesParams* p, void* stream) {
+    if (p == nullptr || !pages_pool_ok(p) || p->n < 0 || (p->n > 0 && (p->src == nullptr || p->dst == nullptr))) return int(cudaErrorInvalidValue);
+    if (p->n == 0) return 0;
+    return int(launch(kv_copy_pages_kernel, copy_grid(int64_t(p->n) * p->layers * kCopyBatches), kPagesThreads, 0, static_cast<cudaStream_t>(stream), pages_args(p)));
+}
+
+extern "C" int dsv4_kv_entries_move(const Dsv4KvPagesParams* p, void* stream) {
+    if (p == nullptr || p->pool == nullptr || !aligned(p->pool, 16) || p->layers <= 0 || p->layers > 0x7FFFFFFF || p->entries <= 0) return int(cudaErrorInvalidValue);
+    if (p->n < 0 || (p->n > 0 && (p->src == nullptr || p->dst == nullptr))) return int(cudaErrorInvalidValue);
+    if (p->n == 0) return 0;
+    return int(launch(kv_move_entries_kernel, copy_grid(int64_t(p->n) * p->layers), kPagesThreads, 0, static_cast<cudaStream_t>(stream), pages_args(p)));
+}
+
+extern "C" int dsv4_kv_pages_free(const Dsv4KvPagesParams* p, void* stream) {
+    if (p == nullptr || !pages_table_ok(p) || p->kv_len == nullptr || p->n < 0 || (p->n > 0 && p->src == nullptr)) return int(cudaErrorInvalidValue);
+    if (p->n == 0) return 0;
+    return int(launch(kv_free_kernel, dim3(unsigned(p->n)), kPagesThreads, 0, static_cast<cudaStream_t>(stream), pages_args(p)));
+}
+
+extern "C" int dsv4_kv_pages_fork(const Dsv4KvPagesParams* p, void* stream) {
+    if (p == nullptr || !pages_pool_ok(p) || !pages_table_ok(p) || p->kv_len == nullptr || p->n < 0 || (p->n > 0 && (p->src == nullptr || p->dst == nullptr)))
+        return int(cudaErrorInvalidValue);
+    if (p->n == 0) return 0;
+    const KvPagesArgs a = pages_args(p);
+    const cudaError_t e = launch(kv_fork_plan_kernel, dim3(1), kPagesPlanThreads, 0, static_cast<cudaStream_t>(stream), a);
+    if (e != cudaSuccess) return int(e);
+    return int(launch(kv_fork_apply_kernel, copy_grid(int64_t(p->n) * (1 + p->layers * kCopyBatches)), kPagesThreads, 0, static_cast<cudaStream_t>(stream), a));
+}
+
+extern "C" int dsv4_kv_pages_compact(const Dsv4KvPagesParams* p, void* stream) {
+    if (p == nullptr || !pages_pool_ok(p) || !pages_table_ok(p) || p->new_table == nullptr || p->new_refs == nullptr || p->count == nullptr || p->scratch == nullptr)
+        return int(cudaErrorInvalidValue);
+    KvPagesArgs a = pages_args(p);
+    a.remap = p->scratch;
+    a.from = a.remap + p->num_pages;
+    a.to = a.from + p->num_pages;
+    a.moves = a.to + p->num_pages;
+    const cudaError_t e = launch(kv_compact_plan_kernel, dim3(1), kPagesPlanThreads, 0, static_cast<cudaStream_t>(stream), a);
+    if (e != cudaSuccess) return int(e);
+    // (the host does not know how many pages move: as many blocks as half of the pool would take)
+    return int(launch(kv_compact_apply_kernel, copy_grid((p->num_pages + 1) / 2 * p->layers * kCopyBatches), kPagesThreads, 0, static_cast<cudaStream_t>(stream), a));
+}
+
+namespace {
+template <typename T>
+cudaError_t launch_sample(SampleArgs& a, cudaStream_t stream) {
+    // A block keeps up to 16,384 logits (64 KB: three blocks an SM, one computes while another loads).  Where the rows leave SMs without work, up to eight
+    // blocks share one as long as each has 4,096.
+    const int span = a.V + 16 / int(sizeof(T)) - 1;                        // with what a row's alignment may put before it
+    int blocks = 1;
+    while (blocks < kSampleMaxCluster && (span > blocks * 16384 || (int64_t(a.N) * blocks * 2 <= device_sms() && span > blocks * 4096))) blocks *= 2;
+    const int per_warp = (span + blocks * kSampleWarps - 1) / (blocks * kSampleWarps);
+    a.warp_span = (per_warp + kSampleStep - 1) / kSampleStep * kSampleStep;
+    const int64_t bytes = int64_t(a.warp_span) * kSampleWarps * sizeof(float);
+    const bool resident = bytes <= 200 * 1024;
+    static std::atomic<bool> done[kMaxDevices];
+    const cudaError_t e = ensure_smem(sample_kernel<T, true>, 200 * 1024, done);
+    if (e != cudaSuccess) return e;
+    return launch(resident ? sample_kernel<T, true> : sample_kernel<T, false>, dim3(unsigned(int64_t(a.N) * blocks)), kSampleThreads, resident ? size_t(bytes) : 0,
+                  stream, a, blocks);
+}
+}  // namespace
+
+extern "C" int dsv4_sample_fwd(const Dsv4SampleParams* p, void* stream) {
+    if (p == nullptr || p->N < 0 || p->N > 0x7FFFFFFF / kSampleMaxCluster || p->V <= 0 || p->V > (1 << 22) || p->stride_n < p->V) return int(cudaErrorInvalidValue);
+    if (p->logits == nullptr || p->u == nullptr || p->token == nullptr) return int(cudaErrorInvalidValue);
+    if (p->N == 0) return 0;
+    SampleArgs a{};
+    a.logits = p->logits;  a.stride = p->stride_n;  a.N = p->N;  a.V = p->V;
+    a.u = p->u;  a.temperature = p->temperature;  a.top_k = p->top_k;  a.top_p = p->top_p;  a.min_p = p->min_p;
+    a.token = p->token;  a.logprob = p->logprob;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (p->dtype == DSV4_DTYPE_F32 && aligned(p->logits, 4)) return int(launch_sample<float>(a, s));
+    if (p->dtype == DSV4_DTYPE_BF16 && aligned(p->logits, 2)) return int(launch_sample<__nv_bfloat16>(a, s));
+    if (p->dtype == DSV4_DTYPE_F16 && aligned(p->logits, 2)) return int(launch_sample<__half>(a, s));
+    return int(cudaErrorInvalidValue);
 }

@@ -7,6 +7,7 @@
 
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <math_constants.h>
 #include <stdint.h>
 
@@ -25,13 +26,15 @@ struct CombineArgs {
     int64_t stride_pl_split, stride_pl_n;
     int64_t stride_out_n, stride_out_h;
     int64_t stride_lse_n;
-    int partial_bf16;          // partial_o holds BF16 (strides then count BF16 elements): the library's own split path
+    int partial_bf16;          // partial_o holds BF16, or with `half` FP16 (strides then count BF16 elements): the library's own split path
     // Scheduled decode (sched.cuh): the pieces of unit (row, head group) lie in partial slots
     // unit_slot[u] .. + unit_nsplits[u] - 1, a slot being 128 head rows of 512 BF16 (and 128 LSEs); a unit
     // with one piece was written out by the decode kernel itself and is skipped here.
     const int32_t* unit_nsplits;
     const int32_t* unit_slot;
     int hgs;
+    bool half;
+    int sink_heads;            // trees: H counts (node, head) rows, and attn_sink has this many heads; 0: H
 };
 
 constexpr int kCombineWarps = 8;
@@ -48,7 +51,9 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
+// HALF: 16-bit partials are FP16 (what a tree decode writes) instead of BF16.
 // One (row, head): its S partial rows of 512 columns, po_stride elements apart from po_off, under the LSEs at pl.
+template <bool HALF>
 __device__ __forceinline__ void merge_head(const CombineArgs& a, int n, int h, int lane, int S, const float* pl, int64_t pl_stride,
                                            int64_t po_off, int64_t po_stride) {
     // pass 1: maximum and sum over splits.  The first 32 LSEs are loaded once (one per lane) and serve the maximum,
@@ -68,7 +73,7 @@ __device__ __forceinline__ void merge_head(const CombineArgs& a, int n, int h, i
         a.lse[int64_t(n) * a.stride_lse_n + h] = has ? glse * 0.6931471805599453f : -CUDART_INF_F;
     float denom = glse;
     if (a.attn_sink != nullptr) {
-        const float s2 = ptx::ld(a.attn_sink + h) * 1.4426950408889634f;
+        const float s2 = ptx::ld(a.attn_sink + (a.sink_heads > 0 ? h % a.sink_heads : h)) * 1.4426950408889634f;
         denom = has ? glse + log2f(1.f + exp2f(s2 - glse)) : s2;
     }
 
@@ -110,8 +115,10 @@ __device__ __forceinline__ void merge_head(const CombineArgs& a, int n, int h, i
                         const uint32_t u[4] = {v[j][i].x, v[j][i].y, v[j][i].z, v[j][i].w};
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
-                            acc[i][2 * q] = fmaf(w[j], __uint_as_float(u[q] << 16), acc[i][2 * q]);
-                            acc[i][2 * q + 1] = fmaf(w[j], __uint_as_float(u[q] & 0xFFFF0000u), acc[i][2 * q + 1]);
+                            float2 x = make_float2(__uint_as_float(u[q] << 16), __uint_as_float(u[q] & 0xFFFF0000u));
+                            if constexpr (HALF) x = __half22float2(*reinterpret_cast<const __half2*>(&u[q]));
+                            acc[i][2 * q] = fmaf(w[j], x.x, acc[i][2 * q]);
+                            acc[i][2 * q + 1] = fmaf(w[j], x.y, acc[i][2 * q + 1]);
                         }
                     }
             } else {
@@ -155,6 +162,7 @@ __device__ __forceinline__ void merge_head(const CombineArgs& a, int n, int h, i
 }
 
 // One warp per (row, head) of the batch: every one has num_splits partials, or those the plan says.
+template <bool HALF>
 __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const CombineArgs a) {
     ptx::pdl_trigger();
     ptx::pdl_wait();
@@ -180,12 +188,13 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_kernel(const Combi
         po_off = int64_t(n) * a.stride_po_n + int64_t(h) * a.stride_po_h + lane * 8;
         po_stride = a.stride_po_split;
     }
-    merge_head(a, n, h, lane, S, pl, pl_stride, po_off, po_stride);
+    merge_head<HALF>(a, n, h, lane, S, pl, pl_stride, po_off, po_stride);
 }
 
 // After a scheduled decode of a large batch.  A plan cuts at most as many units as there are block pairs, usually far fewer than the batch has, so
 // the grid is what is resident at once and its blocks share the cut units out, eight heads at a time: each block gathers them from
 // the plan's list (256 requests, mixed lengths: 12.5 -> 10 us cold against one warp per (row, head) of the batch, of which nine in ten had nothing to do).
+template <bool HALF>
 __global__ void __launch_bounds__(kCombineWarps * 32) combine_sched_kernel(const __grid_constant__ CombineArgs a) {
     constexpr int kPerThread = 4, kChunk = kCombineWarps * 32 * kPerThread;
     __shared__ int s_unit[kChunk];
@@ -228,7 +237,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) combine_sched_kernel(const
             const int in_group = int(j % slices) * kCombineWarps + warp, h = (u % a.hgs) * 128 + in_group;
             if (h >= a.H) continue;
             const int64_t row = int64_t(ptx::ld(a.unit_slot + u)) * 128 + in_group;
-            merge_head(a, n, h, lane, ptx::ld(a.unit_nsplits + u), a.partial_lse + row, 128, row * 512 + lane * 8, 128 * 512);
+            merge_head<HALF>(a, n, h, lane, ptx::ld(a.unit_nsplits + u), a.partial_lse + row, 128, row * 512 + lane * 8, 128 * 512);
         }
         job0 += jobs;
     }

@@ -85,7 +85,11 @@ enum SourceKind : int {
     kSrcRef = 2,   // reference layout: separate planes, 448 e4m3 + 7 UE8M0 + 64 bf16
     kSrcRefPaged = 3,   // the same bytes in packed pages: per page, page_size tokens of [448 e4m3 | 64 bf16]
                         // followed by page_size x 8 scale bytes (7 UE8M0 + 1 pad), behind block tables
+    kSrcTree = 4,  // as kSrcHca, for the drafted nodes of a tree: a row of the MMAs is (node, head), and a node sees the
+                   // window rows that its bit mask names
 };
+// [0, kv_len) through the block table, then the window buffer
+__host__ __device__ constexpr bool is_dense(int src) { return src == kSrcHca || src == kSrcTree; }
 
 // both kinds with the reference's quantisation (448 latent elements, one UE8M0 byte per 64)
 __host__ __device__ constexpr bool is_ref_layout(int src) { return src == kSrcRef || src == kSrcRefPaged; }
@@ -98,6 +102,10 @@ __host__ __device__ constexpr bool is_ref_layout(int src) { return src == kSrcRe
 // BF16 route's own limit on scales is 128).
 // The reference layouts keep BF16: their power-of-two scales span BF16's exponent range.
 __host__ __device__ constexpr bool use_f16(int src) { return !is_ref_layout(src); }
+
+// Split partials are BF16, of a tree FP16: its rows can be short (a few drafts), where partial outputs are larger than their
+// weighted sum, and BF16's 2^-9 of them would show in it.  V has been through FP16 already, so that FP16's range loses nothing.
+__host__ __device__ constexpr bool half_partials(int src) { return src == kSrcTree; }
 
 enum StatusCode : int {
     kStatusOk = 0,
@@ -163,6 +171,9 @@ struct DecodeArgs {
     int pg_page_shift;           // log2(page_size), page_size <= 64
     int64_t pg_page_bytes;       // page_size * 584
     int64_t pg_num_pages, pg_swa_num_pages;
+    // trees (kSrcTree): H above counts (node, head) rows, nodes x tree_heads of them
+    const int32_t* tree_mask;    // [B, nodes, tree_words]: bit w: the node sees window row w
+    int tree_words, tree_heads;
 };
 
 // One unit of work of a pair: tiles [tile0, tile0 + ntiles) of row n for head group hg.
@@ -372,6 +383,17 @@ __device__ __forceinline__ int resolve_index(const DecodeArgs& a, const TileCtx&
     return -1;
 }
 
+// Whether any node of the tile's row group sees window row w.
+__device__ __forceinline__ bool tree_group_sees(const DecodeArgs& a, const TileCtx& c, int w) {
+    if ((w >> 5) >= a.tree_words) return false;
+    const int nodes = a.H / a.tree_heads, t0 = c.hg * kHeadsPerCta / a.tree_heads, t1 = min(c.hg * kHeadsPerCta + kHeadsPerCta - 1, a.H - 1) / a.tree_heads;
+    const int32_t* word = a.tree_mask + (int64_t(c.n) * nodes + t0) * a.tree_words + (w >> 5);
+    uint32_t any = 0u;
+#pragma unroll 4
+    for (int t = t0; t <= t1; ++t, word += a.tree_words) any |= uint32_t(ptx::ld(word));
+    return (any >> (w & 31)) & 1u;
+}
+
 // Stage 2: issue the block-table load (where there is one).  `e` is the index-list value (CSA).  An entry
 // whose page slot lies outside the block table, or whose window row lies outside the window buffer, is
 // reported and left out; nothing is read through it.
@@ -389,7 +411,7 @@ __device__ __forceinline__ PendingId resolve_issue(const DecodeArgs& a, const Ti
                 report_status(a.status, kStatusBadIndex, 4, e);
             }
         }
-    } else if constexpr (SRC == kSrcHca) {
+    } else if constexpr (is_dense(SRC)) {
         if (in_row) {
             if (v < c.kv_len_n) {
                 if ((v >> 6) < a.max_pages) {
@@ -399,7 +421,8 @@ __device__ __forceinline__ PendingId resolve_issue(const DecodeArgs& a, const Ti
                     report_status(a.status, kStatusBadIndex, 4, v);
                 }
             } else if (v - c.kv_len_n < a.win_cap) {
-                p.id = kIdValid | kIdSecond | uint32_t(c.b * a.win_cap + (v - c.kv_len_n));
+                // (a row that no node of the group sees is left out, not read: whatever it holds)
+                if (SRC != kSrcTree || tree_group_sees(a, c, v - c.kv_len_n)) p.id = kIdValid | kIdSecond | uint32_t(c.b * a.win_cap + (v - c.kv_len_n));
             } else {
                 report_status(a.status, kStatusBadIndex, 4, v);
             }
@@ -492,7 +515,7 @@ __device__ __forceinline__ void row_lengths(const DecodeArgs& a, int n, int& n_t
         const int raw = (a.topk_len != nullptr) ? ptx::ld(a.topk_len + n) : a.topk;
         n_tok = min(max(raw, 0), a.topk);
         kv_len_n = (a.kv_len != nullptr) ? ptx::ld(a.kv_len + n) : 0x7FFFFFFF;
-    } else if constexpr (SRC == kSrcHca || SRC == kSrcRefPaged) {
+    } else if constexpr (is_dense(SRC) || SRC == kSrcRefPaged) {
         kv_len_n = max(ptx::ld(a.kv_len + n), 0);
         n_tok = kv_len_n + max(ptx::ld(a.win_len + n), 0);
     } else {
@@ -704,6 +727,25 @@ __device__ __forceinline__ void q_to_tmem(uint32_t src, uint32_t dst, int vw, in
         if constexpr (F16) { x = bf16x8_to_f16x8(x);  y = bf16x8_to_f16x8(y); }
         ptx::tmem_st8(dst + lanes + uint32_t(u) * 4u, x, y);
     }
+}
+
+// Which of the 32 entries that block `colhalf` of the pair supplies to a tile a node of a tree sees.  Entry s of the tile is entry
+// v0 + s of the row: one of the cache's (seen by every node) below kv_len, else window row v0 + s - kv_len, whose bit in the node's
+// mask decides.
+__device__ __forceinline__ uint32_t tree_bits(const DecodeArgs& a, const int32_t* mask, int v0, int kv_len, int colhalf) {
+    const int o = v0 - kv_len;                        // window row of entry 0 (negative: the tile begins with entries of the cache)
+    if (o <= -kTileN) return ~0u;
+    const int first = max(o, 0), w = first >> 5, shift = first & 31;
+    uint32_t x[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) x[i] = w + i < a.tree_words ? uint32_t(ptx::ld(mask + w + i)) : 0u;
+    uint64_t m = uint64_t(__funnelshift_r(x[0], x[1], shift)) | (uint64_t(__funnelshift_r(x[1], x[2], shift)) << 32);
+    if (o < 0) m = (m << -o) | ((1ull << -o) - 1ull);
+    // K row r of block c is entry 8 (r / 4) + 4 c + r % 4: nibble c of every byte
+    m = (m >> (4 * colhalf)) & 0x0F0F0F0F0F0F0F0Full;
+    m = (m | (m >> 4)) & 0x00FF00FF00FF00FFull;
+    m = (m | (m >> 8)) & 0x0000FFFF0000FFFFull;
+    return uint32_t(m | (m >> 16));
 }
 
 template <int NCHUNK, int SRC>
@@ -1272,6 +1314,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNumThreads, 1) deco
                 if (k + 1 < n_items) cur = get_item(k + 1);
                 continue;
             }
+            // (rows past the last node are computed but not written)
+            const int32_t* node_mask = nullptr;
+            if constexpr (SRC == kSrcTree) node_mask = a.tree_mask + (int64_t(n) * (a.H / a.tree_heads) + min(h0 + r, a.H - 1) / a.tree_heads) * a.tree_words;
             float m_ref = -CUDART_INF_F;                   // reference maximum used in exp2 (log2 units)
             float l_sum = 0.f;                             // of this thread's entries
             bool left = false;
@@ -1279,10 +1324,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNumThreads, 1) deco
             for (int it = 0; it < nb; ++it) {
                 const uint32_t g = gt + uint32_t(it);
                 const uint32_t s_tmem = tmem + lane_addr + kTmemS + (g & 1u) * 32u;
+                uint32_t seen = ~0u;
+                if constexpr (SRC == kSrcTree) seen = tree_bits(a, node_mask, (cur.tile0 + it) * kTileN, cur.kv_len_n, colhalf);
                 if (ok) ok = wait_for(bar_s_full + 8 * (g & 1u), g >> 1, kStatusWaitSFull, 0, int(g));
                 ptx::tc_fence_after_sync();
                 if (tid == 0) trace_mark(a, 0, 4 * int(g));
-                const uint32_t vmask = *reinterpret_cast<volatile uint32_t*>(&misc->mask[g % kTagRing][colhalf]);
+                const uint32_t vmask = *reinterpret_cast<volatile uint32_t*>(&misc->mask[g % kTagRing][colhalf]) & seen;
                 uint32_t s0[32];
                 ptx::tmem_ld32(s_tmem, s0);
                 ptx::tmem_wait_ld();
@@ -1375,7 +1422,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNumThreads, 1) deco
             if (tid == 0 && k == n_items - 1 && (sched || a.num_splits > 1)) ptx::pdl_trigger();
             float denom = l_sum;
             if (final_out && a.attn_sink != nullptr && write) {
-                const float s2 = ptx::ld(a.attn_sink + h0 + r) * 1.4426950408889634f;
+                const float s2 = ptx::ld(a.attn_sink + (SRC == kSrcTree ? (h0 + r) % a.tree_heads : h0 + r)) * 1.4426950408889634f;
                 denom = (l_sum != 0.f) ? l_sum + ptx::ex2(s2 - m_ref) : 1.f;   // empty row: O is 0 anyway
             }
             const float inv = (l_sum != 0.f) ? 1.f / denom : 0.f;
@@ -1400,6 +1447,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNumThreads, 1) deco
                         w.y = ptx::pack_bf16x2(__uint_as_float(o[8 * v + 2]) * inv, __uint_as_float(o[8 * v + 3]) * inv);
                         w.z = ptx::pack_bf16x2(__uint_as_float(o[8 * v + 4]) * inv, __uint_as_float(o[8 * v + 5]) * inv);
                         w.w = ptx::pack_bf16x2(__uint_as_float(o[8 * v + 6]) * inv, __uint_as_float(o[8 * v + 7]) * inv);
+                        if (half_partials(SRC) && !final_out) {
+                            w.x = ptx::pack_f16x2(__uint_as_float(o[8 * v + 0]) * inv, __uint_as_float(o[8 * v + 1]) * inv);
+                            w.y = ptx::pack_f16x2(__uint_as_float(o[8 * v + 2]) * inv, __uint_as_float(o[8 * v + 3]) * inv);
+                            w.z = ptx::pack_f16x2(__uint_as_float(o[8 * v + 4]) * inv, __uint_as_float(o[8 * v + 5]) * inv);
+                            w.w = ptx::pack_f16x2(__uint_as_float(o[8 * v + 6]) * inv, __uint_as_float(o[8 * v + 7]) * inv);
+                        }
                         ptx::sts_v4(p_row + uint32_t(hc) * kQChunkBytes + (p_sw ^ (uint32_t(v) << 4)), w);
                     }
                 }

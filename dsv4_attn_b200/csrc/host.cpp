@@ -16,6 +16,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/dsv4_attn.h"
+#include "../../include/dsv4_speculative.h"
 
 namespace {
 
@@ -33,6 +34,14 @@ struct Library {
     decltype(&dsv4_attn_combine) combine;
     decltype(&dsv4_attn_plan) plan;
     decltype(&dsv4_attn_plan_splits) plan_splits;
+    decltype(&dsv4_hca_tree_decode_fwd) tree;
+    decltype(&dsv4_attn_sched_bytes) sched_bytes;
+    decltype(&dsv4_kv_pages_copy) pages_copy;
+    decltype(&dsv4_kv_pages_fork) pages_fork;
+    decltype(&dsv4_kv_pages_free) pages_free;
+    decltype(&dsv4_kv_pages_compact) pages_compact;
+    decltype(&dsv4_kv_entries_move) entries_move;
+    decltype(&dsv4_sample_fwd) sample;
 } lib;
 
 constexpr int kLatent = 512, kQk = 576, kEntry = DSV4_ENTRY_BYTES, kPage = DSV4_PAGE_ENTRIES;
@@ -467,6 +476,187 @@ PyObject* combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return rc != 0 ? code(rc) : pair(out, lse);
 }
 
+// Where the library plans the work of a tree decode in the call: more row groups than the device has pairs of SMs (74).  Below that one wave of pairs is
+// enough, with rows split so that it is full.
+constexpr int64_t kTreePlanGroups = 74;
+
+// (q, kv_pool, block_table, kv_len, win_pool, win_len, tree_mask, sm_scale, attn_sink, num_splits, out, lse, workspace, status, max_len, plan)
+PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 16) return none();
+    const at::Tensor *q = tensor(a[0], at::kBFloat16, 4), *pool = tensor(a[1], at::kByte, 3), *table = tensor(a[2], at::kInt, 2), *kv_len = tensor(a[3], at::kInt, 1);
+    const at::Tensor *win = tensor(a[4], at::kByte, 3), *win_len = tensor(a[5], at::kInt, 1), *mask = tensor(a[6], at::kInt, 3), *sink, *status;
+    Dsv4HcaTreeDecodeParams p{};
+    if (q == nullptr || pool == nullptr || table == nullptr || kv_len == nullptr || win == nullptr || win_len == nullptr || mask == nullptr || !number(a[7], &p.sm_scale))
+        return none();
+    const int64_t B = q->size(0), T = q->size(1), H = q->size(2), W = win->size(1), rows = B * T * H;
+    if (B <= 0 || T <= 0 || H <= 0 || !fits32(B) || !fits32(T) || !fits32(H) || !fits32(T * H) || !fits32(rows) || q->size(3) != kQk) return none();
+    if (pool->size(0) <= 0 || pool->size(1) != kPage || pool->size(2) != kEntry || table->size(0) != B || table->size(1) <= 0 || !fits32(table->size(1))) return none();
+    if (win->size(0) != B || win->size(2) != kEntry || !fits32(W) || mask->size(0) != B || mask->size(1) != T || !fits32(mask->size(2))) return none();
+    if (!has_shape(kv_len, {B}) || !has_shape(win_len, {B}) || !optional_tensor(a[8], at::kFloat, 1, &sink) || !has_shape(sink, {H})) return none();
+    if (!optional_tensor(a[13], at::kInt, 1, &status) || (status != nullptr && status->numel() < DSV4_STATUS_WORDS)) return none();
+    int64_t max_len = table->size(1) * kPage + W, splits;
+    if (a[14] != Py_None && !integer(a[14], &max_len)) return none();
+    if (!fits32(max_len)) return none();
+    const at::Tensor *po = nullptr, *pl = nullptr, *sched = nullptr;
+    at::Tensor own_po, own_pl, own_sched;
+    const int64_t groups = B * ((T * H + 127) / 128);
+    if (a[15] != Py_None) {                                                // a plan made before
+        int64_t v[4];
+        if (!PyTuple_Check(a[15]) || PyTuple_GET_SIZE(a[15]) != 8) return none();
+        for (int i = 0; i < 4; ++i)
+            if (!integer(PyTuple_GET_ITEM(a[15], i), &v[i])) return none();
+        if (v[0] != DSV4_PLAN_HCA || v[1] != B || v[2] != 1 || v[3] != T * H) return none();
+        sched = any_tensor(PyTuple_GET_ITEM(a[15], 5));
+        po = any_tensor(PyTuple_GET_ITEM(a[15], 6));
+        pl = any_tensor(PyTuple_GET_ITEM(a[15], 7));
+        if (sched == nullptr || po == nullptr || pl == nullptr) return none();
+        splits = 0;
+    } else if (a[9] == Py_None && a[12] == Py_None && groups > kTreePlanGroups) {
+        int64_t po_bytes, pl_bytes;
+        const int64_t bytes = lib.sched_bytes(int(B), int(T * H), 0, 0, &po_bytes, &pl_bytes);
+        if (bytes <= 0) return none();
+        own_sched = empty({bytes / 4}, at::kInt, q);
+        own_po = empty({po_bytes / 4 + 4}, at::kFloat, q);
+        own_pl = empty({pl_bytes / 4 + 4}, at::kFloat, q);
+        sched = &own_sched;  po = &own_po;  pl = &own_pl;
+        p.make_plan = 1;
+        p.sched_bytes = bytes;
+        splits = 0;
+    } else {
+        if (a[9] == Py_None) splits = lib.plan_splits(int(B), int(T * H), int(max_len), 0);
+        else if (!integer(a[9], &splits)) return none();
+        if (splits < 1 || splits > DSV4_MAX_SPLITS) return none();
+        if (a[12] != Py_None) {
+            if (!PyTuple_Check(a[12]) || PyTuple_GET_SIZE(a[12]) != 2) return none();
+            po = tensor(PyTuple_GET_ITEM(a[12], 0), at::kFloat, -1);
+            pl = tensor(PyTuple_GET_ITEM(a[12], 1), at::kFloat, -1);
+            if (po == nullptr || pl == nullptr || po->numel() < splits * rows * kLatent || pl->numel() < splits * rows) return none();
+        } else if (splits > 1) {
+            own_po = empty({splits * rows * kLatent}, at::kFloat, q);
+            own_pl = empty({splits * rows}, at::kFloat, q);
+            po = &own_po;  pl = &own_pl;
+        }
+    }
+    Output out, lse;
+    if (!out.take(a[10], at::kBFloat16, {B, T, H, kLatent}, q) || !lse.take(a[11], at::kFloat, {B, T, H}, q)) return none();
+    p.B = int(B);  p.T = int(T);  p.H = int(H);  p.max_pages = int(table->size(1));  p.win_cap = int(W);  p.mask_words = int(mask->size(2));
+    p.num_splits = int(splits);  p.num_pages = pool->size(0);
+    p.q = ptr(q);  p.kv_pool = ptr(pool);  p.block_table = ptr<int32_t>(table);  p.kv_len = ptr<int32_t>(kv_len);
+    p.win_pool = ptr(win);  p.win_len = ptr<int32_t>(win_len);  p.tree_mask = ptr<int32_t>(mask);  p.attn_sink = ptr<float>(sink);
+    p.out = ptr(out.t);  p.lse = ptr<float>(lse.t);  p.partial_o = ptr<float>(po);  p.partial_lse = ptr<float>(pl);
+    p.status = ptr<int32_t>(status);  p.sched = ptr(sched);
+    const int rc = launch(lib.tree, &p, stream_of(q));
+    return rc != 0 ? code(rc) : pair(out, lse);
+}
+
+// (logits, u, temperature, top_k, top_p, min_p, out, logprob)
+PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 8) return none();
+    const at::Tensor *logits = any_tensor(a[0]), *u = tensor(a[1], at::kFloat, 1), *t[4];
+    if (logits == nullptr || !logits->is_cuda() || logits->dim() != 2 || u == nullptr) return none();
+    Dsv4SampleParams p{};
+    switch (logits->scalar_type()) {
+        case at::kFloat: p.dtype = DSV4_DTYPE_F32;  break;
+        case at::kBFloat16: p.dtype = DSV4_DTYPE_BF16;  break;
+        case at::kHalf: p.dtype = DSV4_DTYPE_F16;  break;
+        default: return none();
+    }
+    const int64_t N = logits->size(0), V = logits->size(1), stride = N > 1 ? logits->stride(0) : V;
+    if (V <= 0 || V > (1 << 22) || !fits32(N) || (V > 1 && logits->stride(1) != 1) || stride < V || !has_shape(u, {N})) return none();
+    for (int i = 0; i < 4; ++i)
+        if (!optional_tensor(a[2 + i], i == 1 ? at::kInt : at::kFloat, 1, &t[i]) || !has_shape(t[i], {N})) return none();
+    Output out, logprob;
+    if (!out.take(a[6], at::kInt, {N}, logits) || !logprob.take(a[7], at::kFloat, {N}, logits)) return none();
+    p.N = int(N);  p.V = int(V);  p.stride_n = stride;
+    p.logits = logits->data_ptr();  p.u = ptr<float>(u);
+    p.temperature = ptr<float>(t[0]);  p.top_k = ptr<int32_t>(t[1]);  p.top_p = ptr<float>(t[2]);  p.min_p = ptr<float>(t[3]);
+    p.token = ptr<int32_t>(out.t);  p.logprob = ptr<float>(logprob.t);
+    const int rc = N == 0 ? 0 : launch(lib.sample, &p, stream_of(logits));
+    return rc != 0 ? code(rc) : pair(out, logprob);
+}
+
+// A pool [pages, 64, 656] or [layers, pages, 64, 656] (`paged`), or any rows of entries
+bool pages_pool(PyObject* o, bool paged, Dsv4KvPagesParams* p, const at::Tensor** pool) {
+    const at::Tensor* t = *pool = tensor(o, at::kByte, -1);
+    if (t == nullptr || (t->dim() != 3 && t->dim() != 4) || t->numel() <= 0 || t->size(-1) != kEntry || (paged && t->size(-2) != kPage)) return false;
+    p->pool = ptr(t);
+    p->layers = t->dim() == 4 ? t->size(0) : 1;
+    p->num_pages = t->size(-3);
+    p->entries = t->size(-3) * t->size(-2);
+    return fits32(p->num_pages);
+}
+bool pages_items(PyObject* src_, PyObject* dst_, PyObject* status_, Dsv4KvPagesParams* p) {
+    const at::Tensor *src = tensor(src_, at::kInt, 1), *dst = dst_ == nullptr ? src : tensor(dst_, at::kInt, 1), *status;
+    if (src == nullptr || dst == nullptr || !fits32(src->size(0)) || src->size(0) != dst->size(0)) return false;
+    if (!optional_tensor(status_, at::kInt, 1, &status) || (status != nullptr && status->numel() < DSV4_STATUS_WORDS)) return false;
+    p->n = int(src->size(0));  p->src = ptr<int32_t>(src);  p->dst = dst_ == nullptr ? nullptr : ptr<int32_t>(dst);  p->status = ptr<int32_t>(status);
+    return true;
+}
+// (num_pages < 0: as many as page_refs has)
+bool pages_tables(PyObject* table_, PyObject* len_, PyObject* refs_, int64_t num_pages, Dsv4KvPagesParams* p) {
+    const at::Tensor *table = tensor(table_, at::kInt, 2), *len = len_ == nullptr ? nullptr : tensor(len_, at::kInt, 1), *refs = tensor(refs_, at::kInt, 1);
+    if (table == nullptr || table->numel() <= 0 || !fits32(table->size(0)) || !fits32(table->size(1)) || refs == nullptr || refs->size(0) <= 0 || !fits32(refs->size(0))) return false;
+    if ((len_ != nullptr && (len == nullptr || !has_shape(len, {table->size(0)}))) || (num_pages >= 0 && refs->size(0) != num_pages)) return false;
+    p->B = int(table->size(0));  p->max_pages = int(table->size(1));  p->num_pages = refs->size(0);
+    p->block_table = ptr<int32_t>(table);  p->kv_len = ptr<int32_t>(len);  p->refs = ptr<int32_t>(refs);
+    return true;
+}
+
+// (kv_pool, src, dst, status) -> the library's code
+PyObject* pages_copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    Dsv4KvPagesParams p{};
+    const at::Tensor* pool;
+    if (n != 4 || !pages_pool(a[0], true, &p, &pool) || !pages_items(a[1], a[2], a[3], &p)) return none();
+    return code(launch(lib.pages_copy, &p, stream_of(pool)));
+}
+
+// (pool, src, dst, status)
+PyObject* entries_move(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    Dsv4KvPagesParams p{};
+    const at::Tensor* pool;
+    if (n != 4 || !pages_pool(a[0], false, &p, &pool) || !pages_items(a[1], a[2], a[3], &p)) return none();
+    return code(launch(lib.entries_move, &p, stream_of(pool)));
+}
+
+// (block_table, kv_len, page_refs, requests, status)
+PyObject* pages_free(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    Dsv4KvPagesParams p{};
+    if (n != 5 || !pages_tables(a[0], a[1], a[2], -1, &p) || !pages_items(a[3], nullptr, a[4], &p)) return none();
+    return code(launch(lib.pages_free, &p, stream_of(any_tensor(a[0]))));
+}
+
+// (kv_pool, block_table, kv_len, page_refs, parent, child, status)
+PyObject* pages_fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    Dsv4KvPagesParams p{};
+    const at::Tensor* pool;
+    if (n != 7 || !pages_pool(a[0], true, &p, &pool) || !pages_tables(a[1], a[2], a[3], p.num_pages, &p) || !pages_items(a[4], a[5], a[6], &p)) return none();
+    return code(launch(lib.pages_fork, &p, stream_of(pool)));
+}
+
+// (kv_pool, block_table, page_refs, new_table, new_refs, count, workspace, status) -> (table, refs, count) or the library's code
+PyObject* pages_compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    Dsv4KvPagesParams p{};
+    const at::Tensor *pool, *status, *scratch;
+    if (n != 8 || !pages_pool(a[0], true, &p, &pool) || !pages_tables(a[1], nullptr, a[2], p.num_pages, &p)) return none();
+    if (!optional_tensor(a[7], at::kInt, 1, &status) || (status != nullptr && status->numel() < DSV4_STATUS_WORDS)) return none();
+    if (!optional_tensor(a[6], at::kInt, 1, &scratch) || (scratch != nullptr && scratch->numel() < 3 * p.num_pages + 1)) return none();
+    Output out[3];
+    const int64_t B = p.B, width = p.max_pages;
+    if (!out[0].take(a[3], at::kInt, {B, width}, pool) || !out[1].take(a[4], at::kInt, {p.num_pages}, pool) || !out[2].take(a[5], at::kInt, {1}, pool)) return none();
+    at::Tensor own;
+    if (scratch == nullptr) {
+        own = empty({3 * p.num_pages + 1}, at::kInt, pool);
+        scratch = &own;
+    }
+    p.new_table = ptr<int32_t>(out[0].t);  p.new_refs = ptr<int32_t>(out[1].t);  p.count = ptr<int32_t>(out[2].t);  p.scratch = ptr<int32_t>(scratch);
+    p.status = ptr<int32_t>(status);
+    const int rc = launch(lib.pages_compact, &p, stream_of(pool));
+    if (rc != 0) return code(rc);
+    PyObject* r = PyTuple_New(3);
+    for (int i = 0; i < 3; ++i) PyTuple_SET_ITEM(r, i, out[i].result());
+    return r;
+}
+
 // C++ exceptions (the allocator's out-of-memory error among them) become None: the slow path meets the same error and raises it.
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
@@ -497,6 +687,7 @@ PyMethodDef methods[] = {
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&bind)), METH_FASTCALL, nullptr},
     DSV4_FAST(csa), DSV4_FAST(hca), DSV4_FAST(packed), DSV4_FAST(planes), DSV4_FAST(rope_norm), DSV4_FAST(insert), DSV4_FAST(csa_compress),
     DSV4_FAST(hca_compress), DSV4_FAST(indexer), DSV4_FAST(plan), DSV4_FAST(combine),
+    DSV4_FAST(tree), DSV4_FAST(sample), DSV4_FAST(pages_copy), DSV4_FAST(entries_move), DSV4_FAST(pages_free), DSV4_FAST(pages_fork), DSV4_FAST(pages_compact),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

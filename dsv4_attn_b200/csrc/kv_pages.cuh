@@ -1,0 +1,318 @@
+// Pages of the cache: copying, forking, freeing, compacting; and moving single entries.
+//
+// A page holds 64 entries of 656 bytes; a pool has `layers` times `num_pages` of them, one block table per request serves all layers.
+// refs[p] counts the block-table slots that hold page p; a page with a count of 0 is free.  The bytes that move bound the large
+// calls (a copy reads and writes every byte once), launches and the chain lengths -> table -> page the small ones.  Every answer is a
+// function of the arguments alone: free pages are taken in ascending order, and counts are integers, whose atomics commute.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "ptx.cuh"
+#include "decode_kernel.cuh"
+
+namespace dsv4 {
+
+constexpr int kPageEntries = 64;
+constexpr int kEntryVecs = 41;                                   // 656 bytes as 16-byte vectors
+constexpr int kPageVecs = kPageEntries * kEntryVecs;             // 2624
+constexpr int kPagesThreads = 256;
+constexpr int kPagesPlanThreads = 1024;
+// A warp copies 256 vectors (4 KB) at a time, eight loads in flight per lane: 16 warps an SM then have more on the way than a DRAM
+// access takes, and a single page still spreads over eleven warps.
+constexpr int kCopyVecs = 256;
+constexpr int kCopyBatches = (kPageVecs + kCopyVecs - 1) / kCopyVecs;
+constexpr int kStatusNoPage = 10;                                // a fork found no free page
+
+struct KvPagesArgs {
+    uint4* pool;                 // [layers, num_pages, 64, 656 bytes]
+    int64_t num_pages, layers;
+    int B, max_pages;
+    int n;                       // copy: pairs; fork: children; free: requests
+    const int32_t* src;          // copy: pages; fork: parents; free: requests; move: entries
+    const int32_t* dst;          // copy: pages; fork: children; move: entries
+    int32_t* block_table;        // [B, max_pages]
+    int32_t* kv_len;             // [B]
+    int32_t* refs;               // [num_pages]
+    // compact
+    int32_t* new_table;          // may be block_table
+    int32_t* new_refs;           // may be refs
+    int32_t* count;              // live pages
+    int32_t* remap;              // scratch [num_pages]: where a page goes
+    int32_t* from;               // scratch [num_pages]: pages that move
+    int32_t* to;                 // scratch [num_pages]: where they go
+    int32_t* moves;              // scratch [1]: how many move
+    int64_t entries;             // move: entries per layer
+    int32_t* status;
+};
+
+// Vectors [at, at + 256) of `total`, from src to dst, by one warp.
+__device__ __forceinline__ void copy_batch(uint4* dst, const uint4* src, int at, int total, int lane) {
+    uint4 v[kCopyVecs / 32];
+#pragma unroll
+    for (int i = 0; i < kCopyVecs / 32; ++i)
+        if (at + i * 32 + lane < total) v[i] = ptx::ldg_stream_v4(src + at + i * 32 + lane);
+#pragma unroll
+    for (int i = 0; i < kCopyVecs / 32; ++i)
+        if (at + i * 32 + lane < total) dst[at + i * 32 + lane] = v[i];
+}
+
+__device__ __forceinline__ bool in_pool(const KvPagesArgs& a, int page) { return page >= 0 && page < a.num_pages; }
+
+// Page src[i] of every layer to page dst[i].  A negative number leaves the pair out; one beyond the pool is reported.
+__global__ void __launch_bounds__(kPagesThreads) kv_copy_pages_kernel(const __grid_constant__ KvPagesArgs a) {
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t units = int64_t(a.n) * a.layers * kCopyBatches;
+    for (int64_t u = int64_t(blockIdx.x) * (kPagesThreads / 32) + (threadIdx.x >> 5); u < units; u += int64_t(gridDim.x) * (kPagesThreads / 32)) {
+        const int batch = int(u % kCopyBatches);
+        const int64_t page = u / kCopyBatches, layer = page / a.n;
+        const int i = int(page % a.n), s = ptx::ld(a.src + i), d = ptx::ld(a.dst + i);
+        if (s < 0 || d < 0) continue;
+        if (!in_pool(a, s) || !in_pool(a, d)) {
+            if (lane == 0) report_status(a.status, kStatusBadIndex, 6, i);
+            continue;
+        }
+        copy_batch(a.pool + (layer * a.num_pages + d) * kPageVecs, a.pool + (layer * a.num_pages + s) * kPageVecs, batch * kCopyVecs, kPageVecs, lane);
+    }
+}
+
+// Entry src[i] of every layer to entry dst[i] (numbers within a layer).
+__global__ void __launch_bounds__(kPagesThreads) kv_move_entries_kernel(const __grid_constant__ KvPagesArgs a) {
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t units = int64_t(a.n) * a.layers;
+    for (int64_t u = int64_t(blockIdx.x) * (kPagesThreads / 32) + (threadIdx.x >> 5); u < units; u += int64_t(gridDim.x) * (kPagesThreads / 32)) {
+        const int64_t layer = u / a.n;
+        const int i = int(u % a.n), s = ptx::ld(a.src + i), d = ptx::ld(a.dst + i);
+        if (s < 0 || d < 0) continue;
+        if (s >= a.entries || d >= a.entries) {
+            if (lane == 0) report_status(a.status, kStatusBadIndex, 6, i);
+            continue;
+        }
+        copy_batch(a.pool + (layer * a.entries + d) * kEntryVecs, a.pool + (layer * a.entries + s) * kEntryVecs, 0, kEntryVecs, lane);
+    }
+}
+
+// The pages of request src[i] are given back: one reference less each, its row of the table -1, its length 0.  One block per request.
+__global__ void __launch_bounds__(kPagesThreads) kv_free_kernel(const __grid_constant__ KvPagesArgs a) {
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    const int r = ptx::ld(a.src + blockIdx.x);
+    if (r < 0) return;
+    if (r >= a.B) {
+        if (threadIdx.x == 0) report_status(a.status, kStatusBadIndex, 6, int(blockIdx.x));
+        return;
+    }
+    const int len = ptx::ld(a.kv_len + r), held = len > 0 ? (len - 1) / kPageEntries + 1 : 0;
+    int32_t* row = a.block_table + int64_t(r) * a.max_pages;
+    for (int i = threadIdx.x; i < a.max_pages; i += kPagesThreads) {
+        const int page = row[i];
+        if (i < held && in_pool(a, page)) atomicSub(a.refs + page, 1);
+        row[i] = -1;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) a.kv_len[r] = 0;
+}
+
+// A parent's length as a fork sees it.
+__device__ __forceinline__ int fork_length(const KvPagesArgs& a, int parent) {
+    return int(min(int64_t(max(ptx::ld(a.kv_len + parent), 0)), int64_t(a.max_pages) * kPageEntries));
+}
+__device__ __forceinline__ bool fork_pair(const KvPagesArgs& a, int i, int& parent, int& child) {
+    parent = ptx::ld(a.src + i);
+    child = ptx::ld(a.dst + i);
+    return parent >= 0 && parent < a.B && child >= 0 && child < a.B;
+}
+
+// Exclusive prefix sum of `v` over the block, and the block's total; every thread calls.
+__device__ __forceinline__ int block_prefix(int v, int* s_warp, int& total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();                  // the sums of the call before have been read
+    if (lane == 31) s_warp[warp] = x;
+    __syncthreads();
+    int w = s_warp[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xFFFFFFFFu, w, o);
+        if (lane >= o) w += y;
+    }
+    total = __shfl_sync(0xFFFFFFFFu, w, 31);
+    return x - v + (warp > 0 ? __shfl_sync(0xFFFFFFFFu, w, warp - 1) : 0);
+}
+
+// First half of a fork, one block: the children whose parent ends in a partly filled page get the lowest-numbered free pages, in the order
+// of the children.  Writes those pages' table slots and counts, and the children's lengths.
+__global__ void __launch_bounds__(kPagesPlanThreads) kv_fork_plan_kernel(const __grid_constant__ KvPagesArgs a) {
+    constexpr int kPerThread = 4, kChunk = kPagesPlanThreads * kPerThread;
+    __shared__ int s_warp[32];
+    __shared__ int s_free[kPagesPlanThreads];          // free pages for the children of this round
+    __shared__ int s_last;
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    const int tid = threadIdx.x;
+    int64_t page0 = 0;                                 // pages before this one are taken
+    for (int base = 0; base < a.n; base += kPagesPlanThreads) {
+        const int i = base + tid;
+        int parent = 0, child = 0, len = 0;
+        bool ok = false;
+        if (i < a.n) {
+            ok = fork_pair(a, i, parent, child);
+            if (!ok && (parent >= 0 && child >= 0)) report_status(a.status, kStatusBadIndex, 6, i);
+            if (ok) len = fork_length(a, parent);
+        }
+        const bool need = len % kPageEntries != 0;
+        int wanted, found = 0;
+        const int rank = block_prefix(need ? 1 : 0, s_warp, wanted);
+        // pages in ascending order, four a thread, until there are enough
+        while (found < wanted && page0 < a.num_pages) {
+            const int64_t p = page0 + tid * kPerThread;
+            int free_bits = 0;
+#pragma unroll
+            for (int j = 0; j < kPerThread; ++j)
+                if (p + j < a.num_pages && ptx::ld(a.refs + p + j) <= 0) free_bits |= 1 << j;
+            int in_chunk, at = found + block_prefix(__popc(free_bits), s_warp, in_chunk);
+#pragma unroll
+            for (int j = 0; j < kPerThread; ++j)
+                if ((free_bits >> j) & 1) {
+                    if (at < wanted) s_free[at] = int(p + j);
+                    if (at == wanted - 1) s_last = int(p + j);
+                    ++at;
+                }
+            __syncthreads();
+            found += in_chunk;
+            page0 = found >= wanted ? int64_t(s_last) + 1 : page0 + kChunk;
+        }
+        if (ok) {
+            const int full = len / kPageEntries;
+            if (need) {
+                const bool has = rank < found;
+                const int page = has ? s_free[rank] : -1;
+                a.block_table[int64_t(child) * a.max_pages + full] = page;
+                if (has) a.refs[page] = 1;
+                else report_status(a.status, kStatusNoPage, 6, i);
+                if (!has) len = full * kPageEntries;
+            }
+            a.kv_len[child] = len;
+        }
+        __syncthreads();                               // s_free is read before the next round fills it
+    }
+}
+
+// Second half: units of a child are its table row and 4 KB batches of its partly filled page in every layer.
+__global__ void __launch_bounds__(kPagesThreads) kv_fork_apply_kernel(const __grid_constant__ KvPagesArgs a) {
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t per_child = 1 + a.layers * kCopyBatches, units = a.n * per_child;
+    for (int64_t u = int64_t(blockIdx.x) * (kPagesThreads / 32) + (threadIdx.x >> 5); u < units; u += int64_t(gridDim.x) * (kPagesThreads / 32)) {
+        // (rows first, batches afterwards: neighbouring warps then copy neighbouring bytes)
+        const bool row = u < a.n;
+        const int64_t v = u - a.n;
+        const int i = row ? int(u) : int(v / (a.layers * kCopyBatches));
+        int parent, child;
+        if (!fork_pair(a, i, parent, child)) continue;
+        const int len = fork_length(a, parent), full = len / kPageEntries, rest = len % kPageEntries;
+        const int32_t* from = a.block_table + int64_t(parent) * a.max_pages;
+        int32_t* to = a.block_table + int64_t(child) * a.max_pages;
+        if (row) {
+            for (int k = lane; k < a.max_pages; k += 32) {
+                if (k < full) {
+                    const int page = ptx::ld(from + k);
+                    to[k] = page;
+                    if (in_pool(a, page)) atomicAdd(a.refs + page, 1);
+                } else if (k > full || rest == 0) {
+                    to[k] = -1;
+                }
+            }
+        } else if (rest != 0) {
+            const int s = ptx::ld(from + full), d = ptx::ld(to + full);
+            const int64_t w = v % (a.layers * kCopyBatches), layer = w / kCopyBatches;
+            const int at = int(w % kCopyBatches) * kCopyVecs;
+            if (d < 0 || at >= rest * kEntryVecs) continue;
+            if (!in_pool(a, s)) {
+                if (lane == 0) report_status(a.status, kStatusBadIndex, 6, s);
+                continue;
+            }
+            copy_batch(a.pool + (layer * a.num_pages + d) * kPageVecs, a.pool + (layer * a.num_pages + s) * kPageVecs, at, rest * kEntryVecs, lane);
+        }
+    }
+}
+
+// First half of a compaction, one block: with `count` live pages, the k-th live page from `count` on goes to the k-th free page below it (which
+// moves as few pages as possible, and none over another that has yet to move).
+__global__ void __launch_bounds__(kPagesPlanThreads) kv_compact_plan_kernel(const __grid_constant__ KvPagesArgs a) {
+    constexpr int kPerThread = 4, kChunk = kPagesPlanThreads * kPerThread;
+    __shared__ int s_warp[32];
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    const int tid = threadIdx.x;
+    int mine = 0, live = 0;
+    for (int64_t p = tid; p < a.num_pages; p += kPagesPlanThreads) mine += ptx::ld(a.refs + p) > 0;
+    block_prefix(mine, s_warp, live);
+    int holes = 0, movers = 0;
+    for (int64_t base = 0; base < a.num_pages; base += kChunk) {
+        const int64_t p = base + tid * kPerThread;
+        int hole_bits = 0, mover_bits = 0;
+#pragma unroll
+        for (int j = 0; j < kPerThread; ++j)
+            if (p + j < a.num_pages) {
+                const bool held = ptx::ld(a.refs + p + j) > 0;
+                a.remap[p + j] = int(p + j);
+                if (p + j < live ? !held : held) (p + j < live ? hole_bits : mover_bits) |= 1 << j;
+            }
+        int found_holes, found_movers;
+        int h = holes + block_prefix(__popc(hole_bits), s_warp, found_holes), m = movers + block_prefix(__popc(mover_bits), s_warp, found_movers);
+#pragma unroll
+        for (int j = 0; j < kPerThread; ++j) {
+            if ((hole_bits >> j) & 1) a.to[h++] = int(p + j);
+            if ((mover_bits >> j) & 1) a.from[m++] = int(p + j);
+        }
+        holes += found_holes;
+        movers += found_movers;
+    }
+    __syncthreads();
+    if (a.new_refs != a.refs)
+        for (int64_t p = tid; p < a.num_pages; p += kPagesPlanThreads) a.new_refs[p] = ptx::ld(a.refs + p);
+    __syncthreads();
+    // (as many holes below `live` as live pages above it)
+    for (int k = tid; k < movers; k += kPagesPlanThreads) {
+        const int s = a.from[k], d = a.to[k];
+        a.remap[s] = d;
+        a.new_refs[d] = a.new_refs[s];
+        a.new_refs[s] = 0;
+    }
+    if (tid == 0) {
+        *a.moves = movers;
+        *a.count = live;
+    }
+}
+
+// Second half: the pages move, and the tables name their new places.
+__global__ void __launch_bounds__(kPagesThreads) kv_compact_apply_kernel(const __grid_constant__ KvPagesArgs a) {
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t slots = int64_t(a.B) * a.max_pages, stride = int64_t(gridDim.x) * kPagesThreads;
+    for (int64_t i = int64_t(blockIdx.x) * kPagesThreads + threadIdx.x; i < slots; i += stride) {
+        const int page = a.block_table[i];
+        a.new_table[i] = in_pool(a, page) ? ptx::ld(a.remap + page) : page;
+    }
+    const int64_t moves = ptx::ld(a.moves), units = moves * a.layers * kCopyBatches;
+    for (int64_t u = int64_t(blockIdx.x) * (kPagesThreads / 32) + (threadIdx.x >> 5); u < units; u += int64_t(gridDim.x) * (kPagesThreads / 32)) {
+        const int64_t page = u / kCopyBatches, layer = page / moves, k = page % moves;
+        const int s = ptx::ld(a.from + k), d = ptx::ld(a.to + k);
+        copy_batch(a.pool + (layer * a.num_pages + d) * kPageVecs, a.pool + (layer * a.num_pages + s) * kPageVecs, int(u % kCopyBatches) * kCopyVecs, kPageVecs, lane);
+    }
+}
+
+}  // namespace dsv4

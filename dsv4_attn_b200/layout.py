@@ -44,3 +44,29 @@ def unpack_entries(entries: torch.Tensor) -> torch.Tensor:
     lat = (lat.reshape(*lead, N_SCALES, SCALE_BLOCK) * scale.reshape(*lead, N_SCALES, 1)).reshape(*lead, D_LATENT)
     rope = entries[..., ROPE_OFF:].contiguous().view(torch.bfloat16).float().reshape(*lead, D_ROPE)
     return torch.cat([lat, rope], dim=-1)
+
+
+def pack_tree_mask(sees: torch.Tensor) -> torch.Tensor:
+    """bool [B, T, W] (node t of request b sees window row w) -> int32 [B, T, ceil(W / 32)], the mask `hca_tree_decode` takes."""
+    if sees.dtype != torch.bool or sees.dim() != 3:
+        raise ValueError(f"expected bool [B, T, W], got {sees.dtype} {tuple(sees.shape)}")
+    B, T, W = sees.shape
+    bits = torch.nn.functional.pad(sees, (0, -W % 32)).reshape(B, T, -1, 32).to(torch.int64) << torch.arange(32, device=sees.device)
+    word = bits.sum(-1)
+    return torch.where(word >= 1 << 31, word - (1 << 32), word).to(torch.int32)
+
+
+def tree_sees(parents: torch.Tensor, committed: int) -> torch.Tensor:
+    """What the nodes of trees see of a window buffer that holds `committed` tokens, the oldest first, and then the drafts.
+    parents [B, T]: the node that node t hangs on, smaller than t, or -1 for a node that hangs on the last committed token.  A node of depth d (its
+    ancestors among the drafts) sees its ancestors, itself and the committed tokens but the d + 1 oldest: a window of `committed` tokens that ends with
+    it.  Returns bool [B, T, committed + T]."""
+    B, T = parents.shape
+    draft = torch.zeros(B, T, T, dtype=torch.bool, device=parents.device)
+    rows = torch.arange(B, device=parents.device)
+    for t in range(T):
+        up = parents[:, t].to(torch.int64)
+        draft[:, t] = draft[rows, up.clamp(min=0)] & (up >= 0)[:, None]
+        draft[:, t, t] = True
+    slid_out = draft.sum(-1, keepdim=True)
+    return torch.cat([torch.arange(committed, device=parents.device) >= slid_out, draft], dim=-1)
