@@ -9,6 +9,9 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <cmath>
+#ifdef PROBE
+#include <cstdlib>
+#endif
 #include <cstring>
 #include <atomic>
 
@@ -1021,20 +1024,15 @@ extern "C" int dsv4_kv_pages_compact(const Dsv4KvPagesParams* p, void* stream) {
 namespace {
 template <typename T>
 cudaError_t launch_sample(SampleArgs& a, cudaStream_t stream) {
-    // A block keeps up to 16,384 logits (64 KB: three blocks an SM, one computes while another loads).  Where the rows leave SMs without work, up to eight
-    // blocks share one as long as each has 4,096.
+    // Up to eight blocks share a row where the rows leave SMs without one of the two blocks they hold, as long as each has 4,096 logits; a FixedSum has a limit.
     const int span = a.V + 16 / int(sizeof(T)) - 1;                        // with what a row's alignment may put before it
     int blocks = 1;
-    while (blocks < kSampleMaxCluster && (span > blocks * 16384 || (int64_t(a.N) * blocks * 2 <= device_sms() && span > blocks * 4096))) blocks *= 2;
-    const int per_warp = (span + blocks * kSampleWarps - 1) / (blocks * kSampleWarps);
-    a.warp_span = (per_warp + kSampleStep - 1) / kSampleStep * kSampleStep;
-    const int64_t bytes = int64_t(a.warp_span) * kSampleWarps * sizeof(float);
-    const bool resident = bytes <= 200 * 1024;
-    static std::atomic<bool> done[kMaxDevices];
-    const cudaError_t e = ensure_smem(sample_kernel<T, true>, 200 * 1024, done);
-    if (e != cudaSuccess) return e;
-    return launch(resident ? sample_kernel<T, true> : sample_kernel<T, false>, dim3(unsigned(int64_t(a.N) * blocks)), kSampleThreads, resident ? size_t(bytes) : 0,
-                  stream, a, blocks);
+    while (blocks < kSampleMaxCluster && ((int64_t(a.N) * blocks <= device_sms() && span > blocks * 4096) || span / kSampleThreads / blocks >= kSampleMostTerms)) blocks *= 2;
+#ifdef PROBE
+    if (getenv("PB")) blocks = atoi(getenv("PB"));
+#endif
+    for (a.hist_shift = 0; (span / blocks + kSampleStep) >> a.hist_shift > 0xFFFF;) ++a.hist_shift;     // times 2^16 and less
+    return launch(sample_kernel<T>, dim3(unsigned(int64_t(a.N) * blocks)), kSampleThreads, 0, stream, a, blocks > 1 ? blocks : 0);
 }
 }  // namespace
 

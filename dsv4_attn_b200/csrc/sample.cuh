@@ -4,11 +4,19 @@
 // cluster size, the batch around the row or the way the sums are split (in FP32, sums in another order move the borders of the
 // distribution by 1e-7, and one row in a few hundred with a flat distribution draws its neighbour).
 //
-// A cluster of up to eight blocks works on a row.  Each block reads its part of the row once, keeps it in shared memory as FP32
-// and takes part in
-//   maximum -> (top-k, top-p: the cut, by digits of the ordered bits of the logits, with histograms that the blocks add up) -> sums of the
-//   kept weights per warp -> the warp in whose part the random number falls finds the token.
-// A cut is a pair (key, ties): kept are the tokens whose key is above it, and the first `ties` of those that have it.
+// A block, or a cluster of up to eight where there are few rows, works on a row; every warp owns neighbouring logits.  The row is read from DRAM once, for
+// its maximum; what is looked at again comes from L1 or L2 (kept in shared memory, rows of 131,072 left room for clusters of eight blocks of 16,384 only,
+// whose barriers cost more than the second reading: 1,024 rows, greedy, 302 us against 245).  Then
+//   maximum -> (top-k, top-p: the cut) -> sums of the kept weights per warp -> the part of the row in which the random number falls, again by
+//   warps -> the token.
+// A cut is a pair (logit, ties): kept are the tokens above it, and the first `ties` of those that are equal to it.
+//
+// Top-k of up to 512 a block is sought among candidates: every thread has the largest of its logits at hand, and where ceil(k / blocks) threads of each
+// block have one of at least x, at least k logits are, so that all logits from x on (some 2 k of them) hold the cut.  Only the threads that have one look
+// again.  With up to 128 tokens left, the token itself is found in the list.
+// Any other cut: a histogram over (l_max - l) / t in steps of 1/32, one 32-bit atomic per logit, says in which step the cut lies (the weights in it are
+// rounded to 16 bits of the step's largest); what lies above it is then summed exactly and the logits inside are the candidates, the neighbouring
+// step's if the exact sums say so.  Candidates too many for the lists (thousands of equal logits) are gone through by digits of their ordered bits.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -16,6 +24,7 @@
 #include <cuda_fp16.h>
 #include <math_constants.h>
 #include <stdint.h>
+#include <type_traits>
 
 #include "ptx.cuh"
 
@@ -24,14 +33,19 @@ namespace dsv4 {
 constexpr int kSampleThreads = 512;
 constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleMaxCluster = 8;
-constexpr int kSampleStep = 256;                 // elements a warp looks at at a time, eight neighbouring ones a lane
+constexpr int kSampleStep = 256;                 // logits a warp looks at at a time, eight neighbouring ones a lane
 constexpr int kSampleOneBits = 40;               // weights are multiples of 2^-40
+constexpr int kSampleBlockList = 1024;           // candidates of a block,
+constexpr int kSampleList = 2048;                // and of the cluster
+constexpr int kSampleWalk = 128;                 // kept candidates among which the token is looked for directly
+constexpr int kSampleSteps = 1024;               // steps of 1/32 in (l_max - l) / t
+constexpr int kSampleMostTerms = 4095;           // of a FixedSum
 
 struct SampleArgs {
     const void* logits;
     int64_t stride;
     int N, V;
-    int warp_span;           // elements a warp owns, a multiple of kSampleStep: neighbouring ones, in the order of the vocabulary
+    int hist_shift;          // bits left out of the histograms' weights, so that a block's sums fit 32 bits
     const float* u;
     const float* temperature;
     const int32_t* top_k;
@@ -42,14 +56,29 @@ struct SampleArgs {
 };
 
 struct SampleShared {
-    float max[kSampleMaxCluster];                                // written by every block of the cluster
-    unsigned long long sum[kSampleMaxCluster * kSampleWarps];    // kept weight above the cut, per warp of the cluster
-    uint32_t ties[kSampleMaxCluster * kSampleWarps];             // tokens at the cut
-    unsigned long long hist[2][256];                             // this block's histogram of one digit, read by the others
-    unsigned long long all[256];                                 // the cluster's
+    // written by every block of the cluster, for itself
+    float max[kSampleMaxCluster];
+    uint32_t bound[kSampleMaxCluster];                           // a key that enough of its threads reach
+    // of row_totals, in turn: a block may be at the next call while another still reads the results of one
+    uint32_t found[2][kSampleMaxCluster];                        // candidates
+    unsigned long long x[2][kSampleMaxCluster], y[2][kSampleMaxCluster];
+    unsigned long long sum[kSampleMaxCluster * kSampleWarps];    // per warp: kept weight above the cut
+    uint32_t ties[kSampleMaxCluster * kSampleWarps];             // and tokens at the cut
+    // read by the other blocks
+    unsigned long long hist[2][256];                             // one digit
+    uint32_t step_hist[kSampleSteps];                            // the distance from the maximum
+    unsigned long long list[kSampleBlockList];                   // candidates: key << 32 | ~index
+    // the block's own
+    unsigned long long sorted[kSampleList];
+    unsigned long long all[256];
     unsigned long long digit_above;
-    uint32_t digit;
+    unsigned long long warp_x[kSampleWarps], warp_y[kSampleWarps];
     float warp_max[kSampleWarps];
+    uint32_t digit, count;
+    int step;
+    // the cut, from the first block to all
+    uint32_t cut, kept;
+    unsigned long long cut_ties;
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -61,6 +90,11 @@ __device__ __forceinline__ uint32_t cluster_blocks() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
     return r;
+}
+// A rendezvous of all of the row's blocks, after which each sees what the others wrote.
+__device__ __forceinline__ void sync_row(uint32_t blocks) {
+    if (blocks > 1u) ptx::cluster_sync();
+    else __syncthreads();
 }
 __device__ __forceinline__ void sts_cluster_u64(uint32_t caddr, unsigned long long v) {
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(caddr), "l"(v) : "memory");
@@ -80,6 +114,32 @@ __device__ __forceinline__ float key_value(uint32_t k) {
     return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
 }
 
+// Sums of floor(2^40 e), e <= 1, as two sums of 20 bits each.  Added to 2^23 and rounded towards zero, e 2^20 leaves its whole part in the low bits of
+// the sum; what is left of it is exact, and gives the other 20 bits the same way: five instructions, where shifting and adding in 64 bits take ten.
+// At most 4,095 terms.
+struct FixedSum {
+    uint32_t hi = 0, lo = 0;     // less 0x4B000000, the bits of 2^23, per term
+    int terms = 0;
+    __device__ __forceinline__ void add(float e) {
+        const float h = __fmaf_rz(e, 1048576.f, 8388608.f), rest = __fmaf_rn(e, 1048576.f, 8388608.f - h);
+        hi += __float_as_uint(h);
+        lo += __float_as_uint(__fmaf_rz(rest, 1048576.f, 8388608.f));
+        ++terms;
+    }
+    __device__ __forceinline__ unsigned long long total() const {
+        const uint32_t off = uint32_t(terms) * 0x4B000000u;
+        return ((unsigned long long)(hi - off) << 20) + (lo - off);
+    }
+};
+__device__ __forceinline__ unsigned long long fixed(float e) {
+    FixedSum s;
+    s.add(e);
+    return s.total();
+}
+__device__ __forceinline__ float max_of(const float (&v)[8]) {
+    return fmaxf(ptx::max3(ptx::max3(v[0], v[1], v[2]), v[3], v[4]), ptx::max3(v[5], v[6], v[7]));
+}
+
 // What a row's settings come to.
 struct SampleRow {
     float top;               // largest logit
@@ -89,19 +149,24 @@ struct SampleRow {
     int p24;                 // top-p in multiples of 2^-24, -1: off
     bool greedy;
 
-    // exp((l - top) / t), in the operations and the order in which it is defined (no contraction, CUDA's expf)
-    __device__ __forceinline__ float exponent(float l) const { return l == top ? 0.f : __fmul_rn(__fsub_rn(l, top), per); }
+    // The exponent (l - top) / t of a logit: the operations of the definition, in its order.  The minimum turns the NaN of inf - inf and 0 * inf, which
+    // only the largest logits can come to, into 0.
+    __device__ __forceinline__ float exponent(float l) const { return fminf(__fmul_rn(__fsub_rn(l, top), per), 0.f); }
     __device__ __forceinline__ float ratio(float l) const { return expf(exponent(l)); }
-    // floor(2^40 e) from the bits of e <= 1 (a conversion of the product to 64 bits takes four times as long)
-    static __device__ __forceinline__ unsigned long long fixed(float e) {
-        const uint32_t b = __float_as_uint(e), shift = 127u - (b >> 23);
-        return (uint64_t((b & 0x7FFFFFu) | 0x800000u) << (kSampleOneBits - 23)) >> min(shift, 63u);
+    // the step of a finite logit in (l_max - l) / t
+    __device__ __forceinline__ int step(float x) const { return min(int(x * -32.f), kSampleSteps - 1); }
+    // Biased exponent above that of the step's largest weight, exp(-step / 32).
+    static __device__ __forceinline__ int step_exponent(int step) { return 128 - ((step * 1477) >> 15); }
+    // exp(x) in 16 bits below it
+    static __device__ __forceinline__ uint32_t step_weight(float e, int step, int drop) {
+        const uint32_t b = __float_as_uint(e);
+        const int shift = 8 + drop + step_exponent(step) - int(b >> 23);
+        return ((b & 0x7FFFFFu) | 0x800000u) >> min(max(shift, 0), 31);
     }
     __device__ __forceinline__ unsigned long long weight(float l) const {
         const float e = ratio(l);
         return e >= min_p ? fixed(e) : 0ull;
     }
-    __device__ __forceinline__ unsigned long long weight_unfiltered(float l) const { return fixed(ratio(l)); }
 };
 
 // floor(total * m / 2^24)
@@ -115,45 +180,114 @@ __device__ __forceinline__ uint32_t in_24_bits(float x) {       // floor(2^24 x)
 __device__ __forceinline__ float logit_value(float x) { return x; }
 __device__ __forceinline__ float logit_value(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float logit_value(__half x) { return __half2float(x); }
-// NaN counts as -inf, and -0 as 0
-__device__ __forceinline__ float clean_logit(float x) { return x == x ? x + 0.f : -CUDART_INF_F; }
+template <typename T> __device__ __forceinline__ T no_logit();
+template <> __device__ __forceinline__ float no_logit<float>() { return -CUDART_INF_F; }
+template <> __device__ __forceinline__ __nv_bfloat16 no_logit<__nv_bfloat16>() { return __ushort_as_bfloat16(0xFF80); }
+template <> __device__ __forceinline__ __half no_logit<__half>() { return __ushort_as_half(0xFC00); }
 
-// The row as a warp sees it: the elements it owns, eight a lane and step.
-template <typename T, bool RESIDENT>
-struct RowPart {
-    const T* base;           // 16-byte aligned: element 0 is `lead` elements before the row's first
-    int lead, end;           // the row is [lead, end)
-    int first;               // the warp's first element
-    float* kept;             // resident: the warp's elements as FP32, step by step, the lanes' first four and then their last four
-    int lane;
+// A row, whose elements are counted from the 16-byte boundary at or before its start: it is [lead, end).
+template <typename T>
+struct LogitRow {
+    static constexpr int kBatch = 4;             // steps whose loads are in flight at once
+    static constexpr int kVecs = int(sizeof(T)) / 2;
+    const T* base;
+    int lead, end, lane;
 
-    __device__ __forceinline__ int at(int step) const { return first + step * kSampleStep + lane * 8; }
-    __device__ __forceinline__ void load(int step, float (&v)[8]) const {
-        const int e = at(step);
-        if (e >= lead && e + 8 <= end) {
-            alignas(16) T x[8];
+    // The largest logit of this thread's, for the warp's `steps` steps from element `first` on; NaN left out, -inf where there is none.  Sixteen-bit logits
+    // are compared two at a time.
+    __device__ __forceinline__ float largest(int first, int steps) const {
+        constexpr int kDeep = 16 / kVecs;        // loads in flight: 16 of 16 bytes
+        float top = -CUDART_INF_F;
+        int s = 0;
+        // (the warp's first step may begin before the row, its last one end behind it)
+        while (s < steps && first + s * kSampleStep < lead) top = fmaxf(top, largest_of_edge(first + s++ * kSampleStep + lane * 8));
+        const int whole = min(steps, (end - first) / kSampleStep);
+        Pair best[4];
 #pragma unroll
-            for (int i = 0; i < int(sizeof(x) / 16); ++i) reinterpret_cast<uint4*>(x)[i] = ptx::ldg_stream_v4(reinterpret_cast<const uint4*>(base + e) + i);
+        for (int i = 0; i < 4; ++i) best[i] = none();
+#pragma unroll 1
+        for (; s + kDeep <= whole; s += kDeep) {
+            uint4 x[kDeep][kVecs];
+            const uint4* p = reinterpret_cast<const uint4*>(base + first + s * kSampleStep + lane * 8);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = clean_logit(logit_value(x[i]));
-        } else {
+            for (int j = 0; j < kDeep; ++j)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = e + i >= lead && e + i < end ? clean_logit(logit_value(ptx::ld(base + e + i))) : -CUDART_INF_F;
+                for (int i = 0; i < kVecs; ++i) x[j][i] = ptx::ld(p + j * 32 * kVecs + i);
+#pragma unroll
+            for (int j = 0; j < kDeep; ++j)
+#pragma unroll
+                for (int i = 0; i < kVecs; ++i) keep(best, x[j][i]);
         }
+        for (; s < whole; ++s)
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) keep(best, ptx::ld(reinterpret_cast<const uint4*>(base + first + s * kSampleStep + lane * 8) + i));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, value(best[i]));
+        for (; s < steps; ++s) top = fmaxf(top, largest_of_edge(first + s * kSampleStep + lane * 8));
+        return top;
     }
-    __device__ __forceinline__ void keep(int step, const float (&v)[8]) const {
-        float4* p = reinterpret_cast<float4*>(kept + step * kSampleStep) + lane;
-        p[0] = make_float4(v[0], v[1], v[2], v[3]);
-        p[32] = make_float4(v[4], v[5], v[6], v[7]);
+    __device__ __forceinline__ float largest_of_edge(int e) const {
+        float top = -CUDART_INF_F;
+        for (int i = max(e, lead); i < min(e + 8, end); ++i) top = fmaxf(top, logit_value(ptx::ld(base + i)));
+        return top;
     }
-    __device__ __forceinline__ void get(int step, float (&v)[8]) const {
-        if constexpr (RESIDENT) {
-            const float4* p = reinterpret_cast<const float4*>(kept + step * kSampleStep) + lane;
-            const float4 a = p[0], b = p[32];
-            v[0] = a.x;  v[1] = a.y;  v[2] = a.z;  v[3] = a.w;
-            v[4] = b.x;  v[5] = b.y;  v[6] = b.z;  v[7] = b.w;
-        } else {
-            load(step, v);
+    // two 16-bit logits, or one of 32 bits
+    struct Pair { uint32_t bits; };
+    static __device__ __forceinline__ Pair none() { return {sizeof(T) == 4 ? 0xFF800000u : (sizeof(T) == 2 && is_bf16() ? 0xFF80FF80u : 0xFC00FC00u)}; }
+    static __host__ __device__ constexpr bool is_bf16() { return std::is_same<T, __nv_bfloat16>::value; }
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+        uint32_t r;
+        if constexpr (sizeof(T) == 4) return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+        else if constexpr (is_bf16()) asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        else asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ void keep(Pair (&best)[4], const uint4& x) {
+        best[0].bits = larger(best[0].bits, x.x);
+        best[1].bits = larger(best[1].bits, x.y);
+        best[2].bits = larger(best[2].bits, x.z);
+        best[3].bits = larger(best[3].bits, x.w);
+    }
+    static __device__ __forceinline__ float value(Pair p) {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(p.bits);
+        else if constexpr (is_bf16()) return fmaxf(__uint_as_float(p.bits << 16), __uint_as_float(p.bits & 0xFFFF0000u));
+        else { const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p.bits));  return fmaxf(f.x, f.y); }
+    }
+
+    // visit(v, e): the eight logits from e on, for the warp's `steps` steps from element `first` on.  NaN, and what is not of the row, is -inf.
+    template <typename Visit>
+    __device__ __forceinline__ void each(int first, int steps, Visit visit) const {
+#pragma unroll 1
+        for (int s = 0; s < steps; s += kBatch) {
+            const int e0 = first + s * kSampleStep;
+            alignas(16) T x[kBatch][8];
+            if (e0 >= lead && e0 + kBatch * kSampleStep <= end) {
+                const uint4* p = reinterpret_cast<const uint4*>(base + e0 + lane * 8);
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+                    for (int i = 0; i < kVecs; ++i) reinterpret_cast<uint4*>(x[j])[i] = ptx::ld(p + j * 32 * kVecs + i);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j) {
+                    const int e = e0 + j * kSampleStep + lane * 8;
+                    if (e >= lead && e + 8 <= end) {
+#pragma unroll
+                        for (int i = 0; i < kVecs; ++i) reinterpret_cast<uint4*>(x[j])[i] = ptx::ld(reinterpret_cast<const uint4*>(base + e) + i);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) x[j][i] = e + i >= lead && e + i < end ? ptx::ld(base + e + i) : no_logit<T>();
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j)
+                if (s + j < steps) {
+                    float v[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = fmaxf(logit_value(x[j][i]), -CUDART_INF_F);
+                    visit(v, e0 + j * kSampleStep + lane * 8);
+                }
         }
     }
 };
@@ -172,11 +306,32 @@ __device__ __forceinline__ unsigned long long warp_upto(unsigned long long v, in
     return v;
 }
 
-// One digit of a cut.  The blocks' histograms of bits [shift, shift + 8) have been filled; in descending order of the digit, the first one up to which
-// at least `wanted` lies goes to sh.digit, what lies above it to sh.digit_above.  Returns the sum over all digits.  Every thread of the
-// cluster calls.
-__device__ __forceinline__ unsigned long long find_digit(SampleShared& sh, int buffer, unsigned long long wanted, uint32_t blocks) {
-    ptx::cluster_sync();                           // (releases and acquires: every block's histogram is complete)
+// Two sums over the row, and the blocks' counts of candidates.  `turn` changes with every call.  Every thread of the cluster calls.
+__device__ __forceinline__ void row_totals(SampleShared& sh, uint32_t blocks, uint32_t rank, int& turn, unsigned long long& x, unsigned long long& y) {
+    turn ^= 1;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    x = warp_total(x);
+    y = warp_total(y);
+    if (lane == 0) { sh.warp_x[warp] = x;  sh.warp_y[warp] = y; }
+    __syncthreads();
+    if (warp == 0) {
+        x = warp_total(lane < kSampleWarps ? sh.warp_x[lane] : 0ull);
+        y = warp_total(lane < kSampleWarps ? sh.warp_y[lane] : 0ull);
+        if (lane < int(blocks)) {
+            ptx::sts_cluster_u32(ptx::mapa(ptx::smem_u32(&sh.found[turn][rank]), lane), sh.count);
+            sts_cluster_u64(ptx::mapa(ptx::smem_u32(&sh.x[turn][rank]), lane), x);
+            sts_cluster_u64(ptx::mapa(ptx::smem_u32(&sh.y[turn][rank]), lane), y);
+        }
+    }
+    sync_row(blocks);
+    x = y = 0ull;
+    for (uint32_t b = 0; b < blocks; ++b) { x += sh.x[turn][b];  y += sh.y[turn][b]; }
+}
+
+// One digit of a cut.  The blocks' histograms of one digit have been filled; in descending order of the digit, the first one up to which
+// at least `wanted` lies goes to sh.digit, what lies above it to sh.digit_above.  Every thread of the cluster calls.
+__device__ __forceinline__ void find_digit(SampleShared& sh, int buffer, unsigned long long wanted, uint32_t blocks) {
+    sync_row(blocks);
     const int tid = threadIdx.x, lane = tid & 31;
     if (tid < 256) {
         const uint32_t at = ptx::smem_u32(&sh.hist[buffer][tid]);
@@ -185,25 +340,148 @@ __device__ __forceinline__ unsigned long long find_digit(SampleShared& sh, int b
         sh.all[255 - tid] = s;
     }
     __syncthreads();
-    // all warps alike: lane l has the digits 255 - 8 l down to 248 - 8 l
-    unsigned long long v[8], mine = 0;
+    if (tid < 32) {
+        // lane l has the digits 255 - 8 l down to 248 - 8 l
+        unsigned long long v[8], mine = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) { v[i] = sh.all[lane * 8 + i];  mine += v[i]; }
-    const unsigned long long upto = warp_upto(mine, lane);
-    unsigned long long above = upto - mine;
-    if (tid < 32 && above < wanted && upto >= wanted) {
-        int i = 0;
-        while (i < 7 && above + v[i] < wanted) above += v[i++];
-        sh.digit = uint32_t(255 - (lane * 8 + i));
-        sh.digit_above = above;
+        for (int i = 0; i < 8; ++i) { v[i] = sh.all[lane * 8 + i];  mine += v[i]; }
+        const unsigned long long upto = warp_upto(mine, lane);
+        unsigned long long above = upto - mine;
+        if (above < wanted && upto >= wanted) {
+            int i = 0;
+#pragma unroll
+            for (int j = 0; j < 7; ++j)
+                if (i == j && above + v[j] < wanted) { above += v[j];  i = j + 1; }
+            sh.digit = uint32_t(255 - (lane * 8 + i));
+            sh.digit_above = above;
+        }
     }
     __syncthreads();
-    return __shfl_sync(0xFFFFFFFFu, upto, 31);
 }
 
-template <typename T, bool RESIDENT>
-__global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_constant__ SampleArgs a) {
-    extern __shared__ __align__(16) float s_row[];
+// sh.sorted[0, n) into descending order; filled up with zeros to a power of two.  Every thread of the block calls.
+__device__ __forceinline__ void sort_list(SampleShared& sh, int n) {
+    const int tid = threadIdx.x;
+    int size = 64;
+    while (size < n) size *= 2;
+    for (int i = n + tid; i < size; i += kSampleThreads) sh.sorted[i] = 0ull;
+    __syncthreads();
+#pragma unroll 1
+    for (int run = 2; run <= size; run *= 2)
+#pragma unroll 1
+        for (int stride = run / 2; stride > 0; stride /= 2) {
+            for (int p = tid; p < size / 2; p += kSampleThreads) {
+                const int i = 2 * p - (p & (stride - 1)), j = i + stride;
+                const unsigned long long x = sh.sorted[i], y = sh.sorted[j];
+                const bool up = (i & run) != 0;
+                if ((x < y) != up) { sh.sorted[i] = y;  sh.sorted[j] = x; }
+            }
+            // (from a stride of 32 down a warp's pairs are those of 64 neighbouring entries, here and in the next step)
+            if (stride > 32 || (stride == 1 && run >= 64)) __syncthreads();
+            else __syncwarp();
+        }
+    __syncthreads();
+}
+
+// A logit goes to the block's list.  (+ 0: -0 is 0)
+__device__ __forceinline__ void list_logit(SampleShared& sh, float l, int index) {
+    const uint32_t at = atomicAdd(&sh.count, 1u);
+    if (at < uint32_t(kSampleBlockList)) sh.list[at] = (static_cast<unsigned long long>(order_key(l + 0.f)) << 32) | uint32_t(~index);
+}
+
+// How many candidates the lists have (-1: too many), after row_totals.
+__device__ __forceinline__ int listed(const SampleShared& sh, uint32_t blocks, int turn) {
+    int n = 0;
+    bool fits = true;
+    for (uint32_t b = 0; b < blocks; ++b) {
+        fits = fits && sh.found[turn][b] <= uint32_t(kSampleBlockList);
+        n += int(min(sh.found[turn][b], uint32_t(kSampleList)));
+    }
+    return fits && n <= kSampleList ? n : -1;
+}
+
+// The cut among the candidates of all blocks (n of them, in sh.sorted afterwards, in descending order): the first k, and of those the ones before which less
+// than `most` lies (0: the share of the k that top-p says).  To sh.cut, sh.cut_ties and sh.kept.  Every thread of the first block calls.
+__device__ __forceinline__ void cut_of_list(SampleShared& sh, const SampleRow& r, uint32_t blocks, int turn, int n, int k, unsigned long long most) {
+    constexpr int kPer = kSampleList / kSampleThreads;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    for (int i = tid; i < n; i += kSampleThreads) {
+        uint32_t b = 0, at = uint32_t(i);
+        while (at >= sh.found[turn][b]) at -= sh.found[turn][b++];
+        sh.sorted[i] = blocks > 1u ? lds_cluster_u64(ptx::mapa(ptx::smem_u32(&sh.list[at]), b)) : sh.list[at];
+    }
+    sort_list(sh, n);
+    unsigned long long w[kPer], mine = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int at = tid * kPer + i;
+        w[i] = at < k ? fixed(r.ratio(key_value(uint32_t(sh.sorted[at] >> 32)))) : 0ull;
+        mine += w[i];
+    }
+    unsigned long long ahead = warp_upto(mine, lane) - mine;
+    if (lane == 31) sh.warp_x[warp] = ahead + mine;
+    __syncthreads();
+    const unsigned long long of_warp = lane < kSampleWarps ? sh.warp_x[lane] : 0ull, upto = warp_upto(of_warp, lane);
+    if (most == 0ull) most = max(share_of(__shfl_sync(0xFFFFFFFFu, upto, 31), uint32_t(r.p24)), 1ull);
+    ahead += __shfl_sync(0xFFFFFFFFu, upto - of_warp, warp);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int at = tid * kPer + i;
+        const bool kept = at < k && ahead < most;
+        ahead += w[i];
+        if (kept && (at + 1 >= k || ahead >= most)) {              // the last one kept
+            const uint32_t key = uint32_t(sh.sorted[at] >> 32);
+            int lo = 0, hi = at;                                   // the first one with its key
+            while (lo < hi) {
+                const int mid = (lo + hi) / 2;
+                if (uint32_t(sh.sorted[mid] >> 32) > key) lo = mid + 1;
+                else hi = mid;
+            }
+            sh.cut = key;
+            sh.cut_ties = static_cast<unsigned long long>(at - lo + 1);
+            sh.kept = uint32_t(at + 1);
+        }
+    }
+    __syncthreads();
+    if (tid > 0 && tid < int(blocks)) {
+        ptx::sts_cluster_u32(ptx::mapa(ptx::smem_u32(&sh.cut), tid), sh.cut);
+        ptx::sts_cluster_u32(ptx::mapa(ptx::smem_u32(&sh.kept), tid), sh.kept);
+        sts_cluster_u64(ptx::mapa(ptx::smem_u32(&sh.cut_ties), tid), sh.cut_ties);
+    }
+}
+
+// The token among the sh.kept <= kSampleWalk candidates of sh.sorted: a thread each adds up what the kept candidates of lower index weigh.
+__device__ __forceinline__ void token_of_list(SampleShared& sh, const SampleRow& r, const SampleArgs& a, int n, uint32_t u24) {
+    const int tid = threadIdx.x, kept = int(sh.kept);
+    float x = 0.f;
+    unsigned long long w = 0;
+    int index = 0;
+    if (tid < kept) {
+        const unsigned long long c = sh.sorted[tid];
+        x = r.exponent(key_value(uint32_t(c >> 32)));
+        const float e = expf(x);
+        w = e >= r.min_p ? fixed(e) : 0ull;
+        index = int(~uint32_t(c));
+        sh.all[tid] = w;
+    }
+    __syncthreads();
+    if (tid >= kept) return;
+    unsigned long long total = 0, before = 0;
+#pragma unroll 4
+    for (int j = 0; j < kept; ++j) {
+        const unsigned long long wj = sh.all[j];
+        total += wj;
+        if (int(~uint32_t(sh.sorted[j])) < index) before += wj;
+    }
+    const unsigned long long target = share_of(total, u24);
+    if (target >= before && target < before + w) {
+        a.token[n] = index;
+        if (a.logprob != nullptr) a.logprob[n] = x - logf(__ull2float_rn(total) * 9.094947017729282e-13f);
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a) {
     __shared__ SampleShared sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = cluster_rank(), blocks = cluster_blocks();
@@ -211,32 +489,25 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
     ptx::pdl_trigger();
     ptx::pdl_wait();
     // (the other blocks' shared memory may be written once they are there; that is waited for below)
-    asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+    if (blocks > 1u) asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
 
-    const T* row = static_cast<const T*>(a.logits) + int64_t(n) * a.stride;
-    RowPart<T, RESIDENT> part;
-    part.lead = int((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
-    part.base = row - part.lead;
-    part.end = part.lead + a.V;
-    part.first = (int(rank) * kSampleWarps + warp) * a.warp_span;
-    part.kept = s_row + warp * a.warp_span;
-    part.lane = lane;
-    const int steps = a.warp_span / kSampleStep;
+    const T* start = static_cast<const T*>(a.logits) + int64_t(n) * a.stride;
+    LogitRow<T> row;
+    row.lead = int((reinterpret_cast<uintptr_t>(start) & 15u) / sizeof(T));
+    row.base = start - row.lead;
+    row.end = row.lead + a.V;
+    row.lane = lane;
+    // The row's steps are dealt out evenly: every warp of the cluster has neighbouring ones, in the order of the vocabulary.
+    const int row_steps = (row.end + kSampleStep - 1) / kSampleStep, parts = int(blocks) * kSampleWarps, me = int(rank) * kSampleWarps + warp;
+    auto first_step = [&](int part) { return int(int64_t(row_steps) * part / parts); };
+    const int first = first_step(me) * kSampleStep, steps = first_step(me + 1) - first_step(me);
 
     // ── maximum ──
+    const float mine = row.largest(first, steps);
     SampleRow r;
-    r.top = -CUDART_INF_F;
-#pragma unroll 4
-    for (int s = 0; s < steps; ++s) {
-        float v[8];
-        part.load(s, v);
-        if constexpr (RESIDENT) part.keep(s, v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) r.top = fmaxf(r.top, v[i]);
-    }
     const float t = a.temperature != nullptr ? ptx::ld(a.temperature + n) : 1.f;
     r.greedy = !(t > 0.f);
-    r.per = r.greedy ? 1.f : __frcp_rn(t);
+    r.per = r.greedy ? 1.f : fmaxf(__frcp_rn(t), __uint_as_float(1u));      // (an infinite temperature: -inf has to stay -inf)
     const int k = a.top_k != nullptr ? ptx::ld(a.top_k + n) : 0;
     r.k = k > 0 && k < a.V ? k : 0;
     const float p = a.top_p != nullptr ? ptx::ld(a.top_p + n) : 1.f;
@@ -244,18 +515,37 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
     const float mp = a.min_p != nullptr ? ptx::ld(a.min_p + n) : 0.f;
     r.min_p = mp > 0.f ? fminf(mp, 1.f) : 0.f;
     const uint32_t u24 = min(in_24_bits(ptx::ld(a.u + n)), 0xFFFFFFu);
+    r.top = mine;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) r.top = fmaxf(r.top, __shfl_xor_sync(0xFFFFFFFFu, r.top, o));
     if (lane == 0) sh.warp_max[warp] = r.top;
-    for (int i = tid; i < 512; i += kSampleThreads) (&sh.hist[0][0])[i] = 0ull;
+    if (tid == 0) { sh.count = 0u;  sh.kept = 0x7FFFFFFFu; }
     __syncthreads();
+    // a key that enough threads' largest logits reach: from the top, a bit at a time
+    const int groups = (r.k + int(blocks) - 1) / int(blocks);
+    const bool by_list = !r.greedy && r.k > 0 && groups <= kSampleThreads;
+    uint32_t bound = 0u;
+    if (by_list) {
+        const uint32_t key = order_key(mine);
+#pragma unroll 1
+        for (uint32_t bit = 0x80000000u; bit >= 0x8000u; bit >>= 1)
+            if (__syncthreads_count(key >= (bound | bit)) >= groups) bound |= bit;
+    }
     r.top = sh.warp_max[lane & (kSampleWarps - 1)];
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) r.top = fmaxf(r.top, __shfl_xor_sync(0xFFFFFFFFu, r.top, o));
-    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
-    if (tid < int(blocks)) ptx::sts_cluster_u32(ptx::mapa(ptx::smem_u32(&sh.max[rank]), tid), __float_as_uint(r.top));
-    ptx::cluster_sync();
-    for (uint32_t b = 0; b < blocks; ++b) r.top = fmaxf(r.top, sh.max[b]);
+    if (blocks > 1u) {
+        asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+        if (tid < int(blocks)) {
+            ptx::sts_cluster_u32(ptx::mapa(ptx::smem_u32(&sh.max[rank]), tid), __float_as_uint(r.top));
+            ptx::sts_cluster_u32(ptx::mapa(ptx::smem_u32(&sh.bound[rank]), tid), bound);
+        }
+        ptx::cluster_sync();
+        for (uint32_t b = 0; b < blocks; ++b) {
+            r.top = fmaxf(r.top, sh.max[b]);
+            bound = min(bound, sh.bound[b]);
+        }
+    }
     if (r.top == -CUDART_INF_F) {                  // the same in every block: nothing to draw from
         if (rank == 0 && tid == 0) {
             a.token[n] = -1;
@@ -263,175 +553,325 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(const __grid_con
         }
         return;
     }
+    if (r.greedy) {
+        // the lowest index of the largest logit
+        if (mine == r.top)
+            row.each(first, steps, [&](const float (&v)[8], int e) {
+#pragma unroll
+                for (int i = 7; i >= 0; --i)
+                    if (v[i] == r.top) atomicMin(&sh.kept, uint32_t(e + i - row.lead));
+            });
+        __syncthreads();
+        uint32_t token = sh.kept;
+        if (blocks > 1u) {
+            if (tid == 0) ptx::sts_cluster_u32(ptx::mapa(ptx::smem_u32(&sh.found[0][rank]), 0), token);
+            ptx::cluster_sync();
+            for (uint32_t b = 0; b < blocks; ++b) token = min(token, sh.found[0][b]);
+        }
+        if (rank == 0 && tid == 0) {
+            a.token[n] = int(token);
+            if (a.logprob != nullptr) a.logprob[n] = 0.f;
+        }
+        return;
+    }
 
     // ── the cut ──
-    uint32_t cut = 0;                              // every key is above 0
+    uint32_t cut = 0;                              // a key; every key is above 0
     unsigned long long cut_ties = 0;
-    int buffer = 0;
-    auto clear = [&](int b) {
-        __syncthreads();
-        for (int i = tid; i < 256; i += kSampleThreads) sh.hist[b][i] = 0ull;
-        __syncthreads();
-    };
-    if (r.greedy) {
-        cut = order_key(r.top);
-        cut_ties = 1;
-    } else {
-        if (r.k > 0) {
-            unsigned long long wanted = (unsigned long long)(r.k);
-            for (int shift = 24; shift >= 0; shift -= 8) {
-                for (int s = 0; s < steps; ++s) {
-                    float v[8];
-                    part.get(s, v);
+    int turn = 0;
+    bool have_cut = r.k == 0 && r.p24 < 0;
+    if (by_list) {
+        const float from = fmaxf(key_value(bound), -3.402823466e38f);       // (-inf is no candidate)
+        if (mine >= from)
+            row.each(first, steps, [&](const float (&v)[8], int e) {
+                if (max_of(v) < from) return;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const uint32_t key = order_key(v[i]);
-                        if (shift == 24 || (key >> (shift + 8)) == (cut >> (shift + 8))) atomicAdd(&sh.hist[buffer][(key >> shift) & 255u], 1ull);
+                for (int i = 0; i < 8; ++i)
+                    if (v[i] >= from) list_logit(sh, v[i], e + i - row.lead);
+            });
+        unsigned long long x = 0, y = 0;
+        row_totals(sh, blocks, rank, turn, x, y);
+        const int m = listed(sh, blocks, turn);
+        if (m >= 0) {
+            if (rank == 0) cut_of_list(sh, r, blocks, turn, m, min(r.k, m), r.p24 < 0 ? ~0ull : 0ull);
+            sync_row(blocks);
+            if (sh.kept <= uint32_t(kSampleWalk)) {
+                if (rank == 0) token_of_list(sh, r, a, n, u24);
+                return;
+            }
+            cut = sh.cut;
+            cut_ties = sh.cut_ties;
+            have_cut = true;
+        }
+    }
+    if (!have_cut) {
+        // The cut up to which `wanted` lies, among the finite logits above `above` (a key): tokens, or weight, of which `wanted` is then the share that
+        // top-p says of all of it and of `ties`, the weight of the tokens kept at `above`.  False: it lies beyond (in the ties; no cut at all).
+        auto find_cut = [&](bool by_weight, uint32_t above, unsigned long long wanted, unsigned long long ties, unsigned long long& over) -> bool {
+            const float above_value = above != 0u ? key_value(above) : -CUDART_INF_F;
+            for (int i = tid; i < kSampleSteps; i += kSampleThreads) sh.step_hist[i] = 0u;
+            if (tid == 0) sh.step = 0;
+            __syncthreads();
+            FixedSum sum;
+            uint32_t count = 0;
+            row.each(first, steps, [&](const float (&v)[8], int) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const bool in = v[i] > above_value;
+                    const float x = r.exponent(v[i]), e = in ? expf(x) : 0.f;
+                    const int step = r.step(x);
+                    if (by_weight) {
+                        sum.add(e);
+                        if (in && x > -28.f) atomicAdd(&sh.step_hist[step], SampleRow::step_weight(e, step, a.hist_shift));       // (a weight below 2^-40 is 0)
+                    } else if (in) {
+                        ++count;
+                        atomicAdd(&sh.step_hist[step], 1u);
                     }
                 }
-                find_digit(sh, buffer, wanted, blocks);
-                cut |= sh.digit << shift;
-                wanted -= sh.digit_above;
-                buffer ^= 1;
-                clear(buffer);                     // (two uses ago: every block has read it, since it has come to the barrier of the last one)
+            });
+            unsigned long long unused = 0;
+            over = by_weight ? sum.total() : count;
+            row_totals(sh, blocks, rank, turn, over, unused);
+            if (by_weight) wanted = max(share_of(over + ties, uint32_t(r.p24)), 1ull);
+            if (wanted > over) { over = wanted - over;  return false; }
+            // two neighbouring steps a thread
+            unsigned long long v[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int step = 2 * tid + i;
+                const uint32_t at = ptx::smem_u32(&sh.step_hist[step]);
+                unsigned long long steps_sum = 0;
+                if (blocks > 1u)
+                    for (uint32_t b = 0; b < blocks; ++b) steps_sum += ptx::lds_cluster_u32(ptx::mapa(at, b));
+                else
+                    steps_sum = sh.step_hist[step];
+                if (steps_sum != 0ull) atomicMax(&sh.step, step);      // (the last one, where rounding leaves the sum short of `wanted`)
+                const int up = SampleRow::step_exponent(step) - 102 + a.hist_shift;
+                v[i] = !by_weight ? steps_sum : (up >= 0 ? steps_sum << up : steps_sum >> -up);
             }
-            cut_ties = wanted;
-        }
-        if (r.p24 >= 0) {
-            const uint32_t above = cut;            // top-p looks at the tokens above top-k's cut, and at those of its ties that are kept
-            unsigned long long most = 0, ahead = 0;
-            uint32_t found = 0;
-            bool inside = true;
-            for (int shift = 24; shift >= 0 && inside; shift -= 8) {
-                for (int s = 0; s < steps; ++s) {
-                    float v[8];
-                    part.get(s, v);
+            unsigned long long before = warp_upto(v[0] + v[1], lane) - v[0] - v[1];
+            if (lane == 31) sh.warp_x[warp] = before + v[0] + v[1];
+            __syncthreads();
+            const unsigned long long of_warp = lane < kSampleWarps ? sh.warp_x[lane] : 0ull, upto_warp = warp_upto(of_warp, lane);
+            before += __shfl_sync(0xFFFFFFFFu, upto_warp - of_warp, warp);
+            if (before < wanted && before + v[0] + v[1] >= wanted) sh.step = 2 * tid + (before + v[0] < wanted ? 1 : 0);
+            __syncthreads();
+            int step = sh.step;
+            unsigned long long ahead, inside;
+            for (int moved = 0;;) {
+                __syncthreads();
+                if (tid == 0) sh.count = 0u;
+                __syncthreads();
+                FixedSum sum_ahead, sum_inside;
+                uint32_t n_ahead = 0, n_inside = 0;
+                // (a logit below `reach` is beyond the step for certain: a little further than the step's end)
+                const float from = float(step), to = step == kSampleSteps - 1 ? CUDART_INF_F : from + 1.f;
+                float reach = r.top - to * 0.03126f / r.per - 1e-5f * fabsf(r.top);
+                if (!(reach < r.top)) reach = -CUDART_INF_F;
+                row.each(first, steps, [&](const float (&v)[8], int e) {
+                    if (!__any_sync(0xFFFFFFFFu, max_of(v) >= reach)) return;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const uint32_t key = order_key(v[i]);
-                        if (key > above && (shift == 24 || (key >> (shift + 8)) == (found >> (shift + 8)))) {
-                            const unsigned long long w = r.weight_unfiltered(v[i]);
-                            if (w != 0ull) atomicAdd(&sh.hist[buffer][(key >> shift) & 255u], w);
+                        const float x = r.exponent(v[i]), at = x * -32.f;
+                        const bool in = v[i] > above_value && at < to, is_inside = in && at >= from;
+                        if (by_weight) {
+                            const float w = in ? expf(x) : 0.f;
+                            sum_ahead.add(is_inside ? 0.f : w);
+                            if (is_inside) sum_inside.add(w);
+                        } else {
+                            n_ahead += in && !is_inside;
+                            n_inside += is_inside;
+                        }
+                        if (is_inside) list_logit(sh, v[i], e + i - row.lead);
+                    }
+                });
+                ahead = by_weight ? sum_ahead.total() : n_ahead;
+                inside = by_weight ? sum_inside.total() : n_inside;
+                row_totals(sh, blocks, rank, turn, ahead, inside);
+                // (the rounded sums can be off by a step: towards the top and then back again cannot be)
+                if (wanted <= ahead && step > 0 && moved <= 0) { --step;  moved = -1;  continue; }
+                if (wanted > ahead + inside && step + 1 < kSampleSteps && moved >= 0) { ++step;  moved = 1;  continue; }
+                break;
+            }
+            wanted -= ahead;
+            const int m = listed(sh, blocks, turn);
+            if (m >= 0) {
+                if (rank == 0) cut_of_list(sh, r, blocks, turn, m, by_weight ? m : int(wanted), by_weight ? wanted : ~0ull);
+                sync_row(blocks);
+                cut = sh.cut;
+                cut_ties = sh.cut_ties;
+                return true;
+            }
+            uint32_t found = 0;
+            int buffer = 0;
+            for (int i = tid; i < 256; i += kSampleThreads) sh.hist[0][i] = 0ull;
+#pragma unroll 1
+            for (int shift = 24; shift >= 0; shift -= 8) {
+                __syncthreads();
+                row.each(first, steps, [&](const float (&v)[8], int) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const uint32_t key = order_key(v[i] + 0.f);
+                        const float x = r.exponent(v[i]);
+                        const bool in = v[i] > above_value && r.step(x) == step && (shift == 24 || (key >> (shift + 8)) == (found >> (shift + 8)));
+                        const uint32_t digit = (key >> shift) & 255u, who = __ballot_sync(0xFFFFFFFFu, in);
+                        if (who != 0u) {
+                            unsigned long long w = in ? (by_weight ? fixed(expf(x)) : 1ull) : 0ull;
+                            // (equal logits, the usual case here, with one atomic a warp)
+                            const uint32_t same = __shfl_sync(0xFFFFFFFFu, digit, __ffs(who) - 1);
+                            if (__all_sync(0xFFFFFFFFu, !in || digit == same)) {
+                                w = warp_total(w);
+                                if (lane == 0) atomicAdd(&sh.hist[buffer][same], w);
+                            } else if (in) {
+                                atomicAdd(&sh.hist[buffer][digit], w);
+                            }
                         }
                     }
-                }
-                if (shift == 24) {
-                    // (the sum comes with the first digit, so that its search follows with the share known)
-                    const unsigned long long over = find_digit(sh, buffer, 1ull, blocks);
-                    const unsigned long long tie = cut_ties != 0ull ? r.weight_unfiltered(key_value(above)) : 0ull;
-                    most = max(share_of(over + cut_ties * tie, uint32_t(r.p24)), 1ull);
-                    if (most > over) {             // all above the cut, and some of the ties
-                        cut_ties = min(cut_ties, (most - over + tie - 1ull) / tie);
-                        inside = false;
-                    } else {
-                        find_digit(sh, buffer, most, blocks);
-                    }
-                } else {
-                    find_digit(sh, buffer, most - ahead, blocks);
-                }
-                if (inside) {
-                    found |= sh.digit << shift;
-                    ahead += sh.digit_above;
-                }
+                });
+                find_digit(sh, buffer, wanted, blocks);
+                found |= sh.digit << shift;
+                wanted -= sh.digit_above;
                 buffer ^= 1;
-                clear(buffer);
+                for (int i = tid; i < 256; i += kSampleThreads) sh.hist[buffer][i] = 0ull;      // (two uses ago: read by every block before the last barrier)
             }
-            if (inside) {
-                cut = found;
-                const unsigned long long tie = r.weight_unfiltered(key_value(cut));
-                cut_ties = (most - ahead + tie - 1ull) / tie;
-            }
+            cut = found;
+            const unsigned long long each = by_weight ? fixed(r.ratio(key_value(cut))) : 1ull;
+            cut_ties = (wanted + each - 1ull) / each;
+            return true;
+        };
+        unsigned long long beyond;
+        if (r.k > 0) find_cut(false, 0u, static_cast<unsigned long long>(r.k), 0ull, beyond);
+        if (r.p24 >= 0) {
+            // top-p looks at the tokens above top-k's cut, and at those of its ties that are kept
+            const unsigned long long tie = cut_ties != 0ull ? fixed(r.ratio(key_value(cut))) : 0ull;
+            if (!find_cut(true, cut, 0ull, cut_ties * tie, beyond)) cut_ties = min(cut_ties, (beyond + tie - 1ull) / tie);
         }
     }
 
     // ── sums of the kept weights, per warp ──
-    {
-        unsigned long long sum = 0;
-        uint32_t ties = 0;
-        for (int s = 0; s < steps; ++s) {
-            float v[8];
-            part.get(s, v);
+    const float cut_value = cut != 0u ? key_value(cut) : -CUDART_INF_F;
+    const unsigned long long tie_weight = cut_ties != 0ull ? r.weight(cut_value) : 0ull;
+    auto part_sums = [&](int from, int count, unsigned long long& sum, uint32_t& ties) {
+        FixedSum kept;
+        ties = 0;
+        row.each(from, count, [&](const float (&v)[8], int) {
+            if (cut_ties == 0ull) {
+                if (r.min_p > 0.f) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint32_t key = order_key(v[i]);
-                if (key > cut) sum += r.weight(v[i]);
-                ties += key == cut;
+                    for (int i = 0; i < 8; ++i) {
+                        const float e = r.ratio(v[i]);
+                        kept.add(e >= r.min_p ? e : 0.f);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) kept.add(r.ratio(v[i]));
+                }
+            } else if (__any_sync(0xFFFFFFFFu, max_of(v) >= cut_value)) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float e = r.ratio(v[i]);
+                    kept.add(v[i] > cut_value && e >= r.min_p ? e : 0.f);
+                    ties += v[i] == cut_value;
+                }
             }
-        }
-        sum = warp_total(sum);
+        });
+        sum = warp_total(kept.total());
         ties = __reduce_add_sync(0xFFFFFFFFu, ties);
+    };
+    // Of `parts` neighbouring parts of the row with these sums and ties: the one in which more than `target` is reached, if that is in them.  before and
+    // tie_before: what lies before the first, and afterwards before the part.
+    auto find_part = [&](const unsigned long long* sums, const uint32_t* ties, int parts, unsigned long long target, unsigned long long& before,
+                         unsigned long long& tie_before) -> int {
+        unsigned long long v[4], all = 0;
+        uint32_t c[4], all_ties = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            c[i] = lane * 4 + i < parts ? ties[lane * 4 + i] : 0u;
+            all_ties += c[i];
+        }
+        unsigned long long tie_at = tie_before + warp_upto(all_ties, lane) - all_ties;
+        const unsigned long long lane_ties = tie_at;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned long long left = cut_ties > tie_at ? cut_ties - tie_at : 0ull;
+            v[i] = lane * 4 + i < parts ? sums[lane * 4 + i] + min(left, static_cast<unsigned long long>(c[i])) * tie_weight : 0ull;
+            tie_at += c[i];
+            all += v[i];
+        }
+        unsigned long long at = before + warp_upto(all, lane) - all;
+        const uint32_t hit = __ballot_sync(0xFFFFFFFFu, target >= at && target < at + all);
+        int part = 0;
+        tie_at = lane_ties;
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+            if (part == i && target >= at + v[i]) { at += v[i];  tie_at += c[i];  part = i + 1; }
+        const int from = __ffs(hit) - 1;
+        before = __shfl_sync(0xFFFFFFFFu, at, from & 31);
+        tie_before = __shfl_sync(0xFFFFFFFFu, tie_at, from & 31);
+        return from * 4 + __shfl_sync(0xFFFFFFFFu, part, from & 31);
+    };
+    auto total_of = [&](const unsigned long long* sums, const uint32_t* ties, int parts) -> unsigned long long {
+        unsigned long long v = 0, c = 0;
+        for (int i = lane; i < parts; i += 32) { v += sums[i];  c += ties[i]; }
+        return warp_total(v) + min(cut_ties, warp_total(c)) * tie_weight;
+    };
+    {
+        unsigned long long sum;
+        uint32_t ties;
+        part_sums(first, steps, sum, ties);
         if (lane < int(blocks)) {
             sts_cluster_u64(ptx::mapa(ptx::smem_u32(&sh.sum[rank * kSampleWarps + warp]), lane), sum);
             ptx::sts_cluster_u32(ptx::mapa(ptx::smem_u32(&sh.ties[rank * kSampleWarps + warp]), lane), ties);
         }
-        ptx::cluster_sync();
+        sync_row(blocks);
     }
-
-    // ── the warp that has the token (every warp finds out for itself) ──
-    const unsigned long long tie_weight = cut_ties != 0ull ? r.weight(key_value(cut)) : 0ull;
-    const int parts = int(blocks) * kSampleWarps, me = int(rank) * kSampleWarps + warp;
-    unsigned long long sums[4], mine = 0, tie_before = 0;
-    uint32_t ties[4], my_ties = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        ties[i] = lane * 4 + i < parts ? sh.ties[lane * 4 + i] : 0u;
-        my_ties += ties[i];
+    // ── the warp's part that has the token, by all warps of its block in finer parts, and of those the one that has it ──
+    const unsigned long long total = total_of(sh.sum, sh.ties, parts), target = share_of(total, u24);
+    unsigned long long before = 0, tie_before = 0;
+    const int owner = find_part(sh.sum, sh.ties, parts, target, before, tie_before);
+    if (owner / kSampleWarps != int(rank)) return;
+    const int owner_first = first_step(owner), owner_steps = first_step(owner + 1) - owner_first;
+    const int fine_first = owner_steps * warp / kSampleWarps, mine_steps = owner_steps * (warp + 1) / kSampleWarps - fine_first;
+    const int mine_first = (owner_first + fine_first) * kSampleStep;
+    {
+        unsigned long long sum;
+        uint32_t ties;
+        part_sums(mine_first, mine_steps, sum, ties);
+        __syncthreads();
+        if (lane == 0) { sh.sum[warp] = sum;  sh.ties[warp] = ties; }
+        __syncthreads();
+        if (find_part(sh.sum, sh.ties, kSampleWarps, target, before, tie_before) != warp) return;
     }
-    tie_before = warp_upto(my_ties, lane) - my_ties;
-    unsigned long long my_tie_before = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const unsigned long long left = cut_ties > tie_before ? cut_ties - tie_before : 0ull;
-        if (lane * 4 + i == me) my_tie_before = tie_before;
-        tie_before += ties[i];
-        sums[i] = lane * 4 + i < parts ? sh.sum[lane * 4 + i] + min(left, (unsigned long long)(ties[i])) * tie_weight : 0ull;
-        mine += sums[i];
-    }
-    const unsigned long long upto = warp_upto(mine, lane), total = __shfl_sync(0xFFFFFFFFu, upto, 31);
-    const unsigned long long target = share_of(total, u24);
-    unsigned long long before = upto - mine, my_before = 0, my_sum = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (lane * 4 + i == me) { my_before = before;  my_sum = sums[i]; }
-        before += sums[i];
-    }
-    my_before = __shfl_sync(0xFFFFFFFFu, my_before, me >> 2);
-    my_sum = __shfl_sync(0xFFFFFFFFu, my_sum, me >> 2);
-    my_tie_before = __shfl_sync(0xFFFFFFFFu, my_tie_before, me >> 2);
-    if (target < my_before || target >= my_before + my_sum) return;
-
-    unsigned long long run = my_before, tie_run = my_tie_before;
-    for (int s = 0; s < steps; ++s) {
-        float v[8];
-        part.get(s, v);
+    bool searching = true;
+    row.each(mine_first, mine_steps, [&](const float (&v)[8], int e) {
+        if (!searching) return;
         uint32_t here = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) here += order_key(v[i]) == cut;
-        unsigned long long tie_at = tie_run + warp_upto(here, lane) - here, w[8], sum = 0;
+        for (int i = 0; i < 8; ++i) here += v[i] == cut_value;
+        unsigned long long tie_at = tie_before + warp_upto(here, lane) - here, w[8], sum = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const uint32_t key = order_key(v[i]);
-            w[i] = key > cut ? r.weight(v[i]) : 0ull;
-            if (key == cut && tie_at++ < cut_ties) w[i] = tie_weight;
+            w[i] = v[i] > cut_value ? r.weight(v[i]) : 0ull;
+            if (v[i] == cut_value && tie_at++ < cut_ties) w[i] = tie_weight;
             sum += w[i];
         }
-        const unsigned long long lane_upto = run + warp_upto(sum, lane);
+        const unsigned long long lane_upto = before + warp_upto(sum, lane);
         unsigned long long at = lane_upto - sum;
         if (target >= at && target < lane_upto) {
             int i = 0;
 #pragma unroll
             for (int j = 0; j < 7; ++j)
                 if (i == j && target >= at + w[j]) { at += w[j];  i = j + 1; }
-            float x = v[0];
+            float l = v[0];
 #pragma unroll
-            for (int j = 1; j < 8; ++j) x = i == j ? v[j] : x;
-            a.token[n] = part.at(s) + i - part.lead;
-            if (a.logprob != nullptr) a.logprob[n] = r.exponent(x) - logf(__ull2float_rn(total) * 9.094947017729282e-13f);
+            for (int j = 1; j < 8; ++j) l = i == j ? v[j] : l;
+            a.token[n] = e + i - row.lead;
+            if (a.logprob != nullptr) a.logprob[n] = r.exponent(l) - logf(__ull2float_rn(total) * 9.094947017729282e-13f);
         }
-        run = __shfl_sync(0xFFFFFFFFu, lane_upto, 31);
-        tie_run = tie_run + __reduce_add_sync(0xFFFFFFFFu, here);
-        if (target < run) return;
-    }
+        before = __shfl_sync(0xFFFFFFFFu, lane_upto, 31);
+        tie_before += __reduce_add_sync(0xFFFFFFFFu, here);
+        searching = target >= before;
+    });
 }
 
 }  // namespace dsv4
