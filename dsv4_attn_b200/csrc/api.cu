@@ -1031,8 +1031,10 @@ cudaError_t launch_sample(SampleArgs& a, cudaStream_t stream) {
 #ifdef PROBE
     if (getenv("PB")) blocks = atoi(getenv("PB"));
 #endif
-    for (a.hist_shift = 0; (span / blocks + kSampleStep) >> a.hist_shift > 0xFFFF;) ++a.hist_shift;     // times 2^16 and less
-    return launch(sample_kernel<T>, dim3(unsigned(int64_t(a.N) * blocks)), kSampleThreads, 0, stream, a, blocks > 1 ? blocks : 0);
+    static std::atomic<bool> done[kMaxDevices];
+    const cudaError_t e = ensure_smem(sample_kernel<T>, int(sizeof(SampleShared)), done);
+    if (e != cudaSuccess) return e;
+    return launch(sample_kernel<T>, dim3(unsigned(int64_t(a.N) * blocks)), kSampleThreads, sizeof(SampleShared), stream, a, blocks > 1 ? blocks : 0);
 }
 }  // namespace
 

@@ -14,9 +14,9 @@
 // Top-k of up to 512 a block is sought among candidates: every thread has the largest of its logits at hand, and where ceil(k / blocks) threads of each
 // block have one of at least x, at least k logits are, so that all logits from x on (some 2 k of them) hold the cut.  Only the threads that have one look
 // again.  With up to 128 tokens left, the token itself is found in the list.
-// Any other cut: a histogram over (l_max - l) / t in steps of 1/32, one 32-bit atomic per logit, says in which step the cut lies (the weights in it are
-// rounded to 16 bits of the step's largest); what lies above it is then summed exactly and the logits inside are the candidates, the neighbouring
-// step's if the exact sums say so.  Candidates too many for the lists (thousands of equal logits) are gone through by digits of their ordered bits.
+// Any other cut: a histogram over (l_max - l) / t in bins of 1/128, a count per bin, says where it should be; what lies above is then summed
+// exactly and the logits of two and a half bins there are the candidates, those of the bins next to them if the exact sums say so.  Candidates
+// too many for the lists (thousands of equal logits) are gone through by digits of their ordered bits.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -35,17 +35,18 @@ constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleMaxCluster = 8;
 constexpr int kSampleStep = 256;                 // logits a warp looks at at a time, eight neighbouring ones a lane
 constexpr int kSampleOneBits = 40;               // weights are multiples of 2^-40
-constexpr int kSampleBlockList = 1024;           // candidates of a block,
-constexpr int kSampleList = 2048;                // and of the cluster
+constexpr int kSampleList = 2048;                // candidates
 constexpr int kSampleWalk = 128;                 // kept candidates among which the token is looked for directly
-constexpr int kSampleSteps = 1024;               // steps of 1/32 in (l_max - l) / t
+constexpr int kSampleBins = 4096;                // of the histogram over (l_max - l) / t,
+constexpr float kSampleBin = 128.f;              // 1/128 each
+constexpr uint32_t kSampleSpare = 200;           // candidates next to the bin of a cut
+constexpr int kSampleQuarters = 4;               // a thread knows the largest logit of each quarter of its own
 constexpr int kSampleMostTerms = 4095;           // of a FixedSum
 
 struct SampleArgs {
     const void* logits;
     int64_t stride;
     int N, V;
-    int hist_shift;          // bits left out of the histograms' weights, so that a block's sums fit 32 bits
     const float* u;
     const float* temperature;
     const int32_t* top_k;
@@ -66,8 +67,8 @@ struct SampleShared {
     uint32_t ties[kSampleMaxCluster * kSampleWarps];             // and tokens at the cut
     // read by the other blocks
     unsigned long long hist[2][256];                             // one digit
-    uint32_t step_hist[kSampleSteps];                            // the distance from the maximum
-    unsigned long long list[kSampleBlockList];                   // candidates: key << 32 | ~index
+    uint32_t bins[kSampleBins];
+    unsigned long long list[kSampleList];                        // candidates: key << 32 | ~index
     // the block's own
     unsigned long long sorted[kSampleList];
     unsigned long long all[256];
@@ -75,9 +76,9 @@ struct SampleShared {
     unsigned long long warp_x[kSampleWarps], warp_y[kSampleWarps];
     float warp_max[kSampleWarps];
     uint32_t digit, count;
-    int step;
+    int bin;
     // the cut, from the first block to all
-    uint32_t cut, kept;
+    uint32_t cut, kept, reached;                                 // reached: all of what was wanted lies up to it
     unsigned long long cut_ties;
 };
 
@@ -153,16 +154,6 @@ struct SampleRow {
     // only the largest logits can come to, into 0.
     __device__ __forceinline__ float exponent(float l) const { return fminf(__fmul_rn(__fsub_rn(l, top), per), 0.f); }
     __device__ __forceinline__ float ratio(float l) const { return expf(exponent(l)); }
-    // the step of a finite logit in (l_max - l) / t
-    __device__ __forceinline__ int step(float x) const { return min(int(x * -32.f), kSampleSteps - 1); }
-    // Biased exponent above that of the step's largest weight, exp(-step / 32).
-    static __device__ __forceinline__ int step_exponent(int step) { return 128 - ((step * 1477) >> 15); }
-    // exp(x) in 16 bits below it
-    static __device__ __forceinline__ uint32_t step_weight(float e, int step, int drop) {
-        const uint32_t b = __float_as_uint(e);
-        const int shift = 8 + drop + step_exponent(step) - int(b >> 23);
-        return ((b & 0x7FFFFFu) | 0x800000u) >> min(max(shift, 0), 31);
-    }
     __device__ __forceinline__ unsigned long long weight(float l) const {
         const float e = ratio(l);
         return e >= min_p ? fixed(e) : 0ull;
@@ -386,18 +377,14 @@ __device__ __forceinline__ void sort_list(SampleShared& sh, int n) {
 // A logit goes to the block's list.  (+ 0: -0 is 0)
 __device__ __forceinline__ void list_logit(SampleShared& sh, float l, int index) {
     const uint32_t at = atomicAdd(&sh.count, 1u);
-    if (at < uint32_t(kSampleBlockList)) sh.list[at] = (static_cast<unsigned long long>(order_key(l + 0.f)) << 32) | uint32_t(~index);
+    if (at < uint32_t(kSampleList)) sh.list[at] = (static_cast<unsigned long long>(order_key(l + 0.f)) << 32) | uint32_t(~index);
 }
 
 // How many candidates the lists have (-1: too many), after row_totals.
 __device__ __forceinline__ int listed(const SampleShared& sh, uint32_t blocks, int turn) {
     int n = 0;
-    bool fits = true;
-    for (uint32_t b = 0; b < blocks; ++b) {
-        fits = fits && sh.found[turn][b] <= uint32_t(kSampleBlockList);
-        n += int(min(sh.found[turn][b], uint32_t(kSampleList)));
-    }
-    return fits && n <= kSampleList ? n : -1;
+    for (uint32_t b = 0; b < blocks; ++b) n += int(min(sh.found[turn][b], uint32_t(kSampleList) + 1u));
+    return n <= kSampleList ? n : -1;
 }
 
 // The cut among the candidates of all blocks (n of them, in sh.sorted afterwards, in descending order): the first k, and of those the ones before which less
@@ -405,6 +392,7 @@ __device__ __forceinline__ int listed(const SampleShared& sh, uint32_t blocks, i
 __device__ __forceinline__ void cut_of_list(SampleShared& sh, const SampleRow& r, uint32_t blocks, int turn, int n, int k, unsigned long long most) {
     constexpr int kPer = kSampleList / kSampleThreads;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) sh.reached = 0u;
     for (int i = tid; i < n; i += kSampleThreads) {
         uint32_t b = 0, at = uint32_t(i);
         while (at >= sh.found[turn][b]) at -= sh.found[turn][b++];
@@ -440,12 +428,14 @@ __device__ __forceinline__ void cut_of_list(SampleShared& sh, const SampleRow& r
             sh.cut = key;
             sh.cut_ties = static_cast<unsigned long long>(at - lo + 1);
             sh.kept = uint32_t(at + 1);
+            sh.reached = most == ~0ull || ahead >= most;
         }
     }
     __syncthreads();
     if (tid > 0 && tid < int(blocks)) {
         ptx::sts_cluster_u32(ptx::mapa(ptx::smem_u32(&sh.cut), tid), sh.cut);
         ptx::sts_cluster_u32(ptx::mapa(ptx::smem_u32(&sh.kept), tid), sh.kept);
+        ptx::sts_cluster_u32(ptx::mapa(ptx::smem_u32(&sh.reached), tid), sh.reached);
         sts_cluster_u64(ptx::mapa(ptx::smem_u32(&sh.cut_ties), tid), sh.cut_ties);
     }
 }
@@ -482,7 +472,8 @@ __device__ __forceinline__ void token_of_list(SampleShared& sh, const SampleRow&
 
 template <typename T>
 __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a) {
-    __shared__ SampleShared sh;
+    extern __shared__ __align__(16) uint8_t s_sample[];
+    SampleShared& sh = *reinterpret_cast<SampleShared*>(s_sample);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = cluster_rank(), blocks = cluster_blocks();
     const int n = int(blockIdx.x / blocks);
@@ -503,7 +494,13 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     const int first = first_step(me) * kSampleStep, steps = first_step(me + 1) - first_step(me);
 
     // ── maximum ──
-    const float mine = row.largest(first, steps);
+    float quarter[kSampleQuarters], mine = -CUDART_INF_F;
+    auto quarter_step = [&](int q) { return steps * q / kSampleQuarters; };
+#pragma unroll
+    for (int q = 0; q < kSampleQuarters; ++q) {
+        quarter[q] = row.largest(first + quarter_step(q) * kSampleStep, quarter_step(q + 1) - quarter_step(q));
+        mine = fmaxf(mine, quarter[q]);
+    }
     SampleRow r;
     const float t = a.temperature != nullptr ? ptx::ld(a.temperature + n) : 1.f;
     r.greedy = !(t > 0.f);
@@ -523,13 +520,20 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     __syncthreads();
     // a key that enough threads' largest logits reach: from the top, a bit at a time
     const int groups = (r.k + int(blocks) - 1) / int(blocks);
-    const bool by_list = !r.greedy && r.k > 0 && groups <= kSampleThreads;
+    // (half of the threads, or of their quarters: more would bring the bound down to logits that most of them exceed several times)
+    const bool by_list = !r.greedy && r.k > 0 && groups <= kSampleThreads * kSampleQuarters / 2;
     uint32_t bound = 0u;
     if (by_list) {
+        const bool few = groups <= kSampleThreads / 2;
         const uint32_t key = order_key(mine);
 #pragma unroll 1
-        for (uint32_t bit = 0x80000000u; bit >= 0x8000u; bit >>= 1)
-            if (__syncthreads_count(key >= (bound | bit)) >= groups) bound |= bit;
+        for (uint32_t bit = 0x80000000u; bit >= 0x8000u; bit >>= 1) {
+            int reach = __syncthreads_count((few ? key : order_key(quarter[0])) >= (bound | bit));
+            if (!few)
+#pragma unroll
+                for (int q = 1; q < kSampleQuarters; ++q) reach += __syncthreads_count(order_key(quarter[q]) >= (bound | bit));
+            if (reach >= groups) bound |= bit;
+        }
     }
     r.top = sh.warp_max[lane & (kSampleWarps - 1)];
 #pragma unroll
@@ -579,16 +583,22 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     uint32_t cut = 0;                              // a key; every key is above 0
     unsigned long long cut_ties = 0;
     int turn = 0;
+    bool sums_known = false;                       // of the kept weights, per warp
+    auto part_of = [&](int index) { return int((int64_t((index + row.lead) / kSampleStep + 1) * parts - 1) / row_steps); };
     bool have_cut = r.k == 0 && r.p24 < 0;
     if (by_list) {
         const float from = fmaxf(key_value(bound), -3.402823466e38f);       // (-inf is no candidate)
-        if (mine >= from)
-            row.each(first, steps, [&](const float (&v)[8], int e) {
+#pragma unroll 1
+        for (int q = 0; q < kSampleQuarters; ++q) {
+            const float largest = q < 2 ? (q == 0 ? quarter[0] : quarter[1]) : (q == 2 ? quarter[2] : quarter[3]);
+            if (largest < from) continue;
+            row.each(first + quarter_step(q) * kSampleStep, quarter_step(q + 1) - quarter_step(q), [&](const float (&v)[8], int e) {
                 if (max_of(v) < from) return;
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     if (v[i] >= from) list_logit(sh, v[i], e + i - row.lead);
             });
+        }
         unsigned long long x = 0, y = 0;
         row_totals(sh, blocks, rank, turn, x, y);
         const int m = listed(sh, blocks, turn);
@@ -609,99 +619,176 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         // top-p says of all of it and of `ties`, the weight of the tokens kept at `above`.  False: it lies beyond (in the ties; no cut at all).
         auto find_cut = [&](bool by_weight, uint32_t above, unsigned long long wanted, unsigned long long ties, unsigned long long& over) -> bool {
             const float above_value = above != 0u ? key_value(above) : -CUDART_INF_F;
-            for (int i = tid; i < kSampleSteps; i += kSampleThreads) sh.step_hist[i] = 0u;
-            if (tid == 0) sh.step = 0;
+            for (int i = tid; i < kSampleBins; i += kSampleThreads) sh.bins[i] = 0u;
             __syncthreads();
-            FixedSum sum;
-            uint32_t count = 0;
+            // Bin of a logit: 1, its distance in bins and `off`, rounded to a whole number by the addition of 2^23.  (Near enough: what is decided
+            // by it is checked with the exact sums.)  The last bin is for what is further away, and not counted.
+            const float slope = -kSampleBin * r.per, offset = fmaf(-slope, r.top, 8388609.f), off = fmaf(slope, r.top, offset - 8388609.f);
             row.each(first, steps, [&](const float (&v)[8], int) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const bool in = v[i] > above_value;
-                    const float x = r.exponent(v[i]), e = in ? expf(x) : 0.f;
-                    const int step = r.step(x);
-                    if (by_weight) {
-                        sum.add(e);
-                        if (in && x > -28.f) atomicAdd(&sh.step_hist[step], SampleRow::step_weight(e, step, a.hist_shift));       // (a weight below 2^-40 is 0)
-                    } else if (in) {
-                        ++count;
-                        atomicAdd(&sh.step_hist[step], 1u);
-                    }
+                    const uint32_t bin = __float_as_uint(fminf(fmaf(v[i], slope, offset), 8388608.f + kSampleBins - 1)) & (kSampleBins - 1);
+                    if (v[i] > above_value && bin < kSampleBins - 1) atomicAdd(&sh.bins[bin], 1u);
                 }
             });
-            unsigned long long unused = 0;
-            over = by_weight ? sum.total() : count;
-            row_totals(sh, blocks, rank, turn, over, unused);
-            if (by_weight) wanted = max(share_of(over + ties, uint32_t(r.p24)), 1ull);
-            if (wanted > over) { over = wanted - over;  return false; }
-            // two neighbouring steps a thread
-            unsigned long long v[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int step = 2 * tid + i;
-                const uint32_t at = ptx::smem_u32(&sh.step_hist[step]);
-                unsigned long long steps_sum = 0;
-                if (blocks > 1u)
-                    for (uint32_t b = 0; b < blocks; ++b) steps_sum += ptx::lds_cluster_u32(ptx::mapa(at, b));
-                else
-                    steps_sum = sh.step_hist[step];
-                if (steps_sum != 0ull) atomicMax(&sh.step, step);      // (the last one, where rounding leaves the sum short of `wanted`)
-                const int up = SampleRow::step_exponent(step) - 102 + a.hist_shift;
-                v[i] = !by_weight ? steps_sum : (up >= 0 ? steps_sum << up : steps_sum >> -up);
+            sync_row(blocks);
+            uint32_t* const counts = reinterpret_cast<uint32_t*>(sh.sorted);       // of the row
+            if (blocks > 1u) {
+                // every block adds up a part of the bins, and tells the others
+                const int share = kSampleBins / int(blocks);
+                for (int i = tid; i < share; i += kSampleThreads) {
+                    const int bin = int(rank) * share + i;
+                    uint32_t c = 0;
+                    for (uint32_t b = 0; b < blocks; ++b) c += ptx::lds_cluster_u32(ptx::mapa(ptx::smem_u32(&sh.bins[bin]), b));
+                    for (uint32_t b = 0; b < blocks; ++b) ptx::sts_cluster_u32(ptx::mapa(ptx::smem_u32(&counts[bin]), b), c);
+                }
+                ptx::cluster_sync();
             }
-            unsigned long long before = warp_upto(v[0] + v[1], lane) - v[0] - v[1];
-            if (lane == 31) sh.warp_x[warp] = before + v[0] + v[1];
-            __syncthreads();
-            const unsigned long long of_warp = lane < kSampleWarps ? sh.warp_x[lane] : 0ull, upto_warp = warp_upto(of_warp, lane);
-            before += __shfl_sync(0xFFFFFFFFu, upto_warp - of_warp, warp);
-            if (before < wanted && before + v[0] + v[1] >= wanted) sh.step = 2 * tid + (before + v[0] < wanted ? 1 : 0);
-            __syncthreads();
-            int step = sh.step;
-            unsigned long long ahead, inside;
-            for (int moved = 0;;) {
+            // The first bin up to which the tokens, or the share of the weight, lie; and the counts up to every bin.  Eight neighbouring bins a thread.
+            {
+                constexpr int kPer = kSampleBins / kSampleThreads;
+                const uint32_t* const from = blocks > 1u ? counts : sh.bins;
+                uint32_t c[kPer], n_mine = 0;
+                float mine_sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    const int bin = kPer * tid + i;
+                    c[i] = from[bin];
+                    n_mine += c[i];
+                    mine_sum += by_weight ? float(c[i]) * __expf(float(1 - bin) / kSampleBin) : float(c[i]);
+                }
+                float upto = mine_sum;
+                uint32_t n_upto = n_mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const float y = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+                    const uint32_t z = __shfl_up_sync(0xFFFFFFFFu, n_upto, o);
+                    if (lane >= o) { upto += y;  n_upto += z; }
+                }
+                if (tid == 0) sh.bin = kSampleBins - 1;
+                if (lane == 31) { sh.warp_max[warp] = upto;  sh.warp_x[warp] = n_upto; }
+                __syncthreads();
+                float before = upto - mine_sum, total = 0.f;
+                uint32_t n_before = n_upto - n_mine;
+                for (int w = 0; w < kSampleWarps; ++w) {
+                    if (w < warp) { before += sh.warp_max[w];  n_before += uint32_t(sh.warp_x[w]); }
+                    total += sh.warp_max[w];
+                }
+                // (ties: in units of the largest weight)
+                const float goal = by_weight ? float(r.p24) * 5.9604645e-8f * (total + __ull2float_rn(ties) * 9.094947e-13f) : float(wanted);
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    const int bin = kPer * tid + i;
+                    const float v = by_weight ? float(c[i]) * __expf(float(1 - bin) / kSampleBin) : float(c[i]);
+                    if (before < goal && before + v >= goal) atomicMin(&sh.bin, bin);
+                    before += v;
+                    counts[bin] = n_before += c[i];
+                }
+                __syncthreads();
+            }
+            // That bin, one and a quarter each way, and as far each way as there are not more than kSampleSpare tokens: where they are few, rounding
+            // moves the cut from one to the next, bins away.
+            int low = 0, high = kSampleBins - 1;
+            {
+                const int bin = sh.bin;
+                const uint32_t left = bin > 0 ? counts[bin - 1] : 0u, right = counts[bin];
+                for (int hi = bin; low < hi;) {                        // the first bin from which at most so many lie before `bin`
+                    const int mid = (low + hi) / 2;
+                    if (left - (mid > 0 ? counts[mid - 1] : 0u) <= kSampleSpare) hi = mid;
+                    else low = mid + 1;
+                }
+                for (int lo = bin; lo < high;) {
+                    const int mid = (lo + high + 1) / 2;
+                    if (counts[mid] - right <= kSampleSpare) lo = mid;
+                    else high = mid - 1;
+                }
+                low = min(low, bin);
+                high = max(high, bin);
+            }
+            __syncthreads();                       // (the counts lie where the candidates will be sorted)
+            // Exactly: what all weigh, what lies nearer than `from`, and the candidates from there to `to`.
+            float from = fminf(float(low - 1) - off - 0.5f, float(sh.bin - 1) - off - 1.25f), to = fmaxf(float(high - 1) - off + 0.5f, float(sh.bin - 1) - off + 1.25f);
+            unsigned long long ahead;
+            for (int moved = 0, tries = 0;; ++tries) {
+                // (a few steps the same way: all the way; and what is not a number, with infinite logits, is everything)
+                if (!(from >= 1.f) || (tries > 2 && moved < 0)) from = -1.f;
+                if (!(to <= kSampleBins - 8) || (tries > 2 && moved > 0)) to = CUDART_INF_F;
+                const bool open = to == CUDART_INF_F;
                 __syncthreads();
                 if (tid == 0) sh.count = 0u;
                 __syncthreads();
-                FixedSum sum_ahead, sum_inside;
-                uint32_t n_ahead = 0, n_inside = 0;
-                // (a logit below `reach` is beyond the step for certain: a little further than the step's end)
-                const float from = float(step), to = step == kSampleSteps - 1 ? CUDART_INF_F : from + 1.f;
-                float reach = r.top - to * 0.03126f / r.per - 1e-5f * fabsf(r.top);
-                if (!(reach < r.top)) reach = -CUDART_INF_F;
+                FixedSum sum_all, sum_ahead;
+                uint32_t n_all = 0, n_ahead = 0;
                 row.each(first, steps, [&](const float (&v)[8], int e) {
-                    if (!__any_sync(0xFFFFFFFFu, max_of(v) >= reach)) return;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const float x = r.exponent(v[i]), at = x * -32.f;
-                        const bool in = v[i] > above_value && at < to, is_inside = in && at >= from;
+                        const float x = r.exponent(v[i]), at = x * -kSampleBin;
+                        const bool in = v[i] > above_value, is_ahead = in && at < from;
                         if (by_weight) {
                             const float w = in ? expf(x) : 0.f;
-                            sum_ahead.add(is_inside ? 0.f : w);
-                            if (is_inside) sum_inside.add(w);
+                            sum_all.add(w);
+                            sum_ahead.add(is_ahead ? w : 0.f);
                         } else {
-                            n_ahead += in && !is_inside;
-                            n_inside += is_inside;
+                            n_all += in;
+                            n_ahead += is_ahead;
                         }
-                        if (is_inside) list_logit(sh, v[i], e + i - row.lead);
+                        if (in && !is_ahead && (open || at < to)) list_logit(sh, v[i], e + i - row.lead);
                     }
                 });
+                over = by_weight ? sum_all.total() : n_all;
                 ahead = by_weight ? sum_ahead.total() : n_ahead;
-                inside = by_weight ? sum_inside.total() : n_inside;
-                row_totals(sh, blocks, rank, turn, ahead, inside);
-                // (the rounded sums can be off by a step: towards the top and then back again cannot be)
-                if (wanted <= ahead && step > 0 && moved <= 0) { --step;  moved = -1;  continue; }
-                if (wanted > ahead + inside && step + 1 < kSampleSteps && moved >= 0) { ++step;  moved = 1;  continue; }
-                break;
+                if (blocks == 1u) {                // (kept for the token, where this turns out to be the cut)
+                    const unsigned long long of_warp = warp_total(ahead);
+                    if (lane == 0) { sh.sum[warp] = of_warp;  sh.ties[warp] = 0u; }
+                }
+                row_totals(sh, blocks, rank, turn, over, ahead);
+                if (by_weight) wanted = max(share_of(over + ties, uint32_t(r.p24)), 1ull);
+                if (wanted > over) { over = wanted - over;  return false; }
+                if (wanted <= ahead) { to = from;  from -= 2.5f;  moved = -1;  continue; }
+                const int m = listed(sh, blocks, turn);
+                if (m >= 0 && (by_weight || wanted - ahead <= static_cast<unsigned long long>(m))) {
+                    if (rank == 0) cut_of_list(sh, r, blocks, turn, m, by_weight ? m : int(wanted - ahead), by_weight ? wanted - ahead : ~0ull);
+                    sync_row(blocks);
+                    if (sh.reached) {
+                        cut = sh.cut;
+                        cut_ties = sh.cut_ties;
+                        if (by_weight && blocks == 1u && r.min_p == 0.f) {
+                            for (int i = tid; i < m; i += kSampleThreads) {
+                                const unsigned long long c = sh.sorted[i];
+                                const uint32_t key = uint32_t(c >> 32);
+                                const int of = part_of(int(~uint32_t(c)));
+                                if (key > cut) atomicAdd(&sh.sum[of], fixed(r.ratio(key_value(key))));
+                                else if (key == cut) atomicAdd(&sh.ties[of], 1u);
+                            }
+                            sums_known = true;
+                        }
+                        return true;
+                    }
+                }
+                if (m < 0) {
+                    // more candidates than the lists hold: do they reach the cut?
+                    FixedSum sum_upto;
+                    uint32_t n_upto = 0;
+                    row.each(first, steps, [&](const float (&v)[8], int) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float x = r.exponent(v[i]);
+                            const bool in = v[i] > above_value && (open || x * -kSampleBin < to);
+                            if (by_weight) sum_upto.add(in ? expf(x) : 0.f);
+                            n_upto += in;
+                        }
+                    });
+                    unsigned long long upto = by_weight ? sum_upto.total() : n_upto, unused = 0;
+                    row_totals(sh, blocks, rank, turn, upto, unused);
+                    if (wanted <= upto) break;
+                }
+                from = to;
+                to += 2.5f;
+                moved = 1;
             }
             wanted -= ahead;
-            const int m = listed(sh, blocks, turn);
-            if (m >= 0) {
-                if (rank == 0) cut_of_list(sh, r, blocks, turn, m, by_weight ? m : int(wanted), by_weight ? wanted : ~0ull);
-                sync_row(blocks);
-                cut = sh.cut;
-                cut_ties = sh.cut_ties;
-                return true;
-            }
+            // Digit by digit, then.
+            const bool open = to == CUDART_INF_F;
             uint32_t found = 0;
             int buffer = 0;
             for (int i = tid; i < 256; i += kSampleThreads) sh.hist[0][i] = 0ull;
@@ -713,7 +800,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                     for (int i = 0; i < 8; ++i) {
                         const uint32_t key = order_key(v[i] + 0.f);
                         const float x = r.exponent(v[i]);
-                        const bool in = v[i] > above_value && r.step(x) == step && (shift == 24 || (key >> (shift + 8)) == (found >> (shift + 8)));
+                        const float at = x * -kSampleBin;
+                        const bool in = v[i] > above_value && at >= from && (open || at < to) && (shift == 24 || (key >> (shift + 8)) == (found >> (shift + 8)));
                         const uint32_t digit = (key >> shift) & 255u, who = __ballot_sync(0xFFFFFFFFu, in);
                         if (who != 0u) {
                             unsigned long long w = in ? (by_weight ? fixed(expf(x)) : 1ull) : 0ull;
@@ -815,7 +903,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         for (int i = lane; i < parts; i += 32) { v += sums[i];  c += ties[i]; }
         return warp_total(v) + min(cut_ties, warp_total(c)) * tie_weight;
     };
-    {
+    if (!sums_known) {
         unsigned long long sum;
         uint32_t ties;
         part_sums(first, steps, sum, ties);
@@ -823,8 +911,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
             sts_cluster_u64(ptx::mapa(ptx::smem_u32(&sh.sum[rank * kSampleWarps + warp]), lane), sum);
             ptx::sts_cluster_u32(ptx::mapa(ptx::smem_u32(&sh.ties[rank * kSampleWarps + warp]), lane), ties);
         }
-        sync_row(blocks);
     }
+    sync_row(blocks);
     // ── the warp's part that has the token, by all warps of its block in finer parts, and of those the one that has it ──
     const unsigned long long total = total_of(sh.sum, sh.ties, parts), target = share_of(total, u24);
     unsigned long long before = 0, tie_before = 0;
