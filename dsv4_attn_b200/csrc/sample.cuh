@@ -13,7 +13,7 @@
 //
 // Top-k of up to 512 a block is sought among candidates: every thread has the largest of its logits at hand, and where ceil(k / blocks) threads of each
 // block have one of at least x, at least k logits are, so that all logits from x on (some 2 k of them) hold the cut.  Only the threads that have one look
-// again.  With up to 128 tokens left, the token itself is found in the list.
+// again, and the token is found among them.
 // Any other cut: a histogram over (l_max - l) / t in bins of 1/128, a count per bin, says where it should be; what lies above is then summed
 // exactly and the logits of two and a half bins there are the candidates, those of the bins next to them if the exact sums say so.  Candidates
 // too many for the lists (thousands of equal logits) are gone through by digits of their ordered bits.
@@ -36,7 +36,6 @@ constexpr int kSampleMaxCluster = 8;
 constexpr int kSampleStep = 256;                 // logits a warp looks at at a time, eight neighbouring ones a lane
 constexpr int kSampleOneBits = 40;               // weights are multiples of 2^-40
 constexpr int kSampleList = 2048;                // candidates
-constexpr int kSampleWalk = 128;                 // kept candidates among which the token is looked for directly
 constexpr int kSampleBins = 4096;                // of the histogram over (l_max - l) / t,
 constexpr float kSampleBin = 128.f;              // 1/128 each
 constexpr uint32_t kSampleSpare = 200;           // candidates next to the bin of a cut
@@ -121,11 +120,19 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 struct FixedSum {
     uint32_t hi = 0, lo = 0;     // less 0x4B000000, the bits of 2^23, per term
     int terms = 0;
-    __device__ __forceinline__ void add(float e) {
+    __device__ __forceinline__ void add(float e) { add_if(e, *this, false); }
+    // and, where `too`, to another sum as well
+    __device__ __forceinline__ void add_if(float e, FixedSum& other, bool too) {
         const float h = __fmaf_rz(e, 1048576.f, 8388608.f), rest = __fmaf_rn(e, 1048576.f, 8388608.f - h);
-        hi += __float_as_uint(h);
-        lo += __float_as_uint(__fmaf_rz(rest, 1048576.f, 8388608.f));
+        const uint32_t x = __float_as_uint(h), y = __float_as_uint(__fmaf_rz(rest, 1048576.f, 8388608.f));
+        hi += x;
+        lo += y;
         ++terms;
+        if (too) {
+            other.hi += x;
+            other.lo += y;
+            ++other.terms;
+        }
     }
     __device__ __forceinline__ unsigned long long total() const {
         const uint32_t off = uint32_t(terms) * 0x4B000000u;
@@ -150,9 +157,12 @@ struct SampleRow {
     int p24;                 // top-p in multiples of 2^-24, -1: off
     bool greedy;
 
-    // The exponent (l - top) / t of a logit: the operations of the definition, in its order.  The minimum turns the NaN of inf - inf and 0 * inf, which
-    // only the largest logits can come to, into 0.
-    __device__ __forceinline__ float exponent(float l) const { return fminf(__fmul_rn(__fsub_rn(l, top), per), 0.f); }
+    // Infinite logits, or a temperature whose reciprocal is infinite: all tokens with the largest logit weigh 1, the others nothing.
+    bool odd;
+
+    // The exponent (l - top) / t of a logit, in the operations and the order of the definition; from -200 down, where NaN ends up as well, it makes no
+    // difference any more.  Not for odd rows.
+    __device__ __forceinline__ float exponent(float l) const { return fmaxf(__fmul_rn(__fsub_rn(l, top), per), -200.f); }
     __device__ __forceinline__ float ratio(float l) const { return expf(exponent(l)); }
     __device__ __forceinline__ unsigned long long weight(float l) const {
         const float e = ratio(l);
@@ -179,7 +189,6 @@ template <> __device__ __forceinline__ __half no_logit<__half>() { return __usho
 // A row, whose elements are counted from the 16-byte boundary at or before its start: it is [lead, end).
 template <typename T>
 struct LogitRow {
-    static constexpr int kBatch = 4;             // steps whose loads are in flight at once
     static constexpr int kVecs = int(sizeof(T)) / 2;
     const T* base;
     int lead, end, lane;
@@ -245,40 +254,32 @@ struct LogitRow {
         else { const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p.bits));  return fmaxf(f.x, f.y); }
     }
 
-    // visit(v, e): the eight logits from e on, for the warp's `steps` steps from element `first` on.  NaN, and what is not of the row, is -inf.
+    // Eight logits from e on, -inf where that is not of the row.
+    __device__ __forceinline__ void load(int e, T (&x)[8]) const {
+        if (e >= lead && e + 8 <= end) {
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) reinterpret_cast<uint4*>(x)[i] = ptx::ld(reinterpret_cast<const uint4*>(base + e) + i);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = e + i >= lead && e + i < end ? ptx::ld(base + e + i) : no_logit<T>();
+        }
+    }
+    // visit(v, e): the eight logits from e on, for the warp's `steps` steps from element `first` on; -inf where that is not of the row.  A step at a time,
+    // with the next one on its way: what is done with a step takes longer than a load from L2, and with four steps in a loop body the instructions did not
+    // come fast enough.
     template <typename Visit>
     __device__ __forceinline__ void each(int first, int steps, Visit visit) const {
+        if (steps <= 0) return;
+        int e = first + lane * 8;
+        alignas(16) T next[8];
+        load(e, next);
 #pragma unroll 1
-        for (int s = 0; s < steps; s += kBatch) {
-            const int e0 = first + s * kSampleStep;
-            alignas(16) T x[kBatch][8];
-            if (e0 >= lead && e0 + kBatch * kSampleStep <= end) {
-                const uint4* p = reinterpret_cast<const uint4*>(base + e0 + lane * 8);
+        for (int s = 0; s < steps; ++s, e += kSampleStep) {
+            float v[8];
 #pragma unroll
-                for (int j = 0; j < kBatch; ++j)
-#pragma unroll
-                    for (int i = 0; i < kVecs; ++i) reinterpret_cast<uint4*>(x[j])[i] = ptx::ld(p + j * 32 * kVecs + i);
-            } else {
-#pragma unroll
-                for (int j = 0; j < kBatch; ++j) {
-                    const int e = e0 + j * kSampleStep + lane * 8;
-                    if (e >= lead && e + 8 <= end) {
-#pragma unroll
-                        for (int i = 0; i < kVecs; ++i) reinterpret_cast<uint4*>(x[j])[i] = ptx::ld(reinterpret_cast<const uint4*>(base + e) + i);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) x[j][i] = e + i >= lead && e + i < end ? ptx::ld(base + e + i) : no_logit<T>();
-                    }
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < kBatch; ++j)
-                if (s + j < steps) {
-                    float v[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = fmaxf(logit_value(x[j][i]), -CUDART_INF_F);
-                    visit(v, e0 + j * kSampleStep + lane * 8);
-                }
+            for (int i = 0; i < 8; ++i) v[i] = logit_value(next[i]);
+            if (s + 1 < steps) load(e + kSampleStep, next);
+            visit(v, e);
         }
     }
 };
@@ -286,6 +287,14 @@ struct LogitRow {
 __device__ __forceinline__ unsigned long long warp_total(unsigned long long v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+__device__ __forceinline__ uint32_t warp_upto32(uint32_t v, int lane) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, v, o);
+        if (lane >= o) v += y;
+    }
     return v;
 }
 __device__ __forceinline__ unsigned long long warp_upto(unsigned long long v, int lane) {
@@ -350,26 +359,63 @@ __device__ __forceinline__ void find_digit(SampleShared& sh, int buffer, unsigne
     __syncthreads();
 }
 
-// sh.sorted[0, n) into descending order; filled up with zeros to a power of two.  Every thread of the block calls.
+// sh.sorted[0, n) into descending order, by way of sh.list: 2,048 buckets over the range of the keys, and within a bucket by comparing all with all
+// (there are two or three in one, unless many logits are equal).  A bitonic network took 4 us for 200 candidates and 26 for 1,400, this 2 to 3.
+// Every thread of the block calls.
 __device__ __forceinline__ void sort_list(SampleShared& sh, int n) {
-    const int tid = threadIdx.x;
-    int size = 64;
-    while (size < n) size *= 2;
-    for (int i = n + tid; i < size; i += kSampleThreads) sh.sorted[i] = 0ull;
+    constexpr int kBuckets = 2048, kPer = kBuckets / kSampleThreads, kMine = kSampleList / kSampleThreads;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint32_t* const count = sh.bins;
+    uint32_t* const start = sh.bins + kBuckets;
+    for (int i = tid; i < kBuckets; i += kSampleThreads) count[i] = 0u;
+    uint32_t top = 0u, bottom = 0xFFFFFFFFu;
+    unsigned long long mine[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+        if (tid + i * kSampleThreads < n) {
+            mine[i] = sh.sorted[tid + i * kSampleThreads];
+            top = max(top, uint32_t(mine[i] >> 32));
+            bottom = min(bottom, uint32_t(mine[i] >> 32));
+        }
+    top = __reduce_max_sync(0xFFFFFFFFu, top);
+    bottom = __reduce_min_sync(0xFFFFFFFFu, bottom);
+    if (lane == 0) sh.warp_x[warp] = (static_cast<unsigned long long>(top) << 32) | bottom;
     __syncthreads();
-#pragma unroll 1
-    for (int run = 2; run <= size; run *= 2)
-#pragma unroll 1
-        for (int stride = run / 2; stride > 0; stride /= 2) {
-            for (int p = tid; p < size / 2; p += kSampleThreads) {
-                const int i = 2 * p - (p & (stride - 1)), j = i + stride;
-                const unsigned long long x = sh.sorted[i], y = sh.sorted[j];
-                const bool up = (i & run) != 0;
-                if ((x < y) != up) { sh.sorted[i] = y;  sh.sorted[j] = x; }
-            }
-            // (from a stride of 32 down a warp's pairs are those of 64 neighbouring entries, here and in the next step)
-            if (stride > 32 || (stride == 1 && run >= 64)) __syncthreads();
-            else __syncwarp();
+    {
+        const unsigned long long x = sh.warp_x[lane & (kSampleWarps - 1)];
+        top = __reduce_max_sync(0xFFFFFFFFu, uint32_t(x >> 32));
+        bottom = __reduce_min_sync(0xFFFFFFFFu, uint32_t(x));
+    }
+    const int shift = max(21 - __clz(max(top - bottom, 1u)), 0);       // (top - bottom) >> shift < 2,048
+    uint32_t place[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+        if (tid + i * kSampleThreads < n) place[i] = atomicAdd(&count[(top - uint32_t(mine[i] >> 32)) >> shift], 1u);
+    __syncthreads();
+    uint32_t c[kPer], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) { c[i] = count[tid * kPer + i];  sum += c[i]; }
+    uint32_t at = warp_upto32(sum, lane);
+    if (lane == 31) sh.warp_y[warp] = at;
+    __syncthreads();
+    at -= sum;
+#pragma unroll
+    for (int w = 0; w < kSampleWarps - 1; ++w) at += w < warp ? uint32_t(sh.warp_y[w]) : 0u;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) { start[tid * kPer + i] = at;  at += c[i]; }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+        if (tid + i * kSampleThreads < n) sh.list[start[(top - uint32_t(mine[i] >> 32)) >> shift] + place[i]] = mine[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+        if (tid + i * kSampleThreads < n) {
+            const uint32_t bucket = (top - uint32_t(mine[i] >> 32)) >> shift, from = start[bucket], m = count[bucket];
+            uint32_t rank = 0;
+            if (m > 1u)
+                for (uint32_t j = 0; j < m; ++j) rank += sh.list[from + j] > mine[i];
+            sh.sorted[from + rank] = mine[i];
         }
     __syncthreads();
 }
@@ -398,6 +444,7 @@ __device__ __forceinline__ void cut_of_list(SampleShared& sh, const SampleRow& r
         while (at >= sh.found[turn][b]) at -= sh.found[turn][b++];
         sh.sorted[i] = blocks > 1u ? lds_cluster_u64(ptx::mapa(ptx::smem_u32(&sh.list[at]), b)) : sh.list[at];
     }
+    __syncthreads();
     sort_list(sh, n);
     unsigned long long w[kPer], mine = 0;
 #pragma unroll
@@ -440,33 +487,59 @@ __device__ __forceinline__ void cut_of_list(SampleShared& sh, const SampleRow& r
     }
 }
 
-// The token among the sh.kept <= kSampleWalk candidates of sh.sorted: a thread each adds up what the kept candidates of lower index weigh.
+// The token among the sh.kept candidates at the front of sh.sorted: the weights of 256 equal parts of the vocabulary say in which part it is, and those of its
+// part are compared with one another.  Every thread of the first block calls.
 __device__ __forceinline__ void token_of_list(SampleShared& sh, const SampleRow& r, const SampleArgs& a, int n, uint32_t u24) {
-    const int tid = threadIdx.x, kept = int(sh.kept);
-    float x = 0.f;
-    unsigned long long w = 0;
-    int index = 0;
-    if (tid < kept) {
-        const unsigned long long c = sh.sorted[tid];
-        x = r.exponent(key_value(uint32_t(c >> 32)));
-        const float e = expf(x);
-        w = e >= r.min_p ? fixed(e) : 0ull;
-        index = int(~uint32_t(c));
-        sh.all[tid] = w;
-    }
+    constexpr int kMine = kSampleList / kSampleThreads;
+    const int tid = threadIdx.x, lane = tid & 31, kept = int(sh.kept), shift = max(24 - __clz(a.V), 0);      // V >> shift < 256
+    if (tid < 256) sh.all[tid] = 0ull;
+    if (tid == 0) sh.count = 0u;
     __syncthreads();
-    if (tid >= kept) return;
-    unsigned long long total = 0, before = 0;
-#pragma unroll 4
-    for (int j = 0; j < kept; ++j) {
-        const unsigned long long wj = sh.all[j];
-        total += wj;
-        if (int(~uint32_t(sh.sorted[j])) < index) before += wj;
-    }
-    const unsigned long long target = share_of(total, u24);
-    if (target >= before && target < before + w) {
-        a.token[n] = index;
-        if (a.logprob != nullptr) a.logprob[n] = x - logf(__ull2float_rn(total) * 9.094947017729282e-13f);
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+        if (tid + i * kSampleThreads < kept) {
+            const unsigned long long c = sh.sorted[tid + i * kSampleThreads];
+            const float e = r.ratio(key_value(uint32_t(c >> 32)));
+            if (e >= r.min_p) atomicAdd(&sh.all[~uint32_t(c) >> shift], fixed(e));
+        }
+    __syncthreads();
+    unsigned long long v[8], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { v[i] = sh.all[lane * 8 + i];  sum += v[i]; }
+    const unsigned long long upto = warp_upto(sum, lane), total = __shfl_sync(0xFFFFFFFFu, upto, 31), target = share_of(total, u24);
+    unsigned long long before = upto - sum;
+    const uint32_t hit = __ballot_sync(0xFFFFFFFFu, target >= before && target < upto);
+    int part = 0;
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+        if (part == i && target >= before + v[i]) { before += v[i];  part = i + 1; }
+    const int from = __ffs(hit) - 1;
+    part = from * 8 + __shfl_sync(0xFFFFFFFFu, part, from);
+    before = __shfl_sync(0xFFFFFFFFu, before, from);
+#pragma unroll
+    for (int i = 0; i < kMine; ++i)
+        if (tid + i * kSampleThreads < kept) {
+            const unsigned long long c = sh.sorted[tid + i * kSampleThreads];
+            if (int(~uint32_t(c) >> shift) == part) sh.list[atomicAdd(&sh.count, 1u)] = c;
+        }
+    __syncthreads();
+    const int m = int(sh.count);
+    for (int i = tid; i < m; i += kSampleThreads) {
+        const uint32_t index = ~uint32_t(sh.list[i]);
+        unsigned long long at = before, w = 0;
+        float l = 0.f;
+        for (int j = 0; j < m; ++j) {
+            const unsigned long long c = sh.list[j];
+            if (~uint32_t(c) > index) continue;
+            const float lj = key_value(uint32_t(c >> 32)), e = r.ratio(lj);
+            const unsigned long long wj = e >= r.min_p ? fixed(e) : 0ull;
+            if (j == i) { w = wj;  l = lj; }
+            else at += wj;
+        }
+        if (target >= at && target < at + w) {
+            a.token[n] = int(index);
+            if (a.logprob != nullptr) a.logprob[n] = r.exponent(l) - logf(__ull2float_rn(total) * 9.094947017729282e-13f);
+        }
     }
 }
 
@@ -490,7 +563,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     row.lane = lane;
     // The row's steps are dealt out evenly: every warp of the cluster has neighbouring ones, in the order of the vocabulary.
     const int row_steps = (row.end + kSampleStep - 1) / kSampleStep, parts = int(blocks) * kSampleWarps, me = int(rank) * kSampleWarps + warp;
-    auto first_step = [&](int part) { return int(int64_t(row_steps) * part / parts); };
+    auto first_step = [&](int part) { return row_steps * part / parts; };       // (at most 16,385 steps and 128 parts)
     const int first = first_step(me) * kSampleStep, steps = first_step(me + 1) - first_step(me);
 
     // ── maximum ──
@@ -504,7 +577,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     SampleRow r;
     const float t = a.temperature != nullptr ? ptx::ld(a.temperature + n) : 1.f;
     r.greedy = !(t > 0.f);
-    r.per = r.greedy ? 1.f : fmaxf(__frcp_rn(t), __uint_as_float(1u));      // (an infinite temperature: -inf has to stay -inf)
+    r.per = r.greedy ? 1.f : fmaxf(__frcp_rn(t), __uint_as_float(1u));      // (an infinite temperature: -inf has to stay below all)
     const int k = a.top_k != nullptr ? ptx::ld(a.top_k + n) : 0;
     r.k = k > 0 && k < a.V ? k : 0;
     const float p = a.top_p != nullptr ? ptx::ld(a.top_p + n) : 1.f;
@@ -516,7 +589,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) r.top = fmaxf(r.top, __shfl_xor_sync(0xFFFFFFFFu, r.top, o));
     if (lane == 0) sh.warp_max[warp] = r.top;
-    if (tid == 0) { sh.count = 0u;  sh.kept = 0x7FFFFFFFu; }
+    if (tid == 0) { sh.count = sh.digit = 0u;  sh.kept = 0x7FFFFFFFu; }
     __syncthreads();
     // a key that enough threads' largest logits reach: from the top, a bit at a time
     const int groups = (r.k + int(blocks) - 1) / int(blocks);
@@ -532,7 +605,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
             if (!few)
 #pragma unroll
                 for (int q = 1; q < kSampleQuarters; ++q) reach += __syncthreads_count(order_key(quarter[q]) >= (bound | bit));
-            if (reach >= groups) bound |= bit;
+            if (reach >= groups) {
+                bound |= bit;
+                if (reach <= groups + groups / 4 + 4) break;                     // (near enough)
+            }
         }
     }
     r.top = sh.warp_max[lane & (kSampleWarps - 1)];
@@ -557,6 +633,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         }
         return;
     }
+    r.odd = r.top == CUDART_INF_F || r.per == CUDART_INF_F;
     if (r.greedy) {
         // the lowest index of the largest logit
         if (mine == r.top)
@@ -584,40 +661,73 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     unsigned long long cut_ties = 0;
     int turn = 0;
     bool sums_known = false;                       // of the kept weights, per warp
-    auto part_of = [&](int index) { return int((int64_t((index + row.lead) / kSampleStep + 1) * parts - 1) / row_steps); };
+    auto part_of = [&](int index) { return (((index + row.lead) / kSampleStep + 1) * parts - 1) / row_steps; };
     bool have_cut = r.k == 0 && r.p24 < 0;
-    if (by_list) {
-        const float from = fmaxf(key_value(bound), -3.402823466e38f);       // (-inf is no candidate)
-#pragma unroll 1
-        for (int q = 0; q < kSampleQuarters; ++q) {
-            const float largest = q < 2 ? (q == 0 ? quarter[0] : quarter[1]) : (q == 2 ? quarter[2] : quarter[3]);
-            if (largest < from) continue;
-            row.each(first + quarter_step(q) * kSampleStep, quarter_step(q + 1) - quarter_step(q), [&](const float (&v)[8], int e) {
-                if (max_of(v) < from) return;
+    if (r.odd) {
+        // the tokens with the largest logit, of equal weight, as far as the filters let them
+        uint32_t mine_count = 0;
+        row.each(first, steps, [&](const float (&v)[8], int) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (v[i] >= from) list_logit(sh, v[i], e + i - row.lead);
-            });
+            for (int i = 0; i < 8; ++i) mine_count += v[i] == r.top;
+        });
+        unsigned long long x = mine_count, y = 0;
+        row_totals(sh, blocks, rank, turn, x, y);
+        cut = order_key(r.top + 0.f);
+        cut_ties = r.k > 0 ? min(x, static_cast<unsigned long long>(r.k)) : x;
+        if (r.p24 >= 0) cut_ties = min(cut_ties, (max(share_of(cut_ties << kSampleOneBits, uint32_t(r.p24)), 1ull) + (1ull << kSampleOneBits) - 1ull) >> kSampleOneBits);
+        have_cut = true;
+    } else if (by_list) {
+        const float from = fmaxf(key_value(bound), -3.402823466e38f);       // (-inf is no candidate)
+        // The quarters that have a candidate go to a list, and all threads share out their eights of logits: each waits for one or two loads.
+        uint32_t* const hits = reinterpret_cast<uint32_t*>(sh.sorted);
+#pragma unroll
+        for (int q = 0; q < kSampleQuarters; ++q)
+            if (quarter[q] >= from) hits[atomicAdd(&sh.digit, 1u)] = uint32_t(q * kSampleThreads + tid);
+        __syncthreads();
+        const int most = (row_steps / parts + 1 + kSampleQuarters - 1) / kSampleQuarters, eights = int(sh.digit) * most;       // steps of a quarter, at most
+        constexpr int kDeep = 4;
+#pragma unroll 1
+        for (int i0 = tid; i0 < eights; i0 += kDeep * kSampleThreads) {
+            alignas(16) T x[kDeep][8];
+            int e[kDeep];
+#pragma unroll
+            for (int d = 0; d < kDeep; ++d) {
+                const int i = i0 + d * kSampleThreads;
+                e[d] = row.end;                    // (nothing)
+                if (i < eights) {
+                    const int hit = int(hits[i / most]), q = hit / kSampleThreads, of = hit % kSampleThreads, part = int(rank) * kSampleWarps + of / 32;
+                    const int part_first = first_step(part), part_steps = first_step(part + 1) - part_first;
+                    const int step = part_steps * q / kSampleQuarters + i % most;
+                    if (step < part_steps * (q + 1) / kSampleQuarters) e[d] = (part_first + step) * kSampleStep + of % 32 * 8;
+                }
+                row.load(e[d], x[d]);
+            }
+#pragma unroll
+            for (int d = 0; d < kDeep; ++d) {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = logit_value(x[d][j]);
+                if (max_of(v) < from) continue;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (v[j] >= from) list_logit(sh, v[j], e[d] + j - row.lead);
+            }
         }
         unsigned long long x = 0, y = 0;
         row_totals(sh, blocks, rank, turn, x, y);
         const int m = listed(sh, blocks, turn);
         if (m >= 0) {
             if (rank == 0) cut_of_list(sh, r, blocks, turn, m, min(r.k, m), r.p24 < 0 ? ~0ull : 0ull);
-            sync_row(blocks);
-            if (sh.kept <= uint32_t(kSampleWalk)) {
-                if (rank == 0) token_of_list(sh, r, a, n, u24);
-                return;
-            }
-            cut = sh.cut;
-            cut_ties = sh.cut_ties;
-            have_cut = true;
+            sync_row(blocks);                      // (the lists have been read)
+            if (rank == 0) token_of_list(sh, r, a, n, u24);
+            return;
         }
     }
     if (!have_cut) {
         // The cut up to which `wanted` lies, among the finite logits above `above` (a key): tokens, or weight, of which `wanted` is then the share that
         // top-p says of all of it and of `ties`, the weight of the tokens kept at `above`.  False: it lies beyond (in the ties; no cut at all).
-        auto find_cut = [&](bool by_weight, uint32_t above, unsigned long long wanted, unsigned long long ties, unsigned long long& over) -> bool {
+        auto find_cut = [&](auto weights, uint32_t above, unsigned long long wanted, unsigned long long ties, unsigned long long& over) -> bool {
+            constexpr bool BY_WEIGHT = decltype(weights)::value, by_weight = BY_WEIGHT;
             const float above_value = above != 0u ? key_value(above) : -CUDART_INF_F;
             for (int i = tid; i < kSampleBins; i += kSampleThreads) sh.bins[i] = 0u;
             __syncthreads();
@@ -719,20 +829,31 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                 __syncthreads();
                 FixedSum sum_all, sum_ahead;
                 uint32_t n_all = 0, n_ahead = 0;
+                // (bins are powers of two: the same comparisons on the exponent itself)
+                const float x_from = from * (-1.f / kSampleBin), x_to = open ? -CUDART_INF_F : to * (-1.f / kSampleBin);
+                // (candidates are within `near` of `mid`, a little more than they need to be; where that is not a number, any may be one)
+                const float mid = r.top + 0.5f * (x_from + x_to) / r.per, near_by = 0.5001f * (x_from - x_to) / r.per + 1e-6f * (fabsf(r.top) + fabsf(mid));
+                const bool may_be = !(near_by < CUDART_INF_F) || !(fabsf(mid) < CUDART_INF_F);
                 row.each(first, steps, [&](const float (&v)[8], int e) {
+                    float off = CUDART_INF_F;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const float x = r.exponent(v[i]), at = x * -kSampleBin;
-                        const bool in = v[i] > above_value, is_ahead = in && at < from;
-                        if (by_weight) {
-                            const float w = in ? expf(x) : 0.f;
-                            sum_all.add(w);
-                            sum_ahead.add(is_ahead ? w : 0.f);
+                        const float x = r.exponent(v[i]);
+                        const bool in = v[i] > above_value, is_ahead = in && x > x_from;
+                        if constexpr (BY_WEIGHT) {
+                            sum_all.add_if(in ? expf(x) : 0.f, sum_ahead, is_ahead);
                         } else {
                             n_all += in;
                             n_ahead += is_ahead;
                         }
-                        if (in && !is_ahead && (open || at < to)) list_logit(sh, v[i], e + i - row.lead);
+                        off = fminf(off, fabsf(v[i] - mid));
+                    }
+                    if (off <= near_by || may_be) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const float x = r.exponent(v[i]);
+                            if (v[i] > above_value && !(x > x_from) && x > x_to) list_logit(sh, v[i], e + i - row.lead);
+                        }
                     }
                 });
                 over = by_weight ? sum_all.total() : n_all;
@@ -773,7 +894,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             const float x = r.exponent(v[i]);
-                            const bool in = v[i] > above_value && (open || x * -kSampleBin < to);
+                            const bool in = v[i] > above_value && x > x_to;
                             if (by_weight) sum_upto.add(in ? expf(x) : 0.f);
                             n_upto += in;
                         }
@@ -788,7 +909,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
             }
             wanted -= ahead;
             // Digit by digit, then.
-            const bool open = to == CUDART_INF_F;
+            const float x_from = from * (-1.f / kSampleBin), x_to = to == CUDART_INF_F ? -CUDART_INF_F : to * (-1.f / kSampleBin);
             uint32_t found = 0;
             int buffer = 0;
             for (int i = tid; i < 256; i += kSampleThreads) sh.hist[0][i] = 0ull;
@@ -800,8 +921,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                     for (int i = 0; i < 8; ++i) {
                         const uint32_t key = order_key(v[i] + 0.f);
                         const float x = r.exponent(v[i]);
-                        const float at = x * -kSampleBin;
-                        const bool in = v[i] > above_value && at >= from && (open || at < to) && (shift == 24 || (key >> (shift + 8)) == (found >> (shift + 8)));
+                        const bool in = v[i] > above_value && !(x > x_from) && x > x_to && (shift == 24 || (key >> (shift + 8)) == (found >> (shift + 8)));
                         const uint32_t digit = (key >> shift) & 255u, who = __ballot_sync(0xFFFFFFFFu, in);
                         if (who != 0u) {
                             unsigned long long w = in ? (by_weight ? fixed(expf(x)) : 1ull) : 0ull;
@@ -828,17 +948,17 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
             return true;
         };
         unsigned long long beyond;
-        if (r.k > 0) find_cut(false, 0u, static_cast<unsigned long long>(r.k), 0ull, beyond);
+        if (r.k > 0) find_cut(std::false_type{}, 0u, static_cast<unsigned long long>(r.k), 0ull, beyond);
         if (r.p24 >= 0) {
             // top-p looks at the tokens above top-k's cut, and at those of its ties that are kept
             const unsigned long long tie = cut_ties != 0ull ? fixed(r.ratio(key_value(cut))) : 0ull;
-            if (!find_cut(true, cut, 0ull, cut_ties * tie, beyond)) cut_ties = min(cut_ties, (beyond + tie - 1ull) / tie);
+            if (!find_cut(std::true_type{}, cut, 0ull, cut_ties * tie, beyond)) cut_ties = min(cut_ties, (beyond + tie - 1ull) / tie);
         }
     }
 
     // ── sums of the kept weights, per warp ──
     const float cut_value = cut != 0u ? key_value(cut) : -CUDART_INF_F;
-    const unsigned long long tie_weight = cut_ties != 0ull ? r.weight(cut_value) : 0ull;
+    const unsigned long long tie_weight = cut_ties != 0ull ? (r.odd ? 1ull << kSampleOneBits : r.weight(cut_value)) : 0ull;
     auto part_sums = [&](int from, int count, unsigned long long& sum, uint32_t& ties) {
         FixedSum kept;
         ties = 0;
@@ -954,7 +1074,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
 #pragma unroll
             for (int j = 1; j < 8; ++j) l = i == j ? v[j] : l;
             a.token[n] = e + i - row.lead;
-            if (a.logprob != nullptr) a.logprob[n] = r.exponent(l) - logf(__ull2float_rn(total) * 9.094947017729282e-13f);
+            if (a.logprob != nullptr) a.logprob[n] = (l == r.top ? 0.f : r.exponent(l)) - logf(__ull2float_rn(total) * 9.094947017729282e-13f);
         }
         before = __shfl_sync(0xFFFFFFFFu, lane_upto, 31);
         tie_before += __reduce_add_sync(0xFFFFFFFFu, here);
