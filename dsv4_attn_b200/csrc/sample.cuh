@@ -359,7 +359,7 @@ __device__ __forceinline__ void find_digit(SampleShared& sh, int buffer, unsigne
     __syncthreads();
 }
 
-// sh.sorted[0, n) into descending order, by way of sh.list: 2,048 buckets over the range of the keys, and within a bucket by comparing all with all
+// sh.sorted[0, n) into descending order, by way of sh.list: 2,048 buckets over the range of the logits, and within a bucket by comparing all with all
 // (there are two or three in one, unless many logits are equal).  A bitonic network took 4 us for 200 candidates and 26 for 1,400, this 2 to 3.
 // Every thread of the block calls.
 __device__ __forceinline__ void sort_list(SampleShared& sh, int n) {
@@ -386,11 +386,13 @@ __device__ __forceinline__ void sort_list(SampleShared& sh, int n) {
         top = __reduce_max_sync(0xFFFFFFFFu, uint32_t(x >> 32));
         bottom = __reduce_min_sync(0xFFFFFFFFu, uint32_t(x));
     }
-    const int shift = max(21 - __clz(max(top - bottom, 1u)), 0);       // (top - bottom) >> shift < 2,048
+    // (never decreasing as the logit falls; evenly over the logits, not over their bits, which are denser towards 0)
+    const float highest = key_value(top), scale = float(kBuckets - 1) / fmaxf(highest - key_value(bottom), 1e-30f);
+    auto bucket_of = [&](unsigned long long c) { return min(uint32_t((highest - key_value(uint32_t(c >> 32))) * scale), uint32_t(kBuckets - 1)); };
     uint32_t place[kMine];
 #pragma unroll
     for (int i = 0; i < kMine; ++i)
-        if (tid + i * kSampleThreads < n) place[i] = atomicAdd(&count[(top - uint32_t(mine[i] >> 32)) >> shift], 1u);
+        if (tid + i * kSampleThreads < n) place[i] = atomicAdd(&count[bucket_of(mine[i])], 1u);
     __syncthreads();
     uint32_t c[kPer], sum = 0;
 #pragma unroll
@@ -406,12 +408,12 @@ __device__ __forceinline__ void sort_list(SampleShared& sh, int n) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kMine; ++i)
-        if (tid + i * kSampleThreads < n) sh.list[start[(top - uint32_t(mine[i] >> 32)) >> shift] + place[i]] = mine[i];
+        if (tid + i * kSampleThreads < n) sh.list[start[bucket_of(mine[i])] + place[i]] = mine[i];
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kMine; ++i)
         if (tid + i * kSampleThreads < n) {
-            const uint32_t bucket = (top - uint32_t(mine[i] >> 32)) >> shift, from = start[bucket], m = count[bucket];
+            const uint32_t bucket = bucket_of(mine[i]), from = start[bucket], m = count[bucket];
             uint32_t rank = 0;
             if (m > 1u)
                 for (uint32_t j = 0; j < m; ++j) rank += sh.list[from + j] > mine[i];
