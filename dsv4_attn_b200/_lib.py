@@ -69,7 +69,7 @@ EXPORTS = ("dsv4_attn_version", "dsv4_debug_set_wait", "dsv4_debug_set_flags", "
            "dsv4_hca_dense_decode_fwd", "dsv4_hca_dense_decode_simt", "dsv4_attn_combine", "dsv4_attn_plan_splits",
            "dsv4_attn_workspace_bytes", "hca_decode_fwd", "dsv4_hca_compress_fwd", "dsv4_kv_quantize_insert",
            "dsv4_hca_packed_decode_fwd", "dsv4_rope_norm_fwd", "dsv4_indexer_topk_fwd",
-           "dsv4_hca_tree_decode_fwd", "dsv4_kv_pages_copy", "dsv4_kv_pages_fork", "dsv4_kv_pages_free", "dsv4_kv_pages_compact", "dsv4_kv_entries_move",
+           "dsv4_hca_tree_decode_fwd", "dsv4_hca_tree_rows_bytes", "dsv4_kv_pages_copy", "dsv4_kv_pages_fork", "dsv4_kv_pages_free", "dsv4_kv_pages_compact", "dsv4_kv_entries_move",
            "dsv4_sample_fwd")
 
 
@@ -143,7 +143,7 @@ class HcaTreeDecodeParams(C.Structure):
         ("q", C.c_void_p), ("kv_pool", C.c_void_p), ("block_table", C.c_void_p), ("kv_len", C.c_void_p),
         ("win_pool", C.c_void_p), ("win_len", C.c_void_p), ("tree_mask", C.c_void_p), ("attn_sink", C.c_void_p),
         ("out", C.c_void_p), ("lse", C.c_void_p), ("partial_o", C.c_void_p), ("partial_lse", C.c_void_p),
-        ("status", C.c_void_p), ("sched", C.c_void_p), ("sched_bytes", C.c_int64),
+        ("status", C.c_void_p), ("sched", C.c_void_p), ("sched_bytes", C.c_int64), ("rows", C.c_void_p), ("rows_bytes", C.c_int64),
     ]
 
 
@@ -209,6 +209,8 @@ def _load() -> C.CDLL:
     lib.dsv4_attn_plan_host.argtypes = [P(PlanParams)]
     lib.dsv4_attn_sched_bytes.restype = C.c_int64
     lib.dsv4_attn_sched_bytes.argtypes = [C.c_int, C.c_int, C.c_int, C.c_int, P(C.c_int64), P(C.c_int64)]
+    lib.dsv4_hca_tree_rows_bytes.restype = C.c_int64
+    lib.dsv4_hca_tree_rows_bytes.argtypes = [C.c_int, C.c_int, C.c_int]
     lib.dsv4_noalloc_scratch_bytes.restype = C.c_int64
     lib.dsv4_noalloc_scratch_bytes.argtypes = []
     lib.dsv4_attn_last_error.restype = C.c_char_p

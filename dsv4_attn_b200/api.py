@@ -62,7 +62,7 @@ ENTRY_POINTS = (
     "dsv4_kv_quantize_insert", "dsv4_csa_compress_reduce_fwd", "dsv4_hca_compress_fwd", "dsv4_indexer_topk_fwd", "dsv4_attn_combine",
     "dsv4_attn_plan", "dsv4_attn_plan_splits",
     "dsv4_hca_tree_decode_fwd", "dsv4_attn_sched_bytes", "dsv4_kv_pages_copy", "dsv4_kv_pages_fork", "dsv4_kv_pages_free", "dsv4_kv_pages_compact",
-    "dsv4_kv_entries_move", "dsv4_sample_fwd")
+    "dsv4_kv_entries_move", "dsv4_sample_fwd", "dsv4_hca_tree_rows_bytes")
 _host.bind(*(C.cast(getattr(_lib.LIB, name), C.c_void_p).value for name in ENTRY_POINTS))
 
 
@@ -591,7 +591,7 @@ def indexer_topk(q_fp8, q_weight, key_pages, block_table, n_vis, k, *, scores=No
 
 # ── a speculative step (include/dsv4_speculative.h) ──
 def hca_tree_decode(q, kv_pool, block_table, kv_len, win_pool, win_len, tree_mask, sm_scale, *, attn_sink=None, num_splits=None,
-                    out=None, lse=None, workspace=None, status=None, max_len=None, plan=None):
+                    out=None, lse=None, workspace=None, status=None, max_len=None, plan=None, share_rows=None):
     """HCA decode of the T drafted nodes of a tree per request, in one call: every node attends to the request's
     compressed entries [0, kv_len[b]) and to the rows of its window buffer that the node's mask names.
     q bf16 [B, T, H, 576]; kv_pool uint8 [P, 64, 656]; block_table int32 [B, max_pages]; kv_len / win_len int32 [B];
@@ -600,9 +600,12 @@ def hca_tree_decode(q, kv_pool, block_table, kv_len, win_pool, win_len, tree_mas
 
     `num_splits` None: where the nodes fill the device more than once the call plans the work on the device
     (as `plan_hca(B, 1, T * H, kv_len[:, None], win_len[:, None])` does, which can be passed as `plan` to all layers
-    of a step instead); otherwise rows are split so that it is full."""
+    of a step instead); otherwise rows are split so that it is full.
+    `share_rows` None: where a request has several groups of 128 (node, head) rows, its entries are dequantised once, into a
+    workspace of `tree_rows_bytes(B, max_pages, W)` that the call allocates, instead of by each group; True and False say so,
+    and a uint8 tensor is the workspace."""
     r = _host.tree(q, kv_pool, block_table, kv_len, win_pool, win_len, tree_mask, sm_scale, attn_sink, num_splits, out, lse, workspace, status, max_len,
-                   None if plan is None else plan.fast)
+                   None if plan is None else plan.fast, share_rows)
     if r is not None:
         return r if type(r) is tuple else _rc(r, "dsv4_hca_tree_decode_fwd")
     _cuda_contig(q, "q", torch.bfloat16, 4)
@@ -638,7 +641,17 @@ def hca_tree_decode(q, kv_pool, block_table, kv_len, win_pool, win_len, tree_mas
         _cuda_contig(pl, "partial_lse", torch.float32)
         _check(num_splits is not None and po.numel() >= num_splits * B * T * H * D_LATENT and pl.numel() >= num_splits * B * T * H,
                "workspace needs num_splits, and room for that many")
+    if isinstance(share_rows, torch.Tensor):
+        _cuda_contig(share_rows, "share_rows", torch.uint8, 1)
+        _check(share_rows.numel() >= tree_rows_bytes(B, block_table.shape[1], win_pool.shape[1]) > 0, "share_rows must hold tree_rows_bytes()")
+    else:
+        _check(share_rows in (None, True, False), "share_rows must be None, True, False or a workspace")
     raise Dsv4Error("dsv4_hca_tree_decode_fwd refused the call (sizes out of range, or no device memory)")
+
+
+def tree_rows_bytes(B, max_pages, W) -> int:
+    """Size of the workspace in which the groups of a tree decode share a request's dequantised entries (0: not for such sizes)."""
+    return int(_lib.LIB.dsv4_hca_tree_rows_bytes(int(B), int(max_pages), int(W)))
 
 
 def sample(logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None, out=None, logprob=None):

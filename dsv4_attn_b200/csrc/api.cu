@@ -23,6 +23,7 @@
 #include "decode_kernel.cuh"
 #include "sched.cuh"
 #include "decode_simt.cuh"
+#include "tree_kernel.cuh"
 #include "kv_pages.cuh"
 #include "sample.cuh"
 
@@ -368,13 +369,11 @@ int launch_failed(cudaError_t e) {
     return int(e);
 }
 
-// Decode (+ merge when split) for the packed-entry sources.  With a plan, the resident blocks walk it and the
-// merge adds up the units the plan cut.
+// The merge after a decode, where it was split or the plan cut units.
 template <int SRC>
-int decode_fwd(DecodeArgs& a, const void* sched, cudaStream_t stream) {
+int merge_fwd(const DecodeArgs& a, const void* sched, cudaStream_t stream) {
     const int rows = a.B * a.s_q;
-    cudaError_t e = launch_mma<9, SRC>(a, rows, sched, stream);
-    if (e != cudaSuccess) return launch_failed(e);
+    cudaError_t e = cudaSuccess;
     if (sched != nullptr) {
         const int hgs = (a.H + kHeadsPerCta - 1) / kHeadsPerCta;
         const SchedLayout l = sched_layout(rows * hgs, 0);
@@ -393,6 +392,14 @@ int decode_fwd(DecodeArgs& a, const void* sched, cudaStream_t stream) {
         e = launch_combine(c, stream);
     }
     return e == cudaSuccess ? 0 : launch_failed(e);
+}
+
+// Decode (+ merge when split) for the packed-entry sources.  With a plan, the resident blocks walk it and the
+// merge adds up the units the plan cut.
+template <int SRC>
+int decode_fwd(DecodeArgs& a, const void* sched, cudaStream_t stream) {
+    const cudaError_t e = launch_mma<9, SRC>(a, a.B * a.s_q, sched, stream);
+    return e != cudaSuccess ? launch_failed(e) : merge_fwd<SRC>(a, sched, stream);
 }
 
 }  // namespace
@@ -916,6 +923,71 @@ extern "C" int dsv4_indexer_topk_fwd(const Dsv4IndexerTopkParams* p, void* strea
 
 // ── a speculative step: tree decode, pages, sampling (dsv4_speculative.h) ──
 
+namespace {
+// Rows a request has in the workspace of a tree decode.
+int64_t tree_rows(int max_pages, int win_cap) { return (int64_t(max_pages) * DSV4_PAGE_ENTRIES + win_cap + kTileN - 1) / kTileN * kTileN; }
+
+// FP16 rows of 576, `box_rows` by 64 columns, 128-byte swizzle.
+cudaError_t make_tile_map(CUtensorMap* map, const void* base, int64_t rows, int box_rows) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (fn == nullptr) return cudaErrorNotSupported;
+    const cuuint64_t dims[2] = {576, cuuint64_t(rows)};
+    const cuuint64_t strides[1] = {1152};
+    const cuuint32_t box[2] = {64, cuuint32_t(box_rows)};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+// The entries into the workspace, and the attention over them.
+cudaError_t launch_tree(const DecodeArgs& d, const Dsv4HcaTreeDecodeParams* p, const void* sched, cudaStream_t stream) {
+    const int64_t cap = tree_rows(p->max_pages, p->win_cap);
+    TreeUnpackArgs u{};
+    u.B = p->B;  u.T = p->T;  u.max_pages = p->max_pages;  u.win_cap = p->win_cap;  u.mask_words = p->mask_words;  u.cap = int(cap);
+    u.num_pages = p->num_pages;
+    u.kv_pool = d.kv_pool;  u.win_pool = d.win_pool;  u.block_table = d.block_table;  u.kv_len = d.kv_len;  u.win_len = d.win_len;  u.tree_mask = d.tree_mask;
+    u.rows = static_cast<uint8_t*>(p->rows);
+    u.valid = reinterpret_cast<uint32_t*>(u.rows + p->B * cap * 1152);
+    u.status = d.status;
+    const int64_t tiles = p->B * (cap / kTileN), resident = int64_t(device_sms()) * 8;
+    cudaError_t e = launch(tree_unpack_kernel, dim3(unsigned(tiles < resident ? tiles : resident)), kUnpackThreads, 0, stream, u);
+    if (e != cudaSuccess) return e;
+    TreeArgs a{};
+    e = make_q_map(&a.q_map, d.q, int64_t(d.B) * d.H, 576);
+    if (e == cudaSuccess) e = make_tile_map(&a.k_map, u.rows, p->B * cap, kRowsPerBlock);
+    if (e == cudaSuccess) e = make_tile_map(&a.v_map, u.rows, p->B * cap, kTileN);
+    if (e != cudaSuccess) return e;
+    a.B = d.B;  a.H = d.H;  a.heads = d.tree_heads;  a.cap = int(cap);  a.mask_words = d.tree_words;  a.num_splits = d.num_splits;  a.scale_log2 = d.scale_log2;
+    a.valid = u.valid;  a.kv_len = d.kv_len;  a.win_len = d.win_len;  a.tree_mask = d.tree_mask;  a.attn_sink = d.attn_sink;
+    a.out = d.out;  a.lse = d.lse;  a.partial_o = d.partial_o;  a.partial_lse = d.partial_lse;  a.status = d.status;
+    const unsigned long long wait_ns = g_wait_ns.load(std::memory_order_relaxed);
+    a.wait_ns = uint32_t(wait_ns < 4000000000ull ? wait_ns : 4000000000ull);
+    a.dbg_drop_tile = g_drop_tile.load(std::memory_order_relaxed);
+    const int groups = (a.H + kHeadsPerCta - 1) / kHeadsPerCta;
+    dim3 grid(2 * groups, a.B, a.num_splits);
+    if (sched != nullptr) {
+        const SchedLayout l = sched_layout(a.B * groups, 0);
+        const int32_t* base = static_cast<const int32_t*>(sched);
+        a.sched_pair_begin = base + l.pair_begin;
+        a.sched_items = base + l.items;
+        int pairs = device_sms() / 2;
+        if (pairs > kPlanMaxPairs) pairs = kPlanMaxPairs;
+        grid = dim3(2 * (pairs > 0 ? pairs : 1), 1, 1);
+    }
+    static std::atomic<bool> done[kMaxDevices];
+    e = ensure_smem(tree_mma_kernel, TreeSmem::kTotal, done);
+    if (e != cudaSuccess) return e;
+    return launch(tree_mma_kernel, grid, kTreeThreads, TreeSmem::kTotal, stream, a);
+}
+}  // namespace
+
+extern "C" int64_t dsv4_hca_tree_rows_bytes(int B, int max_pages, int win_cap) {
+    if (B <= 0 || max_pages <= 0 || win_cap < 0) return 0;
+    const int64_t cap = tree_rows(max_pages, win_cap);
+    return B * cap > 0x7FFFFFFF ? 0 : B * cap * 1152 + B * cap / 8;        // (TMA coordinates are 32-bit)
+}
+
 extern "C" int dsv4_hca_tree_decode_fwd(const Dsv4HcaTreeDecodeParams* p, void* stream) {
     t_last_error = "invalid argument";
     if (p == nullptr || p->T <= 0 || p->H <= 0 || p->num_splits < 0 || p->mask_words < 0) return int(cudaErrorInvalidValue);
@@ -927,6 +999,13 @@ extern "C" int dsv4_hca_tree_decode_fwd(const Dsv4HcaTreeDecodeParams* p, void* 
     if (p->kv_pool == nullptr || p->block_table == nullptr || p->kv_len == nullptr || p->win_len == nullptr) return int(cudaErrorInvalidValue);
     if ((p->win_cap > 0 && p->win_pool == nullptr) || (p->mask_words > 0 && p->tree_mask == nullptr)) return int(cudaErrorInvalidValue);
     if (!aligned(p->kv_pool, 16) || !aligned(p->win_pool, 16)) return int(cudaErrorInvalidValue);
+    if (p->rows != nullptr) {
+        const int64_t bytes = dsv4_hca_tree_rows_bytes(p->B, p->max_pages, p->win_cap);
+        if (bytes <= 0 || p->rows_bytes < bytes || !aligned(p->rows, 16)) {
+            t_last_error = "workspace smaller than dsv4_hca_tree_rows_bytes() for this shape";
+            return int(cudaErrorInvalidValue);
+        }
+    }
     t_last_error = "";
     DecodeArgs a{};
     a.B = p->B;  a.s_q = 1;  a.H = int(rows);  a.max_pages = p->max_pages;  a.win_cap = p->win_cap;
@@ -950,7 +1029,10 @@ extern "C" int dsv4_hca_tree_decode_fwd(const Dsv4HcaTreeDecodeParams* p, void* 
         const int rc = dsv4_attn_plan(&q, stream);
         if (rc != 0) return rc;
     }
-    return decode_fwd<kSrcTree>(a, scheduled ? p->sched : nullptr, static_cast<cudaStream_t>(stream));
+    const void* sched = scheduled ? p->sched : nullptr;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const cudaError_t e = p->rows != nullptr ? launch_tree(a, p, sched, s) : launch_mma<9, kSrcTree>(a, a.B, sched, s);
+    return e != cudaSuccess ? launch_failed(e) : merge_fwd<kSrcTree>(a, sched, s);
 }
 
 namespace {

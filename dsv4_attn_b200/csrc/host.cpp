@@ -42,6 +42,7 @@ struct Library {
     decltype(&dsv4_kv_pages_compact) pages_compact;
     decltype(&dsv4_kv_entries_move) entries_move;
     decltype(&dsv4_sample_fwd) sample;
+    decltype(&dsv4_hca_tree_rows_bytes) tree_rows_bytes;
 } lib;
 
 constexpr int kLatent = 512, kQk = 576, kEntry = DSV4_ENTRY_BYTES, kPage = DSV4_PAGE_ENTRIES;
@@ -479,10 +480,12 @@ PyObject* combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // Where the library plans the work of a tree decode in the call: more row groups than the device has pairs of SMs (74).  Below that one wave of pairs is
 // enough, with rows split so that it is full.
 constexpr int64_t kTreePlanGroups = 74;
+// Where the groups of a request share its dequantised entries: from this many groups on, for workspaces of up to this size.
+constexpr int64_t kTreeShareGroups = 4, kTreeShareBytes = int64_t(4) << 30;
 
-// (q, kv_pool, block_table, kv_len, win_pool, win_len, tree_mask, sm_scale, attn_sink, num_splits, out, lse, workspace, status, max_len, plan)
+// (q, kv_pool, block_table, kv_len, win_pool, win_len, tree_mask, sm_scale, attn_sink, num_splits, out, lse, workspace, status, max_len, plan, share_rows)
 PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
-    if (n != 16) return none();
+    if (n != 17) return none();
     const at::Tensor *q = tensor(a[0], at::kBFloat16, 4), *pool = tensor(a[1], at::kByte, 3), *table = tensor(a[2], at::kInt, 2), *kv_len = tensor(a[3], at::kInt, 1);
     const at::Tensor *win = tensor(a[4], at::kByte, 3), *win_len = tensor(a[5], at::kInt, 1), *mask = tensor(a[6], at::kInt, 3), *sink, *status;
     Dsv4HcaTreeDecodeParams p{};
@@ -536,6 +539,21 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
             own_pl = empty({splits * rows}, at::kFloat, q);
             po = &own_po;  pl = &own_pl;
         }
+    }
+    at::Tensor own_rows;
+    const at::Tensor* shared = nullptr;
+    const int64_t rows_bytes = lib.tree_rows_bytes(int(B), int(table->size(1)), int(W));
+    if (a[16] == Py_True || (a[16] == Py_None && groups >= kTreeShareGroups * B && rows_bytes > 0 && rows_bytes <= kTreeShareBytes)) {
+        if (rows_bytes <= 0) return none();
+        own_rows = empty({rows_bytes}, at::kByte, q);
+        shared = &own_rows;
+    } else if (a[16] != Py_None && a[16] != Py_False) {
+        shared = tensor(a[16], at::kByte, 1);
+        if (shared == nullptr || rows_bytes <= 0 || shared->numel() < rows_bytes) return none();
+    }
+    if (shared != nullptr) {
+        p.rows = ptr(shared);
+        p.rows_bytes = shared->numel();
     }
     Output out, lse;
     if (!out.take(a[10], at::kBFloat16, {B, T, H, kLatent}, q) || !lse.take(a[11], at::kFloat, {B, T, H}, q)) return none();

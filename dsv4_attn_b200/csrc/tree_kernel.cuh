@@ -1,0 +1,643 @@
+// Tree decode for many (node, head) rows per request: every group of 128 rows reads the same entries, so these are dequantised once, into FP16 rows
+// in a workspace, and the attention kernel gets its operands from there by TMA, in the layout the MMAs want.
+//
+//   tree_unpack_kernel   entries of a request (cache, then window) -> FP16 [B, cap, 576] and a bit per entry that takes part
+//   tree_mma_kernel      the pair scheme of decode_kernel.cuh (cta_group::2, M = 128: 64 rows, half of the entries and half of the value columns a
+//                        block; S and O in tensor memory) without its resolve, fetch and dequantise warps; two buffers for K and V.
+//
+// What that changes per tile of 64 entries and SM: 69 KB by TMA from L2 instead of 30 KB of raw records, but no raw reads, conversions and
+// operand stores, which kept the shared-memory port busy for 1130 of its 2000 cycles.  Bounds, in SM cycles: tensor pipe 1244 (as there), shared-memory port 540
+// in + 860 out, L2 at the measured 16.4 TB/s (58 bytes a cycle and SM) 1190.  The direct kernel takes 2570.
+//
+// Rounding: an entry is e4m3 x scale in FP16, in the same operations as in the direct kernel; results differ from it in nothing but the
+// order of sums.
+#pragma once
+
+#include "decode_kernel.cuh"
+
+namespace dsv4 {
+
+constexpr int kUnpackThreads = 256;
+
+struct TreeUnpackArgs {
+    int B, T, max_pages, win_cap, mask_words, cap;
+    int64_t num_pages;
+    const uint8_t* kv_pool;
+    const uint8_t* win_pool;
+    const int32_t* block_table;
+    const int32_t* kv_len;
+    const int32_t* win_len;
+    const int32_t* tree_mask;
+    uint8_t* rows;             // FP16 [B, cap, 576]
+    uint32_t* valid;           // [B, cap / 32]
+    int32_t* status;
+};
+
+// A block takes tiles of 64 entries, a warp eight entries of one.  An entry: a lane has 16 latent bytes and their block's scale, eight lanes a piece of
+// the RoPE tail.  Rows that take no part (out of range, or window rows that no node sees) are zero: whatever probability they get is zero too,
+// and zero times what the memory held might not be.  DRAM-bound: 656 bytes read and 1152 written an entry.
+__global__ void __launch_bounds__(kUnpackThreads) tree_unpack_kernel(const __grid_constant__ TreeUnpackArgs a) {
+    constexpr int kEach = 8;
+    __shared__ uint32_t s_valid[8];
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tiles = a.cap / kTileN;
+    for (int64_t u = blockIdx.x; u < int64_t(a.B) * tiles; u += gridDim.x) {
+        const int b = int(u / tiles), v0 = int(u % tiles) * kTileN;
+        const int kv_len = max(ptx::ld(a.kv_len + b), 0), win_len = max(ptx::ld(a.win_len + b), 0);
+        const int64_t n_tok = int64_t(kv_len) + win_len;
+        if (v0 == 0 && n_tok > a.cap && threadIdx.x == 0) report_status(a.status, kStatusBadIndex, 4, kv_len);
+        if (v0 >= n_tok) continue;
+        // where the warp's entries live (lane i: entry i)
+        const uint8_t* rec = nullptr;
+        const int v = v0 + warp * kEach + (lane & (kEach - 1));
+        if (v < n_tok) {
+            if (v < kv_len) {
+                const int slot = v >> 6, page = slot < a.max_pages ? ptx::ld(a.block_table + int64_t(b) * a.max_pages + slot) : -1;
+                if (page >= 0 && page < a.num_pages) rec = a.kv_pool + (int64_t(page) * 64 + (v & 63)) * 656;
+                else if (lane < kEach) report_status(a.status, kStatusBadIndex, 4, slot < a.max_pages ? page : v);
+            } else if (v - kv_len < a.win_cap) {
+                rec = a.win_pool + (int64_t(b) * a.win_cap + (v - kv_len)) * 656;
+            } else if (lane < kEach) {
+                report_status(a.status, kStatusBadIndex, 4, v);
+            }
+        }
+        if (v0 + kTileN > kv_len) {
+            // (a tile with window rows) the rows that any node sees
+#pragma unroll 1
+            for (int i = 0; i < kEach; ++i) {
+                const int w = v0 + warp * kEach + i - kv_len;
+                if (w < 0) continue;
+                uint32_t any = 0u;
+                if ((w >> 5) < a.mask_words)
+                    for (int t = lane; t < a.T; t += 32) any |= uint32_t(ptx::ld(a.tree_mask + (int64_t(b) * a.T + t) * a.mask_words + (w >> 5)));
+                if (!__any_sync(0xFFFFFFFFu, (any >> (w & 31)) & 1u) && (lane & (kEach - 1)) == i) rec = nullptr;
+            }
+        }
+        const uint32_t valid = __ballot_sync(0xFFFFFFFFu, rec != nullptr) & ((1u << kEach) - 1u);
+        uint4 x[kEach], rope[kEach];
+        float scale[kEach];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const uint8_t* p = reinterpret_cast<const uint8_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(rec), i));
+            x[i] = rope[i] = make_uint4(0, 0, 0, 0);
+            scale[i] = 0.f;
+            if (p != nullptr) {
+                x[i] = ptx::ldg_stream_v4(p + lane * 16);
+                scale[i] = ptx::ld(reinterpret_cast<const float*>(p + 512) + (lane >> 3));
+                if (lane < 8) rope[i] = ptx::ldg_stream_v4(p + 528 + lane * 16);
+            }
+        }
+        uint8_t* row = a.rows + (int64_t(b) * a.cap + v0 + warp * kEach) * 1152;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i, row += 1152) {
+            const __half2 scale2 = __float2half2_rn(fminf(scale[i], 146.f));
+            uint4 lo, hi;
+            dequant4_f16(x[i].x, scale2, lo.x, lo.y);
+            dequant4_f16(x[i].y, scale2, lo.z, lo.w);
+            dequant4_f16(x[i].z, scale2, hi.x, hi.y);
+            dequant4_f16(x[i].w, scale2, hi.z, hi.w);
+            reinterpret_cast<uint4*>(row)[2 * lane] = lo;
+            reinterpret_cast<uint4*>(row)[2 * lane + 1] = hi;
+            if (lane < 8) reinterpret_cast<uint4*>(row + 1024)[lane] = bf16x8_to_f16x8(rope[i]);
+        }
+        __syncthreads();                           // the bits of the tile before have been read
+        if (lane == 0) s_valid[warp] = valid;
+        __syncthreads();
+        if (threadIdx.x < 2) {
+            const uint32_t* s = s_valid + 4 * threadIdx.x;
+            a.valid[(int64_t(b) * a.cap + v0) / 32 + threadIdx.x] = s[0] | (s[1] << 8) | (s[2] << 16) | (s[3] << 24);
+        }
+    }
+}
+
+// Warp roles of the attention kernel.
+constexpr int kTreeQWarps = 8;                 // warps 4-11: Q into tensor memory, BF16 to FP16
+constexpr int kTreeFirstQWarp = 4;
+constexpr int kTreeSWarp = 12;                 // tensor-memory allocation; (even block) issue of the S MMAs
+constexpr int kTreeOWarp = 13;                 // (even block) issue of the O MMAs
+constexpr int kTreeLoadWarp = 14;              // K and V tiles
+constexpr int kTreeRelayWarp = 15;             // tells the even block that a tile has landed here
+constexpr int kTreeSendWarp = 16;              // Q
+constexpr int kTreeThreads = 17 * 32;
+
+struct TreeArgs {
+    alignas(64) CUtensorMap q_map;             // BF16 [B * H, 576], box 64 x 64
+    alignas(64) CUtensorMap k_map;             // FP16 [B * cap, 576], box 64 columns x 32 rows
+    alignas(64) CUtensorMap v_map;             // the same, 64 columns x 64 rows
+    int B, H, heads;                           // H: (node, head) rows of a request
+    int cap;                                   // rows per request in the workspace, a multiple of 64
+    int mask_words;
+    int num_splits;
+    float scale_log2;
+    const uint32_t* valid;
+    const int32_t* kv_len;
+    const int32_t* win_len;
+    const int32_t* tree_mask;
+    const float* attn_sink;
+    __nv_bfloat16* out;
+    float* lse;
+    float* partial_o;
+    float* partial_lse;
+    int32_t* status;
+    const int32_t* sched_pair_begin;
+    const int32_t* sched_items;
+    uint32_t wait_ns;
+    int dbg_drop_tile;
+};
+
+struct TreeSmem {
+    static constexpr int kQBytes = 3 * kQChunkBytes;            // chunks 6-8 stay here
+    static constexpr int kStageBytes = 6 * kQChunkBytes;        // chunks 0-5 on their way to tensor memory
+    static constexpr int kKBytes = 9 * kKChunkBytes;
+    static constexpr int kVBytes = 4 * kVChunkBytes;
+    static constexpr int kQOff = 0;
+    static constexpr int kStageOff = kQOff + kQBytes;
+    static constexpr int kKOff = kStageOff + kStageBytes;
+    static constexpr int kVOff = kKOff + 2 * kKBytes;
+    static constexpr int kPOff = kVOff + 2 * kVBytes;
+    static constexpr int kMiscOff = kPOff + 2 * kQChunkBytes;
+    static constexpr int kTotal = kMiscOff + 3072;
+    static_assert(kTotal <= 232448, "shared memory of a block");
+    static_assert(kKOff % 1024 == 0 && kVOff % 1024 == 0 && kPOff % 1024 == 0, "swizzled operands");
+};
+
+struct TreeMisc {
+    float exch[2 * kHeadsPerBlock];
+    uint64_t bar_tmem;
+    uint64_t bar_q_full[2];          // per item: chunks 0-5 / 6-8 landed
+    uint64_t bar_q_copied;           // per item: chunks 0-5 copied out by every Q warp
+    uint64_t bar_land[2][2];         // K / V tile landed in this block, by buffer
+    // signalled in both blocks by the commits of the MMA warps
+    uint64_t bar_q_free;             // per item: its S MMAs complete
+    uint64_t bar_s_full[2];          // S of a tile complete: S buffer full, K buffer free
+    uint64_t bar_o_full[2];          // P.V of a tile complete: V and P buffer free, O up to date
+    // in the even block only, signalled by the warps of both
+    uint64_t bar_q_ready;
+    uint64_t bar_k_full[2], bar_v_full[2], bar_p_full[2];
+    uint32_t tmem_base;
+};
+static_assert(sizeof(TreeMisc) <= 3072 - 16, "the last word of the block's shared memory is failed_flag()");
+
+// The window rows [o, o + 32) that a node sees; rows below 0 are entries of the cache, which every node sees.
+__device__ __forceinline__ uint32_t window_bits(const int32_t* mask, int words, int o) {
+    if (o <= -32) return ~0u;
+    const int first = max(o, 0), w = first >> 5;
+    const uint32_t lo = w < words ? uint32_t(ptx::ld(mask + w)) : 0u, hi = w + 1 < words ? uint32_t(ptx::ld(mask + w + 1)) : 0u;
+    const uint32_t m = __funnelshift_r(lo, hi, first & 31);
+    return o < 0 ? (m << -o) | ((1u << -o) - 1u) : m;
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tree_mma_kernel(const __grid_constant__ TreeArgs a) {
+    using L = TreeSmem;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    const uint32_t smem_base = ptx::smem_u32(smem_raw);
+    if (smem_base & 1023u) {                      // the operand layout needs it; the same answer in every block
+        report_status(a.status, kStatusWaitQ, 5, -1);
+        return;
+    }
+    const uint32_t q_base = smem_base + L::kQOff, q_stage = smem_base + L::kStageOff, k_base = smem_base + L::kKOff, v_base = smem_base + L::kVOff,
+                   p_base = smem_base + L::kPOff;
+    TreeMisc* misc = reinterpret_cast<TreeMisc*>(smem_raw + L::kMiscOff);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = int(blockIdx.x & 1u);
+    const bool sched = a.sched_pair_begin != nullptr;
+    const uint32_t wait_ns = a.wait_ns;
+
+    int item_begin = 0, n_items = 1;
+    auto get_item = [&](int k) -> Item {
+        Item it;
+        if (sched) {
+            const int4* rec = reinterpret_cast<const int4*>(a.sched_items + int64_t(item_begin + k) * kItemWords);
+            const int4 r0 = ptx::ld(rec), r1 = ptx::ld(rec + 1);
+            it.n = r0.x;  it.hg = r0.y;  it.tile0 = r0.z;  it.ntiles = r0.w;
+            it.slot = r1.x;  it.n_tok = r1.y;  it.kv_len_n = r1.z;
+            // (lengths beyond the workspace have been reported: what lies there is left out)
+            it.n_tok = min(it.n_tok, a.cap);
+            it.ntiles = min(it.ntiles, max(a.cap / kTileN - it.tile0, 0));
+        } else {
+            it.n = blockIdx.y;  it.hg = blockIdx.x >> 1;
+            it.kv_len_n = max(ptx::ld(a.kv_len + it.n), 0);
+            it.n_tok = int(min(int64_t(it.kv_len_n) + max(ptx::ld(a.win_len + it.n), 0), int64_t(a.cap)));
+            const int split = blockIdx.z;
+            const int tiles_total = (it.n_tok + kTileN - 1) / kTileN;
+            const int tiles_per_split = (tiles_total + a.num_splits - 1) / a.num_splits;
+            it.tile0 = min(split * tiles_per_split, tiles_total);
+            it.ntiles = min(it.tile0 + tiles_per_split, tiles_total) - it.tile0;
+            it.slot = a.num_splits > 1 ? split : -1;
+        }
+        return it;
+    };
+
+    const uint32_t bar_tmem = ptx::smem_u32(&misc->bar_tmem), bar_q_full = ptx::smem_u32(&misc->bar_q_full[0]), bar_q_copied = ptx::smem_u32(&misc->bar_q_copied),
+                   bar_k_land = ptx::smem_u32(&misc->bar_land[0][0]), bar_v_land = ptx::smem_u32(&misc->bar_land[1][0]), bar_q_free = ptx::smem_u32(&misc->bar_q_free),
+                   bar_s_full = ptx::smem_u32(&misc->bar_s_full[0]), bar_o_full = ptx::smem_u32(&misc->bar_o_full[0]), bar_q_ready = ptx::smem_u32(&misc->bar_q_ready),
+                   bar_k_full = ptx::smem_u32(&misc->bar_k_full[0]), bar_v_full = ptx::smem_u32(&misc->bar_v_full[0]), bar_p_full = ptx::smem_u32(&misc->bar_p_full[0]);
+    auto arrive_even = [&](uint32_t bar) {
+        if (rank == 0) ptx::mbar_arrive(bar);
+        else ptx::mbar_arrive_remote(ptx::mapa(bar, 0));
+    };
+
+    // ── set-up ──
+    if (warp == kTreeSendWarp && lane == 0) { ptx::prefetch_tensormap(&a.q_map);  ptx::prefetch_tensormap(&a.k_map);  ptx::prefetch_tensormap(&a.v_map); }
+    if (tid == 0) {
+        ptx::sts_u32(failed_flag(), 0u);
+        ptx::mbar_init(bar_tmem, 1);
+        ptx::mbar_init(bar_q_copied, kTreeQWarps);
+        ptx::mbar_init(bar_q_free, 1);
+        ptx::mbar_init(bar_q_ready, 2 * kTreeQWarps);
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbar_init(bar_q_full + 8 * i, 1);
+            ptx::mbar_init(bar_k_land + 8 * i, 1);
+            ptx::mbar_init(bar_v_land + 8 * i, 1);
+            ptx::mbar_init(bar_s_full + 8 * i, 1);
+            ptx::mbar_init(bar_o_full + 8 * i, 1);
+            ptx::mbar_init(bar_k_full + 8 * i, 2);
+            ptx::mbar_init(bar_v_full + 8 * i, 2);
+            ptx::mbar_init(bar_p_full + 8 * i, 2 * kNumSoftmaxWarps);
+        }
+        ptx::fence_mbar_init();
+    }
+    __syncwarp();
+    ptx::cluster_sync();
+    ptx::pdl_wait();
+    if (sched) {
+        const int pair = blockIdx.x >> 1;
+        item_begin = ptx::ld(a.sched_pair_begin + pair);
+        n_items = ptx::ld(a.sched_pair_begin + pair + 1) - item_begin;
+    }
+    constexpr uint32_t tmem = 0;                  // all 512 columns are allocated (checked)
+    auto wait_tmem = [&]() -> bool {
+        const bool w = ptx::mbar_wait_warp(bar_tmem, 0u, wait_ns);
+        ptx::tc_fence_after_sync();
+        return w;
+    };
+    auto wait_for = [&](uint32_t bar, uint32_t phase, int code, int role, int at) -> bool {
+        const bool w = ptx::mbar_wait_warp(bar, phase & 1u, wait_ns);
+        if (!w) wait_ran_out(a.status, code, role, at);
+        return w;
+    };
+
+    // Running counters, as in decode_kernel.cuh: `g` the tiles over all items, `qn` the items that had tiles.  Tile g is the (g / 2)-th use of K, V, S and P
+    // buffer g % 2.  Every waiter goes through a barrier's phases one by one.
+    if (warp >= kTreeFirstQWarp && warp < kTreeSWarp) {
+        // ───────────── Q warps ─────────────
+        const int qw = warp - kTreeFirstQWarp;
+        bool ok = wait_tmem();
+        if (!ok) wait_ran_out(a.status, kStatusWaitQ, 2, -1);
+        uint32_t qn = 0;
+#pragma unroll 1
+        for (int k = 0; k < n_items && ok; ++k) {
+            if (get_item(k).ntiles <= 0) continue;
+            if (!wait_for(bar_q_full, qn, kStatusWaitQ, 2, k) || (qn > 0u && !wait_for(bar_q_free, qn - 1u, kStatusWaitSFull, 2, k))) break;
+            ptx::tc_fence_after_sync();
+            q_to_tmem<true>(q_stage, tmem + kTmemQ, qw, lane);
+            q_to_tmem<true>(q_stage + 3 * kQChunkBytes, tmem + kTmemQ + 96, qw, lane);
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(bar_q_copied);
+            if (!wait_for(bar_q_full + 8, qn, kStatusWaitQ, 2, k)) break;
+            constexpr int kVecs = L::kQBytes / 16 / (kTreeQWarps * 32);
+#pragma unroll 1
+            for (int i = 0; i < kVecs; ++i) {
+                const uint32_t at = q_base + uint32_t((i * kTreeQWarps + qw) * 32 + lane) * 16u;
+                ptx::sts_v4(at, bf16x8_to_f16x8(ptx::lds_v4(at)));
+            }
+            ptx::tmem_wait_st();
+            ptx::tc_fence_before_sync();
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) arrive_even(bar_q_ready);
+            ++qn;
+        }
+        __syncwarp();
+    } else if (warp == kTreeSendWarp) {
+        // ───────────── Q by TMA: chunks 0-5 of the next item while this one is at work, the others when its S MMAs are done ─────────────
+        uint32_t qn = 0;
+#pragma unroll 1
+        for (int k = 0; k < n_items; ++k) {
+            const Item it = get_item(k);
+            if (it.ntiles <= 0) continue;
+            const int row = it.n * a.H + it.hg * kHeadsPerCta + rank * kHeadsPerBlock;
+            if (qn > 0u && !wait_for(bar_q_copied, qn - 1u, kStatusWaitQ, 5, k)) break;
+            if (ptx::elect_one()) {
+                ptx::mbar_arrive_expect_tx(bar_q_full, L::kStageBytes);
+#pragma unroll
+                for (int c = 0; c < 6; ++c) ptx::tma_load_2d(q_stage + c * kQChunkBytes, &a.q_map, c * 64, row, bar_q_full);
+            }
+            __syncwarp();
+            if (qn > 0u && !wait_for(bar_q_free, qn - 1u, kStatusWaitSFull, 5, k)) break;
+            if (ptx::elect_one()) {
+                ptx::mbar_arrive_expect_tx(bar_q_full + 8, L::kQBytes);
+#pragma unroll
+                for (int c = 0; c < 3; ++c) ptx::tma_load_2d(q_base + c * kQChunkBytes, &a.q_map, (6 + c) * 64, row, bar_q_full + 8);
+            }
+            __syncwarp();
+            ++qn;
+        }
+        __syncwarp();
+    } else if (warp == kTreeLoadWarp) {
+        // ───────────── K and V tiles ─────────────
+        bool ok = true;
+        uint32_t g = 0;
+#pragma unroll 1
+        for (int k = 0; k < n_items && ok; ++k) {
+            const Item it = get_item(k);
+#pragma unroll 1
+            for (int i = 0; i < it.ntiles; ++i, ++g) {
+                const uint32_t buf = g & 1u;
+                const int row = it.n * a.cap + (it.tile0 + i) * kTileN;
+                if (g >= 2u && !wait_for(bar_s_full + 8 * buf, (g - 2u) >> 1, kStatusWaitKvFree, 4, int(g))) { ok = false;  break; }
+                if (ptx::elect_one()) {
+                    ptx::mbar_arrive_expect_tx(bar_k_land + 8 * buf, L::kKBytes);
+#pragma unroll
+                    for (int c = 0; c < 9; ++c)
+                        ptx::tma_load_2d(k_base + buf * L::kKBytes + c * kKChunkBytes, &a.k_map, c * 64, row + rank * kRowsPerBlock, bar_k_land + 8 * buf);
+                }
+                __syncwarp();
+                if (g >= 2u && !wait_for(bar_o_full + 8 * buf, (g - 2u) >> 1, kStatusWaitKvFree, 4, int(g))) { ok = false;  break; }
+                if (ptx::elect_one()) {
+                    ptx::mbar_arrive_expect_tx(bar_v_land + 8 * buf, L::kVBytes);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) ptx::tma_load_2d(v_base + buf * L::kVBytes + c * kVChunkBytes, &a.v_map, rank * 256 + c * 64, row, bar_v_land + 8 * buf);
+                }
+                __syncwarp();
+            }
+        }
+        __syncwarp();
+    } else if (warp == kTreeRelayWarp) {
+        // ───────────── what has landed here is told to the even block ─────────────
+        bool ok = true;
+        uint32_t g = 0;
+#pragma unroll 1
+        for (int k = 0; k < n_items && ok; ++k) {
+            const int ntiles = get_item(k).ntiles;
+#pragma unroll 1
+            for (int i = 0; i < ntiles; ++i, ++g) {
+                const uint32_t buf = g & 1u;
+                if (!wait_for(bar_k_land + 8 * buf, g >> 1, kStatusWaitRaw, 6, int(g))) { ok = false;  break; }
+                if (lane == 0 && !(a.dbg_drop_tile >= 0 && g == uint32_t(a.dbg_drop_tile))) arrive_even(bar_k_full + 8 * buf);
+                if (!wait_for(bar_v_land + 8 * buf, g >> 1, kStatusWaitRaw, 6, int(g))) { ok = false;  break; }
+                if (lane == 0) arrive_even(bar_v_full + 8 * buf);
+            }
+        }
+        __syncwarp();
+    } else if (warp == kTreeSWarp) {
+        // ───────────── tensor-memory allocation, S = Q . K^T ─────────────
+        ptx::tmem2_alloc(ptx::smem_u32(&misc->tmem_base), kTmemCols);
+        ptx::tmem2_relinquish();
+        ptx::tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0 && *reinterpret_cast<volatile uint32_t*>(&misc->tmem_base) == tmem) ptx::mbar_arrive(bar_tmem);
+        bool ok = wait_tmem();
+        if (rank == 0) {
+            constexpr uint32_t kDescHi = ptx::smem_desc_hi(1024), idesc = ptx::make_idesc_f16(128, kTileN, false, false);
+            const uint32_t q_lo = ptx::smem_desc_lo(q_base, 16), k_lo0 = ptx::smem_desc_lo(k_base, 16);
+            uint32_t g = 0, qn = 0;
+#pragma unroll 1
+            for (int k = 0; k < n_items && ok; ++k) {
+                const int ntiles = get_item(k).ntiles;
+                if (ntiles <= 0) continue;
+                if (!wait_for(bar_q_ready, qn, kStatusWaitQ, 1, int(g))) break;
+#pragma unroll 1
+                for (int i = 0; i < ntiles; ++i, ++g) {
+                    const uint32_t buf = g & 1u;
+                    // the S buffer has been read by the softmax of the tile two before
+                    if ((g >= 2u && !wait_for(bar_p_full + 8 * buf, (g - 2u) >> 1, kStatusWaitPFull, 1, int(g))) ||
+                        !wait_for(bar_k_full + 8 * buf, g >> 1, kStatusWaitKvFull, 1, int(g))) { ok = false;  break; }
+                    ptx::tc_fence_after_sync();
+                    const uint32_t d = tmem + kTmemS + buf * 32u, k_lo = k_lo0 + buf * uint32_t(L::kKBytes >> 4);
+                    if (ptx::elect_one()) {
+#pragma unroll
+                        for (int c = 0; c < 9; ++c)
+#pragma unroll
+                            for (int s = 0; s < 4; ++s) {
+                                const uint32_t b_lo = k_lo + uint32_t((c * kKChunkBytes + s * 32) >> 4);
+                                if (c < kQTmemChunks) ptx::mma2_ts(d, tmem + kTmemQ + c * 32 + s * 8, b_lo, kDescHi, idesc, (c | s) ? 1u : 0u);
+                                else ptx::mma2_ss(d, q_lo + uint32_t(((c - kQTmemChunks) * kQChunkBytes + s * 32) >> 4), b_lo, kDescHi, idesc, 1u);
+                            }
+                        ptx::mma2_commit(bar_s_full + 8 * buf);
+                        if (i + 1 == ntiles) ptx::mma2_commit(bar_q_free);
+                    }
+                    __syncwarp();
+                }
+                ++qn;
+            }
+        }
+        __syncwarp();
+    } else if (warp == kTreeOWarp) {
+        // ───────────── O += P . V ─────────────
+        if (rank == 0) {
+            constexpr uint32_t kDescHi = ptx::smem_desc_hi(1024), idesc = ptx::make_idesc_f16(128, 256, false, true);
+            bool ok = wait_tmem();
+            const uint32_t p_lo0 = ptx::smem_desc_lo(p_base, 16), v_lo0 = ptx::smem_desc_lo(v_base, kVChunkBytes);
+            uint32_t g = 0;
+#pragma unroll 1
+            for (int k = 0; k < n_items && ok; ++k) {
+                const Item it = get_item(k);
+#pragma unroll 1
+                for (int i = 0; i < it.ntiles; ++i, ++g) {
+                    const uint32_t buf = g & 1u;
+                    const int ksteps = (it.tile_entries(i) + 15) >> 4;
+                    if (!wait_for(bar_p_full + 8 * buf, g >> 1, kStatusWaitPFull, 3, int(g)) || !wait_for(bar_v_full + 8 * buf, g >> 1, kStatusWaitKvFull, 3, int(g))) {
+                        ok = false;
+                        break;
+                    }
+                    ptx::tc_fence_after_sync();
+                    const uint32_t p_lo = p_lo0 + buf * uint32_t(kQChunkBytes >> 4), v_lo = v_lo0 + buf * uint32_t(L::kVBytes >> 4);
+                    if (ptx::elect_one()) {
+#pragma unroll
+                        for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+                            for (int s = 0; s < 4; ++s)
+                                if (s < ksteps)
+                                    ptx::mma2_ss(tmem + kTmemO + jj * 128, p_lo + uint32_t((s * 32) >> 4), v_lo + uint32_t((2 * jj * kVChunkBytes + s * 16 * 128) >> 4), kDescHi,
+                                                 idesc, (i > 0 || s > 0) ? 1u : 0u);
+                        ptx::mma2_commit(bar_o_full + 8 * buf);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        // ───────────── softmax + epilogue warps: as in decode_kernel.cuh ─────────────
+        // Thread tid owns row tid % 64 of this block and, of its S row, the entries 32 (tid / 64) .. +31 of the tile; of its O row the value columns
+        // [256 (tid / 64), +256).
+        const int r = tid & 63, colhalf = tid >> 6;
+        const uint32_t lane_addr = uint32_t(warp * 32) << 16;
+        const uint32_t pair_bar = 1u + uint32_t(warp & 1);
+        bool ok = wait_tmem();
+        if (!ok) wait_ran_out(a.status, kStatusWaitQ, 0, -1);
+        ok = !ptx::bar_any(pair_bar, 64, !ok);
+        const uint32_t p_row = p_base + uint32_t(r) * 128u;
+        const uint32_t p_sw = (uint32_t(4 * colhalf) ^ uint32_t(r & 7)) << 4;
+        uint32_t gt = 0;
+        Item cur = get_item(0);
+#pragma unroll 1
+        for (int k = 0; k < n_items && ok; ++k) {
+            const int nb = cur.ntiles;
+            const int n = cur.n, h0 = cur.hg * kHeadsPerCta + rank * kHeadsPerBlock, slot = cur.slot;
+            const bool final_out = slot < 0, write = h0 + r < a.H;
+            const int64_t prow0 = final_out ? 0 : (sched ? int64_t(slot) * kHeadsPerCta + rank * kHeadsPerBlock : (int64_t(slot) * a.B + n) * a.H + h0);
+            __nv_bfloat16* const out_rows = final_out ? a.out + (int64_t(n) * a.H + h0) * 512 : reinterpret_cast<__nv_bfloat16*>(a.partial_o) + prow0 * 512;
+            if (nb <= 0) {
+#pragma unroll 1
+                for (int i = tid; i < kHeadsPerBlock * 64; i += kNumSoftmaxWarps * 32)
+                    if (h0 + (i >> 6) < a.H) *reinterpret_cast<uint4*>(out_rows + int64_t(i >> 6) * 512 + (i & 63) * 8) = make_uint4(0, 0, 0, 0);
+                if (colhalf == 0 && write) {
+                    if (!final_out) a.partial_lse[prow0 + r] = -CUDART_INF_F;
+                    else if (a.lse != nullptr) a.lse[int64_t(n) * a.H + h0 + r] = -CUDART_INF_F;
+                }
+                if (k + 1 < n_items) cur = get_item(k + 1);
+                continue;
+            }
+            // (rows past the last node are computed but not written)
+            const int32_t* const node_mask = a.tree_mask + (int64_t(n) * (a.H / a.heads) + min(h0 + r, a.H - 1) / a.heads) * a.mask_words;
+            auto sees = [&](int i) -> uint32_t {
+                const int v0 = (cur.tile0 + i) * kTileN + 32 * colhalf;
+                return v0 >= cur.n_tok ? 0u : uint32_t(ptx::ld(reinterpret_cast<const int32_t*>(a.valid) + (int64_t(n) * a.cap + v0) / 32)) &
+                       window_bits(node_mask, a.mask_words, v0 - cur.kv_len_n);
+            };
+            uint32_t next_seen = sees(0);
+            float m_ref = -CUDART_INF_F, l_sum = 0.f;
+            bool left = false;
+#pragma unroll 1
+            for (int it = 0; it < nb; ++it) {
+                const uint32_t g = gt + uint32_t(it), vmask = next_seen;
+                if (it + 1 < nb) next_seen = sees(it + 1);
+                const uint32_t s_tmem = tmem + lane_addr + kTmemS + (g & 1u) * 32u;
+                if (ok) ok = wait_for(bar_s_full + 8 * (g & 1u), g >> 1, kStatusWaitSFull, 0, int(g));
+                ptx::tc_fence_after_sync();
+                uint32_t s0[32];
+                ptx::tmem_ld32(s_tmem, s0);
+                ptx::tmem_wait_ld();
+                if (vmask != ~0u) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (!((vmask >> i) & 1u)) s0[i] = 0xFF800000u;
+                }
+                float t4[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) t4[i] = fmaxf(__uint_as_float(s0[i]), __uint_as_float(s0[i + 4]));
+#pragma unroll
+                for (int i = 8; i < 32; i += 8)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) t4[j] = ptx::max3(t4[j], __uint_as_float(s0[i + 2 * j]), __uint_as_float(s0[i + 2 * j + 1]));
+                const float tmax = ptx::max3(ptx::max3(t4[0], t4[1], t4[2]), t4[3], -CUDART_INF_F) * a.scale_log2;
+                float alpha = 1.f;
+                const bool moved = ptx::bar_any(pair_bar, 64, !ok || tmax > m_ref + kRescaleThreshold);
+                if (moved) {
+                    misc->exch[tid] = tmax;
+                    if (ptx::bar_any(pair_bar + 2u, 64, !ok)) { ok = false;  left = true;  break; }
+                    const float rmax = fmaxf(tmax, misc->exch[tid ^ 64]);
+                    if (rmax > m_ref + kRescaleThreshold) {
+                        alpha = (m_ref == -CUDART_INF_F) ? 0.f : ptx::ex2(m_ref - rmax);
+                        m_ref = rmax;
+                    }
+                }
+                const float neg_m = (m_ref == -CUDART_INF_F) ? 0.f : -m_ref;
+                const uint64_t scale2 = ptx::pack_f32x2(a.scale_log2, a.scale_log2), neg2 = ptx::pack_f32x2(neg_m, neg_m);
+                uint64_t ps2[2] = {0ull, 0ull};
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float e0, e1;
+                    ptx::unpack_f32x2(ptx::fma_f32x2(ptx::pack_f32x2(__uint_as_float(s0[2 * i]), __uint_as_float(s0[2 * i + 1])), scale2, neg2), e0, e1);
+                    const float p0 = ptx::ex2(e0), p1 = ptx::ex2(e1);
+                    ps2[i & 1] = ptx::add_f32x2(ps2[i & 1], ptx::pack_f32x2(p0, p1));
+                    s0[i] = ptx::pack_f16x2(p0, p1);
+                }
+                float ps_lo, ps_hi;
+                ptx::unpack_f32x2(ptx::add_f32x2(ps2[0], ps2[1]), ps_lo, ps_hi);
+                l_sum = l_sum * alpha + (ps_lo + ps_hi);
+                // the P buffer has been read by the O MMAs of the tile two before
+                if (g >= 2u && !(ok = wait_for(bar_o_full + 8 * (g & 1u), (g - 2u) >> 1, kStatusWaitOFull, 0, int(g)))) continue;      // leaves at the next barrier
+                if (it > 0 && moved && __any_sync(0xFFFFFFFFu, alpha != 1.f)) {
+                    if (!(ok = wait_for(bar_o_full + 8 * ((g - 1u) & 1u), (g - 1u) >> 1, kStatusWaitOFull, 0, int(g)))) continue;
+                    ptx::tc_fence_after_sync();
+#pragma unroll 1
+                    for (int c = 0; c < 8; ++c) {
+                        uint32_t o[32];
+                        ptx::tmem_ld32(tmem + lane_addr + kTmemO + c * 32, o);
+                        ptx::tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                        ptx::tmem_st32(tmem + lane_addr + kTmemO + c * 32, o);
+                    }
+                    ptx::tmem_wait_st();
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    ptx::sts_v4(p_row + (g & 1u) * kQChunkBytes + (p_sw ^ (uint32_t(c) << 4)), make_uint4(s0[4 * c], s0[4 * c + 1], s0[4 * c + 2], s0[4 * c + 3]));
+                ptx::fence_proxy_async_smem();
+                ptx::tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) arrive_even(bar_p_full + 8 * (g & 1u));
+            }
+            if (left) break;
+            // ── epilogue ──
+            gt += uint32_t(nb);
+            if (k + 1 < n_items) cur = get_item(k + 1);
+            if (ok) ok = wait_for(bar_o_full + 8 * ((gt - 1u) & 1u), (gt - 1u) >> 1, kStatusWaitOFull, 0, int(gt));
+            if (ptx::bar_any(pair_bar, 64, !ok)) { ok = false;  break; }
+            misc->exch[tid] = l_sum;
+            ptx::bar_sync(pair_bar + 2u, 64);
+            l_sum += misc->exch[tid ^ 64];
+            ptx::tc_fence_after_sync();
+            if (tid == 0 && k == n_items - 1 && (sched || a.num_splits > 1)) ptx::pdl_trigger();      // (a merge follows)
+            float denom = l_sum;
+            if (final_out && a.attn_sink != nullptr && write) {
+                const float s2 = ptx::ld(a.attn_sink + (h0 + r) % a.heads) * 1.4426950408889634f;
+                denom = (l_sum != 0.f) ? l_sum + ptx::ex2(s2 - m_ref) : 1.f;
+            }
+            const float inv = (l_sum != 0.f) ? 1.f / denom : 0.f;
+            const int row0 = (warp & 1) * 32;
+            uint8_t* gbase = reinterpret_cast<uint8_t*>(out_rows + int64_t(row0) * 512 + colhalf * 256);
+#pragma unroll 1
+            for (int pass = 0; pass < 4; ++pass) {
+#pragma unroll
+                for (int hc = 0; hc < 2; ++hc) {
+                    uint32_t o[32];
+                    ptx::tmem_ld32(tmem + lane_addr + kTmemO + pass * 64 + hc * 32, o);
+                    ptx::tmem_wait_ld();
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float x = __uint_as_float(o[8 * v + 2 * i]) * inv, y = __uint_as_float(o[8 * v + 2 * i + 1]) * inv;
+                            w[i] = final_out ? ptx::pack_bf16x2(x, y) : ptx::pack_f16x2(x, y);
+                        }
+                        ptx::sts_v4(p_row + uint32_t(hc) * kQChunkBytes + (p_sw ^ (uint32_t(v) << 4)), make_uint4(w[0], w[1], w[2], w[3]));
+                    }
+                }
+                __syncwarp();
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const uint32_t rl = uint32_t(q * 4 + (lane >> 3)), vc = uint32_t(lane & 7);
+                    const uint32_t at = p_base + (vc >> 2) * kQChunkBytes + uint32_t(row0 + rl) * 128u + (((4u * colhalf + (vc & 3u)) ^ (rl & 7u)) << 4);
+                    if (h0 + row0 + int(rl) < a.H)
+                        *reinterpret_cast<uint4*>(gbase + int64_t(rl) * 1024 + pass * 128 + vc * 16u) = ptx::lds_v4(at);
+                }
+                __syncwarp();
+            }
+            if (write && colhalf == 0) {
+                const float lse2 = (l_sum != 0.f) ? m_ref + log2f(l_sum) : -CUDART_INF_F;
+                if (!final_out) a.partial_lse[prow0 + r] = lse2;
+                else if (a.lse != nullptr) a.lse[int64_t(n) * a.H + h0 + r] = (l_sum != 0.f) ? lse2 * 0.6931471805599453f : -CUDART_INF_F;
+            }
+        }
+    }
+
+    // ── common exit ──
+    __syncwarp();
+    ptx::tc_fence_before_sync();
+    ptx::cluster_sync();
+    if (warp == kTreeSWarp) {
+        ptx::tc_fence_after_sync();
+        if (ptx::lds_u32(failed_flag())) hold_block();
+        ptx::tmem2_dealloc(misc->tmem_base, kTmemCols);
+    }
+}
+
+}  // namespace dsv4

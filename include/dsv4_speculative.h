@@ -58,7 +58,12 @@ typedef struct Dsv4HcaTreeDecodeParams {
     int32_t*       status;
     void*          sched;
     int64_t        sched_bytes; /* read with make_plan */
+    void*          rows;        /* optional workspace of dsv4_hca_tree_rows_bytes(): the entries are dequantised into it once, and all of a
+                                   request's nodes read them there; without it every group of 128 (node, head) rows dequantises them for itself */
+    int64_t        rows_bytes;
 } Dsv4HcaTreeDecodeParams;
+
+int64_t dsv4_hca_tree_rows_bytes(int B, int max_pages, int win_cap);
 
 int dsv4_hca_tree_decode_fwd(const Dsv4HcaTreeDecodeParams* p, void* stream);
 

@@ -95,38 +95,43 @@ CASES = [
 
 
 @pytest.mark.parametrize("case", range(len(CASES)))
-@pytest.mark.parametrize("route", ["auto", "one", "three", "plan"])
+@pytest.mark.parametrize("route", ["auto", "one", "three", "plan", "rows", "rows_three", "rows_plan"])
 def test_against_the_formula(lib, case, route):
     B, T, H, kv_len, W, win_len = CASES[case]
     c = make(100 + case, B, T, H, kv_len, W, win_len)
     sink = torch.randn(H, device="cuda") if case % 2 else None
-    kw = dict(auto={}, one=dict(num_splits=1), three=dict(num_splits=3), plan={})[route]
-    if route == "plan":
-        kw = dict(plan=lib.plan_hca(B, 1, T * H, c["kv_len"][:, None].contiguous(), c["win_len"][:, None].contiguous()))
+    kw = dict(auto={}, one=dict(num_splits=1), three=dict(num_splits=3), plan={}, rows=dict(num_splits=1), rows_three=dict(num_splits=3), rows_plan={})[route]
+    if route != "auto":
+        kw["share_rows"] = route.startswith("rows")
+    if route.endswith("plan"):
+        kw |= dict(plan=lib.plan_hca(B, 1, T * H, c["kv_len"][:, None].contiguous(), c["win_len"][:, None].contiguous()))
     check(call(lib, c, SCALE, attn_sink=sink, **kw), want(c, SCALE, sink))
 
 
+@pytest.mark.parametrize("rows", [False, True])
 @pytest.mark.parametrize("H", [8, 100, 128])
-def test_nodes_that_see_nothing(lib, H):
+def test_nodes_that_see_nothing(lib, H, rows):
     """No cache, and masks that leave every second node empty: 0 and -inf there, also next to nodes that see something."""
     c = make(7, 2, 6, H, [0, 0], 70)
     c["sees"][:, ::2] = False
-    got = call(lib, c, SCALE)
+    got = call(lib, c, SCALE, share_rows=rows)
     check(got, want(c, SCALE))
     assert torch.isneginf(got[1][:, ::2]).all() and torch.isfinite(got[1][:, 1::2]).all()
 
 
-def test_mask_shorter_and_longer_than_the_window(lib):
+@pytest.mark.parametrize("rows", [False, True])
+def test_mask_shorter_and_longer_than_the_window(lib, rows):
     from dsv4_attn_b200 import layout
     c = make(8, 2, 4, 64, [100, 3], 96)
     short = layout.pack_tree_mask(c["sees"])[..., :2].contiguous()
     c["sees"][..., 64:] = False                  # rows beyond the mask's words are seen by no node
-    check(call(lib, c, SCALE, mask=short), want(c, SCALE))
+    check(call(lib, c, SCALE, mask=short, share_rows=rows), want(c, SCALE))
     longer = torch.nn.functional.pad(layout.pack_tree_mask(c["sees"]), (0, 2), value=-1)
-    check(call(lib, c, SCALE, mask=longer), want(c, SCALE))
+    check(call(lib, c, SCALE, mask=longer, share_rows=rows), want(c, SCALE))
 
 
-def test_what_masked_rows_hold_does_not_matter(lib):
+@pytest.mark.parametrize("rows", [False, True])
+def test_what_masked_rows_hold_does_not_matter(lib, rows):
     """Rows that no node sees hold NaN and infinities in every field; a row that some nodes see has a NaN RoPE tail: only they are NaN."""
     c = make(9, 2, 4, 32, [70, 0], 80)
     c["sees"][:, :, 10] = False
@@ -134,11 +139,11 @@ def test_what_masked_rows_hold_does_not_matter(lib):
     c["win_pool"][:, 10] = 0xFF
     c["win_pool"][:, 79, :528] = 0x7F
     exp = want({**c, "win_pool": torch.where(torch.arange(80, device="cuda")[None, :, None] % 69 == 10, torch.zeros_like(c["win_pool"]), c["win_pool"])}, SCALE)
-    check(call(lib, c, SCALE), exp)
+    check(call(lib, c, SCALE, share_rows=rows), exp)
     c["sees"][:, :, 20] = False
     c["sees"][:, 1, 20] = True
     c["win_pool"][:, 20, 528:] = 0xFF
-    out, lse = call(lib, c, SCALE)
+    out, lse = call(lib, c, SCALE, share_rows=rows)
     c["win_pool"][:, 10] = c["win_pool"][:, 79] = c["win_pool"][:, 20] = 0
     o, l = want(c, SCALE)
     nan = torch.zeros_like(l, dtype=torch.bool)
@@ -163,7 +168,8 @@ def test_tree_sees():
     assert got == [[0, 1, 1, 1, 0, 0, 0], [0, 0, 1, 1, 1, 0, 0], [0, 0, 1, 1, 0, 1, 0], [0, 0, 0, 1, 0, 1, 1]]
 
 
-def test_entries_out_of_range_are_reported(lib):
+@pytest.mark.parametrize("rows", [False, True])
+def test_entries_out_of_range_are_reported(lib, rows):
     from dsv4_attn_b200 import layout
     c = make(11, 1, 2, 16, [100], 40)
     c["sees"][:] = True
@@ -173,7 +179,7 @@ def test_entries_out_of_range_are_reported(lib):
         d = {**c, **change}
         st = lib.new_status("cuda")
         longer = torch.nn.functional.pad(mask, (0, 1), value=-1)
-        lib.hca_tree_decode(d["q"], d["kv_pool"], d["block_table"], d["kv_len"], d["win_pool"], d["win_len"], longer, SCALE, status=st)
+        lib.hca_tree_decode(d["q"], d["kv_pool"], d["block_table"], d["kv_len"], d["win_pool"], d["win_len"], longer, SCALE, status=st, share_rows=rows)
         torch.cuda.synchronize()
         assert st[0].item() == 7, change
 
@@ -200,6 +206,23 @@ def test_graph_replay_and_another_stream(lib):
         assert torch.equal(r[0], base[0]) and torch.equal(r[1], base[1])
 
 
+def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_unaffected(lib):
+    """The hand-over of a tile is withheld in every pair: the kernel returns with a status, and the next launch is right."""
+    from dsv4_attn_b200 import layout
+    c = make(14, 2, 8, 128, [300, 100], 40)
+    args = (c["q"], c["kv_pool"], c["block_table"], c["kv_len"], c["win_pool"], c["win_len"], layout.pack_tree_mask(c["sees"]), SCALE)
+    for rows in (False, True):
+        st = lib.new_status("cuda")
+        lib.LIB.dsv4_debug_set_wait(20_000_000, 1)
+        try:
+            lib.hca_tree_decode(*args, status=st, share_rows=rows)
+            torch.cuda.synchronize()
+        finally:
+            lib.LIB.dsv4_debug_set_wait(0, -1)
+        assert st[0].item() in (1, 2, 3, 4, 5, 6, 9)
+        check(call(lib, c, SCALE, share_rows=rows), want(c, SCALE))
+
+
 def test_refusals(lib):
     from dsv4_attn_b200 import layout
     c = make(13, 2, 3, 16, [64, 10], 40)
@@ -209,7 +232,7 @@ def test_refusals(lib):
     for bad in (dict(q=c["q"].float()), dict(q=c["q"][..., :512].contiguous()), dict(q=c["q"].transpose(1, 2)), dict(kv_len=c["kv_len"].long()), dict(kv_len=c["kv_len"][:1]),
                 dict(win_len=c["win_len"][:, None].contiguous()), dict(win_pool=c["win_pool"][:1]), dict(tree_mask=mask[:, :2].contiguous()), dict(tree_mask=mask.long()),
                 dict(attn_sink=torch.zeros(4, device="cuda")), dict(num_splits=0), dict(num_splits=65), dict(out=torch.empty(2, 3, 16, 576, device="cuda", dtype=torch.bfloat16)),
-                dict(lse=torch.empty(2, 3, device="cuda")), dict(block_table=c["block_table"].cpu()),
+                dict(lse=torch.empty(2, 3, device="cuda")), dict(share_rows=torch.empty(100, device="cuda", dtype=torch.uint8)), dict(share_rows=3), dict(block_table=c["block_table"].cpu()),
                 dict(plan=lib.plan_hca(2, 3, 16, torch.zeros(2, 3, device="cuda", dtype=torch.int32), torch.zeros(2, 3, device="cuda", dtype=torch.int32)))):
         with pytest.raises(ValueError):
             lib.hca_tree_decode(**{**good, **bad})
