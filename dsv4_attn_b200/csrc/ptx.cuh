@@ -341,6 +341,15 @@ __device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const void* tenso
         : "memory");
 }
 
+// The same in a cluster pair, reporting to a barrier that may be the other block's (`cbar`: its address in the cluster).
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t smem_dst, const void* tensor_map, int x, int y, uint32_t cbar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+        :
+        : "r"(smem_dst), "l"(reinterpret_cast<uint64_t>(tensor_map)), "r"(x), "r"(y), "r"(cbar)
+        : "memory");
+}
+
 __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const void* tensor_map, int x, int y, int z, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"

@@ -118,9 +118,8 @@ constexpr int kTreeFirstQWarp = 4;
 constexpr int kTreeSWarp = 12;                 // tensor-memory allocation; (even block) issue of the S MMAs
 constexpr int kTreeOWarp = 13;                 // (even block) issue of the O MMAs
 constexpr int kTreeLoadWarp = 14;              // K and V tiles
-constexpr int kTreeRelayWarp = 15;             // tells the even block that a tile has landed here
-constexpr int kTreeSendWarp = 16;              // Q
-constexpr int kTreeThreads = 17 * 32;
+constexpr int kTreeSendWarp = 15;              // Q
+constexpr int kTreeThreads = 16 * 32;
 
 struct TreeArgs {
     alignas(64) CUtensorMap q_map;             // BF16 [B * H, 576], box 64 x 64
@@ -168,14 +167,14 @@ struct TreeMisc {
     uint64_t bar_tmem;
     uint64_t bar_q_full[2];          // per item: chunks 0-5 / 6-8 landed
     uint64_t bar_q_copied;           // per item: chunks 0-5 copied out by every Q warp
-    uint64_t bar_land[2][2];         // K / V tile landed in this block, by buffer
     // signalled in both blocks by the commits of the MMA warps
     uint64_t bar_q_free;             // per item: its S MMAs complete
     uint64_t bar_s_full[2];          // S of a tile complete: S buffer full, K buffer free
     uint64_t bar_o_full[2];          // P.V of a tile complete: V and P buffer free, O up to date
     // in the even block only, signalled by the warps of both
     uint64_t bar_q_ready;
-    uint64_t bar_k_full[2], bar_v_full[2], bar_p_full[2];
+    uint64_t bar_k_full[2], bar_v_full[2];                // both blocks' halves of a tile landed (TMA transaction count, by the copies themselves)
+    uint64_t bar_p_full[2];
     uint32_t tmem_base;
 };
 static_assert(sizeof(TreeMisc) <= 3072 - 16, "the last word of the block's shared memory is failed_flag()");
@@ -231,7 +230,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
     };
 
     const uint32_t bar_tmem = ptx::smem_u32(&misc->bar_tmem), bar_q_full = ptx::smem_u32(&misc->bar_q_full[0]), bar_q_copied = ptx::smem_u32(&misc->bar_q_copied),
-                   bar_k_land = ptx::smem_u32(&misc->bar_land[0][0]), bar_v_land = ptx::smem_u32(&misc->bar_land[1][0]), bar_q_free = ptx::smem_u32(&misc->bar_q_free),
+                   bar_q_free = ptx::smem_u32(&misc->bar_q_free),
                    bar_s_full = ptx::smem_u32(&misc->bar_s_full[0]), bar_o_full = ptx::smem_u32(&misc->bar_o_full[0]), bar_q_ready = ptx::smem_u32(&misc->bar_q_ready),
                    bar_k_full = ptx::smem_u32(&misc->bar_k_full[0]), bar_v_full = ptx::smem_u32(&misc->bar_v_full[0]), bar_p_full = ptx::smem_u32(&misc->bar_p_full[0]);
     auto arrive_even = [&](uint32_t bar) {
@@ -249,12 +248,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
         ptx::mbar_init(bar_q_ready, 2 * kTreeQWarps);
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(bar_q_full + 8 * i, 1);
-            ptx::mbar_init(bar_k_land + 8 * i, 1);
-            ptx::mbar_init(bar_v_land + 8 * i, 1);
             ptx::mbar_init(bar_s_full + 8 * i, 1);
             ptx::mbar_init(bar_o_full + 8 * i, 1);
-            ptx::mbar_init(bar_k_full + 8 * i, 2);
-            ptx::mbar_init(bar_v_full + 8 * i, 2);
+            ptx::mbar_init(bar_k_full + 8 * i, 1);
+            ptx::mbar_init(bar_v_full + 8 * i, 1);
             ptx::mbar_init(bar_p_full + 8 * i, 2 * kNumSoftmaxWarps);
         }
         ptx::fence_mbar_init();
@@ -337,7 +334,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
         }
         __syncwarp();
     } else if (warp == kTreeLoadWarp) {
-        // ───────────── K and V tiles ─────────────
+        // ───────────── K and V tiles: both blocks' copies report to the even one, which expects the bytes of both ─────────────
+        const uint32_t k_full = ptx::mapa(bar_k_full, 0), v_full = ptx::mapa(bar_v_full, 0);
         bool ok = true;
         uint32_t g = 0;
 #pragma unroll 1
@@ -349,36 +347,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
                 const int row = it.n * a.cap + (it.tile0 + i) * kTileN;
                 if (g >= 2u && !wait_for(bar_s_full + 8 * buf, (g - 2u) >> 1, kStatusWaitKvFree, 4, int(g))) { ok = false;  break; }
                 if (ptx::elect_one()) {
-                    ptx::mbar_arrive_expect_tx(bar_k_land + 8 * buf, L::kKBytes);
+                    if (rank == 0 && !(a.dbg_drop_tile >= 0 && g == uint32_t(a.dbg_drop_tile))) ptx::mbar_arrive_expect_tx(bar_k_full + 8 * buf, 2 * L::kKBytes);
 #pragma unroll
                     for (int c = 0; c < 9; ++c)
-                        ptx::tma_load_2d(k_base + buf * L::kKBytes + c * kKChunkBytes, &a.k_map, c * 64, row + rank * kRowsPerBlock, bar_k_land + 8 * buf);
+                        ptx::tma_load_2d_pair(k_base + buf * L::kKBytes + c * kKChunkBytes, &a.k_map, c * 64, row + rank * kRowsPerBlock, k_full + 8 * buf);
                 }
                 __syncwarp();
                 if (g >= 2u && !wait_for(bar_o_full + 8 * buf, (g - 2u) >> 1, kStatusWaitKvFree, 4, int(g))) { ok = false;  break; }
                 if (ptx::elect_one()) {
-                    ptx::mbar_arrive_expect_tx(bar_v_land + 8 * buf, L::kVBytes);
+                    if (rank == 0) ptx::mbar_arrive_expect_tx(bar_v_full + 8 * buf, 2 * L::kVBytes);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) ptx::tma_load_2d(v_base + buf * L::kVBytes + c * kVChunkBytes, &a.v_map, rank * 256 + c * 64, row, bar_v_land + 8 * buf);
+                    for (int c = 0; c < 4; ++c) ptx::tma_load_2d_pair(v_base + buf * L::kVBytes + c * kVChunkBytes, &a.v_map, rank * 256 + c * 64, row, v_full + 8 * buf);
                 }
                 __syncwarp();
-            }
-        }
-        __syncwarp();
-    } else if (warp == kTreeRelayWarp) {
-        // ───────────── what has landed here is told to the even block ─────────────
-        bool ok = true;
-        uint32_t g = 0;
-#pragma unroll 1
-        for (int k = 0; k < n_items && ok; ++k) {
-            const int ntiles = get_item(k).ntiles;
-#pragma unroll 1
-            for (int i = 0; i < ntiles; ++i, ++g) {
-                const uint32_t buf = g & 1u;
-                if (!wait_for(bar_k_land + 8 * buf, g >> 1, kStatusWaitRaw, 6, int(g))) { ok = false;  break; }
-                if (lane == 0 && !(a.dbg_drop_tile >= 0 && g == uint32_t(a.dbg_drop_tile))) arrive_even(bar_k_full + 8 * buf);
-                if (!wait_for(bar_v_land + 8 * buf, g >> 1, kStatusWaitRaw, 6, int(g))) { ok = false;  break; }
-                if (lane == 0) arrive_even(bar_v_full + 8 * buf);
             }
         }
         __syncwarp();
