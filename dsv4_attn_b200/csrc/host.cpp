@@ -477,11 +477,13 @@ PyObject* combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return rc != 0 ? code(rc) : pair(out, lse);
 }
 
-// Where the library plans the work of a tree decode in the call: more row groups than the device has pairs of SMs (74).  Below that one wave of pairs is
-// enough, with rows split so that it is full.
-constexpr int64_t kTreePlanGroups = 74;
-// Where the groups of a request share its dequantised entries: from this many groups on, for workspaces of up to this size.
-constexpr int64_t kTreeShareGroups = 4, kTreeShareBytes = int64_t(4) << 30;
+// Where the library plans the work of a tree decode in the call: more than four row groups for every pair of SMs (74).  A plan overlaps the set-up of
+// one group with the end of another's and costs 6 us and a merge: 1,024 groups of 15 tiles 301 us against 331 on a static grid, 256 groups 119 either way, 128 groups 58
+// against 53, 92 ragged ones 90 against 81.
+constexpr int64_t kTreePlanGroups = 4 * 74;
+// Where the groups of a request share its dequantised entries: from four groups a request and 900 tiles over all groups on (960 tiles in 64 groups: 32 us against
+// 34, 480 in 32 groups 28 against 27; three groups a request 158 against 149), for workspaces of up to 4 GB.
+constexpr int64_t kTreeShareGroups = 4, kTreeShareTiles = 900, kTreeShareBytes = int64_t(4) << 30;
 
 // (q, kv_pool, block_table, kv_len, win_pool, win_len, tree_mask, sm_scale, attn_sink, num_splits, out, lse, workspace, status, max_len, plan, share_rows)
 PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -543,7 +545,7 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
     at::Tensor own_rows;
     const at::Tensor* shared = nullptr;
     const int64_t rows_bytes = lib.tree_rows_bytes(int(B), int(table->size(1)), int(W));
-    if (a[16] == Py_True || (a[16] == Py_None && groups >= kTreeShareGroups * B && rows_bytes > 0 && rows_bytes <= kTreeShareBytes)) {
+    if (a[16] == Py_True || (a[16] == Py_None && groups >= kTreeShareGroups * B && groups * ((max_len + 63) / 64) >= kTreeShareTiles && rows_bytes > 0 && rows_bytes <= kTreeShareBytes)) {
         if (rows_bytes <= 0) return none();
         own_rows = empty({rows_bytes}, at::kByte, q);
         shared = &own_rows;

@@ -117,8 +117,8 @@ constexpr int kTreeQWarps = 8;                 // warps 4-11: Q into tensor memo
 constexpr int kTreeFirstQWarp = 4;
 constexpr int kTreeSWarp = 12;                 // tensor-memory allocation; (even block) issue of the S MMAs
 constexpr int kTreeOWarp = 13;                 // (even block) issue of the O MMAs
-constexpr int kTreeLoadWarp = 14;              // K and V tiles
-constexpr int kTreeSendWarp = 15;              // Q
+constexpr int kTreeKWarp = 14;                 // K tiles
+constexpr int kTreeVWarp = 15;                 // V tiles, and Q (with K and V in one warp, K waited behind V: 1650 cycles a tile)
 constexpr int kTreeThreads = 16 * 32;
 
 struct TreeArgs {
@@ -239,7 +239,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
     };
 
     // ── set-up ──
-    if (warp == kTreeSendWarp && lane == 0) { ptx::prefetch_tensormap(&a.q_map);  ptx::prefetch_tensormap(&a.k_map);  ptx::prefetch_tensormap(&a.v_map); }
+    if (warp == kTreeVWarp && lane == 0) { ptx::prefetch_tensormap(&a.q_map);  ptx::prefetch_tensormap(&a.k_map);  ptx::prefetch_tensormap(&a.v_map); }
     if (tid == 0) {
         ptx::sts_u32(failed_flag(), 0u);
         ptx::mbar_init(bar_tmem, 1);
@@ -308,34 +308,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
             ++qn;
         }
         __syncwarp();
-    } else if (warp == kTreeSendWarp) {
-        // ───────────── Q by TMA: chunks 0-5 of the next item while this one is at work, the others when its S MMAs are done ─────────────
-        uint32_t qn = 0;
-#pragma unroll 1
-        for (int k = 0; k < n_items; ++k) {
-            const Item it = get_item(k);
-            if (it.ntiles <= 0) continue;
-            const int row = it.n * a.H + it.hg * kHeadsPerCta + rank * kHeadsPerBlock;
-            if (qn > 0u && !wait_for(bar_q_copied, qn - 1u, kStatusWaitQ, 5, k)) break;
-            if (ptx::elect_one()) {
-                ptx::mbar_arrive_expect_tx(bar_q_full, L::kStageBytes);
-#pragma unroll
-                for (int c = 0; c < 6; ++c) ptx::tma_load_2d(q_stage + c * kQChunkBytes, &a.q_map, c * 64, row, bar_q_full);
-            }
-            __syncwarp();
-            if (qn > 0u && !wait_for(bar_q_free, qn - 1u, kStatusWaitSFull, 5, k)) break;
-            if (ptx::elect_one()) {
-                ptx::mbar_arrive_expect_tx(bar_q_full + 8, L::kQBytes);
-#pragma unroll
-                for (int c = 0; c < 3; ++c) ptx::tma_load_2d(q_base + c * kQChunkBytes, &a.q_map, (6 + c) * 64, row, bar_q_full + 8);
-            }
-            __syncwarp();
-            ++qn;
-        }
-        __syncwarp();
-    } else if (warp == kTreeLoadWarp) {
-        // ───────────── K and V tiles: both blocks' copies report to the even one, which expects the bytes of both ─────────────
-        const uint32_t k_full = ptx::mapa(bar_k_full, 0), v_full = ptx::mapa(bar_v_full, 0);
+    } else if (warp == kTreeKWarp) {
+        // ───────────── K tiles: both blocks' copies report to the even one, which expects the bytes of both ─────────────
+        const uint32_t k_full = ptx::mapa(bar_k_full, 0);
         bool ok = true;
         uint32_t g = 0;
 #pragma unroll 1
@@ -344,15 +319,58 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
 #pragma unroll 1
             for (int i = 0; i < it.ntiles; ++i, ++g) {
                 const uint32_t buf = g & 1u;
-                const int row = it.n * a.cap + (it.tile0 + i) * kTileN;
+                const int row = it.n * a.cap + (it.tile0 + i) * kTileN + rank * kRowsPerBlock;
                 if (g >= 2u && !wait_for(bar_s_full + 8 * buf, (g - 2u) >> 1, kStatusWaitKvFree, 4, int(g))) { ok = false;  break; }
                 if (ptx::elect_one()) {
                     if (rank == 0 && !(a.dbg_drop_tile >= 0 && g == uint32_t(a.dbg_drop_tile))) ptx::mbar_arrive_expect_tx(bar_k_full + 8 * buf, 2 * L::kKBytes);
 #pragma unroll
-                    for (int c = 0; c < 9; ++c)
-                        ptx::tma_load_2d_pair(k_base + buf * L::kKBytes + c * kKChunkBytes, &a.k_map, c * 64, row + rank * kRowsPerBlock, k_full + 8 * buf);
+                    for (int c = 0; c < 9; ++c) ptx::tma_load_2d_pair(k_base + buf * L::kKBytes + c * kKChunkBytes, &a.k_map, c * 64, row, k_full + 8 * buf);
                 }
                 __syncwarp();
+            }
+        }
+        __syncwarp();
+    } else if (warp == kTreeVWarp) {
+        // ───────────── V tiles; Q: chunks 0-5 of the next item while this one is at work, the others when its S MMAs are done ─────────────
+        const uint32_t v_full = ptx::mapa(bar_v_full, 0);
+        bool ok = true;
+        uint32_t g = 0, qn = 0;
+        auto send_stage = [&](const Item& it) {
+            if (ptx::elect_one()) {
+                const int row = it.n * a.H + it.hg * kHeadsPerCta + rank * kHeadsPerBlock;
+                ptx::mbar_arrive_expect_tx(bar_q_full, L::kStageBytes);
+#pragma unroll
+                for (int c = 0; c < 6; ++c) ptx::tma_load_2d(q_stage + c * kQChunkBytes, &a.q_map, c * 64, row, bar_q_full);
+            }
+            __syncwarp();
+        };
+        auto next_item = [&](int& k) -> Item {         // the next one with tiles
+            Item it{};
+            while (++k < n_items) {
+                it = get_item(k);
+                if (it.ntiles > 0) break;
+            }
+            return it;
+        };
+        int k = -1;
+        Item it = next_item(k);
+        if (k < n_items) send_stage(it);
+#pragma unroll 1
+        while (k < n_items && ok) {
+            if (qn > 0u && !wait_for(bar_q_free, qn - 1u, kStatusWaitSFull, 5, k)) break;
+            if (ptx::elect_one()) {
+                const int row = it.n * a.H + it.hg * kHeadsPerCta + rank * kHeadsPerBlock;
+                ptx::mbar_arrive_expect_tx(bar_q_full + 8, L::kQBytes);
+#pragma unroll
+                for (int c = 0; c < 3; ++c) ptx::tma_load_2d(q_base + c * kQChunkBytes, &a.q_map, (6 + c) * 64, row, bar_q_full + 8);
+            }
+            __syncwarp();
+            int k2 = k;
+            const Item next = next_item(k2);
+#pragma unroll 1
+            for (int i = 0; i < it.ntiles; ++i, ++g) {
+                const uint32_t buf = g & 1u;
+                const int row = it.n * a.cap + (it.tile0 + i) * kTileN;
                 if (g >= 2u && !wait_for(bar_o_full + 8 * buf, (g - 2u) >> 1, kStatusWaitKvFree, 4, int(g))) { ok = false;  break; }
                 if (ptx::elect_one()) {
                     if (rank == 0) ptx::mbar_arrive_expect_tx(bar_v_full + 8 * buf, 2 * L::kVBytes);
@@ -360,7 +378,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
                     for (int c = 0; c < 4; ++c) ptx::tma_load_2d_pair(v_base + buf * L::kVBytes + c * kVChunkBytes, &a.v_map, rank * 256 + c * 64, row, v_full + 8 * buf);
                 }
                 __syncwarp();
+                if (i == min(it.ntiles - 1, 2) && k2 < n_items) {
+                    if (!wait_for(bar_q_copied, qn, kStatusWaitQ, 5, k)) { ok = false;  break; }
+                    send_stage(next);
+                }
             }
+            k = k2;
+            it = next;
+            ++qn;
         }
         __syncwarp();
     } else if (warp == kTreeSWarp) {
