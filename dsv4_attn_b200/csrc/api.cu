@@ -1116,6 +1116,8 @@ cudaError_t launch_sample(SampleArgs& a, cudaStream_t stream) {
     static std::atomic<bool> done[kMaxDevices];
     const cudaError_t e = ensure_smem(sample_kernel<T>, int(sizeof(SampleShared)), done);
     if (e != cudaSuccess) return e;
+    // (where not all rows are begun at once; a block reads all settings)
+    a.heavy_first = (a.top_k != nullptr || a.top_p != nullptr) && a.N > 2 * device_sms() && a.N <= 16 * kSampleThreads;
     return launch(sample_kernel<T>, dim3(unsigned(int64_t(a.N) * blocks)), kSampleThreads, sizeof(SampleShared), stream, a, blocks > 1 ? blocks : 0);
 }
 }  // namespace
