@@ -765,7 +765,7 @@ def kv_pages_fork(kv_pool, block_table, kv_len, page_refs, parent, child, *, sta
 def kv_pages_compact(kv_pool, block_table, page_refs, *, new_table=None, new_refs=None, count=None, workspace=None, status=None):
     """Live pages move to the front of the pool (every layer), as few as possible: with `count` of them the k-th live page from number `count` on
     goes to the k-th free page below it.  Returns (block_table, page_refs, count int32 [1]) as they are afterwards; the tensors passed in are left as
-    they were unless they are passed as new_table / new_refs too.  workspace: int32 [3 * pages + 1]."""
+    they were unless they are passed as new_table / new_refs too.  workspace: int32 [2 * pages + 1]."""
     r = _host.pages_compact(kv_pool, block_table, page_refs, new_table, new_refs, count, workspace, status)
     if r is None:
         _pages_pool(kv_pool)
@@ -777,7 +777,7 @@ def kv_pages_compact(kv_pool, block_table, page_refs, *, new_table=None, new_ref
                 _check(tuple(t.shape) == tuple(shape), f"{name} must be {list(shape)}")
         if workspace is not None:
             _cuda_contig(workspace, "workspace", torch.int32, 1)
-            _check(workspace.numel() >= 3 * pages + 1, "workspace must hold 3 * pages + 1 int32")
+            _check(workspace.numel() >= 2 * pages + 1, "workspace must hold 2 * pages + 1 int32")
         _pages_status(status)
     if type(r) is tuple:
         return r

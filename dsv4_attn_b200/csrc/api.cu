@@ -1093,8 +1093,7 @@ extern "C" int dsv4_kv_pages_compact(const Dsv4KvPagesParams* p, void* stream) {
     if (p == nullptr || !pages_pool_ok(p) || !pages_table_ok(p) || p->new_table == nullptr || p->new_refs == nullptr || p->count == nullptr || p->scratch == nullptr)
         return int(cudaErrorInvalidValue);
     KvPagesArgs a = pages_args(p);
-    a.remap = p->scratch;
-    a.from = a.remap + p->num_pages;
+    a.from = p->scratch;
     a.to = a.from + p->num_pages;
     a.moves = a.to + p->num_pages;
     const cudaError_t e = launch(kv_compact_plan_kernel, dim3(1), kPagesPlanThreads, 0, static_cast<cudaStream_t>(stream), a);

@@ -659,13 +659,13 @@ PyObject* pages_compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor *pool, *status, *scratch;
     if (n != 8 || !pages_pool(a[0], true, &p, &pool) || !pages_tables(a[1], nullptr, a[2], p.num_pages, &p)) return none();
     if (!optional_tensor(a[7], at::kInt, 1, &status) || (status != nullptr && status->numel() < DSV4_STATUS_WORDS)) return none();
-    if (!optional_tensor(a[6], at::kInt, 1, &scratch) || (scratch != nullptr && scratch->numel() < 3 * p.num_pages + 1)) return none();
+    if (!optional_tensor(a[6], at::kInt, 1, &scratch) || (scratch != nullptr && scratch->numel() < 2 * p.num_pages + 1)) return none();
     Output out[3];
     const int64_t B = p.B, width = p.max_pages;
     if (!out[0].take(a[3], at::kInt, {B, width}, pool) || !out[1].take(a[4], at::kInt, {p.num_pages}, pool) || !out[2].take(a[5], at::kInt, {1}, pool)) return none();
     at::Tensor own;
     if (scratch == nullptr) {
-        own = empty({3 * p.num_pages + 1}, at::kInt, pool);
+        own = empty({2 * p.num_pages + 1}, at::kInt, pool);
         scratch = &own;
     }
     p.new_table = ptr<int32_t>(out[0].t);  p.new_refs = ptr<int32_t>(out[1].t);  p.count = ptr<int32_t>(out[2].t);  p.scratch = ptr<int32_t>(scratch);

@@ -39,9 +39,8 @@ struct KvPagesArgs {
     int32_t* new_table;          // may be block_table
     int32_t* new_refs;           // may be refs
     int32_t* count;              // live pages
-    int32_t* remap;              // scratch [num_pages]: where a page goes
-    int32_t* from;               // scratch [num_pages]: pages that move
-    int32_t* to;                 // scratch [num_pages]: where they go
+    int32_t* from;               // scratch [num_pages]: pages that move, ascending
+    int32_t* to;                 // scratch [num_pages]: where they go, ascending
     int32_t* moves;              // scratch [1]: how many move
     int64_t entries;             // move: entries per layer
     int32_t* status;
@@ -150,17 +149,41 @@ __device__ __forceinline__ int block_prefix(int v, int* s_warp, int& total) {
     return x - v + (warp > 0 ? __shfl_sync(0xFFFFFFFFu, w, warp - 1) : 0);
 }
 
+// A planning block goes through the counts 16 neighbouring pages a thread at a time, with four loads in flight each (100,000 pages: four at a time took 66 us for
+// a compaction's plan).
+constexpr int kPlanPages = 16, kPlanChunk = kPagesPlanThreads * kPlanPages;
+// Bit j: page p + j is one of the pool and held.
+__device__ __forceinline__ uint32_t held_pages(const KvPagesArgs& a, int64_t p, int32_t (&refs)[kPlanPages]) {
+    if (p + kPlanPages <= a.num_pages && (reinterpret_cast<uintptr_t>(a.refs) & 15u) == 0u) {
+#pragma unroll
+        for (int j = 0; j < kPlanPages / 4; ++j) {
+            const int4 v = ptx::ld(reinterpret_cast<const int4*>(a.refs + p) + j);
+            refs[4 * j] = v.x;  refs[4 * j + 1] = v.y;  refs[4 * j + 2] = v.z;  refs[4 * j + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kPlanPages; ++j) refs[j] = p + j < a.num_pages ? ptx::ld(a.refs + p + j) : 0;
+    }
+    uint32_t held = 0u;
+#pragma unroll
+    for (int j = 0; j < kPlanPages; ++j) held |= uint32_t(refs[j] > 0) << j;
+    return held;
+}
+// Bit j: page p + j is one of the pool.
+__device__ __forceinline__ uint32_t pool_pages(const KvPagesArgs& a, int64_t p) {
+    return p + kPlanPages <= a.num_pages ? (1u << kPlanPages) - 1u : (p < a.num_pages ? (1u << (a.num_pages - p)) - 1u : 0u);
+}
+
 // First half of a fork, one block: the children whose parent ends in a partly filled page get the lowest-numbered free pages, in the order
 // of the children.  Writes those pages' table slots and counts, and the children's lengths.
 __global__ void __launch_bounds__(kPagesPlanThreads) kv_fork_plan_kernel(const __grid_constant__ KvPagesArgs a) {
-    constexpr int kPerThread = 4, kChunk = kPagesPlanThreads * kPerThread;
     __shared__ int s_warp[32];
     __shared__ int s_free[kPagesPlanThreads];          // free pages for the children of this round
     __shared__ int s_last;
     ptx::pdl_trigger();
     ptx::pdl_wait();
     const int tid = threadIdx.x;
-    int64_t page0 = 0;                                 // pages before this one are taken
+    int64_t page0 = 0, next = 0;                       // pages before `next` are taken; page0: where to look, a multiple of 16
     for (int base = 0; base < a.n; base += kPagesPlanThreads) {
         const int i = base + tid;
         int parent = 0, child = 0, len = 0;
@@ -173,24 +196,27 @@ __global__ void __launch_bounds__(kPagesPlanThreads) kv_fork_plan_kernel(const _
         const bool need = len % kPageEntries != 0;
         int wanted, found = 0;
         const int rank = block_prefix(need ? 1 : 0, s_warp, wanted);
-        // pages in ascending order, four a thread, until there are enough
+        // pages in ascending order until there are enough
         while (found < wanted && page0 < a.num_pages) {
-            const int64_t p = page0 + tid * kPerThread;
-            int free_bits = 0;
-#pragma unroll
-            for (int j = 0; j < kPerThread; ++j)
-                if (p + j < a.num_pages && ptx::ld(a.refs + p + j) <= 0) free_bits |= 1 << j;
+            const int64_t p = page0 + tid * kPlanPages;
+            int32_t refs[kPlanPages];
+            uint32_t free_bits = ~held_pages(a, p, refs) & pool_pages(a, p);
+            if (p < next) free_bits &= next - p >= kPlanPages ? 0u : ~0u << (next - p);        // (taken in the round before)
             int in_chunk, at = found + block_prefix(__popc(free_bits), s_warp, in_chunk);
-#pragma unroll
-            for (int j = 0; j < kPerThread; ++j)
-                if ((free_bits >> j) & 1) {
-                    if (at < wanted) s_free[at] = int(p + j);
-                    if (at == wanted - 1) s_last = int(p + j);
-                    ++at;
-                }
+            for (uint32_t bits = free_bits; bits != 0u && at < wanted; bits &= bits - 1u, ++at) {
+                const int page = int(p) + __ffs(bits) - 1;
+                s_free[at] = page;
+                if (at == wanted - 1) s_last = page;
+            }
             __syncthreads();
             found += in_chunk;
-            page0 = found >= wanted ? int64_t(s_last) + 1 : page0 + kChunk;
+            if (found >= wanted) {
+                // (the next round begins behind the last page taken, in the same group of 16)
+                next = int64_t(s_last) + 1;
+                page0 = next / kPlanPages * kPlanPages;
+            } else {
+                page0 += kPlanChunk;
+            }
         }
         if (ok) {
             const int full = len / kPageEntries;
@@ -251,43 +277,44 @@ __global__ void __launch_bounds__(kPagesThreads) kv_fork_apply_kernel(const __gr
 // First half of a compaction, one block: with `count` live pages, the k-th live page from `count` on goes to the k-th free page below it (which
 // moves as few pages as possible, and none over another that has yet to move).
 __global__ void __launch_bounds__(kPagesPlanThreads) kv_compact_plan_kernel(const __grid_constant__ KvPagesArgs a) {
-    constexpr int kPerThread = 4, kChunk = kPagesPlanThreads * kPerThread;
     __shared__ int s_warp[32];
     ptx::pdl_trigger();
     ptx::pdl_wait();
     const int tid = threadIdx.x;
     int mine = 0, live = 0;
-    for (int64_t p = tid; p < a.num_pages; p += kPagesPlanThreads) mine += ptx::ld(a.refs + p) > 0;
+    int32_t refs[kPlanPages];
+    for (int64_t p = int64_t(tid) * kPlanPages; p < a.num_pages; p += kPlanChunk) mine += __popc(held_pages(a, p, refs));
     block_prefix(mine, s_warp, live);
     int holes = 0, movers = 0;
-    for (int64_t base = 0; base < a.num_pages; base += kChunk) {
-        const int64_t p = base + tid * kPerThread;
-        int hole_bits = 0, mover_bits = 0;
-#pragma unroll
-        for (int j = 0; j < kPerThread; ++j)
-            if (p + j < a.num_pages) {
-                const bool held = ptx::ld(a.refs + p + j) > 0;
-                a.remap[p + j] = int(p + j);
-                if (p + j < live ? !held : held) (p + j < live ? hole_bits : mover_bits) |= 1 << j;
-            }
-        int found_holes, found_movers;
-        int h = holes + block_prefix(__popc(hole_bits), s_warp, found_holes), m = movers + block_prefix(__popc(mover_bits), s_warp, found_movers);
-#pragma unroll
-        for (int j = 0; j < kPerThread; ++j) {
-            if ((hole_bits >> j) & 1) a.to[h++] = int(p + j);
-            if ((mover_bits >> j) & 1) a.from[m++] = int(p + j);
-        }
-        holes += found_holes;
-        movers += found_movers;
+    for (int64_t base = 0; base < a.num_pages; base += kPlanChunk) {
+        const int64_t p = base + int64_t(tid) * kPlanPages;
+        const uint32_t held = held_pages(a, p, refs), all = pool_pages(a, p);
+        const uint32_t low = p + kPlanPages <= live ? ~0u : (p < live ? (1u << (live - p)) - 1u : 0u);      // pages below `live`
+        uint32_t hole_bits = ~held & all & low, mover_bits = held & ~low;
+        // (both counts of a chunk fit 16 bits)
+        int found;
+        const int before = block_prefix((__popc(hole_bits) << 16) | __popc(mover_bits), s_warp, found);
+        int h = holes + (before >> 16), m = movers + (before & 0xFFFF);
+        for (; hole_bits != 0u; hole_bits &= hole_bits - 1u) a.to[h++] = int(p) + __ffs(hole_bits) - 1;
+        for (; mover_bits != 0u; mover_bits &= mover_bits - 1u) a.from[m++] = int(p) + __ffs(mover_bits) - 1;
+        holes += found >> 16;
+        movers += found & 0xFFFF;
     }
-    __syncthreads();
-    if (a.new_refs != a.refs)
-        for (int64_t p = tid; p < a.num_pages; p += kPagesPlanThreads) a.new_refs[p] = ptx::ld(a.refs + p);
+    if (a.new_refs != a.refs) {
+        constexpr int kDeep = 8;
+        for (int64_t p0 = tid; p0 < a.num_pages; p0 += kDeep * kPagesPlanThreads) {
+            int v[kDeep];
+#pragma unroll
+            for (int j = 0; j < kDeep; ++j) v[j] = p0 + j * kPagesPlanThreads < a.num_pages ? ptx::ld(a.refs + p0 + j * kPagesPlanThreads) : 0;
+#pragma unroll
+            for (int j = 0; j < kDeep; ++j)
+                if (p0 + j * kPagesPlanThreads < a.num_pages) a.new_refs[p0 + j * kPagesPlanThreads] = v[j];
+        }
+    }
     __syncthreads();
     // (as many holes below `live` as live pages above it)
     for (int k = tid; k < movers; k += kPagesPlanThreads) {
         const int s = a.from[k], d = a.to[k];
-        a.remap[s] = d;
         a.new_refs[d] = a.new_refs[s];
         a.new_refs[s] = 0;
     }
@@ -303,11 +330,22 @@ __global__ void __launch_bounds__(kPagesThreads) kv_compact_apply_kernel(const _
     ptx::pdl_wait();
     const int lane = threadIdx.x & 31;
     const int64_t slots = int64_t(a.B) * a.max_pages, stride = int64_t(gridDim.x) * kPagesThreads;
+    const int64_t moves = ptx::ld(a.moves);
+    const int live = ptx::ld(a.count);
     for (int64_t i = int64_t(blockIdx.x) * kPagesThreads + threadIdx.x; i < slots; i += stride) {
-        const int page = a.block_table[i];
-        a.new_table[i] = in_pool(a, page) ? ptx::ld(a.remap + page) : page;
+        int page = a.block_table[i];
+        if (page >= live && moves > 0) {
+            int64_t lo = 0, hi = moves - 1;            // among the pages that move
+            while (lo < hi) {
+                const int64_t mid = (lo + hi) / 2;
+                if (ptx::ld(a.from + mid) < page) lo = mid + 1;
+                else hi = mid;
+            }
+            if (ptx::ld(a.from + lo) == page) page = ptx::ld(a.to + lo);
+        }
+        a.new_table[i] = page;
     }
-    const int64_t moves = ptx::ld(a.moves), units = moves * a.layers * kCopyBatches;
+    const int64_t units = moves * a.layers * kCopyBatches;
     for (int64_t u = int64_t(blockIdx.x) * (kPagesThreads / 32) + (threadIdx.x >> 5); u < units; u += int64_t(gridDim.x) * (kPagesThreads / 32)) {
         const int64_t page = u / kCopyBatches, layer = page / moves, k = page % moves;
         const int s = ptx::ld(a.from + k), d = ptx::ld(a.to + k);

@@ -92,7 +92,7 @@ typedef struct Dsv4KvPagesParams {
     int32_t*       new_table;   /* compact: [B, max_pages], may be block_table */
     int32_t*       new_refs;    /* compact: [num_pages], may be refs */
     int32_t*       count;       /* compact: [1], live pages */
-    int32_t*       scratch;     /* compact: 3 * num_pages + 1 */
+    int32_t*       scratch;     /* compact: 2 * num_pages + 1 */
     int32_t*       status;
 } Dsv4KvPagesParams;
 
