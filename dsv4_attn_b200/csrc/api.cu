@@ -1107,8 +1107,10 @@ template <typename T>
 cudaError_t launch_sample(SampleArgs& a, cudaStream_t stream) {
     // Up to eight blocks share a row where the rows leave SMs without one of the two blocks they hold, as long as each has 4,096 logits; a FixedSum has a limit.
     const int span = a.V + 16 / int(sizeof(T)) - 1;                        // with what a row's alignment may put before it
+    const int steps = (span + kSampleStep - 1) / kSampleStep;
     int blocks = 1;
-    while (blocks < kSampleMaxCluster && ((int64_t(a.N) * blocks <= device_sms() && span > blocks * 4096) || span / kSampleThreads / blocks >= kSampleMostTerms)) blocks *= 2;
+    auto terms = [&] { return (steps + blocks * kSampleWarps - 1) / (blocks * kSampleWarps) * (kSampleStep / 32); };
+    while (blocks < kSampleMaxCluster && ((int64_t(a.N) * blocks <= device_sms() && span > blocks * 4096) || terms() > kSampleMostTerms)) blocks *= 2;
 #ifdef PROBE
     if (getenv("PB")) blocks = atoi(getenv("PB"));
 #endif

@@ -477,6 +477,13 @@ PyObject* combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return rc != 0 ? code(rc) : pair(out, lse);
 }
 
+// Whether the tensors that are there live on the device of `like` (whose stream the launch goes to).
+bool same_device(const at::Tensor* like, std::initializer_list<const at::Tensor*> others) {
+    for (const at::Tensor* t : others)
+        if (t != nullptr && t->device() != like->device()) return false;
+    return true;
+}
+
 // Where the library plans the work of a tree decode in the call: more than four row groups for every pair of SMs (74).  A plan overlaps the set-up of
 // one group with the end of another's and costs 6 us and a merge: 1,024 groups of 15 tiles 301 us against 331 on a static grid, 256 groups 119 either way, 128 groups 58
 // against 53, 92 ragged ones 90 against 81.
@@ -547,8 +554,12 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t rows_bytes = lib.tree_rows_bytes(int(B), int(table->size(1)), int(W));
     if (a[16] == Py_True || (a[16] == Py_None && groups >= kTreeShareGroups * B && groups * ((max_len + 63) / 64) >= kTreeShareTiles && rows_bytes > 0 && rows_bytes <= kTreeShareBytes)) {
         if (rows_bytes <= 0) return none();
-        own_rows = empty({rows_bytes}, at::kByte, q);
-        shared = &own_rows;
+        try {
+            own_rows = empty({rows_bytes}, at::kByte, q);
+            shared = &own_rows;
+        } catch (...) {
+            if (a[16] == Py_True) throw;                                   // without room for it the groups dequantise for themselves
+        }
     } else if (a[16] != Py_None && a[16] != Py_False) {
         shared = tensor(a[16], at::kByte, 1);
         if (shared == nullptr || rows_bytes <= 0 || shared->numel() < rows_bytes) return none();
@@ -559,6 +570,7 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     Output out, lse;
     if (!out.take(a[10], at::kBFloat16, {B, T, H, kLatent}, q) || !lse.take(a[11], at::kFloat, {B, T, H}, q)) return none();
+    if (!same_device(q, {pool, table, kv_len, win, win_len, mask, sink, status, po, pl, sched, shared, out.t, lse.t})) return none();
     p.B = int(B);  p.T = int(T);  p.H = int(H);  p.max_pages = int(table->size(1));  p.win_cap = int(W);  p.mask_words = int(mask->size(2));
     p.num_splits = int(splits);  p.num_pages = pool->size(0);
     p.q = ptr(q);  p.kv_pool = ptr(pool);  p.block_table = ptr<int32_t>(table);  p.kv_len = ptr<int32_t>(kv_len);
@@ -587,6 +599,7 @@ PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (!optional_tensor(a[2 + i], i == 1 ? at::kInt : at::kFloat, 1, &t[i]) || !has_shape(t[i], {N})) return none();
     Output out, logprob;
     if (!out.take(a[6], at::kInt, {N}, logits) || !logprob.take(a[7], at::kFloat, {N}, logits)) return none();
+    if (!same_device(logits, {u, t[0], t[1], t[2], t[3], out.t, logprob.t})) return none();
     p.N = int(N);  p.V = int(V);  p.stride_n = stride;
     p.logits = logits->data_ptr();  p.u = ptr<float>(u);
     p.temperature = ptr<float>(t[0]);  p.top_k = ptr<int32_t>(t[1]);  p.top_p = ptr<float>(t[2]);  p.min_p = ptr<float>(t[3]);
@@ -605,18 +618,20 @@ bool pages_pool(PyObject* o, bool paged, Dsv4KvPagesParams* p, const at::Tensor*
     p->entries = t->size(-3) * t->size(-2);
     return fits32(p->num_pages);
 }
-bool pages_items(PyObject* src_, PyObject* dst_, PyObject* status_, Dsv4KvPagesParams* p) {
+bool pages_items(const at::Tensor* like, PyObject* src_, PyObject* dst_, PyObject* status_, Dsv4KvPagesParams* p) {
     const at::Tensor *src = tensor(src_, at::kInt, 1), *dst = dst_ == nullptr ? src : tensor(dst_, at::kInt, 1), *status;
     if (src == nullptr || dst == nullptr || !fits32(src->size(0)) || src->size(0) != dst->size(0)) return false;
     if (!optional_tensor(status_, at::kInt, 1, &status) || (status != nullptr && status->numel() < DSV4_STATUS_WORDS)) return false;
+    if (!same_device(like, {src, dst, status})) return false;
     p->n = int(src->size(0));  p->src = ptr<int32_t>(src);  p->dst = dst_ == nullptr ? nullptr : ptr<int32_t>(dst);  p->status = ptr<int32_t>(status);
     return true;
 }
 // (num_pages < 0: as many as page_refs has)
-bool pages_tables(PyObject* table_, PyObject* len_, PyObject* refs_, int64_t num_pages, Dsv4KvPagesParams* p) {
+bool pages_tables(const at::Tensor* like, PyObject* table_, PyObject* len_, PyObject* refs_, int64_t num_pages, Dsv4KvPagesParams* p) {
     const at::Tensor *table = tensor(table_, at::kInt, 2), *len = len_ == nullptr ? nullptr : tensor(len_, at::kInt, 1), *refs = tensor(refs_, at::kInt, 1);
     if (table == nullptr || table->numel() <= 0 || !fits32(table->size(0)) || !fits32(table->size(1)) || refs == nullptr || refs->size(0) <= 0 || !fits32(refs->size(0))) return false;
     if ((len_ != nullptr && (len == nullptr || !has_shape(len, {table->size(0)}))) || (num_pages >= 0 && refs->size(0) != num_pages)) return false;
+    if (!same_device(like != nullptr ? like : table, {table, len, refs})) return false;
     p->B = int(table->size(0));  p->max_pages = int(table->size(1));  p->num_pages = refs->size(0);
     p->block_table = ptr<int32_t>(table);  p->kv_len = ptr<int32_t>(len);  p->refs = ptr<int32_t>(refs);
     return true;
@@ -626,7 +641,7 @@ bool pages_tables(PyObject* table_, PyObject* len_, PyObject* refs_, int64_t num
 PyObject* pages_copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Dsv4KvPagesParams p{};
     const at::Tensor* pool;
-    if (n != 4 || !pages_pool(a[0], true, &p, &pool) || !pages_items(a[1], a[2], a[3], &p)) return none();
+    if (n != 4 || !pages_pool(a[0], true, &p, &pool) || !pages_items(pool, a[1], a[2], a[3], &p)) return none();
     return code(launch(lib.pages_copy, &p, stream_of(pool)));
 }
 
@@ -634,14 +649,14 @@ PyObject* pages_copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* entries_move(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Dsv4KvPagesParams p{};
     const at::Tensor* pool;
-    if (n != 4 || !pages_pool(a[0], false, &p, &pool) || !pages_items(a[1], a[2], a[3], &p)) return none();
+    if (n != 4 || !pages_pool(a[0], false, &p, &pool) || !pages_items(pool, a[1], a[2], a[3], &p)) return none();
     return code(launch(lib.entries_move, &p, stream_of(pool)));
 }
 
 // (block_table, kv_len, page_refs, requests, status)
 PyObject* pages_free(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Dsv4KvPagesParams p{};
-    if (n != 5 || !pages_tables(a[0], a[1], a[2], -1, &p) || !pages_items(a[3], nullptr, a[4], &p)) return none();
+    if (n != 5 || !pages_tables(nullptr, a[0], a[1], a[2], -1, &p) || !pages_items(any_tensor(a[0]), a[3], nullptr, a[4], &p)) return none();
     return code(launch(lib.pages_free, &p, stream_of(any_tensor(a[0]))));
 }
 
@@ -649,7 +664,7 @@ PyObject* pages_free(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* pages_fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Dsv4KvPagesParams p{};
     const at::Tensor* pool;
-    if (n != 7 || !pages_pool(a[0], true, &p, &pool) || !pages_tables(a[1], a[2], a[3], p.num_pages, &p) || !pages_items(a[4], a[5], a[6], &p)) return none();
+    if (n != 7 || !pages_pool(a[0], true, &p, &pool) || !pages_tables(pool, a[1], a[2], a[3], p.num_pages, &p) || !pages_items(pool, a[4], a[5], a[6], &p)) return none();
     return code(launch(lib.pages_fork, &p, stream_of(pool)));
 }
 
@@ -657,7 +672,7 @@ PyObject* pages_fork(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* pages_compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Dsv4KvPagesParams p{};
     const at::Tensor *pool, *status, *scratch;
-    if (n != 8 || !pages_pool(a[0], true, &p, &pool) || !pages_tables(a[1], nullptr, a[2], p.num_pages, &p)) return none();
+    if (n != 8 || !pages_pool(a[0], true, &p, &pool) || !pages_tables(pool, a[1], nullptr, a[2], p.num_pages, &p)) return none();
     if (!optional_tensor(a[7], at::kInt, 1, &status) || (status != nullptr && status->numel() < DSV4_STATUS_WORDS)) return none();
     if (!optional_tensor(a[6], at::kInt, 1, &scratch) || (scratch != nullptr && scratch->numel() < 2 * p.num_pages + 1)) return none();
     Output out[3];
@@ -668,6 +683,7 @@ PyObject* pages_compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
         own = empty({2 * p.num_pages + 1}, at::kInt, pool);
         scratch = &own;
     }
+    if (!same_device(pool, {out[0].t, out[1].t, out[2].t, scratch, status})) return none();
     p.new_table = ptr<int32_t>(out[0].t);  p.new_refs = ptr<int32_t>(out[1].t);  p.count = ptr<int32_t>(out[2].t);  p.scratch = ptr<int32_t>(scratch);
     p.status = ptr<int32_t>(status);
     const int rc = launch(lib.pages_compact, &p, stream_of(pool));

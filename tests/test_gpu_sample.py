@@ -202,6 +202,15 @@ def test_the_longest_rows(lib):
         check(lib.sample(logits, u, **s), want(logits, u, **s))
 
 
+def test_sums_at_their_limit(lib):
+    """A thread's sum of weights takes 4,095 terms: rows of equal logits, of the length from which two blocks share one and just below."""
+    for V in (8176 * 256, 8180 * 256, 8192 * 256):
+        logits = torch.full((2, V), 0.25, device="cuda", dtype=torch.bfloat16)
+        u = torch.tensor([0.0, 0.999], device="cuda")
+        for s in (dict(), dict(top_p=torch.full((2,), 0.75, device="cuda"))):
+            check(lib.sample(logits, u, **s), want(logits, u, **s))
+
+
 def test_no_rows_outputs_and_graph(lib):
     empty = lib.sample(torch.empty(0, 100, device="cuda"), torch.empty(0, device="cuda"))
     assert empty[0].shape == (0,)
