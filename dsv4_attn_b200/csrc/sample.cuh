@@ -713,11 +713,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     __syncthreads();
     // a key that enough threads' largest logits reach: from the top, a bit at a time
     const int groups = (r.k + int(blocks) - 1) / int(blocks);
-    // (half of the threads, or of their quarters: more would bring the bound down to logits that most of them exceed several times)
+    // (a quarter of the threads, or half of their quarters: more would bring the bound down to logits that most of them exceed several times, and the
+    // lists would not hold the candidates)
     const bool by_list = !r.greedy && r.k > 0 && groups <= kSampleThreads * kSampleQuarters / 2;
     uint32_t bound = 0u;
     if (by_list) {
-        const bool few = groups <= kSampleThreads / 2;
+        const bool few = groups <= kSampleThreads / 4;
         const uint32_t key = order_key(mine);
 #pragma unroll 1
         for (uint32_t bit = 0x80000000u; bit >= 0x8000u; bit >>= 1) {
@@ -727,7 +728,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                 for (int q = 1; q < kSampleQuarters; ++q) reach += __syncthreads_count(order_key(quarter[q]) >= (bound | bit));
             if (reach >= groups) {
                 bound |= bit;
-                if (reach <= groups + groups / 4 + 4) break;                     // (near enough)
+                if (reach <= groups + groups / 8 + 4) break;                     // (near enough)
             }
         }
     }
@@ -999,9 +1000,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                 });
                 over = by_weight ? sum_all.total() : n_all;
                 ahead = by_weight ? sum_ahead.total() : n_ahead;
-                if (blocks == 1u) {                // (kept for the token, where this turns out to be the cut)
+                if (by_weight) {                   // (per warp, for the token, where this turns out to be the cut)
                     const unsigned long long of_warp = warp_total(ahead);
-                    if (lane == 0) { sh.sum[warp] = of_warp;  sh.ties[warp] = 0u; }
+                    if (lane < int(blocks)) sts_cluster_u64(ptx::mapa(ptx::smem_u32(&sh.sum[me]), lane), of_warp);
                 }
                 row_totals(sh, blocks, rank, turn, over, ahead);
                 if (by_weight) wanted = max(share_of(over + ties, uint32_t(r.p24)), 1ull);
@@ -1009,21 +1010,32 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                 if (wanted <= ahead) { to = from;  from -= 2.5f;  moved = -1;  continue; }
                 const int m = listed(sh, blocks, turn);
                 if (m >= 0 && (by_weight || wanted - ahead <= static_cast<unsigned long long>(m))) {
-                    if (rank == 0) cut_of_list(sh, r, blocks, turn, m, by_weight ? m : int(wanted - ahead), by_weight ? wanted - ahead : ~0ull);
-                    sync_row(blocks);
-                    if (sh.reached) {
-                        cut = sh.cut;
-                        cut_ties = sh.cut_ties;
-                        if (by_weight && blocks == 1u && r.min_p == 0.f) {
+                    if (rank == 0) {
+                        cut_of_list(sh, r, blocks, turn, m, by_weight ? m : int(wanted - ahead), by_weight ? wanted - ahead : ~0ull);
+                        if (by_weight && r.min_p == 0.f && sh.reached) {
+                            // what the candidates above the cut add to their warps' sums, and the ties; to all blocks
+                            if (tid < parts) sh.ties[tid] = 0u;
+                            __syncthreads();
                             for (int i = tid; i < m; i += kSampleThreads) {
                                 const unsigned long long c = sh.sorted[i];
                                 const uint32_t key = uint32_t(c >> 32);
                                 const int of = part_of(int(~uint32_t(c)));
-                                if (key > cut) atomicAdd(&sh.sum[of], fixed(r.ratio(key_value(key))));
-                                else if (key == cut) atomicAdd(&sh.ties[of], 1u);
+                                if (key > sh.cut) atomicAdd(&sh.sum[of], fixed(r.ratio(key_value(key))));
+                                else if (key == sh.cut) atomicAdd(&sh.ties[of], 1u);
                             }
-                            sums_known = true;
+                            __syncthreads();
+                            for (int i = tid; i < parts * (int(blocks) - 1); i += kSampleThreads) {
+                                const int part = i % parts, to_block = 1 + i / parts;
+                                sts_cluster_u64(ptx::mapa(ptx::smem_u32(&sh.sum[part]), to_block), sh.sum[part]);
+                                ptx::sts_cluster_u32(ptx::mapa(ptx::smem_u32(&sh.ties[part]), to_block), sh.ties[part]);
+                            }
                         }
+                    }
+                    sync_row(blocks);
+                    if (sh.reached) {
+                        cut = sh.cut;
+                        cut_ties = sh.cut_ties;
+                        sums_known = by_weight && r.min_p == 0.f;
                         return true;
                     }
                 }
@@ -1100,27 +1112,32 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     // ── sums of the kept weights, per warp ──
     const float cut_value = cut != 0u ? key_value(cut) : -CUDART_INF_F;
     const unsigned long long tie_weight = cut_ties != 0ull ? (r.odd ? 1ull << kSampleOneBits : r.weight(cut_value)) : 0ull;
+    // Below this no token is kept: the cut, or a little below where min-p is.  (Ties at a cut that min-p leaves out weigh nothing, counted or not.)
+    float floor_value = cut_value;
+    if (r.min_p > 0.f && !r.odd) floor_value = fmaxf(floor_value, r.top + (logf(r.min_p) - 1e-4f) / r.per - 1e-5f * fabsf(r.top));
     auto part_sums = [&](int from, int count, unsigned long long& sum, uint32_t& ties) {
         FixedSum kept;
         ties = 0;
-        row.each(from, count, [&](const float (&v)[8], int) {
-            if (cut_ties == 0ull) {
+        if (cut_ties == 0ull && r.min_p == 0.f) {
+            row.each(from, count, [&](const float (&v)[8], int) {
 #pragma unroll
                 for (int i = 0; i < 8; i += 2) {
                     float x0, x1;
                     r.exponents(v[i], v[i + 1], x0, x1);
-                    const float e0 = expf(x0), e1 = expf(x1);
-                    kept.add2(e0 >= r.min_p ? e0 : 0.f, e1 >= r.min_p ? e1 : 0.f);
+                    kept.add2(expf(x0), expf(x1));
                 }
-            } else if (__any_sync(0xFFFFFFFFu, max_of(v) >= cut_value)) {
+            });
+        } else {
+            row.each(from, count, [&](const float (&v)[8], int) {
+                if (!__any_sync(0xFFFFFFFFu, max_of(v) >= floor_value)) return;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float e = r.ratio(v[i]);
                     kept.add(v[i] > cut_value && e >= r.min_p ? e : 0.f);
                     ties += v[i] == cut_value;
                 }
-            }
-        });
+            });
+        }
         sum = warp_total(kept.total());
         ties = __reduce_add_sync(0xFFFFFFFFu, ties);
     };
