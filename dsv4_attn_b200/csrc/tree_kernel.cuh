@@ -17,7 +17,7 @@
 
 namespace dsv4 {
 
-constexpr int kUnpackThreads = 256;
+constexpr int kUnpackThreads = 512;
 
 struct TreeUnpackArgs {
     int B, T, max_pages, win_cap, mask_words, cap;
@@ -33,12 +33,12 @@ struct TreeUnpackArgs {
     int32_t* status;
 };
 
-// A block takes tiles of 64 entries, a warp eight entries of one.  An entry: a lane has 16 latent bytes and their block's scale, eight lanes a piece of
+// A block takes tiles of 64 entries, a warp four entries of one (with eight, two blocks of eight warps fitted an SM: 17 us for 30,000 entries, now %UNPACK%).  An entry: a lane has 16 latent bytes and their block's scale, eight lanes a piece of
 // the RoPE tail.  Rows that take no part (out of range, or window rows that no node sees) are zero: whatever probability they get is zero too,
 // and zero times what the memory held might not be.  DRAM-bound: 656 bytes read and 1152 written an entry.
-__global__ void __launch_bounds__(kUnpackThreads) tree_unpack_kernel(const __grid_constant__ TreeUnpackArgs a) {
-    constexpr int kEach = 8;
-    __shared__ uint32_t s_valid[8];
+__global__ void __launch_bounds__(kUnpackThreads, 2) tree_unpack_kernel(const __grid_constant__ TreeUnpackArgs a) {
+    constexpr int kEach = 4;
+    __shared__ uint32_t s_valid[kTileN / kEach];
     ptx::pdl_trigger();
     ptx::pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -106,14 +106,16 @@ __global__ void __launch_bounds__(kUnpackThreads) tree_unpack_kernel(const __gri
         if (lane == 0) s_valid[warp] = valid;
         __syncthreads();
         if (threadIdx.x < 2) {
-            const uint32_t* s = s_valid + 4 * threadIdx.x;
-            a.valid[(int64_t(b) * a.cap + v0) / 32 + threadIdx.x] = s[0] | (s[1] << 8) | (s[2] << 16) | (s[3] << 24);
+            uint32_t bits = 0u;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) bits |= s_valid[8 * threadIdx.x + i] << (kEach * i);
+            a.valid[(int64_t(b) * a.cap + v0) / 32 + threadIdx.x] = bits;
         }
     }
 }
 
 // Warp roles of the attention kernel.
-constexpr int kTreeQWarps = 8;                 // warps 4-11: Q into tensor memory, BF16 to FP16
+constexpr int kTreeQWarps = 8;                 // warps 4-11: Q into tensor memory, BF16 to FP16; and the output
 constexpr int kTreeFirstQWarp = 4;
 constexpr int kTreeSWarp = 12;                 // tensor-memory allocation; (even block) issue of the S MMAs
 constexpr int kTreeOWarp = 13;                 // (even block) issue of the O MMAs
@@ -130,6 +132,7 @@ struct TreeArgs {
     int mask_words;
     int num_splits;
     float scale_log2;
+    const __nv_bfloat16* q;
     const uint32_t* valid;
     const int32_t* kv_len;
     const int32_t* win_len;
@@ -164,15 +167,19 @@ struct TreeSmem {
 
 struct TreeMisc {
     float exch[2 * kHeadsPerBlock];
+    float inv[2][kHeadsPerBlock];    // per item, in turn: what the rows' outputs are multiplied by
     uint64_t bar_tmem;
-    uint64_t bar_q_full[2];          // per item: chunks 0-5 / 6-8 landed
+    uint64_t bar_q_full[2];          // per item: chunks 0-5 / 6-8 of Q landed
     uint64_t bar_q_copied;           // per item: chunks 0-5 copied out by every Q warp
+    uint64_t bar_inv[2];             // per item, in turn: inv written (the softmax warps may finish the next item before the last Q warp comes to this)
     // signalled in both blocks by the commits of the MMA warps
     uint64_t bar_q_free;             // per item: its S MMAs complete
+    uint64_t bar_o_last;             // per item: its P.V complete
     uint64_t bar_s_full[2];          // S of a tile complete: S buffer full, K buffer free
     uint64_t bar_o_full[2];          // P.V of a tile complete: V and P buffer free, O up to date
     // in the even block only, signalled by the warps of both
     uint64_t bar_q_ready;
+    uint64_t bar_o_read;             // per item: its O has been read
     uint64_t bar_k_full[2], bar_v_full[2];                // both blocks' halves of a tile landed (TMA transaction count, by the copies themselves)
     uint64_t bar_p_full[2];
     uint32_t tmem_base;
@@ -230,7 +237,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
     };
 
     const uint32_t bar_tmem = ptx::smem_u32(&misc->bar_tmem), bar_q_full = ptx::smem_u32(&misc->bar_q_full[0]), bar_q_copied = ptx::smem_u32(&misc->bar_q_copied),
-                   bar_q_free = ptx::smem_u32(&misc->bar_q_free),
+                   bar_q_free = ptx::smem_u32(&misc->bar_q_free), bar_o_last = ptx::smem_u32(&misc->bar_o_last), bar_inv = ptx::smem_u32(&misc->bar_inv[0]),
+                   bar_o_read = ptx::smem_u32(&misc->bar_o_read),
                    bar_s_full = ptx::smem_u32(&misc->bar_s_full[0]), bar_o_full = ptx::smem_u32(&misc->bar_o_full[0]), bar_q_ready = ptx::smem_u32(&misc->bar_q_ready),
                    bar_k_full = ptx::smem_u32(&misc->bar_k_full[0]), bar_v_full = ptx::smem_u32(&misc->bar_v_full[0]), bar_p_full = ptx::smem_u32(&misc->bar_p_full[0]);
     auto arrive_even = [&](uint32_t bar) {
@@ -245,6 +253,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
         ptx::mbar_init(bar_tmem, 1);
         ptx::mbar_init(bar_q_copied, kTreeQWarps);
         ptx::mbar_init(bar_q_free, 1);
+        ptx::mbar_init(bar_o_last, 1);
+        ptx::mbar_init(bar_inv, kNumSoftmaxWarps);
+        ptx::mbar_init(bar_inv + 8, kNumSoftmaxWarps);
+        ptx::mbar_init(bar_o_read, 2 * kTreeQWarps);
         ptx::mbar_init(bar_q_ready, 2 * kTreeQWarps);
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(bar_q_full + 8 * i, 1);
@@ -279,23 +291,68 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
     // Running counters, as in decode_kernel.cuh: `g` the tiles over all items, `qn` the items that had tiles.  Tile g is the (g / 2)-th use of K, V, S and P
     // buffer g % 2.  Every waiter goes through a barrier's phases one by one.
     if (warp >= kTreeFirstQWarp && warp < kTreeSWarp) {
-        // ───────────── Q warps ─────────────
+        // ───────────── Q warps: Q of the next item, then the output of this one ─────────────
+        // Between two items the tensor pipe waits for Q (into tensor memory, and its last chunks) and for O to be read:
+        // by eight warps that have nothing else to do then, while the softmax warps are at the next item's first tiles.  (With the output written by the softmax
+        // warps, through shared memory, an item of 15 tiles cost five tiles more.)
         const int qw = warp - kTreeFirstQWarp;
         bool ok = wait_tmem();
         if (!ok) wait_ran_out(a.status, kStatusWaitQ, 2, -1);
         uint32_t qn = 0;
+        Item last{};                                   // the item whose output is to be written
+        auto write_out = [&]() -> bool {
+            // row r of this block, value columns [256 half + 128 (qw / 4), +128): 32 at a time, 64 bytes of 16-bit values
+            const int r = (qw & 1) * 32 + lane, half = (qw >> 1) & 1;
+            const int h0 = last.hg * kHeadsPerCta + rank * kHeadsPerBlock;
+            const bool final_out = last.slot < 0;
+            if (!wait_for(bar_inv + 8 * ((qn - 1u) & 1u), (qn - 1u) >> 1, kStatusWaitOFull, 2, 0) || !wait_for(bar_o_last, qn - 1u, kStatusWaitOFull, 2, 0)) return false;
+            ptx::tc_fence_after_sync();
+            const float inv = misc->inv[(qn - 1u) & 1u][r];
+            const int64_t prow0 = final_out ? 0 : (sched ? int64_t(last.slot) * kHeadsPerCta + rank * kHeadsPerBlock : (int64_t(last.slot) * a.B + last.n) * a.H + h0);
+            __nv_bfloat16* const row = (final_out ? a.out + (int64_t(last.n) * a.H + h0) * 512 : reinterpret_cast<__nv_bfloat16*>(a.partial_o) + prow0 * 512) + int64_t(r) * 512 +
+                                       256 * half + 128 * (qw >> 2);
+            const bool whole_sectors = (reinterpret_cast<uintptr_t>(row) & 31u) == 0u;      // (the caller's tensors are aligned to 16 bytes)
+            const uint32_t from = tmem + (uint32_t((qw & 3) * 32) << 16) + kTmemO + 128u * uint32_t(qw >> 2);
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+                uint32_t o[32];
+                ptx::tmem_ld32(from + 32u * uint32_t(c), o);
+                ptx::tmem_wait_ld();
+                if (c == 3) {
+                    ptx::tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) arrive_even(bar_o_read);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float x = __uint_as_float(o[2 * i]) * inv, y = __uint_as_float(o[2 * i + 1]) * inv;
+                    o[i] = final_out ? ptx::pack_bf16x2(x, y) : ptx::pack_f16x2(x, y);
+                }
+                if (h0 + r < a.H) {
+                    if (whole_sectors) {
+                        ptx::stg_v8(row + 32 * c, o);
+                        ptx::stg_v8(row + 32 * c + 16, o + 8);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(row + 32 * c)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    }
+                }
+            }
+            return true;
+        };
 #pragma unroll 1
         for (int k = 0; k < n_items && ok; ++k) {
-            if (get_item(k).ntiles <= 0) continue;
-            if (!wait_for(bar_q_full, qn, kStatusWaitQ, 2, k) || (qn > 0u && !wait_for(bar_q_free, qn - 1u, kStatusWaitSFull, 2, k))) break;
+            const Item it = get_item(k);
+            if (it.ntiles <= 0) continue;
+            if (!wait_for(bar_q_full, qn, kStatusWaitQ, 2, k) || (qn > 0u && !wait_for(bar_q_free, qn - 1u, kStatusWaitSFull, 2, k))) { ok = false;  break; }
             ptx::tc_fence_after_sync();
             q_to_tmem<true>(q_stage, tmem + kTmemQ, qw, lane);
             q_to_tmem<true>(q_stage + 3 * kQChunkBytes, tmem + kTmemQ + 96, qw, lane);
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(bar_q_copied);
-            if (!wait_for(bar_q_full + 8, qn, kStatusWaitQ, 2, k)) break;
+            if (!wait_for(bar_q_full + 8, qn, kStatusWaitQ, 2, k)) { ok = false;  break; }
             constexpr int kVecs = L::kQBytes / 16 / (kTreeQWarps * 32);
-#pragma unroll 1
+#pragma unroll
             for (int i = 0; i < kVecs; ++i) {
                 const uint32_t at = q_base + uint32_t((i * kTreeQWarps + qw) * 32 + lane) * 16u;
                 ptx::sts_v4(at, bf16x8_to_f16x8(ptx::lds_v4(at)));
@@ -305,8 +362,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
             ptx::fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) arrive_even(bar_q_ready);
+            if (qn > 0u && !write_out()) { ok = false;  break; }
+            last = it;
             ++qn;
         }
+        if (ok && qn > 0u) write_out();
         __syncwarp();
     } else if (warp == kTreeKWarp) {
         // ───────────── K tiles: both blocks' copies report to the even one, which expects the bytes of both ─────────────
@@ -331,16 +391,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
         }
         __syncwarp();
     } else if (warp == kTreeVWarp) {
-        // ───────────── V tiles; Q: chunks 0-5 of the next item while this one is at work, the others when its S MMAs are done ─────────────
+        // ───────────── V tiles; Q of the next item while this one is at work ─────────────
         const uint32_t v_full = ptx::mapa(bar_v_full, 0);
         bool ok = true;
         uint32_t g = 0, qn = 0;
+        auto q_row = [&](const Item& it) { return it.n * a.H + it.hg * kHeadsPerCta + rank * kHeadsPerBlock; };
+        // chunks 0-5 to the staging area, and the others into L2: their place is free when the S MMAs of the item before are done
         auto send_stage = [&](const Item& it) {
             if (ptx::elect_one()) {
-                const int row = it.n * a.H + it.hg * kHeadsPerCta + rank * kHeadsPerBlock;
                 ptx::mbar_arrive_expect_tx(bar_q_full, L::kStageBytes);
 #pragma unroll
-                for (int c = 0; c < 6; ++c) ptx::tma_load_2d(q_stage + c * kQChunkBytes, &a.q_map, c * 64, row, bar_q_full);
+                for (int c = 0; c < 6; ++c) ptx::tma_load_2d(q_stage + c * kQChunkBytes, &a.q_map, c * 64, q_row(it), bar_q_full);
+            }
+            __syncwarp();
+            const int rows = min(kHeadsPerBlock, a.H - (it.hg * kHeadsPerCta + rank * kHeadsPerBlock));
+            const uint8_t* base = reinterpret_cast<const uint8_t*>(a.q) + int64_t(q_row(it)) * 1152 + 768;
+#pragma unroll 1
+            for (int i = lane; i < 3 * rows; i += 32) ptx::prefetch_l2(base + int64_t(i / 3) * 1152 + i % 3 * 128);
+        };
+        auto send_rest = [&](const Item& it) {
+            if (ptx::elect_one()) {
+                ptx::mbar_arrive_expect_tx(bar_q_full + 8, L::kQBytes);
+#pragma unroll
+                for (int c = 0; c < 3; ++c) ptx::tma_load_2d(q_base + c * kQChunkBytes, &a.q_map, (6 + c) * 64, q_row(it), bar_q_full + 8);
             }
             __syncwarp();
         };
@@ -358,13 +431,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
 #pragma unroll 1
         while (k < n_items && ok) {
             if (qn > 0u && !wait_for(bar_q_free, qn - 1u, kStatusWaitSFull, 5, k)) break;
-            if (ptx::elect_one()) {
-                const int row = it.n * a.H + it.hg * kHeadsPerCta + rank * kHeadsPerBlock;
-                ptx::mbar_arrive_expect_tx(bar_q_full + 8, L::kQBytes);
-#pragma unroll
-                for (int c = 0; c < 3; ++c) ptx::tma_load_2d(q_base + c * kQChunkBytes, &a.q_map, (6 + c) * 64, row, bar_q_full + 8);
-            }
-            __syncwarp();
+            send_rest(it);
             int k2 = k;
             const Item next = next_item(k2);
 #pragma unroll 1
@@ -437,10 +504,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
             constexpr uint32_t kDescHi = ptx::smem_desc_hi(1024), idesc = ptx::make_idesc_f16(128, 256, false, true);
             bool ok = wait_tmem();
             const uint32_t p_lo0 = ptx::smem_desc_lo(p_base, 16), v_lo0 = ptx::smem_desc_lo(v_base, kVChunkBytes);
-            uint32_t g = 0;
+            uint32_t g = 0, qn = 0;
 #pragma unroll 1
             for (int k = 0; k < n_items && ok; ++k) {
                 const Item it = get_item(k);
+                if (it.ntiles <= 0) continue;
+                // O of the item before has been read
+                if (qn > 0u && !wait_for(bar_o_read, qn - 1u, kStatusWaitOFull, 3, int(g))) break;
+                ++qn;
 #pragma unroll 1
                 for (int i = 0; i < it.ntiles; ++i, ++g) {
                     const uint32_t buf = g & 1u;
@@ -460,6 +531,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
                                     ptx::mma2_ss(tmem + kTmemO + jj * 128, p_lo + uint32_t((s * 32) >> 4), v_lo + uint32_t((2 * jj * kVChunkBytes + s * 16 * 128) >> 4), kDescHi,
                                                  idesc, (i > 0 || s > 0) ? 1u : 0u);
                         ptx::mma2_commit(bar_o_full + 8 * buf);
+                        if (i + 1 == it.ntiles) ptx::mma2_commit(bar_o_last);
                     }
                     __syncwarp();
                 }
@@ -467,9 +539,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
         }
         __syncwarp();
     } else {
-        // ───────────── softmax + epilogue warps: as in decode_kernel.cuh ─────────────
-        // Thread tid owns row tid % 64 of this block and, of its S row, the entries 32 (tid / 64) .. +31 of the tile; of its O row the value columns
-        // [256 (tid / 64), +256).
+        // ───────────── softmax warps: as in decode_kernel.cuh, but for the output ─────────────
+        // Thread tid owns row tid % 64 of this block and, of its S row, the entries 32 (tid / 64) .. +31 of the tile.
         const int r = tid & 63, colhalf = tid >> 6;
         const uint32_t lane_addr = uint32_t(warp * 32) << 16;
         const uint32_t pair_bar = 1u + uint32_t(warp & 1);
@@ -478,7 +549,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
         ok = !ptx::bar_any(pair_bar, 64, !ok);
         const uint32_t p_row = p_base + uint32_t(r) * 128u;
         const uint32_t p_sw = (uint32_t(4 * colhalf) ^ uint32_t(r & 7)) << 4;
-        uint32_t gt = 0;
+        uint32_t gt = 0, qn = 0;
         Item cur = get_item(0);
 #pragma unroll 1
         for (int k = 0; k < n_items && ok; ++k) {
@@ -581,52 +652,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
                 if (lane == 0) arrive_even(bar_p_full + 8 * (g & 1u));
             }
             if (left) break;
-            // ── epilogue ──
+            // ── the row's sum, and what its output is multiplied by ──
             gt += uint32_t(nb);
             if (k + 1 < n_items) cur = get_item(k + 1);
-            if (ok) ok = wait_for(bar_o_full + 8 * ((gt - 1u) & 1u), (gt - 1u) >> 1, kStatusWaitOFull, 0, int(gt));
             if (ptx::bar_any(pair_bar, 64, !ok)) { ok = false;  break; }
             misc->exch[tid] = l_sum;
             ptx::bar_sync(pair_bar + 2u, 64);
             l_sum += misc->exch[tid ^ 64];
-            ptx::tc_fence_after_sync();
             if (tid == 0 && k == n_items - 1 && (sched || a.num_splits > 1)) ptx::pdl_trigger();      // (a merge follows)
             float denom = l_sum;
             if (final_out && a.attn_sink != nullptr && write) {
                 const float s2 = ptx::ld(a.attn_sink + (h0 + r) % a.heads) * 1.4426950408889634f;
                 denom = (l_sum != 0.f) ? l_sum + ptx::ex2(s2 - m_ref) : 1.f;
             }
-            const float inv = (l_sum != 0.f) ? 1.f / denom : 0.f;
-            const int row0 = (warp & 1) * 32;
-            uint8_t* gbase = reinterpret_cast<uint8_t*>(out_rows + int64_t(row0) * 512 + colhalf * 256);
-#pragma unroll 1
-            for (int pass = 0; pass < 4; ++pass) {
-#pragma unroll
-                for (int hc = 0; hc < 2; ++hc) {
-                    uint32_t o[32];
-                    ptx::tmem_ld32(tmem + lane_addr + kTmemO + pass * 64 + hc * 32, o);
-                    ptx::tmem_wait_ld();
-#pragma unroll
-                    for (int v = 0; v < 4; ++v) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float x = __uint_as_float(o[8 * v + 2 * i]) * inv, y = __uint_as_float(o[8 * v + 2 * i + 1]) * inv;
-                            w[i] = final_out ? ptx::pack_bf16x2(x, y) : ptx::pack_f16x2(x, y);
-                        }
-                        ptx::sts_v4(p_row + uint32_t(hc) * kQChunkBytes + (p_sw ^ (uint32_t(v) << 4)), make_uint4(w[0], w[1], w[2], w[3]));
-                    }
-                }
-                __syncwarp();
-#pragma unroll
-                for (int q = 0; q < 8; ++q) {
-                    const uint32_t rl = uint32_t(q * 4 + (lane >> 3)), vc = uint32_t(lane & 7);
-                    const uint32_t at = p_base + (vc >> 2) * kQChunkBytes + uint32_t(row0 + rl) * 128u + (((4u * colhalf + (vc & 3u)) ^ (rl & 7u)) << 4);
-                    if (h0 + row0 + int(rl) < a.H)
-                        *reinterpret_cast<uint4*>(gbase + int64_t(rl) * 1024 + pass * 128 + vc * 16u) = ptx::lds_v4(at);
-                }
-                __syncwarp();
-            }
+            if (colhalf == 0) misc->inv[qn & 1u][r] = (l_sum != 0.f) ? 1.f / denom : 0.f;
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(bar_inv + 8 * (qn & 1u));
+            ++qn;
             if (write && colhalf == 0) {
                 const float lse2 = (l_sum != 0.f) ? m_ref + log2f(l_sum) : -CUDART_INF_F;
                 if (!final_out) a.partial_lse[prow0 + r] = lse2;

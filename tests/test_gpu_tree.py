@@ -161,6 +161,19 @@ def test_a_chain_is_the_plain_decode(lib):
     assert torch.equal(out, o) and torch.equal(lse, l)
 
 
+@pytest.mark.parametrize("rows", [False, True])
+def test_outputs_of_any_alignment(lib, rows):
+    """`out` at 16 bytes from a sector's start, and many items of one and two tiles a pair of blocks."""
+    from dsv4_attn_b200 import layout
+    B, T, H = 40, 10, 128
+    c = make(15, B, T, H, [(7 * b) % 90 for b in range(B)], 40)
+    buffer = torch.zeros(B * T * H * 512 + 8, device="cuda", dtype=torch.bfloat16)
+    out = buffer[8:].view(B, T, H, 512)
+    got = call(lib, c, SCALE, out=out, share_rows=rows)
+    assert got[0] is out and buffer[:8].eq(0).all()
+    check(got, want(c, SCALE))
+
+
 def test_tree_sees():
     """Ancestors, the node itself, and the committed tokens that have not slid out."""
     from dsv4_attn_b200 import layout
