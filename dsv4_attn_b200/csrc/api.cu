@@ -959,7 +959,7 @@ cudaError_t launch_tree(const DecodeArgs& d, const Dsv4HcaTreeDecodeParams* p, c
     if (e == cudaSuccess) e = make_tile_map(&a.v_map, u.rows, p->B * cap, kTileN);
     if (e != cudaSuccess) return e;
     a.B = d.B;  a.H = d.H;  a.heads = d.tree_heads;  a.cap = int(cap);  a.mask_words = d.tree_words;  a.num_splits = d.num_splits;  a.scale_log2 = d.scale_log2;
-    a.q = d.q;  a.valid = u.valid;  a.kv_len = d.kv_len;  a.win_len = d.win_len;  a.tree_mask = d.tree_mask;  a.attn_sink = d.attn_sink;
+    a.valid = u.valid;  a.kv_len = d.kv_len;  a.win_len = d.win_len;  a.tree_mask = d.tree_mask;  a.attn_sink = d.attn_sink;
     a.out = d.out;  a.lse = d.lse;  a.partial_o = d.partial_o;  a.partial_lse = d.partial_lse;  a.status = d.status;
     const unsigned long long wait_ns = g_wait_ns.load(std::memory_order_relaxed);
     a.wait_ns = uint32_t(wait_ns < 4000000000ull ? wait_ns : 4000000000ull);

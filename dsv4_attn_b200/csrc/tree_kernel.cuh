@@ -132,7 +132,6 @@ struct TreeArgs {
     int mask_words;
     int num_splits;
     float scale_log2;
-    const __nv_bfloat16* q;
     const uint32_t* valid;
     const int32_t* kv_len;
     const int32_t* win_len;
@@ -151,7 +150,7 @@ struct TreeArgs {
 
 struct TreeSmem {
     static constexpr int kQBytes = 3 * kQChunkBytes;            // chunks 6-8 stay here
-    static constexpr int kStageBytes = 6 * kQChunkBytes;        // chunks 0-5 on their way to tensor memory
+    static constexpr int kStageBytes = 6 * kQChunkBytes;        // chunks 0-5 on their way to tensor memory, then 6-8
     static constexpr int kKBytes = 9 * kKChunkBytes;
     static constexpr int kVBytes = 4 * kVChunkBytes;
     static constexpr int kQOff = 0;
@@ -169,8 +168,8 @@ struct TreeMisc {
     float exch[2 * kHeadsPerBlock];
     float inv[2][kHeadsPerBlock];    // per item, in turn: what the rows' outputs are multiplied by
     uint64_t bar_tmem;
-    uint64_t bar_q_full[2];          // per item: chunks 0-5 / 6-8 of Q landed
-    uint64_t bar_q_copied;           // per item: chunks 0-5 copied out by every Q warp
+    uint64_t bar_q_full[2];          // per item: chunks 0-5 / 6-8 of Q landed in the staging area
+    uint64_t bar_q_read[2];          // per item: they have been read there by every Q warp
     uint64_t bar_inv[2];             // per item, in turn: inv written (the softmax warps may finish the next item before the last Q warp comes to this)
     // signalled in both blocks by the commits of the MMA warps
     uint64_t bar_q_free;             // per item: its S MMAs complete
@@ -236,7 +235,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
         return it;
     };
 
-    const uint32_t bar_tmem = ptx::smem_u32(&misc->bar_tmem), bar_q_full = ptx::smem_u32(&misc->bar_q_full[0]), bar_q_copied = ptx::smem_u32(&misc->bar_q_copied),
+    const uint32_t bar_tmem = ptx::smem_u32(&misc->bar_tmem), bar_q_full = ptx::smem_u32(&misc->bar_q_full[0]), bar_q_read = ptx::smem_u32(&misc->bar_q_read[0]),
                    bar_q_free = ptx::smem_u32(&misc->bar_q_free), bar_o_last = ptx::smem_u32(&misc->bar_o_last), bar_inv = ptx::smem_u32(&misc->bar_inv[0]),
                    bar_o_read = ptx::smem_u32(&misc->bar_o_read),
                    bar_s_full = ptx::smem_u32(&misc->bar_s_full[0]), bar_o_full = ptx::smem_u32(&misc->bar_o_full[0]), bar_q_ready = ptx::smem_u32(&misc->bar_q_ready),
@@ -251,7 +250,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
     if (tid == 0) {
         ptx::sts_u32(failed_flag(), 0u);
         ptx::mbar_init(bar_tmem, 1);
-        ptx::mbar_init(bar_q_copied, kTreeQWarps);
+        ptx::mbar_init(bar_q_read, kTreeQWarps);
+        ptx::mbar_init(bar_q_read + 8, kTreeQWarps);
         ptx::mbar_init(bar_q_free, 1);
         ptx::mbar_init(bar_o_last, 1);
         ptx::mbar_init(bar_inv, kNumSoftmaxWarps);
@@ -344,24 +344,45 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
         for (int k = 0; k < n_items && ok; ++k) {
             const Item it = get_item(k);
             if (it.ntiles <= 0) continue;
-            if (!wait_for(bar_q_full, qn, kStatusWaitQ, 2, k) || (qn > 0u && !wait_for(bar_q_free, qn - 1u, kStatusWaitSFull, 2, k))) { ok = false;  break; }
-            ptx::tc_fence_after_sync();
-            q_to_tmem<true>(q_stage, tmem + kTmemQ, qw, lane);
-            q_to_tmem<true>(q_stage + 3 * kQChunkBytes, tmem + kTmemQ + 96, qw, lane);
+            // Chunks 0-5 wait for their place in tensor memory in registers (96 a thread: half of a row's columns, as FP16), so that the others can come to
+            // the staging area meanwhile.
+            if (!wait_for(bar_q_full, qn, kStatusWaitQ, 2, k)) { ok = false;  break; }
+            uint32_t x[2][48];
+            const int half = qw >> 2;
+            const uint32_t q_rows = q_stage + uint32_t((qw & 1) * 32 + lane) * 128u, sw = uint32_t(lane & 7) << 4;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < 12; ++i) {
+                    const uint32_t u = uint32_t(half * 12 + i);
+                    const uint4 v = bf16x8_to_f16x8(ptx::lds_v4(q_rows + (3u * j + (u >> 3)) * kQChunkBytes + (((u & 7u) << 4) ^ sw)));
+                    x[j][4 * i] = v.x;  x[j][4 * i + 1] = v.y;  x[j][4 * i + 2] = v.z;  x[j][4 * i + 3] = v.w;
+                }
             __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(bar_q_copied);
-            if (!wait_for(bar_q_full + 8, qn, kStatusWaitQ, 2, k)) { ok = false;  break; }
+            if (lane == 0) ptx::mbar_arrive(bar_q_read);
+            if (!wait_for(bar_q_full + 8, qn, kStatusWaitQ, 2, k) || (qn > 0u && !wait_for(bar_q_free, qn - 1u, kStatusWaitSFull, 2, k))) { ok = false;  break; }
+            ptx::tc_fence_after_sync();
+            const uint32_t q_tmem = tmem + (uint32_t((qw & 3) * 32) << 16) + kTmemQ + 48u * uint32_t(half);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                ptx::tmem_st32(q_tmem + 96u * j, reinterpret_cast<const uint32_t(&)[32]>(x[j][0]));
+                ptx::tmem_st8(q_tmem + 96u * j + 32u, make_uint4(x[j][32], x[j][33], x[j][34], x[j][35]), make_uint4(x[j][36], x[j][37], x[j][38], x[j][39]));
+                ptx::tmem_st8(q_tmem + 96u * j + 40u, make_uint4(x[j][40], x[j][41], x[j][42], x[j][43]), make_uint4(x[j][44], x[j][45], x[j][46], x[j][47]));
+            }
             constexpr int kVecs = L::kQBytes / 16 / (kTreeQWarps * 32);
 #pragma unroll
             for (int i = 0; i < kVecs; ++i) {
-                const uint32_t at = q_base + uint32_t((i * kTreeQWarps + qw) * 32 + lane) * 16u;
-                ptx::sts_v4(at, bf16x8_to_f16x8(ptx::lds_v4(at)));
+                const uint32_t at = uint32_t((i * kTreeQWarps + qw) * 32 + lane) * 16u;
+                ptx::sts_v4(q_base + at, bf16x8_to_f16x8(ptx::lds_v4(q_stage + at)));
             }
             ptx::tmem_wait_st();
             ptx::tc_fence_before_sync();
             ptx::fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) arrive_even(bar_q_ready);
+            if (lane == 0) {
+                arrive_even(bar_q_ready);
+                ptx::mbar_arrive(bar_q_read + 8);
+            }
             if (qn > 0u && !write_out()) { ok = false;  break; }
             last = it;
             ++qn;
@@ -396,24 +417,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
         bool ok = true;
         uint32_t g = 0, qn = 0;
         auto q_row = [&](const Item& it) { return it.n * a.H + it.hg * kHeadsPerCta + rank * kHeadsPerBlock; };
-        // chunks 0-5 to the staging area, and the others into L2: their place is free when the S MMAs of the item before are done
-        auto send_stage = [&](const Item& it) {
+        // chunks 0-5, and when these have been read the others, to the staging area
+        auto send_q = [&](const Item& it, int part) {
             if (ptx::elect_one()) {
-                ptx::mbar_arrive_expect_tx(bar_q_full, L::kStageBytes);
+                ptx::mbar_arrive_expect_tx(bar_q_full + 8 * part, part ? L::kQBytes : L::kStageBytes);
 #pragma unroll
-                for (int c = 0; c < 6; ++c) ptx::tma_load_2d(q_stage + c * kQChunkBytes, &a.q_map, c * 64, q_row(it), bar_q_full);
-            }
-            __syncwarp();
-            const int rows = min(kHeadsPerBlock, a.H - (it.hg * kHeadsPerCta + rank * kHeadsPerBlock));
-            const uint8_t* base = reinterpret_cast<const uint8_t*>(a.q) + int64_t(q_row(it)) * 1152 + 768;
-#pragma unroll 1
-            for (int i = lane; i < 3 * rows; i += 32) ptx::prefetch_l2(base + int64_t(i / 3) * 1152 + i % 3 * 128);
-        };
-        auto send_rest = [&](const Item& it) {
-            if (ptx::elect_one()) {
-                ptx::mbar_arrive_expect_tx(bar_q_full + 8, L::kQBytes);
-#pragma unroll
-                for (int c = 0; c < 3; ++c) ptx::tma_load_2d(q_base + c * kQChunkBytes, &a.q_map, (6 + c) * 64, q_row(it), bar_q_full + 8);
+                for (int c = 0; c < 6; ++c)
+                    if (part == 0 || c < 3) ptx::tma_load_2d(q_stage + c * kQChunkBytes, &a.q_map, (6 * part + c) * 64, q_row(it), bar_q_full + 8 * part);
             }
             __syncwarp();
         };
@@ -427,11 +437,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
         };
         int k = -1;
         Item it = next_item(k);
-        if (k < n_items) send_stage(it);
+        if (k < n_items) {
+            send_q(it, 0);
+            if (wait_for(bar_q_read, 0u, kStatusWaitQ, 5, 0)) send_q(it, 1);
+            else ok = false;
+        }
 #pragma unroll 1
         while (k < n_items && ok) {
-            if (qn > 0u && !wait_for(bar_q_free, qn - 1u, kStatusWaitSFull, 5, k)) break;
-            send_rest(it);
             int k2 = k;
             const Item next = next_item(k2);
 #pragma unroll 1
@@ -445,9 +457,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
                     for (int c = 0; c < 4; ++c) ptx::tma_load_2d_pair(v_base + buf * L::kVBytes + c * kVChunkBytes, &a.v_map, rank * 256 + c * 64, row, v_full + 8 * buf);
                 }
                 __syncwarp();
+                // (by the third tile this item's Q is in place, by the sixth the Q warps have written the output of the one before)
                 if (i == min(it.ntiles - 1, 2) && k2 < n_items) {
-                    if (!wait_for(bar_q_copied, qn, kStatusWaitQ, 5, k)) { ok = false;  break; }
-                    send_stage(next);
+                    if (!wait_for(bar_q_read + 8, qn, kStatusWaitQ, 5, k)) { ok = false;  break; }
+                    send_q(next, 0);
+                }
+                if (i == min(it.ntiles - 1, 5) && k2 < n_items) {
+                    if (!wait_for(bar_q_read, qn + 1u, kStatusWaitQ, 5, k)) { ok = false;  break; }
+                    send_q(next, 1);
                 }
             }
             k = k2;
