@@ -940,6 +940,19 @@ cudaError_t make_tile_map(CUtensorMap* map, const void* base, int64_t rows, int 
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
+// 16-bit rows of 512 in `groups` of `rows`, box of 64 columns by 32 rows, 128-byte swizzle.
+cudaError_t make_out_map(CUtensorMap* map, void* base, int64_t rows, int64_t groups) {
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (fn == nullptr) return cudaErrorNotSupported;
+    const cuuint64_t dims[3] = {512, cuuint64_t(rows), cuuint64_t(groups)};
+    const cuuint64_t strides[2] = {1024, cuuint64_t(rows) * 1024};
+    const cuuint32_t box[3] = {64, 32, 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 // The entries into the workspace, and the attention over them.
 cudaError_t launch_tree(const DecodeArgs& d, const Dsv4HcaTreeDecodeParams* p, const void* sched, cudaStream_t stream) {
     const int64_t cap = tree_rows(p->max_pages, p->win_cap);
@@ -957,6 +970,10 @@ cudaError_t launch_tree(const DecodeArgs& d, const Dsv4HcaTreeDecodeParams* p, c
     e = make_q_map(&a.q_map, d.q, int64_t(d.B) * d.H, 576);
     if (e == cudaSuccess) e = make_tile_map(&a.k_map, u.rows, p->B * cap, kRowsPerBlock);
     if (e == cudaSuccess) e = make_tile_map(&a.v_map, u.rows, p->B * cap, kTileN);
+    if (e == cudaSuccess) e = make_out_map(&a.out_map, d.out, d.H, d.B);
+    // (how many slots a plan has is not known here: more than any memory holds)
+    if (e == cudaSuccess && sched != nullptr) e = make_out_map(&a.part_map, d.partial_o, kHeadsPerCta, int64_t(1) << 24);
+    else if (e == cudaSuccess && d.num_splits > 1) e = make_out_map(&a.part_map, d.partial_o, d.H, int64_t(d.num_splits) * d.B);
     if (e != cudaSuccess) return e;
     a.B = d.B;  a.H = d.H;  a.heads = d.tree_heads;  a.cap = int(cap);  a.mask_words = d.tree_words;  a.num_splits = d.num_splits;  a.scale_log2 = d.scale_log2;
     a.valid = u.valid;  a.kv_len = d.kv_len;  a.win_len = d.win_len;  a.tree_mask = d.tree_mask;  a.attn_sink = d.attn_sink;

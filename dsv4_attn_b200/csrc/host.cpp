@@ -512,6 +512,25 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor *po = nullptr, *pl = nullptr, *sched = nullptr;
     at::Tensor own_po, own_pl, own_sched;
     const int64_t groups = B * ((T * H + 127) / 128);
+    at::Tensor own_rows;
+    const at::Tensor* shared = nullptr;
+    const int64_t rows_bytes = lib.tree_rows_bytes(int(B), int(table->size(1)), int(W));
+    if (a[16] == Py_True || (a[16] == Py_None && groups >= kTreeShareGroups * B && groups * ((max_len + 63) / 64) >= kTreeShareTiles && rows_bytes > 0 && rows_bytes <= kTreeShareBytes)) {
+        if (rows_bytes <= 0) return none();
+        try {
+            own_rows = empty({rows_bytes}, at::kByte, q);
+            shared = &own_rows;
+        } catch (...) {
+            if (a[16] == Py_True) throw;                                   // without room for it the groups dequantise for themselves
+        }
+    } else if (a[16] != Py_None && a[16] != Py_False) {
+        shared = tensor(a[16], at::kByte, 1);
+        if (shared == nullptr || rows_bytes <= 0 || shared->numel() < rows_bytes) return none();
+    }
+    if (shared != nullptr) {
+        p.rows = ptr(shared);
+        p.rows_bytes = shared->numel();
+    }
     if (a[15] != Py_None) {                                                // a plan made before
         int64_t v[4];
         if (!PyTuple_Check(a[15]) || PyTuple_GET_SIZE(a[15]) != 8) return none();
@@ -535,7 +554,8 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
         p.sched_bytes = bytes;
         splits = 0;
     } else {
-        if (a[9] == Py_None) splits = lib.plan_splits(int(B), int(T * H), int(max_len), 0);
+        // (a row group for every pair, over shared rows: a second wave costs less than the partials of splits, 80 us against 95 for 92 ragged groups)
+        if (a[9] == Py_None) splits = shared != nullptr && groups >= 74 ? 1 : lib.plan_splits(int(B), int(T * H), int(max_len), 0);
         else if (!integer(a[9], &splits)) return none();
         if (splits < 1 || splits > DSV4_MAX_SPLITS) return none();
         if (a[12] != Py_None) {
@@ -548,25 +568,6 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
             own_pl = empty({splits * rows}, at::kFloat, q);
             po = &own_po;  pl = &own_pl;
         }
-    }
-    at::Tensor own_rows;
-    const at::Tensor* shared = nullptr;
-    const int64_t rows_bytes = lib.tree_rows_bytes(int(B), int(table->size(1)), int(W));
-    if (a[16] == Py_True || (a[16] == Py_None && groups >= kTreeShareGroups * B && groups * ((max_len + 63) / 64) >= kTreeShareTiles && rows_bytes > 0 && rows_bytes <= kTreeShareBytes)) {
-        if (rows_bytes <= 0) return none();
-        try {
-            own_rows = empty({rows_bytes}, at::kByte, q);
-            shared = &own_rows;
-        } catch (...) {
-            if (a[16] == Py_True) throw;                                   // without room for it the groups dequantise for themselves
-        }
-    } else if (a[16] != Py_None && a[16] != Py_False) {
-        shared = tensor(a[16], at::kByte, 1);
-        if (shared == nullptr || rows_bytes <= 0 || shared->numel() < rows_bytes) return none();
-    }
-    if (shared != nullptr) {
-        p.rows = ptr(shared);
-        p.rows_bytes = shared->numel();
     }
     Output out, lse;
     if (!out.take(a[10], at::kBFloat16, {B, T, H, kLatent}, q) || !lse.take(a[11], at::kFloat, {B, T, H}, q)) return none();

@@ -358,6 +358,17 @@ __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const void* tenso
         : "memory");
 }
 
+// Tiled 3-D store from this block's shared memory; what lies outside the tensor is left out (no coordinate may be negative).  The thread that issues it waits for
+// its groups: until they have been read (the shared memory is free), or written.
+__device__ __forceinline__ void tma_store_3d(const void* tensor_map, int x, int y, int z, uint32_t smem_src) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];\n\tcp.async.bulk.commit_group;"
+                 :
+                 : "l"(reinterpret_cast<uint64_t>(tensor_map)), "r"(x), "r"(y), "r"(z), "r"(smem_src)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tma_stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 // Four rows of a row-major tensor named by their numbers (tile::gather4; the map's box is one row high), laid down one
 // after the other at smem_dst, which is a multiple of 128 bytes.
 __device__ __forceinline__ void tma_gather4(uint32_t smem_dst, const void* tensor_map, int x, const int4& rows, uint32_t bar) {
@@ -424,11 +435,6 @@ __device__ __forceinline__ uint4 ldg_stream_v4(const void* p) {
     return v;
 }
 
-// 32 contiguous bytes, a whole sector of L2; p is a multiple of 32 bytes
-__device__ __forceinline__ void stg_v8(void* p, const uint32_t* v) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-                 : "memory");
-}
 __device__ __forceinline__ void prefetch_tensormap(const void* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 __device__ __forceinline__ void prefetch_l2(const void* p) {
     asm volatile("prefetch.global.L2 [%0];" ::"l"(p));

@@ -33,7 +33,7 @@ struct TreeUnpackArgs {
     int32_t* status;
 };
 
-// A block takes tiles of 64 entries, a warp four entries of one (with eight, two blocks of eight warps fitted an SM: 17 us for 30,000 entries, now %UNPACK%).  An entry: a lane has 16 latent bytes and their block's scale, eight lanes a piece of
+// A block takes tiles of 64 entries, a warp four entries of one (with eight, two blocks of eight warps fitted an SM: 17 us for 30,000 entries).  An entry: a lane has 16 latent bytes and their block's scale, eight lanes a piece of
 // the RoPE tail.  Rows that take no part (out of range, or window rows that no node sees) are zero: whatever probability they get is zero too,
 // and zero times what the memory held might not be.  DRAM-bound: 656 bytes read and 1152 written an entry.
 __global__ void __launch_bounds__(kUnpackThreads, 2) tree_unpack_kernel(const __grid_constant__ TreeUnpackArgs a) {
@@ -127,6 +127,8 @@ struct TreeArgs {
     alignas(64) CUtensorMap q_map;             // BF16 [B * H, 576], box 64 x 64
     alignas(64) CUtensorMap k_map;             // FP16 [B * cap, 576], box 64 columns x 32 rows
     alignas(64) CUtensorMap v_map;             // the same, 64 columns x 64 rows
+    alignas(64) CUtensorMap out_map;           // BF16 [B, H, 512], box 64 columns x 32 rows
+    alignas(64) CUtensorMap part_map;          // FP16 partials: [slots, 128, 512] with a plan, else [num_splits * B, H, 512]
     int B, H, heads;                           // H: (node, head) rows of a request
     int cap;                                   // rows per request in the workspace, a multiple of 64
     int mask_words;
@@ -169,7 +171,9 @@ struct TreeMisc {
     float inv[2][kHeadsPerBlock];    // per item, in turn: what the rows' outputs are multiplied by
     uint64_t bar_tmem;
     uint64_t bar_q_full[2];          // per item: chunks 0-5 / 6-8 of Q landed in the staging area
-    uint64_t bar_q_read[2];          // per item: they have been read there by every Q warp
+    uint64_t bar_q_read;             // per item: chunks 0-5 have been read there by every Q warp
+    uint64_t bar_q_placed;           // per item: 6-8 have been copied to their place by every Q warp
+    uint64_t bar_stage_free;         // per item: 6-8 have been, and the output of the item before has left it
     uint64_t bar_inv[2];             // per item, in turn: inv written (the softmax warps may finish the next item before the last Q warp comes to this)
     // signalled in both blocks by the commits of the MMA warps
     uint64_t bar_q_free;             // per item: its S MMAs complete
@@ -235,7 +239,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
         return it;
     };
 
-    const uint32_t bar_tmem = ptx::smem_u32(&misc->bar_tmem), bar_q_full = ptx::smem_u32(&misc->bar_q_full[0]), bar_q_read = ptx::smem_u32(&misc->bar_q_read[0]),
+    const uint32_t bar_tmem = ptx::smem_u32(&misc->bar_tmem), bar_q_full = ptx::smem_u32(&misc->bar_q_full[0]), bar_q_read = ptx::smem_u32(&misc->bar_q_read), bar_stage_free = ptx::smem_u32(&misc->bar_stage_free), bar_q_placed = ptx::smem_u32(&misc->bar_q_placed),
                    bar_q_free = ptx::smem_u32(&misc->bar_q_free), bar_o_last = ptx::smem_u32(&misc->bar_o_last), bar_inv = ptx::smem_u32(&misc->bar_inv[0]),
                    bar_o_read = ptx::smem_u32(&misc->bar_o_read),
                    bar_s_full = ptx::smem_u32(&misc->bar_s_full[0]), bar_o_full = ptx::smem_u32(&misc->bar_o_full[0]), bar_q_ready = ptx::smem_u32(&misc->bar_q_ready),
@@ -246,12 +250,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
     };
 
     // ── set-up ──
-    if (warp == kTreeVWarp && lane == 0) { ptx::prefetch_tensormap(&a.q_map);  ptx::prefetch_tensormap(&a.k_map);  ptx::prefetch_tensormap(&a.v_map); }
+    if (warp == kTreeVWarp && lane == 0) { ptx::prefetch_tensormap(&a.out_map);  ptx::prefetch_tensormap(&a.q_map);  ptx::prefetch_tensormap(&a.k_map);  ptx::prefetch_tensormap(&a.v_map); }
     if (tid == 0) {
         ptx::sts_u32(failed_flag(), 0u);
         ptx::mbar_init(bar_tmem, 1);
         ptx::mbar_init(bar_q_read, kTreeQWarps);
-        ptx::mbar_init(bar_q_read + 8, kTreeQWarps);
+        ptx::mbar_init(bar_stage_free, kTreeQWarps);
+        ptx::mbar_init(bar_q_placed, kTreeQWarps);
         ptx::mbar_init(bar_q_free, 1);
         ptx::mbar_init(bar_o_last, 1);
         ptx::mbar_init(bar_inv, kNumSoftmaxWarps);
@@ -301,18 +306,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
         uint32_t qn = 0;
         Item last{};                                   // the item whose output is to be written
         auto write_out = [&]() -> bool {
-            // row r of this block, value columns [256 half + 128 (qw / 4), +128): 32 at a time, 64 bytes of 16-bit values
-            const int r = (qw & 1) * 32 + lane, half = (qw >> 1) & 1;
-            const int h0 = last.hg * kHeadsPerCta + rank * kHeadsPerBlock;
+            // 32 rows of this block, value columns [256 half + 128 (qw / 4), +128): 64 columns at a time through this warp's 4 KB of the staging area, and from there
+            // by TMA, which leaves the rows past the last one out.  (Stored from registers, 32 bytes a row and lane, they kept the load/store unit busy
+            // for 3,000 cycles, in which the MMAs did not get at their operands: 1,950 cycles a tile over items of 15, now 1,790.)
+            const int row0 = rank * kHeadsPerBlock + (qw & 1) * 32, half = (qw >> 1) & 1, r = (qw & 1) * 32 + lane;
             const bool final_out = last.slot < 0;
             if (!wait_for(bar_inv + 8 * ((qn - 1u) & 1u), (qn - 1u) >> 1, kStatusWaitOFull, 2, 0) || !wait_for(bar_o_last, qn - 1u, kStatusWaitOFull, 2, 0)) return false;
             ptx::tc_fence_after_sync();
             const float inv = misc->inv[(qn - 1u) & 1u][r];
-            const int64_t prow0 = final_out ? 0 : (sched ? int64_t(last.slot) * kHeadsPerCta + rank * kHeadsPerBlock : (int64_t(last.slot) * a.B + last.n) * a.H + h0);
-            __nv_bfloat16* const row = (final_out ? a.out + (int64_t(last.n) * a.H + h0) * 512 : reinterpret_cast<__nv_bfloat16*>(a.partial_o) + prow0 * 512) + int64_t(r) * 512 +
-                                       256 * half + 128 * (qw >> 2);
-            const bool whole_sectors = (reinterpret_cast<uintptr_t>(row) & 31u) == 0u;      // (the caller's tensors are aligned to 16 bytes)
             const uint32_t from = tmem + (uint32_t((qw & 3) * 32) << 16) + kTmemO + 128u * uint32_t(qw >> 2);
+            const uint32_t box = q_stage + uint32_t(qw) * 4096u, line = box + uint32_t(lane) * 128u, sw = uint32_t(lane & 7) << 4;
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
                 uint32_t o[32];
@@ -323,21 +326,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
                     __syncwarp();
                     if (lane == 0) arrive_even(bar_o_read);
                 }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float x = __uint_as_float(o[2 * i]) * inv, y = __uint_as_float(o[2 * i + 1]) * inv;
-                    o[i] = final_out ? ptx::pack_bf16x2(x, y) : ptx::pack_f16x2(x, y);
+                if (c == 2) {                          // the first half has left
+                    if (lane == 0) ptx::tma_stores_read();
+                    __syncwarp();
                 }
-                if (h0 + r < a.H) {
-                    if (whole_sectors) {
-                        ptx::stg_v8(row + 32 * c, o);
-                        ptx::stg_v8(row + 32 * c + 16, o + 8);
-                    } else {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(row + 32 * c)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float x = __uint_as_float(o[8 * i + 2 * j]) * inv, y = __uint_as_float(o[8 * i + 2 * j + 1]) * inv;
+                        w[j] = final_out ? ptx::pack_bf16x2(x, y) : ptx::pack_f16x2(x, y);
                     }
+                    ptx::sts_v4(line + ((uint32_t(4 * (c & 1) + i) << 4) ^ sw), make_uint4(w[0], w[1], w[2], w[3]));
+                }
+                if (c & 1) {
+                    ptx::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        const int x = 256 * half + 128 * (qw >> 2) + 32 * (c - 1);
+                        if (final_out) ptx::tma_store_3d(&a.out_map, x, last.hg * kHeadsPerCta + row0, last.n, box);
+                        else if (sched) ptx::tma_store_3d(&a.part_map, x, row0, last.slot, box);
+                        else ptx::tma_store_3d(&a.part_map, x, last.hg * kHeadsPerCta + row0, last.slot * a.B + last.n, box);
+                    }
+                    __syncwarp();
                 }
             }
+            if (lane == 0) ptx::tma_stores_read();
+            __syncwarp();
             return true;
         };
 #pragma unroll 1
@@ -381,13 +397,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
             __syncwarp();
             if (lane == 0) {
                 arrive_even(bar_q_ready);
-                ptx::mbar_arrive(bar_q_read + 8);
+                ptx::mbar_arrive(bar_q_placed);
             }
-            if (qn > 0u && !write_out()) { ok = false;  break; }
+            // (the output goes through the staging area, which the other Q warps may still be reading)
+            if (qn > 0u && (!wait_for(bar_q_placed, qn, kStatusWaitQ, 2, k) || !write_out())) { ok = false;  break; }
+            if (lane == 0) ptx::mbar_arrive(bar_stage_free);
             last = it;
             ++qn;
         }
         if (ok && qn > 0u) write_out();
+        if (lane == 0) ptx::tma_stores_done();
         __syncwarp();
     } else if (warp == kTreeKWarp) {
         // ───────────── K tiles: both blocks' copies report to the even one, which expects the bytes of both ─────────────
@@ -457,12 +476,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
                     for (int c = 0; c < 4; ++c) ptx::tma_load_2d_pair(v_base + buf * L::kVBytes + c * kVChunkBytes, &a.v_map, rank * 256 + c * 64, row, v_full + 8 * buf);
                 }
                 __syncwarp();
-                // (by the third tile this item's Q is in place, by the sixth the Q warps have written the output of the one before)
-                if (i == min(it.ntiles - 1, 2) && k2 < n_items) {
-                    if (!wait_for(bar_q_read + 8, qn, kStatusWaitQ, 5, k)) { ok = false;  break; }
+                // (by the fifth tile this item's Q is in place, and the output of the one before has left the staging area)
+                if (i == min(it.ntiles - 1, 4) && k2 < n_items) {
+                    if (!wait_for(bar_stage_free, qn, kStatusWaitQ, 5, k)) { ok = false;  break; }
                     send_q(next, 0);
                 }
-                if (i == min(it.ntiles - 1, 5) && k2 < n_items) {
+                if (i == min(it.ntiles - 1, 7) && k2 < n_items) {
                     if (!wait_for(bar_q_read, qn + 1u, kStatusWaitQ, 5, k)) { ok = false;  break; }
                     send_q(next, 1);
                 }
