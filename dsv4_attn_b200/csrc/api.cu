@@ -9,9 +9,6 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <cmath>
-#ifdef PROBE
-#include <cstdlib>
-#endif
 #include <cstring>
 #include <atomic>
 
@@ -1128,9 +1125,6 @@ cudaError_t launch_sample(SampleArgs& a, cudaStream_t stream) {
     int blocks = 1;
     auto terms = [&] { return (steps + blocks * kSampleWarps - 1) / (blocks * kSampleWarps) * (kSampleStep / 32); };
     while (blocks < kSampleMaxCluster && ((int64_t(a.N) * blocks <= device_sms() && span > blocks * 4096) || terms() > kSampleMostTerms)) blocks *= 2;
-#ifdef PROBE
-    if (getenv("PB")) blocks = atoi(getenv("PB"));
-#endif
     static std::atomic<bool> done[kMaxDevices];
     const cudaError_t e = ensure_smem(sample_kernel<T>, int(sizeof(SampleShared)), done);
     if (e != cudaSuccess) return e;

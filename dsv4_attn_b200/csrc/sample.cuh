@@ -41,6 +41,7 @@ constexpr int kSampleBins = 4096;                // of the histogram over (l_max
 constexpr float kSampleBin = 128.f;              // 1/128 each
 constexpr uint32_t kSampleSpare = 200;           // candidates next to the bin of a cut
 constexpr int kSampleQuarters = 4;               // a thread knows the largest logit of each quarter of its own
+constexpr int kSampleValues = 128;               // different logits, of sixteen bits, that may be near a cut
 constexpr int kSampleMostTerms = 4095;           // of a FixedSum
 
 struct SampleArgs {
@@ -78,6 +79,8 @@ struct SampleShared {
     float warp_max[kSampleWarps];
     uint32_t digit, count;
     int bin;
+    float place;                                                 // where in that bin the cut should be
+    float by_min_p;                                              // what lies above the logit that min-p asks for, by the histogram
     // the cut, from the first block to all
     uint32_t cut, kept, reached;                                 // reached: all of what was wanted lies up to it
     unsigned long long cut_ties;
@@ -250,6 +253,8 @@ struct LogitRow {
     // two 16-bit logits, or one of 32 bits
     struct Pair { uint32_t bits; };
     static __device__ __forceinline__ Pair none() { return {sizeof(T) == 4 ? 0xFF800000u : (sizeof(T) == 2 && is_bf16() ? 0xFF80FF80u : 0xFC00FC00u)}; }
+    // Sixteen-bit logits: the bits of their keys from this one on say all.
+    static constexpr int kKeyShift = std::is_same<T, __nv_bfloat16>::value ? 16 : 13;
     static __host__ __device__ constexpr bool is_bf16() { return std::is_same<T, __nv_bfloat16>::value; }
     static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
         uint32_t r;
@@ -865,11 +870,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         }
     }
     if (!have_cut) {
+        // min-p keeps all of what a cut keeps (with room for the rounding of expf)
+        auto min_p_idle = [&](uint32_t key) { return r.min_p == 0.f || r.ratio(key_value(key)) >= r.min_p * 1.0001f; };
         // The cut up to which `wanted` lies, among the finite logits above `above` (a key): tokens, or weight, of which `wanted` is then the share that
         // top-p says of all of it and of `ties`, the weight of the tokens kept at `above`.  False: it lies beyond (in the ties; no cut at all).
-        auto find_cut = [&](auto weights, uint32_t above, unsigned long long wanted, unsigned long long ties, unsigned long long& over) -> bool {
-            constexpr bool BY_WEIGHT = decltype(weights)::value, by_weight = BY_WEIGHT;
-            const float above_value = above != 0u ? key_value(above) : -CUDART_INF_F;
+        auto find_cut = [&](auto weights, auto limited, uint32_t above, unsigned long long wanted, unsigned long long ties, unsigned long long& over) -> bool {
+            constexpr bool BY_WEIGHT = decltype(weights)::value, by_weight = BY_WEIGHT, LIMITED = decltype(limited)::value;
+            constexpr bool all_in = BY_WEIGHT && !LIMITED;                         // (-inf weighs nothing)
+            const float above_value = LIMITED ? key_value(above) : -CUDART_INF_F;
             for (int i = tid; i < kSampleBins; i += kSampleThreads) sh.bins[i] = 0u;
             __syncthreads();
             // Bin of a logit: 1, its distance in bins and `off`, rounded to a whole number by the addition of 2^23.  (Near enough: what is decided
@@ -879,7 +887,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const uint32_t bin = __float_as_uint(fminf(fmaf(v[i], slope, offset), 8388608.f + kSampleBins - 1)) & (kSampleBins - 1);
-                    if (v[i] > above_value && bin < kSampleBins - 1) atomicAdd(&sh.bins[bin], 1u);
+                    if ((!LIMITED || v[i] > above_value) && bin < kSampleBins - 1) atomicAdd(&sh.bins[bin], 1u);
                 }
             });
             sync_row(blocks);
@@ -916,7 +924,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                     const uint32_t z = __shfl_up_sync(0xFFFFFFFFu, n_upto, o);
                     if (lane >= o) { upto += y;  n_upto += z; }
                 }
-                if (tid == 0) sh.bin = kSampleBins - 1;
+                if (tid == 0) { sh.bin = kSampleBins - 1;  sh.by_min_p = CUDART_INF_F;  sh.place = 0.5f; }
                 if (lane == 31) { sh.warp_max[warp] = upto;  sh.warp_x[warp] = n_upto; }
                 __syncthreads();
                 float before = upto - mine_sum, total = 0.f;
@@ -926,20 +934,34 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                     total += sh.warp_max[w];
                 }
                 // (ties: in units of the largest weight)
+                // (min-p: the bin of the smallest weight it keeps, and two for rounding)
+                const int floor_bin = by_weight && !LIMITED && r.min_p > 0.f ? int(-kSampleBin * logf(r.min_p)) + 3 : kSampleBins;
                 const float goal = by_weight ? float(r.p24) * 5.9604645e-8f * (total + __ull2float_rn(ties) * 9.094947e-13f) : float(wanted);
+                float place = 0.5f;
+                int crossed = -1;
 #pragma unroll
                 for (int i = 0; i < kPer; ++i) {
                     const int bin = kPer * tid + i;
                     const float v = by_weight ? float(c[i]) * __expf(float(1 - bin) / kSampleBin) : float(c[i]);
-                    if (before < goal && before + v >= goal) atomicMin(&sh.bin, bin);
+                    if (before < goal && before + v >= goal && crossed < 0) {
+                        atomicMin(&sh.bin, bin);
+                        crossed = bin;
+                        place = (goal - before) / v;
+                    }
                     before += v;
+                    if (bin == floor_bin) sh.by_min_p = before;
                     counts[bin] = n_before += c[i];
                 }
                 __syncthreads();
+                if (crossed == sh.bin) sh.place = place;
+                // Where all that min-p keeps weighs clearly less than top-p's share, top-p leaves out none of it: no cut.  A bin's tokens are within one bin of
+                // it (as long as 2^23 and their distance add up exactly), which is 0.8% of their weight.
+                if (sh.by_min_p * 1.03f < goal && fabsf(slope * r.top) < 1e6f) { over = 0ull;  return true; }
             }
             // That bin, one and a quarter each way, and as far each way as there are not more than kSampleSpare tokens: where they are few, rounding
             // moves the cut from one to the next, bins away.
             int low = 0, high = kSampleBins - 1;
+            float half_width = 0.f;
             {
                 const int bin = sh.bin;
                 const uint32_t left = bin > 0 ? counts[bin - 1] : 0u, right = counts[bin];
@@ -955,10 +977,19 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                 }
                 low = min(low, bin);
                 high = max(high, bin);
+                // Where they are many, and spread evenly (32-bit logits), less will do, around the place in the bin: what an estimate from counts is off by there
+                // is a small part of a bin.
+                const uint32_t near = counts[min(bin + 1, kSampleBins - 1)] - (bin > 1 ? counts[bin - 2] : 0u);
+                if (sizeof(T) == 4 && near > uint32_t(kSampleList) / 2) half_width = fmaxf(1.5f * float(kSampleList / 4) / float(near), 0.05f);
             }
             __syncthreads();                       // (the counts lie where the candidates will be sorted)
             // Exactly: what all weigh, what lies nearer than `from`, and the candidates from there to `to`.
             float from = fminf(float(low - 1) - off - 0.5f, float(sh.bin - 1) - off - 1.25f), to = fmaxf(float(high - 1) - off + 0.5f, float(sh.bin - 1) - off + 1.25f);
+            if (half_width > 0.f) {
+                from = float(sh.bin - 1) - off + sh.place - 0.5f - half_width;
+                to = from + 2.f * half_width;
+            }
+            const float next = half_width > 0.f ? 2.f * half_width : 2.5f;
             unsigned long long ahead;
             for (int moved = 0, tries = 0;; ++tries) {
                 // (a few steps the same way: all the way; and what is not a number, with infinite logits, is everything)
@@ -975,13 +1006,21 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                 // (candidates are within `near` of `mid`, a little more than they need to be; where that is not a number, any may be one)
                 const float mid = r.top + 0.5f * (x_from + x_to) / r.per, near_by = 0.5001f * (x_from - x_to) / r.per + 1e-6f * (fabsf(r.top) + fabsf(mid));
                 const bool may_be = !(near_by < CUDART_INF_F) || !(fabsf(mid) < CUDART_INF_F);
+                // Logits of sixteen bits: there are few different ones there, equal ones by the hundred, and instead of a list to be sorted every warp has a
+                // table of how often it meets each.
+                uint32_t* const table = reinterpret_cast<uint32_t*>(sh.list) + warp * kSampleValues;
+                const uint32_t top_value = (order_key(mid + near_by) >> row.kKeyShift) + 1u;
+                const bool by_value = sizeof(T) == 2 && !may_be && top_value - (order_key(mid - near_by) >> row.kKeyShift) < uint32_t(kSampleValues - 1);
+                if (by_value)
+                    for (int i = lane; i < kSampleValues; i += 32) table[i] = 0u;
+                __syncwarp();
                 row.each(first, steps, [&](const float (&v)[8], int e) {
                     float off = CUDART_INF_F;
 #pragma unroll
                     for (int i = 0; i < 8; i += 2) {
                         float x0, x1;
                         r.exponents(v[i], v[i + 1], x0, x1);
-                        const bool in0 = v[i] > above_value, in1 = v[i + 1] > above_value, ahead0 = in0 && x0 > x_from, ahead1 = in1 && x1 > x_from;
+                        const bool in0 = all_in || v[i] > above_value, in1 = all_in || v[i + 1] > above_value, ahead0 = in0 && x0 > x_from, ahead1 = in1 && x1 > x_from;
                         if constexpr (BY_WEIGHT) {
                             sum_all.add2(in0 ? expf(x0) : 0.f, in1 ? expf(x1) : 0.f, &sum_ahead, ahead0, ahead1);
                         } else {
@@ -994,25 +1033,95 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
                             const float x = r.exponent(v[i]);
-                            if (v[i] > above_value && !(x > x_from) && x > x_to) list_logit(sh, v[i], e + i - row.lead);
+                            if (v[i] > above_value && !(x > x_from) && x > x_to) {
+                                if (by_value) atomicAdd(&table[min(top_value - (order_key(v[i] + 0.f) >> row.kKeyShift), uint32_t(kSampleValues - 1))], 1u);
+                                else list_logit(sh, v[i], e + i - row.lead);
+                            }
                         }
                     }
                 });
                 over = by_weight ? sum_all.total() : n_all;
                 ahead = by_weight ? sum_ahead.total() : n_ahead;
-                if (by_weight) {                   // (per warp, for the token, where this turns out to be the cut)
-                    const unsigned long long of_warp = warp_total(ahead);
-                    if (lane < int(blocks)) sts_cluster_u64(ptx::mapa(ptx::smem_u32(&sh.sum[me]), lane), of_warp);
+                const unsigned long long of_warp = warp_total(ahead);
+                // (per warp, for the token, where this turns out to be the cut)
+                if (by_weight && lane < int(blocks)) sts_cluster_u64(ptx::mapa(ptx::smem_u32(&sh.sum[me]), lane), of_warp);
+                uint32_t* const values = sh.bins + (turn ^ 1) * kSampleValues;         // (in turn, as in row_totals)
+                if (by_value) {
+                    __syncthreads();
+                    if (tid < kSampleValues) {
+                        uint32_t c = 0;
+                        for (int w = 0; w < kSampleWarps; ++w) c += reinterpret_cast<const uint32_t*>(sh.list)[w * kSampleValues + tid];
+                        values[tid] = c;
+                    }
                 }
                 row_totals(sh, blocks, rank, turn, over, ahead);
                 if (by_weight) wanted = max(share_of(over + ties, uint32_t(r.p24)), 1ull);
                 if (wanted > over) { over = wanted - over;  return false; }
-                if (wanted <= ahead) { to = from;  from -= 2.5f;  moved = -1;  continue; }
+                if (wanted <= ahead) { to = from;  from -= next;  moved = -1;  continue; }
+                if (by_value) {
+                    // Every warp for itself: four neighbouring values a lane, the largest first.
+                    constexpr int kPer = kSampleValues / 32;
+                    uint32_t* const all = sh.bins + 2 * kSampleValues;
+                    if (tid < kSampleValues) {
+                        uint32_t c = 0;
+                        for (uint32_t b = 0; b < blocks; ++b) c += ptx::lds_cluster_u32(ptx::mapa(ptx::smem_u32(values + tid), b));
+                        all[tid] = c;
+                    }
+                    __syncthreads();
+                    auto key_of = [&](int i) {
+                        const uint32_t q = (top_value - uint32_t(i)) << row.kKeyShift;
+                        return (q >> 31) ? q : q | ((1u << row.kKeyShift) - 1u);
+                    };
+                    unsigned long long each[kPer], mine_sum = 0;
+#pragma unroll
+                    for (int i = 0; i < kPer; ++i) {
+                        each[i] = !by_weight ? 1ull : all[kPer * lane + i] != 0u ? fixed(r.ratio(key_value(key_of(kPer * lane + i)))) : 0ull;
+                        mine_sum += all[kPer * lane + i] * each[i];
+                    }
+                    const unsigned long long upto = warp_upto(mine_sum, lane), want = wanted - ahead;
+                    unsigned long long before = upto - mine_sum, ties_there = 0, my_sum = 0;
+                    const uint32_t hit = __ballot_sync(0xFFFFFFFFu, upto >= want);
+                    if (hit != 0u) {
+                        int at = 0;
+                        bool done = false;
+#pragma unroll
+                        for (int i = 0; i < kPer; ++i) {
+                            const unsigned long long v = all[kPer * lane + i] * each[i];
+                            if (!done && before + v >= want) {
+                                at = kPer * lane + i;
+                                ties_there = (want - before + each[i] - 1ull) / max(each[i], 1ull);
+                                done = true;
+                            }
+                            before += v;
+                        }
+                        const int from_lane = __ffs(hit) - 1;
+                        at = __shfl_sync(0xFFFFFFFFu, at, from_lane);
+                        cut = key_of(at);
+                        cut_ties = __shfl_sync(0xFFFFFFFFu, ties_there, from_lane);
+                        if (by_weight && min_p_idle(cut)) {
+                            // what this warp has above the cut, and at it
+#pragma unroll
+                            for (int i = 0; i < kPer; ++i) my_sum += kPer * lane + i < at ? table[kPer * lane + i] * each[i] : 0ull;
+                            my_sum = warp_total(my_sum) + of_warp;
+                            if (lane < int(blocks)) {
+                                sts_cluster_u64(ptx::mapa(ptx::smem_u32(&sh.sum[me]), lane), my_sum);
+                                ptx::sts_cluster_u32(ptx::mapa(ptx::smem_u32(&sh.ties[me]), lane), table[at]);
+                            }
+                            sums_known = true;
+                        }
+                        if (!by_weight) sync_row(blocks);              // (the bins are cleared next)
+                        return true;
+                    }
+                    from = to;                     // (a little further away)
+                    to += next;
+                    moved = 1;
+                    continue;
+                }
                 const int m = listed(sh, blocks, turn);
                 if (m >= 0 && (by_weight || wanted - ahead <= static_cast<unsigned long long>(m))) {
                     if (rank == 0) {
                         cut_of_list(sh, r, blocks, turn, m, by_weight ? m : int(wanted - ahead), by_weight ? wanted - ahead : ~0ull);
-                        if (by_weight && r.min_p == 0.f && sh.reached) {
+                        if (by_weight && sh.reached && min_p_idle(sh.cut)) {
                             // what the candidates above the cut add to their warps' sums, and the ties; to all blocks
                             if (tid < parts) sh.ties[tid] = 0u;
                             __syncthreads();
@@ -1035,7 +1144,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                     if (sh.reached) {
                         cut = sh.cut;
                         cut_ties = sh.cut_ties;
-                        sums_known = by_weight && r.min_p == 0.f;
+                        sums_known = by_weight && min_p_idle(cut);
                         return true;
                     }
                 }
@@ -1057,7 +1166,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                     if (wanted <= upto) break;
                 }
                 from = to;
-                to += 2.5f;
+                to += next;
                 moved = 1;
             }
             wanted -= ahead;
@@ -1101,11 +1210,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
             return true;
         };
         unsigned long long beyond;
-        if (r.k > 0) find_cut(std::false_type{}, 0u, static_cast<unsigned long long>(r.k), 0ull, beyond);
+        if (r.k > 0) find_cut(std::false_type{}, std::false_type{}, 0u, static_cast<unsigned long long>(r.k), 0ull, beyond);
         if (r.p24 >= 0) {
             // top-p looks at the tokens above top-k's cut, and at those of its ties that are kept
             const unsigned long long tie = cut_ties != 0ull ? fixed(r.ratio(key_value(cut))) : 0ull;
-            if (!find_cut(std::true_type{}, cut, 0ull, cut_ties * tie, beyond)) cut_ties = min(cut_ties, (beyond + tie - 1ull) / tie);
+            if (r.k == 0 || cut_ties == 0ull) find_cut(std::true_type{}, std::false_type{}, 0u, 0ull, 0ull, beyond);
+            else if (!find_cut(std::true_type{}, std::true_type{}, cut, 0ull, cut_ties * tie, beyond)) cut_ties = min(cut_ties, (beyond + tie - 1ull) / tie);
         }
     }
 

@@ -145,6 +145,46 @@ def test_ties(lib, V):
         check(lib.sample(logits, u, **s), want(logits, u, **s))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("N,V", [(1, 40000), (5, 200001), (20, 262144), (150, 60000)])
+@pytest.mark.parametrize("spread", [0.02, 0.5, 1.0])
+def test_many_tokens_near_the_cut(lib, N, V, dtype, spread):
+    """Flat rows, whose cuts lie among thousands of nearly equal logits (in 16 bits, of equal ones); a third of the 32-bit rows are such of 16 bits."""
+    logits, u, g = rows(N + V, N, V, dtype, spread)
+    if dtype == torch.float32:
+        logits[::3] = logits[::3].bfloat16().float()
+    s = dict(temperature=0.5 + torch.rand(N, device="cuda", generator=g), top_p=0.2 + 0.79 * torch.rand(N, device="cuda", generator=g),
+             top_k=torch.randint(3000, 30000, (N,), device="cuda", generator=g, dtype=torch.int32))
+    s["top_k"][::2] = 0
+    check(lib.sample(logits, u, **s), want(logits, u, **s))
+    s.pop("top_p")
+    check(lib.sample(logits, u, **s), want(logits, u, **s))
+
+
+@pytest.mark.parametrize("N,V", [(64, 3000), (64, 70000)])
+def test_min_p_on_both_sides_of_the_cut(lib, N, V):
+    """min-p thresholds that are far above the cut of top-p, far below it, and within parts in a thousand of it."""
+    logits, u, g = rows(V, N, V, torch.float32, 1.5)
+    top_p = 0.3 + 0.65 * torch.rand(N, device="cuda", generator=g)
+    e = torch.exp((logits - logits.amax(1, keepdim=True)).double()).sort(1, descending=True).values
+    at_cut = e.gather(1, ((e.cumsum(1) < top_p[:, None] * e.sum(1, keepdim=True)).sum(1, keepdim=True)).clamp(max=V - 1))[:, 0]
+    factor = torch.tensor([0.01, 0.5, 0.97, 0.999, 0.9999, 1.0, 1.0001, 1.001, 1.03, 2.0, 1e-30, 30.0, 0.99, 1.01, 1.02, 0.98], device="cuda").repeat(N // 16)
+    min_p = (at_cut * factor).float()
+    for t in (None, torch.ones(N, device="cuda")):
+        check(lib.sample(logits, u, temperature=t, top_p=top_p, min_p=min_p), want(logits, u, t, None, top_p, min_p))
+
+
+@pytest.mark.parametrize("t", [1e-30, 1e-6, 1e-4, 1e4, 1e30])
+def test_temperatures_far_from_one(lib, t):
+    N, V = 6, 30000
+    logits, u, g = rows(11, N, V, torch.float32)
+    logits += torch.tensor([0.0, 1e4, -1e4, 1.0, 100.0, -100.0], device="cuda")[:, None]
+    s = dict(temperature=torch.full((N,), t, device="cuda"), top_p=torch.tensor([0.5, 0.9, 0.99, 0.9, 0.9, 0.1], device="cuda"))
+    check(lib.sample(logits, u, **s), want(logits, u, **s))
+    s["min_p"] = torch.tensor([0.1, 0.9, 1e-3, 0.5, 0.999, 0.01], device="cuda")
+    check(lib.sample(logits, u, **s), want(logits, u, **s))
+
+
 def test_masked_infinite_and_nan_logits(lib):
     V = 9000
     logits, u, _ = rows(5, 12, V, torch.float32)
