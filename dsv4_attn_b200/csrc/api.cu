@@ -960,8 +960,8 @@ cudaError_t launch_tree(const DecodeArgs& d, const Dsv4HcaTreeDecodeParams* p, c
     u.rows = static_cast<uint8_t*>(p->rows);
     u.valid = reinterpret_cast<uint32_t*>(u.rows + p->B * cap * 1152);
     u.status = d.status;
-    const int64_t tiles = p->B * (cap / kTileN), resident = int64_t(device_sms()) * 8;
-    cudaError_t e = launch(tree_unpack_kernel, dim3(unsigned(tiles < resident ? tiles : resident)), kUnpackThreads, 0, stream, u);
+    const int64_t unpack = (p->B * cap / kUnpackEach + kUnpackThreads / 32 - 1) / (kUnpackThreads / 32), resident = int64_t(device_sms()) * 2;
+    cudaError_t e = launch(tree_unpack_kernel, dim3(unsigned(unpack < resident ? unpack : resident)), kUnpackThreads, 0, stream, u);
     if (e != cudaSuccess) return e;
     TreeArgs a{};
     e = make_q_map(&a.q_map, d.q, int64_t(d.B) * d.H, 576);
@@ -1015,8 +1015,8 @@ extern "C" int dsv4_hca_tree_decode_fwd(const Dsv4HcaTreeDecodeParams* p, void* 
     if (!aligned(p->kv_pool, 16) || !aligned(p->win_pool, 16)) return int(cudaErrorInvalidValue);
     if (p->rows != nullptr) {
         const int64_t bytes = dsv4_hca_tree_rows_bytes(p->B, p->max_pages, p->win_cap);
-        if (bytes <= 0 || p->rows_bytes < bytes || !aligned(p->rows, 16)) {
-            t_last_error = "workspace smaller than dsv4_hca_tree_rows_bytes() for this shape";
+        if (bytes <= 0 || p->rows_bytes < bytes || !aligned(p->rows, 32)) {
+            t_last_error = "workspace smaller than dsv4_hca_tree_rows_bytes() for this shape, or not on a 32-byte boundary";
             return int(cudaErrorInvalidValue);
         }
     }

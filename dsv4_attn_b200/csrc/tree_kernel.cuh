@@ -18,6 +18,7 @@
 namespace dsv4 {
 
 constexpr int kUnpackThreads = 512;
+constexpr int kUnpackEach = 8;                 // entries of a warp
 
 struct TreeUnpackArgs {
     int B, T, max_pages, win_cap, mask_words, cap;
@@ -33,28 +34,27 @@ struct TreeUnpackArgs {
     int32_t* status;
 };
 
-// A block takes tiles of 64 entries, a warp four entries of one (with eight, two blocks of eight warps fitted an SM: 17 us for 30,000 entries).  An entry: a lane has 16 latent bytes and their block's scale, eight lanes a piece of
-// the RoPE tail.  Rows that take no part (out of range, or window rows that no node sees) are zero: whatever probability they get is zero too,
-// and zero times what the memory held might not be.  DRAM-bound: 656 bytes read and 1152 written an entry.
+// A warp takes eight entries at a time and has all of their bytes on the way at once; a lane has 16 latent bytes of each and their block's scale, and a piece
+// of two of the RoPE tails.  Rows that take no part (out of range, or window rows that no node sees) are zero: whatever probability they get is zero too,
+// and zero times what the memory held might not be.  Bound by the chain
+// of its loads (lengths and page, record) and by memory, 656 bytes read and 1152 written an entry: 51,000 entries in 20 us, 23 with four entries a warp and
+// blocks that met for the bits of a tile.
 __global__ void __launch_bounds__(kUnpackThreads, 2) tree_unpack_kernel(const __grid_constant__ TreeUnpackArgs a) {
-    constexpr int kEach = 4;
-    __shared__ uint32_t s_valid[kTileN / kEach];
+    constexpr int kEach = kUnpackEach, kParts = kTileN / kEach;
     ptx::pdl_trigger();
     ptx::pdl_wait();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int tiles = a.cap / kTileN;
-    for (int64_t u = blockIdx.x; u < int64_t(a.B) * tiles; u += gridDim.x) {
-        const int b = int(u / tiles), v0 = int(u % tiles) * kTileN;
+    const int lane = threadIdx.x & 31, tiles = a.cap / kTileN, units = a.B * tiles * kParts;
+    for (int u = (blockIdx.x * kUnpackThreads + threadIdx.x) >> 5; u < units; u += gridDim.x * (kUnpackThreads / 32)) {
+        const int b = u / (tiles * kParts), v0 = (u - b * tiles * kParts) * kEach;
+        // where the warp's entries live (lane i: entry i)
+        const int v = v0 + (lane & (kEach - 1)), slot = v >> 6, page = slot < a.max_pages ? ptx::ld(a.block_table + int64_t(b) * a.max_pages + slot) : -1;
         const int kv_len = max(ptx::ld(a.kv_len + b), 0), win_len = max(ptx::ld(a.win_len + b), 0);
         const int64_t n_tok = int64_t(kv_len) + win_len;
-        if (v0 == 0 && n_tok > a.cap && threadIdx.x == 0) report_status(a.status, kStatusBadIndex, 4, kv_len);
-        if (v0 >= n_tok) continue;
-        // where the warp's entries live (lane i: entry i)
+        if (v0 == 0 && n_tok > a.cap && lane == 0) report_status(a.status, kStatusBadIndex, 4, kv_len);
+        if (v0 / kTileN * kTileN >= n_tok) continue;
         const uint8_t* rec = nullptr;
-        const int v = v0 + warp * kEach + (lane & (kEach - 1));
         if (v < n_tok) {
             if (v < kv_len) {
-                const int slot = v >> 6, page = slot < a.max_pages ? ptx::ld(a.block_table + int64_t(b) * a.max_pages + slot) : -1;
                 if (page >= 0 && page < a.num_pages) rec = a.kv_pool + (int64_t(page) * 64 + (v & 63)) * 656;
                 else if (lane < kEach) report_status(a.status, kStatusBadIndex, 4, slot < a.max_pages ? page : v);
             } else if (v - kv_len < a.win_cap) {
@@ -63,54 +63,54 @@ __global__ void __launch_bounds__(kUnpackThreads, 2) tree_unpack_kernel(const __
                 report_status(a.status, kStatusBadIndex, 4, v);
             }
         }
-        if (v0 + kTileN > kv_len) {
-            // (a tile with window rows) the rows that any node sees
-#pragma unroll 1
-            for (int i = 0; i < kEach; ++i) {
-                const int w = v0 + warp * kEach + i - kv_len;
-                if (w < 0) continue;
-                uint32_t any = 0u;
-                if ((w >> 5) < a.mask_words)
-                    for (int t = lane; t < a.T; t += 32) any |= uint32_t(ptx::ld(a.tree_mask + (int64_t(b) * a.T + t) * a.mask_words + (w >> 5)));
-                if (!__any_sync(0xFFFFFFFFu, (any >> (w & 31)) & 1u) && (lane & (kEach - 1)) == i) rec = nullptr;
+        if (v0 + kEach > kv_len) {
+            // (window rows among them) the rows that any node sees: their bits lie in two words at most
+            const int w0 = max(v0 - kv_len, 0) >> 5;
+            uint32_t any0 = 0u, any1 = 0u;
+            for (int t = lane; t < a.T; t += 32) {
+                const int32_t* words = a.tree_mask + (int64_t(b) * a.T + t) * a.mask_words;
+                if (w0 < a.mask_words) any0 |= uint32_t(ptx::ld(words + w0));
+                if (w0 + 1 < a.mask_words) any1 |= uint32_t(ptx::ld(words + w0 + 1));
             }
+            any0 = __reduce_or_sync(0xFFFFFFFFu, any0);
+            any1 = __reduce_or_sync(0xFFFFFFFFu, any1);
+            const int w = v - kv_len;
+            if (w >= 0 && !(((w >> 5) == w0 ? any0 : any1) >> (w & 31) & 1u)) rec = nullptr;
         }
-        const uint32_t valid = __ballot_sync(0xFFFFFFFFu, rec != nullptr) & ((1u << kEach) - 1u);
-        uint4 x[kEach], rope[kEach];
+        const uint32_t valid = __ballot_sync(0xFFFFFFFFu, rec != nullptr);
+        const unsigned long long rec_bits = reinterpret_cast<unsigned long long>(rec);
+        uint4 x[kEach], rope[kEach / 4];
         float scale[kEach];
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
-            const uint8_t* p = reinterpret_cast<const uint8_t*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(rec), i));
-            x[i] = rope[i] = make_uint4(0, 0, 0, 0);
+            const uint8_t* p = reinterpret_cast<const uint8_t*>(__shfl_sync(0xFFFFFFFFu, rec_bits, i));
+            x[i] = make_uint4(0, 0, 0, 0);
             scale[i] = 0.f;
             if (p != nullptr) {
                 x[i] = ptx::ldg_stream_v4(p + lane * 16);
                 scale[i] = ptx::ld(reinterpret_cast<const float*>(p + 512) + (lane >> 3));
-                if (lane < 8) rope[i] = ptx::ldg_stream_v4(p + 528 + lane * 16);
             }
         }
-        uint8_t* row = a.rows + (int64_t(b) * a.cap + v0 + warp * kEach) * 1152;
 #pragma unroll
-        for (int i = 0; i < kEach; ++i, row += 1152) {
+        for (int i = 0; i < kEach / 4; ++i) {
+            const uint8_t* p = reinterpret_cast<const uint8_t*>(__shfl_sync(0xFFFFFFFFu, rec_bits, 4 * i + (lane >> 3)));
+            rope[i] = make_uint4(0, 0, 0, 0);
+            if (p != nullptr) rope[i] = ptx::ldg_stream_v4(p + 528 + (lane & 7) * 16);
+        }
+        uint8_t* const row = a.rows + (int64_t(b) * a.cap + v0) * 1152;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
             const __half2 scale2 = __float2half2_rn(fminf(scale[i], 146.f));
             uint4 lo, hi;
             dequant4_f16(x[i].x, scale2, lo.x, lo.y);
             dequant4_f16(x[i].y, scale2, lo.z, lo.w);
             dequant4_f16(x[i].z, scale2, hi.x, hi.y);
             dequant4_f16(x[i].w, scale2, hi.z, hi.w);
-            reinterpret_cast<uint4*>(row)[2 * lane] = lo;
-            reinterpret_cast<uint4*>(row)[2 * lane + 1] = hi;
-            if (lane < 8) reinterpret_cast<uint4*>(row + 1024)[lane] = bf16x8_to_f16x8(rope[i]);
+            ptx::stg_v8(row + i * 1152 + lane * 32, lo, hi);
         }
-        __syncthreads();                           // the bits of the tile before have been read
-        if (lane == 0) s_valid[warp] = valid;
-        __syncthreads();
-        if (threadIdx.x < 2) {
-            uint32_t bits = 0u;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) bits |= s_valid[8 * threadIdx.x + i] << (kEach * i);
-            a.valid[(int64_t(b) * a.cap + v0) / 32 + threadIdx.x] = bits;
-        }
+        for (int i = 0; i < kEach / 4; ++i) *reinterpret_cast<uint4*>(row + (4 * i + (lane >> 3)) * 1152 + 1024 + (lane & 7) * 16) = bf16x8_to_f16x8(rope[i]);
+        if (lane == 0) reinterpret_cast<uint8_t*>(a.valid)[(int64_t(b) * a.cap + v0) / 8] = uint8_t(valid);
     }
 }
 

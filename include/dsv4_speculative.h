@@ -58,7 +58,7 @@ typedef struct Dsv4HcaTreeDecodeParams {
     int32_t*       status;
     void*          sched;
     int64_t        sched_bytes; /* read with make_plan */
-    void*          rows;        /* optional workspace of dsv4_hca_tree_rows_bytes(): the entries are dequantised into it once, and all of a
+    void*          rows;        /* optional workspace of dsv4_hca_tree_rows_bytes(), 32-byte aligned: the entries are dequantised into it once, and all of a
                                    request's nodes read them there; without it every group of 128 (node, head) rows dequantises them for itself */
     int64_t        rows_bytes;
 } Dsv4HcaTreeDecodeParams;
