@@ -980,14 +980,16 @@ cudaError_t launch_tree(const DecodeArgs& d, const Dsv4HcaTreeDecodeParams* p, c
     a.dbg_drop_tile = g_drop_tile.load(std::memory_order_relaxed);
     const int groups = (a.H + kHeadsPerCta - 1) / kHeadsPerCta;
     dim3 grid(2 * groups, a.B, a.num_splits);
+    int pairs = device_sms() / 2;
+    if (pairs < 1) pairs = 1;
+    a.dealt = sched == nullptr && a.num_splits == 1 && a.B <= kTreeDealt && groups * int64_t(a.B) > pairs;
+    if (a.dealt) grid = dim3(2 * pairs, 1, 1);
     if (sched != nullptr) {
         const SchedLayout l = sched_layout(a.B * groups, 0);
         const int32_t* base = static_cast<const int32_t*>(sched);
         a.sched_pair_begin = base + l.pair_begin;
         a.sched_items = base + l.items;
-        int pairs = device_sms() / 2;
-        if (pairs > kPlanMaxPairs) pairs = kPlanMaxPairs;
-        grid = dim3(2 * (pairs > 0 ? pairs : 1), 1, 1);
+        grid = dim3(2 * (pairs < kPlanMaxPairs ? pairs : kPlanMaxPairs), 1, 1);
     }
     static std::atomic<bool> done[kMaxDevices];
     e = ensure_smem(tree_mma_kernel, TreeSmem::kTotal, done);

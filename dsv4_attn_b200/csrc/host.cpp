@@ -484,10 +484,11 @@ bool same_device(const at::Tensor* like, std::initializer_list<const at::Tensor*
     return true;
 }
 
-// Where the library plans the work of a tree decode in the call: more than four row groups for every pair of SMs (74).  A plan overlaps the set-up of
-// one group with the end of another's and costs 6 us and a merge: 1,024 groups of 15 tiles 301 us against 331 on a static grid, 256 groups 119 either way, 128 groups 58
-// against 53, 92 ragged ones 90 against 81.
-constexpr int64_t kTreePlanGroups = 4 * 74;
+// Over shared rows, and with a row group for every pair of SMs (74), the pairs share out whole groups, the longest first: 1,024 groups of 15 tiles 264 us,
+// with a plan that cuts them evenly 302 and its own 12; 92 ragged groups 71 against 90 and 12; 304 ragged groups 170 against 215.  (Groups of one length whose number
+// is just above a multiple of 74 pay for it, 304 of 49 tiles 328 us against 293: who knows that passes a plan.)  Groups that dequantise for themselves are planned in
+// the call from four for every pair on: a plan overlaps the set-up of one with the end of another's and costs 6 us and a merge.
+constexpr int64_t kTreeDealtGroups = 74, kTreeDealtRequests = 256, kTreePlanGroups = 4 * 74;
 // Where the groups of a request share its dequantised entries: from four groups a request and 900 tiles over all groups on (960 tiles in 64 groups: 32 us against
 // 34, 480 in 32 groups 28 against 27; three groups a request 158 against 149), for workspaces of up to 4 GB.
 constexpr int64_t kTreeShareGroups = 4, kTreeShareTiles = 900, kTreeShareBytes = int64_t(4) << 30;
@@ -531,6 +532,7 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
         p.rows = ptr(shared);
         p.rows_bytes = shared->numel();
     }
+    const bool dealt = shared != nullptr && groups >= kTreeDealtGroups && B <= kTreeDealtRequests;
     if (a[15] != Py_None) {                                                // a plan made before
         int64_t v[4];
         if (!PyTuple_Check(a[15]) || PyTuple_GET_SIZE(a[15]) != 8) return none();
@@ -542,7 +544,7 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
         pl = any_tensor(PyTuple_GET_ITEM(a[15], 7));
         if (sched == nullptr || po == nullptr || pl == nullptr) return none();
         splits = 0;
-    } else if (a[9] == Py_None && a[12] == Py_None && groups > kTreePlanGroups) {
+    } else if (a[9] == Py_None && a[12] == Py_None && groups > kTreePlanGroups && !dealt) {
         int64_t po_bytes, pl_bytes;
         const int64_t bytes = lib.sched_bytes(int(B), int(T * H), 0, 0, &po_bytes, &pl_bytes);
         if (bytes <= 0) return none();
@@ -554,8 +556,7 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
         p.sched_bytes = bytes;
         splits = 0;
     } else {
-        // (a row group for every pair, over shared rows: a second wave costs less than the partials of splits, 80 us against 95 for 92 ragged groups)
-        if (a[9] == Py_None) splits = shared != nullptr && groups >= 74 ? 1 : lib.plan_splits(int(B), int(T * H), int(max_len), 0);
+        if (a[9] == Py_None) splits = dealt ? 1 : lib.plan_splits(int(B), int(T * H), int(max_len), 0);
         else if (!integer(a[9], &splits)) return none();
         if (splits < 1 || splits > DSV4_MAX_SPLITS) return none();
         if (a[12] != Py_None) {

@@ -148,7 +148,9 @@ struct TreeArgs {
     const int32_t* sched_items;
     uint32_t wait_ns;
     int dbg_drop_tile;
+    bool dealt;                                // without a plan, resident pairs share out the row groups
 };
+constexpr int kTreeDealt = 256;                // requests at most of which that is done
 
 struct TreeSmem {
     static constexpr int kQBytes = 3 * kQChunkBytes;            // chunks 6-8 stay here
@@ -186,6 +188,8 @@ struct TreeMisc {
     uint64_t bar_k_full[2], bar_v_full[2];                // both blocks' halves of a tile landed (TMA transaction count, by the copies themselves)
     uint64_t bar_p_full[2];
     uint32_t tmem_base;
+    uint8_t order[kTreeDealt];       // requests by length, the longest first
+    int len[kTreeDealt];
 };
 static_assert(sizeof(TreeMisc) <= 3072 - 16, "the last word of the block's shared memory is failed_flag()");
 
@@ -215,6 +219,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
     const uint32_t wait_ns = a.wait_ns;
 
     int item_begin = 0, n_items = 1;
+    const int hgs = (a.H + kHeadsPerCta - 1) / kHeadsPerCta, pairs = int(gridDim.x >> 1), my_pair = int(blockIdx.x >> 1);
     auto get_item = [&](int k) -> Item {
         Item it;
         if (sched) {
@@ -226,7 +231,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
             it.n_tok = min(it.n_tok, a.cap);
             it.ntiles = min(it.ntiles, max(a.cap / kTileN - it.tile0, 0));
         } else {
-            it.n = blockIdx.y;  it.hg = blockIdx.x >> 1;
+            it.n = blockIdx.y;  it.hg = my_pair;
+            if (a.dealt) {
+                const int at = k * pairs + ((k & 1) ? pairs - 1 - my_pair : my_pair);
+                it.n = misc->order[at / hgs];  it.hg = at % hgs;
+            }
             it.kv_len_n = max(ptx::ld(a.kv_len + it.n), 0);
             it.n_tok = int(min(int64_t(it.kv_len_n) + max(ptx::ld(a.win_len + it.n), 0), int64_t(a.cap)));
             const int split = blockIdx.z;
@@ -280,6 +289,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTreeThreads, 1) tre
         const int pair = blockIdx.x >> 1;
         item_begin = ptx::ld(a.sched_pair_begin + pair);
         n_items = ptx::ld(a.sched_pair_begin + pair + 1) - item_begin;
+    } else if (a.dealt) {
+        // The groups of the longest request come first, and every other round of them goes round backwards: nobody begins a long one last (92 ragged groups
+        // in the order of the batch 83 us, so 71; 128 groups of 12,800 entries on average 440 and 390), and a pair's next Q and last output are under way during its tiles as they are with a plan.
+        if (tid < a.B) misc->len[tid] = int(min(int64_t(max(ptx::ld(a.kv_len + tid), 0)) + max(ptx::ld(a.win_len + tid), 0), int64_t(a.cap)));
+        __syncthreads();
+        if (tid < a.B) {
+            const int mine = misc->len[tid];
+            int before = 0;
+#pragma unroll 4
+            for (int i = 0; i < a.B; ++i) before += misc->len[i] > mine || (misc->len[i] == mine && i < tid);
+            misc->order[before] = uint8_t(tid);
+        }
+        __syncthreads();
+        const int groups = a.B * hgs, rounds = groups / pairs, left = groups - rounds * pairs;      // (the last round may be a part of one)
+        n_items = rounds + (((rounds & 1) ? pairs - 1 - my_pair : my_pair) < left ? 1 : 0);
     }
     constexpr uint32_t tmem = 0;                  // all 512 columns are allocated (checked)
     auto wait_tmem = [&]() -> bool {
