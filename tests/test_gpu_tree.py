@@ -174,6 +174,25 @@ def test_outputs_of_any_alignment(lib, rows):
     check(got, want(c, SCALE))
 
 
+@pytest.mark.parametrize("B,T,H", [(20, 9, 128), (40, 33, 20), (7, 32, 128), (257, 1, 128)])
+def test_row_groups_dealt_to_pairs(lib, B, T, H):
+    """Several rounds of row groups for every pair, the last one partly filled, over requests of equal, very different and no lengths; and more
+    requests than are put in order."""
+    kv_len = [(37 * b * b) % 700 if b % 4 else (0, 640)[b % 8 == 0] for b in range(B)]
+    win_len = [0 if b % 5 == 3 else 33 - b % 3 for b in range(B)]
+    c = make(B, B, T, H, kv_len, 33, win_len)
+    sink = torch.randn(H, device="cuda")
+    check(call(lib, c, SCALE, attn_sink=sink, num_splits=1, share_rows=True), want(c, SCALE, sink))
+
+
+def test_a_workspace_off_its_boundary_is_refused(lib):
+    c = make(2, 2, 16, 64, [100, 200], 8)
+    room = torch.empty(lib.tree_rows_bytes(2, c["block_table"].shape[1], 8) + 32, device="cuda", dtype=torch.uint8)
+    with pytest.raises(lib.Dsv4Error):
+        call(lib, c, SCALE, share_rows=room[16:])
+    check(call(lib, c, SCALE, share_rows=room[32:]), want(c, SCALE))
+
+
 def test_tree_sees():
     """Ancestors, the node itself, and the committed tokens that have not slid out."""
     from dsv4_attn_b200 import layout
