@@ -215,31 +215,32 @@ struct LogitRow {
     // The largest logit of this thread's, for the warp's `steps` steps from element `first` on; NaN left out, -inf where there is none.  Sixteen-bit logits
     // are compared two at a time.
     __device__ __forceinline__ float largest(int first, int steps) const {
-        constexpr int kDeep = 16 / kVecs;        // loads in flight: 16 of 16 bytes
+        constexpr int kDeep = 8 / kVecs;         // loads in flight: 8 of 16 bytes
         float top = -CUDART_INF_F;
         int s = 0;
         // (the warp's first step may begin before the row, its last one end behind it)
         while (s < steps && first + s * kSampleStep < lead) top = fmaxf(top, largest_of_edge(first + s++ * kSampleStep + lane * 8));
-        const int whole = min(steps, (end - first) / kSampleStep);
+        const int whole = max(s, min(steps, (end - first) / kSampleStep));
         Pair best[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) best[i] = none();
 #pragma unroll 1
-        for (; s + kDeep <= whole; s += kDeep) {
+        for (; s < whole; s += kDeep) {
             uint4 x[kDeep][kVecs];
             const uint4* p = reinterpret_cast<const uint4*>(base + first + s * kSampleStep + lane * 8);
 #pragma unroll
             for (int j = 0; j < kDeep; ++j)
 #pragma unroll
-                for (int i = 0; i < kVecs; ++i) x[j][i] = ptx::ld(p + j * 32 * kVecs + i);
+                for (int i = 0; i < kVecs; ++i) {
+                    x[j][i] = make_uint4(none().bits, none().bits, none().bits, none().bits);
+                    if (s + j < whole) x[j][i] = ptx::ld(p + j * 32 * kVecs + i);
+                }
 #pragma unroll
             for (int j = 0; j < kDeep; ++j)
 #pragma unroll
                 for (int i = 0; i < kVecs; ++i) keep(best, x[j][i]);
         }
-        for (; s < whole; ++s)
-#pragma unroll
-            for (int i = 0; i < kVecs; ++i) keep(best, ptx::ld(reinterpret_cast<const uint4*>(base + first + s * kSampleStep + lane * 8) + i));
+        s = whole;
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = fmaxf(top, value(best[i]));
         for (; s < steps; ++s) top = fmaxf(top, largest_of_edge(first + s * kSampleStep + lane * 8));
