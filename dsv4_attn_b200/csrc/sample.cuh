@@ -626,15 +626,23 @@ __device__ __forceinline__ void token_of_list(SampleShared& sh, const SampleRow&
 __device__ __forceinline__ int row_in_order(SampleShared& sh, const SampleArgs& a, int at) {
     uint32_t* const flags = sh.bins;
     const int lane = threadIdx.x & 31;
-    for (int n0 = int(threadIdx.x) - lane; n0 < a.N; n0 += kSampleThreads) {
-        const int n = n0 + lane;
-        bool heavy = false;
-        if (n < a.N && (a.temperature == nullptr || ptx::ld(a.temperature + n) > 0.f)) {
-            const int k = a.top_k != nullptr ? ptx::ld(a.top_k + n) : 0;
-            heavy = k <= 0 || k >= a.V ? a.top_p != nullptr && ptx::ld(a.top_p + n) < 1.f : k > kSampleThreads * kSampleQuarters / 2;
+    // (two rows a thread at a time, their settings on the way together: one after the other, and only as far as needed, they took 2 us)
+    for (int n0 = int(threadIdx.x) - lane; n0 < a.N; n0 += 2 * kSampleThreads) {
+        float t[2], p[2];
+        int k[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int n = min(n0 + i * kSampleThreads + lane, a.N - 1);
+            t[i] = a.temperature != nullptr ? ptx::ld(a.temperature + n) : 1.f;
+            k[i] = a.top_k != nullptr ? ptx::ld(a.top_k + n) : 0;
+            p[i] = a.top_p != nullptr ? ptx::ld(a.top_p + n) : 1.f;
         }
-        const uint32_t b = __ballot_sync(0xFFFFFFFFu, heavy);
-        if (lane == 0) flags[n0 >> 5] = b;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const bool heavy = t[i] > 0.f && (k[i] <= 0 || k[i] >= a.V ? p[i] < 1.f : k[i] > kSampleThreads * kSampleQuarters / 2);
+            const uint32_t b = __ballot_sync(0xFFFFFFFFu, heavy && n0 + i * kSampleThreads + lane < a.N);
+            if (lane == 0 && n0 + i * kSampleThreads < a.N) flags[(n0 + i * kSampleThreads) >> 5] = b;
+        }
     }
     __syncthreads();
     // every warp for itself: the words in runs, one a lane
