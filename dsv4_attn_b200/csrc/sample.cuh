@@ -771,12 +771,24 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     r.odd = r.top == CUDART_INF_F || r.per == CUDART_INF_F;
     if (r.greedy) {
         // the lowest index of the largest logit
-        if (mine == r.top)
-            row.each(first, steps, [&](const float (&v)[8], int e) {
+        constexpr int kDeep = 4;
+#pragma unroll 1
+        for (int q = 0; q < kSampleQuarters; ++q) {
+            const int from = first + quarter_step(q) * kSampleStep + lane * 8, many = quarter_step(q + 1) - quarter_step(q);
+            if (!(q == 0 ? quarter[0] == r.top : q == 1 ? quarter[1] == r.top : q == 2 ? quarter[2] == r.top : quarter[3] == r.top)) continue;
+#pragma unroll 1
+            for (int s = 0; s < many; s += kDeep) {
+                alignas(16) T x[kDeep][8];
 #pragma unroll
-                for (int i = 7; i >= 0; --i)
-                    if (v[i] == r.top) atomicMin(&sh.kept, uint32_t(e + i - row.lead));
-            });
+                for (int d = 0; d < kDeep; ++d)
+                    if (s + d < many) row.load(from + (s + d) * kSampleStep, x[d]);
+#pragma unroll
+                for (int d = kDeep - 1; d >= 0; --d)
+#pragma unroll
+                    for (int i = 7; i >= 0; --i)
+                        if (s + d < many && logit_value(x[d][i]) == r.top) atomicMin(&sh.kept, uint32_t(from + (s + d) * kSampleStep + i - row.lead));
+            }
+        }
         __syncthreads();
         uint32_t token = sh.kept;
         if (blocks > 1u) {
