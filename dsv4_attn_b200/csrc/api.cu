@@ -1121,7 +1121,9 @@ extern "C" int dsv4_kv_pages_compact(const Dsv4KvPagesParams* p, void* stream) {
 namespace {
 template <typename T>
 cudaError_t launch_sample(SampleArgs& a, cudaStream_t stream) {
-    // Up to eight blocks share a row where the rows leave SMs without one of the two blocks they hold, as long as each has 4,096 logits; a FixedSum has a limit.
+    // Up to eight blocks share a row where the rows leave SMs without one of the two blocks they hold, as long as each has 4,096 logits; a FixedSum has a
+    // limit.  (Rows of 131,072 with mixed settings: 16 of them in clusters of eight 34 us, one block each 65; 64 in clusters of four 42, one block each 69, of
+    // eight 52.  150 by temperature 21 with one block each, in pairs 26.)
     const int span = a.V + 16 / int(sizeof(T)) - 1;                        // with what a row's alignment may put before it
     const int steps = (span + kSampleStep - 1) / kSampleStep;
     int blocks = 1;

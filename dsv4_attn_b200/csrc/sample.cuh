@@ -6,17 +6,22 @@
 //
 // A block, or a cluster of up to eight where there are few rows, works on a row; every warp owns neighbouring logits.  The row is read from DRAM once, for
 // its maximum; what is looked at again comes from L1 or L2 (kept in shared memory, rows of 131,072 left room for clusters of eight blocks of 16,384 only,
-// whose barriers cost more than the second reading: 1,024 rows, greedy, 302 us against 245).  Then
+// whose barriers cost more than the second reading: 1,024 rows, as first built, 302 us against 245).  Then
 //   maximum -> (top-k, top-p: the cut) -> sums of the kept weights per warp -> the part of the row in which the random number falls, again by
 //   warps -> the token.
 // A cut is a pair (logit, ties): kept are the tokens above it, and the first `ties` of those that are equal to it.
 //
-// Top-k of up to 512 a block is sought among candidates: every thread has the largest of its logits at hand, and where ceil(k / blocks) threads of each
-// block have one of at least x, at least k logits are, so that all logits from x on (some 2 k of them) hold the cut.  Only the threads that have one look
-// again, and the token is found among them.
-// Any other cut: a histogram over (l_max - l) / t in bins of 1/128, a count per bin, says where it should be; what lies above is then summed
-// exactly and the logits of two and a half bins there are the candidates, those of the bins next to them if the exact sums say so.  Candidates
-// too many for the lists (thousands of equal logits) are gone through by digits of their ordered bits.
+// Top-k of up to 1,024 a block is sought among candidates: every thread has the largest of each quarter of its logits at hand, and where ceil(k / blocks)
+// of a block's are at least x, at least k logits are, so that all logits from x on (some 2 k of them) hold the cut.  Only the quarters that have one are
+// looked at again, and the token is found among them.
+// Any other cut: a histogram over (l_max - l) / t in bins of 1/128, a count per bin, says where it should be (and, where min-p keeps less than that,
+// that there is no need of it); what lies above is then summed exactly, and the logits of two and a half bins there are the candidates, those of the bins
+// next to them if the exact sums say so.  Equal logits of sixteen bits are counted, not listed; what else is too much for the lists is gone through
+// by digits of ordered bits.
+//
+// Bounds, at 1,024 rows of 131,072 BF16 logits (268 MB, 41 us at the measured copy rate): a greedy row is read once, 51 us; temperature alone 126 and
+// top-p alone 290 to 320 are expf and its surroundings, 62 % of the issue slots in use; top-k 50 72 to 78, with the chain of its short steps; a mixture of
+// all 157.  A single row of 32,000: 12 us, of which the barriers and reads of its chain are nearly all.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -119,37 +124,22 @@ __device__ __forceinline__ float key_value(uint32_t k) {
     return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
 }
 
-// Sums of floor(2^40 e), e <= 1, as two sums of 20 bits each.  Added to 2^23 and rounded towards zero, e 2^20 leaves its whole part in the low bits of
-// the sum; what is left of it is exact, and gives the other 20 bits the same way: five instructions, where shifting and adding in 64 bits take ten.
-// At most 4,095 terms.
+// A sum of floor(2^40 e), e <= 1: next to 4096 a 64-bit number counts in steps of 2^-40, and a sum that is rounded towards zero takes in of each e
+// the whole steps.  A conversion and an addition a term (1,024 rows by temperature alone: 126 us, with two sums of 20 bits each in 32-bit numbers 135, with the
+// conversion by shifts 132).  At most 4,095 terms.
 struct FixedSum {
-    uint32_t hi = 0, lo = 0;     // less 0x4B000000, the bits of 2^23, per term
-    int terms = 0;
-    __device__ __forceinline__ void add(float e) {
-        const float h = __fmaf_rz(e, 1048576.f, 8388608.f), rest = __fmaf_rn(e, 1048576.f, 8388608.f - h);
-        hi += __float_as_uint(h);
-        lo += __float_as_uint(__fmaf_rz(rest, 1048576.f, 8388608.f));
-        ++terms;
-    }
-    // Two terms in packed operations; each also to another sum where `too` says so.
+    double sum = 4096.0;
+    __device__ __forceinline__ void add(float e) { sum = __dadd_rz(sum, double(e)); }
+    // Two terms; each also to another sum where `too` says so.
     __device__ __forceinline__ void add2(float e0, float e1, FixedSum* other = nullptr, bool too0 = false, bool too1 = false) {
-        const uint64_t scale = ptx::pack_f32x2(1048576.f, 1048576.f), one = ptx::pack_f32x2(8388608.f, 8388608.f), minus = ptx::pack_f32x2(-1.f, -1.f);
-        const uint64_t e = ptx::pack_f32x2(e0, e1), h = ptx::fma_rz_f32x2(e, scale, one), rest = ptx::fma_f32x2(e, scale, ptx::fma_f32x2(h, minus, one));
-        float x0, x1, y0, y1;
-        ptx::unpack_f32x2(h, x0, x1);
-        ptx::unpack_f32x2(ptx::fma_rz_f32x2(rest, scale, one), y0, y1);
-        hi += __float_as_uint(x0) + __float_as_uint(x1);
-        lo += __float_as_uint(y0) + __float_as_uint(y1);
-        terms += 2;
+        const double d0 = e0, d1 = e1;
+        sum = __dadd_rz(__dadd_rz(sum, d0), d1);
         if (other != nullptr) {
-            if (too0) { other->hi += __float_as_uint(x0);  other->lo += __float_as_uint(y0);  ++other->terms; }
-            if (too1) { other->hi += __float_as_uint(x1);  other->lo += __float_as_uint(y1);  ++other->terms; }
+            if (too0) other->sum = __dadd_rz(other->sum, d0);
+            if (too1) other->sum = __dadd_rz(other->sum, d1);
         }
     }
-    __device__ __forceinline__ unsigned long long total() const {
-        const uint32_t off = uint32_t(terms) * 0x4B000000u;
-        return ((unsigned long long)(hi - off) << 20) + (lo - off);
-    }
+    __device__ __forceinline__ unsigned long long total() const { return static_cast<unsigned long long>(__double_as_longlong(sum) - __double_as_longlong(4096.0)); }
 };
 __device__ __forceinline__ unsigned long long fixed(float e) {
     FixedSum s;
@@ -622,7 +612,7 @@ __device__ __forceinline__ void token_of_list(SampleShared& sh, const SampleRow&
 }
 
 // The row at place `at` where those that take longest, with a cut that no list of candidates gives (top-p alone, a large top-k), come first: they take three
-// times as long, and one that is begun last is waited for by the whole call (1,024 rows, one in four of them: 243 us, heavy ones first 203).  Every block looks at all rows' settings.
+// times as long, and one that is begun last is waited for by the whole call (1,024 rows, one in five of them: 169 us, heavy ones first 157).  Every block looks at all rows' settings.
 __device__ __forceinline__ int row_in_order(SampleShared& sh, const SampleArgs& a, int at) {
     uint32_t* const flags = sh.bins;
     const int lane = threadIdx.x & 31;
