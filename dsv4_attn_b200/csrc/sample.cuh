@@ -292,6 +292,7 @@ struct LogitRow {
             for (int i = 0; i < 8; ++i) v[i] = logit_value(next[i]);
             if (s + 1 < steps) load(e + kSampleStep, next);
             visit(v, e);
+            __syncwarp();                          // (lanes that had more to do: the next loads go out together again)
         }
     }
 };
@@ -451,18 +452,16 @@ __device__ __forceinline__ void list_logit(SampleShared& sh, float l, int index)
     if (at < uint32_t(kSampleList)) sh.list[at] = (static_cast<unsigned long long>(order_key(l + 0.f)) << 32) | uint32_t(~index);
 }
 
-// The logits from e on that `here` names go to the block's list, one atomic a warp.  Every lane of the warp calls.
-__device__ __forceinline__ void list_logits(SampleShared& sh, const float (&v)[8], uint32_t here, int index, int lane) {
-    const uint32_t mine = uint32_t(__popc(here)), upto = warp_upto32(mine, lane);
-    uint32_t base = 0;
-    if (lane == 31) base = atomicAdd(&sh.count, upto);
-    uint32_t at = __shfl_sync(0xFFFFFFFFu, base, 31) + upto - mine;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if ((here >> i) & 1u) {
-            if (at < uint32_t(kSampleList)) sh.list[at] = (static_cast<unsigned long long>(order_key(v[i] + 0.f)) << 32) | uint32_t(~(index + i));
-            ++at;
-        }
+// take(v[i], i) for the bits of `here`, a lane's eight logits: there are one or two in a warp's 256, so a short loop takes less than eight tests in a row do.
+template <typename Take>
+__device__ __forceinline__ void each_of(uint32_t here, const float (&v)[8], Take take) {
+#pragma unroll 1
+    for (; here != 0u; here &= here - 1u) {
+        const int i = __ffs(here) - 1;
+        const float a = (i & 1) ? v[1] : v[0], b = (i & 1) ? v[3] : v[2], c = (i & 1) ? v[5] : v[4], d = (i & 1) ? v[7] : v[6];
+        const float low = (i & 2) ? b : a, high = (i & 2) ? d : c;
+        take((i & 4) ? high : low, i);
+    }
 }
 
 // How many candidates the lists have (-1: too many), after row_totals.
@@ -830,11 +829,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
         const int eights = sweep ? 0 : int(sh.digit) << shift;
         if (sweep)
             row.each(first, steps, [&](const float (&v)[8], int e) {
-                if (!__any_sync(0xFFFFFFFFu, max_of(v) >= from)) return;
+                if (max_of(v) < from) return;
                 uint32_t here = 0;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) here |= uint32_t(v[j] >= from) << j;
-                list_logits(sh, v, here, e - row.lead, lane);
+                each_of(here, v, [&](float l, int j) { list_logit(sh, l, e + j - row.lead); });
             });
         constexpr int kDeep = 4;
 #pragma unroll 1
@@ -861,7 +860,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                     here |= uint32_t(v[j] >= from) << j;
                 }
                 if (e[d] < 0) here = 0u;
-                if (__any_sync(0xFFFFFFFFu, here != 0u)) list_logits(sh, v, here, e[d] - row.lead, lane);
+                each_of(here, v, [&](float l, int j) { list_logit(sh, l, e[d] + j - row.lead); });
             }
         }
         if (blocks > 1u) {
@@ -1041,14 +1040,15 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                         off = fminf(off, fminf(fabsf(v[i] - mid), fabsf(v[i + 1] - mid)));
                     }
                     if (off <= near_by || may_be) {
+                        uint32_t here = 0;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const float x = r.exponent(v[i]);
-                            if (v[i] > above_value && !(x > x_from) && x > x_to) {
-                                if (by_value) atomicAdd(&table[min(top_value - (order_key(v[i] + 0.f) >> row.kKeyShift), uint32_t(kSampleValues - 1))], 1u);
-                                else list_logit(sh, v[i], e + i - row.lead);
-                            }
-                        }
+                        for (int i = 0; i < 8; ++i) here |= uint32_t(may_be || fabsf(v[i] - mid) <= near_by) << i;
+                        each_of(here, v, [&](float l, int i) {
+                            const float x = r.exponent(l);
+                            if (!(l > above_value && !(x > x_from) && x > x_to)) return;
+                            if (by_value) atomicAdd(&table[min(top_value - (order_key(l + 0.f) >> row.kKeyShift), uint32_t(kSampleValues - 1))], 1u);
+                            else list_logit(sh, l, e + i - row.lead);
+                        });
                     }
                 });
                 over = by_weight ? sum_all.total() : n_all;
