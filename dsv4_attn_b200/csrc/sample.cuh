@@ -19,9 +19,10 @@
 // next to them if the exact sums say so.  Equal logits of sixteen bits are counted, not listed; what else is too much for the lists is gone through
 // by digits of ordered bits.
 //
-// Bounds, at 1,024 rows of 131,072 BF16 logits (268 MB, 41 us at the measured copy rate): a greedy row is read once, 51 us; temperature alone 126 and
-// top-p alone 290 to 320 are expf and its surroundings, 62 % of the issue slots in use; top-k 50 72 to 78, with the chain of its short steps; a mixture of
-// all 157.  A single row of 32,000: 12 us, of which the barriers and reads of its chain are nearly all.
+// Bounds, at 1,024 rows of 131,072 BF16 logits (268 MB, 41 us at the measured copy rate): greedy rows, read once, 51 us; by temperature alone 126, 17
+// instructions a logit, 14 of them expf and the sum; top-p alone 250 to 295, nearly 40 (a histogram, then that sum with the candidates); both with some
+// 60 % of the issue slots in use; top-k 50 72 to 78, with the chain of its short steps; a mixture of all 137.  A single row of 32,000: 12 us, of which the
+// barriers and reads of its chain are nearly all.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -44,8 +45,9 @@ constexpr int kSampleList = 2048;                // candidates
 constexpr int kSampleShort = 256;                // candidates that are compared all with all
 constexpr int kSampleBins = 4096;                // of the histogram over (l_max - l) / t,
 constexpr float kSampleBin = 128.f;              // 1/128 each
-constexpr uint32_t kSampleSpare = 200;           // candidates next to the bin of a cut
+constexpr uint32_t kSampleSpare = 64;           // candidates next to the bin of a cut
 constexpr int kSampleQuarters = 4;               // a thread knows the largest logit of each quarter of its own
+constexpr uint32_t kSampleMany = 300;           // within three bins of it: a part of a bin will do
 constexpr int kSampleValues = 128;               // different logits, of sixteen bits, that may be near a cut
 constexpr int kSampleMostTerms = 4095;           // of a FixedSum
 
@@ -611,7 +613,7 @@ __device__ __forceinline__ void token_of_list(SampleShared& sh, const SampleRow&
 }
 
 // The row at place `at` where those that take longest, with a cut that no list of candidates gives (top-p alone, a large top-k), come first: they take three
-// times as long, and one that is begun last is waited for by the whole call (1,024 rows, one in five of them: 169 us, heavy ones first 157).  Every block looks at all rows' settings.
+// times as long, and one that is begun last is waited for by the whole call (1,024 rows, one in five of them, at a time when they took a sixth longer: 169 us, heavy ones first 157).  Every block looks at all rows' settings.
 __device__ __forceinline__ int row_in_order(SampleShared& sh, const SampleArgs& a, int at) {
     uint32_t* const flags = sh.bins;
     const int lane = threadIdx.x & 31;
@@ -891,13 +893,13 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
             for (int i = tid; i < kSampleBins; i += kSampleThreads) sh.bins[i] = 0u;
             __syncthreads();
             // Bin of a logit: 1, its distance in bins and `off`, rounded to a whole number by the addition of 2^23.  (Near enough: what is decided
-            // by it is checked with the exact sums.)  The last bin is for what is further away, and not counted.
+            // by it is checked with the exact sums.)  The last bin is for what is further away, and left out below.
             const float slope = -kSampleBin * r.per, offset = fmaf(-slope, r.top, 8388609.f), off = fmaf(slope, r.top, offset - 8388609.f);
             row.each(first, steps, [&](const float (&v)[8], int) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const uint32_t bin = __float_as_uint(fminf(fmaf(v[i], slope, offset), 8388608.f + kSampleBins - 1)) & (kSampleBins - 1);
-                    if ((!LIMITED || v[i] > above_value) && bin < kSampleBins - 1) atomicAdd(&sh.bins[bin], 1u);
+                    if (!LIMITED || v[i] > above_value) atomicAdd(&sh.bins[bin], 1u);
                 }
             });
             sync_row(blocks);
@@ -922,7 +924,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
 #pragma unroll
                 for (int i = 0; i < kPer; ++i) {
                     const int bin = kPer * tid + i;
-                    c[i] = from[bin];
+                    c[i] = bin < kSampleBins - 1 ? from[bin] : 0u;
                     n_mine += c[i];
                     mine_sum += by_weight ? float(c[i]) * __expf(float(1 - bin) / kSampleBin) : float(c[i]);
                 }
@@ -990,7 +992,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                 // Where they are many, and spread evenly (32-bit logits), less will do, around the place in the bin: what an estimate from counts is off by there
                 // is a small part of a bin.
                 const uint32_t near = counts[min(bin + 1, kSampleBins - 1)] - (bin > 1 ? counts[bin - 2] : 0u);
-                if (sizeof(T) == 4 && near > uint32_t(kSampleList) / 2) half_width = fmaxf(1.5f * float(kSampleList / 4) / float(near), 0.05f);
+                if (sizeof(T) == 4 && near > kSampleMany) half_width = fmaxf(float(kSampleMany) / float(near), 0.05f);
             }
             __syncthreads();                       // (the counts lie where the candidates will be sorted)
             // Exactly: what all weigh, what lies nearer than `from`, and the candidates from there to `to`.
@@ -999,12 +1001,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                 from = float(sh.bin - 1) - off + sh.place - 0.5f - half_width;
                 to = from + 2.f * half_width;
             }
-            const float next = half_width > 0.f ? 2.f * half_width : 2.5f;
+            float next = half_width > 0.f ? 2.f * half_width : 2.5f;                // (where the cut is not there after all: the next part, twice as long each time)
             unsigned long long ahead;
             for (int moved = 0, tries = 0;; ++tries) {
-                // (a few steps the same way: all the way; and what is not a number, with infinite logits, is everything)
-                if (!(from >= 1.f) || (tries > 2 && moved < 0)) from = -1.f;
-                if (!(to <= kSampleBins - 8) || (tries > 2 && moved > 0)) to = CUDART_INF_F;
+                // (many steps: all the way; and what is not a number is everything)
+                if (!(from >= 1.f) || (tries > 8 && moved < 0)) from = -1.f;
+                if (!(to <= kSampleBins - 8) || (tries > 8 && moved > 0)) to = CUDART_INF_F;
                 const bool open = to == CUDART_INF_F;
                 __syncthreads();
                 if (tid == 0) sh.count = 0u;
@@ -1068,7 +1070,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                 row_totals(sh, blocks, rank, turn, over, ahead);
                 if (by_weight) wanted = max(share_of(over + ties, uint32_t(r.p24)), 1ull);
                 if (wanted > over) { over = wanted - over;  return false; }
-                if (wanted <= ahead) { to = from;  from -= next;  moved = -1;  continue; }
+                if (wanted <= ahead) { to = from;  from -= next;  next *= 2.f;  moved = -1;  continue; }
                 if (by_value) {
                     // Every warp for itself: four neighbouring values a lane, the largest first.
                     constexpr int kPer = kSampleValues / 32;
@@ -1124,7 +1126,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                         return true;
                     }
                     from = to;                     // (a little further away)
-                    to += next;
+                    to += next;  next *= 2.f;
                     moved = 1;
                     continue;
                 }
@@ -1177,7 +1179,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                     if (wanted <= upto) break;
                 }
                 from = to;
-                to += next;
+                to += next;  next *= 2.f;
                 moved = 1;
             }
             wanted -= ahead;
