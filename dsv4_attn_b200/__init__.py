@@ -1,5 +1,6 @@
 """dsv4_attn_b200: decode attention for DeepSeek-V4-style compressed KV caches
-on NVIDIA B200 (sm_100a).  CSA sparse decode, HCA dense decode, split-KV merge.
+on NVIDIA B200 (sm_100a).  CSA sparse decode, HCA dense decode, split-KV merge; tree
+decode, sampling and cache pages for speculative decoding.
 
 The operators live in libdsv4_attn.so (built by `python -m dsv4_attn_b200.build`).
 The shared object is loaded on first use of any operator or of `LIB`; if it is

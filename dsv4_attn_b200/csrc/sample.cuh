@@ -45,9 +45,9 @@ constexpr int kSampleList = 2048;                // candidates
 constexpr int kSampleShort = 256;                // candidates that are compared all with all
 constexpr int kSampleBins = 4096;                // of the histogram over (l_max - l) / t,
 constexpr float kSampleBin = 128.f;              // 1/128 each
-constexpr uint32_t kSampleSpare = 64;           // candidates next to the bin of a cut
+constexpr uint32_t kSampleSpare = 64;            // candidates next to the bin of a cut
 constexpr int kSampleQuarters = 4;               // a thread knows the largest logit of each quarter of its own
-constexpr uint32_t kSampleMany = 300;           // within three bins of it: a part of a bin will do
+constexpr uint32_t kSampleMany = 300;            // within three bins of it: a part of a bin will do
 constexpr int kSampleValues = 128;               // different logits, of sixteen bits, that may be near a cut
 constexpr int kSampleMostTerms = 4095;           // of a FixedSum
 
