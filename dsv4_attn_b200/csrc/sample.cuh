@@ -612,6 +612,60 @@ __device__ __forceinline__ void token_of_list(SampleShared& sh, const SampleRow&
     }
 }
 
+// The token among up to kSampleShort candidates (n of them, in the lists of all blocks), of which the first k and top-p's share are kept: a thread has one, and
+// adds up what comes before it, in their order for the cut and in the vocabulary's for the token.  Every thread of the first block calls; `read` is called when the
+// lists have been read.
+template <typename Read>
+__device__ __forceinline__ void token_of_few(SampleShared& sh, const SampleRow& r, const SampleArgs& a, uint32_t blocks, int turn, int n, int k, int row, uint32_t u24, Read read) {
+    const int tid = threadIdx.x;
+    unsigned long long c = 0, w = 0;
+    float x = 0.f, e = 0.f;
+    if (tid < n) {
+        uint32_t b = 0, at = uint32_t(tid);
+        while (at >= sh.found[turn][b]) at -= sh.found[turn][b++];
+        c = blocks > 1u ? lds_cluster_u64(ptx::mapa(ptx::smem_u32(&sh.list[at]), b)) : sh.list[at];
+        x = r.exponent(key_value(uint32_t(c >> 32)));
+        e = expf(x);
+        w = fixed(e);
+        sh.sorted[tid] = c;
+        sh.all[tid] = w;
+    }
+    __syncthreads();
+    read();
+    int rank = 0;
+    unsigned long long before = 0;
+    if (tid < n) {
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) {
+            const bool first = sh.sorted[j] > c;
+            rank += first;
+            before += first ? sh.all[j] : 0ull;
+        }
+        if (rank == k - 1) sh.digit_above = before + w;
+    }
+    __syncthreads();
+    if (tid < n) {
+        if (rank >= k || (r.p24 >= 0 && before >= max(share_of(sh.digit_above, uint32_t(r.p24)), 1ull)) || e < r.min_p) w = 0ull;
+        sh.all[tid] = w;
+    }
+    __syncthreads();
+    if (w == 0ull) return;
+    const uint32_t index = ~uint32_t(c);
+    unsigned long long total = 0;
+    before = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+        const unsigned long long wj = sh.all[j];
+        total += wj;
+        before += ~uint32_t(sh.sorted[j]) < index ? wj : 0ull;
+    }
+    const unsigned long long target = share_of(total, u24);
+    if (target >= before && target < before + w) {
+        a.token[row] = int(index);
+        if (a.logprob != nullptr) a.logprob[row] = x - logf(__ull2float_rn(total) * 9.094947017729282e-13f);
+    }
+}
+
 // The row at place `at` where those that take longest, with a cut that no list of candidates gives (top-p alone, a large top-k), come first: they take three
 // times as long, and one that is begun last is waited for by the whole call (1,024 rows, one in five of them, at a time when they took a sixth longer: 169 us, heavy ones first 157).  Every block looks at all rows' settings.
 __device__ __forceinline__ int row_in_order(SampleShared& sh, const SampleArgs& a, int at) {
@@ -874,6 +928,17 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
             __syncthreads();
         }
         const int m = listed(sh, blocks, turn);
+        if (m >= 0 && m <= kSampleShort) {
+            // (the other blocks may leave when their lists have been read)
+            if (rank == 0)
+                token_of_few(sh, r, a, blocks, turn, m, min(r.k, m), n, u24, [&] {
+                    if (blocks > 1u) asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+                });
+            else asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+            __syncwarp();
+            if (blocks > 1u) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+            return;
+        }
         if (m >= 0) {
             if (rank == 0) cut_of_list(sh, r, blocks, turn, m, min(r.k, m), r.p24 < 0 ? ~0ull : 0ull);
             sync_row(blocks);                      // (the lists have been read)
