@@ -1121,14 +1121,15 @@ extern "C" int dsv4_kv_pages_compact(const Dsv4KvPagesParams* p, void* stream) {
 namespace {
 template <typename T>
 cudaError_t launch_sample(SampleArgs& a, cudaStream_t stream) {
-    // Up to eight blocks share a row where the rows leave SMs without one of the two blocks they hold, as long as each has 4,096 logits; a FixedSum has a
-    // limit.  (Rows of 131,072 with mixed settings: 16 of them in clusters of eight 34 us, one block each 65; 64 in clusters of four 42, one block each 69, of
-    // eight 52.  150 by temperature 21 with one block each, in pairs 26.)
+    // Up to four blocks share a row of more than 32,768 logits where the rows leave SMs without one of the two blocks they hold; a FixedSum has a limit.  In us,
+    // 1 / 2 / 4 / 8 blocks: one row of 131,072 by temperature 23 / 17 / 13 / 12, by top-k 50 and top-p 12 / 12 / 12 / 14, by top-p alone 55 / 42 / 34 / 30; 64 of
+    // them 39 / 26 / 19 / 32, 18 / 15 / 15 / 34, 86 / 60 / 45 / 76; one row of 32,000 12 / 11 / 10 / 10, 9 / 11 / 10 / 12, 30 / 30 / 27 / 26, 32 of them
+    // 12 / 15 / 13 / 13, 10 / 14 / 13 / 20, 30 / 36 / 32 / 37.
     const int span = a.V + 16 / int(sizeof(T)) - 1;                        // with what a row's alignment may put before it
     const int steps = (span + kSampleStep - 1) / kSampleStep;
     int blocks = 1;
     auto terms = [&] { return (steps + blocks * kSampleWarps - 1) / (blocks * kSampleWarps) * (kSampleStep / 32); };
-    while (blocks < kSampleMaxCluster && ((int64_t(a.N) * blocks <= device_sms() && span > blocks * 4096) || terms() > kSampleMostTerms)) blocks *= 2;
+    while (blocks < kSampleMaxCluster && ((int64_t(a.N) * blocks <= device_sms() && a.V > 32768) || terms() > kSampleMostTerms)) blocks *= 2;
     static std::atomic<bool> done[kMaxDevices];
     const cudaError_t e = ensure_smem(sample_kernel<T>, int(sizeof(SampleShared)), done);
     if (e != cudaSuccess) return e;

@@ -4,7 +4,7 @@
 // cluster size, the batch around the row or the way the sums are split (in FP32, sums in another order move the borders of the
 // distribution by 1e-7, and one row in a few hundred with a flat distribution draws its neighbour).
 //
-// A block, or a cluster of up to eight where there are few rows, works on a row; every warp owns neighbouring logits.  The row is read from DRAM once, for
+// A block, or a cluster of up to four where there are few and long rows, works on a row; every warp owns neighbouring logits.  The row is read from DRAM once, for
 // its maximum; what is looked at again comes from L1 or L2 (kept in shared memory, rows of 131,072 left room for clusters of eight blocks of 16,384 only,
 // whose barriers cost more than the second reading: 1,024 rows, as first built, 302 us against 245).  Then
 //   maximum -> (top-k, top-p: the cut) -> sums of the kept weights per warp -> the part of the row in which the random number falls, again by
@@ -21,7 +21,7 @@
 //
 // Bounds, at 1,024 rows of 131,072 BF16 logits (268 MB, 41 us at the measured copy rate): greedy rows, read once, 51 us; by temperature alone 126, 17
 // instructions a logit, 14 of them expf and the sum; top-p alone 250 to 295, nearly 40 (a histogram, then that sum with the candidates); both with some
-// 60 % of the issue slots in use; top-k 50 72 to 78, with the chain of its short steps; a mixture of all 137.  A single row of 32,000: 12 us, of which the
+// 60 % of the issue slots in use; top-k 50 72 to 78, with the chain of its short steps; a mixture of all 137.  A single row of 32,000: 9 us, of which the
 // barriers and reads of its chain are nearly all.
 #pragma once
 
@@ -38,7 +38,7 @@ namespace dsv4 {
 
 constexpr int kSampleThreads = 512;
 constexpr int kSampleWarps = kSampleThreads / 32;
-constexpr int kSampleMaxCluster = 8;
+constexpr int kSampleMaxCluster = 4;
 constexpr int kSampleStep = 256;                 // logits a warp looks at at a time, eight neighbouring ones a lane
 constexpr int kSampleOneBits = 40;               // weights are multiples of 2^-40
 constexpr int kSampleList = 2048;                // candidates
