@@ -21,7 +21,7 @@
 //
 // Bounds, at 1,024 rows of 131,072 BF16 logits (268 MB, 41 us at the measured copy rate): greedy rows, read once, 51 us; by temperature alone 126, 17
 // instructions a logit, 14 of them expf and the sum; top-p alone 250 to 295, nearly 40 (a histogram, then that sum with the candidates); both with some
-// 60 % of the issue slots in use; top-k 50 72 to 78, with the chain of its short steps; a mixture of all 137.  A single row of 32,000: 9 us, of which the
+// 60 % of the issue slots in use; top-k 50 65 to 71, with the chain of its short steps; a mixture of all 134.  A single row of 32,000: 9 us, of which the
 // barriers and reads of its chain are nearly all.
 #pragma once
 
