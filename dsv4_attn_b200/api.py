@@ -598,12 +598,12 @@ def hca_tree_decode(q, kv_pool, block_table, kv_len, win_pool, win_len, tree_mas
     win_pool uint8 [B, W, 656] (committed tokens and drafts); tree_mask int32 [B, T, words], bit w % 32 of word w // 32:
     the node sees window row w (`layout.pack_tree_mask`).  Returns (out bf16 [B, T, H, 512], lse f32 [B, T, H]).
 
-    `num_splits` None: where the nodes fill the device more than once the call plans the work on the device
-    (as `plan_hca(B, 1, T * H, kv_len[:, None], win_len[:, None])` does, which can be passed as `plan` to all layers
-    of a step instead); otherwise rows are split so that it is full.
     `share_rows` None: where a request has several groups of 128 (node, head) rows, its entries are dequantised once, into a
     workspace of `tree_rows_bytes(B, max_pages, W)` that the call allocates, instead of by each group; True and False say so,
-    and a uint8 tensor is the workspace."""
+    and a uint8 tensor (on a 32-byte boundary) is the workspace.
+    `num_splits` None: few groups are split so that the device is full; many are dealt out whole, the longest first, where
+    they share rows, and else planned on the device in the call.  A plan that cuts them evenly, made once for all layers of a
+    step by `plan_hca(B, 1, T * H, kv_len[:, None], win_len[:, None])`, goes to `plan`."""
     r = _host.tree(q, kv_pool, block_table, kv_len, win_pool, win_len, tree_mask, sm_scale, attn_sink, num_splits, out, lse, workspace, status, max_len,
                    None if plan is None else plan.fast, share_rows)
     if r is not None:

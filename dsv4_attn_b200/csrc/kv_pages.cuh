@@ -286,12 +286,13 @@ __global__ void __launch_bounds__(kPagesPlanThreads) kv_compact_plan_kernel(cons
     const int tid = threadIdx.x;
     int mine = 0, live = 0;
     int32_t refs[kPlanPages];
-    for (int64_t p = int64_t(tid) * kPlanPages; p < a.num_pages; p += kPlanChunk) mine += __popc(held_pages(a, p, refs));
+    uint32_t last = 0u;                                // of the chunk looked at last, which is the only one of most pools
+    for (int64_t p = int64_t(tid) * kPlanPages; p < a.num_pages; p += kPlanChunk) mine += __popc(last = held_pages(a, p, refs));
     block_prefix(mine, s_warp, live);
     int holes = 0, movers = 0;
     for (int64_t base = 0; base < a.num_pages; base += kPlanChunk) {
         const int64_t p = base + int64_t(tid) * kPlanPages;
-        const uint32_t held = held_pages(a, p, refs), all = pool_pages(a, p);
+        const uint32_t held = a.num_pages <= kPlanChunk ? last : held_pages(a, p, refs), all = pool_pages(a, p);
         const uint32_t low = p + kPlanPages <= live ? ~0u : (p < live ? (1u << (live - p)) - 1u : 0u);      // pages below `live`
         uint32_t hole_bits = ~held & all & low, mover_bits = held & ~low;
         // (both counts of a chunk fit 16 bits)
