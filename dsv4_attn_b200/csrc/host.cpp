@@ -490,8 +490,10 @@ bool same_device(const at::Tensor* like, std::initializer_list<const at::Tensor*
 // the call from four for every pair on: a plan overlaps the set-up of one with the end of another's and costs 6 us and a merge.
 constexpr int64_t kTreeDealtGroups = 74, kTreeDealtRequests = 256, kTreePlanGroups = 4 * 74;
 // Where the groups of a request share its dequantised entries: from four groups a request and 900 tiles over all groups on (960 tiles in 64 groups: 32 us against
-// 34, 480 in 32 groups 28 against 27; three groups a request 158 against 149), for workspaces of up to 4 GB.
-constexpr int64_t kTreeShareGroups = 4, kTreeShareTiles = 900, kTreeShareBytes = int64_t(4) << 30;
+// 34, 480 in 32 groups 28 against 27); where there are more groups than pairs from three a request on (64 x 3 groups of 15 tiles 78 us against 99, 30 x 3 of 7
+// tiles 35 against 47, 100 x 3 ragged ones of up to 127 tiles 512 against 557), and with two while the rows stay near L2 (100 x 2 ragged ones of up to 34
+// tiles, 230 MB, 118 against 136; 64 x 2 of up to 393, 1.9 GB, 741 against 678); for workspaces of up to 4 GB.  (One group a request: 212 against 170.)
+constexpr int64_t kTreeShareGroups = 4, kTreeShareTiles = 900, kTreeShareTwoBytes = int64_t(256) << 20, kTreeShareBytes = int64_t(4) << 30;
 
 // (q, kv_pool, block_table, kv_len, win_pool, win_len, tree_mask, sm_scale, attn_sink, num_splits, out, lse, workspace, status, max_len, plan, share_rows)
 PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -516,7 +518,9 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
     at::Tensor own_rows;
     const at::Tensor* shared = nullptr;
     const int64_t rows_bytes = lib.tree_rows_bytes(int(B), int(table->size(1)), int(W));
-    if (a[16] == Py_True || (a[16] == Py_None && groups >= kTreeShareGroups * B && groups * ((max_len + 63) / 64) >= kTreeShareTiles && rows_bytes > 0 && rows_bytes <= kTreeShareBytes)) {
+    const bool waves = groups > kTreeDealtGroups && B <= kTreeDealtRequests && (groups >= 3 * B || (groups >= 2 * B && rows_bytes <= kTreeShareTwoBytes));
+    const bool share = (waves || (groups >= kTreeShareGroups * B && groups * ((max_len + 63) / 64) >= kTreeShareTiles)) && rows_bytes > 0 && rows_bytes <= kTreeShareBytes;
+    if (a[16] == Py_True || (a[16] == Py_None && share)) {
         if (rows_bytes <= 0) return none();
         try {
             own_rows = empty({rows_bytes}, at::kByte, q);
