@@ -714,7 +714,7 @@ def _pages_done(r, what):
 
 def kv_pages_copy(kv_pool, src, dst, *, status=None) -> None:
     """Page src[i] to page dst[i] (int32, negative: left out) in every layer of kv_pool uint8 [pages, 64, 656] or
-    [layers, pages, 64, 656].  No page is named twice among dst, nor in both lists."""
+    [layers, pages, 64, 656].  No page is named twice among dst, nor in both lists (the latter is reported: status says 11)."""
     r = _host.pages_copy(kv_pool, src, dst, status)
     if r is None:
         _pages_pool(kv_pool)
@@ -725,8 +725,9 @@ def kv_pages_copy(kv_pool, src, dst, *, status=None) -> None:
 
 def kv_entries_move(pool, src, dst, *, status=None) -> None:
     """Entry src[i] to entry dst[i] (int32, negative: left out) in every layer.  pool uint8 [layers, rows, n, 656] or [rows, n, 656]
-    (a window buffer, or a cache by pages); entry numbers count through a layer: row * n + place.  Accepted drafts to their places.
-    No entry is named twice among dst, nor in both lists."""
+    (a window buffer, or a cache by pages); entry numbers count through a layer: row * n + place.  Accepted drafts to their places, a window
+    that slides: all entries are read before any is written, so that the lists may overlap (beyond 16,384 entries a call they must not: nothing is moved
+    then, and status says 11).  No entry is named twice among dst."""
     r = _host.entries_move(pool, src, dst, status)
     if r is None:
         _check(isinstance(pool, torch.Tensor) and pool.dim() in (3, 4), f"pool must be [rows, n, {ENTRY_BYTES}] or [layers, rows, n, {ENTRY_BYTES}]")

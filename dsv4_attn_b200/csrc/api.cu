@@ -1079,14 +1079,31 @@ dim3 copy_grid(int64_t units) {
 extern "C" int dsv4_kv_pages_copy(const Dsv4KvPagesParams* p, void* stream) {
     if (p == nullptr || !pages_pool_ok(p) || p->n < 0 || (p->n > 0 && (p->src == nullptr || p->dst == nullptr))) return int(cudaErrorInvalidValue);
     if (p->n == 0) return 0;
-    return int(launch(kv_copy_pages_kernel, copy_grid(int64_t(p->n) * p->layers * kCopyBatches), kPagesThreads, 0, static_cast<cudaStream_t>(stream), pages_args(p)));
+    dim3 grid = copy_grid(int64_t(p->n) * p->layers * kCopyBatches);
+    if (p->status != nullptr) grid.x += 1;                       // (the block that compares the lists)
+    return int(launch(kv_copy_pages_kernel, grid, kPagesThreads, p->status != nullptr ? PagesMeet::bytes(p->n, p->num_pages) : 0, static_cast<cudaStream_t>(stream), pages_args(p)));
 }
 
 extern "C" int dsv4_kv_entries_move(const Dsv4KvPagesParams* p, void* stream) {
     if (p == nullptr || p->pool == nullptr || !aligned(p->pool, 16) || p->layers <= 0 || p->layers > 0x7FFFFFFF || p->entries <= 0) return int(cudaErrorInvalidValue);
     if (p->n < 0 || (p->n > 0 && (p->src == nullptr || p->dst == nullptr))) return int(cudaErrorInvalidValue);
     if (p->n == 0) return 0;
-    return int(launch(kv_move_entries_kernel, copy_grid(int64_t(p->n) * p->layers), kPagesThreads, 0, static_cast<cudaStream_t>(stream), pages_args(p)));
+    KvPagesArgs a = pages_args(p);
+    // blocks that are resident at once, whose warps take as many entries at a time as make their rounds equal
+    const int64_t resident = int64_t(device_sms()) * kMoveBlocks, warps = resident * (kMoveThreads / 32), each = (int64_t(a.n) * a.layers + warps - 1) / warps;
+    const int64_t rounds = (each + kMoveGroup - 1) / kMoveGroup;
+    a.group = int((each + rounds - 1) / rounds);
+    const int64_t units = (a.n + a.group - 1) / a.group * a.layers, blocks = (units + kMoveThreads / 32 - 1) / (kMoveThreads / 32);
+    // shared memory: for the comparison of the lists; and a column of eight vectors of all entries, or what there is room for, down to a 32-bit word
+    int64_t bytes = EntriesMeet::bytes(a.n, a.entries);
+    const bool vectors = a.n <= kMoveStage / 4;
+    a.width = vectors ? (kMoveStage / 4 / a.n < 8 ? kMoveStage / 4 / a.n : 8) : a.n <= kMoveStage ? kMoveStage / a.n : 0;
+    const int64_t column = int64_t(a.width) * a.n * (vectors ? 16 : 4);
+    if (column > bytes) bytes = column;
+    static std::atomic<bool> done[kMaxDevices];
+    const cudaError_t e = ensure_smem(kv_move_entries_kernel, kMoveStage * 4, done);
+    if (e != cudaSuccess) return int(e);
+    return int(launch(kv_move_entries_kernel, dim3(unsigned(blocks < resident ? blocks : resident)), kMoveThreads, size_t(bytes + 15) / 16 * 16, static_cast<cudaStream_t>(stream), a));
 }
 
 extern "C" int dsv4_kv_pages_free(const Dsv4KvPagesParams* p, void* stream) {

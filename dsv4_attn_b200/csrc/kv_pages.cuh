@@ -6,7 +6,7 @@
 // function of the arguments alone: free pages are taken in ascending order, and counts are integers, whose atomics commute.
 //
 // Measured: a pool of 4,600 pages in eight layers packed (751 MB moved) 126 us, 5.9 TB/s, of which the plan by one block is 9; 48 requests of 4,000 entries
-// forked through 16 layers 12.8 us and four in one layer 8.6, two launches in a chain each; accepted rows of 64 requests in 16 layers 3.2.
+// forked through 16 layers 12.8 us and four in one layer 8.6, two launches in a chain each; accepted rows of 64 requests in 16 layers 3.7, of which the comparison of the lists is 0.8.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -27,6 +27,12 @@ constexpr int kPagesPlanThreads = 1024;
 constexpr int kCopyVecs = 256;
 constexpr int kCopyBatches = (kPageVecs + kCopyVecs - 1) / kCopyVecs;
 constexpr int kStatusNoPage = 10;                                // a fork found no free page
+constexpr int kStatusOverlap = 11;                               // too long a list of copies or moves whose sources and destinations overlap
+// Comparing the lists of a copy or a move.
+constexpr int kMeetTable = 4096, kMeetFew = kMeetTable / 2;
+constexpr int kMoveThreads = 512, kMoveBlocks = 2;                // an SM
+constexpr int kMoveStage = 16384;                                // 32-bit words of a column
+constexpr int kMoveGroup = kCopyVecs / kEntryVecs;               // entries of a warp at a time, at most
 
 struct KvPagesArgs {
     uint4* pool;                 // [layers, num_pages, 64, 656 bytes]
@@ -46,6 +52,8 @@ struct KvPagesArgs {
     int32_t* to;                 // scratch [num_pages]: where they go, ascending
     int32_t* moves;              // scratch [1]: how many move
     int64_t entries;             // move: entries per layer
+    int width;                   // move: words of an entry in a column
+    int group;                   // move: entries of a warp at a time
     int32_t* status;
 };
 
@@ -62,40 +70,183 @@ __device__ __forceinline__ void copy_batch(uint4* dst, const uint4* src, int at,
 
 __device__ __forceinline__ bool in_pool(const KvPagesArgs& a, int page) { return page >= 0 && page < a.num_pages; }
 
-// Page src[i] of every layer to page dst[i].  A negative number leaves the pair out; one beyond the pool is reported.
+// Whether pair i, of items below `count`, is copied: a negative number leaves it out, and so does one out of range.
+__device__ __forceinline__ bool item_pair(const KvPagesArgs& a, int64_t count, int i, int& s, int& d) {
+    s = ptx::ld(a.src + i);
+    d = ptx::ld(a.dst + i);
+    return s >= 0 && d >= 0 && s < count && d < count;
+}
+
+// Whether any item is in both lists, found out by one block; every thread calls.  A bit per item of the pool, ROOM of them at a time: the sources set theirs, the
+// destinations look.  Short lists in a pool of more than ROOM: a table of the sources, at most half full.
+template <int THREADS, int ROOM>
+struct Meet {
+    static_assert(ROOM / 8 >= kMeetTable * 4, "room for the table");
+    static __host__ __device__ bool by_table(int n, int64_t count) { return n <= kMeetFew && count > ROOM; }
+    // (shared memory that it takes)
+    static __host__ __device__ int bytes(int n, int64_t count) { return by_table(n, count) ? kMeetTable * 4 : int((count < ROOM ? count : ROOM) + 127) / 128 * 16; }
+    // (needs no global memory: before the wait)
+    static __device__ __forceinline__ void clear(const KvPagesArgs& a, int64_t count, int32_t* words) {
+        const int vecs = bytes(a.n, count) / 16, fill = by_table(a.n, count) ? -1 : 0;
+        for (int i = threadIdx.x; i < vecs; i += THREADS) reinterpret_cast<int4*>(words)[i] = make_int4(fill, fill, fill, fill);
+        __syncthreads();
+    }
+    static __device__ __forceinline__ bool find(const KvPagesArgs& a, int64_t count, int32_t* words) {
+        const int tid = threadIdx.x;
+        if (by_table(a.n, count)) {
+            auto place_of = [](int item) { return (uint32_t(item) * 2654435769u) >> 20; };       // 12 bits; then the first free place from there on
+            constexpr uint32_t kLast = kMeetTable - 1;
+            for (int i = tid; i < a.n; i += THREADS) {
+                int s, d;
+                if (!item_pair(a, count, i, s, d)) continue;
+                for (uint32_t at = place_of(s);; at = (at + 1u) & kLast) {
+                    const int there = atomicCAS(&words[at], -1, s);
+                    if (there == -1 || there == s) break;
+                }
+            }
+            __syncthreads();
+            bool mine = false;
+            for (int i = tid; i < a.n; i += THREADS) {
+                int s, d;
+                if (item_pair(a, count, i, s, d))
+                    for (uint32_t at = place_of(d); words[at] != -1; at = (at + 1u) & kLast) mine |= words[at] == d;
+            }
+            return __syncthreads_or(mine);
+        }
+        uint32_t* const bits = reinterpret_cast<uint32_t*>(words);
+        for (int64_t begin = 0;;) {
+            const int64_t end = min(count, begin + ROOM);
+#pragma unroll 4
+            for (int i = tid; i < a.n; i += THREADS) {
+                int s, d;
+                if (item_pair(a, count, i, s, d) && s >= begin && s < end) atomicOr(&bits[(s - begin) >> 5], 1u << ((s - begin) & 31));
+            }
+            __syncthreads();
+            bool mine = false;
+#pragma unroll 4
+            for (int i = tid; i < a.n; i += THREADS) {
+                int s, d;
+                if (item_pair(a, count, i, s, d) && d >= begin && d < end) mine |= (bits[(d - begin) >> 5] >> ((d - begin) & 31)) & 1u;
+            }
+            if (__syncthreads_or(mine)) return true;
+            begin = end;
+            if (begin >= count) return false;
+            for (int i = tid; i < ROOM / 32; i += THREADS) bits[i] = 0u;
+            __syncthreads();
+        }
+    }
+};
+using PagesMeet = Meet<kPagesThreads, 1 << 17>;
+using EntriesMeet = Meet<kMoveThreads, kMoveStage * 32>;
+
+// Page src[i] of every layer to page dst[i].  A negative number leaves the pair out; one beyond the pool is reported.  So are lists that overlap, by a block
+// more (where there is a status): nobody waits for it, and what such pages hold is not known afterwards.
 __global__ void __launch_bounds__(kPagesThreads) kv_copy_pages_kernel(const __grid_constant__ KvPagesArgs a) {
+    extern __shared__ __align__(16) int32_t s_words[];
     ptx::pdl_trigger();
     ptx::pdl_wait();
-    const int lane = threadIdx.x & 31;
+    const int blocks = int(gridDim.x) - (a.status != nullptr), lane = threadIdx.x & 31;
+    if (int(blockIdx.x) == blocks) {
+        PagesMeet::clear(a, a.num_pages, s_words);
+        if (PagesMeet::find(a, a.num_pages, s_words) && threadIdx.x == 0) report_status(a.status, kStatusOverlap, 6, a.n);
+        return;
+    }
     const int64_t units = int64_t(a.n) * a.layers * kCopyBatches;
-    for (int64_t u = int64_t(blockIdx.x) * (kPagesThreads / 32) + (threadIdx.x >> 5); u < units; u += int64_t(gridDim.x) * (kPagesThreads / 32)) {
+    for (int64_t u = int64_t(blockIdx.x) * (kPagesThreads / 32) + (threadIdx.x >> 5); u < units; u += int64_t(blocks) * (kPagesThreads / 32)) {
         const int batch = int(u % kCopyBatches);
         const int64_t page = u / kCopyBatches, layer = page / a.n;
-        const int i = int(page % a.n), s = ptx::ld(a.src + i), d = ptx::ld(a.dst + i);
-        if (s < 0 || d < 0) continue;
-        if (!in_pool(a, s) || !in_pool(a, d)) {
-            if (lane == 0) report_status(a.status, kStatusBadIndex, 6, i);
+        int s, d;
+        if (!item_pair(a, a.num_pages, int(page % a.n), s, d)) {
+            if (lane == 0 && s >= 0 && d >= 0) report_status(a.status, kStatusBadIndex, 6, int(page % a.n));
             continue;
         }
         copy_batch(a.pool + (layer * a.num_pages + d) * kPageVecs, a.pool + (layer * a.num_pages + s) * kPageVecs, batch * kCopyVecs, kPageVecs, lane);
     }
 }
 
-// Entry src[i] of every layer to entry dst[i] (numbers within a layer).
-__global__ void __launch_bounds__(kPagesThreads) kv_move_entries_kernel(const __grid_constant__ KvPagesArgs a) {
-    ptx::pdl_trigger();
-    ptx::pdl_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t units = int64_t(a.n) * a.layers;
-    for (int64_t u = int64_t(blockIdx.x) * (kPagesThreads / 32) + (threadIdx.x >> 5); u < units; u += int64_t(gridDim.x) * (kPagesThreads / 32)) {
-        const int64_t layer = u / a.n;
-        const int i = int(u % a.n), s = ptx::ld(a.src + i), d = ptx::ld(a.dst + i);
-        if (s < 0 || d < 0) continue;
-        if (s >= a.entries || d >= a.entries) {
-            if (lane == 0) report_status(a.status, kStatusBadIndex, 6, i);
-            continue;
+// Moved entries of lists that overlap.  The same few words of every entry, a.width of T, are a column of a layer; no two columns touch the same bytes.  A block
+// brings a column of all entries to shared memory, meets, and writes it.
+template <typename T>
+__device__ __forceinline__ void move_columns(const KvPagesArgs& a, T* s_stage) {
+    constexpr int kWords = kEntryVecs * 16 / int(sizeof(T));
+    const int tid = threadIdx.x;
+    const int64_t columns = (kWords + a.width - 1) / a.width, units = columns * a.layers;
+#pragma unroll 1
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const int first = int(u % columns) * a.width, w = min(a.width, kWords - first), total = a.n * w;
+        T* const base = reinterpret_cast<T*>(a.pool) + u / columns * a.entries * kWords + first;
+#pragma unroll 4
+        for (int at = tid; at < total; at += kMoveThreads) {
+            const int i = at / w;
+            int s, d;
+            if (item_pair(a, a.entries, i, s, d)) s_stage[at] = ptx::ld(base + int64_t(s) * kWords + (at - i * w));
         }
-        copy_batch(a.pool + (layer * a.entries + d) * kEntryVecs, a.pool + (layer * a.entries + s) * kEntryVecs, 0, kEntryVecs, lane);
+        __syncthreads();
+        // (a thread takes back what it put there: the next column needs no barrier before it)
+#pragma unroll 4
+        for (int at = tid; at < total; at += kMoveThreads) {
+            const int i = at / w;
+            int s, d;
+            if (item_pair(a, a.entries, i, s, d)) base[int64_t(d) * kWords + (at - i * w)] = s_stage[at];
+        }
+    }
+}
+
+// Entry src[i] of every layer to entry dst[i] (numbers within a layer), as if all were read before any is written: accepted rows close up, a window slides.
+// A warp takes up to six entries of a layer at a time.  The first ones are on their way while every block finds out whether the lists overlap; if they do not, as
+// with rows that go to places of their own, the order does not matter; else the entries go by columns, as long as one of a single 32-bit word fits.
+__global__ void __launch_bounds__(kMoveThreads, kMoveBlocks) kv_move_entries_kernel(const __grid_constant__ KvPagesArgs a) {
+    extern __shared__ __align__(16) uint4 s_stage[];
+    int32_t* const s_words = reinterpret_cast<int32_t*>(s_stage);
+    ptx::pdl_trigger();
+    EntriesMeet::clear(a, a.entries, s_words);
+    ptx::pdl_wait();
+    constexpr int kWarps = kMoveThreads / 32;
+    const int lane = threadIdx.x & 31, vecs = a.group * kEntryVecs;
+    const int64_t groups = (a.n + a.group - 1) / a.group, units = groups * a.layers;
+    int64_t u = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+    uint4 v[kCopyVecs / 32];
+    int to = -1;                                       // of entry `lane` of the group
+    uint4* base = a.pool;
+    auto read = [&]() {
+        const int i = int(u % groups) * a.group + lane;
+        int s = -1;
+        to = -1;
+        if (u < units && lane < a.group && i < a.n && !item_pair(a, a.entries, i, s, to)) {
+            if (s >= 0 && to >= 0) report_status(a.status, kStatusBadIndex, 6, i);
+            to = -1;
+        }
+        base = a.pool + u / groups * a.entries * kEntryVecs;
+#pragma unroll
+        for (int j = 0; j < kCopyVecs / 32; ++j) {
+            if (j * 32 >= vecs) break;
+            const int at = j * 32 + lane, of = at / kEntryVecs, s_of = __shfl_sync(0xFFFFFFFFu, s, of), to_of = __shfl_sync(0xFFFFFFFFu, to, of);
+            if (at < vecs && to_of >= 0) v[j] = ptx::ldg_stream_v4(base + int64_t(s_of) * kEntryVecs + (at - of * kEntryVecs));
+        }
+    };
+    read();
+    if (EntriesMeet::find(a, a.entries, s_words)) {
+        if (blockIdx.x == 0)                           // (those that no warp has come to)
+            for (int i = threadIdx.x; i < a.n; i += kMoveThreads) {
+                int s, d;
+                if (!item_pair(a, a.entries, i, s, d) && s >= 0 && d >= 0) report_status(a.status, kStatusBadIndex, 6, i);
+            }
+        if (a.n <= kMoveStage / 4) move_columns(a, s_stage);
+        else if (a.n <= kMoveStage) move_columns(a, s_words);
+        else if (blockIdx.x == 0 && threadIdx.x == 0) report_status(a.status, kStatusOverlap, 6, a.n);
+        return;
+    }
+#pragma unroll 1
+    for (;;) {
+#pragma unroll
+        for (int j = 0; j < kCopyVecs / 32; ++j) {
+            if (j * 32 >= vecs) break;
+            const int at = j * 32 + lane, of = at / kEntryVecs, to_of = __shfl_sync(0xFFFFFFFFu, to, of);
+            if (at < vecs && to_of >= 0) base[int64_t(to_of) * kEntryVecs + (at - of * kEntryVecs)] = v[j];
+        }
+        u += int64_t(gridDim.x) * kWarps;
+        if (u >= units) break;
+        read();
     }
 }
 

@@ -96,7 +96,10 @@ typedef struct Dsv4KvPagesParams {
     int32_t*       status;
 } Dsv4KvPagesParams;
 
-/* Page src[i] to page dst[i] in every layer.  No page is named twice among dst, nor in both lists. */
+#define DSV4_STATUS_OVERLAP 11  /* lists of a copy or a move overlap where they must not */
+
+/* Page src[i] to page dst[i] in every layer.  No page is named twice among dst, nor in both lists: the latter is reported (DSV4_STATUS_OVERLAP), and what
+ * such pages hold afterwards is unspecified. */
 int dsv4_kv_pages_copy(const Dsv4KvPagesParams* p, void* stream);
 
 /* Child dst[i] becomes a copy of parent src[i]: it shares the parent's full pages (one reference more each), and
@@ -112,8 +115,9 @@ int dsv4_kv_pages_free(const Dsv4KvPagesParams* p, void* stream);
  * the k-th free page below it, in every layer.  new_table and new_refs are the tables afterwards. */
 int dsv4_kv_pages_compact(const Dsv4KvPagesParams* p, void* stream);
 
-/* Entry src[i] to entry dst[i] in every layer (accepted drafts to their places).  No entry is named twice among dst, nor in
- * both lists. */
+/* Entry src[i] to entry dst[i] in every layer, as if all of them were read before any is written: accepted drafts to their places, also where those
+ * are other accepted drafts' (rows that close up, a window that slides).  No entry is named twice among dst.  Lists of more than 16,384 entries must not
+ * overlap: if they do, nothing is moved, and it is reported (DSV4_STATUS_OVERLAP). */
 int dsv4_kv_entries_move(const Dsv4KvPagesParams* p, void* stream);
 
 /*
