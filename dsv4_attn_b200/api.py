@@ -591,7 +591,7 @@ def indexer_topk(q_fp8, q_weight, key_pages, block_table, n_vis, k, *, scores=No
 
 # ── a speculative step (include/dsv4_speculative.h) ──
 def hca_tree_decode(q, kv_pool, block_table, kv_len, win_pool, win_len, tree_mask, sm_scale, *, attn_sink=None, num_splits=None,
-                    out=None, lse=None, workspace=None, status=None, max_len=None, plan=None, share_rows=None):
+                    out=None, lse=None, workspace=None, status=None, max_len=None, plan=None, share_rows=None, check_fp16_range=False):
     """HCA decode of the T drafted nodes of a tree per request, in one call: every node attends to the request's
     compressed entries [0, kv_len[b]) and to the rows of its window buffer that the node's mask names.
     q bf16 [B, T, H, 576]; kv_pool uint8 [P, 64, 656]; block_table int32 [B, max_pages]; kv_len / win_len int32 [B];
@@ -603,7 +603,16 @@ def hca_tree_decode(q, kv_pool, block_table, kv_len, win_pool, win_len, tree_mas
     and a uint8 tensor (on a 32-byte boundary) is the workspace.
     `num_splits` None: few groups are split so that the device is full; many are dealt out whole, the longest first, where
     they share rows, and else planned on the device in the call.  A plan that cuts them evenly, made once for all layers of a
-    step by `plan_hca(B, 1, T * H, kv_len[:, None], win_len[:, None])`, goes to `plan`."""
+    step by `plan_hca(B, 1, T * H, kv_len[:, None], win_len[:, None])`, goes to `plan`.  `max_len` (longest kv_len + win_len) only steers
+    these choices; without it they go by the block table's capacity.
+    Operands pass through FP16: |q| < 65504 and block scales <= 146 (larger ones are clamped), no e4m3 NaN in rows that any node sees.
+    `check_fp16_range` looks at the first two on the host, for callers that cannot vouch for them."""
+    if check_fp16_range:
+        _cuda_contig(q, "q", torch.bfloat16, 4)
+        for name, t in (("kv_pool", kv_pool), ("win_pool", win_pool)):
+            _cuda_contig(t, name, torch.uint8, 3)
+            _check(t.shape[2] == ENTRY_BYTES, f"{name}'s last dim must be {ENTRY_BYTES}")
+        check_fp16_operand_range(q, kv_pool, win_pool)
     r = _host.tree(q, kv_pool, block_table, kv_len, win_pool, win_len, tree_mask, sm_scale, attn_sink, num_splits, out, lse, workspace, status, max_len,
                    None if plan is None else plan.fast, share_rows)
     if r is not None:
