@@ -10,6 +10,8 @@
 // wrong, so that messages and exception types are defined in one place.
 #include <Python.h>
 
+#include <algorithm>
+
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
@@ -518,7 +520,9 @@ PyObject* tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
     at::Tensor own_rows;
     const at::Tensor* shared = nullptr;
     const int64_t rows_bytes = lib.tree_rows_bytes(int(B), int(table->size(1)), int(W));
-    const bool waves = groups > kTreeDealtGroups && B <= kTreeDealtRequests && (groups >= 3 * B || (groups >= 2 * B && rows_bytes <= kTreeShareTwoBytes));
+    // (what is read of the rows: with max_len less than the table has room for)
+    const int64_t rows_read = B * ((std::min(max_len, table->size(1) * kPage + W) + 63) / 64) * 64 * 1152;
+    const bool waves = groups > kTreeDealtGroups && B <= kTreeDealtRequests && (groups >= 3 * B || (groups >= 2 * B && rows_read <= kTreeShareTwoBytes));
     const bool share = (waves || (groups >= kTreeShareGroups * B && groups * ((max_len + 63) / 64) >= kTreeShareTiles)) && rows_bytes > 0 && rows_bytes <= kTreeShareBytes;
     if (a[16] == Py_True || (a[16] == Py_None && share)) {
         if (rows_bytes <= 0) return none();
