@@ -1013,22 +1013,26 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
                 // (ties: in units of the largest weight)
                 // (min-p: the bin of the smallest weight it keeps, and two for rounding)
                 const int floor_bin = by_weight && !LIMITED && r.min_p > 0.f ? int(-kSampleBin * logf(r.min_p)) + 3 : kSampleBins;
-                const float goal = by_weight ? float(r.p24) * 5.9604645e-8f * (total + __ull2float_rn(ties) * 9.094947e-13f) : float(wanted);
+                // (top-p 0: the first bin that has any)
+                const float goal = by_weight ? fmaxf(float(r.p24) * 5.9604645e-8f * (total + __ull2float_rn(ties) * 9.094947e-13f), 1e-30f) : float(wanted);
+                // The first bin up to which the goal lies: every thread has its first one, whether or not its bins begin below the goal.  (A sum up to a thread's first
+                // bin is rounded otherwise than the sum up to the last one of the thread before it; where the goal lay between the two, a condition on both sides found no bin.)
                 float place = 0.5f;
-                int crossed = -1;
+                int crossed = kSampleBins - 1;
 #pragma unroll
                 for (int i = 0; i < kPer; ++i) {
                     const int bin = kPer * tid + i;
                     const float v = by_weight ? float(c[i]) * __expf(float(1 - bin) / kSampleBin) : float(c[i]);
-                    if (before < goal && before + v >= goal && crossed < 0) {
-                        atomicMin(&sh.bin, bin);
+                    if (before + v >= goal && crossed == kSampleBins - 1) {
                         crossed = bin;
-                        place = (goal - before) / v;
+                        if (v > 0.f) place = __saturatef((goal - before) / v);
                     }
                     before += v;
                     if (bin == floor_bin) sh.by_min_p = before;
                     counts[bin] = n_before += c[i];
                 }
+                const int first_bin = __reduce_min_sync(0xFFFFFFFFu, crossed);
+                if (lane == 0) atomicMin(&sh.bin, first_bin);
                 __syncthreads();
                 if (crossed == sh.bin) sh.place = place;
                 // Where all that min-p keeps weighs clearly less than top-p's share, top-p leaves out none of it: no cut.  A bin's tokens are within one bin of
