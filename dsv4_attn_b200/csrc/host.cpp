@@ -486,15 +486,14 @@ bool same_device(const at::Tensor* like, std::initializer_list<const at::Tensor*
     return true;
 }
 
-// Over shared rows, and with a row group for every pair of SMs (74), the pairs share out whole groups, the longest first: 1,024 groups of 15 tiles 264 us,
-// with a plan that cuts them evenly 302 and its own 12; 92 ragged groups 71 against 90 and 12; 304 ragged groups 170 against 215.  (Groups of one length whose number
-// is just above a multiple of 74 pay for it, 304 of 49 tiles 328 us against 293: who knows that passes a plan.)  Groups that dequantise for themselves are planned in
+// Over shared rows, and with a row group for every pair of SMs (74), the pairs share out whole groups, the longest first: 1,024 groups of 15 tiles 308 us under
+// load, with a plan that cuts them evenly, made before, 330; 92 ragged groups 71 against 80; 304 ragged groups 173 against 206; 304 of 49 tiles, one more round for eight of them, 325 against 357.  Groups that dequantise for themselves are planned in
 // the call from four for every pair on: a plan overlaps the set-up of one with the end of another's and costs 6 us and a merge.
 constexpr int64_t kTreeDealtGroups = 74, kTreeDealtRequests = 256, kTreePlanGroups = 4 * 74;
-// Where the groups of a request share its dequantised entries: from four groups a request and 900 tiles over all groups on (960 tiles in 64 groups: 32 us against
-// 34, 480 in 32 groups 28 against 27); where there are more groups than pairs from three a request on (64 x 3 groups of 15 tiles 78 us against 99, 30 x 3 of 7
-// tiles 35 against 47, 100 x 3 ragged ones of up to 127 tiles 512 against 557), and with two while the rows stay near L2 (100 x 2 ragged ones of up to 34
-// tiles, 230 MB, 118 against 136; 64 x 2 of up to 393, 1.9 GB, 741 against 678); for workspaces of up to 4 GB.  (One group a request: 212 against 170.)
+// Where the groups of a request share its dequantised entries: from four groups a request and 900 tiles over all groups on (960 tiles in 64 groups: 29 us against
+// 33, 480 in 32 groups 30 against 25); where there are more groups than pairs from three a request on (64 x 3 groups of 15 tiles 86 us against 98, 30 x 3 of 7
+// tiles 31 against 40, 100 x 3 ragged ones of up to 127 tiles 473 against 503), and with two while the rows stay near L2 (100 x 2 ragged ones of up to 34
+// tiles, 230 MB, 121 against 127; 64 x 2 of up to 393, 1.9 GB, 817 against 718); for workspaces of up to 4 GB.  (One group a request: 178 against 132.)
 constexpr int64_t kTreeShareGroups = 4, kTreeShareTiles = 900, kTreeShareTwoBytes = int64_t(256) << 20, kTreeShareBytes = int64_t(4) << 30;
 
 // (q, kv_pool, block_table, kv_len, win_pool, win_len, tree_mask, sm_scale, attn_sink, num_splits, out, lse, workspace, status, max_len, plan, share_rows)

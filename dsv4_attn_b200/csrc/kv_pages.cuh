@@ -250,7 +250,8 @@ __global__ void __launch_bounds__(kMoveThreads, kMoveBlocks) kv_move_entries_ker
     }
 }
 
-// The pages of request src[i] are given back: one reference less each, its row of the table -1, its length 0.  One block per request.
+// The pages of request src[i] are given back: one reference less each, its row of the table -1, its length 0.  One block per request: all
+// of its threads have read the length before the barrier behind which it is written.
 __global__ void __launch_bounds__(kPagesThreads) kv_free_kernel(const __grid_constant__ KvPagesArgs a) {
     ptx::pdl_trigger();
     ptx::pdl_wait();
@@ -329,7 +330,8 @@ __device__ __forceinline__ uint32_t pool_pages(const KvPagesArgs& a, int64_t p) 
 }
 
 // First half of a fork, one block: the children whose parent ends in a partly filled page get the lowest-numbered free pages, in the order
-// of the children.  Writes those pages' table slots and counts, and the children's lengths.
+// of the children.  Writes those pages' table slots and counts, and the children's lengths:
+// places that it does not read again, the lengths because no child is a parent, the counts because a later round looks at pages from `next` on.
 __global__ void __launch_bounds__(kPagesPlanThreads) kv_fork_plan_kernel(const __grid_constant__ KvPagesArgs a) {
     __shared__ int s_warp[32];
     __shared__ int s_free[kPagesPlanThreads];          // free pages for the children of this round
@@ -388,7 +390,8 @@ __global__ void __launch_bounds__(kPagesPlanThreads) kv_fork_plan_kernel(const _
     }
 }
 
-// Second half: units of a child are its table row and 4 KB batches of its partly filled page in every layer.
+// Second half: units of a child are its table row and 4 KB batches of its partly filled page in every layer.  (A row's unit leaves the slot of that page, which the
+// batches read, as the plan wrote it; parents' rows are only read.)
 __global__ void __launch_bounds__(kPagesThreads) kv_fork_apply_kernel(const __grid_constant__ KvPagesArgs a) {
     ptx::pdl_trigger();
     ptx::pdl_wait();
@@ -429,7 +432,7 @@ __global__ void __launch_bounds__(kPagesThreads) kv_fork_apply_kernel(const __gr
 }
 
 // First half of a compaction, one block: with `count` live pages, the k-th live page from `count` on goes to the k-th free page below it (which
-// moves as few pages as possible, and none over another that has yet to move).
+// moves as few pages as possible, and none over another that has yet to move).  new_refs may be refs: all counts have been read before the barrier behind which they change.
 __global__ void __launch_bounds__(kPagesPlanThreads) kv_compact_plan_kernel(const __grid_constant__ KvPagesArgs a) {
     __shared__ int s_warp[32];
     ptx::pdl_trigger();

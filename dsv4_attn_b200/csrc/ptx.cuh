@@ -39,8 +39,9 @@ __device__ __forceinline__ uint32_t globaltimer_lo() {
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 template <class T>
 __device__ __forceinline__ T ld(const T* p) { return *p; }
-// Lengths, tables and plans, which no kernel both reads and writes: in volatile asm they stay below the wait as well, without being ordered
+// Lengths, tables, counts and plans: in volatile asm they stay below the wait as well, without being ordered
 // against every other memory access of the kernel (as ordinary loads they made the decode kernel 4 KB longer and 6 % slower).
+// A kernel that writes such an array too has a barrier between a place's loads and its stores, or does not read what it has written (kv_pages.cuh).
 __device__ __forceinline__ int32_t ld(const int32_t* p) {
     int32_t v;
     asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(p));

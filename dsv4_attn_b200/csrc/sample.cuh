@@ -19,9 +19,10 @@
 // next to them if the exact sums say so.  Equal logits of sixteen bits are counted, not listed; what else is too much for the lists is gone through
 // by digits of ordered bits.
 //
-// Bounds, at 1,024 rows of 131,072 BF16 logits (268 MB, 41 us at the measured copy rate): greedy rows, read once, 51 us; by temperature alone 126, 17
-// instructions a logit, 14 of them expf and the sum; top-p alone 250 to 295, nearly 40 (a histogram, then that sum with the candidates); both with some
-// 60 % of the issue slots in use; top-k 50 65 to 71, with the chain of its short steps; a mixture of all 134.  A single row of 32,000: 9 us, of which the
+// Bounds, at 1,024 rows of 131,072 BF16 logits (268 MB, 41 us at the measured copy rate): greedy rows, read once, 54 us; by temperature alone 125, 18
+// instructions a logit, 14 of them expf and the sum, and 1,760 a warp whatever its row's length; top-p alone 255 to 315, 36 and 3,800 (a histogram, then that sum with the
+// candidates); both with some 60 % of the issue slots in use, at 64 registers a thread, of which 72 to 152 bytes are spilled; top-k 50 71, with the chain of its short
+// steps; a mixture of all 134.  A cut among thousands of nearly equal logits, found digit by digit, takes ten to twenty times as long as others.  A single row of 32,000: 9 us, of which the
 // barriers and reads of its chain are nearly all.
 #pragma once
 
@@ -742,7 +743,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const __grid_
     row.lane = lane;
     // The row's steps are dealt out evenly: every warp of the cluster has neighbouring ones, in the order of the vocabulary.
     const int row_steps = (row.end + kSampleStep - 1) / kSampleStep, parts = int(blocks) * kSampleWarps, me = int(rank) * kSampleWarps + warp;
-    auto first_step = [&](int part) { return row_steps * part / parts; };       // (at most 16,385 steps and 128 parts)
+    auto first_step = [&](int part) { return row_steps * part / parts; };       // (at most 16,385 steps and 64 parts)
     const int first = first_step(me) * kSampleStep, steps = first_step(me + 1) - first_step(me);
 
     // ── maximum ──

@@ -8,11 +8,11 @@
 // What that changes per tile of 64 entries and SM: 69 KB by TMA from L2 instead of 30 KB of raw records, but no raw reads, conversions and
 // operand stores, which kept the shared-memory port busy for 1130 of its 2000 cycles.  Bounds, in SM cycles: tensor pipe 1244 (as there), shared-memory port 540
 // in + 860 out, L2 at the measured 16.4 TB/s (58 bytes a cycle and SM) 1190.  The direct kernel takes 2570.  512 groups of 15 tiles take 2000 with their
-// set-up and output, and the tensor pipe is at work for 68 % of the kernel's cycles; from some 500 groups on the power limit holds the clock at 1.4 to
-// 1.6 GHz (1,024 groups: 265 us, 1.0 PFLOP/s, where a library product sustains 1.38).
+// set-up and output, and the tensor pipe is at work for 68 % of the kernel's cycles; from some 500 groups on the power limit holds the clock at
+// 1.5 GHz: 1,024 groups take 265 to 269 us for the first calls after a pause and 308 under load, 0.86 PFLOP/s (a library product: 1.39, at 1.32 GHz).
 //
-// Rounding: an entry is e4m3 x scale in FP16, in the same operations as in the direct kernel; results differ from it in nothing but the
-// order of sums.
+// Rounding: an entry is e4m3 x scale in FP16, in the same operations as in the direct kernel (the scale is rounded, then the product: up to 2^-10 of an element);
+// results differ from it in nothing but the order of sums.  At its 128 registers the attention kernel spills 44 bytes, the unpacking 4 at 64.
 #pragma once
 
 #include "decode_kernel.cuh"

@@ -23,7 +23,8 @@ extern "C" {
  * tree_mask[b][t] is set where node t sees window row w.  The window buffer holds the last
  * committed tokens and the drafted ones; a node's bits leave out tokens that have slid out
  * of its window and drafts that are not its ancestors.  A node that sees nothing gives 0 and
- * an lse of -inf.  Arithmetic, preconditions and NaN rows as for dsv4_hca_dense_decode_fwd.
+ * an lse of -inf.  Arithmetic, preconditions and NaN rows as for dsv4_hca_dense_decode_fwd: |q| < 65504, block scales <= 146 (below 6e-5, FP16's smallest normal
+ * number, they lose accuracy), no e4m3 NaN in a row that any node sees.
  *
  * num_splits >= 1: a static grid of that many pieces per row group (> 1 needs partial_o and partial_lse of
  * num_splits * B * T * H rows, as dsv4_attn_workspace_bytes(B, T * H, ...) says).  num_splits = 0: `sched` is a plan;
