@@ -92,13 +92,13 @@ struct Meet {
         __syncthreads();
     }
     static __device__ __forceinline__ bool find(const KvPagesArgs& a, int64_t count, int32_t* words) {
-        const int tid = threadIdx.x;
+        const uint32_t n = uint32_t(a.n), tid = threadIdx.x;      // (a counter that passes n may pass 2^31)
         if (by_table(a.n, count)) {
             auto place_of = [](int item) { return (uint32_t(item) * 2654435769u) >> 20; };       // 12 bits; then the first free place from there on
             constexpr uint32_t kLast = kMeetTable - 1;
-            for (int i = tid; i < a.n; i += THREADS) {
+            for (uint32_t i = tid; i < n; i += THREADS) {
                 int s, d;
-                if (!item_pair(a, count, i, s, d)) continue;
+                if (!item_pair(a, count, int(i), s, d)) continue;
                 for (uint32_t at = place_of(s);; at = (at + 1u) & kLast) {
                     const int there = atomicCAS(&words[at], -1, s);
                     if (there == -1 || there == s) break;
@@ -106,9 +106,9 @@ struct Meet {
             }
             __syncthreads();
             bool mine = false;
-            for (int i = tid; i < a.n; i += THREADS) {
+            for (uint32_t i = tid; i < n; i += THREADS) {
                 int s, d;
-                if (item_pair(a, count, i, s, d))
+                if (item_pair(a, count, int(i), s, d))
                     for (uint32_t at = place_of(d); words[at] != -1; at = (at + 1u) & kLast) mine |= words[at] == d;
             }
             return __syncthreads_or(mine);
@@ -117,21 +117,21 @@ struct Meet {
         for (int64_t begin = 0;;) {
             const int64_t end = min(count, begin + ROOM);
 #pragma unroll 4
-            for (int i = tid; i < a.n; i += THREADS) {
+            for (uint32_t i = tid; i < n; i += THREADS) {
                 int s, d;
-                if (item_pair(a, count, i, s, d) && s >= begin && s < end) atomicOr(&bits[(s - begin) >> 5], 1u << ((s - begin) & 31));
+                if (item_pair(a, count, int(i), s, d) && s >= begin && s < end) atomicOr(&bits[(s - begin) >> 5], 1u << ((s - begin) & 31));
             }
             __syncthreads();
             bool mine = false;
 #pragma unroll 4
-            for (int i = tid; i < a.n; i += THREADS) {
+            for (uint32_t i = tid; i < n; i += THREADS) {
                 int s, d;
-                if (item_pair(a, count, i, s, d) && d >= begin && d < end) mine |= (bits[(d - begin) >> 5] >> ((d - begin) & 31)) & 1u;
+                if (item_pair(a, count, int(i), s, d) && d >= begin && d < end) mine |= (bits[(d - begin) >> 5] >> ((d - begin) & 31)) & 1u;
             }
             if (__syncthreads_or(mine)) return true;
             begin = end;
             if (begin >= count) return false;
-            for (int i = tid; i < ROOM / 32; i += THREADS) bits[i] = 0u;
+            for (uint32_t i = tid; i < ROOM / 32; i += THREADS) bits[i] = 0u;
             __syncthreads();
         }
     }
@@ -209,11 +209,11 @@ __global__ void __launch_bounds__(kMoveThreads, kMoveBlocks) kv_move_entries_ker
     int to = -1;                                       // of entry `lane` of the group
     uint4* base = a.pool;
     auto read = [&]() {
-        const int i = int(u % groups) * a.group + lane;
+        const int64_t i = u % groups * a.group + lane;
         int s = -1;
         to = -1;
-        if (u < units && lane < a.group && i < a.n && !item_pair(a, a.entries, i, s, to)) {
-            if (s >= 0 && to >= 0) report_status(a.status, kStatusBadIndex, 6, i);
+        if (u < units && lane < a.group && i < a.n && !item_pair(a, a.entries, int(i), s, to)) {
+            if (s >= 0 && to >= 0) report_status(a.status, kStatusBadIndex, 6, int(i));
             to = -1;
         }
         base = a.pool + u / groups * a.entries * kEntryVecs;
@@ -227,9 +227,9 @@ __global__ void __launch_bounds__(kMoveThreads, kMoveBlocks) kv_move_entries_ker
     read();
     if (EntriesMeet::find(a, a.entries, s_words)) {
         if (blockIdx.x == 0)                           // (those that no warp has come to)
-            for (int i = threadIdx.x; i < a.n; i += kMoveThreads) {
+            for (uint32_t i = threadIdx.x; i < uint32_t(a.n); i += kMoveThreads) {
                 int s, d;
-                if (!item_pair(a, a.entries, i, s, d) && s >= 0 && d >= 0) report_status(a.status, kStatusBadIndex, 6, i);
+                if (!item_pair(a, a.entries, int(i), s, d) && s >= 0 && d >= 0) report_status(a.status, kStatusBadIndex, 6, int(i));
             }
         if (a.n <= kMoveStage / 4) move_columns(a, s_stage);
         else if (a.n <= kMoveStage) move_columns(a, s_words);
