@@ -140,3 +140,17 @@ def test_numbers_out_of_range_next_to_others(lib, what, n):
     st = lib.new_status("cuda")
     (lib.kv_pages_copy if what == "pages" else lib.kv_entries_move)(items, i32(src), i32(dst), status=st)
     assert st[0].item() == 7 and torch.equal(flat, want)
+
+
+@pytest.mark.parametrize("layers,n", [(1, 1), (7, 5), (16, 321), (40, 1024), (61, 2049), (9, 16385)])
+def test_lists_that_do_not_overlap(lib, layers, n):
+    """As many entries as a warp takes at once, and several rounds of them for every warp, the last one a part of one; some left out."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    items = filled(layers, 1, 2 * n + 3, seed=n)
+    order = torch.randperm(2 * n + 3, device="cuda", generator=g)
+    src, dst = order[:n].clone(), order[n:2 * n].clone()
+    src[1::5], dst[4::7] = -1, -1
+    want = moved(items[:, 0], src, dst)
+    st = lib.new_status("cuda")
+    lib.kv_entries_move(items, i32(src), i32(dst), status=st)
+    assert torch.equal(items[:, 0], want) and st.tolist() == [0, 0, 0, 0]
