@@ -12,7 +12,8 @@ import importlib
 
 _API = ("Dsv4Error", "alloc_workspace", "combine", "csa_sparse_decode", "csa_sparse_decode_noalloc", "csa_compress_reduce_fwd", "hca_compress_fwd", "kv_quantize_insert", "hca_packed_decode", "rope_norm", "indexer_topk", "hca_decode_fwd", "hca_dense_decode",
         "new_status", "plan_splits", "plan_csa", "plan_hca", "Plan", "check_fp16_operand_range",
-        "hca_tree_decode", "tree_rows_bytes", "sample", "kv_pages_copy", "kv_pages_fork", "kv_pages_free", "kv_pages_compact", "kv_entries_move")
+        "hca_tree_decode", "tree_rows_bytes", "sample", "kv_pages_copy", "kv_pages_fork", "kv_pages_free", "kv_pages_compact", "kv_entries_move",
+        "gqa_decode", "gqa_prefill", "gqa_insert", "kv_evict")
 __all__ = ["LIB", "library_path", "layout", "synth", *_API]
 
 

@@ -70,7 +70,7 @@ EXPORTS = ("dsv4_attn_version", "dsv4_debug_set_wait", "dsv4_debug_set_flags", "
            "dsv4_attn_workspace_bytes", "hca_decode_fwd", "dsv4_hca_compress_fwd", "dsv4_kv_quantize_insert",
            "dsv4_hca_packed_decode_fwd", "dsv4_rope_norm_fwd", "dsv4_indexer_topk_fwd",
            "dsv4_hca_tree_decode_fwd", "dsv4_hca_tree_rows_bytes", "dsv4_kv_pages_copy", "dsv4_kv_pages_fork", "dsv4_kv_pages_free", "dsv4_kv_pages_compact", "dsv4_kv_entries_move",
-           "dsv4_sample_fwd")
+           "dsv4_sample_fwd", "dsv4_gqa_decode_fwd", "dsv4_gqa_prefill_fwd", "dsv4_gqa_workspace_bytes", "dsv4_gqa_insert", "dsv4_kv_evict")
 
 
 class CsaCompressReduceParams(C.Structure):
@@ -165,6 +165,36 @@ class SampleParams(C.Structure):
     ]
 
 
+class GqaParams(C.Structure):
+    _fields_ = [
+        ("B", C.c_int32), ("T", C.c_int32), ("Hkv", C.c_int32), ("G", C.c_int32), ("D", C.c_int32), ("max_pages", C.c_int32), ("window", C.c_int32), ("first", C.c_int32),
+        ("q_dtype", C.c_int32), ("kv_dtype", C.c_int32), ("sm_scale", C.c_float), ("max_len", C.c_int32), ("rows", C.c_int64), ("num_pages", C.c_int64),
+        ("q_stride_b", C.c_int64), ("q_stride_t", C.c_int64), ("q_stride_h", C.c_int64), ("q", C.c_void_p), ("q_start", C.c_void_p), ("k_pool", C.c_void_p),
+        ("v_pool", C.c_void_p), ("block_table", C.c_void_p), ("kv_len", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p), ("attn_sink", C.c_void_p),
+        ("out", C.c_void_p), ("lse", C.c_void_p), ("weights", C.c_void_p), ("weight_stride", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+        ("status", C.c_void_p),
+    ]
+
+
+class GqaInsertParams(C.Structure):
+    _fields_ = [
+        ("B", C.c_int32), ("T", C.c_int32), ("Hkv", C.c_int32), ("D", C.c_int32), ("max_pages", C.c_int32), ("src_dtype", C.c_int32), ("kv_dtype", C.c_int32),
+        ("reserved0", C.c_int32), ("rows", C.c_int64), ("num_pages", C.c_int64), ("k_stride_b", C.c_int64), ("k_stride_t", C.c_int64), ("k_stride_h", C.c_int64),
+        ("v_stride_b", C.c_int64), ("v_stride_t", C.c_int64), ("v_stride_h", C.c_int64), ("k", C.c_void_p), ("v", C.c_void_p), ("q_start", C.c_void_p),
+        ("n_rows", C.c_void_p), ("k_pool", C.c_void_p), ("v_pool", C.c_void_p), ("block_table", C.c_void_p), ("insert_pos", C.c_void_p), ("k_scale", C.c_void_p),
+        ("v_scale", C.c_void_p), ("status", C.c_void_p),
+    ]
+
+
+class KvEvictParams(C.Structure):
+    _fields_ = [
+        ("B", C.c_int32), ("max_pages", C.c_int32), ("pools", C.c_int32), ("keep", C.c_int32), ("first", C.c_int32), ("recent", C.c_int32), ("num_pages", C.c_int64),
+        ("layers", C.c_int64), ("keep_each", C.c_void_p), ("block_table", C.c_void_p), ("kv_len", C.c_void_p), ("refs", C.c_void_p), ("weights", C.c_void_p),
+        ("weight_stride", C.c_int64), ("new_table", C.c_void_p), ("new_len", C.c_void_p), ("new_refs", C.c_void_p), ("new_weights", C.c_void_p), ("kept", C.c_void_p),
+        ("scratch", C.c_void_p), ("status", C.c_void_p), ("pool", C.c_void_p * 4), ("entry_bytes", C.c_int64 * 4),
+    ]
+
+
 def _load() -> C.CDLL:
     path = library_path()
     if not path.exists():
@@ -197,7 +227,11 @@ def _load() -> C.CDLL:
                      ("dsv4_kv_pages_free", KvPagesParams),
                      ("dsv4_kv_pages_compact", KvPagesParams),
                      ("dsv4_kv_entries_move", KvPagesParams),
-                     ("dsv4_sample_fwd", SampleParams)):
+                     ("dsv4_sample_fwd", SampleParams),
+                     ("dsv4_gqa_decode_fwd", GqaParams),
+                     ("dsv4_gqa_prefill_fwd", GqaParams),
+                     ("dsv4_gqa_insert", GqaInsertParams),
+                     ("dsv4_kv_evict", KvEvictParams)):
         fn = getattr(lib, name)
         fn.restype = C.c_int
         fn.argtypes = [P(st), C.c_void_p]
@@ -211,6 +245,8 @@ def _load() -> C.CDLL:
     lib.dsv4_attn_sched_bytes.argtypes = [C.c_int, C.c_int, C.c_int, C.c_int, P(C.c_int64), P(C.c_int64)]
     lib.dsv4_hca_tree_rows_bytes.restype = C.c_int64
     lib.dsv4_hca_tree_rows_bytes.argtypes = [C.c_int, C.c_int, C.c_int]
+    lib.dsv4_gqa_workspace_bytes.restype = C.c_int64
+    lib.dsv4_gqa_workspace_bytes.argtypes = [P(GqaParams)]
     lib.dsv4_noalloc_scratch_bytes.restype = C.c_int64
     lib.dsv4_noalloc_scratch_bytes.argtypes = []
     lib.dsv4_attn_last_error.restype = C.c_char_p

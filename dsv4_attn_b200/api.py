@@ -62,7 +62,8 @@ ENTRY_POINTS = (
     "dsv4_kv_quantize_insert", "dsv4_csa_compress_reduce_fwd", "dsv4_hca_compress_fwd", "dsv4_indexer_topk_fwd", "dsv4_attn_combine",
     "dsv4_attn_plan", "dsv4_attn_plan_splits",
     "dsv4_hca_tree_decode_fwd", "dsv4_attn_sched_bytes", "dsv4_kv_pages_copy", "dsv4_kv_pages_fork", "dsv4_kv_pages_free", "dsv4_kv_pages_compact",
-    "dsv4_kv_entries_move", "dsv4_sample_fwd", "dsv4_hca_tree_rows_bytes")
+    "dsv4_kv_entries_move", "dsv4_sample_fwd", "dsv4_hca_tree_rows_bytes",
+    "dsv4_gqa_decode_fwd", "dsv4_gqa_prefill_fwd", "dsv4_gqa_workspace_bytes", "dsv4_gqa_insert", "dsv4_kv_evict")
 _host.bind(*(C.cast(getattr(_lib.LIB, name), C.c_void_p).value for name in ENTRY_POINTS))
 
 
@@ -792,3 +793,156 @@ def kv_pages_compact(kv_pool, block_table, page_refs, *, new_table=None, new_ref
     if type(r) is tuple:
         return r
     _pages_done(r, "dsv4_kv_pages_compact")
+
+
+# ── pages of ordinary K and V heads (include/dsv4_gqa.h) ──
+_GQA_TYPES = (torch.bfloat16, torch.float16)
+
+
+def _gqa_pools(k_pool, v_pool, k_scale, v_scale, block_table, B, dtype):
+    """Checks of K and V pages; returns (Hkv, D)."""
+    for name, t in (("k_pool", k_pool), ("v_pool", v_pool)):
+        _check(isinstance(t, torch.Tensor) and t.is_cuda and t.is_contiguous(), f"{name} must be a contiguous cuda tensor")
+        _check(t.dim() == 4 and t.shape[1] == PAGE_ENTRIES and t.numel() > 0, f"{name} must be [pages, {PAGE_ENTRIES}, kv_heads, head_dim]")
+        _check(t.dtype in (*_GQA_TYPES, torch.float8_e4m3fn), f"{name} must be bf16, f16 or float8_e4m3fn, got {t.dtype}")
+    _check(k_pool.shape == v_pool.shape and k_pool.dtype == v_pool.dtype, "k_pool and v_pool must have one shape and type")
+    Hkv, D = k_pool.shape[2:]
+    eight = k_pool.dtype == torch.float8_e4m3fn
+    _check(eight or k_pool.dtype == dtype, f"pools must be {dtype} or float8_e4m3fn, got {k_pool.dtype}")
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        _check((t is not None) == eight, f"{name} goes with float8_e4m3fn pools, and only with those")
+        if t is not None:
+            _cuda_contig(t, name, torch.float32, 1)
+            _check(t.shape[0] == Hkv, f"{name} must be [kv_heads]")
+    _cuda_contig(block_table, "block_table", torch.int32, 2)
+    _check(block_table.shape[0] == B and block_table.shape[1] > 0, "block_table must be [B, max_pages]")
+    return Hkv, D
+
+
+def _gqa_rows(t, name, packed):
+    _check(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a cuda tensor")
+    _check(t.dim() == (3 if packed else 4), f"{name} must be {'[rows, heads, head_dim]' if packed else '[B, T, heads, head_dim]'}")
+    _check(t.dtype in _GQA_TYPES, f"{name} must be bf16 or f16, got {t.dtype}")
+    _check(t.shape[-1] <= 1 or t.stride(-1) == 1, f"the elements of a head of {name} must be contiguous")
+    _check(all(n <= 1 or (s % 8 == 0 and s >= 0) for n, s in zip(t.shape[:-1], t.stride()[:-1])), f"the strides of {name} must be multiples of 8")
+    _check(t.data_ptr() % 16 == 0, f"{name} must start on a 16-byte boundary")
+
+
+def _gqa(what, q, q_start, k_pool, v_pool, block_table, kv_len, sm_scale, window, first, k_scale, v_scale, attn_sink, weights, max_len, out, lse, status):
+    r = _host.gqa(q, q_start, k_pool, v_pool, block_table, kv_len, sm_scale, window, first, k_scale, v_scale, attn_sink, weights, max_len, out, lse, status)
+    if r is not None:
+        return r if type(r) is tuple else _rc(r, what)
+    packed = what == "dsv4_gqa_prefill_fwd"
+    _gqa_rows(q, "q", packed)
+    _cuda_contig(kv_len, "kv_len", torch.int32, 1)
+    B, H = kv_len.shape[0], q.shape[-2]
+    _check(B > 0 and (packed or q.shape[0] == B), "kv_len must be [B], B > 0")
+    if packed:
+        _cuda_contig(q_start, "q_start", torch.int32, 1)
+        _check(q_start.shape[0] == B + 1, "q_start must be [B + 1]")
+    Hkv, D = _gqa_pools(k_pool, v_pool, k_scale, v_scale, block_table, B, q.dtype)
+    _check(q.shape[-1] == D, f"q's last dim must be the pools' head_dim {D}")
+    _check(D in (64, 128, 256), f"head_dim must be 64, 128 or 256, got {D}")
+    _check(H > 0 and H % Hkv == 0, "q's heads must be a multiple of the pools'")
+    _check(float(sm_scale) > 0, "sm_scale must be positive")
+    for name, x in (("window", window), ("first", first), ("max_len", 0 if max_len is None else max_len)):
+        _check(type(x) is int and 0 <= x < 1 << 31, f"{name} must be an int in [0, 2^31)")
+    if attn_sink is not None:
+        _cuda_contig(attn_sink, "attn_sink", torch.float32, 1)
+        _check(attn_sink.shape[0] == H, "attn_sink must be [heads]")
+    if weights is not None:
+        _cuda_contig(weights, "weights", torch.float32, 2)
+        _check(weights.shape[0] == B and weights.shape[1] >= block_table.shape[1] * PAGE_ENTRIES, f"weights must be [B, >= max_pages * {PAGE_ENTRIES}]")
+    for name, t, dtype, shape in (("out", out, q.dtype, q.shape), ("lse", lse, torch.float32, q.shape[:-1])):
+        if t is not None:
+            _cuda_contig(t, name, dtype, len(shape))
+            _check(t.shape == shape, f"{name} must be {list(shape)}")
+            _check(t.data_ptr() % 16 == 0 or name == "lse", f"{name} must start on a 16-byte boundary")
+    _pages_status(status)
+    _check(all(t is None or t.device == q.device for t in (q_start, k_pool, v_pool, block_table, kv_len, k_scale, v_scale, attn_sink, weights, out, lse, status)),
+           "all tensors must be on one device")
+    raise Dsv4Error(f"{what} refused the call (sizes out of range, or no device memory)")
+
+
+def gqa_decode(q, k_pool, v_pool, block_table, kv_len, sm_scale, *, window=0, first=0, k_scale=None, v_scale=None, attn_sink=None, weights=None, max_len=None,
+               out=None, lse=None, status=None):
+    """Attention of T new tokens per request over pages of K and V heads.  q bf16 or f16 [B, T, H, D] (strided rows of a fused projection will do), D 64, 128 or 256; k_pool, v_pool
+    [P, 64, Hkv, D] of q's type, or float8_e4m3fn with k_scale, v_scale f32 [Hkv]; H a multiple of Hkv; block_table int32 [B, max_pages]; kv_len int32 [B]: entries of a
+    request, the new tokens' own (`gqa_insert`) among them.  Token t stands at place kv_len - T + t and sees the entries up to its own, with `window` > 0 those of
+    the last `window` places and the `first` ones only.  Returns (out [B, T, H, D], lse f32 [B, T, H]); a token that sees nothing gives 0 and -inf.
+
+    attn_sink f32 [H]: a logit per head in the denominator.  weights f32 [B, >= max_pages * 64]: to every entry is added what it got of the softmax weights of the call's tokens and
+    heads (what `kv_evict` goes by).  max_len: no kv_len is larger; it steers the launch only, but for `weights`, which entries beyond it do not get.
+    Entries that no token of the call sees may hold anything; the others must be finite."""
+    return _gqa("dsv4_gqa_decode_fwd", q, None, k_pool, v_pool, block_table, kv_len, sm_scale, window, first, k_scale, v_scale, attn_sink, weights, max_len, out, lse, status)
+
+
+def gqa_prefill(q, q_start, k_pool, v_pool, block_table, kv_len, sm_scale, *, window=0, first=0, k_scale=None, v_scale=None, attn_sink=None, out=None, lse=None, status=None):
+    """The same for prompts, or pieces of them: q [rows, H, D] holds the tokens of all requests one behind the other, those of request b in rows q_start[b] to
+    q_start[b + 1] - 1 (int32 [B + 1]); the last of them stands at place kv_len[b] - 1.  Returns (out [rows, H, D], lse f32 [rows, H]); rows of no request are left as they are."""
+    _check(q_start is not None, "q_start must be a tensor")
+    return _gqa("dsv4_gqa_prefill_fwd", q, q_start, k_pool, v_pool, block_table, kv_len, sm_scale, window, first, k_scale, v_scale, attn_sink, None, None, out, lse, status)
+
+
+def gqa_insert(k, v, k_pool, v_pool, block_table, insert_pos, *, q_start=None, n_rows=None, k_scale=None, v_scale=None, status=None) -> None:
+    """New rows of K and V, bf16 or f16 [B, T, Hkv, D], into the pages: row t of request b becomes its entry insert_pos[b] + t (int32 [B]; of the first n_rows[b] rows only
+    where that is given).  With q_start int32 [B + 1] the rows are packed, [rows, Hkv, D], as for `gqa_prefill`.  Pools as for `gqa_decode`; into float8_e4m3fn ones go
+    value / scale[head], rounded to the nearest.  A place outside the table or the pool is left out; status then says 16."""
+    r = _host.gqa_insert(k, v, k_pool, v_pool, block_table, insert_pos, q_start, n_rows, k_scale, v_scale, status)
+    if r is not None:
+        return None if r == 0 else _rc(r, "dsv4_gqa_insert")
+    packed = q_start is not None
+    for name, t in (("k", k), ("v", v)):
+        _gqa_rows(t, name, packed)
+    _check(k.shape == v.shape and k.dtype == v.dtype, "k and v must have one shape and type")
+    _cuda_contig(insert_pos, "insert_pos", torch.int32, 1)
+    B = insert_pos.shape[0]
+    _check(B > 0 and (packed or k.shape[0] == B), "insert_pos must be [B], B > 0")
+    _check(not (packed and n_rows is not None), "n_rows goes with rows that are not packed")
+    for name, t, n in (("q_start", q_start, B + 1), ("n_rows", n_rows, B)):
+        if t is not None:
+            _cuda_contig(t, name, torch.int32, 1)
+            _check(t.shape[0] == n, f"{name} must have {n} values")
+    Hkv, D = _gqa_pools(k_pool, v_pool, k_scale, v_scale, block_table, B, k.dtype)
+    _check(tuple(k.shape[-2:]) == (Hkv, D), "k and v must have the pools' heads and head_dim")
+    _check(D % 8 == 0, "head_dim must be a multiple of 8")
+    _pages_status(status)
+    _check(all(t is None or t.device == k.device for t in (v, k_pool, v_pool, block_table, insert_pos, q_start, n_rows, k_scale, v_scale, status)), "all tensors must be on one device")
+    raise Dsv4Error("dsv4_gqa_insert refused the call (sizes out of range)")
+
+
+def kv_evict(pools, block_table, kv_len, page_refs, weights, keep, *, first=0, recent=0, new_table=None, new_len=None, new_refs=None, new_weights=None, kept=None, status=None):
+    """Requests with more than `keep` entries (an int, or int32 [B]) keep their `first` entries, their last `recent` ones and, of the others, those with the largest weights f32
+    [B, >= max_pages * 64] (as `gqa_decode` adds them up), `keep` in all; equal weights: the lower place.  The entries close up in their order, in place, in every layer of `pools`: one tensor
+    or up to four, each [layers, P, 64, ...] with entries of a multiple of 16 bytes (K and V pages, or the latent cache).  Pages behind the new end are given back, as by
+    `kv_pages_free`.  Returns (block_table, kv_len, page_refs, weights, kept int32 [B, max_pages * 64]: the old places of the entries, -1 behind the last) as they are
+    afterwards; the tensors passed in are left as they were unless they are passed as new_table, new_len, new_refs and new_weights too.
+    A request with a shared page among those that would be written (status says 12) or a page outside the pool (7) stays as it is."""
+    if isinstance(pools, torch.Tensor):
+        pools = (pools,)
+    r = _host.evict(tuple(pools), block_table, kv_len, page_refs, weights, keep, first, recent, new_table, new_len, new_refs, new_weights, kept, status)
+    if r is not None:
+        return r if type(r) is tuple else _rc(r, "dsv4_kv_evict")
+    _pages_tables(block_table, kv_len, page_refs)
+    B, cap, P = block_table.shape[0], block_table.shape[1] * PAGE_ENTRIES, page_refs.shape[0]
+    _check(1 <= len(pools) <= 4, "pools must be one tensor or up to four")
+    for t in pools:
+        _check(isinstance(t, torch.Tensor) and t.is_cuda and t.is_contiguous() and t.dim() >= 4 and t.numel() > 0, "a pool must be a contiguous cuda tensor [layers, pages, 64, ...]")
+        _check(t.shape[1] == P and t.shape[2] == PAGE_ENTRIES and t.shape[0] == pools[0].shape[0], f"pools must be [layers, {P}, {PAGE_ENTRIES}, ...] with the same layers")
+        _check(t[0, 0, 0].numel() * t.element_size() % 16 == 0, "the entries of a pool must be a multiple of 16 bytes")
+    _cuda_contig(weights, "weights", torch.float32, 2)
+    _check(weights.shape[0] == B and weights.shape[1] >= cap, f"weights must be [B, >= max_pages * {PAGE_ENTRIES}]")
+    if isinstance(keep, torch.Tensor):
+        _cuda_contig(keep, "keep", torch.int32, 1)
+        _check(keep.shape[0] == B, "keep must be an int or [B]")
+    for name, x in (("keep", 0 if isinstance(keep, torch.Tensor) else keep), ("first", first), ("recent", recent)):
+        _check(type(x) is int and 0 <= x < 1 << 31, f"{name} must be an int in [0, 2^31)")
+    for name, t, dtype, shape in (("new_table", new_table, torch.int32, block_table.shape), ("new_len", new_len, torch.int32, kv_len.shape),
+                                  ("new_refs", new_refs, torch.int32, page_refs.shape), ("new_weights", new_weights, torch.float32, weights.shape), ("kept", kept, torch.int32, (B, cap))):
+        if t is not None:
+            _cuda_contig(t, name, dtype, len(shape))
+            _check(tuple(t.shape) == tuple(shape), f"{name} must be {list(shape)}")
+    _pages_status(status)
+    given = (*pools, kv_len, page_refs, weights, keep if isinstance(keep, torch.Tensor) else None, new_table, new_len, new_refs, new_weights, kept, status)
+    _check(all(t is None or t.device == block_table.device for t in given), "all tensors must be on one device")
+    raise Dsv4Error("dsv4_kv_evict refused the call (sizes out of range, or no device memory)")

@@ -20,10 +20,10 @@ import sys
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
-SOURCE = HERE / "csrc" / "api.cu"
+SOURCES = (HERE / "csrc" / "api.cu", HERE / "csrc" / "gqa.cu")
 OUT = HERE / "libdsv4_attn.so"
 HEADER = HERE.parent / "include" / "dsv4_attn.h"
-HEADERS = (HEADER, HEADER.with_name("dsv4_speculative.h"))
+HEADERS = (HEADER, HEADER.with_name("dsv4_speculative.h"), HEADER.with_name("dsv4_gqa.h"))
 HOST_SOURCE = HERE / "csrc" / "host.cpp"
 DEPS = [p for p in sorted((HERE / "csrc").glob("*")) if p != HOST_SOURCE] + list(HEADERS)
 
@@ -69,7 +69,7 @@ def build(force: bool = False, ptxas_v: bool = False, quiet: bool = False) -> Pa
     cmd = [nvcc, "-std=c++17", "-O3", "-lineinfo",
            "-gencode", "arch=compute_100a,code=sm_100a",
            "-shared", "-Xcompiler", "-fPIC",
-           "-o", str(OUT), str(SOURCE)]
+           f"--threads={len(SOURCES)}", "-o", str(OUT), *map(str, SOURCES)]
     if ptxas_v:
         cmd[1:1] = ["-Xptxas", "-v"]
     if not quiet:

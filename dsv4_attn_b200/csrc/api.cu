@@ -23,6 +23,7 @@
 #include "tree_kernel.cuh"
 #include "kv_pages.cuh"
 #include "sample.cuh"
+#include "host_state.h"
 
 namespace dsv4 {
 namespace {
@@ -39,11 +40,9 @@ std::atomic<unsigned long long*> g_trace{nullptr};
 
 thread_local const char* t_last_error = "";
 
-// cuTensorMapEncodeTiled, looked up through the runtime so that the library does
-// not link against libcuda.
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+}  // namespace
+
+HostState host_state() { return {g_dbg.load(std::memory_order_relaxed), g_wait_ns.load(std::memory_order_relaxed), g_drop_tile.load(std::memory_order_relaxed)}; }
 
 EncodeTiledFn encode_tiled_fn() {
     static EncodeTiledFn fn = [] {
@@ -56,6 +55,19 @@ EncodeTiledFn encode_tiled_fn() {
     }();
     return fn;
 }
+
+// SMs of the current device (asked for once per device).
+int device_sms() {
+    static std::atomic<int> known[kMaxDevices];
+    int dev = 0, sms = 148;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return sms;
+    const int k = known[dev].load(std::memory_order_relaxed);
+    if (k > 0) return k;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) known[dev].store(sms, std::memory_order_relaxed);
+    return sms;
+}
+
+namespace {
 
 // Q as a 2-D BF16 tensor [rows, cols], row-major; box = 64 columns x 64 rows (a block's heads), 128-byte swizzle.
 cudaError_t make_q_map(CUtensorMap* map, const void* q, int64_t rows, int cols) {
@@ -140,17 +152,6 @@ cudaError_t ensure_smem(Kernel kernel, int bytes, std::atomic<bool>* done_per_de
         done_per_device[dev].store(true, std::memory_order_release);
     }
     return cudaSuccess;
-}
-
-// SMs of the current device (asked for once per device).
-int device_sms() {
-    static std::atomic<int> known[kMaxDevices];
-    int dev = 0, sms = 148;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return sms;
-    const int k = known[dev].load(std::memory_order_relaxed);
-    if (k > 0) return k;
-    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess) known[dev].store(sms, std::memory_order_relaxed);
-    return sms;
 }
 
 // Layout of a schedule buffer (int32 words); a function of the batch shape only, so that the planner and

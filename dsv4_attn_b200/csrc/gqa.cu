@@ -1,0 +1,258 @@
+// Entry points of include/dsv4_gqa.h: argument validation, tensor maps, launches.  No allocation, no synchronisation, and nothing kept between calls but facts
+// about the device.
+#include "../../include/dsv4_gqa.h"
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <atomic>
+
+#include "gqa_decode.cuh"
+#include "kv_evict.cuh"
+#include "host_state.h"
+
+namespace dsv4 {
+namespace {
+
+constexpr int kMaxDevices = 64;
+
+bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+
+template <typename Kernel>
+cudaError_t ensure_smem(Kernel kernel, int bytes, std::atomic<bool>* done_per_device) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+    if (!done_per_device[dev].load(std::memory_order_acquire)) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e != cudaSuccess) return e;
+        done_per_device[dev].store(true, std::memory_order_release);
+    }
+    return cudaSuccess;
+}
+
+// Every kernel is a programmatic dependent of whatever precedes it in the stream, as in api.cu.
+template <class Args>
+cudaError_t launch(void (*kernel)(Args), dim3 grid, int threads, size_t smem, cudaStream_t stream, const Args& args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = (host_state().flags & 64) ? 0 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args);
+}
+
+// A pool of K or V heads by (element, head, entry): boxes of 128 bytes (or a shorter row) of one head in 64 entries.
+cudaError_t make_pool_map(CUtensorMap* map, const void* pool, int64_t pages, int Hkv, int D, int kv_dtype) {
+    const EncodeTiledFn fn = encode_tiled_fn();
+    if (fn == nullptr) return cudaErrorNotSupported;
+    const bool bytes = kv_dtype == DSV4_DTYPE_E4M3;
+    const int es = bytes ? 1 : 2, box_bytes = D * es < 128 ? D * es : 128;
+    const cuuint64_t dims[3] = {cuuint64_t(D), cuuint64_t(Hkv), cuuint64_t(pages) * kGqaTile};
+    const cuuint64_t strides[2] = {cuuint64_t(D) * es, cuuint64_t(Hkv) * D * es};
+    const cuuint32_t box[3] = {cuuint32_t(box_bytes / es), 1, kGqaTile}, estr[3] = {1, 1, 1};
+    const CUresult r = fn(map, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(pool), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+// ── which form of the kernel ──
+// Rows of a KV head: 16, 32 or 64 in a group, the fewest that hold a request's (with 64: several groups).
+int group_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+constexpr int kMinShare = 2;
+
+template <class C>
+cudaError_t run_decode(GqaArgs& a, cudaStream_t stream) {
+    static std::atomic<bool> done[kMaxDevices];
+    cudaError_t e = ensure_smem(gqa_decode_kernel<C>, C::Bytes, done);
+    if (e != cudaSuccess) return e;
+    return launch(gqa_decode_kernel<C>, dim3(unsigned(a.blocks)), kGqaThreads, C::Bytes, stream, a);
+}
+template <int D, int KVT>
+cudaError_t run_decode(GqaArgs& a, cudaStream_t stream) {
+    if (a.group_rows == 16) return run_decode<GqaCfg<D, KVT, 1, 1>>(a, stream);
+    if (a.group_rows == 32) return run_decode<GqaCfg<D, KVT, 1, 2>>(a, stream);
+    return run_decode<GqaCfg<D, KVT, 1, 4>>(a, stream);
+}
+template <int D>
+cudaError_t run_decode(GqaArgs& a, int kv_dtype, cudaStream_t stream) {
+    if (kv_dtype == DSV4_DTYPE_BF16) return run_decode<D, kGqaBf16>(a, stream);
+    if (kv_dtype == DSV4_DTYPE_F16) return run_decode<D, kGqaF16>(a, stream);
+    return run_decode<D, kGqaE4m3>(a, stream);
+}
+
+// Sizes that a call's blocks and workspace follow from.
+struct Sizes {
+    int blocks, group_rows;
+    int64_t parts;                   // partial rows
+    int64_t logit_rows, logit_stride;
+};
+bool gqa_sizes(const Dsv4GqaParams* p, Sizes& s) {
+    if (p == nullptr || p->B <= 0 || p->Hkv <= 0 || p->G <= 0 || p->max_pages <= 0 || p->T < 0 || p->rows < 0) return false;
+    if (p->D != 64 && p->D != 128 && p->D != 256) return false;
+    const int64_t tokens = p->q_start != nullptr ? p->rows : p->T;          // of a request, at most
+    if (tokens <= 0 || int64_t(p->Hkv) * p->G > 65536 || tokens > (1 << 24) || tokens * p->G > 0x7FFFFFFF / 4 || int64_t(p->max_pages) * kGqaTile > 0x7FFFFFFF) return false;
+    s.group_rows = group_rows(tokens * p->G);
+    const int64_t entries = int64_t(p->max_pages) * kGqaTile;
+    int64_t longest = p->max_len > 0 && p->max_len < entries ? p->max_len : entries;
+    if (p->window > 0 && longest > int64_t(p->window) + p->first + tokens + 2 * kGqaTile) longest = int64_t(p->window) + p->first + tokens + 2 * kGqaTile;
+    const int64_t groups = p->q_start != nullptr ? (p->rows * p->G + s.group_rows - 1) / s.group_rows + p->B : int64_t(p->B) * ((tokens * p->G + s.group_rows - 1) / s.group_rows);
+    const int64_t tiles = groups * p->Hkv * ((longest + kGqaTile - 1) / kGqaTile + 1);
+    const int64_t resident = int64_t(device_sms()) * (p->D > 128 ? 1 : 2), want = (tiles + kMinShare - 1) / kMinShare;
+    s.blocks = int(want < resident ? want : resident);
+    s.parts = 2 * int64_t(s.blocks) * s.group_rows;
+    s.logit_rows = p->weights != nullptr ? int64_t(p->B) * p->Hkv * p->T * p->G : 0;
+    s.logit_stride = entries;
+    return true;
+}
+int64_t up(int64_t n) { return (n + 127) / 128 * 128; }
+
+}  // namespace
+}  // namespace dsv4
+
+using namespace dsv4;
+
+extern "C" int64_t dsv4_gqa_workspace_bytes(const Dsv4GqaParams* p) {
+    Sizes s;
+    if (!gqa_sizes(p, s)) return -1;
+    return up(s.parts * p->D * 4) + up(s.parts * 4) + up(s.logit_rows * s.logit_stride * 4) + up(s.logit_rows * 4);
+}
+
+static int gqa_fwd(const Dsv4GqaParams* p, void* stream_) {
+    Sizes s;
+    if (!gqa_sizes(p, s)) return int(cudaErrorInvalidValue);
+    const bool e4m3 = p->kv_dtype == DSV4_DTYPE_E4M3;
+    if ((p->q_dtype != DSV4_DTYPE_BF16 && p->q_dtype != DSV4_DTYPE_F16) || (!e4m3 && p->kv_dtype != p->q_dtype)) return int(cudaErrorInvalidValue);
+    if (p->num_pages <= 0 || p->num_pages * kGqaTile > 0x7FFFFFFF - kGqaTile || p->window < 0 || p->first < 0 || !(p->sm_scale > 0.f)) return int(cudaErrorInvalidValue);
+    if (!p->q || !p->k_pool || !p->v_pool || !p->block_table || !p->kv_len || !p->out || (e4m3 && (!p->k_scale || !p->v_scale))) return int(cudaErrorInvalidValue);
+    if (p->q_start == nullptr && p->rows != int64_t(p->B) * p->T) return int(cudaErrorInvalidValue);
+    if (!aligned(p->q, 16) || !aligned(p->k_pool, 16) || !aligned(p->v_pool, 16) || !aligned(p->out, 16)) return int(cudaErrorInvalidValue);
+    if (p->q_stride_b % 8 || p->q_stride_t % 8 || p->q_stride_h % 8) return int(cudaErrorInvalidValue);
+    if (p->weights != nullptr && (p->q_start != nullptr || p->weight_stride < s.logit_stride)) return int(cudaErrorInvalidValue);
+    if (p->workspace == nullptr || !aligned(p->workspace, 128) || p->workspace_bytes < dsv4_gqa_workspace_bytes(p)) return int(cudaErrorInvalidValue);
+    const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    const HostState state = host_state();
+
+    GqaArgs a{};
+    a.B = p->B;  a.T = p->T;  a.Hkv = p->Hkv;  a.G = p->G;  a.max_pages = p->max_pages;
+    constexpr int kFar = 1 << 30;                                             // (sums of places stay within 32 bits; no entry is further back)
+    a.window = p->window < kFar ? p->window : kFar;
+    a.first = p->first;
+    a.rows = p->rows;  a.q_start = p->q_start;  a.kv_len = p->kv_len;  a.block_table = p->block_table;  a.num_pages = p->num_pages;
+    a.q = p->q;  a.q_stride_b = p->q_stride_b;  a.q_stride_t = p->q_stride_t;  a.q_stride_h = p->q_stride_h;  a.q_bf16 = p->q_dtype == DSV4_DTYPE_BF16;
+    a.k_scale = e4m3 ? p->k_scale : nullptr;  a.v_scale = e4m3 ? p->v_scale : nullptr;  a.sink = p->attn_sink;
+    a.scale_log2 = p->sm_scale * 1.4426950408889634f;
+    a.out = p->out;  a.lse = p->lse;
+    a.blocks = s.blocks;  a.group_rows = s.group_rows;  a.min_share = kMinShare;
+    uint8_t* ws = static_cast<uint8_t*>(p->workspace);
+    a.part_o = reinterpret_cast<float*>(ws);  ws += up(s.parts * p->D * 4);
+    a.part_lse = reinterpret_cast<float*>(ws);  ws += up(s.parts * 4);
+    if (p->weights != nullptr) {
+        a.logits = reinterpret_cast<float*>(ws);  ws += up(s.logit_rows * s.logit_stride * 4);
+        a.total = reinterpret_cast<float*>(ws);
+        a.logit_stride = s.logit_stride;
+        a.weights = p->weights;  a.weight_stride = p->weight_stride;
+    }
+    a.wait_ns = uint32_t(state.wait_ns < 4000000000ull ? state.wait_ns : 4000000000ull);
+    a.dbg_drop_tile = state.drop_tile;
+    a.status = p->status;
+    cudaError_t e = make_pool_map(&a.k_map, p->k_pool, p->num_pages, p->Hkv, p->D, p->kv_dtype);
+    if (e == cudaSuccess) e = make_pool_map(&a.v_map, p->v_pool, p->num_pages, p->Hkv, p->D, p->kv_dtype);
+    if (e != cudaSuccess) return int(e);
+    e = p->D == 64 ? run_decode<64>(a, p->kv_dtype, stream) : p->D == 128 ? run_decode<128>(a, p->kv_dtype, stream) : run_decode<256>(a, p->kv_dtype, stream);
+    if (e != cudaSuccess) return int(e);
+    const int64_t merge_rows = p->rows * p->Hkv * p->G, merge_blocks = (merge_rows + kGqaMergeRows - 1) / kGqaMergeRows;
+    if (s.blocks > 1) {
+        const dim3 grid{unsigned(merge_blocks)};
+        e = p->D == 64 ? launch(gqa_merge_kernel<64>, grid, kGqaMergeThreads, 0, stream, a)
+                       : p->D == 128 ? launch(gqa_merge_kernel<128>, grid, kGqaMergeThreads, 0, stream, a) : launch(gqa_merge_kernel<256>, grid, kGqaMergeThreads, 0, stream, a);
+        if (e != cudaSuccess) return int(e);
+    }
+    if (p->weights != nullptr) {
+        const int64_t longest = p->max_len > 0 && p->max_len < s.logit_stride ? p->max_len : s.logit_stride;
+        e = launch(gqa_weights_kernel, dim3(unsigned((longest + kGqaWeightThreads - 1) / kGqaWeightThreads), unsigned(p->B)), kGqaWeightThreads, 0, stream, a);
+    }
+    return int(e);
+}
+
+extern "C" int dsv4_gqa_decode_fwd(const Dsv4GqaParams* p, void* stream) {
+    if (p == nullptr || p->q_start != nullptr) return int(cudaErrorInvalidValue);
+    return gqa_fwd(p, stream);
+}
+
+extern "C" int dsv4_gqa_prefill_fwd(const Dsv4GqaParams* p, void* stream) {
+    if (p == nullptr || p->q_start == nullptr || p->weights != nullptr) return int(cudaErrorInvalidValue);
+    return gqa_fwd(p, stream);
+}
+
+extern "C" int dsv4_gqa_insert(const Dsv4GqaInsertParams* p, void* stream) {
+    if (p == nullptr || p->B <= 0 || p->T < 0 || p->rows < 0 || p->Hkv <= 0 || p->max_pages <= 0 || p->num_pages <= 0) return int(cudaErrorInvalidValue);
+    if (p->D <= 0 || p->D % 8 != 0 || int64_t(p->Hkv) * p->D > (1 << 24) || p->num_pages > 0x7FFFFFFF) return int(cudaErrorInvalidValue);
+    const bool e4m3 = p->kv_dtype == DSV4_DTYPE_E4M3;
+    if ((p->src_dtype != DSV4_DTYPE_BF16 && p->src_dtype != DSV4_DTYPE_F16) || (!e4m3 && p->kv_dtype != p->src_dtype)) return int(cudaErrorInvalidValue);
+    if (!p->k || !p->v || !p->k_pool || !p->v_pool || !p->block_table || !p->insert_pos || (e4m3 && (!p->k_scale || !p->v_scale))) return int(cudaErrorInvalidValue);
+    if (!aligned(p->k, 16) || !aligned(p->v, 16) || !aligned(p->k_pool, 16) || !aligned(p->v_pool, 16)) return int(cudaErrorInvalidValue);
+    if (p->q_start == nullptr && (p->T == 0 ? p->rows != 0 : p->rows != int64_t(p->B) * p->T)) return int(cudaErrorInvalidValue);
+    GqaInsertArgs a{};
+    const int64_t strides[6] = {p->k_stride_b, p->k_stride_t, p->k_stride_h, p->v_stride_b, p->v_stride_t, p->v_stride_h};
+    for (int i = 0; i < 6; ++i)
+        if (strides[i] % 8 != 0) return int(cudaErrorInvalidValue);
+    if (p->rows == 0) return 0;
+    a.B = p->B;  a.T = p->T;  a.Hkv = p->Hkv;  a.D = p->D;  a.max_pages = p->max_pages;  a.rows = p->rows;
+    a.q_start = p->q_start;  a.n_rows = p->n_rows;  a.insert_pos = p->insert_pos;  a.block_table = p->block_table;  a.num_pages = p->num_pages;
+    a.src[0] = p->k;  a.src[1] = p->v;
+    for (int i = 0; i < 2; ++i) { a.stride_b[i] = strides[3 * i];  a.stride_t[i] = strides[3 * i + 1];  a.stride_h[i] = strides[3 * i + 2]; }
+    a.src_bf16 = p->src_dtype == DSV4_DTYPE_BF16;
+    a.scale[0] = p->k_scale;  a.scale[1] = p->v_scale;
+    a.pool[0] = p->k_pool;  a.pool[1] = p->v_pool;
+    a.status = p->status;
+    constexpr int kWarps = kGqaInsertThreads / 32;
+    const int64_t blocks = (2 * p->rows + kWarps - 1) / kWarps, most = int64_t(device_sms()) * 8;
+    return int(launch(e4m3 ? gqa_insert_kernel<true> : gqa_insert_kernel<false>, dim3(unsigned(blocks < most ? blocks : most)), kGqaInsertThreads, 0,
+                      static_cast<cudaStream_t>(stream), a));
+}
+
+extern "C" int dsv4_kv_evict(const Dsv4KvEvictParams* p, void* stream_) {
+    if (p == nullptr || p->B <= 0 || p->B > 65535 || p->max_pages <= 0 || p->num_pages <= 0 || p->layers <= 0 || p->pools < 0 || p->pools > DSV4_EVICT_POOLS) return int(cudaErrorInvalidValue);
+    const int64_t cap = int64_t(p->max_pages) * 64;
+    if (p->num_pages * 64 > 0x7FFFFFFF || cap > 0x7FFFFFFF - kEvictPlanThreads * kEvictEach || p->first < 0 || p->recent < 0 || (p->keep_each == nullptr && p->keep < 0))
+        return int(cudaErrorInvalidValue);
+    if (!p->block_table || !p->kv_len || !p->refs || !p->weights || !p->new_table || !p->new_len || !p->new_refs || !p->new_weights || !p->kept || !p->scratch)
+        return int(cudaErrorInvalidValue);
+    if (p->weight_stride < cap || p->weight_stride > 0x7FFFFFFF - kEvictPlanThreads || !aligned(p->scratch, 16)) return int(cudaErrorInvalidValue);
+    const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    KvEvictArgs a{};
+    a.B = p->B;  a.max_pages = p->max_pages;  a.pools = p->pools;  a.num_pages = p->num_pages;  a.layers = p->layers;
+    a.keep = p->keep;  a.first = p->first;  a.recent = p->recent;  a.keep_each = p->keep_each;
+    a.block_table = p->block_table;  a.kv_len = p->kv_len;  a.refs = p->refs;  a.weights = p->weights;  a.weight_stride = p->weight_stride;
+    a.new_table = p->new_table;  a.new_len = p->new_len;  a.new_refs = p->new_refs;  a.new_weights = p->new_weights;  a.kept = p->kept;
+    a.moves = p->scratch;  a.from = p->scratch + 4 * int64_t(p->B);
+    a.status = p->status;
+    int64_t vecs_of_all = 0;
+    for (int i = 0; i < p->pools; ++i) {
+        if (p->pool[i] == nullptr || !aligned(p->pool[i], 16) || p->entry_bytes[i] <= 0 || p->entry_bytes[i] % 16 != 0 || p->entry_bytes[i] > (1 << 20)) return int(cudaErrorInvalidValue);
+        a.pool[i] = static_cast<uint4*>(p->pool[i]);
+        a.vecs[i] = int(p->entry_bytes[i] / 16);
+        vecs_of_all += p->layers * a.vecs[i];
+    }
+    // as wide columns as leave four blocks for every SM, from 512 bytes down to a sector
+    int width = 32;
+    while (width > 2 && vecs_of_all * p->B / width < int64_t(device_sms()) * 4) width /= 2;
+    int64_t columns = 0;
+    for (int i = 0; i < p->pools; ++i) {
+        a.width[i] = width;
+        a.columns[i] = (a.vecs[i] + width - 1) / width;
+        columns += p->layers * a.columns[i];
+    }
+    if (columns > 0x7FFFFFFF) return int(cudaErrorInvalidValue);
+    a.all_columns = int(columns);
+    cudaError_t e = launch(evict_plan_kernel, dim3(unsigned(p->B)), kEvictPlanThreads, 0, stream, a);
+    if (e == cudaSuccess) e = launch(evict_move_kernel, dim3(unsigned(columns < 1 ? 1 : columns), unsigned(p->B)), kEvictMoveThreads, 0, stream, a);
+    return int(e);
+}

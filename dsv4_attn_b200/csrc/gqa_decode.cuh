@@ -1,0 +1,952 @@
+// Attention of new tokens over pages of ordinary K and V heads (grouped queries): the cache's length is shared out evenly over resident blocks.
+//
+// For request b, KV head h and query head h * G + g, a token at place p of its request sees the entries j <= p that exist, with a window those with
+// p - j < window or j < first only, and
+//     out = sum_j exp(x_j - m) v_j / (sum_j exp(x_j - m) + exp(sink - m)),   x_j = sm_scale q . k_j,   lse = m + log sum_j exp(x_j - m)
+//
+// Layout of the work.  The rows of a KV head are its (token, query head) pairs, in groups of R = 16 to 64; a unit is (request, KV head, row group), its tiles the
+// pages of 64 entries that some row of the group sees.  All units' tiles lie behind one another on one axis, which is cut into equal shares, one per resident block: every
+// block streams the same number of tiles whatever the lengths are.  Each block finds its place on the axis by a scan over the
+// lengths (no planner, nothing read back).  A unit inside one share writes its output; one that a cut runs through leaves FP32 partials, which gqa_merge_kernel joins.
+//
+// What bounds it: the bytes of K and V, each read once.  A producer warp keeps a ring of K and V tiles filled by TMA (128-byte swizzle) across the
+// block's units; four warps take 16 entries of a tile each (with more rows: fewer entries, more rows), S = Q K^T and O += P V by mma.sync m16n8k16 with FP32
+// accumulators, the running maximum and sum in registers.  A tile of 64 entries x 128 in 16 bits is 128 instructions of 16 rows: a fifth of the time
+// that its 32 KB take from memory, so that tcgen05's M = 128 would multiply padding and its way through tensor memory would only lengthen
+// the chain; prompts, which do have 128 rows, take gqa_prefill_kernel.
+//
+// Rounding: P is rounded to the type of V (BF16: 2^-9, FP16: 2^-12 of a weight, at most, and at random), everything else is FP32.  An e4m3 cache is read as
+// FP16, which holds its values exactly; BF16 queries then go through FP16 after each row has been brought near 1 by a power of two, which is exact but for elements
+// below 2^-14 of the row's largest (off by 2^-25 of that).
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "ptx.cuh"
+
+namespace dsv4 {
+
+constexpr int kGqaBf16 = 0, kGqaF16 = 1, kGqaE4m3 = 2;            // types of K and V
+constexpr int kGqaTile = 64;                                      // entries of a tile: a page
+constexpr int kGqaConsumers = 128, kGqaThreads = kGqaConsumers + 32;
+constexpr int kGqaMergeThreads = 256, kGqaWeightThreads = 256;
+constexpr int kGqaStatusBadIndex = 7, kGqaStatusWait = 1;
+
+struct GqaArgs {
+    int B, T, Hkv, G, max_pages, window, first;
+    int64_t rows;                    // tokens of all requests (rows of q)
+    const int32_t* q_start;          // [B + 1], or null: T tokens each
+    const int32_t* kv_len;           // [B]
+    const int32_t* block_table;      // [B, max_pages]
+    int64_t num_pages;
+    const void* q;
+    int64_t q_stride_b, q_stride_t, q_stride_h;    // elements (packed tokens: stride_b is not read)
+    int q_bf16;                      // type of q and out
+    const float* k_scale;            // [Hkv], e4m3
+    const float* v_scale;
+    const float* sink;               // [H]
+    float scale_log2;                // sm_scale * log2(e)
+    void* out;                       // [rows, H, D]
+    float* lse;                      // [rows, H]
+    float* part_o;                   // [2 * blocks][R][D]
+    float* part_lse;                 // [2 * blocks][R], log2
+    int blocks;                      // of the attention kernel
+    int group_rows;                  // R
+    int min_share;                   // tiles of a block, at least
+    // weights of the entries
+    float* logits;                   // [B][Hkv * T * G][logit_stride], log2 units; null: not wanted
+    int64_t logit_stride;
+    float* total;                    // [B][Hkv * T * G]: log2 of the denominators
+    float* weights;                  // [B][weight_stride], added to
+    int64_t weight_stride;
+    uint32_t wait_ns;
+    int dbg_drop_tile;
+    int32_t* status;
+    alignas(64) CUtensorMap k_map, v_map;
+};
+
+// ── one request ──
+struct GqaRequest {
+    int tokens, place0, entries;     // new tokens; place of the first of them (negative where the cache is shorter); entries that can be looked up
+    int64_t row0;                    // the first token's row in q
+    bool bad;                        // lengths or offsets that point outside
+};
+__device__ __forceinline__ GqaRequest gqa_request(const GqaArgs& a, int b) {
+    GqaRequest r;
+    const int n = max(ptx::ld(a.kv_len + b), 0);
+    r.bad = false;
+    if (a.q_start != nullptr) {
+        const int s = ptx::ld(a.q_start + b), e = ptx::ld(a.q_start + b + 1), last = int(a.rows);
+        const int lo = min(max(s, 0), last), hi = min(max(e, lo), last);
+        r.bad = lo != s || hi != e;
+        r.row0 = lo;
+        r.tokens = hi - lo;
+    } else {
+        r.row0 = int64_t(b) * a.T;
+        r.tokens = a.T;
+    }
+    const int64_t room = int64_t(a.max_pages) * kGqaTile;
+    r.entries = n < room ? n : int(room);
+    r.bad |= n > room;
+    r.place0 = n - r.tokens;
+    return r;
+}
+
+// ── the tiles of a row group ──
+struct GqaSpan {
+    int t0, t1;                      // its tokens
+    int lo, hi, first;               // entries that some row sees: [0, first) and [lo, hi)
+    int head, skip, count;           // tiles: `head` from 0 on, the others `skip` pages further on; count >= 1 (a group that sees nothing has an empty one)
+    __device__ __forceinline__ int slot(int k) const { return k < head ? k : k + skip; }
+};
+__device__ __forceinline__ GqaSpan gqa_span(const GqaArgs& a, const GqaRequest& r, int rg) {
+    GqaSpan s;
+    const int64_t row = int64_t(rg) * a.group_rows, rows = int64_t(r.tokens) * a.G;
+    s.t0 = int(row / a.G);
+    s.t1 = int((min(row + a.group_rows, rows) - 1) / a.G);
+    s.hi = max(min(r.place0 + s.t1 + 1, r.entries), 0);
+    s.lo = 0;
+    s.first = 0;
+    if (a.window > 0) {
+        s.lo = max(r.place0 + s.t0 - a.window + 1, 0);
+        s.first = min(a.first, s.hi);
+        if (s.lo > s.hi) s.lo = s.hi;
+    }
+    const int end = (s.hi + kGqaTile - 1) / kGqaTile, heads = (s.first + kGqaTile - 1) / kGqaTile, from = s.lo / kGqaTile;
+    s.head = min(heads, from);
+    s.skip = from - s.head;
+    s.count = max(end - s.skip, 1);
+    return s;
+}
+__device__ __forceinline__ int gqa_groups(const GqaArgs& a, const GqaRequest& r) { return int((int64_t(r.tokens) * a.G + a.group_rows - 1) / a.group_rows); }
+// Tiles of one KV head of a request.
+__device__ __forceinline__ int64_t gqa_head_tiles(const GqaArgs& a, const GqaRequest& r) {
+    int64_t n = 0;
+    for (int rg = 0, groups = gqa_groups(a, r); rg < groups; ++rg) n += gqa_span(a, r, rg).count;
+    return n;
+}
+
+// Sum of one value per thread over the threads before this one, and over all.
+template <int THREADS>
+__device__ __forceinline__ int64_t block_prefix(int64_t v, int64_t& total, int64_t* warp_sums) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t x = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int64_t y = __shfl_up_sync(0xFFFFFFFFu, x, d);
+        if (lane >= d) x += y;
+    }
+    if (lane == 31) warp_sums[warp] = x;
+    __syncthreads();
+    int64_t before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+        if (w < warp) before += warp_sums[w];
+        total += warp_sums[w];
+    }
+    return before + x - v;
+}
+
+// The length of a share, which the attention kernel and the merge work out alike.
+__device__ __forceinline__ int64_t gqa_share(const GqaArgs& a, int64_t total) { return max((total + a.blocks - 1) / a.blocks, int64_t(a.min_share)); }
+
+__device__ __noinline__ void gqa_report(int32_t* status, int code, int role, int what) {
+    if (status != nullptr && atomicCAS(status, 0, code) == 0) {
+        status[1] = int(blockIdx.x);
+        status[2] = role;
+        status[3] = what;
+    }
+}
+
+// ── mma.sync ──
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t saddr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(saddr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t saddr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(saddr) : "memory");
+}
+// two e4m3 in the low half of a word -> two FP16, exact
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t w) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t}" : "=r"(r) : "r"(w));
+    return r;
+}
+
+// D: head dimension; KVT: type of K and V; MW: tiles of 16 rows a warp; WM: warps side by side over the rows (4 / WM over the entries)
+template <int D_, int KVT_, int MW_, int WM_>
+struct GqaCfg {
+    static constexpr int D = D_, KVT = KVT_, MW = MW_, WM = WM_, WN = 4 / WM;
+    static constexpr int R = 16 * MW * WM;
+    static constexpr int ES = KVT == kGqaE4m3 ? 1 : 2;
+    static constexpr int RowBytes = D * ES;
+    static constexpr int Box = RowBytes < 128 ? RowBytes : 128;               // bytes of a row in one TMA box, and the width of the swizzle
+    static constexpr int Boxes = RowBytes / Box;
+    static constexpr int Slot = kGqaTile * RowBytes;
+    // Two blocks an SM with 64 KB each on the way cover 128 KB of it; a head of 256 leaves room for one block, with 128 KB.
+    static constexpr int Ring = D > 128 ? 128 * 1024 : 64 * 1024;
+    static constexpr int Slots = Ring / Slot;
+    static constexpr int BlocksPerSm = D > 128 ? 1 : 2;
+    static constexpr int QPitch = D * 2 + 16;                                 // bytes
+    static constexpr int MergePitch = D + 8;                                  // floats
+    static constexpr int Q = R * QPitch, Merge = 4 * 16 * MergePitch * 4;
+    static constexpr int Shared = Q > Merge ? Q : Merge;                      // Q is done with when the warps' parts are joined
+    static constexpr int OffShared = Ring, OffStats = OffShared + (Shared + 127) / 128 * 128;
+    static constexpr int OffBars = OffStats + (2 * 4 * 16 * MW + R) * 4;
+    static constexpr int OffValid = OffBars + 2 * Slots * 8, OffScan = OffValid + Slots * 4, Bytes = OffScan + 96 + 1024;
+};
+
+// The sequence of pieces (parts of units) of a block, walked by each warp for itself.
+struct GqaWalk {
+    int b, h, rg, k0, k1;            // tiles [k0, k1) of the unit
+    GqaRequest req;
+    GqaSpan span;
+    int64_t left;                    // tiles of the share from this piece on
+    int nth;
+    __device__ __forceinline__ void piece() {
+        k1 = int(min(int64_t(span.count), k0 + left));
+    }
+    __device__ __forceinline__ void begin(const GqaArgs& a, int b0, int64_t off, int64_t tiles) {
+        b = b0;
+        left = tiles;
+        nth = 0;
+        if (left <= 0) return;
+        req = gqa_request(a, b);
+        const int64_t per_head = gqa_head_tiles(a, req);
+        h = int(off / per_head);
+        off -= h * per_head;
+        for (rg = 0;; ++rg) {
+            span = gqa_span(a, req, rg);
+            if (off < span.count) break;
+            off -= span.count;
+        }
+        k0 = int(off);
+        piece();
+    }
+    __device__ __forceinline__ void next(const GqaArgs& a) {
+        left -= k1 - k0;
+        ++nth;
+        if (left <= 0) return;
+        if (++rg >= gqa_groups(a, req)) {
+            rg = 0;
+            if (++h >= a.Hkv) {
+                h = 0;
+                do { req = gqa_request(a, ++b); } while (req.tokens == 0);
+            }
+        }
+        span = gqa_span(a, req, rg);
+        k0 = 0;
+        piece();
+    }
+};
+
+// Four columns, from x on, of a complete row: v = sum of exp2(x_j - top) v_j, sum = sum of exp2(x_j - top).
+template <int D>
+__device__ __forceinline__ void gqa_write_row(const GqaArgs& a, int64_t token, int head, int64_t weight_row, int x, const float4& v, float top, float sum, float v_scale) {
+    const int H = a.Hkv * a.G;
+    const bool none = sum == 0.f;                                             // nothing seen (or nothing but -inf): 0, and an lse of -inf
+    float all = sum, by = 1.f, ref = top;
+    if (a.sink != nullptr && !none) {
+        const float s = ptx::ld(a.sink + head) * 1.4426950408889634f;
+        ref = fmaxf(top, s);
+        by = ptx::ex2(top - ref);
+        all = sum * by + ptx::ex2(s - ref);
+    }
+    const float per = none ? 0.f : by * v_scale / all;
+    const float o[4] = {v.x * per, v.y * per, v.z * per, v.w * per};
+    uint2 w;
+    if (a.q_bf16) w = make_uint2(ptx::pack_bf16x2(o[0], o[1]), ptx::pack_bf16x2(o[2], o[3]));
+    else w = make_uint2(ptx::pack_f16x2(o[0], o[1]), ptx::pack_f16x2(o[2], o[3]));
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + (token * H + head) * D + x) = w;
+    if (x == 0) {
+        if (a.lse != nullptr) a.lse[token * H + head] = none ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+        if (a.total != nullptr) a.total[weight_row] = none ? INFINITY : ref + log2f(all);
+    }
+}
+
+template <class C>
+__global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel(const __grid_constant__ GqaArgs a) {
+    constexpr int D = C::D, MW = C::MW, WN = C::WN, R = C::R;
+    constexpr bool kE4m3 = C::KVT == kGqaE4m3, kBf16 = C::KVT == kGqaBf16;
+    constexpr bool kQInRegs = MW == 1 && D <= 128;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* const base = smem_raw + (smem - ptx::smem_u32(smem_raw));
+    const uint32_t bar_full = smem + C::OffBars, bar_empty = bar_full + 8 * C::Slots;
+    volatile uint32_t* const valid = reinterpret_cast<volatile uint32_t*>(base + C::OffValid);
+    int64_t* const scan = reinterpret_cast<int64_t*>(base + C::OffScan);                    // 5 warp sums; request and offset of the share
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+    if (tid == 0) {
+        for (int i = 0; i < C::Slots; ++i) {
+            ptx::mbar_init(bar_full + 8 * i, 1);
+            ptx::mbar_init(bar_empty + 8 * i, 4);
+        }
+        ptx::fence_mbar_init();
+        ptx::prefetch_tensormap(&a.k_map);
+        ptx::prefetch_tensormap(&a.v_map);
+    }
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+
+    // where this block's share begins
+    const int each = (a.B + kGqaThreads - 1) / kGqaThreads, b_from = tid * each, b_to = min(b_from + each, a.B);
+    int64_t mine = 0, total;
+    for (int b = b_from; b < b_to; ++b) mine += gqa_head_tiles(a, gqa_request(a, b)) * a.Hkv;
+    const int64_t before = block_prefix<kGqaThreads>(mine, total, scan);
+    const int64_t share = gqa_share(a, total), begin = int64_t(blockIdx.x) * share;
+    const int64_t tiles = min(share, total - begin);
+    if (tiles <= 0) return;
+    if (begin >= before && begin < before + mine) {
+        int64_t off = begin - before;
+        for (int b = b_from; b < b_to; ++b) {
+            const int64_t w = gqa_head_tiles(a, gqa_request(a, b)) * a.Hkv;
+            if (off < w) {
+                scan[5] = b;
+                scan[6] = off;
+                break;
+            }
+            off -= w;
+        }
+    }
+    __syncthreads();
+    GqaWalk w;
+    w.begin(a, int(scan[5]), scan[6], tiles);
+
+    if (warp == 4) {
+        // ── producer ──
+        uint32_t seq = 0;
+        bool ok = true;
+        for (; w.left > 0 && ok; w.next(a)) {
+            if (w.req.bad && lane == 0) gqa_report(a.status, kGqaStatusBadIndex, 4, w.b);
+            for (int k = w.k0; k < w.k1 && ok; k += 32) {
+                // the pages of the next 32 tiles, one per lane
+                int page = -1;
+                if (k + lane < w.k1 && w.span.hi > 0) {
+                    page = ptx::ld(a.block_table + int64_t(w.b) * a.max_pages + w.span.slot(k + lane));
+                    if (page < 0 || page >= a.num_pages) {
+                        gqa_report(a.status, kGqaStatusBadIndex, 4, page);
+                        page = -1;
+                    }
+                }
+                const int n = min(32, w.k1 - k);
+                for (int i = 0; i < n && ok; ++i) {
+                    const int pg = __shfl_sync(0xFFFFFFFFu, page, i);
+#pragma unroll
+                    for (int kv = 0; kv < 2 && ok; ++kv, ++seq) {
+                        const uint32_t st = seq % C::Slots, round = seq / C::Slots;
+                        if (round > 0 && !ptx::mbar_wait_warp(bar_empty + 8 * st, (round - 1) & 1u, a.wait_ns)) {
+                            if (lane == 0) gqa_report(a.status, kGqaStatusWait, 0, int(seq));
+                            ok = false;
+                            break;
+                        }
+                        if (a.dbg_drop_tile >= 0 && int(seq) == 2 * a.dbg_drop_tile) continue;       // a test's lost arrival
+                        if (ptx::elect_one()) {
+                            valid[st] = pg >= 0;
+                            ptx::mbar_arrive_expect_tx(bar_full + 8 * st, C::Slot);
+                            // (a page that is not there: rows behind the pool, which arrive as zeros)
+                            const int row = pg >= 0 ? pg * kGqaTile : int(a.num_pages * kGqaTile);
+#pragma unroll
+                            for (int x = 0; x < C::Boxes; ++x)
+                                ptx::tma_load_3d(smem + st * C::Slot + x * kGqaTile * C::Box, kv ? &a.v_map : &a.k_map, x * C::Box / C::ES, w.h, row, bar_full + 8 * st);
+                        }
+                        __syncwarp();
+                    }
+                }
+            }
+        }
+        if (!ok) {
+            // copies that are on their way land within microseconds
+            const uint32_t t0 = ptx::globaltimer_lo();
+            while (ptx::globaltimer_lo() - t0 < 1000000u) __nanosleep(1000);
+        }
+        return;
+    }
+
+    // ── attention ──
+    const int wm = warp / WN, wn = warp % WN, g = lane >> 2, c = lane & 3;
+    const uint32_t q_sm = smem + C::OffShared;
+    float* const merge = reinterpret_cast<float*>(base + C::OffShared);
+    float* const stat_m = reinterpret_cast<float*>(base + C::OffStats);       // [4][16 * MW]
+    float* const stat_l = stat_m + 4 * 16 * MW;
+    float* const row_factor = stat_l + 4 * 16 * MW;                           // [R]
+    // entry of column n of a block of eight (e4m3 rows of 128 bytes and more: the eight lanes that load together then meet all banks)
+    constexpr bool kPermuted = kE4m3 && C::RowBytes >= 128;
+    auto entry_of = [](int n) { return kPermuted ? (n >> 1) + 4 * (n & 1) : n; };
+    uint32_t seq = 0;
+    bool failed = false;
+
+    for (; w.left > 0; w.next(a)) {
+        const int64_t rows = int64_t(w.req.tokens) * a.G, row_first = int64_t(w.rg) * R;
+        // Q of the group: rows of zeros behind the last one
+        ptx::bar_sync(1, kGqaConsumers);
+        {
+            const uint8_t* const q0 = static_cast<const uint8_t*>(a.q);
+            constexpr int kLanes = D / 8;                                     // 16 bytes each
+            const int l = tid % kLanes;
+#pragma unroll 4
+            for (int r = tid / kLanes; r < R; r += kGqaConsumers / kLanes) {
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (row_first + r < rows) {
+                    const int t = int((row_first + r) / a.G), gg = int(row_first + r - int64_t(t) * a.G);
+                    const int64_t at = (a.q_start != nullptr ? (w.req.row0 + t) * a.q_stride_t : int64_t(w.b) * a.q_stride_b + t * a.q_stride_t) +
+                                       int64_t(w.h * a.G + gg) * a.q_stride_h + 8 * l;
+                    v = *reinterpret_cast<const uint4*>(q0 + at * 2);
+                }
+                if (kE4m3) {
+                    float factor = 1.f;
+                    if (a.q_bf16) {
+                        float f[8], top = 0.f;
+                        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            f[2 * i] = __uint_as_float(u[i] << 16);
+                            f[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+                            top = fmaxf(top, fmaxf(fabsf(f[2 * i]), fabsf(f[2 * i + 1])));
+                        }
+#pragma unroll
+                        for (int d = 1; d < kLanes; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+                        // 2^e <= top < 2^(e + 1); zeros, infinities and what 2^-e cannot bring there stay near enough
+                        const int e = min(max(int(__float_as_uint(top) >> 23) - 127, -100), 126);
+                        const float down = __uint_as_float(uint32_t(127 - e) << 23);
+                        factor = __uint_as_float(uint32_t(127 + e) << 23);
+                        uint32_t o[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) o[i] = ptx::pack_f16x2(f[2 * i] * down, f[2 * i + 1] * down);
+                        v = make_uint4(o[0], o[1], o[2], o[3]);
+                    }
+                    if (l == 0) row_factor[r] = factor;
+                }
+                ptx::sts_v4(q_sm + r * C::QPitch + 16 * l, v);
+            }
+        }
+        ptx::bar_sync(1, kGqaConsumers);
+
+        uint32_t qf[kQInRegs ? D / 16 : 1][4];
+        // A fragment of 16 dimensions; e4m3: of the dimensions that the lanes' 16-byte pieces of K hold (64 j + 16 c + 4 s + 0..3)
+        auto q_fragment = [&](uint32_t (&r)[4], int mt, int ks) {
+            const uint32_t row = q_sm + uint32_t((wm * MW + mt) * 16) * C::QPitch;
+            if (kE4m3) {
+                const uint32_t at = row + g * C::QPitch + (ks / 4) * 128 + c * 32 + (ks % 4) * 8;
+                const uint2 lo = ptx::lds_v2(at), hi = ptx::lds_v2(at + 8 * C::QPitch);
+                r[0] = lo.x;  r[1] = hi.x;  r[2] = lo.y;  r[3] = hi.y;
+            } else {
+                ldmatrix4(r, row + (lane & 15) * C::QPitch + ks * 32 + (lane >> 4) * 16);
+            }
+        };
+        if (kQInRegs) {
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks) q_fragment(qf[kQInRegs ? ks : 0], 0, ks);
+        }
+        int place[MW][2];                                                     // of the rows' tokens; -1: no row
+        float scale[MW][2];
+        const float head_scale = a.scale_log2 * (a.k_scale != nullptr ? ptx::ld(a.k_scale + w.h) : 1.f);
+#pragma unroll
+        for (int mt = 0; mt < MW; ++mt)
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+                const int r = (wm * MW + mt) * 16 + g + 8 * hh;
+                place[mt][hh] = row_first + r < rows ? w.req.place0 + int((row_first + r) / a.G) : -1;
+                scale[mt][hh] = kE4m3 ? head_scale * row_factor[r] : head_scale;
+            }
+        float m[MW][2], l[MW][2], o[MW][D / 8][4];
+#pragma unroll
+        for (int mt = 0; mt < MW; ++mt) {
+            m[mt][0] = m[mt][1] = -INFINITY;
+            l[mt][0] = l[mt][1] = 0.f;
+#pragma unroll
+            for (int j = 0; j < D / 8; ++j) o[mt][j][0] = o[mt][j][1] = o[mt][j][2] = o[mt][j][3] = 0.f;
+        }
+        const int place_first = w.req.place0 + w.span.t0, place_last = w.req.place0 + w.span.t1;
+
+        for (int k = w.k0; k < w.k1; ++k, seq += 2) {
+            const uint32_t ks_ = seq % C::Slots, vs_ = (seq + 1) % C::Slots;
+            auto wait_full = [&](uint32_t s) {
+                if (!failed && !ptx::mbar_wait_warp(bar_full + 8 * (s % C::Slots), (s / C::Slots) & 1u, a.wait_ns)) {
+                    if (lane == 0) gqa_report(a.status, kGqaStatusWait, 1, int(s));
+                    failed = true;                                            // (the rest of the block's work is gone through without waiting)
+                }
+            };
+            wait_full(seq);
+            const bool there = valid[ks_] != 0;
+            const uint32_t k_sm = smem + ks_ * C::Slot, v_sm = smem + vs_ * C::Slot;
+            const int e0 = w.span.slot(k) * kGqaTile;
+            bool v_waited = false, k_given_back = false;
+#pragma unroll 1
+            for (int sl = wn; sl < 4; sl += WN) {
+                const int p0 = e0 + 16 * sl;                                  // entries p0 .. p0 + 15
+                // seen by all rows, or by none, or by some
+                const bool whole = there && p0 + 15 <= place_first && p0 + 15 < w.req.entries && (a.window == 0 || p0 > place_last - a.window || p0 + 15 < a.first);
+                const bool some = p0 < w.span.hi && (p0 + 15 >= w.span.lo || p0 < w.span.first);
+                if (!some) continue;
+                float s[MW][2][4];
+#pragma unroll
+                for (int mt = 0; mt < MW; ++mt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[mt][0][i] = s[mt][1][i] = 0.f;
+                if constexpr (!kE4m3) {
+                    const int e = 16 * sl + (lane & 7) + ((lane >> 4) << 3);
+                    const uint32_t row = k_sm + e * 128, flip = e & 7, half = (lane >> 3) & 1;
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ++ks) {
+                        uint32_t kf[4];
+                        ldmatrix4(kf, row + (ks / 4) * (kGqaTile * 128) + ((((ks % 4) * 2 + half) ^ flip) << 4));
+#pragma unroll
+                        for (int mt = 0; mt < MW; ++mt) {
+                            uint32_t qq[4];
+                            if (!kQInRegs) q_fragment(qq, mt, ks);
+                            const uint32_t(&qa)[4] = kQInRegs ? qf[kQInRegs ? ks : 0] : qq;
+                            mma16816<kBf16>(s[mt][0], qa, kf[0], kf[1]);
+                            mma16816<kBf16>(s[mt][1], qa, kf[2], kf[3]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < D / 64; ++j) {
+                        uint4 kb[2];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const int e = 16 * sl + 8 * i + entry_of(g);
+                            const uint32_t at = C::Box == 128 ? k_sm + (j / 2) * (kGqaTile * 128) + e * 128 + ((((j & 1) * 4 + c) ^ (e & 7)) << 4)
+                                                              : k_sm + e * 64 + ((c ^ ((e >> 1) & 3)) << 4);
+                            kb[i] = ptx::lds_v4(at);
+                        }
+#pragma unroll
+                        for (int st = 0; st < 4; ++st) {
+                            uint32_t kf[4];
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) ptx::e4m3x4_to_f16x4(st == 0 ? kb[i].x : st == 1 ? kb[i].y : st == 2 ? kb[i].z : kb[i].w, kf[2 * i], kf[2 * i + 1]);
+#pragma unroll
+                            for (int mt = 0; mt < MW; ++mt) {
+                                uint32_t qq[4];
+                                if (!kQInRegs) q_fragment(qq, mt, 4 * j + st);
+                                const uint32_t(&qa)[4] = kQInRegs ? qf[kQInRegs ? 4 * j + st : 0] : qq;
+                                mma16816<false>(s[mt][0], qa, kf[0], kf[1]);
+                                mma16816<false>(s[mt][1], qa, kf[2], kf[3]);
+                            }
+                        }
+                    }
+                }
+                // scores in log2 units; what a row does not see is -inf
+#pragma unroll
+                for (int mt = 0; mt < MW; ++mt)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            float x = s[mt][i][q] * scale[mt][q >> 1];
+                            if (!whole) {
+                                const int p = p0 + 8 * i + entry_of(2 * c + (q & 1)), at = place[mt][q >> 1];
+                                if (!(there && p <= at && p < w.req.entries && (a.window == 0 || p > at - a.window || p < a.first))) x = -INFINITY;
+                            }
+                            s[mt][i][q] = x;
+                        }
+                if (a.logits != nullptr) {
+#pragma unroll
+                    for (int mt = 0; mt < MW; ++mt)
+#pragma unroll
+                        for (int hh = 0; hh < 2; ++hh) {
+                            const int64_t r = row_first + (wm * MW + mt) * 16 + g + 8 * hh;
+                            if (r < rows) {
+                                float* const to = a.logits + ((int64_t(w.b) * a.Hkv + w.h) * rows + r) * a.logit_stride + p0;
+#pragma unroll
+                                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                                    for (int q = 0; q < 2; ++q) to[8 * i + entry_of(2 * c + q)] = s[mt][i][2 * hh + q];
+                            }
+                        }
+                }
+                // running maximum and sum
+                uint32_t pf[MW][4];
+#pragma unroll
+                for (int mt = 0; mt < MW; ++mt) {
+                    float top[2];
+#pragma unroll
+                    for (int hh = 0; hh < 2; ++hh) {
+                        top[hh] = fmaxf(fmaxf(s[mt][0][2 * hh], s[mt][0][2 * hh + 1]), fmaxf(s[mt][1][2 * hh], s[mt][1][2 * hh + 1]));
+                        top[hh] = fmaxf(top[hh], __shfl_xor_sync(0xFFFFFFFFu, top[hh], 1));
+                        top[hh] = fmaxf(top[hh], __shfl_xor_sync(0xFFFFFFFFu, top[hh], 2));
+                        top[hh] = fmaxf(top[hh], m[mt][hh]);
+                    }
+                    if (__any_sync(0xFFFFFFFFu, top[0] != m[mt][0] || top[1] != m[mt][1])) {
+#pragma unroll
+                        for (int hh = 0; hh < 2; ++hh) {
+                            const float by = top[hh] == -INFINITY ? 1.f : ptx::ex2(m[mt][hh] - top[hh]);
+                            m[mt][hh] = top[hh];
+                            l[mt][hh] *= by;
+#pragma unroll
+                            for (int j = 0; j < D / 8; ++j) {
+                                o[mt][j][2 * hh] *= by;
+                                o[mt][j][2 * hh + 1] *= by;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int hh = 0; hh < 2; ++hh) {
+                        const float ref = m[mt][hh] == -INFINITY ? 0.f : m[mt][hh];
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float e_lo = ptx::ex2(s[mt][i][2 * hh] - ref), e_hi = ptx::ex2(s[mt][i][2 * hh + 1] - ref);
+                            l[mt][hh] += e_lo + e_hi;
+                            pf[mt][2 * i + hh] = kBf16 ? ptx::pack_bf16x2(e_lo, e_hi) : ptx::pack_f16x2(e_lo, e_hi);
+                        }
+                    }
+                }
+                if (sl + WN >= 4) {
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(bar_empty + 8 * ks_);
+                    k_given_back = true;
+                }
+                if (!v_waited) {
+                    wait_full(seq + 1);
+                    v_waited = true;
+                }
+                // V of entries that no row of the group sees may be anything: it counts as zero (0 * inf is not 0)
+                uint32_t keep[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
+                if (!whole) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        keep[i] = 0;
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            const int p = p0 + 8 * i + entry_of(2 * c + q);
+                            if (p < w.span.hi && (p >= w.span.lo || p < w.span.first)) keep[i] |= q ? 0xFFFF0000u : 0xFFFFu;
+                        }
+                    }
+                }
+                const int ve = 16 * sl + ((lane >> 3) & 1) * 8 + entry_of(lane & 7), vc = lane >> 4;
+#pragma unroll
+                for (int j = 0; j < D * C::ES / 32; ++j) {                    // 32 bytes of a row: 16 dimensions in 16 bits, 32 in 8
+                    uint32_t vf[4];
+                    const int ch = 2 * j + vc;
+                    ldmatrix4_trans(vf, C::Box == 128 ? v_sm + (ch / 8) * (kGqaTile * 128) + ve * 128 + (((ch & 7) ^ (ve & 7)) << 4)
+                                                      : v_sm + ve * 64 + ((ch ^ ((ve >> 1) & 3)) << 4));
+                    if constexpr (!kE4m3) {
+                        if (!whole) { vf[0] &= keep[0];  vf[1] &= keep[1];  vf[2] &= keep[0];  vf[3] &= keep[1]; }
+#pragma unroll
+                        for (int mt = 0; mt < MW; ++mt) {
+                            mma16816<kBf16>(o[mt][2 * j], pf[mt], vf[0], vf[1]);
+                            mma16816<kBf16>(o[mt][2 * j + 1], pf[mt], vf[2], vf[3]);
+                        }
+                    } else {
+                        // a word: dimensions 2n, 2n + 1 of two entries -> two words of one dimension each; o[4 j' ..]: even and odd ones of 16
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            const uint32_t w0 = __byte_perm(vf[2 * q], 0, 0x3120), w1 = __byte_perm(vf[2 * q + 1], 0, 0x3120);
+                            uint32_t b[4];
+                            ptx::e4m3x4_to_f16x4(w0, b[0], b[2]);
+                            ptx::e4m3x4_to_f16x4(w1, b[1], b[3]);
+                            if (!whole) { b[0] &= keep[0];  b[1] &= keep[1];  b[2] &= keep[0];  b[3] &= keep[1]; }
+#pragma unroll
+                            for (int mt = 0; mt < MW; ++mt) {
+                                mma16816<false>(o[mt][4 * j + 2 * q], pf[mt], b[0], b[1]);
+                                mma16816<false>(o[mt][4 * j + 2 * q + 1], pf[mt], b[2], b[3]);
+                            }
+                        }
+                    }
+                }
+            }
+            // (every warp waits for both tiles of every turn: its arrivals then belong to the turn that they are counted in)
+            if (!v_waited) wait_full(seq + 1);
+            __syncwarp();
+            if (lane == 0) {
+                if (!k_given_back) ptx::mbar_arrive(bar_empty + 8 * ks_);
+                ptx::mbar_arrive(bar_empty + 8 * vs_);
+            }
+        }
+
+        // ── the warps' parts of a row are joined ──
+#pragma unroll
+        for (int mt = 0; mt < MW; ++mt)
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+                l[mt][hh] += __shfl_xor_sync(0xFFFFFFFFu, l[mt][hh], 1);
+                l[mt][hh] += __shfl_xor_sync(0xFFFFFFFFu, l[mt][hh], 2);
+                if (c == 0) {
+                    stat_m[warp * 16 * MW + mt * 16 + g + 8 * hh] = m[mt][hh];
+                    stat_l[warp * 16 * MW + mt * 16 + g + 8 * hh] = l[mt][hh];
+                }
+            }
+        const bool complete = w.k0 == 0 && w.k1 == w.span.count;
+        const int64_t part = 2 * int64_t(blockIdx.x) + (w.nth > 0);           // only the first and the last piece of a share can be parts
+        const float v_scale = a.v_scale != nullptr ? ptx::ld(a.v_scale + w.h) : 1.f;
+        ptx::bar_sync(1, kGqaConsumers);
+#pragma unroll
+        for (int mt = 0; mt < MW; ++mt) {
+            auto row_max = [&](int of_wm, int r) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < WN; ++n) top = fmaxf(top, stat_m[(of_wm * WN + n) * 16 * MW + mt * 16 + r]);
+                return top;
+            };
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+                const float top = row_max(wm, g + 8 * hh), by = m[mt][hh] == -INFINITY ? 0.f : ptx::ex2(m[mt][hh] - top);
+                float* const to = merge + (warp * 16 + g + 8 * hh) * C::MergePitch;
+                if constexpr (!kE4m3) {
+#pragma unroll
+                    for (int j = 0; j < D / 8; ++j)
+                        *reinterpret_cast<float2*>(to + 8 * j + 2 * c) = make_float2(o[mt][j][2 * hh] * by, o[mt][j][2 * hh + 1] * by);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < D / 16; ++j)
+                        *reinterpret_cast<float4*>(to + 16 * j + 4 * c) = make_float4(o[mt][2 * j][2 * hh] * by, o[mt][2 * j + 1][2 * hh] * by, o[mt][2 * j][2 * hh + 1] * by,
+                                                                                      o[mt][2 * j + 1][2 * hh + 1] * by);
+                }
+            }
+            ptx::bar_sync(1, kGqaConsumers);
+            constexpr int kLanes = D / 4;
+            const int x = 4 * (tid % kLanes);
+#pragma unroll 2
+            for (int rr = tid / kLanes; rr < 16 * C::WM; rr += kGqaConsumers / kLanes) {
+                const int of_wm = rr >> 4, rl = rr & 15, r = (of_wm * MW + mt) * 16 + rl;
+                const int64_t row = row_first + r;
+                if (row >= rows) continue;
+                const float top = row_max(of_wm, rl);
+                float sum = 0.f;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int n = 0; n < WN; ++n) {
+                    const int at = of_wm * WN + n;
+                    const float mm = stat_m[at * 16 * MW + mt * 16 + rl], ll = stat_l[at * 16 * MW + mt * 16 + rl];
+                    sum += mm == -INFINITY ? ll : ll * ptx::ex2(mm - top);     // (a NaN row has a maximum of -inf and a NaN sum)
+                    const float4 u = *reinterpret_cast<const float4*>(merge + (at * 16 + rl) * C::MergePitch + x);
+                    v.x += u.x;  v.y += u.y;  v.z += u.z;  v.w += u.w;
+                }
+                if (!complete) {
+                    const float per = sum == 0.f ? 0.f : 1.f / sum;
+                    *reinterpret_cast<float4*>(a.part_o + (part * R + r) * D + x) = make_float4(v.x * per, v.y * per, v.z * per, v.w * per);
+                    if (x == 0) a.part_lse[part * R + r] = top + log2f(sum);
+                    continue;
+                }
+                gqa_write_row<D>(a, w.req.row0 + row / a.G, w.h * a.G + int(row % a.G), (int64_t(w.b) * a.Hkv + w.h) * rows + row, x, v, top, sum, v_scale);
+            }
+            ptx::bar_sync(1, kGqaConsumers);
+        }
+    }
+}
+
+// ── parts of units that a cut ran through ──
+// A warp takes a row and finds out, from the same scan as above, which blocks had a part of its unit.
+constexpr int kGqaMergeRows = kGqaMergeThreads / 32;
+template <int D>
+__global__ void __launch_bounds__(kGqaMergeThreads) gqa_merge_kernel(const __grid_constant__ GqaArgs a) {
+    __shared__ int64_t sums[kGqaMergeRows];
+    __shared__ int64_t unit_before[kGqaMergeRows];                            // tiles of the requests before the row's
+    __shared__ int32_t row_request[kGqaMergeRows];
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, H = a.Hkv * a.G;
+    const int64_t row0 = int64_t(blockIdx.x) * kGqaMergeRows;
+    if (tid < kGqaMergeRows) row_request[tid] = -1;
+    const int each = (a.B + kGqaMergeThreads - 1) / kGqaMergeThreads, b_from = tid * each, b_to = min(b_from + each, a.B);
+    int64_t mine = 0, total;
+    for (int b = b_from; b < b_to; ++b) mine += gqa_head_tiles(a, gqa_request(a, b)) * a.Hkv;
+    int64_t before = block_prefix<kGqaMergeThreads>(mine, total, sums);
+    for (int b = b_from; b < b_to; ++b) {
+        const GqaRequest r = gqa_request(a, b);
+#pragma unroll
+        for (int i = 0; i < kGqaMergeRows; ++i) {
+            const int64_t token = (row0 + i) / H;
+            if (token >= r.row0 && token < r.row0 + r.tokens) {
+                row_request[i] = b;
+                unit_before[i] = before;
+            }
+        }
+        before += gqa_head_tiles(a, r) * a.Hkv;
+    }
+    __syncthreads();
+    const int b = row_request[warp];
+    if (b < 0) return;
+    const GqaRequest req = gqa_request(a, b);
+    const int64_t row = row0 + warp, token = row / H, rows = int64_t(req.tokens) * a.G;
+    const int head = int(row - token * H), h = head / a.G;
+    const int64_t at = (token - req.row0) * a.G + head - h * a.G;              // row of the KV head
+    const int rg = int(at / a.group_rows), r = int(at - int64_t(rg) * a.group_rows);
+    int64_t unit = unit_before[warp] + h * gqa_head_tiles(a, req);
+    for (int i = 0; i < rg; ++i) unit += gqa_span(a, req, i).count;
+    const int64_t share = gqa_share(a, total);
+    const int c0 = int(unit / share), c1 = int((unit + gqa_span(a, req, rg).count - 1) / share);
+    if (c0 == c1) return;
+    const int64_t first = 2 * int64_t(c0) + (unit != c0 * share);              // (every later block begins with its part)
+    auto part = [&](int i) { return (i == 0 ? first : 2 * int64_t(c0 + i)) * a.group_rows + r; };
+    const int parts = c1 - c0 + 1;
+    float top = -INFINITY;
+    for (int i = lane; i < parts; i += 32) top = fmaxf(top, a.part_lse[part(i)]);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+    constexpr int kVecs = D > 128 ? D / 128 : 1;
+    float4 v[kVecs];
+#pragma unroll
+    for (int x = 0; x < kVecs; ++x) v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+    const bool in_row = 4 * lane < D;
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+        float weight = 0.f;
+        if (i0 + lane < parts) {
+            const float p = a.part_lse[part(i0 + lane)];
+            weight = p == -INFINITY ? 0.f : ptx::ex2(p - (top == -INFINITY ? 0.f : top));
+        }
+#pragma unroll 4
+        for (int i = 0; i < min(32, parts - i0); ++i) {
+            const float by = __shfl_sync(0xFFFFFFFFu, weight, i);
+            sum += by;
+            if (in_row) {
+                const float* const from = a.part_o + part(i0 + i) * D + 4 * lane;
+#pragma unroll
+                for (int x = 0; x < kVecs; ++x) {
+                    const float4 u = *reinterpret_cast<const float4*>(from + 128 * x);
+                    v[x].x = fmaf(by, u.x, v[x].x);  v[x].y = fmaf(by, u.y, v[x].y);  v[x].z = fmaf(by, u.z, v[x].z);  v[x].w = fmaf(by, u.w, v[x].w);
+                }
+            }
+        }
+    }
+    const float v_scale = a.v_scale != nullptr ? ptx::ld(a.v_scale + h) : 1.f;
+    if (in_row) {
+#pragma unroll
+        for (int x = 0; x < kVecs; ++x) gqa_write_row<D>(a, token, head, (int64_t(b) * a.Hkv + h) * rows + at, 128 * x + 4 * lane, v[x], top, sum, v_scale);
+    }
+}
+
+// ── weights of the entries ──
+// weights[b][j] += sum over the tokens that see j and over the heads of exp(x_j) / denominator, from the scores that the attention kernel has left.  A thread takes an
+// entry and adds in a fixed order.
+__global__ void __launch_bounds__(kGqaWeightThreads) gqa_weights_kernel(const __grid_constant__ GqaArgs a) {
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    const int b = blockIdx.y, p = blockIdx.x * kGqaWeightThreads + threadIdx.x;
+    const GqaRequest req = gqa_request(a, b);
+    if (p >= req.entries) return;
+    const int rows = req.tokens * a.G;
+    const int64_t base = int64_t(b) * a.Hkv * rows;
+    float sum = 0.f;
+    bool any = false;
+    for (int t = 0; t < req.tokens; ++t) {
+        const int at = req.place0 + t;
+        if (!(p <= at && (a.window == 0 || p > at - a.window || p < a.first))) continue;
+        any = true;
+        for (int h = 0; h < a.Hkv; ++h)
+#pragma unroll 4
+            for (int g = 0; g < a.G; ++g) {
+                const int64_t r = base + int64_t(h) * rows + t * a.G + g;
+                sum += ptx::ex2(a.logits[r * a.logit_stride + p] - a.total[r]);
+            }
+    }
+    if (any) a.weights[int64_t(b) * a.weight_stride + p] += sum;
+}
+
+// ── new rows into the pages ──
+struct GqaInsertArgs {
+    int B, T, Hkv, D, max_pages;
+    int64_t rows;                    // tokens of all requests
+    const int32_t* q_start;          // [B + 1], or null: T tokens each
+    const int32_t* n_rows;           // [B], or null: all T
+    const int32_t* insert_pos;       // [B]
+    const int32_t* block_table;      // [B, max_pages]
+    int64_t num_pages;
+    const void* src[2];              // K, V: 16-bit
+    int64_t stride_b[2], stride_t[2], stride_h[2];
+    int src_bf16;
+    const float* scale[2];           // [Hkv], e4m3
+    void* pool[2];                   // [num_pages, 64, Hkv, D]
+    int32_t* status;
+};
+constexpr int kGqaInsertThreads = 256;
+
+__device__ __forceinline__ uint32_t quant_pair(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+
+// A warp takes a token's K or V: 16 bytes a lane and load, up to four of them on the way.  Bound by the chain of its loads (offset, position, page) when small and by
+// memory when large.
+template <bool E4M3>
+__global__ void __launch_bounds__(kGqaInsertThreads) gqa_insert_kernel(const __grid_constant__ GqaInsertArgs a) {
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t items = 2 * a.rows, step = int64_t(gridDim.x) * (kGqaInsertThreads / 32);
+    const int pieces = a.Hkv * a.D / 8, per_head = a.D / 8;
+    for (int64_t item = int64_t(blockIdx.x) * (kGqaInsertThreads / 32) + (threadIdx.x >> 5); item < items; item += step) {
+        const int kv = int(item & 1);
+        const int64_t token = item >> 1;
+        int b, t;
+        if (a.q_start == nullptr) {
+            b = int(token / a.T);
+            t = int(token - int64_t(b) * a.T);
+            if (a.n_rows != nullptr && t >= ptx::ld(a.n_rows + b)) continue;
+        } else {
+            // the request whose rows the token is among: 32 probes at a time
+            int lo = 0, n = a.B;                                              // q_start[lo] <= token (or lo = 0), token < q_start[lo + n] (or lo + n = B)
+            while (n > 1) {
+                const int each = (n + 31) / 32, at = min(lo + (lane + 1) * each, lo + n);
+                const uint32_t over = __ballot_sync(0xFFFFFFFFu, at >= lo + n || ptx::ld(a.q_start + at) > token);
+                const int skip = __ffs(over) - 1;
+                n = min(each, n - skip * each);
+                lo += skip * each;
+            }
+            b = lo;
+            const int from = ptx::ld(a.q_start + b), to = ptx::ld(a.q_start + b + 1);
+            if (token < from || token >= to) continue;                        // behind the last request
+            t = int(token - from);
+        }
+        const int64_t pos = int64_t(ptx::ld(a.insert_pos + b)) + t, slot = pos / kGqaTile;
+        int page = -1;
+        if (pos >= 0 && slot < a.max_pages) page = ptx::ld(a.block_table + int64_t(b) * a.max_pages + slot);
+        if (page < 0 || page >= a.num_pages) {
+            if (lane == 0) gqa_report(a.status, 16, b, int(pos));
+            continue;
+        }
+        const uint8_t* const src = static_cast<const uint8_t*>(a.src[kv]);
+        const int64_t row = (a.q_start == nullptr ? b * a.stride_b[kv] + t * a.stride_t[kv] : token * a.stride_t[kv]);
+        uint8_t* const dst = static_cast<uint8_t*>(a.pool[kv]) + (int64_t(page) * kGqaTile + pos % kGqaTile) * (int64_t(a.Hkv) * a.D * (E4M3 ? 1 : 2));
+        for (int at = lane; at < pieces; at += 128) {
+            uint4 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (at + 32 * i < pieces) {
+                    const int h = (at + 32 * i) / per_head, x = (at + 32 * i) - h * per_head;
+                    v[i] = ptx::ldg_stream_v4(src + (row + h * a.stride_h[kv] + 8 * x) * 2);
+                }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (at + 32 * i >= pieces) break;
+                if constexpr (E4M3) {
+                    const float scale = ptx::ld(a.scale[kv] + (at + 32 * i) / per_head);
+                    const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+                    uint32_t o[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        float lo, hi;
+                        if (a.src_bf16) {
+                            lo = __uint_as_float(u[j] << 16);
+                            hi = __uint_as_float(u[j] & 0xFFFF0000u);
+                        } else {
+                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[j]));
+                            lo = f.x;
+                            hi = f.y;
+                        }
+                        o[j] = quant_pair(__fdiv_rn(lo, scale), __fdiv_rn(hi, scale));
+                    }
+                    *reinterpret_cast<uint2*>(dst + 8 * (at + 32 * i)) = make_uint2(o[0] | (o[1] << 16), o[2] | (o[3] << 16));
+                } else {
+                    *reinterpret_cast<uint4*>(dst + 16 * (at + 32 * i)) = v[i];
+                }
+            }
+        }
+    }
+}
+
+}  // namespace dsv4

@@ -14,11 +14,13 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/dsv4_attn.h"
 #include "../../include/dsv4_speculative.h"
+#include "../../include/dsv4_gqa.h"
 
 namespace {
 
@@ -45,6 +47,11 @@ struct Library {
     decltype(&dsv4_kv_entries_move) entries_move;
     decltype(&dsv4_sample_fwd) sample;
     decltype(&dsv4_hca_tree_rows_bytes) tree_rows_bytes;
+    decltype(&dsv4_gqa_decode_fwd) gqa_decode;
+    decltype(&dsv4_gqa_prefill_fwd) gqa_prefill;
+    decltype(&dsv4_gqa_workspace_bytes) gqa_workspace_bytes;
+    decltype(&dsv4_gqa_insert) gqa_insert;
+    decltype(&dsv4_kv_evict) kv_evict;
 } lib;
 
 constexpr int kLatent = 512, kQk = 576, kEntry = DSV4_ENTRY_BYTES, kPage = DSV4_PAGE_ENTRIES;
@@ -702,6 +709,158 @@ PyObject* pages_compact(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return r;
 }
 
+// ── pages of K and V heads (dsv4_gqa.h) ──
+// BF16 or FP16, and for caches e4m3; -1: another type
+int gqa_type(const at::Tensor* t, bool cache) {
+    switch (t->scalar_type()) {
+        case at::kBFloat16: return DSV4_DTYPE_BF16;
+        case at::kHalf: return DSV4_DTYPE_F16;
+        case at::kFloat8_e4m3fn: return cache ? DSV4_DTYPE_E4M3 : -1;
+        default: return -1;
+    }
+}
+// Pools [num_pages, 64, Hkv, D] of K and V, of one type, with scales [Hkv] each where that is e4m3
+struct GqaPools {
+    const at::Tensor *k, *v, *k_scale, *v_scale, *table;
+    int type;
+    int64_t Hkv, D;
+    bool take(PyObject* k_, PyObject* v_, PyObject* k_scale_, PyObject* v_scale_, PyObject* table_, int64_t B) {
+        k = any_tensor(k_);
+        v = any_tensor(v_);
+        if (k == nullptr || v == nullptr || !k->is_cuda() || !v->is_cuda() || !k->is_contiguous() || !v->is_contiguous() || k->dim() != 4) return false;
+        type = gqa_type(k, true);
+        if (type < 0 || v->scalar_type() != k->scalar_type() || v->sizes() != k->sizes() || k->numel() <= 0 || k->size(1) != kPage) return false;
+        Hkv = k->size(2);
+        D = k->size(3);
+        if (!optional_tensor(k_scale_, at::kFloat, 1, &k_scale) || !optional_tensor(v_scale_, at::kFloat, 1, &v_scale)) return false;
+        if ((k_scale != nullptr) != (type == DSV4_DTYPE_E4M3) || (v_scale != nullptr) != (type == DSV4_DTYPE_E4M3) || !has_shape(k_scale, {Hkv}) || !has_shape(v_scale, {Hkv}))
+            return false;
+        table = tensor(table_, at::kInt, 2);
+        return table != nullptr && table->size(0) == B && table->size(1) > 0 && fits32(table->size(1)) && fits32(k->size(0)) && fits32(Hkv);
+    }
+};
+// Rows [.., heads, D] with D contiguous and 16-byte pieces aligned
+bool gqa_rows(const at::Tensor* t, int64_t dims) {
+    if (t == nullptr || !t->is_cuda() || t->dim() != dims || (t->size(-1) > 1 && t->stride(-1) != 1)) return false;
+    for (int64_t i = 0; i + 1 < dims; ++i)
+        if (t->size(i) > 1 && (t->stride(i) % 8 != 0 || t->stride(i) < 0)) return false;
+    return t->numel() == 0 || reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0;
+}
+int64_t row_stride(const at::Tensor* t, int64_t i) { return t->size(i) > 1 ? t->stride(i) : 0; }
+
+// (q, q_start, k_pool, v_pool, block_table, kv_len, sm_scale, window, first, k_scale, v_scale, attn_sink, weights, max_len, out, lse, status)
+PyObject* gqa(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 17) return none();
+    const bool packed = a[1] != Py_None;
+    const at::Tensor *q = any_tensor(a[0]), *start, *len = tensor(a[5], at::kInt, 1), *sink, *weights, *status;
+    if (!gqa_rows(q, packed ? 3 : 4) || len == nullptr || !optional_tensor(a[1], at::kInt, 1, &start)) return none();
+    const int64_t B = len->size(0);
+    GqaPools pool;
+    if (B <= 0 || !fits32(B) || !has_shape(start, {B + 1}) || (!packed && q->size(0) != B) || !pool.take(a[2], a[3], a[9], a[10], a[4], B)) return none();
+    Dsv4GqaParams p{};
+    p.q_dtype = gqa_type(q, false);
+    p.kv_dtype = pool.type;
+    if (p.q_dtype < 0 || (p.kv_dtype != DSV4_DTYPE_E4M3 && p.kv_dtype != p.q_dtype)) return none();
+    const int64_t H = q->size(-2), T = packed ? 0 : q->size(1), rows = packed ? q->size(0) : B * T;
+    if (q->size(-1) != pool.D || H <= 0 || H % pool.Hkv != 0 || !fits32(H) || !fits32(T)) return none();
+    int64_t window, first, max_len = 0;
+    if (!number(a[6], &p.sm_scale) || !integer(a[7], &window) || !integer(a[8], &first) || window < 0 || first < 0 || !fits32(window) || !fits32(first)) return none();
+    if (a[13] != Py_None && (!integer(a[13], &max_len) || max_len < 0 || !fits32(max_len))) return none();
+    if (!optional_tensor(a[11], at::kFloat, 1, &sink) || !has_shape(sink, {H}) || !optional_tensor(a[12], at::kFloat, 2, &weights)) return none();
+    if (weights != nullptr && (packed || weights->size(0) != B || weights->size(1) < pool.table->size(1) * kPage)) return none();
+    if (!optional_tensor(a[16], at::kInt, 1, &status) || (status != nullptr && status->numel() < DSV4_STATUS_WORDS)) return none();
+    if (!same_device(q, {start, len, sink, weights, status, pool.k, pool.v, pool.k_scale, pool.v_scale, pool.table})) return none();
+    const c10::cuda::CUDAGuard guard(q->device());
+    Output out, lse;
+    if (packed ? !out.take(a[14], q->scalar_type(), {rows, H, pool.D}, q) || !lse.take(a[15], at::kFloat, {rows, H}, q)
+               : !out.take(a[14], q->scalar_type(), {B, T, H, pool.D}, q) || !lse.take(a[15], at::kFloat, {B, T, H}, q)) return none();
+    if (!same_device(q, {out.t, lse.t}) || (reinterpret_cast<uintptr_t>(out.t->data_ptr()) % 16 != 0 && rows > 0)) return none();
+    if (rows == 0) return pair(out, lse);
+    p.B = int(B);  p.T = int(T);  p.Hkv = int(pool.Hkv);  p.G = int(H / pool.Hkv);  p.D = int(pool.D);  p.max_pages = int(pool.table->size(1));
+    p.window = int(window);  p.first = int(first);  p.max_len = int(max_len);  p.rows = rows;  p.num_pages = pool.k->size(0);
+    p.q_stride_b = packed ? 0 : row_stride(q, 0);  p.q_stride_t = row_stride(q, packed ? 0 : 1);  p.q_stride_h = row_stride(q, packed ? 1 : 2);
+    p.q = ptr(q);  p.q_start = ptr<int32_t>(start);  p.k_pool = ptr(pool.k);  p.v_pool = ptr(pool.v);  p.block_table = ptr<int32_t>(pool.table);  p.kv_len = ptr<int32_t>(len);
+    p.k_scale = ptr<float>(pool.k_scale);  p.v_scale = ptr<float>(pool.v_scale);  p.attn_sink = ptr<float>(sink);  p.out = ptr(out.t);  p.lse = ptr<float>(lse.t);
+    p.weights = ptr<float>(weights);  p.weight_stride = weights != nullptr ? weights->size(1) : 0;  p.status = ptr<int32_t>(status);
+    p.workspace_bytes = lib.gqa_workspace_bytes(&p);
+    if (p.workspace_bytes < 0) return none();
+    at::Tensor workspace = empty({p.workspace_bytes}, at::kByte, q);
+    p.workspace = workspace.data_ptr();
+    const int rc = launch(packed ? lib.gqa_prefill : lib.gqa_decode, &p, stream_of(q));
+    return rc != 0 ? code(rc) : pair(out, lse);
+}
+
+// (k, v, k_pool, v_pool, block_table, insert_pos, q_start, n_rows, k_scale, v_scale, status) -> the library's code
+PyObject* gqa_insert(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 11) return none();
+    const bool packed = a[6] != Py_None;
+    const at::Tensor *k = any_tensor(a[0]), *v = any_tensor(a[1]), *pos = tensor(a[5], at::kInt, 1), *start, *n_rows, *status;
+    if (!gqa_rows(k, packed ? 3 : 4) || !gqa_rows(v, packed ? 3 : 4) || k->sizes() != v->sizes() || k->scalar_type() != v->scalar_type() || pos == nullptr) return none();
+    const int64_t B = pos->size(0);
+    GqaPools pool;
+    if (B <= 0 || !fits32(B) || (!packed && k->size(0) != B) || !pool.take(a[2], a[3], a[8], a[9], a[4], B)) return none();
+    if (!optional_tensor(a[6], at::kInt, 1, &start) || !has_shape(start, {B + 1}) || !optional_tensor(a[7], at::kInt, 1, &n_rows) || !has_shape(n_rows, {B})) return none();
+    if ((packed && n_rows != nullptr) || !optional_tensor(a[10], at::kInt, 1, &status) || (status != nullptr && status->numel() < DSV4_STATUS_WORDS)) return none();
+    Dsv4GqaInsertParams p{};
+    p.src_dtype = gqa_type(k, false);
+    p.kv_dtype = pool.type;
+    if (p.src_dtype < 0 || (p.kv_dtype != DSV4_DTYPE_E4M3 && p.kv_dtype != p.src_dtype) || k->size(-1) != pool.D || k->size(-2) != pool.Hkv || pool.D % 8 != 0) return none();
+    const int64_t T = packed ? 0 : k->size(1);
+    if (!fits32(T) || !fits32(pool.D) || !same_device(k, {v, pos, start, n_rows, status, pool.k, pool.v, pool.k_scale, pool.v_scale, pool.table})) return none();
+    const c10::cuda::CUDAGuard guard(k->device());
+    p.B = int(B);  p.T = int(T);  p.Hkv = int(pool.Hkv);  p.D = int(pool.D);  p.max_pages = int(pool.table->size(1));
+    p.rows = packed ? k->size(0) : B * T;  p.num_pages = pool.k->size(0);
+    p.k_stride_b = packed ? 0 : row_stride(k, 0);  p.k_stride_t = row_stride(k, packed ? 0 : 1);  p.k_stride_h = row_stride(k, packed ? 1 : 2);
+    p.v_stride_b = packed ? 0 : row_stride(v, 0);  p.v_stride_t = row_stride(v, packed ? 0 : 1);  p.v_stride_h = row_stride(v, packed ? 1 : 2);
+    p.k = ptr(k);  p.v = ptr(v);  p.q_start = ptr<int32_t>(start);  p.n_rows = ptr<int32_t>(n_rows);  p.k_pool = ptr(pool.k);  p.v_pool = ptr(pool.v);
+    p.block_table = ptr<int32_t>(pool.table);  p.insert_pos = ptr<int32_t>(pos);  p.k_scale = ptr<float>(pool.k_scale);  p.v_scale = ptr<float>(pool.v_scale);
+    p.status = ptr<int32_t>(status);
+    return code(p.rows == 0 ? 0 : launch(lib.gqa_insert, &p, stream_of(k)));
+}
+
+// (pools: a tuple, block_table, kv_len, page_refs, weights, keep, first, recent, new_table, new_len, new_refs, new_weights, kept, status)
+//   -> (table, kv_len, refs, weights, kept) or the library's code
+PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 14 || !PyTuple_Check(a[0]) || PyTuple_GET_SIZE(a[0]) < 1 || PyTuple_GET_SIZE(a[0]) > DSV4_EVICT_POOLS) return none();
+    Dsv4KvEvictParams p{};
+    const at::Tensor *table = tensor(a[1], at::kInt, 2), *len = tensor(a[2], at::kInt, 1), *refs = tensor(a[3], at::kInt, 1), *weights = tensor(a[4], at::kFloat, 2), *each, *status;
+    if (table == nullptr || len == nullptr || refs == nullptr || weights == nullptr || table->numel() <= 0 || refs->size(0) <= 0) return none();
+    const int64_t B = table->size(0), width = table->size(1), cap = width * kPage;
+    if (!has_shape(len, {B}) || weights->size(0) != B || weights->size(1) < cap || !fits32(B) || !fits32(cap) || !fits32(refs->size(0))) return none();
+    p.pools = int(PyTuple_GET_SIZE(a[0]));
+    for (int i = 0; i < p.pools; ++i) {
+        const at::Tensor* t = any_tensor(PyTuple_GET_ITEM(a[0], i));
+        if (t == nullptr || !t->is_cuda() || !t->is_contiguous() || t->dim() < 4 || t->numel() <= 0 || t->size(1) != refs->size(0) || t->size(2) != kPage) return none();
+        if ((i > 0 && t->size(0) != p.layers) || !same_device(table, {t})) return none();
+        p.layers = t->size(0);
+        p.pool[i] = ptr(t);
+        p.entry_bytes[i] = int64_t(t->nbytes()) / (t->size(0) * t->size(1) * kPage);
+        if (p.entry_bytes[i] % 16 != 0) return none();
+    }
+    int64_t keep = 0, first, recent;
+    if (PyLong_Check(a[5]) ? !integer(a[5], &keep) || keep < 0 || !fits32(keep) : (each = tensor(a[5], at::kInt, 1)) == nullptr || !has_shape(each, {B})) return none();
+    if (PyLong_Check(a[5])) each = nullptr;
+    if (!integer(a[6], &first) || !integer(a[7], &recent) || !fits32(first) || !fits32(recent)) return none();
+    if (!optional_tensor(a[13], at::kInt, 1, &status) || (status != nullptr && status->numel() < DSV4_STATUS_WORDS)) return none();
+    const c10::cuda::CUDAGuard guard(table->device());
+    Output out[5];
+    if (!out[0].take(a[8], at::kInt, {B, width}, table) || !out[1].take(a[9], at::kInt, {B}, table) || !out[2].take(a[10], at::kInt, {refs->size(0)}, table) ||
+        !out[3].take(a[11], at::kFloat, weights->sizes(), table) || !out[4].take(a[12], at::kInt, {B, cap}, table))
+        return none();
+    if (!same_device(table, {len, refs, weights, each, status, out[0].t, out[1].t, out[2].t, out[3].t, out[4].t})) return none();
+    at::Tensor scratch = empty({4 * B + B * cap}, at::kInt, table);
+    p.B = int(B);  p.max_pages = int(width);  p.keep = int(keep);  p.first = int(first);  p.recent = int(recent);  p.num_pages = refs->size(0);
+    p.keep_each = ptr<int32_t>(each);  p.block_table = ptr<int32_t>(table);  p.kv_len = ptr<int32_t>(len);  p.refs = ptr<int32_t>(refs);
+    p.weights = ptr<float>(weights);  p.weight_stride = weights->size(1);
+    p.new_table = ptr<int32_t>(out[0].t);  p.new_len = ptr<int32_t>(out[1].t);  p.new_refs = ptr<int32_t>(out[2].t);  p.new_weights = ptr<float>(out[3].t);
+    p.kept = ptr<int32_t>(out[4].t);  p.scratch = ptr<int32_t>(&scratch);  p.status = ptr<int32_t>(status);
+    const int rc = launch(lib.kv_evict, &p, stream_of(table));
+    if (rc != 0) return code(rc);
+    PyObject* r = PyTuple_New(5);
+    for (int i = 0; i < 5; ++i) PyTuple_SET_ITEM(r, i, out[i].result());
+    return r;
+}
+
 // C++ exceptions (the allocator's out-of-memory error among them) become None: the slow path meets the same error and raises it.
 template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
 PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
@@ -733,6 +892,7 @@ PyMethodDef methods[] = {
     DSV4_FAST(csa), DSV4_FAST(hca), DSV4_FAST(packed), DSV4_FAST(planes), DSV4_FAST(rope_norm), DSV4_FAST(insert), DSV4_FAST(csa_compress),
     DSV4_FAST(hca_compress), DSV4_FAST(indexer), DSV4_FAST(plan), DSV4_FAST(combine),
     DSV4_FAST(tree), DSV4_FAST(sample), DSV4_FAST(pages_copy), DSV4_FAST(entries_move), DSV4_FAST(pages_free), DSV4_FAST(pages_fork), DSV4_FAST(pages_compact),
+    DSV4_FAST(gqa), DSV4_FAST(gqa_insert), DSV4_FAST(evict),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

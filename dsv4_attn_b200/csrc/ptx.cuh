@@ -106,7 +106,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint64_
 // The same for a limit below four seconds and for a whole warp (all lanes get the same answer), with everything but the
 // first look out of line: kernels with many roles wait in many places, and code that does not fit the
 // instruction cache stalls all of them.
-__device__ __noinline__ bool mbar_wait_retry(uint32_t bar, uint32_t parity, uint32_t timeout_ns) {
+static __device__ __noinline__ bool mbar_wait_retry(uint32_t bar, uint32_t parity, uint32_t timeout_ns) {
     const uint32_t t0 = globaltimer_lo();
     bool done;
     do { done = mbar_try_wait(bar, parity); } while (!done && globaltimer_lo() - t0 < timeout_ns);

@@ -1,0 +1,208 @@
+"""Attention of new tokens over K and V pages against its definition in 64 bits: types, head layouts, lengths around the tiles' ends, windows, rows that see nothing,
+pages out of range, strides, graphs and streams.  Run with `-m gpu` on a B200."""
+import itertools
+
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+from tests.gqa_util import Case, PAGE  # noqa: E402
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    import dsv4_attn_b200 as d
+    return d
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "e4m3"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_lengths_around_tiles(lib, dtype, D):
+    st = lib.new_status("cuda")
+    c = Case([1, 2, 63, 64, 65, 127, 128, 129, 200, 0, 1000], 1, Hkv=2, G=4, D=D, dtype=dtype, seed=D)
+    c.check(*c.call(lib, status=st))
+    assert st.tolist() == [0, 0, 0, 0]
+
+
+@pytest.mark.parametrize("Hkv,G,T", [(1, 1, 1), (1, 16, 1), (3, 5, 1), (8, 1, 1), (2, 7, 3), (1, 17, 1), (2, 8, 4), (1, 33, 1), (1, 64, 1), (2, 16, 5), (1, 8, 40), (1, 100, 1)])
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+def test_heads_and_tokens(lib, Hkv, G, T, dtype):
+    c = Case([T, T + 1, 70 + T, 500, 3], T, Hkv=Hkv, G=G, D=128, dtype=dtype, seed=Hkv * G + T, sink=True)
+    c.check(*c.call(lib))
+
+
+@pytest.mark.parametrize("window,first", [(1, 0), (1, 1), (10, 0), (10, 3), (64, 64), (100, 65), (130, 500), (1 << 30, 4), ((1 << 31) - 1, 4), (7, (1 << 31) - 1)])
+@pytest.mark.parametrize("T", [1, 5, 70])
+def test_windows(lib, window, first, T):
+    for dtype, D in (("f16", 64), ("e4m3", 128)):
+        c = Case([1, 5, 64, 129, 300, 777], T, Hkv=2, G=3, D=D, dtype=dtype, window=window, first=first, seed=T, sink=T == 5)
+        c.check(*c.call(lib))
+
+
+def test_one_request_and_long_ones_are_shared_out(lib):
+    for kv in ([9000], [20000, 1, 300], [64 * 37]):
+        for dtype in ("bf16", "e4m3"):
+            c = Case(kv, 1, Hkv=4, G=4, D=128, dtype=dtype, seed=len(kv))
+            c.check(*c.call(lib))
+
+
+def test_many_requests(lib):
+    lens = [(i * 37) % 400 for i in range(1500)]
+    c = Case(lens, 1, Hkv=1, G=2, D=64, dtype="f16", seed=3)
+    c.check(*c.call(lib))
+
+
+@pytest.mark.parametrize("dtype,T,G,window", [("bf16", 1, 4, 0), ("f16", 3, 4, 0), ("e4m3", 2, 16, 0), ("bf16", 4, 2, 50), ("e4m3", 5, 16, 100), ("f16", 1, 1, 1)])
+def test_weights(lib, dtype, T, G, window):
+    st = lib.new_status("cuda")
+    c = Case([3, 64, 65, 700, 5, 0], T, Hkv=3, G=G, D=64, dtype=dtype, window=window, first=2 if window else 0, sink=True, seed=T)
+    before = torch.rand(c.B, c.table.shape[1] * PAGE + 5, device="cuda")
+    w = before.clone()
+    out, lse = c.call(lib, weights=w, status=st)
+    c.check(out, lse, w, before)
+    assert st.tolist() == [0, 0, 0, 0]
+    again = before.clone()
+    c.call(lib, weights=again)
+    assert torch.equal(again, w)                        # one order of sums
+
+
+def test_rows_of_a_fused_projection_and_given_outputs(lib):
+    c = Case([100, 300], 2, Hkv=2, G=4, D=128, dtype="bf16", fused=True)
+    assert not c.q.is_contiguous()
+    out = torch.full((2, 2, 8, 128), 7.0, device="cuda", dtype=torch.bfloat16)
+    lse = torch.full((2, 2, 8), 7.0, device="cuda")
+    o, s = c.call(lib, out=out, lse=lse)
+    assert o is out and s is lse
+    c.check(out, lse)
+    # heads before tokens
+    c.q = c.q.transpose(1, 2).contiguous().transpose(1, 2)
+    c.check(*c.call(lib))
+
+
+def test_queries_of_both_types_over_8_bits_and_their_range(lib):
+    for q_dtype in ("bf16", "f16"):
+        c = Case([200, 65], 1, Hkv=2, G=4, D=128, dtype="e4m3", q_dtype=q_dtype)
+        c.check(*c.call(lib))
+    # rows far outside FP16's range, with a scale that brings the scores back
+    for by in (1e30, 1e-30):
+        c = Case([200, 65], 1, Hkv=2, G=4, D=128, dtype="e4m3", by=by)
+        c.scale = 1.0 / (by * 128 ** 0.5)
+        c.check(*c.call(lib))
+
+
+def test_equal_and_extreme_scores(lib):
+    """Scores that are all alike, and one that outweighs the others by far."""
+    c = Case([130, 64], 1, Hkv=1, G=2, D=64, dtype="bf16")
+    c.q.zero_()
+    c.check(*c.call(lib))
+    c = Case([1000], 1, Hkv=1, G=2, D=64, dtype="bf16", by=100.0)
+    c.check(*c.call(lib))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+def test_a_nan_query_spoils_its_own_row_only(lib, dtype):
+    c = Case([500, 30], 1, Hkv=2, G=4, D=128, dtype=dtype)
+    want, want_lse = c.call(lib)
+    c.q[0, 0, 2, 5] = float("nan")
+    out, lse = c.call(lib)
+    assert out[0, 0, 2].isnan().all() and lse[0, 0, 2].isnan()
+    keep = torch.ones_like(lse, dtype=torch.bool)
+    keep[0, 0, 2] = False
+    assert torch.equal(out[keep], want[keep]) and torch.equal(lse[keep], want_lse[keep])
+
+
+def test_pages_out_of_range_are_left_out_and_reported(lib):
+    c = Case([300, 200], 1, Hkv=2, G=4, D=64, dtype="f16")
+    P = c.pools[0].shape[0]
+    for bad in (P, -1, (1 << 31) - 1, -(1 << 31)):
+        st = lib.new_status("cuda")
+        table = c.table.clone()
+        table[0, 2] = bad
+        w = torch.zeros(2, table.shape[1] * PAGE, device="cuda")
+        out, lse = lib.gqa_decode(c.q, *c.pools, table, c.len_t, c.scale, status=st, weights=w)
+        assert st[0] == 7
+        # as if the entries of that page were not there
+        k = torch.cat([c.entries(0, 0)[:128], c.entries(0, 0)[192:]])
+        x = torch.einsum("hd,nhd->hn", c.q[0, 0].double(), k.repeat_interleave(4, 1)) * c.scale
+        assert torch.allclose(lse[0, 0].double(), torch.logsumexp(x, -1), atol=1e-5)
+        assert (w[0, 128:192] == 0).all() and torch.allclose(w[0].sum(), torch.tensor(8.0, device="cuda"), atol=1e-4)
+    # a length beyond the table
+    st = lib.new_status("cuda")
+    longer = c.len_t + torch.tensor([0, 10_000_000], device="cuda", dtype=torch.int32)
+    out, lse = lib.gqa_decode(c.q, *c.pools, c.table, longer, c.scale, status=st)
+    assert st[0] == 7
+    st.zero_()
+    out, lse = lib.gqa_decode(c.q, *c.pools, c.table, torch.tensor([-5, 200], device="cuda", dtype=torch.int32), c.scale, status=st)
+    assert st[0] == 0 and (out[0] == 0).all() and torch.isneginf(lse[0]).all()
+
+
+def test_a_wait_that_runs_out(lib):
+    c = Case([3000, 200], 1, Hkv=2, G=4, D=64, dtype="f16")
+    st = lib.new_status("cuda")
+    lib.LIB.dsv4_debug_set_wait(200_000, 1)
+    try:
+        c.call(lib, status=st)
+        torch.cuda.synchronize()
+    finally:
+        lib.LIB.dsv4_debug_set_wait(0, -1)
+    assert st[0] == 1
+    st.zero_()
+    c.check(*c.call(lib, status=st))
+    assert st[0] == 0
+
+
+def test_captured_and_replayed_with_other_lengths(lib):
+    c = Case([100, 900, 64, 0], 1, Hkv=2, G=4, D=128, dtype="bf16", width=20)
+    c.call(lib)
+    w = torch.zeros(4, c.table.shape[1] * PAGE, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = c.call(lib, weights=w)
+    w.zero_()
+    graph.replay()
+    first = w.clone()
+    c.check(out, lse, w, torch.zeros_like(w))
+    d = Case([333, 1, 1280, 77], 1, Hkv=2, G=4, D=128, dtype="bf16", seed=9, width=20)
+    assert d.table.shape == c.table.shape
+    for to, of in ((c.q, d.q), (c.len_t, d.len_t), (c.table, d.table), (c.pools[0].view(torch.int16), d.pools[0].view(torch.int16)), (c.pools[1].view(torch.int16), d.pools[1].view(torch.int16))):
+        to.copy_(of)
+    w.zero_()
+    graph.replay()
+    d.check(out, lse, w, torch.zeros_like(w))
+    assert not torch.equal(first, w)
+
+
+def test_two_streams_at_once(lib):
+    cases = [Case([5000, 3], 1, Hkv=4, G=4, D=128, dtype="bf16", seed=i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = []
+    for _, (c, s) in itertools.product(range(5), zip(cases, streams)):
+        with torch.cuda.stream(s):
+            got.append((c, c.call(lib)))
+    torch.cuda.synchronize()
+    for c, r in got:
+        c.check(*r)
+
+
+def test_offsets_beyond_32_bits(lib):
+    """A pool of more than 2^32 bytes each for K and V, read at its end."""
+    P, Hkv, D = 70_000, 8, 64                        # 4.6 GB a pool
+    pools = [torch.zeros(P, PAGE, Hkv, D, device="cuda", dtype=torch.bfloat16) for _ in "kv"]
+    c = Case([100, 640], 1, Hkv=Hkv, G=2, D=D, dtype="bf16")
+    n = c.pools[0].shape[0]
+    for big, small in zip(pools, c.pools):
+        big[P - n:] = small
+    c.pools = pools
+    c.table = torch.where(c.table >= 0, c.table + (P - n), c.table)
+    c.check(*c.call(lib))
+
+
+def test_prefill_small(lib):
+    for dtype, D in (("bf16", 128), ("f16", 64), ("e4m3", 128), ("bf16", 256)):
+        for window, first in ((0, 0), (40, 3)):
+            c = Case([5, 70, 200, 1, 300], [5, 6, 150, 1, 0], Hkv=2, G=3, D=D, dtype=dtype, packed=True, window=window, first=first, sink=True)
+            c.check(*c.call(lib))
