@@ -7,6 +7,7 @@
 #include <atomic>
 
 #include "gqa_decode.cuh"
+#include "gqa_prefill.cuh"
 #include "kv_evict.cuh"
 #include "host_state.h"
 
@@ -48,19 +49,21 @@ cudaError_t launch(void (*kernel)(Args), dim3 grid, int threads, size_t smem, cu
 }
 
 // A pool of K or V heads by (element, head, entry): boxes of 128 bytes (or a shorter row) of one head in 64 entries.
-cudaError_t make_pool_map(CUtensorMap* map, const void* pool, int64_t pages, int Hkv, int D, int kv_dtype) {
+cudaError_t make_pool_map(CUtensorMap* map, const void* pool, int64_t pages, int Hkv, int D, int kv_dtype, int box_rows = kGqaTile) {
     const EncodeTiledFn fn = encode_tiled_fn();
     if (fn == nullptr) return cudaErrorNotSupported;
     const bool bytes = kv_dtype == DSV4_DTYPE_E4M3;
     const int es = bytes ? 1 : 2, box_bytes = D * es < 128 ? D * es : 128;
     const cuuint64_t dims[3] = {cuuint64_t(D), cuuint64_t(Hkv), cuuint64_t(pages) * kGqaTile};
     const cuuint64_t strides[2] = {cuuint64_t(D) * es, cuuint64_t(Hkv) * D * es};
-    const cuuint32_t box[3] = {cuuint32_t(box_bytes / es), 1, kGqaTile}, estr[3] = {1, 1, 1};
+    const cuuint32_t box[3] = {cuuint32_t(box_bytes / es), 1, cuuint32_t(box_rows)}, estr[3] = {1, 1, 1};
     const CUresult r = fn(map, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(pool), dims, strides, box, estr,
                           CU_TENSOR_MAP_INTERLEAVE_NONE, box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
+
+int64_t up(int64_t n) { return (n + 127) / 128 * 128; }
 
 // ── which form of the kernel ──
 // Rows of a KV head: 16, 32 or 64 in a group, the fewest that hold a request's (with 64: several groups).
@@ -92,7 +95,15 @@ struct Sizes {
     int blocks, group_rows;
     int64_t parts;                   // partial rows
     int64_t logit_rows, logit_stride;
+    bool prefill;                    // gqa_prefill_kernel
+    int64_t plan_words;
+    int64_t own_rows;                // entries of the call's own 16-bit pages
 };
+
+// ── which kernel takes a prompt ──
+// A block of tokens is 256 rows (heads of 256: 128) in gqa_prefill_kernel, and takes at least a block of the GPU to itself; the decode kernel takes 64 rows at a time and shares the entries out.
+constexpr int kPrefillMinUnits = 8, kPrefillMinRows = 64;
+constexpr int64_t kPrefillOwnBytes = int64_t(4) << 30;              // an 8-bit cache's pages are brought to 16 bits in a workspace of that size at most
 bool gqa_sizes(const Dsv4GqaParams* p, Sizes& s) {
     if (p == nullptr || p->B <= 0 || p->Hkv <= 0 || p->G <= 0 || p->max_pages <= 0 || p->T < 0 || p->rows < 0) return false;
     if (p->D != 64 && p->D != 128 && p->D != 256) return false;
@@ -109,9 +120,88 @@ bool gqa_sizes(const Dsv4GqaParams* p, Sizes& s) {
     s.parts = 2 * int64_t(s.blocks) * s.group_rows;
     s.logit_rows = p->weights != nullptr ? int64_t(p->B) * p->Hkv * p->T * p->G : 0;
     s.logit_stride = entries;
+    s.prefill = false;
+    s.plan_words = s.own_rows = 0;
+    if (p->q_start != nullptr && p->G <= 128 && p->rows < 0x7FFFFFFF) {
+        const int tile_tokens = 128 / p->G, block_tokens = tile_tokens * (p->D > 128 ? 1 : 2);
+        const int64_t blocks = p->rows / block_tokens + p->B, full = (p->rows + block_tokens - 1) / block_tokens;
+        const bool e4m3 = p->kv_dtype == DSV4_DTYPE_E4M3;
+        const int64_t own = e4m3 ? int64_t(p->B) * p->max_pages * kGqaTile : 0;
+        s.prefill = full * p->Hkv >= kPrefillMinUnits && p->rows * p->G >= int64_t(p->B) * kPrefillMinRows && own * p->Hkv * p->D * 4 <= kPrefillOwnBytes && own < 0x7FFFFF00;
+        if (s.prefill) {
+            s.plan_words = 4 + 2 * blocks;
+            s.own_rows = own;
+            const int64_t most = blocks * p->Hkv;
+            s.blocks = int(most < device_sms() ? most : device_sms());
+            s.group_rows = block_tokens * p->G;
+            s.parts = 0;
+        }
+    }
     return true;
 }
-int64_t up(int64_t n) { return (n + 127) / 128 * 128; }
+
+template <int D, bool BF16>
+cudaError_t run_prefill(const GqaPrefillArgs& a, cudaStream_t stream) {
+    using C = PrefillCfg<D, BF16>;
+    static std::atomic<bool> done[kMaxDevices];
+    cudaError_t e = ensure_smem(gqa_prefill_kernel<C>, C::Bytes, done);
+    if (e != cudaSuccess) return e;
+    return launch(gqa_prefill_kernel<C>, dim3(unsigned(a.g.blocks)), C::Threads, C::Bytes, stream, a);
+}
+
+// q by (element, head, row): boxes of 64 elements of a group's heads in a tile's tokens
+cudaError_t make_rows_map(CUtensorMap* map, const Dsv4GqaParams* p, int tile_tokens) {
+    const EncodeTiledFn fn = encode_tiled_fn();
+    if (fn == nullptr) return cudaErrorNotSupported;
+    const int H = p->Hkv * p->G;
+    const cuuint64_t dims[3] = {cuuint64_t(p->D), cuuint64_t(H), cuuint64_t(p->rows)};
+    // (axes of one element have any stride)
+    const cuuint64_t strides[2] = {cuuint64_t(H > 1 ? p->q_stride_h : p->D) * 2, cuuint64_t(p->rows > 1 ? p->q_stride_t : int64_t(H) * p->D) * 2};
+    const cuuint32_t box[3] = {64, cuuint32_t(p->G), cuuint32_t(tile_tokens)}, estr[3] = {1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(p->q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+cudaError_t prefill(GqaArgs& g, const Dsv4GqaParams* p, const Sizes& s, uint8_t* ws, cudaStream_t stream) {
+    GqaPrefillArgs a{};
+    a.plan = reinterpret_cast<int32_t*>(ws);
+    a.plan_units = int((s.plan_words - 4) / 2);
+    ws += up(s.plan_words * 4);
+    const void *k = p->k_pool, *v = p->v_pool;
+    int64_t pages = p->num_pages;
+    a.tile_tokens = 128 / p->G;
+    cudaError_t e = cudaSuccess;
+    if (s.own_rows > 0) {
+        GqaUnpackArgs u{};
+        u.g = g;
+        u.entry = p->Hkv * p->D;
+        for (int i = 0; i < 2; ++i) {
+            u.pool[i] = static_cast<const uint8_t*>(i ? v : k);
+            u.rows[i] = ws;
+            ws += up(s.own_rows * p->Hkv * p->D * 2);
+        }
+        k = u.rows[0];
+        v = u.rows[1];
+        pages = s.own_rows / kGqaTile;
+        a.own_pages = 1;
+        const int64_t most = int64_t(device_sms()) * 8;
+        e = launch(g.q_bf16 ? gqa_unpack_kernel<true> : gqa_unpack_kernel<false>, dim3(unsigned(pages < most ? pages : most)), kGqaUnpackThreads, 0, stream, u);
+        if (e != cudaSuccess) return e;
+    }
+    a.g = g;
+    a.pool_rows = pages * kGqaTile;
+    e = make_pool_map(&a.g.k_map, k, pages, p->Hkv, p->D, p->q_dtype);
+    if (e == cudaSuccess) e = make_pool_map(&a.g.v_map, v, pages, p->Hkv, p->D, p->q_dtype);
+    if (e == cudaSuccess) e = make_pool_map(&a.v8_map, v, pages, p->Hkv, p->D, p->q_dtype, 8);
+    if (e == cudaSuccess) e = make_pool_map(&a.v1_map, v, pages, p->Hkv, p->D, p->q_dtype, 1);
+    if (e == cudaSuccess) e = make_rows_map(&a.q_map, p, a.tile_tokens);
+    if (e == cudaSuccess) e = launch(gqa_plan_kernel, dim3(1), kPrefillPlanThreads, 0, stream, a);
+    if (e != cudaSuccess) return e;
+    if (p->D == 64) return g.q_bf16 ? run_prefill<64, true>(a, stream) : run_prefill<64, false>(a, stream);
+    if (p->D == 128) return g.q_bf16 ? run_prefill<128, true>(a, stream) : run_prefill<128, false>(a, stream);
+    return g.q_bf16 ? run_prefill<256, true>(a, stream) : run_prefill<256, false>(a, stream);
+}
 
 }  // namespace
 }  // namespace dsv4
@@ -121,7 +211,7 @@ using namespace dsv4;
 extern "C" int64_t dsv4_gqa_workspace_bytes(const Dsv4GqaParams* p) {
     Sizes s;
     if (!gqa_sizes(p, s)) return -1;
-    return up(s.parts * p->D * 4) + up(s.parts * 4) + up(s.logit_rows * s.logit_stride * 4) + up(s.logit_rows * 4);
+    return up(s.parts * p->D * 4) + up(s.parts * 4) + up(s.logit_rows * s.logit_stride * 4) + up(s.logit_rows * 4) + up(s.plan_words * 4) + 2 * up(s.own_rows * p->Hkv * p->D * 2);
 }
 
 static int gqa_fwd(const Dsv4GqaParams* p, void* stream_) {
@@ -162,6 +252,7 @@ static int gqa_fwd(const Dsv4GqaParams* p, void* stream_) {
     a.wait_ns = uint32_t(state.wait_ns < 4000000000ull ? state.wait_ns : 4000000000ull);
     a.dbg_drop_tile = state.drop_tile;
     a.status = p->status;
+    if (s.prefill) return int(prefill(a, p, s, ws, stream));
     cudaError_t e = make_pool_map(&a.k_map, p->k_pool, p->num_pages, p->Hkv, p->D, p->kv_dtype);
     if (e == cudaSuccess) e = make_pool_map(&a.v_map, p->v_pool, p->num_pages, p->Hkv, p->D, p->kv_dtype);
     if (e != cudaSuccess) return int(e);

@@ -226,10 +226,10 @@ struct GqaWalk {
         const int64_t per_head = gqa_head_tiles(a, req);
         h = int(off / per_head);
         off -= h * per_head;
-        for (rg = 0;; ++rg) {
-            span = gqa_span(a, req, rg);
-            if (off < span.count) break;
+        span = gqa_span(a, req, rg = 0);
+        for (const int groups = gqa_groups(a, req); off >= span.count && rg + 1 < groups;) {
             off -= span.count;
+            span = gqa_span(a, req, ++rg);
         }
         k0 = int(off);
         piece();
@@ -242,7 +242,7 @@ struct GqaWalk {
             rg = 0;
             if (++h >= a.Hkv) {
                 h = 0;
-                do { req = gqa_request(a, ++b); } while (req.tokens == 0);
+                do { req = gqa_request(a, ++b); } while (req.tokens == 0 && b + 1 < a.B);
             }
         }
         span = gqa_span(a, req, rg);
@@ -303,7 +303,11 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
     // where this block's share begins
     const int each = (a.B + kGqaThreads - 1) / kGqaThreads, b_from = tid * each, b_to = min(b_from + each, a.B);
     int64_t mine = 0, total;
-    for (int b = b_from; b < b_to; ++b) mine += gqa_head_tiles(a, gqa_request(a, b)) * a.Hkv;
+    for (int b = b_from; b < b_to; ++b) {
+        const GqaRequest r = gqa_request(a, b);
+        if (r.bad && blockIdx.x == 0) gqa_report(a.status, kGqaStatusBadIndex, 4, b);
+        mine += gqa_head_tiles(a, r) * a.Hkv;
+    }
     const int64_t before = block_prefix<kGqaThreads>(mine, total, scan);
     const int64_t share = gqa_share(a, total), begin = int64_t(blockIdx.x) * share;
     const int64_t tiles = min(share, total - begin);
@@ -329,7 +333,6 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
         uint32_t seq = 0;
         bool ok = true;
         for (; w.left > 0 && ok; w.next(a)) {
-            if (w.req.bad && lane == 0) gqa_report(a.status, kGqaStatusBadIndex, 4, w.b);
             for (int k = w.k0; k < w.k1 && ok; k += 32) {
                 // the pages of the next 32 tiles, one per lane
                 int page = -1;

@@ -1,0 +1,609 @@
+// Attention of prompts over pages of K and V heads, on the tensor cores.
+//
+// A unit is (request, block of tokens, KV head): 128 rows a tile, row = (token, query head of the group), floor(128 / G) tokens each; two tiles a block (heads of 256: one).
+// It goes through the entries that some row sees in steps of 128 (64), as gqa_span() lists them:
+//     S = Q K^T      tcgen05.mma, M = 128, both operands in shared memory, S in tensor memory
+//     P = exp2(c (S - ref)), in the softmax warps, a thread a row; back to tensor memory over S, in 16 bits
+//     O += P V       A = P from tensor memory, V as it lies in the cache (MN-major)
+// The two tiles take turns: while one tile's scores are in the softmax warps the tensor cores have the other's products.  The reference of a row moves only when its maximum
+// has passed it by 2^8; then O is rescaled in tensor memory by the row's thread (S of a step is complete only after the P V of the step before, so O is at rest).
+// Units are listed by gqa_plan_kernel, those with most steps first, and dealt out to resident blocks; the next unit's Q comes in, and its first scores are
+// computed, while the last one's output is written.
+//
+// What bounds it: per step of two tiles x 128 entries x D = 128 the tensor pipe needs 1024 cycles, the 32,768 exponentials 2048 at 16 a cycle.
+//
+// K and V come by TMA in boxes of a page, 128-byte swizzle.  V of entries that no row sees must count as zero whatever the memory holds: pages at the ends of what is seen
+// are fetched in boxes of eight rows and of one, zeros (rows behind the pool) in the place of those.
+#pragma once
+
+#include "gqa_decode.cuh"
+
+namespace dsv4 {
+
+constexpr int kPrefillPlanThreads = 1024, kPrefillBuckets = 1024;
+constexpr float kPrefillLazy = 8.f;               // log2 of how far a row's maximum may pass its reference
+
+struct GqaPrefillArgs {
+    GqaArgs g;                       // group_rows: rows of a unit (tokens of a block x G); k_map, v_map: boxes of a page
+    alignas(64) CUtensorMap q_map;   // (element, head, row of q): boxes of 64 elements x G heads x the tokens of a tile
+    CUtensorMap v8_map, v1_map;      // boxes of eight entries and of one
+    int32_t* plan;                   // [0] units of one KV head; from [4] on (request, block) pairs
+    int plan_units;                  // room for them
+    int tile_tokens;                 // floor(128 / G)
+    int own_pages;                   // the pools are the call's copies: slot s of request b is page b * max_pages + s
+    int64_t pool_rows;               // entries of the pools: the first row behind them
+};
+
+template <int D_, bool BF16_>
+struct PrefillCfg {
+    static constexpr int D = D_;
+    static constexpr bool BF16 = BF16_;
+    static constexpr int NT = D <= 128 ? 2 : 1, NE = D <= 128 ? 128 : 64, Pages = NE / kGqaTile;
+    static constexpr int Slot = NE * D * 2, QTile = 128 * D * 2;
+    static constexpr int Slots = (225 * 1024 - NT * QTile) / Slot;
+    static constexpr int Flags = 16;              // steps whose page flags are kept: the producer is at most Slots / 2 + 2 ahead of the softmax warps
+    static_assert(Slots / 2 + 2 < Flags, "");
+    static constexpr int SoftmaxWarps = 4 * NT, Threads = SoftmaxWarps * 32 + 64;
+    static constexpr int OffRing = NT * QTile, OffBars = OffRing + Slots * Slot, OffThere = OffBars + 8 * (2 * Slots + 2 * NT + 4 + NT), OffMisc = OffThere + 4 * Flags;
+    static constexpr int Bytes = (OffMisc + 16 + 127) / 128 * 128 + 1024;
+    static constexpr int ColO = 256;
+};
+
+// Entries seen by some row of tokens [t0, t1] of a request, in tiles of `tile` entries (a multiple of a page).
+__device__ __forceinline__ GqaSpan prefill_span(const GqaArgs& a, const GqaRequest& r, int t0, int t1, int tile) {
+    GqaSpan s;
+    s.t0 = t0;
+    s.t1 = t1;
+    s.hi = max(min(r.place0 + t1 + 1, r.entries), 0);
+    s.lo = 0;
+    s.first = 0;
+    if (a.window > 0) {
+        s.lo = min(max(r.place0 + t0 - a.window + 1, 0), s.hi);
+        s.first = min(a.first, s.hi);
+    }
+    const int end = (s.hi + tile - 1) / tile, heads = (s.first + tile - 1) / tile, from = s.lo / tile;
+    s.head = min(heads, from);
+    s.skip = from - s.head;
+    s.count = max(end - s.skip, 1);
+    return s;
+}
+
+// Units in the order of their steps: a counting sort.
+__global__ void __launch_bounds__(kPrefillPlanThreads) gqa_plan_kernel(const __grid_constant__ GqaPrefillArgs p) {
+    __shared__ int count[kPrefillBuckets];
+    __shared__ int64_t sums[kPrefillPlanThreads / 32];
+    __shared__ int most;
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    const GqaArgs& a = p.g;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int block_tokens = a.group_rows / a.G, tile = kGqaTile;
+    for (int i = tid; i < kPrefillBuckets; i += kPrefillPlanThreads) count[i] = 0;
+    if (tid == 0) most = 0;
+    __syncthreads();
+    auto each = [&](auto&& f) {
+        for (int b = warp; b < a.B; b += kPrefillPlanThreads / 32) {
+            const GqaRequest r = gqa_request(a, b);
+            for (int i = lane; i * int64_t(block_tokens) < r.tokens; i += 32) f(b, i, prefill_span(a, r, i * block_tokens, min((i + 1) * block_tokens, r.tokens) - 1, tile).count);
+        }
+    };
+    for (int b = tid; b < a.B; b += kPrefillPlanThreads)
+        if (gqa_request(a, b).bad) gqa_report(a.status, kGqaStatusBadIndex, 4, b);
+    int top = 0;
+    each([&](int, int, int steps) { top = max(top, steps); });
+    atomicMax(&most, top);
+    __syncthreads();
+    const int shift = max(0, 32 - __clz(most) - 10);                          // steps >> shift < 1024
+    each([&](int, int, int steps) { atomicAdd(&count[kPrefillBuckets - 1 - (steps >> shift)], 1); });
+    __syncthreads();
+    int64_t total;
+    const int64_t before = block_prefix<kPrefillPlanThreads>(count[tid], total, sums);
+    __syncthreads();
+    count[tid] = int(before);
+    __syncthreads();
+    int2* const list = reinterpret_cast<int2*>(p.plan + 4);
+    // (offsets that overlap, which are reported, can name more blocks than there are rows for)
+    each([&](int b, int i, int steps) {
+        const int at = atomicAdd(&count[kPrefillBuckets - 1 - (steps >> shift)], 1);
+        if (at < p.plan_units) list[at] = make_int2(b, i);
+    });
+    if (tid == 0) p.plan[0] = int(min(total, int64_t(p.plan_units)));
+}
+
+// ── tcgen05, one block ──
+__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
+                 :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
+                 :: "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+// The units of a block, walked by each role for itself.
+struct PrefillWalk {
+    int u, total, h;
+    GqaRequest req;
+    GqaSpan span;
+    int b;
+    __device__ __forceinline__ void take(const GqaPrefillArgs& p, int tile) {
+        if (u >= total) return;
+        const GqaArgs& a = p.g;
+        h = u % a.Hkv;
+        const int32_t* const at = p.plan + 4 + 2 * (u / a.Hkv);
+        b = ptx::ld(at);
+        const int block = ptx::ld(at + 1), tokens = a.group_rows / a.G;
+        req = gqa_request(a, b);
+        span = prefill_span(a, req, block * tokens, min((block + 1) * tokens, req.tokens) - 1, tile);
+    }
+    __device__ __forceinline__ void begin(const GqaPrefillArgs& p, int tile) {
+        total = ptx::ld(p.plan) * p.g.Hkv;
+        u = blockIdx.x;
+        take(p, tile);
+    }
+    __device__ __forceinline__ bool more() const { return u < total; }
+    __device__ __forceinline__ void next(const GqaPrefillArgs& p, int tile) {
+        u += gridDim.x;
+        take(p, tile);
+    }
+};
+
+template <class C>
+__global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid_constant__ GqaPrefillArgs p) {
+    constexpr int D = C::D, NT = C::NT, NE = C::NE;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t* const base = smem_raw + (smem - ptx::smem_u32(smem_raw));
+    const uint32_t ring = smem + C::OffRing;
+    const uint32_t kv_full = smem + C::OffBars, kv_empty = kv_full + 8 * C::Slots, q_full = kv_empty + 8 * C::Slots, q_empty = q_full + 8 * NT;
+    const uint32_t s_full = q_empty + 8 * NT, p_full = s_full + 16, o_full = p_full + 16;
+    volatile uint32_t* const there = reinterpret_cast<volatile uint32_t*>(base + C::OffThere);      // of a step: a bit per page
+    volatile uint32_t* const tmem_at = reinterpret_cast<volatile uint32_t*>(base + C::OffMisc);
+    const GqaArgs& a = p.g;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+    if (tid == 0) {
+        for (int i = 0; i < C::Slots; ++i) { ptx::mbar_init(kv_full + 8 * i, 1);  ptx::mbar_init(kv_empty + 8 * i, 1); }
+        for (int i = 0; i < NT; ++i) { ptx::mbar_init(q_full + 8 * i, 1);  ptx::mbar_init(q_empty + 8 * i, 1);  ptx::mbar_init(o_full + 8 * i, 1); }
+        for (int i = 0; i < 2; ++i) { ptx::mbar_init(s_full + 8 * i, 1);  ptx::mbar_init(p_full + 8 * i, 4); }
+        ptx::fence_mbar_init();
+        ptx::prefetch_tensormap(&p.q_map);
+        ptx::prefetch_tensormap(&a.k_map);
+        ptx::prefetch_tensormap(&a.v_map);
+    }
+    if (warp == C::SoftmaxWarps + 1) {
+        ptx::tmem_alloc(smem + C::OffMisc, 512);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::tc_fence_after_sync();
+    const uint32_t tmem = *tmem_at;
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    PrefillWalk w;
+    w.begin(p, NE);
+    bool ok = true;
+    auto wait = [&](uint32_t bar, uint32_t turn, int role, int what) {
+        if (!ok) return;
+        if (!ptx::mbar_wait_warp(bar, turn & 1u, a.wait_ns)) {
+            if (lane == 0) gqa_report(a.status, kGqaStatusWait, role, what);
+            ok = false;
+        }
+    };
+
+    if (warp == C::SoftmaxWarps) {
+        // ── producer ──
+        uint32_t seq = 0, unit = 0;
+        for (; w.more() && ok; w.next(p, NE), ++unit) {
+            for (int t = 0; t < NT && ok; ++t) {
+                if (unit > 0) wait(q_empty + 8 * t, unit - 1, 0, int(unit));
+                if (ok && ptx::elect_one()) {
+                    ptx::mbar_arrive_expect_tx(q_full + 8 * t, uint32_t(p.tile_tokens * a.G * D * 2));
+#pragma unroll
+                    for (int x = 0; x < D / 64; ++x)
+                        ptx::tma_load_3d(smem + t * C::QTile + x * (128 * 128), &p.q_map, 64 * x, w.h * a.G, int(w.req.row0) + w.span.t0 + t * p.tile_tokens, q_full + 8 * t);
+                }
+                __syncwarp();
+            }
+            constexpr int kAhead = 32 / C::Pages;                             // steps whose pages the lanes hold
+            for (int k = 0; k < w.span.count && ok; k += kAhead) {
+                int page = -1;
+                const int kk = k + lane / C::Pages, slot = w.span.slot(kk) * C::Pages + lane % C::Pages;
+                if (kk < w.span.count && w.span.hi > 0 && slot * kGqaTile < w.span.hi) {
+                    page = ptx::ld(a.block_table + int64_t(w.b) * a.max_pages + slot);
+                    if (page < 0 || page >= a.num_pages) {
+                        // (pages between the first entries and the window are not read, and may be gone)
+                        const int from = slot * kGqaTile;
+                        if (from < w.span.first || from + kGqaTile > w.span.lo) gqa_report(a.status, kGqaStatusBadIndex, 4, page);
+                        page = -1;
+                    } else if (p.own_pages) {
+                        page = w.b * a.max_pages + slot;
+                    }
+                }
+                const int n = min(kAhead, w.span.count - k);
+                for (int i = 0; i < n && ok; ++i) {
+                    int pg[C::Pages];
+#pragma unroll
+                    for (int j = 0; j < C::Pages; ++j) pg[j] = __shfl_sync(0xFFFFFFFFu, page, i * C::Pages + j);
+                    const int e0 = w.span.slot(k + i) * NE;
+#pragma unroll
+                    for (int kv = 0; kv < 2; ++kv, ++seq) {
+                        const uint32_t st = seq % C::Slots, round = seq / C::Slots;
+                        if (round > 0) wait(kv_empty + 8 * st, round - 1, 0, int(seq));
+                        if (!ok) break;
+                        if (a.dbg_drop_tile >= 0 && int(seq) == 2 * a.dbg_drop_tile) continue;       // a test's lost arrival
+                        if (ptx::elect_one()) {
+                            const uint32_t full = kv_full + 8 * st, at = ring + st * C::Slot;
+                            if (kv == 0) {
+                                uint32_t bits = 0;
+#pragma unroll
+                                for (int j = 0; j < C::Pages; ++j) bits |= uint32_t(pg[j] >= 0) << j;
+                                there[(seq / 2) % C::Flags] = bits;
+                            }
+                            ptx::mbar_arrive_expect_tx(full, C::Slot);
+#pragma unroll
+                            for (int j = 0; j < C::Pages; ++j) {
+                                const int row = pg[j] >= 0 ? pg[j] * kGqaTile : int(p.pool_rows), e = e0 + j * kGqaTile;
+                                const bool whole = pg[j] < 0 || (e + kGqaTile <= w.span.hi && (e >= w.span.lo || e + kGqaTile <= w.span.first));
+                                if (kv == 0 || whole) {
+#pragma unroll
+                                    for (int x = 0; x < D / 64; ++x)
+                                        ptx::tma_load_3d(at + x * (NE * 128) + j * (kGqaTile * 128), kv ? &a.v_map : &a.k_map, 64 * x, w.h, row, full);
+                                } else {
+                                    auto seen = [&](int i) { return i < w.span.hi && (i >= w.span.lo || i < w.span.first); };
+                                    for (int r8 = 0; r8 < kGqaTile; r8 += 8) {
+                                        uint32_t bits = 0;
+                                        for (int r = 0; r < 8; ++r) bits |= uint32_t(seen(e + r8 + r)) << r;
+                                        for (int x = 0; x < D / 64; ++x) {
+                                            const uint32_t to = at + x * (NE * 128) + (j * kGqaTile + r8) * 128;
+                                            if (bits == 0u || bits == 255u) {
+                                                ptx::tma_load_3d(to, &p.v8_map, 64 * x, w.h, bits ? row + r8 : int(p.pool_rows), full);
+                                            } else {
+                                                for (int r = 0; r < 8; ++r)
+                                                    ptx::tma_load_3d(to + r * 128, &p.v1_map, 64 * x, w.h, (bits >> r) & 1u ? row + r8 + r : int(p.pool_rows), full);
+                                            }
+                                        }
+                                    }
+                                }
+                            }
+                        }
+                        __syncwarp();
+                    }
+                }
+            }
+        }
+    } else if (warp == C::SoftmaxWarps + 1) {
+        // ── products ──
+        constexpr uint32_t kIdescS = C::BF16 ? ptx::make_idesc_bf16(128, NE, false, false) : ptx::make_idesc_f16(128, NE, false, false);
+        constexpr uint32_t kIdescO = C::BF16 ? ptx::make_idesc_bf16(128, D, false, true) : ptx::make_idesc_f16(128, D, false, true);
+        // S of tile t from K in slot st, into S buffer i
+        auto scores = [&](int t, int i, uint32_t st) {
+            if (ptx::elect_one()) {
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint64_t ad = ptx::make_smem_desc(smem + t * C::QTile + (k / 4) * (128 * 128) + (k % 4) * 32, 16, 1024);
+                    const uint64_t bd = ptx::make_smem_desc(ring + st * C::Slot + (k / 4) * (NE * 128) + (k % 4) * 32, 16, 1024);
+                    mma_ss(tmem + i * NE, ad, bd, kIdescS, k ? 1u : 0u);
+                }
+                ptx::mma_commit(s_full + 8 * i);
+            }
+            __syncwarp();
+        };
+        auto outputs = [&](int t, int i, uint32_t st, bool add) {
+            if (ptx::elect_one()) {
+#pragma unroll
+                for (int k = 0; k < NE / 16; ++k) {
+                    const uint64_t bd = ptx::make_smem_desc(ring + st * C::Slot + k * 2048, NE * 128, 1024);
+                    mma_ts(tmem + C::ColO + t * D, tmem + i * NE + k * 8, bd, kIdescO, add || k ? 1u : 0u);
+                }
+            }
+            __syncwarp();
+        };
+        auto commit = [&](uint32_t bar) {
+            if (ptx::elect_one()) ptx::mma_commit(bar);
+            __syncwarp();
+        };
+        uint32_t step = 0, unit = 0;                                          // steps of all units so far
+        auto wait_kv = [&](uint32_t s) {
+            wait(kv_full + 8 * (s % C::Slots), s / C::Slots, 1, int(s));
+            ptx::tc_fence_after_sync();
+        };
+        if constexpr (NT == 2) {
+            // the first scores of a unit go out behind the last products of the one before
+            if (w.more()) {
+                wait_kv(0);
+                for (int t = 0; t < 2 && ok; ++t) {
+                    wait(q_full + 8 * t, 0, 1, 0);
+                    ptx::tc_fence_after_sync();
+                    if (!ok) break;
+                    scores(t, t, 0);
+                    if (w.span.count == 1) commit(q_empty + 8 * t);
+                }
+                if (ok) commit(kv_empty);
+            }
+            while (w.more() && ok) {
+                const int n = w.span.count;
+                PrefillWalk ahead = w;
+                ahead.next(p, NE);
+                for (int j = 0; j < n && ok; ++j, ++step) {
+                    const uint32_t ks = 2 * (step + 1), vs = 2 * step + 1;
+                    const bool last = j + 1 == n, on = !last || ahead.more();
+                    for (int t = 0; t < 2 && ok; ++t) {
+                        wait(p_full + 8 * t, step, 1, int(step));
+                        if (t == 0) wait_kv(vs);
+                        ptx::tc_fence_after_sync();
+                        if (!ok) break;
+                        outputs(t, t, vs % C::Slots, j > 0);
+                        if (last) commit(o_full + 8 * t);
+                        if (t == 1) commit(kv_empty + 8 * (vs % C::Slots));
+                        if (on) {
+                            if (t == 0) wait_kv(ks);
+                            if (last) {
+                                wait(q_full + 8 * t, unit + 1, 1, int(unit));
+                                ptx::tc_fence_after_sync();
+                            }
+                            if (!ok) break;
+                            scores(t, t, ks % C::Slots);
+                            if (last ? ahead.span.count == 1 : j + 2 == n) commit(q_empty + 8 * t);
+                            if (t == 1) commit(kv_empty + 8 * (ks % C::Slots));
+                        }
+                    }
+                }
+                w = ahead;
+                ++unit;
+            }
+        } else {
+            for (; w.more() && ok; w.next(p, NE), ++unit) {
+                const int n = w.span.count;
+                wait(q_full, unit, 1, int(unit));
+                for (int j = -1; j < n && ok; ++j) {
+                    if (j + 1 < n) {
+                        const uint32_t at = step + uint32_t(j + 1);
+                        wait_kv(2 * at);
+                        if (!ok) break;
+                        scores(0, at & 1, (2 * at) % C::Slots);
+                        commit(kv_empty + 8 * ((2 * at) % C::Slots));
+                        if (j + 2 == n) commit(q_empty);
+                    }
+                    if (j >= 0) {
+                        const uint32_t at = step + uint32_t(j);
+                        wait(p_full + 8 * (at & 1), at >> 1, 1, int(at));
+                        wait_kv(2 * at + 1);
+                        if (!ok) break;
+                        outputs(0, at & 1, (2 * at + 1) % C::Slots, j > 0);
+                        commit(o_full);
+                        commit(kv_empty + 8 * ((2 * at + 1) % C::Slots));
+                    }
+                }
+                step += uint32_t(n);
+            }
+        }
+    } else {
+        // ── softmax: a thread has a row ──
+        const int t = warp >> 2;
+        const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
+        const int r = (warp & 3) * 32 + lane, tok = r / a.G, gg = r - tok * a.G;
+        const int H = a.Hkv * a.G;
+        const bool real = r < p.tile_tokens * a.G;                            // (rows behind hold what the memory held)
+        const float neg = -INFINITY;
+        uint32_t step = 0, unit = 0;
+        for (; w.more() && ok; w.next(p, NE), ++unit) {
+            const int token = w.span.t0 + t * p.tile_tokens + tok, place = w.req.place0 + token;
+            const int first_place = w.req.place0 + w.span.t0 + t * p.tile_tokens, last_place = first_place + p.tile_tokens - 1;
+            const float scale = a.scale_log2 * (a.k_scale != nullptr ? ptx::ld(a.k_scale + w.h) : 1.f);
+            float ref = neg, l = 0.f;
+            for (int j = 0; j < w.span.count; ++j, ++step) {
+                const int i = NT == 2 ? t : int(step & 1);
+                const uint32_t s_at = lane_base + i * NE;
+                const int e0 = w.span.slot(j) * NE;
+                // (the producer's flags: K has arrived when its scores have)
+                wait(s_full + 8 * i, NT == 2 ? step : step >> 1, 2, int(step));
+                if (!ok) break;
+                ptx::tc_fence_after_sync();
+                const uint32_t pages = there[step % C::Flags];
+                const bool whole = pages == (1u << C::Pages) - 1u && e0 + NE - 1 <= first_place && e0 + NE <= w.req.entries &&
+                                   (a.window == 0 || e0 > last_place - a.window || e0 + NE - 1 < a.first);
+                // scores of 32 entries, those that the row does not see -inf
+                auto load = [&](uint32_t (&v)[32], int c) {
+                    ptx::tmem_ld32(s_at + 32 * c, v);
+                    uint32_t see = 0xFFFFFFFFu;
+                    if (!whole) {
+                        const int at = e0 + 32 * c;
+                        auto below = [](int n) { return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u; };
+                        see = below(min(place + 1, w.req.entries) - at);
+                        if (a.window > 0) see &= ~below(place - a.window + 1 - at) | below(a.first - at);
+                        if (!((pages >> (32 * c / kGqaTile)) & 1u)) see = 0u;
+                    }
+                    ptx::tmem_wait_ld();
+                    if (!whole) {
+#pragma unroll
+                        for (int x = 0; x < 32; ++x)
+                            if (!((see >> x) & 1u)) v[x] = __float_as_uint(neg);
+                    }
+                };
+                uint32_t pk[NE / 2];
+                float sum;
+                if (j == 0) {
+                    float t0 = neg, t1 = neg;
+#pragma unroll
+                    for (int c = 0; c < NE / 32; ++c) {
+                        uint32_t v[32];
+                        load(v, c);
+#pragma unroll
+                        for (int x = 0; x < 32; x += 4) {
+                            t0 = ptx::max3(t0, __uint_as_float(v[x]), __uint_as_float(v[x + 1]));
+                            t1 = ptx::max3(t1, __uint_as_float(v[x + 2]), __uint_as_float(v[x + 3]));
+                        }
+                    }
+                    ref = fmaxf(t0, t1);
+                }
+                // Once, or where a row's maximum has passed its reference by too much (or a row sees its first entry), a second time with the maximum as the reference.
+                // (Differences are taken before they are scaled: at the maximum 0, however large it is.)
+#pragma unroll 1
+                for (int again = 0; again < 2; ++again) {
+                    const float sub = ref == neg ? 0.f : -ref;
+                    const uint64_t sub2 = ptx::pack_f32x2(sub, sub), scale2 = ptx::pack_f32x2(scale, scale);
+                    uint64_t s0 = ptx::pack_f32x2(0.f, 0.f), s1 = s0;
+                    float t0 = neg, t1 = neg;
+#pragma unroll
+                    for (int c = 0; c < NE / 32; ++c) {
+                        uint32_t v[32];
+                        load(v, c);
+#pragma unroll
+                        for (int x = 0; x < 32; x += 4) {
+                            t0 = ptx::max3(t0, __uint_as_float(v[x]), __uint_as_float(v[x + 1]));
+                            t1 = ptx::max3(t1, __uint_as_float(v[x + 2]), __uint_as_float(v[x + 3]));
+#pragma unroll
+                            for (int q = 0; q < 4; q += 2) {
+                                float x0, x1;
+                                ptx::unpack_f32x2(ptx::mul_f32x2(ptx::add_f32x2(ptx::pack_f32x2(__uint_as_float(v[x + q]), __uint_as_float(v[x + q + 1])), sub2), scale2), x0, x1);
+                                const float p0 = ptx::ex2(x0), p1 = ptx::ex2(x1);
+                                if (q == 0) s0 = ptx::add_f32x2(s0, ptx::pack_f32x2(p0, p1));
+                                else s1 = ptx::add_f32x2(s1, ptx::pack_f32x2(p0, p1));
+                                pk[16 * c + (x + q) / 2] = C::BF16 ? ptx::pack_bf16x2(p0, p1) : ptx::pack_f16x2(p0, p1);
+                            }
+                        }
+                    }
+                    float a0, a1;
+                    ptx::unpack_f32x2(ptx::add_f32x2(s0, s1), a0, a1);
+                    sum = a0 + a1;
+                    const float top = fmaxf(t0, t1);
+                    const bool move = real && again == 0 && ((top - ref) * scale > kPrefillLazy || (ref == neg && top > neg));
+                    if (!__any_sync(0xFFFFFFFFu, move)) break;
+                    float by = 1.f;
+                    if (move) {
+                        if (ref != neg) by = ptx::ex2((ref - top) * scale);
+                        ref = top;
+                        l *= by;
+                    }
+                    if (j == 0) continue;
+                    if constexpr (NT == 1) {
+                        wait(o_full, step - 1, 2, int(step));
+                        ptx::tc_fence_after_sync();
+                    }
+                    const uint32_t o_at = lane_base + C::ColO + t * D;
+#pragma unroll 1
+                    for (int c = 0; c < D / 32; ++c) {
+                        uint32_t v[32];
+                        ptx::tmem_ld32(o_at + 32 * c, v);
+                        ptx::tmem_wait_ld();
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) v[x] = __float_as_uint(__uint_as_float(v[x]) * by);
+                        ptx::tmem_st32(o_at + 32 * c, v);
+                    }
+                    ptx::tmem_wait_st();
+                }
+                l += sum;
+                // (every turn of the barrier is waited for, so that the wait for the last one cannot take an earlier one for it)
+                if (NT == 1 && j > 0) wait(o_full, step - 1, 2, int(step));
+#pragma unroll
+                for (int c = 0; c < NE / 64; ++c) {
+                    uint32_t(&v)[32] = *reinterpret_cast<uint32_t(*)[32]>(&pk[32 * c]);
+                    ptx::tmem_st32(s_at + 32 * c, v);
+                }
+                ptx::tmem_wait_st();
+                ptx::tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(p_full + 8 * i);
+            }
+            if (!ok) break;
+            // ── the row's output ──
+            wait(o_full + 8 * t, NT == 2 ? unit : step - 1, 3, int(unit));
+            if (!ok) break;
+            ptx::tc_fence_after_sync();
+            const bool mine = real && token <= w.span.t1;
+            const int head = w.h * a.G + gg;
+            const int64_t row = (w.req.row0 + token) * H + head;
+            const bool none = l == 0.f;
+            float all = l, by = 1.f;
+            if (mine && a.sink != nullptr && !none) {
+                const float s = ptx::ld(a.sink + head) * 1.4426950408889634f, top = ref * scale, m2 = fmaxf(top, s);
+                by = ptx::ex2(top - m2);
+                all = l * by + ptx::ex2(s - m2);
+            }
+            const float per = none ? 0.f : by * (a.v_scale != nullptr ? ptx::ld(a.v_scale + w.h) : 1.f) / all;
+            uint8_t* const to = static_cast<uint8_t*>(a.out) + row * (D * 2);
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t v[32];
+                ptx::tmem_ld32(lane_base + C::ColO + t * D + 32 * c, v);
+                ptx::tmem_wait_ld();
+                if (mine) {
+                    uint32_t o[16];
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) {
+                        const float o0 = none ? 0.f : __uint_as_float(v[2 * x]) * per, o1 = none ? 0.f : __uint_as_float(v[2 * x + 1]) * per;
+                        o[x] = C::BF16 ? ptx::pack_bf16x2(o0, o1) : ptx::pack_f16x2(o0, o1);
+                    }
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) *reinterpret_cast<uint4*>(to + 64 * c + 16 * x) = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
+                }
+            }
+            if (mine && a.lse != nullptr) a.lse[row] = none ? neg : (ref * scale + log2f(l)) * 0.6931471805599453f;
+            ptx::tc_fence_before_sync();
+        }
+    }
+    // common exit: every role comes here, with or without a failure
+    ptx::tc_fence_before_sync();
+    const bool failed = __syncthreads_or(!ok);
+    if (failed) {
+        const uint32_t t0 = ptx::globaltimer_lo();                            // copies and products that are on their way end within microseconds
+        while (ptx::globaltimer_lo() - t0 < 1000000u) __nanosleep(1000);
+    }
+    if (warp == C::SoftmaxWarps + 1) {
+        ptx::tc_fence_after_sync();
+        ptx::tmem_dealloc(tmem, 512);
+    }
+}
+
+// ── an 8-bit cache's pages in 16 bits ──
+// e4m3 values (exact in BF16 and FP16; the scales go into scores and outputs) of every page that some token sees, to pages of the call's own: [B * max_pages][64][Hkv][D].
+constexpr int kGqaUnpackThreads = 256;
+struct GqaUnpackArgs {
+    GqaArgs g;
+    const uint8_t* pool[2];
+    uint8_t* rows[2];
+    int entry;                       // Hkv * D
+};
+template <bool BF16>
+__global__ void __launch_bounds__(kGqaUnpackThreads) gqa_unpack_kernel(const __grid_constant__ GqaUnpackArgs u) {
+    ptx::pdl_trigger();
+    ptx::pdl_wait();
+    const GqaArgs& a = u.g;
+    const int vecs = u.entry * kGqaTile / 16;                                 // of a page
+    const int64_t pages = int64_t(a.B) * a.max_pages;
+    for (int64_t at = blockIdx.x; at < pages; at += gridDim.x) {
+        const int b = int(at / a.max_pages), slot = int(at - int64_t(b) * a.max_pages);
+        const GqaRequest r = gqa_request(a, b);
+        if (r.tokens == 0) continue;
+        const int from = slot * kGqaTile, lo = a.window > 0 ? max(r.place0 - a.window + 1, 0) : 0;
+        if (from >= r.entries || (from + kGqaTile <= lo && from >= a.first)) continue;
+        const int page = ptx::ld(a.block_table + at);
+        if (page < 0 || page >= a.num_pages) continue;
+#pragma unroll 1
+        for (int kv = 0; kv < 2; ++kv) {
+            const uint4* const src = reinterpret_cast<const uint4*>(u.pool[kv]) + int64_t(page) * vecs;
+            uint4* const dst = reinterpret_cast<uint4*>(u.rows[kv]) + at * vecs * 2;
+#pragma unroll 4
+            for (int i = threadIdx.x; i < vecs; i += kGqaUnpackThreads) {
+                const uint4 v = ptx::ldg_stream_v4(src + i);
+                const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+                uint32_t o[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    ptx::e4m3x4_to_f16x4(x[j], o[2 * j], o[2 * j + 1]);
+                    if (BF16)
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&o[2 * j + q]));
+                            o[2 * j + q] = ptx::pack_bf16x2(f.x, f.y);
+                        }
+                }
+                ptx::stg_v8(dst + 2 * i, make_uint4(o[0], o[1], o[2], o[3]), make_uint4(o[4], o[5], o[6], o[7]));
+            }
+        }
+    }
+}
+
+}  // namespace dsv4

@@ -88,7 +88,9 @@ class Case:
         out_tol, lse_tol = torch.zeros_like(out), torch.zeros_like(lse)
         weights, weight_tol = [], []
         half = torch.finfo(self.q_dtype).eps / 2                       # of a rounding of the output
-        p_half = torch.finfo(torch.float16 if self.dtype == torch.float8_e4m3fn else self.dtype).eps / 2
+        # P is rounded to the type that V is multiplied in: half a step, eps / 2 of each weight.  An 8-bit cache is read as FP16 by the decode kernel; for prompts it is
+        # brought to the type of the queries, so that with BF16 ones P is rounded to BF16 there: 2^-8 of a weight instead of 2^-11
+        p_half = torch.finfo(self.dtype if self.dtype != torch.float8_e4m3fn else self.q_dtype if self.packed else torch.float16).eps / 2
         # P in FP16: below its normal numbers a weight is off by up to 2^-25 of the largest one
         p_small = 0.0 if self.dtype == torch.bfloat16 else 2.0 ** -25
         # BF16 queries over an 8-bit cache: elements below 2^-14 of the row's largest are off by up to 2^-25 of it
