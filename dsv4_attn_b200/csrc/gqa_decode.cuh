@@ -153,7 +153,7 @@ __device__ __forceinline__ int64_t block_prefix(int64_t v, int64_t& total, int64
 // The length of a share, which the attention kernel and the merge work out alike.
 __device__ __forceinline__ int64_t gqa_share(const GqaArgs& a, int64_t total) { return max((total + a.blocks - 1) / a.blocks, int64_t(a.min_share)); }
 
-__device__ __noinline__ void gqa_report(int32_t* status, int code, int role, int what) {
+__device__ __forceinline__ void gqa_report(int32_t* status, int code, int role, int what) {
     if (status != nullptr && atomicCAS(status, 0, code) == 0) {
         status[1] = int(blockIdx.x);
         status[2] = role;

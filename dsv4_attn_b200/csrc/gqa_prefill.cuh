@@ -43,7 +43,10 @@ struct PrefillCfg {
     static constexpr int Slots = (225 * 1024 - NT * QTile) / Slot;
     static constexpr int Flags = 16;              // steps whose page flags are kept: the producer is at most Slots / 2 + 2 ahead of the softmax warps
     static_assert(Slots / 2 + 2 < Flags, "");
-    static constexpr int SoftmaxWarps = 4 * NT, Threads = SoftmaxWarps * 32 + 64;
+    static constexpr int SoftmaxWarps = 4 * NT, Threads = SoftmaxWarps * 32 + 128;
+    // Registers of a thread at launch (__launch_bounds__), and as the warpgroups share them out: the softmax warps hold a row's scores.
+    static constexpr int RegsSoftmax = 208, RegsOthers = 88;
+    static_assert(NT == 1 || (4 * NT * RegsSoftmax + 4 * RegsOthers) * 32 <= 168 * Threads, "");
     static constexpr int OffRing = NT * QTile, OffBars = OffRing + Slots * Slot, OffThere = OffBars + 8 * (2 * Slots + 2 * NT + 4 + NT), OffMisc = OffThere + 4 * Flags;
     static constexpr int Bytes = (OffMisc + 16 + 127) / 128 * 128 + 1024;
     static constexpr int ColO = 256;
@@ -120,6 +123,19 @@ __device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_
                  :: "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                   "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+                    "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 // The units of a block, walked by each role for itself.
 struct PrefillWalk {
     int u, total, h;
@@ -186,12 +202,19 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
     bool ok = true;
     auto wait = [&](uint32_t bar, uint32_t turn, int role, int what) {
         if (!ok) return;
-        if (!ptx::mbar_wait_warp(bar, turn & 1u, a.wait_ns)) {
+        // (in line: a called function would take registers by the convention of calls, which the split of registers leaves no room for)
+        if (__all_sync(0xFFFFFFFFu, ptx::mbar_try_wait(bar, turn & 1u))) return;
+        const uint32_t t0 = ptx::globaltimer_lo();
+        bool done;
+        do { done = ptx::mbar_try_wait(bar, turn & 1u); } while (!done && ptx::globaltimer_lo() - t0 < a.wait_ns);
+        if (!__all_sync(0xFFFFFFFFu, done)) {
             if (lane == 0) gqa_report(a.status, kGqaStatusWait, role, what);
             ok = false;
         }
     };
 
+    if (warp >= C::SoftmaxWarps) {
+    if constexpr (NT == 2) regs_dec<C::RegsOthers>();
     if (warp == C::SoftmaxWarps) {
         // ── producer ──
         uint32_t seq = 0, unit = 0;
@@ -379,8 +402,10 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
                 step += uint32_t(n);
             }
         }
+    }
     } else {
         // ── softmax: a thread has a row ──
+        if constexpr (NT == 2) regs_inc<C::RegsSoftmax>();
         const int t = warp >> 2;
         const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
         const int r = (warp & 3) * 32 + lane, tok = r / a.G, gg = r - tok * a.G;
@@ -404,104 +429,118 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
                 const uint32_t pages = there[step % C::Flags];
                 const bool whole = pages == (1u << C::Pages) - 1u && e0 + NE - 1 <= first_place && e0 + NE <= w.req.entries &&
                                    (a.window == 0 || e0 > last_place - a.window || e0 + NE - 1 < a.first);
-                // scores of 32 entries, those that the row does not see -inf
-                auto load = [&](uint32_t (&v)[32], int c) {
-                    ptx::tmem_ld32(s_at + 32 * c, v);
-                    uint32_t see = 0xFFFFFFFFu;
-                    if (!whole) {
-                        const int at = e0 + 32 * c;
-                        auto below = [](int n) { return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u; };
-                        see = below(min(place + 1, w.req.entries) - at);
-                        if (a.window > 0) see &= ~below(place - a.window + 1 - at) | below(a.first - at);
-                        if (!((pages >> (32 * c / kGqaTile)) & 1u)) see = 0u;
-                    }
-                    ptx::tmem_wait_ld();
-                    if (!whole) {
-#pragma unroll
-                        for (int x = 0; x < 32; ++x)
-                            if (!((see >> x) & 1u)) v[x] = __float_as_uint(neg);
-                    }
-                };
-                uint32_t pk[NE / 2];
-                float sum;
-                if (j == 0) {
-                    float t0 = neg, t1 = neg;
-#pragma unroll
-                    for (int c = 0; c < NE / 32; ++c) {
-                        uint32_t v[32];
-                        load(v, c);
-#pragma unroll
-                        for (int x = 0; x < 32; x += 4) {
-                            t0 = ptx::max3(t0, __uint_as_float(v[x]), __uint_as_float(v[x + 1]));
-                            t1 = ptx::max3(t1, __uint_as_float(v[x + 2]), __uint_as_float(v[x + 3]));
-                        }
-                    }
-                    ref = fmaxf(t0, t1);
-                }
-                // Once, or where a row's maximum has passed its reference by too much (or a row sees its first entry), a second time with the maximum as the reference.
-                // (Differences are taken before they are scaled: at the maximum 0, however large it is.)
-#pragma unroll 1
-                for (int again = 0; again < 2; ++again) {
-                    const float sub = ref == neg ? 0.f : -ref;
-                    const uint64_t sub2 = ptx::pack_f32x2(sub, sub), scale2 = ptx::pack_f32x2(scale, scale);
-                    uint64_t s0 = ptx::pack_f32x2(0.f, 0.f), s1 = s0;
-                    float t0 = neg, t1 = neg;
-#pragma unroll
-                    for (int c = 0; c < NE / 32; ++c) {
-                        uint32_t v[32];
-                        load(v, c);
-#pragma unroll
-                        for (int x = 0; x < 32; x += 4) {
-                            t0 = ptx::max3(t0, __uint_as_float(v[x]), __uint_as_float(v[x + 1]));
-                            t1 = ptx::max3(t1, __uint_as_float(v[x + 2]), __uint_as_float(v[x + 3]));
-#pragma unroll
-                            for (int q = 0; q < 4; q += 2) {
-                                float x0, x1;
-                                ptx::unpack_f32x2(ptx::mul_f32x2(ptx::add_f32x2(ptx::pack_f32x2(__uint_as_float(v[x + q]), __uint_as_float(v[x + q + 1])), sub2), scale2), x0, x1);
-                                const float p0 = ptx::ex2(x0), p1 = ptx::ex2(x1);
-                                if (q == 0) s0 = ptx::add_f32x2(s0, ptx::pack_f32x2(p0, p1));
-                                else s1 = ptx::add_f32x2(s1, ptx::pack_f32x2(p0, p1));
-                                pk[16 * c + (x + q) / 2] = C::BF16 ? ptx::pack_bf16x2(p0, p1) : ptx::pack_f16x2(p0, p1);
-                            }
-                        }
-                    }
-                    float a0, a1;
-                    ptx::unpack_f32x2(ptx::add_f32x2(s0, s1), a0, a1);
-                    sum = a0 + a1;
-                    const float top = fmaxf(t0, t1);
-                    const bool move = real && again == 0 && ((top - ref) * scale > kPrefillLazy || (ref == neg && top > neg));
-                    if (!__any_sync(0xFFFFFFFFu, move)) break;
+                // A row whose maximum has passed its reference by too much, or that sees its first entry, takes the maximum as its reference; O so far is rescaled.
+                auto refer = [&](float top) {
+                    const bool move = real && (ref == neg ? top > neg : (top - ref) * scale > kPrefillLazy);
+                    if (!__any_sync(0xFFFFFFFFu, move)) return;
                     float by = 1.f;
                     if (move) {
                         if (ref != neg) by = ptx::ex2((ref - top) * scale);
                         ref = top;
                         l *= by;
                     }
-                    if (j == 0) continue;
+                    if (j == 0) return;
                     if constexpr (NT == 1) {
                         wait(o_full, step - 1, 2, int(step));
                         ptx::tc_fence_after_sync();
                     }
                     const uint32_t o_at = lane_base + C::ColO + t * D;
 #pragma unroll 1
-                    for (int c = 0; c < D / 32; ++c) {
-                        uint32_t v[32];
-                        ptx::tmem_ld32(o_at + 32 * c, v);
+                    for (int c = 0; c < D / 16; ++c) {
+                        uint32_t o[16];
+                        tmem_ld16(o_at + 16 * c, o);
                         ptx::tmem_wait_ld();
 #pragma unroll
-                        for (int x = 0; x < 32; ++x) v[x] = __float_as_uint(__uint_as_float(v[x]) * by);
-                        ptx::tmem_st32(o_at + 32 * c, v);
+                        for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * by);
+                        tmem_st16(o_at + 16 * c, o);
                     }
                     ptx::tmem_wait_st();
-                }
-                l += sum;
-                // (every turn of the barrier is waited for, so that the wait for the last one cannot take an earlier one for it)
-                if (NT == 1 && j > 0) wait(o_full, step - 1, 2, int(step));
+                };
+                bool done = false;
+                if (whole) {
+                    // all of the row's scores in registers
+                    uint32_t v[NE / 32][32];
 #pragma unroll
-                for (int c = 0; c < NE / 64; ++c) {
-                    uint32_t(&v)[32] = *reinterpret_cast<uint32_t(*)[32]>(&pk[32 * c]);
-                    ptx::tmem_st32(s_at + 32 * c, v);
+                    for (int c = 0; c < NE / 32; ++c) ptx::tmem_ld32(s_at + 32 * c, v[c]);
+                    ptx::tmem_wait_ld();
+                    float t0 = neg, t1 = neg;
+#pragma unroll
+                    for (int c = 0; c < NE / 32; ++c)
+#pragma unroll
+                        for (int x = 0; x < 32; x += 4) {
+                            t0 = ptx::max3(t0, __uint_as_float(v[c][x]), __uint_as_float(v[c][x + 1]));
+                            t1 = ptx::max3(t1, __uint_as_float(v[c][x + 2]), __uint_as_float(v[c][x + 3]));
+                        }
+                    refer(fmaxf(t0, t1));
+                    const float sub = ref == neg ? 0.f : -ref * scale;
+                    // (where scores are so large that the rounding of this product would tell, the other way)
+                    done = !__any_sync(0xFFFFFFFFu, fabsf(sub) >= 16777216.f);
+                    if (done) {
+                        const uint64_t sub2 = ptx::pack_f32x2(sub, sub), scale2 = ptx::pack_f32x2(scale, scale);
+                        uint64_t s0 = ptx::pack_f32x2(l, 0.f), s1 = ptx::pack_f32x2(0.f, 0.f);
+#pragma unroll
+                        for (int c = 0; c < NE / 32; ++c) {
+                            uint32_t pk[16];
+#pragma unroll
+                            for (int x = 0; x < 32; x += 2) {
+                                float x0, x1;
+                                ptx::unpack_f32x2(ptx::fma_f32x2(ptx::pack_f32x2(__uint_as_float(v[c][x]), __uint_as_float(v[c][x + 1])), scale2, sub2), x0, x1);
+                                x0 = ptx::ex2(x0);
+                                x1 = ptx::ex2(x1);
+                                if (x & 2) s1 = ptx::add_f32x2(s1, ptx::pack_f32x2(x0, x1));
+                                else s0 = ptx::add_f32x2(s0, ptx::pack_f32x2(x0, x1));
+                                pk[x / 2] = C::BF16 ? ptx::pack_bf16x2(x0, x1) : ptx::pack_f16x2(x0, x1);
+                            }
+                            tmem_st16(s_at + 16 * c, pk);
+                        }
+                        float a0, a1;
+                        ptx::unpack_f32x2(ptx::add_f32x2(s0, s1), a0, a1);
+                        l = a0 + a1;
+                    }
                 }
+                if (!done) {
+                    // 32 scores at a time; what the row does not see is -inf.  Differences are taken before they are scaled: at the maximum 0, however large it is.
+                    auto load = [&](uint32_t (&v)[32], int c) {
+                        ptx::tmem_ld32(s_at + 32 * c, v);
+                        const int at = e0 + 32 * c;
+                        auto below = [](int n) { return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u; };
+                        uint32_t see = below(min(place + 1, w.req.entries) - at);
+                        if (a.window > 0) see &= ~below(place - a.window + 1 - at) | below(a.first - at);
+                        if (!((pages >> (32 * c / kGqaTile)) & 1u)) see = 0u;
+                        ptx::tmem_wait_ld();
+#pragma unroll
+                        for (int x = 0; x < 32; ++x)
+                            if (!((see >> x) & 1u)) v[x] = __float_as_uint(neg);
+                    };
+                    float t0 = neg, t1 = neg;
+#pragma unroll 1
+                    for (int c = 0; c < NE / 32; ++c) {
+                        uint32_t v[32];
+                        load(v, c);
+#pragma unroll
+                        for (int x = 0; x < 32; x += 4) {
+                            t0 = ptx::max3(t0, __uint_as_float(v[x]), __uint_as_float(v[x + 1]));
+                            t1 = ptx::max3(t1, __uint_as_float(v[x + 2]), __uint_as_float(v[x + 3]));
+                        }
+                    }
+                    refer(fmaxf(t0, t1));
+                    const float sub = ref == neg ? 0.f : ref;
+                    // (P of 32 entries takes the place of scores that have been read)
+#pragma unroll 1
+                    for (int c = 0; c < NE / 32; ++c) {
+                        uint32_t v[32], pk[16];
+                        load(v, c);
+#pragma unroll
+                        for (int x = 0; x < 32; x += 2) {
+                            const float x0 = ptx::ex2((__uint_as_float(v[x]) - sub) * scale), x1 = ptx::ex2((__uint_as_float(v[x + 1]) - sub) * scale);
+                            l += x0 + x1;
+                            pk[x / 2] = C::BF16 ? ptx::pack_bf16x2(x0, x1) : ptx::pack_f16x2(x0, x1);
+                        }
+                        tmem_st16(s_at + 16 * c, pk);
+                    }
+                }
+                // (every turn of this barrier is waited for, so that the wait for the last cannot take an earlier one for it)
+                if (NT == 1 && j > 0) wait(o_full, step - 1, 2, int(step));
                 ptx::tmem_wait_st();
                 ptx::tc_fence_before_sync();
                 __syncwarp();
