@@ -1,16 +1,19 @@
 // Attention of prompts over pages of K and V heads, on the tensor cores.
 //
 // A unit is (request, block of tokens, KV head): 128 rows a tile, row = (token, query head of the group), floor(128 / G) tokens each; two tiles a block (heads of 256: one).
-// It goes through the entries that some row sees in steps of 128 (64), as gqa_span() lists them:
-//     S = Q K^T      tcgen05.mma, M = 128, both operands in shared memory, S in tensor memory
-//     P = exp2(c (S - ref)), in the softmax warps, a thread a row; back to tensor memory over S, in 16 bits
-//     O += P V       A = P from tensor memory, V as it lies in the cache (MN-major)
-// The two tiles take turns: while one tile's scores are in the softmax warps the tensor cores have the other's products.  The reference of a row moves only when its maximum
-// has passed it by 2^8; then O is rescaled in tensor memory by the row's thread (S of a step is complete only after the P V of the step before, so O is at rest).
-// Units are listed by gqa_plan_kernel, those with most steps first, and dealt out to resident blocks; the next unit's Q comes in, and its first scores are
-// computed, while the last one's output is written.
+// It goes through the pages that some row sees, 64 entries a step:
+//     S = Q K^T               tcgen05.mma, M = 128, both operands in shared memory, S in tensor memory (two buffers a tile)
+//     P = exp2(c (S - ref))   in the softmax warps, a thread a row; back to tensor memory over S, in 16 bits
+//     O += P V                A = P from tensor memory, V as it lies in the cache (MN-major)
+// The scores of a step are computed while the softmax warps have those of the step before, and the two tiles take turns.  The reference of a row moves only when its maximum has
+// passed it by 2^8; then O is rescaled in tensor memory by the row's thread.  Units are listed by gqa_plan_kernel, those with most steps first, and dealt out to resident
+// blocks, one an SM; the next unit's Q comes in, and its first scores are computed, while the last one's output is written.
 //
-// What bounds it: per step of two tiles x 128 entries x D = 128 the tensor pipe needs 1024 cycles, the 32,768 exponentials 2048 at 16 a cycle.
+// What bounds it, per step of two tiles with D = 128, in cycles of an SM: the tensor pipe 1280 (scores 48 an instruction, bound by their operands' way out of shared memory, outputs 64),
+// the 16,384 exponentials 1024.  A step takes 1800, of which a softmax warp spends 1100 in exponentials, two warps a scheduler; and from some 20 ms on the power limit holds the clock:
+// 4,096 tokens behind 12,288 in 0.91 ms for the first calls after a pause, 0.99 under load, 0.97 PFLOP/s (the library's products: 1.42).  Measured and taken back: steps of 128 entries with
+// one score buffer a tile, where scores, softmax and outputs of a tile follow one another (1.06 ms; a window of 1,024: 320 us against 275); one warp for all products (1.12: a look at a
+// barrier takes 130 to 210 cycles while products keep the shared memory busy); a quarter to a half of the exponentials as polynomials on the multiply-add pipe (0.995 to 1.03).
 //
 // K and V come by TMA in boxes of a page, 128-byte swizzle.  V of entries that no row sees must count as zero whatever the memory holds: pages at the ends of what is seen
 // are fetched in boxes of eight rows and of one, zeros (rows behind the pool) in the place of those.
@@ -38,16 +41,13 @@ template <int D_, bool BF16_>
 struct PrefillCfg {
     static constexpr int D = D_;
     static constexpr bool BF16 = BF16_;
-    static constexpr int NT = D <= 128 ? 2 : 1, NE = D <= 128 ? 128 : 64, Pages = NE / kGqaTile;
+    static constexpr int NT = D <= 128 ? 2 : 1, NE = kGqaTile;
     static constexpr int Slot = NE * D * 2, QTile = 128 * D * 2;
     static constexpr int Slots = (225 * 1024 - NT * QTile) / Slot;
     static constexpr int Flags = 16;              // steps whose page flags are kept: the producer is at most Slots / 2 + 2 ahead of the softmax warps
     static_assert(Slots / 2 + 2 < Flags, "");
-    static constexpr int SoftmaxWarps = 4 * NT, Threads = SoftmaxWarps * 32 + 128;
-    // Registers of a thread at launch (__launch_bounds__), and as the warpgroups share them out: the softmax warps hold a row's scores.
-    static constexpr int RegsSoftmax = 208, RegsOthers = 88;
-    static_assert(NT == 1 || (4 * NT * RegsSoftmax + 4 * RegsOthers) * 32 <= 168 * Threads, "");
-    static constexpr int OffRing = NT * QTile, OffBars = OffRing + Slots * Slot, OffThere = OffBars + 8 * (2 * Slots + 2 * NT + 4 + NT), OffMisc = OffThere + 4 * Flags;
+    static constexpr int SoftmaxWarps = 4 * NT, Threads = (SoftmaxWarps + 2 + NT) * 32;
+    static constexpr int OffRing = NT * QTile, OffBars = OffRing + Slots * Slot, OffThere = OffBars + 8 * (2 * Slots + 2 * NT + 6 * NT), OffMisc = OffThere + 4 * Flags;
     static constexpr int Bytes = (OffMisc + 16 + 127) / 128 * 128 + 1024;
     static constexpr int ColO = 256;
 };
@@ -114,15 +114,17 @@ __global__ void __launch_bounds__(kPrefillPlanThreads) gqa_plan_kernel(const __g
 }
 
 // ── tcgen05, one block ──
-__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n"
-                 :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+// Descriptors as halves: from one instruction to the next only the low one changes, by a constant (computed anew for each they took longer than the products).
+__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}\n"
+                 :: "r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n"
-                 :: "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t desc_hi, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tmov.b64 db, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}\n"
+                 :: "r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate) : "memory");
 }
-
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
@@ -133,8 +135,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
                  :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
                     "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
-template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 // The units of a block, walked by each role for itself.
 struct PrefillWalk {
@@ -172,22 +172,22 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
     uint8_t* const base = smem_raw + (smem - ptx::smem_u32(smem_raw));
     const uint32_t ring = smem + C::OffRing;
     const uint32_t kv_full = smem + C::OffBars, kv_empty = kv_full + 8 * C::Slots, q_full = kv_empty + 8 * C::Slots, q_empty = q_full + 8 * NT;
-    const uint32_t s_full = q_empty + 8 * NT, p_full = s_full + 16, o_full = p_full + 16;
-    volatile uint32_t* const there = reinterpret_cast<volatile uint32_t*>(base + C::OffThere);      // of a step: a bit per page
+    const uint32_t s_full = q_empty + 8 * NT, p_full = s_full + 16 * NT, o_full = p_full + 16 * NT;     // of (tile, buffer)
+    volatile uint32_t* const there = reinterpret_cast<volatile uint32_t*>(base + C::OffThere);      // of a step: its page is in the pool
     volatile uint32_t* const tmem_at = reinterpret_cast<volatile uint32_t*>(base + C::OffMisc);
     const GqaArgs& a = p.g;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
     if (tid == 0) {
-        for (int i = 0; i < C::Slots; ++i) { ptx::mbar_init(kv_full + 8 * i, 1);  ptx::mbar_init(kv_empty + 8 * i, 1); }
-        for (int i = 0; i < NT; ++i) { ptx::mbar_init(q_full + 8 * i, 1);  ptx::mbar_init(q_empty + 8 * i, 1);  ptx::mbar_init(o_full + 8 * i, 1); }
-        for (int i = 0; i < 2; ++i) { ptx::mbar_init(s_full + 8 * i, 1);  ptx::mbar_init(p_full + 8 * i, 4); }
+        for (int i = 0; i < C::Slots; ++i) { ptx::mbar_init(kv_full + 8 * i, 1);  ptx::mbar_init(kv_empty + 8 * i, NT); }
+        for (int i = 0; i < NT; ++i) { ptx::mbar_init(q_full + 8 * i, 1);  ptx::mbar_init(q_empty + 8 * i, 1); }
+        for (int i = 0; i < 2 * NT; ++i) { ptx::mbar_init(s_full + 8 * i, 1);  ptx::mbar_init(p_full + 8 * i, 4);  ptx::mbar_init(o_full + 8 * i, 1); }
         ptx::fence_mbar_init();
         ptx::prefetch_tensormap(&p.q_map);
         ptx::prefetch_tensormap(&a.k_map);
         ptx::prefetch_tensormap(&a.v_map);
     }
-    if (warp == C::SoftmaxWarps + 1) {
+    if (warp == C::SoftmaxWarps) {
         ptx::tmem_alloc(smem + C::OffMisc, 512);
         ptx::tmem_relinquish();
     }
@@ -200,6 +200,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
     PrefillWalk w;
     w.begin(p, NE);
     bool ok = true;
+    // Two barriers at a time where a role waits for two: a look takes long while products keep the shared memory busy.
     auto wait = [&](uint32_t bar, uint32_t turn, int role, int what) {
         if (!ok) return;
         // (in line: a called function would take registers by the convention of calls, which the split of registers leaves no room for)
@@ -213,8 +214,13 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
         }
     };
 
-    if (warp >= C::SoftmaxWarps) {
-    if constexpr (NT == 2) regs_dec<C::RegsOthers>();
+    auto wait2 = [&](uint32_t bar_a, uint32_t turn_a, uint32_t bar_b, uint32_t turn_b, int role, int what) {
+        const bool a_done = ptx::mbar_try_wait(bar_a, turn_a & 1u), b_done = ptx::mbar_try_wait(bar_b, turn_b & 1u);
+        if (__all_sync(0xFFFFFFFFu, a_done && b_done)) return;
+        wait(bar_a, turn_a, role, what);
+        wait(bar_b, turn_b, role, what);
+    };
+
     if (warp == C::SoftmaxWarps) {
         // ── producer ──
         uint32_t seq = 0, unit = 0;
@@ -229,27 +235,22 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
                 }
                 __syncwarp();
             }
-            constexpr int kAhead = 32 / C::Pages;                             // steps whose pages the lanes hold
-            for (int k = 0; k < w.span.count && ok; k += kAhead) {
+            for (int k = 0; k < w.span.count && ok; k += 32) {
+                // the pages of the next 32 steps, one per lane
                 int page = -1;
-                const int kk = k + lane / C::Pages, slot = w.span.slot(kk) * C::Pages + lane % C::Pages;
-                if (kk < w.span.count && w.span.hi > 0 && slot * kGqaTile < w.span.hi) {
+                const int slot = w.span.slot(k + lane), from = slot * kGqaTile;
+                if (k + lane < w.span.count && from < w.span.hi) {
                     page = ptx::ld(a.block_table + int64_t(w.b) * a.max_pages + slot);
                     if (page < 0 || page >= a.num_pages) {
-                        // (pages between the first entries and the window are not read, and may be gone)
-                        const int from = slot * kGqaTile;
-                        if (from < w.span.first || from + kGqaTile > w.span.lo) gqa_report(a.status, kGqaStatusBadIndex, 4, page);
+                        gqa_report(a.status, kGqaStatusBadIndex, 4, page);
                         page = -1;
                     } else if (p.own_pages) {
                         page = w.b * a.max_pages + slot;
                     }
                 }
-                const int n = min(kAhead, w.span.count - k);
+                const int n = min(32, w.span.count - k);
                 for (int i = 0; i < n && ok; ++i) {
-                    int pg[C::Pages];
-#pragma unroll
-                    for (int j = 0; j < C::Pages; ++j) pg[j] = __shfl_sync(0xFFFFFFFFu, page, i * C::Pages + j);
-                    const int e0 = w.span.slot(k + i) * NE;
+                    const int pg = __shfl_sync(0xFFFFFFFFu, page, i), e0 = w.span.slot(k + i) * NE;
 #pragma unroll
                     for (int kv = 0; kv < 2; ++kv, ++seq) {
                         const uint32_t st = seq % C::Slots, round = seq / C::Slots;
@@ -258,34 +259,24 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
                         if (a.dbg_drop_tile >= 0 && int(seq) == 2 * a.dbg_drop_tile) continue;       // a test's lost arrival
                         if (ptx::elect_one()) {
                             const uint32_t full = kv_full + 8 * st, at = ring + st * C::Slot;
-                            if (kv == 0) {
-                                uint32_t bits = 0;
-#pragma unroll
-                                for (int j = 0; j < C::Pages; ++j) bits |= uint32_t(pg[j] >= 0) << j;
-                                there[(seq / 2) % C::Flags] = bits;
-                            }
+                            if (kv == 0) there[(seq / 2) % C::Flags] = pg >= 0;
                             ptx::mbar_arrive_expect_tx(full, C::Slot);
+                            const int row = pg >= 0 ? pg * kGqaTile : int(p.pool_rows);
+                            if (kv == 0 || pg < 0 || (e0 + NE <= w.span.hi && (e0 >= w.span.lo || e0 + NE <= w.span.first))) {
 #pragma unroll
-                            for (int j = 0; j < C::Pages; ++j) {
-                                const int row = pg[j] >= 0 ? pg[j] * kGqaTile : int(p.pool_rows), e = e0 + j * kGqaTile;
-                                const bool whole = pg[j] < 0 || (e + kGqaTile <= w.span.hi && (e >= w.span.lo || e + kGqaTile <= w.span.first));
-                                if (kv == 0 || whole) {
-#pragma unroll
-                                    for (int x = 0; x < D / 64; ++x)
-                                        ptx::tma_load_3d(at + x * (NE * 128) + j * (kGqaTile * 128), kv ? &a.v_map : &a.k_map, 64 * x, w.h, row, full);
-                                } else {
-                                    auto seen = [&](int i) { return i < w.span.hi && (i >= w.span.lo || i < w.span.first); };
-                                    for (int r8 = 0; r8 < kGqaTile; r8 += 8) {
-                                        uint32_t bits = 0;
-                                        for (int r = 0; r < 8; ++r) bits |= uint32_t(seen(e + r8 + r)) << r;
-                                        for (int x = 0; x < D / 64; ++x) {
-                                            const uint32_t to = at + x * (NE * 128) + (j * kGqaTile + r8) * 128;
-                                            if (bits == 0u || bits == 255u) {
-                                                ptx::tma_load_3d(to, &p.v8_map, 64 * x, w.h, bits ? row + r8 : int(p.pool_rows), full);
-                                            } else {
-                                                for (int r = 0; r < 8; ++r)
-                                                    ptx::tma_load_3d(to + r * 128, &p.v1_map, 64 * x, w.h, (bits >> r) & 1u ? row + r8 + r : int(p.pool_rows), full);
-                                            }
+                                for (int x = 0; x < D / 64; ++x) ptx::tma_load_3d(at + x * (NE * 128), kv ? &a.v_map : &a.k_map, 64 * x, w.h, row, full);
+                            } else {
+                                auto seen = [&](int i) { return i < w.span.hi && (i >= w.span.lo || i < w.span.first); };
+                                for (int r8 = 0; r8 < NE; r8 += 8) {
+                                    uint32_t bits = 0;
+                                    for (int r = 0; r < 8; ++r) bits |= uint32_t(seen(e0 + r8 + r)) << r;
+                                    for (int x = 0; x < D / 64; ++x) {
+                                        const uint32_t to = at + x * (NE * 128) + r8 * 128;
+                                        if (bits == 0u || bits == 255u) {
+                                            ptx::tma_load_3d(to, &p.v8_map, 64 * x, w.h, bits ? row + r8 : int(p.pool_rows), full);
+                                        } else {
+                                            for (int r = 0; r < 8; ++r)
+                                                ptx::tma_load_3d(to + r * 128, &p.v1_map, 64 * x, w.h, (bits >> r) & 1u ? row + r8 + r : int(p.pool_rows), full);
                                         }
                                     }
                                 }
@@ -297,115 +288,63 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
             }
         }
     } else if (warp == C::SoftmaxWarps + 1) {
-        // ── products ──
-        constexpr uint32_t kIdescS = C::BF16 ? ptx::make_idesc_bf16(128, NE, false, false) : ptx::make_idesc_f16(128, NE, false, false);
-        constexpr uint32_t kIdescO = C::BF16 ? ptx::make_idesc_bf16(128, D, false, true) : ptx::make_idesc_f16(128, D, false, true);
-        // S of tile t from K in slot st, into S buffer i
-        auto scores = [&](int t, int i, uint32_t st) {
-            if (ptx::elect_one()) {
+        // ── outputs ──
+        // (this warp for these products, one for each tile's scores: while one looks at its barriers, 130 to 210 cycles a look, the tensor cores have the others' products)
+        constexpr uint32_t kIdesc = C::BF16 ? ptx::make_idesc_bf16(128, D, false, true) : ptx::make_idesc_f16(128, D, false, true), kDescHi = ptx::smem_desc_hi(1024);
+        const uint32_t ring_lo = ptx::smem_desc_lo(ring, NE * 128);
+        uint32_t at = 0;                                                      // steps of all units so far
+        for (; w.more() && ok; w.next(p, NE)) {
+            for (int j = 0; j < w.span.count && ok; ++j, ++at) {
+                const uint32_t st = (2 * at + 1) % C::Slots, v_lo = ring_lo + st * (C::Slot >> 4);
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint64_t ad = ptx::make_smem_desc(smem + t * C::QTile + (k / 4) * (128 * 128) + (k % 4) * 32, 16, 1024);
-                    const uint64_t bd = ptx::make_smem_desc(ring + st * C::Slot + (k / 4) * (NE * 128) + (k % 4) * 32, 16, 1024);
-                    mma_ss(tmem + i * NE, ad, bd, kIdescS, k ? 1u : 0u);
-                }
-                ptx::mma_commit(s_full + 8 * i);
-            }
-            __syncwarp();
-        };
-        auto outputs = [&](int t, int i, uint32_t st, bool add) {
-            if (ptx::elect_one()) {
-#pragma unroll
-                for (int k = 0; k < NE / 16; ++k) {
-                    const uint64_t bd = ptx::make_smem_desc(ring + st * C::Slot + k * 2048, NE * 128, 1024);
-                    mma_ts(tmem + C::ColO + t * D, tmem + i * NE + k * 8, bd, kIdescO, add || k ? 1u : 0u);
-                }
-            }
-            __syncwarp();
-        };
-        auto commit = [&](uint32_t bar) {
-            if (ptx::elect_one()) ptx::mma_commit(bar);
-            __syncwarp();
-        };
-        uint32_t step = 0, unit = 0;                                          // steps of all units so far
-        auto wait_kv = [&](uint32_t s) {
-            wait(kv_full + 8 * (s % C::Slots), s / C::Slots, 1, int(s));
-            ptx::tc_fence_after_sync();
-        };
-        if constexpr (NT == 2) {
-            // the first scores of a unit go out behind the last products of the one before
-            if (w.more()) {
-                wait_kv(0);
-                for (int t = 0; t < 2 && ok; ++t) {
-                    wait(q_full + 8 * t, 0, 1, 0);
-                    ptx::tc_fence_after_sync();
+                for (int t = 0; t < NT; ++t) {
+                    const uint32_t bar = p_full + 8 * (2 * t + (at & 1));
+                    if (t == 0) wait2(kv_full + 8 * st, (2 * at + 1) / C::Slots, bar, at >> 1, 1, int(at));
+                    else wait(bar, at >> 1, 1, int(at));
                     if (!ok) break;
-                    scores(t, t, 0);
-                    if (w.span.count == 1) commit(q_empty + 8 * t);
-                }
-                if (ok) commit(kv_empty);
-            }
-            while (w.more() && ok) {
-                const int n = w.span.count;
-                PrefillWalk ahead = w;
-                ahead.next(p, NE);
-                for (int j = 0; j < n && ok; ++j, ++step) {
-                    const uint32_t ks = 2 * (step + 1), vs = 2 * step + 1;
-                    const bool last = j + 1 == n, on = !last || ahead.more();
-                    for (int t = 0; t < 2 && ok; ++t) {
-                        wait(p_full + 8 * t, step, 1, int(step));
-                        if (t == 0) wait_kv(vs);
-                        ptx::tc_fence_after_sync();
-                        if (!ok) break;
-                        outputs(t, t, vs % C::Slots, j > 0);
-                        if (last) commit(o_full + 8 * t);
-                        if (t == 1) commit(kv_empty + 8 * (vs % C::Slots));
-                        if (on) {
-                            if (t == 0) wait_kv(ks);
-                            if (last) {
-                                wait(q_full + 8 * t, unit + 1, 1, int(unit));
-                                ptx::tc_fence_after_sync();
-                            }
-                            if (!ok) break;
-                            scores(t, t, ks % C::Slots);
-                            if (last ? ahead.span.count == 1 : j + 2 == n) commit(q_empty + 8 * t);
-                            if (t == 1) commit(kv_empty + 8 * (ks % C::Slots));
-                        }
+                    ptx::tc_fence_after_sync();
+                    const uint32_t p_at = tmem + (2 * t + (at & 1)) * NE;
+                    if (ptx::elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < NE / 16; ++k) mma_ts(tmem + C::ColO + t * D, p_at + k * 8, v_lo + (k * 2048 >> 4), kDescHi, kIdesc, j > 0 || k ? 1u : 0u);
+                        ptx::mma_commit(o_full + 8 * (2 * t + (at & 1)));
+                        if (t == NT - 1)
+                            for (int i = 0; i < NT; ++i) ptx::mma_commit(kv_empty + 8 * st);         // (as many arrivals as K's slots get)
                     }
+                    __syncwarp();
                 }
-                w = ahead;
-                ++unit;
-            }
-        } else {
-            for (; w.more() && ok; w.next(p, NE), ++unit) {
-                const int n = w.span.count;
-                wait(q_full, unit, 1, int(unit));
-                for (int j = -1; j < n && ok; ++j) {
-                    if (j + 1 < n) {
-                        const uint32_t at = step + uint32_t(j + 1);
-                        wait_kv(2 * at);
-                        if (!ok) break;
-                        scores(0, at & 1, (2 * at) % C::Slots);
-                        commit(kv_empty + 8 * ((2 * at) % C::Slots));
-                        if (j + 2 == n) commit(q_empty);
-                    }
-                    if (j >= 0) {
-                        const uint32_t at = step + uint32_t(j);
-                        wait(p_full + 8 * (at & 1), at >> 1, 1, int(at));
-                        wait_kv(2 * at + 1);
-                        if (!ok) break;
-                        outputs(0, at & 1, (2 * at + 1) % C::Slots, j > 0);
-                        commit(o_full);
-                        commit(kv_empty + 8 * ((2 * at + 1) % C::Slots));
-                    }
-                }
-                step += uint32_t(n);
             }
         }
-    }
+    } else if (warp >= C::SoftmaxWarps + 2) {
+        // ── scores of a tile ──
+        constexpr uint32_t kIdesc = C::BF16 ? ptx::make_idesc_bf16(128, NE, false, false) : ptx::make_idesc_f16(128, NE, false, false), kDescHi = ptx::smem_desc_hi(1024);
+        const int t = warp - C::SoftmaxWarps - 2;
+        const uint32_t q_lo = ptx::smem_desc_lo(smem + t * C::QTile, 16), ring_lo = ptx::smem_desc_lo(ring, 16);
+        uint32_t at = 0, unit = 0;
+        for (; w.more() && ok; w.next(p, NE), ++unit) {
+            wait(q_full + 8 * t, unit, 1, int(unit));
+            for (int j = 0; j < w.span.count; ++j, ++at) {
+                const uint32_t st = (2 * at) % C::Slots, buffer = 2 * t + (at & 1);
+                // K is there, and the buffer's P, of two steps ago, has been multiplied
+                if (at >= 2) wait2(kv_full + 8 * st, (2 * at) / C::Slots, o_full + 8 * buffer, (at - 2) >> 1, 1, int(at));
+                else wait(kv_full + 8 * st, (2 * at) / C::Slots, 1, int(at));
+                if (!ok) break;
+                ptx::tc_fence_after_sync();
+                const uint32_t k_lo = ring_lo + st * (C::Slot >> 4), s_at = tmem + buffer * NE;
+                const bool last = j + 1 == w.span.count;
+                if (ptx::elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k)
+                        mma_ss(s_at, q_lo + (((k / 4) * (128 * 128) + (k % 4) * 32) >> 4), k_lo + (((k / 4) * (NE * 128) + (k % 4) * 32) >> 4), kDescHi, kIdesc, k ? 1u : 0u);
+                    ptx::mma_commit(s_full + 8 * buffer);
+                    if (last) ptx::mma_commit(q_empty + 8 * t);
+                    ptx::mma_commit(kv_empty + 8 * st);
+                }
+                __syncwarp();
+            }
+        }
     } else {
         // ── softmax: a thread has a row ──
-        if constexpr (NT == 2) regs_inc<C::RegsSoftmax>();
         const int t = warp >> 2;
         const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
         const int r = (warp & 3) * 32 + lane, tok = r / a.G, gg = r - tok * a.G;
@@ -413,21 +352,22 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
         const bool real = r < p.tile_tokens * a.G;                            // (rows behind hold what the memory held)
         const float neg = -INFINITY;
         uint32_t step = 0, unit = 0;
+        bool ahead = false;                                                   // the next step's scores are known to be there
         for (; w.more() && ok; w.next(p, NE), ++unit) {
             const int token = w.span.t0 + t * p.tile_tokens + tok, place = w.req.place0 + token;
             const int first_place = w.req.place0 + w.span.t0 + t * p.tile_tokens, last_place = first_place + p.tile_tokens - 1;
             const float scale = a.scale_log2 * (a.k_scale != nullptr ? ptx::ld(a.k_scale + w.h) : 1.f);
             float ref = neg, l = 0.f;
             for (int j = 0; j < w.span.count; ++j, ++step) {
-                const int i = NT == 2 ? t : int(step & 1);
+                const int i = 2 * t + int(step & 1);
                 const uint32_t s_at = lane_base + i * NE;
                 const int e0 = w.span.slot(j) * NE;
                 // (the producer's flags: K has arrived when its scores have)
-                wait(s_full + 8 * i, NT == 2 ? step : step >> 1, 2, int(step));
+                if (!ahead) wait(s_full + 8 * i, step >> 1, 2, int(step));
                 if (!ok) break;
                 ptx::tc_fence_after_sync();
-                const uint32_t pages = there[step % C::Flags];
-                const bool whole = pages == (1u << C::Pages) - 1u && e0 + NE - 1 <= first_place && e0 + NE <= w.req.entries &&
+                const bool page = there[step % C::Flags] != 0;
+                const bool whole = page && e0 + NE - 1 <= first_place && e0 + NE <= w.req.entries &&
                                    (a.window == 0 || e0 > last_place - a.window || e0 + NE - 1 < a.first);
                 // A row whose maximum has passed its reference by too much, or that sees its first entry, takes the maximum as its reference; O so far is rescaled.
                 auto refer = [&](float top) {
@@ -440,10 +380,8 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
                         l *= by;
                     }
                     if (j == 0) return;
-                    if constexpr (NT == 1) {
-                        wait(o_full, step - 1, 2, int(step));
-                        ptx::tc_fence_after_sync();
-                    }
+                    wait(o_full + 8 * (2 * t + int((step - 1) & 1)), (step - 1) >> 1, 2, int(step));
+                    ptx::tc_fence_after_sync();
                     const uint32_t o_at = lane_base + C::ColO + t * D;
 #pragma unroll 1
                     for (int c = 0; c < D / 16; ++c) {
@@ -463,15 +401,14 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
 #pragma unroll
                     for (int c = 0; c < NE / 32; ++c) ptx::tmem_ld32(s_at + 32 * c, v[c]);
                     ptx::tmem_wait_ld();
-                    float t0 = neg, t1 = neg;
+                    float top[4] = {neg, neg, neg, neg};
 #pragma unroll
                     for (int c = 0; c < NE / 32; ++c)
 #pragma unroll
-                        for (int x = 0; x < 32; x += 4) {
-                            t0 = ptx::max3(t0, __uint_as_float(v[c][x]), __uint_as_float(v[c][x + 1]));
-                            t1 = ptx::max3(t1, __uint_as_float(v[c][x + 2]), __uint_as_float(v[c][x + 3]));
-                        }
-                    refer(fmaxf(t0, t1));
+                        for (int x = 0; x < 32; x += 8)
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) top[q] = ptx::max3(top[q], __uint_as_float(v[c][x + 2 * q]), __uint_as_float(v[c][x + 2 * q + 1]));
+                    refer(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
                     const float sub = ref == neg ? 0.f : -ref * scale;
                     // (where scores are so large that the rounding of this product would tell, the other way)
                     done = !__any_sync(0xFFFFFFFFu, fabsf(sub) >= 16777216.f);
@@ -506,7 +443,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
                         auto below = [](int n) { return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u; };
                         uint32_t see = below(min(place + 1, w.req.entries) - at);
                         if (a.window > 0) see &= ~below(place - a.window + 1 - at) | below(a.first - at);
-                        if (!((pages >> (32 * c / kGqaTile)) & 1u)) see = 0u;
+                        if (!page) see = 0u;
                         ptx::tmem_wait_ld();
 #pragma unroll
                         for (int x = 0; x < 32; ++x)
@@ -539,16 +476,17 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
                         tmem_st16(s_at + 16 * c, pk);
                     }
                 }
-                // (every turn of this barrier is waited for, so that the wait for the last cannot take an earlier one for it)
-                if (NT == 1 && j > 0) wait(o_full, step - 1, 2, int(step));
+                // a look at the next step's scores, whose answer comes while P is on its way
+                ahead = ptx::mbar_try_wait(s_full + 8 * (2 * t + int((step + 1) & 1)), ((step + 1) >> 1) & 1u);
                 ptx::tmem_wait_st();
                 ptx::tc_fence_before_sync();
-                __syncwarp();
+                ahead = __all_sync(0xFFFFFFFFu, ahead);
                 if (lane == 0) ptx::mbar_arrive(p_full + 8 * i);
             }
             if (!ok) break;
             // ── the row's output ──
-            wait(o_full + 8 * t, NT == 2 ? unit : step - 1, 3, int(unit));
+            // (scores of the last step came after the outputs of two steps before, so that the wait cannot take an earlier turn of the barrier for this one)
+            wait(o_full + 8 * (2 * t + int((step - 1) & 1)), (step - 1) >> 1, 3, int(unit));
             if (!ok) break;
             ptx::tc_fence_after_sync();
             const bool mine = real && token <= w.span.t1;
@@ -590,7 +528,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
         const uint32_t t0 = ptx::globaltimer_lo();                            // copies and products that are on their way end within microseconds
         while (ptx::globaltimer_lo() - t0 < 1000000u) __nanosleep(1000);
     }
-    if (warp == C::SoftmaxWarps + 1) {
+    if (warp == C::SoftmaxWarps) {
         ptx::tc_fence_after_sync();
         ptx::tmem_dealloc(tmem, 512);
     }
