@@ -240,6 +240,7 @@ static int gqa_fwd(const Dsv4GqaParams* p, void* stream_) {
     a.scale_log2 = p->sm_scale * 1.4426950408889634f;
     a.out = p->out;  a.lse = p->lse;
     a.blocks = s.blocks;  a.group_rows = s.group_rows;  a.min_share = kMinShare;
+    a.one_group = p->q_start == nullptr && int64_t(p->T) * p->G <= s.group_rows;
     uint8_t* ws = static_cast<uint8_t*>(p->workspace);
     a.part_o = reinterpret_cast<float*>(ws);  ws += up(s.parts * p->D * 4);
     a.part_lse = reinterpret_cast<float*>(ws);  ws += up(s.parts * 4);
@@ -284,7 +285,7 @@ extern "C" int dsv4_gqa_prefill_fwd(const Dsv4GqaParams* p, void* stream) {
 
 extern "C" int dsv4_gqa_insert(const Dsv4GqaInsertParams* p, void* stream) {
     if (p == nullptr || p->B <= 0 || p->T < 0 || p->rows < 0 || p->Hkv <= 0 || p->max_pages <= 0 || p->num_pages <= 0) return int(cudaErrorInvalidValue);
-    if (p->D <= 0 || p->D % 8 != 0 || int64_t(p->Hkv) * p->D > (1 << 24) || p->num_pages > 0x7FFFFFFF) return int(cudaErrorInvalidValue);
+    if (p->D <= 0 || p->D % 8 != 0 || int64_t(p->Hkv) * p->D > (1 << 24) || p->num_pages > 0x7FFFFFFF / kGqaTile) return int(cudaErrorInvalidValue);
     const bool e4m3 = p->kv_dtype == DSV4_DTYPE_E4M3;
     if ((p->src_dtype != DSV4_DTYPE_BF16 && p->src_dtype != DSV4_DTYPE_F16) || (!e4m3 && p->kv_dtype != p->src_dtype)) return int(cudaErrorInvalidValue);
     if (!p->k || !p->v || !p->k_pool || !p->v_pool || !p->block_table || !p->insert_pos || (e4m3 && (!p->k_scale || !p->v_scale))) return int(cudaErrorInvalidValue);
@@ -303,10 +304,13 @@ extern "C" int dsv4_gqa_insert(const Dsv4GqaInsertParams* p, void* stream) {
     a.scale[0] = p->k_scale;  a.scale[1] = p->v_scale;
     a.pool[0] = p->k_pool;  a.pool[1] = p->v_pool;
     a.status = p->status;
-    constexpr int kWarps = kGqaInsertThreads / 32;
-    const int64_t blocks = (2 * p->rows + kWarps - 1) / kWarps, most = int64_t(device_sms()) * 8;
-    return int(launch(e4m3 ? gqa_insert_kernel<true> : gqa_insert_kernel<false>, dim3(unsigned(blocks < most ? blocks : most)), kGqaInsertThreads, 0,
-                      static_cast<cudaStream_t>(stream), a));
+    // as many tokens a block (2 to 32) as leave four blocks for every SM
+    int block_tokens = kGqaInsertTokens;
+    while (block_tokens > 2 && p->rows < int64_t(block_tokens) * device_sms() * 4) block_tokens /= 2;
+    a.block_tokens = block_tokens;
+    const int64_t blocks = (p->rows + block_tokens - 1) / block_tokens;
+    if (blocks > 0x7FFFFFFF || int64_t(block_tokens) * p->Hkv * p->D > 0x7FFFFFFF) return int(cudaErrorInvalidValue);
+    return int(launch(e4m3 ? gqa_insert_kernel<true> : gqa_insert_kernel<false>, dim3(unsigned(blocks)), kGqaInsertThreads, 0, static_cast<cudaStream_t>(stream), a));
 }
 
 extern "C" int dsv4_kv_evict(const Dsv4KvEvictParams* p, void* stream_) {

@@ -54,6 +54,7 @@ struct GqaArgs {
     float* part_lse;                 // [2 * blocks][R], log2
     int blocks;                      // of the attention kernel
     int group_rows;                  // R
+    int one_group;                   // not packed, and a request's rows of a KV head fit a group
     int min_share;                   // tiles of a block, at least
     // weights of the entries
     float* logits;                   // [B][Hkv * T * G][logit_stride], log2 units; null: not wanted
@@ -101,18 +102,24 @@ struct GqaSpan {
     int head, skip, count;           // tiles: `head` from 0 on, the others `skip` pages further on; count >= 1 (a group that sees nothing has an empty one)
     __device__ __forceinline__ int slot(int k) const { return k < head ? k : k + skip; }
 };
+// (Rows and tokens of a request are below 2^29: 32-bit divisions, which take a twentieth of the time of 64-bit ones.  With those, and one more for every group, a call for one
+// request took 18 us instead of 10.)
 __device__ __forceinline__ GqaSpan gqa_span(const GqaArgs& a, const GqaRequest& r, int rg) {
     GqaSpan s;
-    const int64_t row = int64_t(rg) * a.group_rows, rows = int64_t(r.tokens) * a.G;
-    s.t0 = int(row / a.G);
-    s.t1 = int((min(row + a.group_rows, rows) - 1) / a.G);
+    if (a.one_group) {
+        s.t0 = 0;
+        s.t1 = r.tokens - 1;
+    } else {
+        const uint32_t row = uint32_t(rg) * uint32_t(a.group_rows), rows = uint32_t(r.tokens) * uint32_t(a.G);
+        s.t0 = int(row / uint32_t(a.G));
+        s.t1 = int((min(row + uint32_t(a.group_rows), rows) - 1) / uint32_t(a.G));
+    }
     s.hi = max(min(r.place0 + s.t1 + 1, r.entries), 0);
     s.lo = 0;
     s.first = 0;
     if (a.window > 0) {
-        s.lo = max(r.place0 + s.t0 - a.window + 1, 0);
+        s.lo = min(max(r.place0 + s.t0 - a.window + 1, 0), s.hi);
         s.first = min(a.first, s.hi);
-        if (s.lo > s.hi) s.lo = s.hi;
     }
     const int end = (s.hi + kGqaTile - 1) / kGqaTile, heads = (s.first + kGqaTile - 1) / kGqaTile, from = s.lo / kGqaTile;
     s.head = min(heads, from);
@@ -120,12 +127,21 @@ __device__ __forceinline__ GqaSpan gqa_span(const GqaArgs& a, const GqaRequest& 
     s.count = max(end - s.skip, 1);
     return s;
 }
-__device__ __forceinline__ int gqa_groups(const GqaArgs& a, const GqaRequest& r) { return int((int64_t(r.tokens) * a.G + a.group_rows - 1) / a.group_rows); }
+__device__ __forceinline__ int gqa_groups(const GqaArgs& a, const GqaRequest& r) {
+    if (a.one_group) return 1;
+    return int((uint32_t(r.tokens) * uint32_t(a.G) + uint32_t(a.group_rows) - 1) / uint32_t(a.group_rows));
+}
 // Tiles of one KV head of a request.
 __device__ __forceinline__ int64_t gqa_head_tiles(const GqaArgs& a, const GqaRequest& r) {
+    if (a.one_group) return gqa_span(a, r, 0).count;
     int64_t n = 0;
     for (int rg = 0, groups = gqa_groups(a, r); rg < groups; ++rg) n += gqa_span(a, r, rg).count;
     return n;
+}
+// a / b, neither negative: in 32 bits where they fit
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    if (((a | b) >> 32) == 0) return uint32_t(a) / uint32_t(b);
+    return a / b;
 }
 
 // Sum of one value per thread over the threads before this one, and over all.
@@ -151,7 +167,7 @@ __device__ __forceinline__ int64_t block_prefix(int64_t v, int64_t& total, int64
 }
 
 // The length of a share, which the attention kernel and the merge work out alike.
-__device__ __forceinline__ int64_t gqa_share(const GqaArgs& a, int64_t total) { return max((total + a.blocks - 1) / a.blocks, int64_t(a.min_share)); }
+__device__ __forceinline__ int64_t gqa_share(const GqaArgs& a, int64_t total) { return max(quotient(total + a.blocks - 1, a.blocks), int64_t(a.min_share)); }
 
 __device__ __forceinline__ void gqa_report(int32_t* status, int code, int role, int what) {
     if (status != nullptr && atomicCAS(status, 0, code) == 0) {
@@ -224,7 +240,7 @@ struct GqaWalk {
         if (left <= 0) return;
         req = gqa_request(a, b);
         const int64_t per_head = gqa_head_tiles(a, req);
-        h = int(off / per_head);
+        h = int(quotient(off, per_head));
         off -= h * per_head;
         span = gqa_span(a, req, rg = 0);
         for (const int groups = gqa_groups(a, req); off >= span.count && rg + 1 < groups;) {
@@ -391,7 +407,7 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
     bool failed = false;
 
     for (; w.left > 0; w.next(a)) {
-        const int64_t rows = int64_t(w.req.tokens) * a.G, row_first = int64_t(w.rg) * R;
+        const int rows = w.req.tokens * a.G, row_first = w.rg * R;
         // Q of the group: rows of zeros behind the last one
         ptx::bar_sync(1, kGqaConsumers);
         {
@@ -402,7 +418,7 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
             for (int r = tid / kLanes; r < R; r += kGqaConsumers / kLanes) {
                 uint4 v = make_uint4(0, 0, 0, 0);
                 if (row_first + r < rows) {
-                    const int t = int((row_first + r) / a.G), gg = int(row_first + r - int64_t(t) * a.G);
+                    const int t = int(uint32_t(row_first + r) / uint32_t(a.G)), gg = row_first + r - t * a.G;
                     const int64_t at = (a.q_start != nullptr ? (w.req.row0 + t) * a.q_stride_t : int64_t(w.b) * a.q_stride_b + t * a.q_stride_t) +
                                        int64_t(w.h * a.G + gg) * a.q_stride_h + 8 * l;
                     v = *reinterpret_cast<const uint4*>(q0 + at * 2);
@@ -460,7 +476,7 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
                 const int r = (wm * MW + mt) * 16 + g + 8 * hh;
-                place[mt][hh] = row_first + r < rows ? w.req.place0 + int((row_first + r) / a.G) : -1;
+                place[mt][hh] = row_first + r < rows ? w.req.place0 + int(uint32_t(row_first + r) / uint32_t(a.G)) : -1;
                 scale[mt][hh] = kE4m3 ? head_scale * row_factor[r] : head_scale;
             }
         float m[MW][2], l[MW][2], o[MW][D / 8][4];
@@ -560,7 +576,7 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
                     for (int mt = 0; mt < MW; ++mt)
 #pragma unroll
                         for (int hh = 0; hh < 2; ++hh) {
-                            const int64_t r = row_first + (wm * MW + mt) * 16 + g + 8 * hh;
+                            const int r = row_first + (wm * MW + mt) * 16 + g + 8 * hh;
                             if (r < rows) {
                                 float* const to = a.logits + ((int64_t(w.b) * a.Hkv + w.h) * rows + r) * a.logit_stride + p0;
 #pragma unroll
@@ -714,8 +730,9 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
 #pragma unroll 2
             for (int rr = tid / kLanes; rr < 16 * C::WM; rr += kGqaConsumers / kLanes) {
                 const int of_wm = rr >> 4, rl = rr & 15, r = (of_wm * MW + mt) * 16 + rl;
-                const int64_t row = row_first + r;
+                const int row = row_first + r;
                 if (row >= rows) continue;
+                const int token = int(uint32_t(row) / uint32_t(a.G));
                 const float top = row_max(of_wm, rl);
                 float sum = 0.f;
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -733,7 +750,7 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
                     if (x == 0) a.part_lse[part * R + r] = top + log2f(sum);
                     continue;
                 }
-                gqa_write_row<D>(a, w.req.row0 + row / a.G, w.h * a.G + int(row % a.G), (int64_t(w.b) * a.Hkv + w.h) * rows + row, x, v, top, sum, v_scale);
+                gqa_write_row<D>(a, w.req.row0 + token, w.h * a.G + row - token * a.G, (int64_t(w.b) * a.Hkv + w.h) * rows + row, x, v, top, sum, v_scale);
             }
             ptx::bar_sync(1, kGqaConsumers);
         }
@@ -745,42 +762,67 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
 constexpr int kGqaMergeRows = kGqaMergeThreads / 32;
 template <int D>
 __global__ void __launch_bounds__(kGqaMergeThreads) gqa_merge_kernel(const __grid_constant__ GqaArgs a) {
-    __shared__ int64_t sums[kGqaMergeRows];
-    __shared__ int64_t unit_before[kGqaMergeRows];                            // tiles of the requests before the row's
-    __shared__ int32_t row_request[kGqaMergeRows];
+    constexpr int kWarps = kGqaMergeThreads / 32;
+    __shared__ int64_t sums[2][kWarps];
+    __shared__ int request;
     ptx::pdl_trigger();
     ptx::pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, H = a.Hkv * a.G;
-    const int64_t row0 = int64_t(blockIdx.x) * kGqaMergeRows;
-    if (tid < kGqaMergeRows) row_request[tid] = -1;
-    const int each = (a.B + kGqaMergeThreads - 1) / kGqaMergeThreads, b_from = tid * each, b_to = min(b_from + each, a.B);
-    int64_t mine = 0, total;
-    for (int b = b_from; b < b_to; ++b) mine += gqa_head_tiles(a, gqa_request(a, b)) * a.Hkv;
-    int64_t before = block_prefix<kGqaMergeThreads>(mine, total, sums);
-    for (int b = b_from; b < b_to; ++b) {
-        const GqaRequest r = gqa_request(a, b);
-#pragma unroll
-        for (int i = 0; i < kGqaMergeRows; ++i) {
-            const int64_t token = (row0 + i) / H;
-            if (token >= r.row0 && token < r.row0 + r.tokens) {
-                row_request[i] = b;
-                unit_before[i] = before;
-            }
+    const int64_t row0 = int64_t(blockIdx.x) * kGqaMergeRows, token0 = quotient(row0, H);
+    // the request of the block's first row
+    int first_b = a.B;
+    if (a.q_start == nullptr) {
+        first_b = int(quotient(token0, a.T));
+    } else {
+        if (tid == 0) request = a.B;
+        __syncthreads();
+        for (int b = tid; b < a.B; b += kGqaMergeThreads) {
+            const GqaRequest r = gqa_request(a, b);
+            if (token0 < r.row0 + r.tokens && r.tokens > 0) atomicMin(&request, b);     // (or the first behind it, where the row is no request's)
         }
-        before += gqa_head_tiles(a, r) * a.Hkv;
+        __syncthreads();
+        first_b = request;
+    }
+    // tiles of all requests, and of those before it
+    int64_t total = 0, ahead = 0;
+    for (int b = tid; b < a.B; b += kGqaMergeThreads) {
+        const int64_t n = gqa_head_tiles(a, gqa_request(a, b)) * a.Hkv;
+        total += n;
+        if (b < first_b) ahead += n;
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+        total += __shfl_xor_sync(0xFFFFFFFFu, total, d);
+        ahead += __shfl_xor_sync(0xFFFFFFFFu, ahead, d);
+    }
+    if (lane == 0) {
+        sums[0][warp] = total;
+        sums[1][warp] = ahead;
     }
     __syncthreads();
-    const int b = row_request[warp];
-    if (b < 0) return;
-    const GqaRequest req = gqa_request(a, b);
-    const int64_t row = row0 + warp, token = row / H, rows = int64_t(req.tokens) * a.G;
-    const int head = int(row - token * H), h = head / a.G;
-    const int64_t at = (token - req.row0) * a.G + head - h * a.G;              // row of the KV head
-    const int rg = int(at / a.group_rows), r = int(at - int64_t(rg) * a.group_rows);
-    int64_t unit = unit_before[warp] + h * gqa_head_tiles(a, req);
+    total = ahead = 0;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+        total += sums[0][i];
+        ahead += sums[1][i];
+    }
+    // this warp's row
+    const int64_t row = row0 + warp, token = token0 + int(uint32_t(row - token0 * H) / uint32_t(H));
+    GqaRequest req{};
+    int b = first_b;
+    for (; b < a.B; ++b) {
+        req = gqa_request(a, b);
+        if (token < req.row0 + req.tokens && req.tokens > 0) break;
+        ahead += gqa_head_tiles(a, req) * a.Hkv;
+    }
+    if (b >= a.B || token < req.row0) return;
+    const int rows = req.tokens * a.G, head = int(row - token * H), h = int(uint32_t(head) / uint32_t(a.G));
+    const int at = int(token - req.row0) * a.G + head - h * a.G;               // row of the KV head
+    const int rg = a.one_group ? 0 : int(uint32_t(at) / uint32_t(a.group_rows)), r = at - rg * a.group_rows;
+    int64_t unit = ahead + h * gqa_head_tiles(a, req);
     for (int i = 0; i < rg; ++i) unit += gqa_span(a, req, i).count;
     const int64_t share = gqa_share(a, total);
-    const int c0 = int(unit / share), c1 = int((unit + gqa_span(a, req, rg).count - 1) / share);
+    const int c0 = int(quotient(unit, share)), c1 = int(quotient(unit + gqa_span(a, req, rg).count - 1, share));
     if (c0 == c1) return;
     const int64_t first = 2 * int64_t(c0) + (unit != c0 * share);              // (every later block begins with its part)
     auto part = [&](int i) { return (i == 0 ? first : 2 * int64_t(c0 + i)) * a.group_rows + r; };
@@ -852,6 +894,7 @@ __global__ void __launch_bounds__(kGqaWeightThreads) gqa_weights_kernel(const __
 // ── new rows into the pages ──
 struct GqaInsertArgs {
     int B, T, Hkv, D, max_pages;
+    int block_tokens;                // of a block, at most kGqaInsertTokens
     int64_t rows;                    // tokens of all requests
     const int32_t* q_start;          // [B + 1], or null: T tokens each
     const int32_t* n_rows;           // [B], or null: all T
@@ -873,80 +916,93 @@ __device__ __forceinline__ uint32_t quant_pair(float lo, float hi) {
     return r;
 }
 
-// A warp takes a token's K or V: 16 bytes a lane and load, up to four of them on the way.  Bound by the chain of its loads (offset, position, page) when small and by
-// memory when large.
+// A block takes some consecutive tokens: a thread each finds out where they go (offset, position, page: one chain of loads for the block), then all threads copy, 16 bytes a thread
+// and load, four on the way.  Bound by that chain when small and by memory when large.
+constexpr int kGqaInsertTokens = 32;
 template <bool E4M3>
 __global__ void __launch_bounds__(kGqaInsertThreads) gqa_insert_kernel(const __grid_constant__ GqaInsertArgs a) {
+    __shared__ int64_t src_row[kGqaInsertTokens];                             // first element of the token's row, of K and V: [token] of K, and by `b`, `t` again for V
+    __shared__ int64_t src_row_v[kGqaInsertTokens];
+    __shared__ int32_t entry[kGqaInsertTokens];                               // where it goes, -1: nowhere
     ptx::pdl_trigger();
     ptx::pdl_wait();
-    const int lane = threadIdx.x & 31;
-    const int64_t items = 2 * a.rows, step = int64_t(gridDim.x) * (kGqaInsertThreads / 32);
-    const int pieces = a.Hkv * a.D / 8, per_head = a.D / 8;
-    for (int64_t item = int64_t(blockIdx.x) * (kGqaInsertThreads / 32) + (threadIdx.x >> 5); item < items; item += step) {
-        const int kv = int(item & 1);
-        const int64_t token = item >> 1;
-        int b, t;
-        if (a.q_start == nullptr) {
-            b = int(token / a.T);
-            t = int(token - int64_t(b) * a.T);
-            if (a.n_rows != nullptr && t >= ptx::ld(a.n_rows + b)) continue;
-        } else {
-            // the request whose rows the token is among: 32 probes at a time
-            int lo = 0, n = a.B;                                              // q_start[lo] <= token (or lo = 0), token < q_start[lo + n] (or lo + n = B)
-            while (n > 1) {
-                const int each = (n + 31) / 32, at = min(lo + (lane + 1) * each, lo + n);
-                const uint32_t over = __ballot_sync(0xFFFFFFFFu, at >= lo + n || ptx::ld(a.q_start + at) > token);
-                const int skip = __ffs(over) - 1;
-                n = min(each, n - skip * each);
-                lo += skip * each;
+    const int tid = threadIdx.x, n = a.block_tokens;
+    const int64_t first = int64_t(blockIdx.x) * n;
+    if (tid < n) {
+        const int64_t token = first + tid;
+        int b = -1, t = 0, to = -1;
+        if (token < a.rows) {
+            if (a.q_start == nullptr) {
+                b = int(quotient(token, a.T));
+                t = int(token - int64_t(b) * a.T);
+                if (a.n_rows != nullptr && t >= ptx::ld(a.n_rows + b)) b = -1;
+            } else {
+                // the last request whose rows begin at or before the token
+                int lo = 0, hi = a.B;                                         // q_start[lo] <= token or lo = 0; q_start[hi] > token or hi = B
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (ptx::ld(a.q_start + mid) <= token) lo = mid;
+                    else hi = mid;
+                }
+                const int from = ptx::ld(a.q_start + lo), end = ptx::ld(a.q_start + lo + 1);
+                if (token >= from && token < end) {
+                    b = lo;
+                    t = int(token - from);
+                }
             }
-            b = lo;
-            const int from = ptx::ld(a.q_start + b), to = ptx::ld(a.q_start + b + 1);
-            if (token < from || token >= to) continue;                        // behind the last request
-            t = int(token - from);
         }
-        const int64_t pos = int64_t(ptx::ld(a.insert_pos + b)) + t, slot = pos / kGqaTile;
-        int page = -1;
-        if (pos >= 0 && slot < a.max_pages) page = ptx::ld(a.block_table + int64_t(b) * a.max_pages + slot);
-        if (page < 0 || page >= a.num_pages) {
-            if (lane == 0) gqa_report(a.status, 16, b, int(pos));
-            continue;
+        if (b >= 0) {
+            const int64_t pos = int64_t(ptx::ld(a.insert_pos + b)) + t, slot = pos >> 6;
+            int page = -1;
+            if (pos >= 0 && slot < a.max_pages) page = ptx::ld(a.block_table + int64_t(b) * a.max_pages + slot);
+            if (page >= 0 && page < a.num_pages) to = page * kGqaTile + int(pos & (kGqaTile - 1));
+            else gqa_report(a.status, 16, b, int(pos));
+            src_row[tid] = a.q_start == nullptr ? b * a.stride_b[0] + t * a.stride_t[0] : token * a.stride_t[0];
+            src_row_v[tid] = a.q_start == nullptr ? b * a.stride_b[1] + t * a.stride_t[1] : token * a.stride_t[1];
         }
-        const uint8_t* const src = static_cast<const uint8_t*>(a.src[kv]);
-        const int64_t row = (a.q_start == nullptr ? b * a.stride_b[kv] + t * a.stride_t[kv] : token * a.stride_t[kv]);
-        uint8_t* const dst = static_cast<uint8_t*>(a.pool[kv]) + (int64_t(page) * kGqaTile + pos % kGqaTile) * (int64_t(a.Hkv) * a.D * (E4M3 ? 1 : 2));
-        for (int at = lane; at < pieces; at += 128) {
-            uint4 v[4];
+        entry[tid] = to;
+    }
+    __syncthreads();
+    const uint32_t per_head = uint32_t(a.D) / 8, pieces = uint32_t(a.Hkv) * per_head, all = uint32_t(n) * 2 * pieces;   // pieces of 16 bytes of a row of K or V
+    for (uint32_t at = tid; at < all; at += 4 * kGqaInsertThreads) {
+        uint4 v[4];
+        uint8_t* to[4];
+        float scale[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (at + 32 * i < pieces) {
-                    const int h = (at + 32 * i) / per_head, x = (at + 32 * i) - h * per_head;
-                    v[i] = ptx::ldg_stream_v4(src + (row + h * a.stride_h[kv] + 8 * x) * 2);
-                }
+        for (int i = 0; i < 4; ++i) {
+            to[i] = nullptr;
+            const uint32_t piece = at + i * kGqaInsertThreads;
+            if (piece >= all) continue;
+            const uint32_t row = piece / pieces, x = piece - row * pieces, h = x / per_head, token = row >> 1, kv = row & 1;
+            const int e = entry[token];
+            if (e < 0) continue;
+            to[i] = static_cast<uint8_t*>(kv ? a.pool[1] : a.pool[0]) + (int64_t(e) * pieces + x) * (E4M3 ? 8 : 16);
+            if (E4M3) scale[i] = ptx::ld((kv ? a.scale[1] : a.scale[0]) + h);
+            v[i] = ptx::ldg_stream_v4(static_cast<const uint8_t*>(kv ? a.src[1] : a.src[0]) +
+                                      ((kv ? src_row_v[token] : src_row[token]) + int64_t(h) * (kv ? a.stride_h[1] : a.stride_h[0]) + 8 * (x - h * per_head)) * 2);
+        }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (at + 32 * i >= pieces) break;
-                if constexpr (E4M3) {
-                    const float scale = ptx::ld(a.scale[kv] + (at + 32 * i) / per_head);
-                    const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-                    uint32_t o[4];
+        for (int i = 0; i < 4; ++i) {
+            if (to[i] == nullptr) continue;
+            if constexpr (E4M3) {
+                const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+                uint32_t o[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        float lo, hi;
-                        if (a.src_bf16) {
-                            lo = __uint_as_float(u[j] << 16);
-                            hi = __uint_as_float(u[j] & 0xFFFF0000u);
-                        } else {
-                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[j]));
-                            lo = f.x;
-                            hi = f.y;
-                        }
-                        o[j] = quant_pair(__fdiv_rn(lo, scale), __fdiv_rn(hi, scale));
+                for (int j = 0; j < 4; ++j) {
+                    float lo, hi;
+                    if (a.src_bf16) {
+                        lo = __uint_as_float(u[j] << 16);
+                        hi = __uint_as_float(u[j] & 0xFFFF0000u);
+                    } else {
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[j]));
+                        lo = f.x;
+                        hi = f.y;
                     }
-                    *reinterpret_cast<uint2*>(dst + 8 * (at + 32 * i)) = make_uint2(o[0] | (o[1] << 16), o[2] | (o[3] << 16));
-                } else {
-                    *reinterpret_cast<uint4*>(dst + 16 * (at + 32 * i)) = v[i];
+                    o[j] = quant_pair(__fdiv_rn(lo, scale[i]), __fdiv_rn(hi, scale[i]));
                 }
+                *reinterpret_cast<uint2*>(to[i]) = make_uint2(o[0] | (o[1] << 16), o[2] | (o[3] << 16));
+            } else {
+                *reinterpret_cast<uint4*>(to[i]) = v[i];
             }
         }
     }
