@@ -79,9 +79,9 @@ cudaError_t run_decode(GqaArgs& a, cudaStream_t stream) {
 }
 template <int D, int KVT>
 cudaError_t run_decode(GqaArgs& a, cudaStream_t stream) {
-    if (a.group_rows == 16) return run_decode<GqaCfg<D, KVT, 1, 1>>(a, stream);
-    if (a.group_rows == 32) return run_decode<GqaCfg<D, KVT, 1, 2>>(a, stream);
-    return run_decode<GqaCfg<D, KVT, 1, 4>>(a, stream);
+    if (a.group_rows == 16) return run_decode<GqaCfg<D, KVT, 1>>(a, stream);
+    if (a.group_rows == 32) return run_decode<GqaCfg<D, KVT, 2>>(a, stream);
+    return run_decode<GqaCfg<D, KVT, 4>>(a, stream);
 }
 template <int D>
 cudaError_t run_decode(GqaArgs& a, int kv_dtype, cudaStream_t stream) {
@@ -115,7 +115,7 @@ bool gqa_sizes(const Dsv4GqaParams* p, Sizes& s) {
     if (p->window > 0 && longest > int64_t(p->window) + p->first + tokens + 2 * kGqaTile) longest = int64_t(p->window) + p->first + tokens + 2 * kGqaTile;
     const int64_t groups = p->q_start != nullptr ? (p->rows * p->G + s.group_rows - 1) / s.group_rows + p->B : int64_t(p->B) * ((tokens * p->G + s.group_rows - 1) / s.group_rows);
     const int64_t tiles = groups * p->Hkv * ((longest + kGqaTile - 1) / kGqaTile + 1);
-    const int64_t resident = int64_t(device_sms()) * (p->D > 128 ? 1 : 2), want = (tiles + kMinShare - 1) / kMinShare;
+    const int64_t resident = int64_t(device_sms()) * gqa_blocks_per_sm(p->D), want = (tiles + kMinShare - 1) / kMinShare;
     s.blocks = int(want < resident ? want : resident);
     s.parts = 2 * int64_t(s.blocks) * s.group_rows;
     s.logit_rows = p->weights != nullptr ? int64_t(p->B) * p->Hkv * p->T * p->G : 0;

@@ -32,6 +32,7 @@ constexpr int kGqaBf16 = 0, kGqaF16 = 1, kGqaE4m3 = 2;            // types of K 
 constexpr int kGqaTile = 64;                                      // entries of a tile: a page
 constexpr int kGqaConsumers = 128, kGqaThreads = kGqaConsumers + 32;
 constexpr int kGqaMergeThreads = 256, kGqaWeightThreads = 256;
+constexpr float kGqaLazy = 8.f;                                   // log2 of how far scores may pass a row's reference
 constexpr int kGqaStatusBadIndex = 7, kGqaStatusWait = 1;
 
 struct GqaArgs {
@@ -200,27 +201,35 @@ __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t w) {
     return r;
 }
 
-// D: head dimension; KVT: type of K and V; MW: tiles of 16 rows a warp; WM: warps side by side over the rows (4 / WM over the entries)
-template <int D_, int KVT_, int MW_, int WM_>
+__host__ __device__ constexpr int gqa_blocks_per_sm(int D) { return D > 128 ? 1 : 2; }
+
+// D: head dimension; KVT: type of K and V; WM: warps side by side over the rows, 16 each
+template <int D_, int KVT_, int WM_>
 struct GqaCfg {
-    static constexpr int D = D_, KVT = KVT_, MW = MW_, WM = WM_, WN = 4 / WM;
-    static constexpr int R = 16 * MW * WM;
+    static constexpr int D = D_, KVT = KVT_, WM = WM_, R = 16 * WM;
     static constexpr int ES = KVT == kGqaE4m3 ? 1 : 2;
     static constexpr int RowBytes = D * ES;
     static constexpr int Box = RowBytes < 128 ? RowBytes : 128;               // bytes of a row in one TMA box, and the width of the swizzle
     static constexpr int Boxes = RowBytes / Box;
     static constexpr int Slot = kGqaTile * RowBytes;
-    // Two blocks an SM with 64 KB each on the way cover 128 KB of it; a head of 256 leaves room for one block, with 128 KB.
-    static constexpr int Ring = D > 128 ? 128 * 1024 : 64 * 1024;
-    static constexpr int Slots = Ring / Slot;
-    static constexpr int BlocksPerSm = D > 128 ? 1 : 2;
+    // Some 130 KB of an SM are on the way: by two blocks with 64 KB each, or one with 128 KB for heads of 256.
+    static constexpr int BlocksPerSm = gqa_blocks_per_sm(D);
+    static constexpr int Ring = (BlocksPerSm == 1 ? 128 : 64) * 1024;
+    static constexpr int Slots = Ring / Slot, Pages = Slots / 2;
+    // Where rows are 16, the four warps share a page's entries, 16 each; where the ring holds four pages or more, two warps have every other page, 32 entries each: what a
+    // visit costs besides its products (barriers, masks, maxima: 260 instructions of 400) then counts for twice as many.
+    static constexpr int PG = WM == 1 && Pages % 4 == 0 ? 2 : 1;              // groups of warps that take turns with the pages
+    static constexpr int WN = 4 / (WM * PG);                                  // warps over a page's entries
+    static constexpr int Sub = WM == 1 && PG == 1 ? 1 : 2;                    // blocks of 16 entries that a warp takes at a time
+    static constexpr int Parts = 4 / WM;                                      // warps that have a part of a row
     static constexpr int QPitch = D * 2 + 16;                                 // bytes
     static constexpr int MergePitch = D + 8;                                  // floats
     static constexpr int Q = R * QPitch, Merge = 4 * 16 * MergePitch * 4;
     static constexpr int Shared = Q > Merge ? Q : Merge;                      // Q is done with when the warps' parts are joined
     static constexpr int OffShared = Ring, OffStats = OffShared + (Shared + 127) / 128 * 128;
-    static constexpr int OffBars = OffStats + (2 * 4 * 16 * MW + R) * 4;
+    static constexpr int OffBars = OffStats + (2 * 4 * 16 + R) * 4;
     static constexpr int OffValid = OffBars + 2 * Slots * 8, OffScan = OffValid + Slots * 4, Bytes = OffScan + 96 + 1024;
+    static_assert((Slots & (Slots - 1)) == 0 && Pages % PG == 0, "a slot's turns belong to one group");
 };
 
 // The sequence of pieces (parts of units) of a block, walked by each warp for itself.
@@ -293,9 +302,9 @@ __device__ __forceinline__ void gqa_write_row(const GqaArgs& a, int64_t token, i
 
 template <class C>
 __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel(const __grid_constant__ GqaArgs a) {
-    constexpr int D = C::D, MW = C::MW, WN = C::WN, R = C::R;
+    constexpr int D = C::D, WN = C::WN, R = C::R, Sub = C::Sub;
     constexpr bool kE4m3 = C::KVT == kGqaE4m3, kBf16 = C::KVT == kGqaBf16;
-    constexpr bool kQInRegs = MW == 1 && D <= 128;
+    constexpr bool kQInRegs = D <= 128;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t* const base = smem_raw + (smem - ptx::smem_u32(smem_raw));
@@ -307,7 +316,7 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
     if (tid == 0) {
         for (int i = 0; i < C::Slots; ++i) {
             ptx::mbar_init(bar_full + 8 * i, 1);
-            ptx::mbar_init(bar_empty + 8 * i, 4);
+            ptx::mbar_init(bar_empty + 8 * i, 4 / C::PG);
         }
         ptx::fence_mbar_init();
         ptx::prefetch_tensormap(&a.k_map);
@@ -394,20 +403,27 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
     }
 
     // ── attention ──
-    const int wm = warp / WN, wn = warp % WN, g = lane >> 2, c = lane & 3;
+    const int wm = warp % C::WM, wn = warp / C::WM % WN, turn = warp / (C::WM * WN), g = lane >> 2, c = lane & 3;
     const uint32_t q_sm = smem + C::OffShared;
     float* const merge = reinterpret_cast<float*>(base + C::OffShared);
-    float* const stat_m = reinterpret_cast<float*>(base + C::OffStats);       // [4][16 * MW]
-    float* const stat_l = stat_m + 4 * 16 * MW;
-    float* const row_factor = stat_l + 4 * 16 * MW;                           // [R]
+    float* const stat_m = reinterpret_cast<float*>(base + C::OffStats);       // [4][16]
+    float* const stat_l = stat_m + 4 * 16;
+    float* const row_factor = stat_l + 4 * 16;                                // [R]
     // entry of column n of a block of eight (e4m3 rows of 128 bytes and more: the eight lanes that load together then meet all banks)
     constexpr bool kPermuted = kE4m3 && C::RowBytes >= 128;
     auto entry_of = [](int n) { return kPermuted ? (n >> 1) + 4 * (n & 1) : n; };
-    uint32_t seq = 0;
+    uint32_t tiles_before = 0;
     bool failed = false;
+    auto wait_full = [&](uint32_t s) {
+        if (!failed && !ptx::mbar_wait_warp(bar_full + 8 * (s % C::Slots), (s / C::Slots) & 1u, a.wait_ns)) {
+            if (lane == 0) gqa_report(a.status, kGqaStatusWait, 1, int(s));
+            failed = true;                                                    // (the rest of the block's work is gone through without waiting)
+        }
+    };
 
     for (; w.left > 0; w.next(a)) {
         const int rows = w.req.tokens * a.G, row_first = w.rg * R;
+        ptx::bar_sync(1, kGqaConsumers);
         // Q of the group: rows of zeros behind the last one
         ptx::bar_sync(1, kGqaConsumers);
         {
@@ -454,8 +470,8 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
 
         uint32_t qf[kQInRegs ? D / 16 : 1][4];
         // A fragment of 16 dimensions; e4m3: of the dimensions that the lanes' 16-byte pieces of K hold (64 j + 16 c + 4 s + 0..3)
-        auto q_fragment = [&](uint32_t (&r)[4], int mt, int ks) {
-            const uint32_t row = q_sm + uint32_t((wm * MW + mt) * 16) * C::QPitch;
+        auto q_fragment = [&](uint32_t (&r)[4], int ks) {
+            const uint32_t row = q_sm + uint32_t(wm * 16) * C::QPitch;
             if (kE4m3) {
                 const uint32_t at = row + g * C::QPitch + (ks / 4) * 128 + c * 32 + (ks % 4) * 8;
                 const uint2 lo = ptx::lds_v2(at), hi = ptx::lds_v2(at + 8 * C::QPitch);
@@ -466,163 +482,154 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
         };
         if (kQInRegs) {
 #pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks) q_fragment(qf[kQInRegs ? ks : 0], 0, ks);
+            for (int ks = 0; ks < D / 16; ++ks) q_fragment(qf[kQInRegs ? ks : 0], ks);
         }
-        int place[MW][2];                                                     // of the rows' tokens; -1: no row
-        float scale[MW][2];
+        int place[2];                                                         // of the rows' tokens; -1: no row
+        float scale[2];
         const float head_scale = a.scale_log2 * (a.k_scale != nullptr ? ptx::ld(a.k_scale + w.h) : 1.f);
 #pragma unroll
-        for (int mt = 0; mt < MW; ++mt)
-#pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-                const int r = (wm * MW + mt) * 16 + g + 8 * hh;
-                place[mt][hh] = row_first + r < rows ? w.req.place0 + int(uint32_t(row_first + r) / uint32_t(a.G)) : -1;
-                scale[mt][hh] = kE4m3 ? head_scale * row_factor[r] : head_scale;
-            }
-        float m[MW][2], l[MW][2], o[MW][D / 8][4];
-#pragma unroll
-        for (int mt = 0; mt < MW; ++mt) {
-            m[mt][0] = m[mt][1] = -INFINITY;
-            l[mt][0] = l[mt][1] = 0.f;
-#pragma unroll
-            for (int j = 0; j < D / 8; ++j) o[mt][j][0] = o[mt][j][1] = o[mt][j][2] = o[mt][j][3] = 0.f;
+        for (int hh = 0; hh < 2; ++hh) {
+            const int r = wm * 16 + g + 8 * hh;
+            place[hh] = row_first + r < rows ? w.req.place0 + int(uint32_t(row_first + r) / uint32_t(a.G)) : -1;
+            scale[hh] = kE4m3 ? head_scale * row_factor[r] : head_scale;
         }
+        // m: reference of a row's weights, in log2 units: a maximum that the row's later ones have not passed by 2^8
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[D / 8][4];
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
         const int place_first = w.req.place0 + w.span.t0, place_last = w.req.place0 + w.span.t1;
 
-        for (int k = w.k0; k < w.k1; ++k, seq += 2) {
-            const uint32_t ks_ = seq % C::Slots, vs_ = (seq + 1) % C::Slots;
-            auto wait_full = [&](uint32_t s) {
-                if (!failed && !ptx::mbar_wait_warp(bar_full + 8 * (s % C::Slots), (s / C::Slots) & 1u, a.wait_ns)) {
-                    if (lane == 0) gqa_report(a.status, kGqaStatusWait, 1, int(s));
-                    failed = true;                                            // (the rest of the block's work is gone through without waiting)
-                }
-            };
+        // this group's pages
+        for (int k = w.k0 + (C::PG > 1 ? int((uint32_t(turn) - tiles_before) % C::PG) : 0); k < w.k1; k += C::PG) {
+            const uint32_t seq = 2 * (tiles_before + uint32_t(k - w.k0)), ks_ = seq % C::Slots, vs_ = (seq + 1) % C::Slots;
             wait_full(seq);
             const bool there = valid[ks_] != 0;
             const uint32_t k_sm = smem + ks_ * C::Slot, v_sm = smem + vs_ * C::Slot;
             const int e0 = w.span.slot(k) * kGqaTile;
+            // a page that all rows see
+            const bool page_whole = there && e0 + kGqaTile - 1 <= place_first && e0 + kGqaTile <= w.req.entries && (a.window == 0 || e0 > place_last - a.window || e0 + kGqaTile <= a.first);
             bool v_waited = false, k_given_back = false;
 #pragma unroll 1
-            for (int sl = wn; sl < 4; sl += WN) {
-                const int p0 = e0 + 16 * sl;                                  // entries p0 .. p0 + 15
+            for (int sl = wn * Sub; sl < 4; sl += WN * Sub) {
+                const int p0 = e0 + 16 * sl;                                  // entries p0 .. p0 + 16 Sub - 1
+                constexpr int kEntries = 16 * Sub;
                 // seen by all rows, or by none, or by some
-                const bool whole = there && p0 + 15 <= place_first && p0 + 15 < w.req.entries && (a.window == 0 || p0 > place_last - a.window || p0 + 15 < a.first);
-                const bool some = p0 < w.span.hi && (p0 + 15 >= w.span.lo || p0 < w.span.first);
-                if (!some) continue;
-                float s[MW][2][4];
+                bool whole = page_whole;
+                if (!page_whole) {
+                    whole = there && p0 + kEntries - 1 <= place_first && p0 + kEntries <= w.req.entries && (a.window == 0 || p0 > place_last - a.window || p0 + kEntries <= a.first);
+                    if (!(p0 < w.span.hi && (p0 + kEntries > w.span.lo || p0 < w.span.first))) continue;
+                }
+                float s[2 * Sub][4];
 #pragma unroll
-                for (int mt = 0; mt < MW; ++mt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[mt][0][i] = s[mt][1][i] = 0.f;
+                for (int i = 0; i < 2 * Sub; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
                 if constexpr (!kE4m3) {
-                    const int e = 16 * sl + (lane & 7) + ((lane >> 4) << 3);
-                    const uint32_t row = k_sm + e * 128, flip = e & 7, half = (lane >> 3) & 1;
 #pragma unroll
                     for (int ks = 0; ks < D / 16; ++ks) {
-                        uint32_t kf[4];
-                        ldmatrix4(kf, row + (ks / 4) * (kGqaTile * 128) + ((((ks % 4) * 2 + half) ^ flip) << 4));
+                        uint32_t qq[4];
+                        if (!kQInRegs) q_fragment(qq, ks);
+                        const uint32_t(&qa)[4] = kQInRegs ? qf[kQInRegs ? ks : 0] : qq;
 #pragma unroll
-                        for (int mt = 0; mt < MW; ++mt) {
-                            uint32_t qq[4];
-                            if (!kQInRegs) q_fragment(qq, mt, ks);
-                            const uint32_t(&qa)[4] = kQInRegs ? qf[kQInRegs ? ks : 0] : qq;
-                            mma16816<kBf16>(s[mt][0], qa, kf[0], kf[1]);
-                            mma16816<kBf16>(s[mt][1], qa, kf[2], kf[3]);
+                        for (int i = 0; i < Sub; ++i) {
+                            const int e = 16 * (sl + i) + (lane & 7) + ((lane >> 4) << 3);
+                            uint32_t kf[4];
+                            ldmatrix4(kf, k_sm + e * 128 + (ks / 4) * (kGqaTile * 128) + ((((ks % 4) * 2 + ((lane >> 3) & 1)) ^ (e & 7)) << 4));
+                            mma16816<kBf16>(s[2 * i], qa, kf[0], kf[1]);
+                            mma16816<kBf16>(s[2 * i + 1], qa, kf[2], kf[3]);
                         }
                     }
                 } else {
 #pragma unroll
                     for (int j = 0; j < D / 64; ++j) {
-                        uint4 kb[2];
+                        uint4 kb[2 * Sub];
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
+                        for (int i = 0; i < 2 * Sub; ++i) {
                             const int e = 16 * sl + 8 * i + entry_of(g);
-                            const uint32_t at = C::Box == 128 ? k_sm + (j / 2) * (kGqaTile * 128) + e * 128 + ((((j & 1) * 4 + c) ^ (e & 7)) << 4)
-                                                              : k_sm + e * 64 + ((c ^ ((e >> 1) & 3)) << 4);
-                            kb[i] = ptx::lds_v4(at);
+                            kb[i] = ptx::lds_v4(C::Box == 128 ? k_sm + (j / 2) * (kGqaTile * 128) + e * 128 + ((((j & 1) * 4 + c) ^ (e & 7)) << 4) : k_sm + e * 64 + ((c ^ ((e >> 1) & 3)) << 4));
                         }
 #pragma unroll
                         for (int st = 0; st < 4; ++st) {
-                            uint32_t kf[4];
+                            uint32_t qq[4];
+                            if (!kQInRegs) q_fragment(qq, 4 * j + st);
+                            const uint32_t(&qa)[4] = kQInRegs ? qf[kQInRegs ? 4 * j + st : 0] : qq;
 #pragma unroll
-                            for (int i = 0; i < 2; ++i) ptx::e4m3x4_to_f16x4(st == 0 ? kb[i].x : st == 1 ? kb[i].y : st == 2 ? kb[i].z : kb[i].w, kf[2 * i], kf[2 * i + 1]);
-#pragma unroll
-                            for (int mt = 0; mt < MW; ++mt) {
-                                uint32_t qq[4];
-                                if (!kQInRegs) q_fragment(qq, mt, 4 * j + st);
-                                const uint32_t(&qa)[4] = kQInRegs ? qf[kQInRegs ? 4 * j + st : 0] : qq;
-                                mma16816<false>(s[mt][0], qa, kf[0], kf[1]);
-                                mma16816<false>(s[mt][1], qa, kf[2], kf[3]);
+                            for (int i = 0; i < 2 * Sub; ++i) {
+                                uint32_t k0, k1;
+                                ptx::e4m3x4_to_f16x4(st == 0 ? kb[i].x : st == 1 ? kb[i].y : st == 2 ? kb[i].z : kb[i].w, k0, k1);
+                                mma16816<false>(s[i], qa, k0, k1);
                             }
                         }
                     }
                 }
                 // scores in log2 units; what a row does not see is -inf
 #pragma unroll
-                for (int mt = 0; mt < MW; ++mt)
+                for (int i = 0; i < 2 * Sub; ++i)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
+                    for (int q = 0; q < 4; ++q) s[i][q] *= scale[q >> 1];
+                if (!whole) {
+#pragma unroll
+                    for (int i = 0; i < 2 * Sub; ++i)
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {
-                            float x = s[mt][i][q] * scale[mt][q >> 1];
-                            if (!whole) {
-                                const int p = p0 + 8 * i + entry_of(2 * c + (q & 1)), at = place[mt][q >> 1];
-                                if (!(there && p <= at && p < w.req.entries && (a.window == 0 || p > at - a.window || p < a.first))) x = -INFINITY;
-                            }
-                            s[mt][i][q] = x;
+                            const int p = p0 + 8 * i + entry_of(2 * c + (q & 1)), at = place[q >> 1];
+                            if (!(there && p <= at && p < w.req.entries && (a.window == 0 || p > at - a.window || p < a.first))) s[i][q] = -INFINITY;
                         }
+                }
                 if (a.logits != nullptr) {
 #pragma unroll
-                    for (int mt = 0; mt < MW; ++mt)
-#pragma unroll
-                        for (int hh = 0; hh < 2; ++hh) {
-                            const int r = row_first + (wm * MW + mt) * 16 + g + 8 * hh;
-                            if (r < rows) {
-                                float* const to = a.logits + ((int64_t(w.b) * a.Hkv + w.h) * rows + r) * a.logit_stride + p0;
-#pragma unroll
-                                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                                    for (int q = 0; q < 2; ++q) to[8 * i + entry_of(2 * c + q)] = s[mt][i][2 * hh + q];
-                            }
-                        }
-                }
-                // running maximum and sum
-                uint32_t pf[MW][4];
-#pragma unroll
-                for (int mt = 0; mt < MW; ++mt) {
-                    float top[2];
-#pragma unroll
                     for (int hh = 0; hh < 2; ++hh) {
-                        top[hh] = fmaxf(fmaxf(s[mt][0][2 * hh], s[mt][0][2 * hh + 1]), fmaxf(s[mt][1][2 * hh], s[mt][1][2 * hh + 1]));
-                        top[hh] = fmaxf(top[hh], __shfl_xor_sync(0xFFFFFFFFu, top[hh], 1));
-                        top[hh] = fmaxf(top[hh], __shfl_xor_sync(0xFFFFFFFFu, top[hh], 2));
-                        top[hh] = fmaxf(top[hh], m[mt][hh]);
-                    }
-                    if (__any_sync(0xFFFFFFFFu, top[0] != m[mt][0] || top[1] != m[mt][1])) {
+                        const int r = row_first + wm * 16 + g + 8 * hh;
+                        if (r < rows) {
+                            float* const to = a.logits + ((int64_t(w.b) * a.Hkv + w.h) * rows + r) * a.logit_stride + p0;
 #pragma unroll
-                        for (int hh = 0; hh < 2; ++hh) {
-                            const float by = top[hh] == -INFINITY ? 1.f : ptx::ex2(m[mt][hh] - top[hh]);
-                            m[mt][hh] = top[hh];
-                            l[mt][hh] *= by;
-#pragma unroll
-                            for (int j = 0; j < D / 8; ++j) {
-                                o[mt][j][2 * hh] *= by;
-                                o[mt][j][2 * hh + 1] *= by;
+                            for (int i = 0; i < 2 * Sub; ++i) {
+                                if (kPermuted) {
+                                    to[8 * i + entry_of(2 * c)] = s[i][2 * hh];
+                                    to[8 * i + entry_of(2 * c + 1)] = s[i][2 * hh + 1];
+                                } else {
+                                    *reinterpret_cast<float2*>(to + 8 * i + 2 * c) = make_float2(s[i][2 * hh], s[i][2 * hh + 1]);
+                                }
                             }
                         }
                     }
+                }
+                // References move where a score has passed them by 2^8 (or at a row's first entry): looked at by each lane, and agreed upon by the four of a row only then.
+                float top[2];
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                    top[hh] = fmaxf(s[0][2 * hh], s[0][2 * hh + 1]);
+#pragma unroll
+                    for (int i = 1; i < 2 * Sub; ++i) top[hh] = ptx::max3(top[hh], s[i][2 * hh], s[i][2 * hh + 1]);
+                }
+                if (__any_sync(0xFFFFFFFFu, (m[0] == -INFINITY ? top[0] > m[0] : top[0] - m[0] > kGqaLazy) || (m[1] == -INFINITY ? top[1] > m[1] : top[1] - m[1] > kGqaLazy))) {
 #pragma unroll
                     for (int hh = 0; hh < 2; ++hh) {
-                        const float ref = m[mt][hh] == -INFINITY ? 0.f : m[mt][hh];
+                        float t = fmaxf(top[hh], m[hh]);
+                        t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 1));
+                        t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 2));
+                        // (a row goes by its own scores only)
+                        const bool first = m[hh] == -INFINITY, moves = first ? t > m[hh] : t - m[hh] > kGqaLazy;
+                        const float by = moves && !first ? ptx::ex2(m[hh] - t) : 1.f;
+                        if (moves) m[hh] = t;
+                        l[hh] *= by;
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const float e_lo = ptx::ex2(s[mt][i][2 * hh] - ref), e_hi = ptx::ex2(s[mt][i][2 * hh + 1] - ref);
-                            l[mt][hh] += e_lo + e_hi;
-                            pf[mt][2 * i + hh] = kBf16 ? ptx::pack_bf16x2(e_lo, e_hi) : ptx::pack_f16x2(e_lo, e_hi);
+                        for (int j = 0; j < D / 8; ++j) {
+                            o[j][2 * hh] *= by;
+                            o[j][2 * hh + 1] *= by;
                         }
                     }
                 }
-                if (sl + WN >= 4) {
+                uint32_t pf[Sub][4];
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                    const float ref = m[hh] == -INFINITY ? 0.f : m[hh];
+#pragma unroll
+                    for (int i = 0; i < 2 * Sub; ++i) {
+                        const float e_lo = ptx::ex2(s[i][2 * hh] - ref), e_hi = ptx::ex2(s[i][2 * hh + 1] - ref);
+                        l[hh] += e_lo + e_hi;
+                        pf[i / 2][2 * (i % 2) + hh] = kBf16 ? ptx::pack_bf16x2(e_lo, e_hi) : ptx::pack_f16x2(e_lo, e_hi);
+                    }
+                }
+                if (sl + WN * Sub >= 4) {
                     __syncwarp();
                     if (lane == 0) ptx::mbar_arrive(bar_empty + 8 * ks_);
                     k_given_back = true;
@@ -631,52 +638,49 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
                     wait_full(seq + 1);
                     v_waited = true;
                 }
-                // V of entries that no row of the group sees may be anything: it counts as zero (0 * inf is not 0)
-                uint32_t keep[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
-                if (!whole) {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        keep[i] = 0;
+                for (int i = 0; i < Sub; ++i) {
+                    // V of entries that no row of the group sees may be anything: it counts as zero (0 * inf is not 0)
+                    uint32_t keep[2] = {0xFFFFFFFFu, 0xFFFFFFFFu};
+                    if (!whole) {
 #pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            const int p = p0 + 8 * i + entry_of(2 * c + q);
-                            if (p < w.span.hi && (p >= w.span.lo || p < w.span.first)) keep[i] |= q ? 0xFFFF0000u : 0xFFFFu;
+                        for (int x = 0; x < 2; ++x) {
+                            keep[x] = 0;
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) {
+                                const int p = p0 + 16 * i + 8 * x + entry_of(2 * c + q);
+                                if (p < w.span.hi && (p >= w.span.lo || p < w.span.first)) keep[x] |= q ? 0xFFFF0000u : 0xFFFFu;
+                            }
                         }
                     }
-                }
-                const int ve = 16 * sl + ((lane >> 3) & 1) * 8 + entry_of(lane & 7), vc = lane >> 4;
+                    const int ve = 16 * (sl + i) + ((lane >> 3) & 1) * 8 + entry_of(lane & 7), vc = lane >> 4;
 #pragma unroll
-                for (int j = 0; j < D * C::ES / 32; ++j) {                    // 32 bytes of a row: 16 dimensions in 16 bits, 32 in 8
-                    uint32_t vf[4];
-                    const int ch = 2 * j + vc;
-                    ldmatrix4_trans(vf, C::Box == 128 ? v_sm + (ch / 8) * (kGqaTile * 128) + ve * 128 + (((ch & 7) ^ (ve & 7)) << 4)
-                                                      : v_sm + ve * 64 + ((ch ^ ((ve >> 1) & 3)) << 4));
-                    if constexpr (!kE4m3) {
-                        if (!whole) { vf[0] &= keep[0];  vf[1] &= keep[1];  vf[2] &= keep[0];  vf[3] &= keep[1]; }
+                    for (int j = 0; j < D * C::ES / 32; ++j) {                // 32 bytes of a row: 16 dimensions in 16 bits, 32 in 8
+                        uint32_t vf[4];
+                        const int ch = 2 * j + vc;
+                        ldmatrix4_trans(vf, C::Box == 128 ? v_sm + (ch / 8) * (kGqaTile * 128) + ve * 128 + (((ch & 7) ^ (ve & 7)) << 4)
+                                                          : v_sm + ve * 64 + ((ch ^ ((ve >> 1) & 3)) << 4));
+                        if constexpr (!kE4m3) {
+                            if (!whole) { vf[0] &= keep[0];  vf[1] &= keep[1];  vf[2] &= keep[0];  vf[3] &= keep[1]; }
+                            mma16816<kBf16>(o[2 * j], pf[i], vf[0], vf[1]);
+                            mma16816<kBf16>(o[2 * j + 1], pf[i], vf[2], vf[3]);
+                        } else {
+                            // a word: dimensions 2n, 2n + 1 of two entries -> two words of one dimension each; o[4 j' ..]: even and odd ones of 16
 #pragma unroll
-                        for (int mt = 0; mt < MW; ++mt) {
-                            mma16816<kBf16>(o[mt][2 * j], pf[mt], vf[0], vf[1]);
-                            mma16816<kBf16>(o[mt][2 * j + 1], pf[mt], vf[2], vf[3]);
-                        }
-                    } else {
-                        // a word: dimensions 2n, 2n + 1 of two entries -> two words of one dimension each; o[4 j' ..]: even and odd ones of 16
-#pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            const uint32_t w0 = __byte_perm(vf[2 * q], 0, 0x3120), w1 = __byte_perm(vf[2 * q + 1], 0, 0x3120);
-                            uint32_t b[4];
-                            ptx::e4m3x4_to_f16x4(w0, b[0], b[2]);
-                            ptx::e4m3x4_to_f16x4(w1, b[1], b[3]);
-                            if (!whole) { b[0] &= keep[0];  b[1] &= keep[1];  b[2] &= keep[0];  b[3] &= keep[1]; }
-#pragma unroll
-                            for (int mt = 0; mt < MW; ++mt) {
-                                mma16816<false>(o[mt][4 * j + 2 * q], pf[mt], b[0], b[1]);
-                                mma16816<false>(o[mt][4 * j + 2 * q + 1], pf[mt], b[2], b[3]);
+                            for (int q = 0; q < 2; ++q) {
+                                const uint32_t w0 = __byte_perm(vf[2 * q], 0, 0x3120), w1 = __byte_perm(vf[2 * q + 1], 0, 0x3120);
+                                uint32_t b[4];
+                                ptx::e4m3x4_to_f16x4(w0, b[0], b[2]);
+                                ptx::e4m3x4_to_f16x4(w1, b[1], b[3]);
+                                if (!whole) { b[0] &= keep[0];  b[1] &= keep[1];  b[2] &= keep[0];  b[3] &= keep[1]; }
+                                mma16816<false>(o[4 * j + 2 * q], pf[i], b[0], b[1]);
+                                mma16816<false>(o[4 * j + 2 * q + 1], pf[i], b[2], b[3]);
                             }
                         }
                     }
                 }
             }
-            // (every warp waits for both tiles of every turn: its arrivals then belong to the turn that they are counted in)
+            // (every warp of the group waits for both tiles of every page of its own: its arrivals then belong to the turn that they are counted in)
             if (!v_waited) wait_full(seq + 1);
             __syncwarp();
             if (lane == 0) {
@@ -684,75 +688,67 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
                 ptx::mbar_arrive(bar_empty + 8 * vs_);
             }
         }
+        tiles_before += uint32_t(w.k1 - w.k0);
 
         // ── the warps' parts of a row are joined ──
 #pragma unroll
-        for (int mt = 0; mt < MW; ++mt)
-#pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-                l[mt][hh] += __shfl_xor_sync(0xFFFFFFFFu, l[mt][hh], 1);
-                l[mt][hh] += __shfl_xor_sync(0xFFFFFFFFu, l[mt][hh], 2);
-                if (c == 0) {
-                    stat_m[warp * 16 * MW + mt * 16 + g + 8 * hh] = m[mt][hh];
-                    stat_l[warp * 16 * MW + mt * 16 + g + 8 * hh] = l[mt][hh];
-                }
+        for (int hh = 0; hh < 2; ++hh) {
+            l[hh] += __shfl_xor_sync(0xFFFFFFFFu, l[hh], 1);
+            l[hh] += __shfl_xor_sync(0xFFFFFFFFu, l[hh], 2);
+            if (c == 0) {
+                stat_m[warp * 16 + g + 8 * hh] = m[hh];
+                stat_l[warp * 16 + g + 8 * hh] = l[hh];
             }
+        }
         const bool complete = w.k0 == 0 && w.k1 == w.span.count;
         const int64_t part = 2 * int64_t(blockIdx.x) + (w.nth > 0);           // only the first and the last piece of a share can be parts
         const float v_scale = a.v_scale != nullptr ? ptx::ld(a.v_scale + w.h) : 1.f;
         ptx::bar_sync(1, kGqaConsumers);
+        auto row_max = [&](int of_wm, int r) {
+            float top = -INFINITY;
 #pragma unroll
-        for (int mt = 0; mt < MW; ++mt) {
-            auto row_max = [&](int of_wm, int r) {
-                float top = -INFINITY;
+            for (int n = 0; n < C::Parts; ++n) top = fmaxf(top, stat_m[(n * C::WM + of_wm) * 16 + r]);
+            return top;
+        };
 #pragma unroll
-                for (int n = 0; n < WN; ++n) top = fmaxf(top, stat_m[(of_wm * WN + n) * 16 * MW + mt * 16 + r]);
-                return top;
-            };
+        for (int hh = 0; hh < 2; ++hh) {
+            const float top = row_max(wm, g + 8 * hh), by = m[hh] == -INFINITY ? 0.f : ptx::ex2(m[hh] - top);
+            float* const to = merge + (warp * 16 + g + 8 * hh) * C::MergePitch;
+            if constexpr (!kE4m3) {
 #pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-                const float top = row_max(wm, g + 8 * hh), by = m[mt][hh] == -INFINITY ? 0.f : ptx::ex2(m[mt][hh] - top);
-                float* const to = merge + (warp * 16 + g + 8 * hh) * C::MergePitch;
-                if constexpr (!kE4m3) {
+                for (int j = 0; j < D / 8; ++j) *reinterpret_cast<float2*>(to + 8 * j + 2 * c) = make_float2(o[j][2 * hh] * by, o[j][2 * hh + 1] * by);
+            } else {
 #pragma unroll
-                    for (int j = 0; j < D / 8; ++j)
-                        *reinterpret_cast<float2*>(to + 8 * j + 2 * c) = make_float2(o[mt][j][2 * hh] * by, o[mt][j][2 * hh + 1] * by);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < D / 16; ++j)
-                        *reinterpret_cast<float4*>(to + 16 * j + 4 * c) = make_float4(o[mt][2 * j][2 * hh] * by, o[mt][2 * j + 1][2 * hh] * by, o[mt][2 * j][2 * hh + 1] * by,
-                                                                                      o[mt][2 * j + 1][2 * hh + 1] * by);
-                }
+                for (int j = 0; j < D / 16; ++j)
+                    *reinterpret_cast<float4*>(to + 16 * j + 4 * c) = make_float4(o[2 * j][2 * hh] * by, o[2 * j + 1][2 * hh] * by, o[2 * j][2 * hh + 1] * by, o[2 * j + 1][2 * hh + 1] * by);
             }
-            ptx::bar_sync(1, kGqaConsumers);
-            constexpr int kLanes = D / 4;
-            const int x = 4 * (tid % kLanes);
+        }
+        ptx::bar_sync(1, kGqaConsumers);
+        constexpr int kLanes = D / 4;
+        const int x = 4 * (tid % kLanes);
 #pragma unroll 2
-            for (int rr = tid / kLanes; rr < 16 * C::WM; rr += kGqaConsumers / kLanes) {
-                const int of_wm = rr >> 4, rl = rr & 15, r = (of_wm * MW + mt) * 16 + rl;
-                const int row = row_first + r;
-                if (row >= rows) continue;
-                const int token = int(uint32_t(row) / uint32_t(a.G));
-                const float top = row_max(of_wm, rl);
-                float sum = 0.f;
-                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int r = tid / kLanes; r < R; r += kGqaConsumers / kLanes) {
+            const int of_wm = r >> 4, rl = r & 15, row = row_first + r;
+            if (row >= rows) break;
+            const int token = int(uint32_t(row) / uint32_t(a.G));
+            const float top = row_max(of_wm, rl);
+            float sum = 0.f;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int n = 0; n < WN; ++n) {
-                    const int at = of_wm * WN + n;
-                    const float mm = stat_m[at * 16 * MW + mt * 16 + rl], ll = stat_l[at * 16 * MW + mt * 16 + rl];
-                    sum += mm == -INFINITY ? ll : ll * ptx::ex2(mm - top);     // (a NaN row has a maximum of -inf and a NaN sum)
-                    const float4 u = *reinterpret_cast<const float4*>(merge + (at * 16 + rl) * C::MergePitch + x);
-                    v.x += u.x;  v.y += u.y;  v.z += u.z;  v.w += u.w;
-                }
-                if (!complete) {
-                    const float per = sum == 0.f ? 0.f : 1.f / sum;
-                    *reinterpret_cast<float4*>(a.part_o + (part * R + r) * D + x) = make_float4(v.x * per, v.y * per, v.z * per, v.w * per);
-                    if (x == 0) a.part_lse[part * R + r] = top + log2f(sum);
-                    continue;
-                }
-                gqa_write_row<D>(a, w.req.row0 + token, w.h * a.G + row - token * a.G, (int64_t(w.b) * a.Hkv + w.h) * rows + row, x, v, top, sum, v_scale);
+            for (int n = 0; n < C::Parts; ++n) {
+                const int at = (n * C::WM + of_wm) * 16 + rl;
+                const float mm = stat_m[at], ll = stat_l[at];
+                sum += mm == -INFINITY ? ll : ll * ptx::ex2(mm - top);         // (a NaN row has a maximum of -inf and a NaN sum)
+                const float4 u = *reinterpret_cast<const float4*>(merge + at * C::MergePitch + x);
+                v.x += u.x;  v.y += u.y;  v.z += u.z;  v.w += u.w;
             }
-            ptx::bar_sync(1, kGqaConsumers);
+            if (!complete) {
+                const float per = sum == 0.f ? 0.f : 1.f / sum;
+                *reinterpret_cast<float4*>(a.part_o + (part * R + r) * D + x) = make_float4(v.x * per, v.y * per, v.z * per, v.w * per);
+                if (x == 0) a.part_lse[part * R + r] = top + log2f(sum);
+                continue;
+            }
+            gqa_write_row<D>(a, w.req.row0 + token, w.h * a.G + row - token * a.G, (int64_t(w.b) * a.Hkv + w.h) * rows + row, x, v, top, sum, v_scale);
         }
     }
 }
@@ -916,6 +912,13 @@ __device__ __forceinline__ uint32_t quant_pair(float lo, float hi) {
     return r;
 }
 
+// x / s from the correctly rounded 1 / s: Markstein's step, which gives the correctly rounded quotient.  Quotients beyond e4m3's range are left as they are (the step would make NaN of
+// infinite ones).
+__device__ __forceinline__ float by_scale(float x, float s, float inverse) {
+    const float q = x * inverse, r = fmaf(fmaf(-q, s, x), inverse, q);
+    return fabsf(q) < 1024.f ? r : q;
+}
+
 // A block takes some consecutive tokens: a thread each finds out where they go (offset, position, page: one chain of loads for the block), then all threads copy, 16 bytes a thread
 // and load, four on the way.  Bound by that chain when small and by memory when large.
 constexpr int kGqaInsertTokens = 32;
@@ -987,6 +990,8 @@ __global__ void __launch_bounds__(kGqaInsertThreads) gqa_insert_kernel(const __g
             if constexpr (E4M3) {
                 const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
                 uint32_t o[4];
+                const float inverse = __frcp_rn(scale[i]);
+                const bool plain = scale[i] > 1e-30f && scale[i] < 1e30f;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     float lo, hi;
@@ -998,7 +1003,7 @@ __global__ void __launch_bounds__(kGqaInsertThreads) gqa_insert_kernel(const __g
                         lo = f.x;
                         hi = f.y;
                     }
-                    o[j] = quant_pair(__fdiv_rn(lo, scale[i]), __fdiv_rn(hi, scale[i]));
+                    o[j] = plain ? quant_pair(by_scale(lo, scale[i], inverse), by_scale(hi, scale[i], inverse)) : quant_pair(__fdiv_rn(lo, scale[i]), __fdiv_rn(hi, scale[i]));
                 }
                 *reinterpret_cast<uint2*>(to[i]) = make_uint2(o[0] | (o[1] << 16), o[2] | (o[3] << 16));
             } else {
