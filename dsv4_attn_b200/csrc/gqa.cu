@@ -295,6 +295,8 @@ extern "C" int dsv4_gqa_insert(const Dsv4GqaInsertParams* p, void* stream) {
     const int64_t strides[6] = {p->k_stride_b, p->k_stride_t, p->k_stride_h, p->v_stride_b, p->v_stride_t, p->v_stride_h};
     for (int i = 0; i < 6; ++i)
         if (strides[i] % 8 != 0) return int(cudaErrorInvalidValue);
+    for (int i = 2; i < 6; i += 3)
+        if (strides[i] < 0 || strides[i] > (int64_t(1) << 30) / p->Hkv) return int(cudaErrorInvalidValue);      // (places within a row stay within 32 bits)
     if (p->rows == 0) return 0;
     a.B = p->B;  a.T = p->T;  a.Hkv = p->Hkv;  a.D = p->D;  a.max_pages = p->max_pages;  a.rows = p->rows;
     a.q_start = p->q_start;  a.n_rows = p->n_rows;  a.insert_pos = p->insert_pos;  a.block_table = p->block_table;  a.num_pages = p->num_pages;

@@ -923,9 +923,8 @@ __device__ __forceinline__ float by_scale(float x, float s, float inverse) {
 // and load, four on the way.  Bound by that chain when small and by memory when large.
 constexpr int kGqaInsertTokens = 32;
 template <bool E4M3>
-__global__ void __launch_bounds__(kGqaInsertThreads) gqa_insert_kernel(const __grid_constant__ GqaInsertArgs a) {
-    __shared__ int64_t src_row[kGqaInsertTokens];                             // first element of the token's row, of K and V: [token] of K, and by `b`, `t` again for V
-    __shared__ int64_t src_row_v[kGqaInsertTokens];
+__global__ void __launch_bounds__(kGqaInsertThreads, 4) gqa_insert_kernel(const __grid_constant__ GqaInsertArgs a) {
+    __shared__ int64_t src_row[kGqaInsertTokens], src_row_v[kGqaInsertTokens];      // first element of the token's row of K and of V
     __shared__ int32_t entry[kGqaInsertTokens];                               // where it goes, -1: nowhere
     ptx::pdl_trigger();
     ptx::pdl_wait();
@@ -966,48 +965,64 @@ __global__ void __launch_bounds__(kGqaInsertThreads) gqa_insert_kernel(const __g
         entry[tid] = to;
     }
     __syncthreads();
-    const uint32_t per_head = uint32_t(a.D) / 8, pieces = uint32_t(a.Hkv) * per_head, all = uint32_t(n) * 2 * pieces;   // pieces of 16 bytes of a row of K or V
-    for (uint32_t at = tid; at < all; at += 4 * kGqaInsertThreads) {
-        uint4 v[4];
-        uint8_t* to[4];
-        float scale[4];
+    // A warp takes whole tokens, a lane four pieces of 16 bytes of K and of V at a time: where they lie in a row, and their heads' scales, are worked out once.
+    const int lane = tid & 31, per_head = a.D / 8, pieces = a.Hkv * per_head;
+    for (int x0 = lane; x0 < pieces; x0 += 128) {
+        int32_t off[2][4];                                                    // (of a row: below 2^31)
+        float scale[2][4];
+        bool plain = true;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            to[i] = nullptr;
-            const uint32_t piece = at + i * kGqaInsertThreads;
-            if (piece >= all) continue;
-            const uint32_t row = piece / pieces, x = piece - row * pieces, h = x / per_head, token = row >> 1, kv = row & 1;
-            const int e = entry[token];
-            if (e < 0) continue;
-            to[i] = static_cast<uint8_t*>(kv ? a.pool[1] : a.pool[0]) + (int64_t(e) * pieces + x) * (E4M3 ? 8 : 16);
-            if (E4M3) scale[i] = ptx::ld((kv ? a.scale[1] : a.scale[0]) + h);
-            v[i] = ptx::ldg_stream_v4(static_cast<const uint8_t*>(kv ? a.src[1] : a.src[0]) +
-                                      ((kv ? src_row_v[token] : src_row[token]) + int64_t(h) * (kv ? a.stride_h[1] : a.stride_h[0]) + 8 * (x - h * per_head)) * 2);
-        }
+            const int x = min(x0 + 32 * i, pieces - 1), h = x / per_head;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (to[i] == nullptr) continue;
-            if constexpr (E4M3) {
-                const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-                uint32_t o[4];
-                const float inverse = __frcp_rn(scale[i]);
-                const bool plain = scale[i] > 1e-30f && scale[i] < 1e30f;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float lo, hi;
-                    if (a.src_bf16) {
-                        lo = __uint_as_float(u[j] << 16);
-                        hi = __uint_as_float(u[j] & 0xFFFF0000u);
-                    } else {
-                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[j]));
-                        lo = f.x;
-                        hi = f.y;
-                    }
-                    o[j] = plain ? quant_pair(by_scale(lo, scale[i], inverse), by_scale(hi, scale[i], inverse)) : quant_pair(__fdiv_rn(lo, scale[i]), __fdiv_rn(hi, scale[i]));
+            for (int kv = 0; kv < 2; ++kv) {
+                off[kv][i] = int32_t(h * a.stride_h[kv]) + 8 * (x - h * per_head);
+                if (E4M3) {
+                    scale[kv][i] = ptx::ld(a.scale[kv] + h);
+                    plain &= scale[kv][i] > 1e-30f && scale[kv][i] < 1e30f;
                 }
-                *reinterpret_cast<uint2*>(to[i]) = make_uint2(o[0] | (o[1] << 16), o[2] | (o[3] << 16));
-            } else {
-                *reinterpret_cast<uint4*>(to[i]) = v[i];
+            }
+        }
+        for (int t = tid >> 5; t < n; t += kGqaInsertThreads / 32) {
+            const int e = entry[t];
+            if (e < 0) continue;
+            uint4 v[2][4];
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+                const uint8_t* const src = static_cast<const uint8_t*>(a.src[kv]) + (kv ? src_row_v[t] : src_row[t]) * 2;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (x0 + 32 * i < pieces) v[kv][i] = ptx::ldg_stream_v4(src + int64_t(off[kv][i]) * 2);
+            }
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+                uint8_t* const dst = static_cast<uint8_t*>(a.pool[kv]) + (int64_t(e) * pieces + x0) * (E4M3 ? 8 : 16);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (x0 + 32 * i >= pieces) continue;
+                    if constexpr (E4M3) {
+                        const uint32_t u[4] = {v[kv][i].x, v[kv][i].y, v[kv][i].z, v[kv][i].w};
+                        uint32_t o[4];
+                        const float inverse = __frcp_rn(scale[kv][i]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            float lo, hi;
+                            if (a.src_bf16) {
+                                lo = __uint_as_float(u[j] << 16);
+                                hi = __uint_as_float(u[j] & 0xFFFF0000u);
+                            } else {
+                                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[j]));
+                                lo = f.x;
+                                hi = f.y;
+                            }
+                            o[j] = plain ? quant_pair(by_scale(lo, scale[kv][i], inverse), by_scale(hi, scale[kv][i], inverse))
+                                         : quant_pair(__fdiv_rn(lo, scale[kv][i]), __fdiv_rn(hi, scale[kv][i]));
+                        }
+                        *reinterpret_cast<uint2*>(dst + 256 * i) = make_uint2(o[0] | (o[1] << 16), o[2] | (o[3] << 16));
+                    } else {
+                        *reinterpret_cast<uint4*>(dst + 512 * i) = v[kv][i];
+                    }
+                }
             }
         }
     }
