@@ -8,6 +8,7 @@
 
 #include "gqa_decode.cuh"
 #include "gqa_prefill.cuh"
+#include "gqa_rows.cuh"
 #include "kv_evict.cuh"
 #include "host_state.h"
 
@@ -65,6 +66,17 @@ cudaError_t make_pool_map(CUtensorMap* map, const void* pool, int64_t pages, int
 
 int64_t up(int64_t n) { return (n + 127) / 128 * 128; }
 
+// An 8-bit pool: boxes of a head's whole rows of a page, as they lie.
+cudaError_t make_raw_map(CUtensorMap* map, const void* pool, int64_t pages, int Hkv, int D) {
+    const EncodeTiledFn fn = encode_tiled_fn();
+    if (fn == nullptr) return cudaErrorNotSupported;
+    const cuuint64_t dims[3] = {cuuint64_t(D), cuuint64_t(Hkv), cuuint64_t(pages) * kGqaTile}, strides[2] = {cuuint64_t(D), cuuint64_t(Hkv) * D};
+    const cuuint32_t box[3] = {cuuint32_t(D), 1, kGqaTile}, estr[3] = {1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(pool), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
 // ── which form of the kernel ──
 // Rows of a KV head: 16, 32 or 64 in a group, the fewest that hold a request's (with 64: several groups).
 int group_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
@@ -96,9 +108,14 @@ struct Sizes {
     int64_t parts;                   // partial rows
     int64_t logit_rows, logit_stride;
     bool prefill;                    // gqa_prefill_kernel
+    int streams;                     // gqa_rows_kernel, if not 0
     int64_t plan_words;
     int64_t own_rows;                // entries of the call's own 16-bit pages
 };
+
+// ── which kernel takes tokens that are not packed ──
+// Rows of a KV head beyond which gqa_rows_kernel takes them.
+constexpr int kRowsMore = 32, kRowsMoreE4m3 = 16;
 
 // ── which kernel takes a prompt ──
 // A block of tokens is 256 rows (heads of 256: 128) in gqa_prefill_kernel, and takes at least a block of the GPU to itself; the decode kernel takes 64 rows at a time and shares the entries out.
@@ -122,7 +139,17 @@ bool gqa_sizes(const Dsv4GqaParams* p, Sizes& s) {
     s.logit_stride = entries;
     s.prefill = false;
     s.plan_words = s.own_rows = 0;
-    if (p->q_start != nullptr && p->G <= 128 && p->rows < 0x7FFFFFFF) {
+    s.streams = 0;
+    // (tensor maps have no axis that stays where it is)
+    const bool spread = (p->Hkv * p->G == 1 || p->q_stride_h > 0) && (tokens == 1 || p->q_stride_t > 0) && (p->q_start != nullptr || p->B == 1 || p->q_stride_b > 0);
+    if (p->q_start == nullptr && p->G <= 128 && (spread || p->kv_dtype == DSV4_DTYPE_E4M3) && tokens * p->G > (p->kv_dtype == DSV4_DTYPE_E4M3 ? kRowsMoreE4m3 : kRowsMore)) {
+        s.streams = p->D > 128 ? 1 : 2;
+        s.group_rows = 128 / p->G * p->G;
+        const int64_t most = int64_t(p->B) * ((tokens * p->G + s.group_rows - 1) / s.group_rows) * p->Hkv * ((longest + kGqaTile - 1) / kGqaTile + 1);
+        s.blocks = int(most < device_sms() ? most : device_sms());
+        s.parts = int64_t(s.blocks) * (2 * s.streams + 1) * s.group_rows;
+    }
+    if (p->q_start != nullptr && p->G <= 128 && p->rows < 0x7FFFFFFF && spread) {
         const int tile_tokens = 128 / p->G, block_tokens = tile_tokens * (p->D > 128 ? 1 : 2);
         const int64_t blocks = p->rows / block_tokens + p->B, full = (p->rows + block_tokens - 1) / block_tokens;
         const bool e4m3 = p->kv_dtype == DSV4_DTYPE_E4M3;
@@ -147,6 +174,55 @@ cudaError_t run_prefill(const GqaPrefillArgs& a, cudaStream_t stream) {
     cudaError_t e = ensure_smem(gqa_prefill_kernel<C>, C::Bytes, done);
     if (e != cudaSuccess) return e;
     return launch(gqa_prefill_kernel<C>, dim3(unsigned(a.g.blocks)), C::Threads, C::Bytes, stream, a);
+}
+
+template <int D, int KVT>
+cudaError_t run_rows(const GqaRowsArgs& a, cudaStream_t stream) {
+    using C = RowsCfg<D, KVT>;
+    static std::atomic<bool> done[kMaxDevices];
+    cudaError_t e = ensure_smem(gqa_rows_kernel<C>, C::Bytes, done);
+    if (e != cudaSuccess) return e;
+    return launch(gqa_rows_kernel<C>, dim3(unsigned(a.g.blocks)), C::Threads, C::Bytes, stream, a);
+}
+template <int D>
+cudaError_t run_rows(const GqaRowsArgs& a, int kv_dtype, cudaStream_t stream) {
+    if (kv_dtype == DSV4_DTYPE_BF16) return run_rows<D, kGqaBf16>(a, stream);
+    if (kv_dtype == DSV4_DTYPE_F16) return run_rows<D, kGqaF16>(a, stream);
+    return run_rows<D, kGqaE4m3>(a, stream);
+}
+
+// q by (element, head, token, request): boxes of 64 elements of a group's heads in a tile's tokens
+cudaError_t make_tokens_map(CUtensorMap* map, const Dsv4GqaParams* p, int tile_tokens) {
+    const EncodeTiledFn fn = encode_tiled_fn();
+    if (fn == nullptr) return cudaErrorNotSupported;
+    const int H = p->Hkv * p->G;
+    const int64_t row = int64_t(H) * p->D;
+    const cuuint64_t dims[4] = {cuuint64_t(p->D), cuuint64_t(H), cuuint64_t(p->T), cuuint64_t(p->B)};
+    // (axes of one element have any stride)
+    const cuuint64_t strides[3] = {cuuint64_t(H > 1 ? p->q_stride_h : p->D) * 2, cuuint64_t(p->T > 1 ? p->q_stride_t : row) * 2, cuuint64_t(p->B > 1 ? p->q_stride_b : row * p->T) * 2};
+    const cuuint32_t box[4] = {64, cuuint32_t(p->G), cuuint32_t(tile_tokens), 1}, estr[4] = {1, 1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(p->q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+cudaError_t decode_rows(const GqaArgs& g, const Dsv4GqaParams* p, cudaStream_t stream) {
+    GqaRowsArgs a{};
+    a.g = g;
+    a.tile_tokens = 128 / p->G;
+    cudaError_t e = cudaSuccess;
+    if (p->kv_dtype == DSV4_DTYPE_E4M3) {
+        e = make_raw_map(&a.g.k_map, p->k_pool, p->num_pages, p->Hkv, p->D);
+        if (e == cudaSuccess) e = make_raw_map(&a.g.v_map, p->v_pool, p->num_pages, p->Hkv, p->D);
+    } else {
+        e = make_pool_map(&a.g.k_map, p->k_pool, p->num_pages, p->Hkv, p->D, p->kv_dtype);
+        if (e == cudaSuccess) e = make_pool_map(&a.g.v_map, p->v_pool, p->num_pages, p->Hkv, p->D, p->kv_dtype);
+        if (e == cudaSuccess) e = make_pool_map(&a.v8_map, p->v_pool, p->num_pages, p->Hkv, p->D, p->kv_dtype, 8);
+        if (e == cudaSuccess) e = make_pool_map(&a.v1_map, p->v_pool, p->num_pages, p->Hkv, p->D, p->kv_dtype, 1);
+        if (e == cudaSuccess) e = make_tokens_map(&a.q_map, p, a.tile_tokens);
+    }
+    if (e != cudaSuccess) return e;
+    return p->D == 64 ? run_rows<64>(a, p->kv_dtype, stream) : p->D == 128 ? run_rows<128>(a, p->kv_dtype, stream) : run_rows<256>(a, p->kv_dtype, stream);
 }
 
 // q by (element, head, row): boxes of 64 elements of a group's heads in a tile's tokens
@@ -254,13 +330,19 @@ static int gqa_fwd(const Dsv4GqaParams* p, void* stream_) {
     a.dbg_drop_tile = state.drop_tile;
     a.status = p->status;
     if (s.prefill) return int(prefill(a, p, s, ws, stream));
-    cudaError_t e = make_pool_map(&a.k_map, p->k_pool, p->num_pages, p->Hkv, p->D, p->kv_dtype);
-    if (e == cudaSuccess) e = make_pool_map(&a.v_map, p->v_pool, p->num_pages, p->Hkv, p->D, p->kv_dtype);
-    if (e != cudaSuccess) return int(e);
-    e = p->D == 64 ? run_decode<64>(a, p->kv_dtype, stream) : p->D == 128 ? run_decode<128>(a, p->kv_dtype, stream) : run_decode<256>(a, p->kv_dtype, stream);
+    a.streams = s.streams;
+    cudaError_t e = cudaSuccess;
+    if (s.streams > 0) {
+        e = decode_rows(a, p, stream);
+    } else {
+        e = make_pool_map(&a.k_map, p->k_pool, p->num_pages, p->Hkv, p->D, p->kv_dtype);
+        if (e == cudaSuccess) e = make_pool_map(&a.v_map, p->v_pool, p->num_pages, p->Hkv, p->D, p->kv_dtype);
+        if (e != cudaSuccess) return int(e);
+        e = p->D == 64 ? run_decode<64>(a, p->kv_dtype, stream) : p->D == 128 ? run_decode<128>(a, p->kv_dtype, stream) : run_decode<256>(a, p->kv_dtype, stream);
+    }
     if (e != cudaSuccess) return int(e);
     const int64_t merge_rows = p->rows * p->Hkv * p->G, merge_blocks = (merge_rows + kGqaMergeRows - 1) / kGqaMergeRows;
-    if (s.blocks > 1) {
+    if (s.blocks > 1 || s.streams > 0) {
         const dim3 grid{unsigned(merge_blocks)};
         e = p->D == 64 ? launch(gqa_merge_kernel<64>, grid, kGqaMergeThreads, 0, stream, a)
                        : p->D == 128 ? launch(gqa_merge_kernel<128>, grid, kGqaMergeThreads, 0, stream, a) : launch(gqa_merge_kernel<256>, grid, kGqaMergeThreads, 0, stream, a);

@@ -57,6 +57,7 @@ struct GqaArgs {
     int group_rows;                  // R
     int one_group;                   // not packed, and a request's rows of a KV head fit a group
     int min_share;                   // tiles of a block, at least
+    int streams;                     // parts that a block leaves of a piece (gqa_rows_kernel; and a place more), or 0: one
     // weights of the entries
     float* logits;                   // [B][Hkv * T * G][logit_stride], log2 units; null: not wanted
     int64_t logit_stride;
@@ -194,13 +195,28 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t saddr) {
 __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t saddr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(saddr) : "memory");
 }
-// two e4m3 in the low half of a word -> two FP16, exact
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t w) {
-    uint32_t r;
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t}" : "=r"(r) : "r"(w));
-    return r;
+// Eight BF16 of a row that LANES lanes hold, brought to FP16 near 1 by a power of two, which is returned inverted: 2^e <= the row's largest < 2^(e + 1); zeros, infinities and what 2^-e cannot
+// bring there stay near enough.
+template <int LANES>
+__device__ __forceinline__ float gqa_near_one(uint4& v) {
+    float f[8], top = 0.f;
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        f[2 * i] = __uint_as_float(u[i] << 16);
+        f[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+        top = fmaxf(top, fmaxf(fabsf(f[2 * i]), fabsf(f[2 * i + 1])));
+    }
+#pragma unroll
+    for (int d = 1; d < LANES; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+    const int e = min(max(int(__float_as_uint(top) >> 23) - 127, -100), 126);
+    const float down = __uint_as_float(uint32_t(127 - e) << 23);
+    v.x = ptx::pack_f16x2(f[0] * down, f[1] * down);
+    v.y = ptx::pack_f16x2(f[2] * down, f[3] * down);
+    v.z = ptx::pack_f16x2(f[4] * down, f[5] * down);
+    v.w = ptx::pack_f16x2(f[6] * down, f[7] * down);
+    return __uint_as_float(uint32_t(127 + e) << 23);
 }
-
 __host__ __device__ constexpr int gqa_blocks_per_sm(int D) { return D > 128 ? 1 : 2; }
 
 // D: head dimension; KVT: type of K and V; WM: warps side by side over the rows, 16 each
@@ -440,27 +456,7 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
                     v = *reinterpret_cast<const uint4*>(q0 + at * 2);
                 }
                 if (kE4m3) {
-                    float factor = 1.f;
-                    if (a.q_bf16) {
-                        float f[8], top = 0.f;
-                        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            f[2 * i] = __uint_as_float(u[i] << 16);
-                            f[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
-                            top = fmaxf(top, fmaxf(fabsf(f[2 * i]), fabsf(f[2 * i + 1])));
-                        }
-#pragma unroll
-                        for (int d = 1; d < kLanes; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-                        // 2^e <= top < 2^(e + 1); zeros, infinities and what 2^-e cannot bring there stay near enough
-                        const int e = min(max(int(__float_as_uint(top) >> 23) - 127, -100), 126);
-                        const float down = __uint_as_float(uint32_t(127 - e) << 23);
-                        factor = __uint_as_float(uint32_t(127 + e) << 23);
-                        uint32_t o[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[i] = ptx::pack_f16x2(f[2 * i] * down, f[2 * i + 1] * down);
-                        v = make_uint4(o[0], o[1], o[2], o[3]);
-                    }
+                    const float factor = a.q_bf16 ? gqa_near_one<kLanes>(v) : 1.f;
                     if (l == 0) row_factor[r] = factor;
                 }
                 ptx::sts_v4(q_sm + r * C::QPitch + 16 * l, v);
@@ -820,9 +816,12 @@ __global__ void __launch_bounds__(kGqaMergeThreads) gqa_merge_kernel(const __gri
     const int64_t share = gqa_share(a, total);
     const int c0 = int(quotient(unit, share)), c1 = int(quotient(unit + gqa_span(a, req, rg).count - 1, share));
     if (c0 == c1) return;
-    const int64_t first = 2 * int64_t(c0) + (unit != c0 * share);              // (every later block begins with its part)
-    auto part = [&](int i) { return (i == 0 ? first : 2 * int64_t(c0 + i)) * a.group_rows + r; };
-    const int parts = c1 - c0 + 1;
+    const int later = unit != c0 * share;                                      // (every later block begins with its part)
+    const int streams = max(a.streams, 1), places = 2 * streams + (a.streams > 0), parts = (c1 - c0 + 1) * streams;
+    auto part = [&](int i) {
+        const int block = streams == 2 ? i >> 1 : i;
+        return (int64_t(c0 + block) * places + (block == 0 ? later * streams : 0) + (i - block * streams)) * a.group_rows + r;
+    };
     float top = -INFINITY;
     for (int i = lane; i < parts; i += 32) top = fmaxf(top, a.part_lse[part(i)]);
 #pragma unroll

@@ -43,7 +43,7 @@ struct PrefillCfg {
     static constexpr bool BF16 = BF16_;
     static constexpr int NT = D <= 128 ? 2 : 1, NE = kGqaTile;
     static constexpr int Slot = NE * D * 2, QTile = 128 * D * 2;
-    static constexpr int Slots = (225 * 1024 - NT * QTile) / Slot;
+    static constexpr int Slots = (225 * 1024 - NT * QTile) / Slot / 2 * 2;      // (even: a slot holds K always, or V, and the same warps see all of its turns)
     static constexpr int Flags = 16;              // steps whose page flags are kept: the producer is at most Slots / 2 + 2 ahead of the softmax warps
     static_assert(Slots / 2 + 2 < Flags, "");
     static constexpr int SoftmaxWarps = 4 * NT, Threads = (SoftmaxWarps + 2 + NT) * 32;
@@ -134,6 +134,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
                  :: "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
                     "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t smem_dst, const void* tensor_map, int x, int y, int z, int w, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 :: "r"(smem_dst), "l"(reinterpret_cast<uint64_t>(tensor_map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar) : "memory");
 }
 
 // The units of a block, walked by each role for itself.

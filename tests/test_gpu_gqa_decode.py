@@ -93,6 +93,50 @@ def test_queries_of_both_types_over_8_bits_and_their_range(lib):
         c.check(*c.call(lib))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "e4m3"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_many_rows_of_a_head(lib, dtype, D):
+    """Drafted tokens x query heads beyond what a few warps hold: one group and several, streams without a page, units that are cut."""
+    for Hkv, G, T, kv in ((2, 8, 5, [64, 5, 65, 128, 129, 700, 0, 3000]), (1, 40, 1, [1, 63, 200, 1000]), (4, 16, 9, [9, 100, 777]), (1, 3, 50, [50, 64, 500]), (1, 128, 2, [300, 2]),
+                          (8, 17, 1, [40, 4000])):
+        c = Case(kv, T, Hkv=Hkv, G=G, D=D, dtype=dtype, seed=G, sink=G == 8)
+        c.check(*c.call(lib))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+def test_many_rows_with_windows_and_weights(lib, dtype):
+    for window, first in ((1, 0), (60, 3), (64, 64), (129, 200), (1 << 30, 0)):
+        c = Case([5, 64, 300, 1000, 12], 5, Hkv=2, G=12, D=128, dtype=dtype, window=window, first=first, seed=first)
+        before = torch.rand(c.B, c.table.shape[1] * PAGE, device="cuda")
+        w = before.clone()
+        out, lse = c.call(lib, weights=w)
+        c.check(out, lse, w, before)
+
+
+def test_scores_that_grow_with_many_rows(lib):
+    for dtype in ("f16", "e4m3"):
+        c = Case([2000], 4, Hkv=2, G=16, D=64, dtype=dtype)
+        n = torch.arange(2000, device="cuda")
+        c.q.fill_(0)
+        c.q[..., 0] = 1.0
+        c.q[..., 1:] = torch.randn(1, 4, 32, 63, device="cuda").to(c.q.dtype)
+        c.pools[0].view(torch.uint8 if dtype == "e4m3" else torch.int16)[c.table[0, n // 64].long(), n % 64, :, 0] = \
+            (n.float() / 2000 * 60).to(c.pools[0].dtype).view(torch.uint8 if dtype == "e4m3" else torch.int16)[:, None]
+        c.scale = 1.0
+        c.check(*c.call(lib))
+
+
+def test_queries_that_share_their_rows(lib):
+    """Expanded queries: axes with a stride of 0."""
+    for G, T in ((4, 1), (48, 1), (8, 5)):
+        c = Case([100, 300], T, Hkv=2, G=G, D=128, dtype="bf16")
+        c.q = c.q[:1].expand(2, -1, -1, -1)
+        a, kw = c.args()
+        out, lse = lib.gqa_decode(c.q, *a, **kw)
+        c.q = c.q.contiguous()
+        c.check(out, lse)
+
+
 def test_equal_and_extreme_scores(lib):
     """Scores that are all alike, and one that outweighs the others by far."""
     c = Case([130, 64], 1, Hkv=1, G=2, D=64, dtype="bf16")
@@ -105,6 +149,11 @@ def test_equal_and_extreme_scores(lib):
 @pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
 def test_a_nan_query_spoils_its_own_row_only(lib, dtype):
     c = Case([500, 30], 1, Hkv=2, G=4, D=128, dtype=dtype)
+    for d in (c, Case([500, 30], 3, Hkv=2, G=20, D=128, dtype=dtype)):
+        nan_query(lib, d)
+
+
+def nan_query(lib, c):
     want, want_lse = c.call(lib)
     c.q[0, 0, 2, 5] = float("nan")
     out, lse = c.call(lib)
@@ -139,8 +188,9 @@ def test_pages_out_of_range_are_left_out_and_reported(lib):
     assert st[0] == 0 and (out[0] == 0).all() and torch.isneginf(lse[0]).all()
 
 
-def test_a_wait_that_runs_out(lib):
-    c = Case([3000, 200], 1, Hkv=2, G=4, D=64, dtype="f16")
+@pytest.mark.parametrize("G,dtype", [(4, "f16"), (4, "e4m3"), (40, "f16"), (40, "e4m3")])
+def test_a_wait_that_runs_out(lib, G, dtype):
+    c = Case([3000, 200], 1, Hkv=2, G=G, D=64, dtype=dtype)
     st = lib.new_status("cuda")
     lib.LIB.dsv4_debug_set_wait(200_000, 1)
     try:
@@ -155,7 +205,12 @@ def test_a_wait_that_runs_out(lib):
 
 
 def test_captured_and_replayed_with_other_lengths(lib):
-    c = Case([100, 900, 64, 0], 1, Hkv=2, G=4, D=128, dtype="bf16", width=20)
+    for G in (4, 48):
+        captured(lib, G)
+
+
+def captured(lib, G):
+    c = Case([100, 900, 64, 0], 1, Hkv=2, G=G, D=128, dtype="bf16", width=20)
     c.call(lib)
     w = torch.zeros(4, c.table.shape[1] * PAGE, device="cuda")
     graph = torch.cuda.CUDAGraph()
@@ -165,7 +220,7 @@ def test_captured_and_replayed_with_other_lengths(lib):
     graph.replay()
     first = w.clone()
     c.check(out, lse, w, torch.zeros_like(w))
-    d = Case([333, 1, 1280, 77], 1, Hkv=2, G=4, D=128, dtype="bf16", seed=9, width=20)
+    d = Case([333, 1, 1280, 77], 1, Hkv=2, G=G, D=128, dtype="bf16", seed=9, width=20)
     assert d.table.shape == c.table.shape
     for to, of in ((c.q, d.q), (c.len_t, d.len_t), (c.table, d.table), (c.pools[0].view(torch.int16), d.pools[0].view(torch.int16)), (c.pools[1].view(torch.int16), d.pools[1].view(torch.int16))):
         to.copy_(of)
