@@ -30,9 +30,9 @@ struct RowsCfg {
     static constexpr int Slot = NE * D * 2, QTile = 128 * D * 2, RawSlot = NE * D;
     // (a multiple of twice the streams: a slot then belongs to one stream's K or V, and the same warp sees all of its turns)
     static constexpr int Slots = E4M3 ? (D > 128 ? 2 : 8) : (D > 128 ? 4 : 8);
-    static constexpr int RawSlots = E4M3 ? (D > 128 ? 4 : 8) : 0;
+    static constexpr int RawSlots = E4M3 ? (D > 128 ? 4 : 8) : 1;
     static constexpr int SoftmaxWarps = 4 * NT, Convert = SoftmaxWarps + 2 + NT, Warps = Convert + (E4M3 ? 4 : 0), Threads = Warps * 32;
-    static constexpr int OffRing = QTile, OffRaw = OffRing + Slots * Slot, OffBars = OffRaw + RawSlots * RawSlot;
+    static constexpr int OffRing = QTile, OffRaw = OffRing + Slots * Slot, OffBars = OffRaw + (E4M3 ? RawSlots * RawSlot : 0);
     static constexpr int Bars = 2 * Slots + 2 * RawSlots + 2 + 6 * NT + 2;
     static constexpr int Flags = 32;                                          // pages whose flags are kept
     static_assert(Slots / 2 + RawSlots / 2 + 2 * NT + 4 < Flags, "");
@@ -60,8 +60,8 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_rows_kernel(const __grid_co
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
     if (tid == 0) {
-        for (int i = 0; i < C::Slots; ++i) { ptx::mbar_init(kv_full + 8 * i, C::E4M3 ? 4 : 1);  ptx::mbar_init(kv_empty + 8 * i, 1); }
-        for (int i = 0; i < C::RawSlots; ++i) { ptx::mbar_init(raw_full + 8 * i, 1);  ptx::mbar_init(raw_empty + 8 * i, 4); }
+        for (int i = 0; i < C::Slots; ++i) { ptx::mbar_init(kv_full + 8 * i, C::E4M3 ? 2 : 1);  ptx::mbar_init(kv_empty + 8 * i, 1); }
+        for (int i = 0; i < C::RawSlots; ++i) { ptx::mbar_init(raw_full + 8 * i, 1);  ptx::mbar_init(raw_empty + 8 * i, 2); }
         ptx::mbar_init(q_full, C::E4M3 ? 4 : 1);
         ptx::mbar_init(q_empty, NT + C::SoftmaxWarps);
         ptx::mbar_init(join_full, 4);
@@ -272,47 +272,42 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_rows_kernel(const __grid_co
             for (int k = w.k0; k < w.k1 && ok; ++k, ++tile) {
                 const int e0 = w.span.slot(k) * NE;
                 const bool all = e0 + NE <= w.span.hi && (e0 >= w.span.lo || e0 + NE <= w.span.first);
-#pragma unroll 1
-                for (int kv = 0; kv < 2 && ok; ++kv) {
-                    const uint32_t seq = 2 * tile + kv, from = seq % C::RawSlots, st = seq % C::Slots;
-                    if (seq >= C::Slots) wait2(raw_full + 8 * from, seq / C::RawSlots, kv_empty + 8 * st, seq / C::Slots - 1, 0, int(seq));
-                    else wait(raw_full + 8 * from, seq / C::RawSlots, 0, int(seq));
-                    if (!ok) break;
-                    // A lane takes 16 bytes: pairs of rows, of which one has the even and the other the odd 64 bytes, so that eight lanes meet all banks both ways.
-                    constexpr int kHalves = D / 64;
-                    const int c = lane & 3, u = (lane >> 2) & 1;
-                    const uint32_t src = raw + from * C::RawSlot, dst = ring + st * C::Slot;
-                    uint4 v[2][kHalves];
+                // Two warps have K, two V, half a page each.  A lane takes 16 bytes: pairs of rows, of which one has the even and the other the odd 64 bytes, so that eight lanes meet all
+                // banks both ways.
+                constexpr int kHalves = D / 64;
+                const int c = lane & 3, u = (lane >> 2) & 1, kv = cw >> 1, e_first = 32 * (cw & 1) + 2 * (lane >> 3) + u;
+                const uint32_t seq = 2 * tile + kv, from = seq % C::RawSlots, st = seq % C::Slots, dst = ring + st * C::Slot;
+                if (seq >= C::Slots) wait2(raw_full + 8 * from, seq / C::RawSlots, kv_empty + 8 * st, seq / C::Slots - 1, 0, int(seq));
+                else wait(raw_full + 8 * from, seq / C::RawSlots, 0, int(seq));
+                if (!ok) break;
+                uint4 v[4][kHalves];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < 4; ++i)
 #pragma unroll
-                        for (int h = 0; h < kHalves; ++h) {
-                            const int e = 16 * cw + 8 * i + 2 * (lane >> 3) + u, ch = 4 * (kHalves > 1 ? h ^ u : 0) + c;
-                            v[i][h] = ptx::lds_v4(src + e * D + 16 * ch);
-                        }
-                    __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(raw_empty + 8 * from);
+                    for (int h = 0; h < kHalves; ++h) v[i][h] = ptx::lds_v4(raw + from * C::RawSlot + (e_first + 8 * i) * D + 16 * (4 * (kHalves > 1 ? h ^ u : 0) + c));
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int e = 16 * cw + 8 * i + 2 * (lane >> 3) + u, at = e0 + e;
-                        const bool zero = kv == 1 && !all && !(at < w.span.hi && (at >= w.span.lo || at < w.span.first));
+                for (int i = 0; i < 4; ++i) {
+                    const int e = e_first + 8 * i, at = e0 + e;
+                    const bool zero = kv == 1 && !all && !(at < w.span.hi && (at >= w.span.lo || at < w.span.first));
 #pragma unroll
-                        for (int h = 0; h < kHalves; ++h) {
-                            const int ch = 4 * (kHalves > 1 ? h ^ u : 0) + c;
-                            uint4 lo, hi;
-                            ptx::e4m3x4_to_f16x4(v[i][h].x, lo.x, lo.y);
-                            ptx::e4m3x4_to_f16x4(v[i][h].y, lo.z, lo.w);
-                            ptx::e4m3x4_to_f16x4(v[i][h].z, hi.x, hi.y);
-                            ptx::e4m3x4_to_f16x4(v[i][h].w, hi.z, hi.w);
-                            if (zero) lo = hi = make_uint4(0, 0, 0, 0);
-                            const uint32_t to = dst + (ch / 4) * (NE * 128) + e * 128;
-                            ptx::sts_v4(to + (((2 * (ch % 4)) ^ (e & 7)) << 4), lo);
-                            ptx::sts_v4(to + (((2 * (ch % 4) + 1) ^ (e & 7)) << 4), hi);
-                        }
+                    for (int h = 0; h < kHalves; ++h) {
+                        const int ch = 4 * (kHalves > 1 ? h ^ u : 0) + c;
+                        uint4 lo, hi;
+                        ptx::e4m3x4_to_f16x4(v[i][h].x, lo.x, lo.y);
+                        ptx::e4m3x4_to_f16x4(v[i][h].y, lo.z, lo.w);
+                        ptx::e4m3x4_to_f16x4(v[i][h].z, hi.x, hi.y);
+                        ptx::e4m3x4_to_f16x4(v[i][h].w, hi.z, hi.w);
+                        if (zero) lo = hi = make_uint4(0, 0, 0, 0);
+                        const uint32_t to = dst + (ch / 4) * (NE * 128) + e * 128;
+                        ptx::sts_v4(to + (((2 * (ch % 4)) ^ (e & 7)) << 4), lo);
+                        ptx::sts_v4(to + (((2 * (ch % 4) + 1) ^ (e & 7)) << 4), hi);
                     }
-                    ptx::fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(kv_full + 8 * st);
+                }
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    ptx::mbar_arrive(kv_full + 8 * st);
+                    ptx::mbar_arrive(raw_empty + 8 * from);
                 }
             }
         }
@@ -350,45 +345,45 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_rows_kernel(const __grid_co
                 const bool page = there[tile % C::Flags] != 0;
                 if (warp_real) {
                     const bool whole = page && e0 + NE - 1 <= first_place && e0 + NE <= w.req.entries && (a.window == 0 || e0 > last_place - a.window || e0 + NE <= a.first);
-                    // 32 scores at a time, in log2 units; what the row does not see is -inf
-                    auto load = [&](float (&v)[32], int c) {
-                        uint32_t u[32];
-                        ptx::tmem_ld32(s_at + 32 * c, u);
-                        uint32_t see = 0xFFFFFFFFu;
-                        if (!whole) {
+                    // the row's scores, not scaled; what it does not see is -inf
+                    uint32_t v[2][32];
+                    ptx::tmem_ld32(s_at, v[0]);
+                    ptx::tmem_ld32(s_at + 32, v[1]);
+                    ptx::tmem_wait_ld();
+                    if (!whole) {
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
                             const int from = e0 + 32 * c;
                             auto below = [](int n) { return n >= 32 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << n) - 1u; };
-                            see = below(min(place + 1, w.req.entries) - from);
+                            uint32_t see = below(min(place + 1, w.req.entries) - from);
                             if (a.window > 0) see &= ~below(place - a.window + 1 - from) | below(a.first - from);
                             if (!page) see = 0u;
-                        }
-                        ptx::tmem_wait_ld();
-#pragma unroll
-                        for (int x = 0; x < 32; ++x) v[x] = __uint_as_float(u[x]) * scale;
-                        if (!whole) {
 #pragma unroll
                             for (int x = 0; x < 32; ++x)
-                                if (!((see >> x) & 1u)) v[x] = neg;
+                                if (!((see >> x) & 1u)) v[c][x] = __float_as_uint(neg);
                         }
-                    };
-                    float v[2][32], top = neg;
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        load(v[c], c);
-#pragma unroll
-                        for (int x = 0; x < 32; x += 2) top = ptx::max3(top, v[c][x], v[c][x + 1]);
                     }
+                    float tops[4] = {neg, neg, neg, neg};
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int x = 0; x < 32; x += 8)
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) tops[q] = ptx::max3(tops[q], __uint_as_float(v[c][x + 2 * q]), __uint_as_float(v[c][x + 2 * q + 1]));
+                    const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                     if (logits != nullptr) {
 #pragma unroll
                         for (int c = 0; c < 2; ++c)
 #pragma unroll
-                            for (int x = 0; x < 32; x += 4) *reinterpret_cast<float4*>(logits + e0 + 32 * c + x) = make_float4(v[c][x], v[c][x + 1], v[c][x + 2], v[c][x + 3]);
+                            for (int x = 0; x < 32; x += 4)
+                                *reinterpret_cast<float4*>(logits + e0 + 32 * c + x) = make_float4(__uint_as_float(v[c][x]) * scale, __uint_as_float(v[c][x + 1]) * scale,
+                                                                                                  __uint_as_float(v[c][x + 2]) * scale, __uint_as_float(v[c][x + 3]) * scale);
                     }
-                    const bool move = real && (ref == neg ? top > neg : top - ref > kPrefillLazy);
+                    const bool move = real && (ref == neg ? top > neg : (top - ref) * scale > kPrefillLazy);
                     if (__any_sync(0xFFFFFFFFu, move)) {
                         float by = 1.f;
                         if (move) {
-                            if (ref != neg) by = ptx::ex2(ref - top);
+                            if (ref != neg) by = ptx::ex2((ref - top) * scale);
                             ref = top;
                             l *= by;
                         }
@@ -409,18 +404,28 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_rows_kernel(const __grid_co
                             ptx::tmem_wait_st();
                         }
                     }
-                    const float sub = ref == neg ? 0.f : ref;
+                    // Differences are taken before they are scaled: at the maximum 0, however large it is.
+                    const float sub = ref == neg ? 0.f : -ref;
+                    const uint64_t sub2 = ptx::pack_f32x2(sub, sub), scale2 = ptx::pack_f32x2(scale, scale);
+                    uint64_t s0 = ptx::pack_f32x2(l, 0.f), s1 = ptx::pack_f32x2(0.f, 0.f);
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         uint32_t pk[16];
 #pragma unroll
                         for (int x = 0; x < 32; x += 2) {
-                            const float x0 = ptx::ex2(v[c][x] - sub), x1 = ptx::ex2(v[c][x + 1] - sub);
-                            l += x0 + x1;
+                            float x0, x1;
+                            ptx::unpack_f32x2(ptx::mul_f32x2(ptx::add_f32x2(ptx::pack_f32x2(__uint_as_float(v[c][x]), __uint_as_float(v[c][x + 1])), sub2), scale2), x0, x1);
+                            x0 = ptx::ex2(x0);
+                            x1 = ptx::ex2(x1);
+                            if (x & 2) s1 = ptx::add_f32x2(s1, ptx::pack_f32x2(x0, x1));
+                            else s0 = ptx::add_f32x2(s0, ptx::pack_f32x2(x0, x1));
                             pk[x / 2] = C::BF16 ? ptx::pack_bf16x2(x0, x1) : ptx::pack_f16x2(x0, x1);
                         }
                         tmem_st16(s_at + 16 * c, pk);
                     }
+                    float a0, a1;
+                    ptx::unpack_f32x2(ptx::add_f32x2(s0, s1), a0, a1);
+                    l = a0 + a1;
                     ptx::tmem_wait_st();
                 }
                 // (a warp of rows that are none leaves whatever stands there: those rows of O are not read)
@@ -437,6 +442,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_rows_kernel(const __grid_co
                 if (!ok) break;
                 ptx::tc_fence_after_sync();
             }
+            ref = ref == neg ? neg : ref * scale;                             // (in log2 units from here on)
             const bool complete = w.k0 == 0 && w.k1 == w.span.count, mine = complete && t == 0;
             // the block's places: two pieces that a cut runs through, and the second stream's part of a unit that none does
             const int64_t part = int64_t(blockIdx.x) * (2 * NT + 1) + (complete ? 2 * NT : (w.nth > 0) * NT + t);
