@@ -144,7 +144,7 @@ bool gqa_sizes(const Dsv4GqaParams* p, Sizes& s) {
     const bool spread = (p->Hkv * p->G == 1 || p->q_stride_h > 0) && (tokens == 1 || p->q_stride_t > 0) && (p->q_start != nullptr || p->B == 1 || p->q_stride_b > 0);
     if (p->q_start == nullptr && p->G <= 128 && (spread || p->kv_dtype == DSV4_DTYPE_E4M3) && tokens * p->G > (p->kv_dtype == DSV4_DTYPE_E4M3 ? kRowsMoreE4m3 : kRowsMore)) {
         s.streams = p->D > 128 ? 1 : 2;
-        s.group_rows = 128 / p->G * p->G;
+        s.group_rows = (s.streams == 2 && tokens * p->G <= 64 ? 64 : 128) / p->G * p->G;
         const int64_t most = int64_t(p->B) * ((tokens * p->G + s.group_rows - 1) / s.group_rows) * p->Hkv * ((longest + kGqaTile - 1) / kGqaTile + 1);
         s.blocks = int(most < device_sms() ? most : device_sms());
         s.parts = int64_t(s.blocks) * (2 * s.streams + 1) * s.group_rows;
@@ -209,7 +209,8 @@ cudaError_t make_tokens_map(CUtensorMap* map, const Dsv4GqaParams* p, int tile_t
 cudaError_t decode_rows(const GqaArgs& g, const Dsv4GqaParams* p, cudaStream_t stream) {
     GqaRowsArgs a{};
     a.g = g;
-    a.tile_tokens = 128 / p->G;
+    a.tile_tokens = g.group_rows / p->G;
+    a.second = g.streams == 2 && g.group_rows <= 64 && int64_t(p->T) * p->G <= 64 ? 64 : 0;
     cudaError_t e = cudaSuccess;
     if (p->kv_dtype == DSV4_DTYPE_E4M3) {
         e = make_raw_map(&a.g.k_map, p->k_pool, p->num_pages, p->Hkv, p->D);

@@ -19,7 +19,8 @@ struct GqaRowsArgs {
     GqaArgs g;                       // group_rows: tile_tokens * G; k_map, v_map: boxes of a page (e4m3: whole rows, not swizzled)
     alignas(64) CUtensorMap q_map;   // 16 bits: (element, head, token, request)
     CUtensorMap v8_map, v1_map;      // 16 bits: boxes of eight entries and of one
-    int tile_tokens;                 // floor(128 / G)
+    int tile_tokens;                 // of a group: floor(128 / G), or floor(64 / G)
+    int second;                      // 64: the second stream has its rows there (groups of up to 64 rows: the streams' softmax warps then sit on different schedulers), or 0
 };
 
 template <int D_, int KVT_>
@@ -137,9 +138,12 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_rows_kernel(const __grid_co
             if (!C::E4M3) {
                 if (piece > 0) wait(q_empty, piece - 1, 0, int(piece));
                 if (ok && ptx::elect_one()) {
-                    ptx::mbar_arrive_expect_tx(q_full, uint32_t(p.tile_tokens * a.G * D * 2));
+                    ptx::mbar_arrive_expect_tx(q_full, uint32_t(p.tile_tokens * a.G * D * 2) * (p.second ? 2u : 1u));
 #pragma unroll
-                    for (int x = 0; x < D / 64; ++x) tma_load_4d(smem + x * (128 * 128), &p.q_map, 64 * x, w.h * a.G, w.span.t0, w.b, q_full);
+                    for (int x = 0; x < D / 64; ++x) {
+                        tma_load_4d(smem + x * (128 * 128), &p.q_map, 64 * x, w.h * a.G, w.span.t0, w.b, q_full);
+                        if (p.second) tma_load_4d(smem + x * (128 * 128) + p.second * 128, &p.q_map, 64 * x, w.h * a.G, w.span.t0, w.b, q_full);
+                    }
                 }
                 __syncwarp();
             }
@@ -255,10 +259,10 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_rows_kernel(const __grid_co
                 const int l = lane % kLanes, rows = w.req.tokens * a.G, first = w.rg * a.group_rows;
 #pragma unroll 4
                 for (int i = 0; i < 32 / kRows; ++i) {
-                    const int r = 32 * cw + i * kRows + lane / kLanes;
+                    const int r = 32 * cw + i * kRows + lane / kLanes, of = p.second > 0 && r >= p.second ? r - p.second : r;
                     uint4 v = make_uint4(0, 0, 0, 0);
-                    if (r < a.group_rows && first + r < rows) {
-                        const int t = int(uint32_t(first + r) / uint32_t(a.G)), gg = first + r - t * a.G;
+                    if (of < a.group_rows && first + of < rows) {
+                        const int t = int(uint32_t(first + of) / uint32_t(a.G)), gg = first + of - t * a.G;
                         v = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(a.q) + 2 * (int64_t(w.b) * a.q_stride_b + t * a.q_stride_t + int64_t(w.h * a.G + gg) * a.q_stride_h + 8 * l));
                     }
                     const float factor = a.q_bf16 ? gqa_near_one<kLanes>(v) : 1.f;
@@ -315,12 +319,12 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_rows_kernel(const __grid_co
         // ── softmax: a thread has a row of a stream ──
         const uint32_t t = warp >> 2;
         const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
-        const int r = (warp & 3) * 32 + lane;
+        const int at_row = (warp & 3) * 32 + lane, r = at_row - (t == 1 ? p.second : 0);      // row of the tile, and of the group
         const float neg = -INFINITY;
         uint32_t joined = 0;                                                  // units that both streams have joined
         for (; w.left > 0 && ok; w.next(a), ++piece) {
             const int rows = w.req.tokens * a.G, row = w.rg * a.group_rows + r;
-            const bool real = r < a.group_rows && row < rows;
+            const bool real = r >= 0 && r < a.group_rows && row < rows;
             const int token = real ? int(uint32_t(row) / uint32_t(a.G)) : w.span.t1, place = w.req.place0 + token;
             const int first_place = w.req.place0 + w.span.t0, last_place = w.req.place0 + w.span.t1;
             const bool warp_real = __any_sync(0xFFFFFFFFu, real);
@@ -328,7 +332,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_rows_kernel(const __grid_co
             // (without the wait a stream that has no tile of a piece would arrive for the next one too early)
             wait(q_full, piece, 2, int(piece));
             if (!ok) break;
-            if (C::E4M3) scale *= row_factor[r];
+            if (C::E4M3) scale *= row_factor[at_row];
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(q_empty);                         // (its factors have been read)
             float* const logits = a.logits != nullptr && real ? a.logits + ((int64_t(w.b) * a.Hkv + w.h) * rows + row) * a.logit_stride : nullptr;
