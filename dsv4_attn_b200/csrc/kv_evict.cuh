@@ -122,6 +122,16 @@ __global__ void __launch_bounds__(kEvictPlanThreads) evict_plan_kernel(const __g
         if (want == 0) {
             threshold = 0xFFFFFFFFu;                              // (no key is that large)
         } else {
+            // (a request of up to 4096 others: their keys stay in registers)
+            uint32_t keys[kEvictEach];
+            const bool few = hi - lo <= kEvictPlanThreads * kEvictEach;
+            if (few) {
+#pragma unroll
+                for (int i = 0; i < kEvictEach; ++i) {
+                    const int j = lo + i * kEvictPlanThreads + tid;
+                    keys[i] = j < hi ? evict_key(ptx::ld(weights + j)) : 0u;
+                }
+            }
             int shift = 32;
 #pragma unroll 1
             for (int pass = 0; pass < 3; ++pass) {
@@ -130,6 +140,11 @@ __global__ void __launch_bounds__(kEvictPlanThreads) evict_plan_kernel(const __g
                 shift -= bits;
                 for (int i = tid; i < kEvictBins; i += kEvictPlanThreads) bins[i] = 0;
                 __syncthreads();
+                if (few) {
+#pragma unroll
+                    for (int i = 0; i < kEvictEach; ++i)
+                        if (lo + i * kEvictPlanThreads + tid < hi && (pass == 0 || (keys[i] >> above) == prefix)) atomicAdd(&bins[(keys[i] >> shift) & ((1u << bits) - 1u)], 1u);
+                } else
 #pragma unroll 4
                 for (int j = lo + tid; j < hi; j += kEvictPlanThreads) {
                     const uint32_t key = evict_key(ptx::ld(weights + j));
@@ -211,18 +226,31 @@ __global__ void __launch_bounds__(kEvictPlanThreads) evict_plan_kernel(const __g
     const int new_len = done ? length : n, changed = done ? change : n, held = (new_len + 63) / 64;
     __syncthreads();
     // weights and sources, in steps: a step's reads lie at or behind its writes
-    for (int j0 = 0; j0 < a.weight_stride; j0 += kEvictPlanThreads) {
-        const int64_t j = int64_t(j0) + tid;
-        float w = 0.f;
-        if (j < new_len) {
-            const int old = kept[j];
-            w = ptx::ld(weights + old);
-            if (j >= changed) from[j] = ptx::ld(table + (old >> 6)) * 64 + (old & 63);
-        } else if (j < cap) {
-            kept[j] = -1;
+    for (int64_t j0 = 0; j0 < a.weight_stride; j0 += kEvictPlanThreads * kEvictEach) {
+        int old[kEvictEach], page[kEvictEach];
+        float w[kEvictEach];
+#pragma unroll
+        for (int i = 0; i < kEvictEach; ++i) {
+            const int64_t j = j0 + i * kEvictPlanThreads + tid;
+            old[i] = j < new_len ? kept[j] : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < kEvictEach; ++i) {
+            const int64_t j = j0 + i * kEvictPlanThreads + tid;
+            w[i] = old[i] >= 0 ? ptx::ld(weights + old[i]) : 0.f;
+            page[i] = old[i] >= 0 && j >= changed ? ptx::ld(table + (old[i] >> 6)) : 0;
         }
         __syncthreads();
-        if (j < a.weight_stride) new_weights[j] = w;
+#pragma unroll
+        for (int i = 0; i < kEvictEach; ++i) {
+            const int64_t j = j0 + i * kEvictPlanThreads + tid;
+            if (j < a.weight_stride) new_weights[j] = w[i];
+            if (old[i] >= 0) {
+                if (j >= changed) from[j] = page[i] * 64 + (old[i] & 63);
+            } else if (j < cap) {
+                kept[j] = -1;
+            }
+        }
     }
     // pages given back: their numbers are kept for the kernel that moves, behind the sources
     for (int s0 = 0; s0 < a.max_pages; s0 += kEvictPlanThreads) {
