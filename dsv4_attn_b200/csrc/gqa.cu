@@ -35,17 +35,27 @@ cudaError_t ensure_smem(Kernel kernel, int bytes, std::atomic<bool>* done_per_de
 
 // Every kernel is a programmatic dependent of whatever precedes it in the stream, as in api.cu.
 template <class Args>
-cudaError_t launch(void (*kernel)(Args), dim3 grid, int threads, size_t smem, cudaStream_t stream, const Args& args) {
+cudaError_t launch(void (*kernel)(Args), dim3 grid, int threads, size_t smem, cudaStream_t stream, const Args& args, int cluster = 0) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1] = {};
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2] = {};
+    unsigned used = 0;
+    if (cluster > 0) {
+        attr[used].id = cudaLaunchAttributeClusterDimension;
+        attr[used].val.clusterDim.x = unsigned(cluster);
+        attr[used].val.clusterDim.y = attr[used].val.clusterDim.z = 1;
+        ++used;
+    }
+    if (!(host_state().flags & 64)) {
+        attr[used].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[used].val.programmaticStreamSerializationAllowed = 1;
+        ++used;
+    }
     cfg.attrs = attr;
-    cfg.numAttrs = (host_state().flags & 64) ? 0 : 1;
+    cfg.numAttrs = used;
     return cudaLaunchKernelEx(&cfg, kernel, args);
 }
 
@@ -81,13 +91,15 @@ cudaError_t make_raw_map(CUtensorMap* map, const void* pool, int64_t pages, int 
 // Rows of a KV head: 16, 32 or 64 in a group, the fewest that hold a request's (with 64: several groups).
 int group_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
 constexpr int kMinShare = 2;
+// A cluster's parts are joined in one kernel, which is worth some tiles that shares would have spread over more blocks.
+constexpr int kClusterTiles = 12;
 
 template <class C>
 cudaError_t run_decode(GqaArgs& a, cudaStream_t stream) {
     static std::atomic<bool> done[kMaxDevices];
     cudaError_t e = ensure_smem(gqa_decode_kernel<C>, C::Bytes, done);
     if (e != cudaSuccess) return e;
-    return launch(gqa_decode_kernel<C>, dim3(unsigned(a.blocks)), kGqaThreads, C::Bytes, stream, a);
+    return launch(gqa_decode_kernel<C>, dim3(unsigned(a.blocks)), kGqaThreads, C::Bytes, stream, a, a.cluster);
 }
 template <int D, int KVT>
 cudaError_t run_decode(GqaArgs& a, cudaStream_t stream) {
@@ -109,6 +121,7 @@ struct Sizes {
     int64_t logit_rows, logit_stride;
     bool prefill;                    // gqa_prefill_kernel
     int streams;                     // gqa_rows_kernel, if not 0
+    int cluster;                     // blocks of a cluster that has a unit, or 0: shares
     int64_t plan_words;
     int64_t own_rows;                // entries of the call's own 16-bit pages
 };
@@ -135,6 +148,17 @@ bool gqa_sizes(const Dsv4GqaParams* p, Sizes& s) {
     const int64_t resident = int64_t(device_sms()) * gqa_blocks_per_sm(p->D), want = (tiles + kMinShare - 1) / kMinShare;
     s.blocks = int(want < resident ? want : resident);
     s.parts = 2 * int64_t(s.blocks) * s.group_rows;
+    s.cluster = 0;
+    if (p->q_start == nullptr && tokens * p->G <= s.group_rows) {
+        // the widest cluster with which all units are resident at once, where no block of it can have more than kClusterTiles tiles
+        const int64_t units = int64_t(p->B) * p->Hkv, most = (longest + kGqaTile - 1) / kGqaTile + 1;
+        for (int c = 8; c > 1 && s.cluster == 0; c /= 2)
+            if (units * c <= resident && most <= int64_t(c) * kClusterTiles) s.cluster = c;
+        if (s.cluster > 0) {
+            s.blocks = int(units) * s.cluster;
+            s.parts = 0;
+        }
+    }
     s.logit_rows = p->weights != nullptr ? int64_t(p->B) * p->Hkv * p->T * p->G : 0;
     s.logit_stride = entries;
     s.prefill = false;
@@ -144,6 +168,7 @@ bool gqa_sizes(const Dsv4GqaParams* p, Sizes& s) {
     const bool spread = (p->Hkv * p->G == 1 || p->q_stride_h > 0) && (tokens == 1 || p->q_stride_t > 0) && (p->q_start != nullptr || p->B == 1 || p->q_stride_b > 0);
     if (p->q_start == nullptr && p->G <= 128 && (spread || p->kv_dtype == DSV4_DTYPE_E4M3) && tokens * p->G > (p->kv_dtype == DSV4_DTYPE_E4M3 ? kRowsMoreE4m3 : kRowsMore)) {
         s.streams = p->D > 128 ? 1 : 2;
+        s.cluster = 0;
         s.group_rows = (s.streams == 2 && tokens * p->G <= 64 ? 64 : 128) / p->G * p->G;
         const int64_t most = int64_t(p->B) * ((tokens * p->G + s.group_rows - 1) / s.group_rows) * p->Hkv * ((longest + kGqaTile - 1) / kGqaTile + 1);
         s.blocks = int(most < device_sms() ? most : device_sms());
@@ -288,7 +313,7 @@ using namespace dsv4;
 extern "C" int64_t dsv4_gqa_workspace_bytes(const Dsv4GqaParams* p) {
     Sizes s;
     if (!gqa_sizes(p, s)) return -1;
-    return up(s.parts * p->D * 4) + up(s.parts * 4) + up(s.logit_rows * s.logit_stride * 4) + up(s.logit_rows * 4) + up(s.plan_words * 4) + 2 * up(s.own_rows * p->Hkv * p->D * 2);
+    return 128 + up(s.parts * p->D * 4) + up(s.parts * 4) + up(s.logit_rows * s.logit_stride * 4) + up(s.logit_rows * 4) + up(s.plan_words * 4) + 2 * up(s.own_rows * p->Hkv * p->D * 2);
 }
 
 static int gqa_fwd(const Dsv4GqaParams* p, void* stream_) {
@@ -332,6 +357,7 @@ static int gqa_fwd(const Dsv4GqaParams* p, void* stream_) {
     a.status = p->status;
     if (s.prefill) return int(prefill(a, p, s, ws, stream));
     a.streams = s.streams;
+    a.cluster = s.cluster;
     cudaError_t e = cudaSuccess;
     if (s.streams > 0) {
         e = decode_rows(a, p, stream);
@@ -343,7 +369,7 @@ static int gqa_fwd(const Dsv4GqaParams* p, void* stream_) {
     }
     if (e != cudaSuccess) return int(e);
     const int64_t merge_rows = p->rows * p->Hkv * p->G, merge_blocks = (merge_rows + kGqaMergeRows - 1) / kGqaMergeRows;
-    if (s.blocks > 1 || s.streams > 0) {
+    if (s.cluster == 0 && (s.blocks > 1 || s.streams > 0)) {
         const dim3 grid{unsigned(merge_blocks)};
         e = p->D == 64 ? launch(gqa_merge_kernel<64>, grid, kGqaMergeThreads, 0, stream, a)
                        : p->D == 128 ? launch(gqa_merge_kernel<128>, grid, kGqaMergeThreads, 0, stream, a) : launch(gqa_merge_kernel<256>, grid, kGqaMergeThreads, 0, stream, a);

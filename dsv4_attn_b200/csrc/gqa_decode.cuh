@@ -55,6 +55,7 @@ struct GqaArgs {
     float* part_lse;                 // [2 * blocks][R], log2
     int blocks;                      // of the attention kernel
     int group_rows;                  // R
+    int cluster;                     // blocks of a cluster that has a unit to itself, or 0: shares
     int one_group;                   // not packed, and a request's rows of a KV head fit a group
     int min_share;                   // tiles of a block, at least
     int streams;                     // parts that a block leaves of a piece (gqa_rows_kernel; and a place more), or 0: one
@@ -292,6 +293,11 @@ struct GqaWalk {
     }
 };
 
+__device__ __forceinline__ float4 gqa_cluster_v4(uint32_t caddr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(caddr) : "memory");
+    return v;
+}
 // Four columns, from x on, of a complete row: v = sum of exp2(x_j - top) v_j, sum = sum of exp2(x_j - top).
 template <int D>
 __device__ __forceinline__ void gqa_write_row(const GqaArgs& a, int64_t token, int head, int64_t weight_row, int x, const float4& v, float top, float sum, float v_scale) {
@@ -341,6 +347,23 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
     ptx::pdl_trigger();
     ptx::pdl_wait();
 
+    GqaWalk w;
+    uint32_t rank = 0;
+    if (a.cluster > 0) {
+        // Small calls: a cluster has a unit to itself, and its blocks' parts are joined through distributed shared memory: no scan over the lengths, and no second kernel.
+        const uint32_t unit = blockIdx.x / uint32_t(a.cluster);
+        rank = blockIdx.x - unit * uint32_t(a.cluster);
+        w.b = int(unit / uint32_t(a.Hkv));
+        w.h = int(unit) - w.b * a.Hkv;
+        w.rg = w.nth = 0;
+        w.req = gqa_request(a, w.b);
+        w.span = gqa_span(a, w.req, 0);
+        w.k0 = int(uint32_t(w.span.count) * rank / uint32_t(a.cluster));
+        w.k1 = int(uint32_t(w.span.count) * (rank + 1) / uint32_t(a.cluster));
+        w.left = w.k1 - w.k0;
+        if (w.req.bad && tid == 0 && w.h == 0 && rank == 0) gqa_report(a.status, kGqaStatusBadIndex, 4, w.b);
+        __syncthreads();                                                      // (the barriers have been initialised)
+    } else {
     // where this block's share begins
     const int each = (a.B + kGqaThreads - 1) / kGqaThreads, b_from = tid * each, b_to = min(b_from + each, a.B);
     int64_t mine = 0, total;
@@ -366,8 +389,8 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
         }
     }
     __syncthreads();
-    GqaWalk w;
     w.begin(a, int(scan[5]), scan[6], tiles);
+    }
 
     if (warp == 4) {
         // ── producer ──
@@ -414,6 +437,10 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
             // copies that are on their way land within microseconds
             const uint32_t t0 = ptx::globaltimer_lo();
             while (ptx::globaltimer_lo() - t0 < 1000000u) __nanosleep(1000);
+        }
+        if (a.cluster > 0) {
+            ptx::cluster_sync();                                              // (the parts are there; they have been read)
+            ptx::cluster_sync();
         }
         return;
     }
@@ -722,6 +749,8 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
         ptx::bar_sync(1, kGqaConsumers);
         constexpr int kLanes = D / 4;
         const int x = 4 * (tid % kLanes);
+        // a cluster's block leaves its joined part in the ring, which is idle: [R][D], then a maximum and a sum a row
+        float* const joined = reinterpret_cast<float*>(base);
 #pragma unroll 2
         for (int r = tid / kLanes; r < R; r += kGqaConsumers / kLanes) {
             const int of_wm = r >> 4, rl = r & 15, row = row_first + r;
@@ -738,6 +767,11 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
                 const float4 u = *reinterpret_cast<const float4*>(merge + at * C::MergePitch + x);
                 v.x += u.x;  v.y += u.y;  v.z += u.z;  v.w += u.w;
             }
+            if (a.cluster > 0) {
+                *reinterpret_cast<float4*>(joined + r * D + x) = v;
+                if (x == 0) *reinterpret_cast<float2*>(joined + R * D + 2 * r) = make_float2(top, sum);
+                continue;
+            }
             if (!complete) {
                 const float per = sum == 0.f ? 0.f : 1.f / sum;
                 *reinterpret_cast<float4*>(a.part_o + (part * R + r) * D + x) = make_float4(v.x * per, v.y * per, v.z * per, v.w * per);
@@ -746,7 +780,42 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
             }
             gqa_write_row<D>(a, w.req.row0 + token, w.h * a.G + row - token * a.G, (int64_t(w.b) * a.Hkv + w.h) * rows + row, x, v, top, sum, v_scale);
         }
+        if (a.cluster > 0) break;
     }
+    if (a.cluster == 0) return;
+    // ── the cluster's blocks share out the rows ──
+    ptx::cluster_sync();
+    const int rows = w.req.tokens * a.G;
+    constexpr int kLanes = D / 4;
+    const uint32_t part = smem;                                               // the same place in every block
+    const float v_scale = a.v_scale != nullptr ? ptx::ld(a.v_scale + w.h) : 1.f;
+    for (uint32_t at = rank * kGqaConsumers + tid; at < uint32_t(rows) * kLanes; at += uint32_t(a.cluster) * kGqaConsumers) {
+        const int row = int(at) / kLanes, x = 4 * (int(at) % kLanes), token = int(uint32_t(row) / uint32_t(a.G));
+        float top = -INFINITY, sum = 0.f, by_of[8], sum_of[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            by_of[i] = -INFINITY;
+            sum_of[i] = 0.f;
+            // (a block without tiles has left nothing)
+            if (i < a.cluster && int(uint32_t(w.span.count) * (i + 1) / uint32_t(a.cluster)) > int(uint32_t(w.span.count) * i / uint32_t(a.cluster))) {
+                const uint32_t from = ptx::mapa(part + (R * D + 2 * row) * 4, i);
+                by_of[i] = __uint_as_float(ptx::lds_cluster_u32(from));
+                sum_of[i] = __uint_as_float(ptx::lds_cluster_u32(from + 4));
+            }
+            top = fmaxf(top, by_of[i]);
+        }
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (i >= a.cluster || sum_of[i] == 0.f) continue;
+            const float by = by_of[i] == -INFINITY ? 1.f : ptx::ex2(by_of[i] - top);       // (a NaN row has a maximum of -inf and a NaN sum)
+            sum = fmaf(sum_of[i], by, sum);
+            const float4 u = gqa_cluster_v4(ptx::mapa(part + (row * D + x) * 4, i));
+            v.x = fmaf(u.x, by, v.x);  v.y = fmaf(u.y, by, v.y);  v.z = fmaf(u.z, by, v.z);  v.w = fmaf(u.w, by, v.w);
+        }
+        gqa_write_row<D>(a, w.req.row0 + token, w.h * a.G + row - token * a.G, (int64_t(w.b) * a.Hkv + w.h) * rows + row, x, v, top, sum, v_scale);
+    }
+    ptx::cluster_sync();
 }
 
 // ── parts of units that a cut ran through ──
