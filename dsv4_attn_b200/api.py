@@ -844,7 +844,7 @@ def _gqa(what, q, q_start, k_pool, v_pool, block_table, kv_len, sm_scale, window
     _check(q.shape[-1] == D, f"q's last dim must be the pools' head_dim {D}")
     _check(D in (64, 128, 256), f"head_dim must be 64, 128 or 256, got {D}")
     _check(H > 0 and H % Hkv == 0, "q's heads must be a multiple of the pools'")
-    _check(float(sm_scale) > 0, "sm_scale must be positive")
+    _check(0 < float(sm_scale) < float("inf"), "sm_scale must be positive and finite")
     for name, x in (("window", window), ("first", first), ("max_len", 0 if max_len is None else max_len)):
         _check(type(x) is int and 0 <= x < 1 << 31, f"{name} must be an int in [0, 2^31)")
     if attn_sink is not None:

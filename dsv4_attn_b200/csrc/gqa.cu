@@ -5,6 +5,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 #include <atomic>
+#include <cmath>
 
 #include "gqa_decode.cuh"
 #include "gqa_prefill.cuh"
@@ -327,7 +328,7 @@ static int gqa_fwd(const Dsv4GqaParams* p, void* stream_) {
     if (!gqa_sizes(p, s)) return int(cudaErrorInvalidValue);
     const bool e4m3 = p->kv_dtype == DSV4_DTYPE_E4M3;
     if ((p->q_dtype != DSV4_DTYPE_BF16 && p->q_dtype != DSV4_DTYPE_F16) || (!e4m3 && p->kv_dtype != p->q_dtype)) return int(cudaErrorInvalidValue);
-    if (p->num_pages <= 0 || p->num_pages * kGqaTile > 0x7FFFFFFF - kGqaTile || p->window < 0 || p->first < 0 || !(p->sm_scale > 0.f)) return int(cudaErrorInvalidValue);
+    if (p->num_pages <= 0 || p->num_pages * kGqaTile > 0x7FFFFFFF - kGqaTile || p->window < 0 || p->first < 0 || !(p->sm_scale > 0.f) || !(p->sm_scale < INFINITY)) return int(cudaErrorInvalidValue);
     if (!p->q || !p->k_pool || !p->v_pool || !p->block_table || !p->kv_len || !p->out || (e4m3 && (!p->k_scale || !p->v_scale))) return int(cudaErrorInvalidValue);
     if (p->q_start == nullptr && p->rows != int64_t(p->B) * p->T) return int(cudaErrorInvalidValue);
     if (!aligned(p->q, 16) || !aligned(p->k_pool, 16) || !aligned(p->v_pool, 16) || !aligned(p->out, 16)) return int(cudaErrorInvalidValue);

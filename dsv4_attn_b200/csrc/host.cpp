@@ -11,6 +11,7 @@
 #include <Python.h>
 
 #include <algorithm>
+#include <limits>
 
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
@@ -764,7 +765,7 @@ PyObject* gqa(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t H = q->size(-2), T = packed ? 0 : q->size(1), rows = packed ? q->size(0) : B * T;
     if (q->size(-1) != pool.D || H <= 0 || H % pool.Hkv != 0 || !fits32(H) || !fits32(T)) return none();
     int64_t window, first, max_len = 0;
-    if (!number(a[6], &p.sm_scale) || !integer(a[7], &window) || !integer(a[8], &first) || window < 0 || first < 0 || !fits32(window) || !fits32(first)) return none();
+    if (!number(a[6], &p.sm_scale) || !(p.sm_scale > 0.f) || !(p.sm_scale <= std::numeric_limits<float>::max()) || !integer(a[7], &window) || !integer(a[8], &first) || window < 0 || first < 0 || !fits32(window) || !fits32(first)) return none();
     if (a[13] != Py_None && (!integer(a[13], &max_len) || max_len < 0 || !fits32(max_len))) return none();
     if (!optional_tensor(a[11], at::kFloat, 1, &sink) || !has_shape(sink, {H}) || !optional_tensor(a[12], at::kFloat, 2, &weights)) return none();
     if (weights != nullptr && (packed || weights->size(0) != B || weights->size(1) < pool.table->size(1) * kPage)) return none();

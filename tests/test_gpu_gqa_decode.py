@@ -27,6 +27,29 @@ def test_lengths_around_tiles(lib, dtype, D):
     assert st.tolist() == [0, 0, 0, 0]
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_lengths_in_wide_tables(lib, dtype, D):
+    """Tables with room for far more than the lengths: the cache is shared out over resident blocks instead of clusters."""
+    for kw in (dict(G=4), dict(G=20), dict(G=3, window=70, first=2)):
+        c = Case([1, 64, 65, 129, 0, 1000, 63], 1, Hkv=2, D=D, dtype=dtype, seed=D, width=200, **kw)
+        c.check(*c.call(lib))
+    st = lib.new_status("cuda")
+    c = Case([700, 2], 1, Hkv=1, G=1, D=D, dtype=dtype, width=300)
+    c.check(*c.call(lib, max_len=700, status=st))        # (steers the launch)
+    w = torch.zeros(2, 300 * PAGE, device="cuda")
+    c.check(*c.call(lib, weights=w, status=st), w, torch.zeros_like(w))
+    assert st.tolist() == [0, 0, 0, 0]
+
+
+@pytest.mark.parametrize("B,Hkv", [(1, 1), (4, 8), (9, 8), (30, 4), (70, 2), (148, 1), (300, 1)])
+def test_clusters_of_all_widths(lib, B, Hkv):
+    """Eight, four and two blocks a unit, and none; units with fewer tiles than blocks."""
+    for D in (64, 256):
+        c = Case([(37 * b) % 600 for b in range(B)], 1, Hkv=Hkv, G=2, D=D, dtype="f16", seed=B)
+        c.check(*c.call(lib))
+
+
 @pytest.mark.parametrize("Hkv,G,T", [(1, 1, 1), (1, 16, 1), (3, 5, 1), (8, 1, 1), (2, 7, 3), (1, 17, 1), (2, 8, 4), (1, 33, 1), (1, 64, 1), (2, 16, 5), (1, 8, 40), (1, 100, 1)])
 @pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
 def test_heads_and_tokens(lib, Hkv, G, T, dtype):
@@ -188,9 +211,10 @@ def test_pages_out_of_range_are_left_out_and_reported(lib):
     assert st[0] == 0 and (out[0] == 0).all() and torch.isneginf(lse[0]).all()
 
 
+@pytest.mark.parametrize("width", [0, 400])
 @pytest.mark.parametrize("G,dtype", [(4, "f16"), (4, "e4m3"), (40, "f16"), (40, "e4m3")])
-def test_a_wait_that_runs_out(lib, G, dtype):
-    c = Case([3000, 200], 1, Hkv=2, G=G, D=64, dtype=dtype)
+def test_a_wait_that_runs_out(lib, G, dtype, width):
+    c = Case([3000, 200], 1, Hkv=2, G=G, D=64, dtype=dtype, width=width)
     st = lib.new_status("cuda")
     lib.LIB.dsv4_debug_set_wait(200_000, 1)
     try:
@@ -261,3 +285,56 @@ def test_prefill_small(lib):
         for window, first in ((0, 0), (40, 3)):
             c = Case([5, 70, 200, 1, 300], [5, 6, 150, 1, 0], Hkv=2, G=3, D=D, dtype=dtype, packed=True, window=window, first=first, sink=True)
             c.check(*c.call(lib))
+
+
+def test_refusals(lib):
+    """What is not a call says so, and launches nothing."""
+    c = Case([100, 65], 1, Hkv=2, G=4, D=128, dtype="bf16")
+    q, k, v, table, n = c.q, *c.pools, c.table, c.len_t
+    w = torch.zeros(2, table.shape[1] * PAGE, device="cuda")
+    ok = dict(q=q, k_pool=k, v_pool=v, block_table=table, kv_len=n, sm_scale=0.1)
+
+    def refused(what, **kw):
+        with pytest.raises((ValueError, lib.Dsv4Error), match=what):
+            lib.gqa_decode(**dict(ok, **kw))
+    refused("q must be \\[B, T", q=q[0])
+    refused("bf16 or f16", q=q.float())
+    refused("strides of q", q=torch.zeros(2, 1, 8, 132, device="cuda", dtype=torch.bfloat16)[..., :128])
+    refused("16-byte", q=torch.zeros(2 * 1024 + 1, device="cuda", dtype=torch.bfloat16)[1:].reshape(2, 1, 8, 128))
+    refused("head_dim", q=q[..., :64])
+    refused("multiple of the pools'", q=q[:, :, :7])
+    refused("kv_len must be", kv_len=n[:1])
+    refused("int32", kv_len=n.long())
+    refused("block_table", block_table=table[:1])
+    refused("one shape", v_pool=v[:1])
+    refused("contiguous", k_pool=k.transpose(1, 2))
+    refused("pools must be", k_pool=k.half(), v_pool=v.half())
+    refused("k_scale goes with", k_scale=torch.ones(2, device="cuda"))
+    refused("k_scale goes with", k_pool=k.to(torch.float8_e4m3fn), v_pool=v.to(torch.float8_e4m3fn))
+    refused("sm_scale", sm_scale=0.0)
+    refused("sm_scale", sm_scale=float("inf"))
+    refused("sm_scale", sm_scale=float("nan"))
+    refused("window", window=-1)
+    refused("first", first=1 << 31)
+    refused("max_len", max_len=-1)
+    refused("attn_sink", attn_sink=torch.zeros(7, device="cuda"))
+    refused("weights", weights=w[:, :-1])
+    refused("out must", out=torch.empty(2, 1, 8, 64, device="cuda", dtype=torch.bfloat16))
+    refused("lse must", lse=torch.empty(2, 8, device="cuda"))
+    refused("status", status=torch.zeros(2, device="cuda", dtype=torch.int32))
+    x = torch.zeros(2, PAGE, 2, 96, device="cuda", dtype=torch.bfloat16)
+    refused("64, 128 or 256", q=q[..., :96].contiguous(), k_pool=x, v_pool=x)
+    with pytest.raises(ValueError, match="q_start must be"):
+        lib.gqa_prefill(q[:, 0], torch.zeros(2, device="cuda", dtype=torch.int32), k, v, table, n, 0.1)
+    with pytest.raises(ValueError, match="n_rows goes with"):
+        lib.gqa_insert(k[:2, 0], v[:2, 0], k, v, table, n, q_start=torch.zeros(3, device="cuda", dtype=torch.int32), n_rows=n)
+    with pytest.raises(ValueError, match="heads and head_dim"):
+        lib.gqa_insert(q[:, :, :1], q[:, :, :1], k, v, table, n)
+    refs = torch.ones(k.shape[0], device="cuda", dtype=torch.int32)
+    for match, kw in (("keep must be", dict(keep=-1)), ("first must be", dict(first=-1)), ("weights must be", dict(weights=w[:, 1:])), ("pools must be", dict(pools=())),
+                      ("16 bytes", dict(pools=torch.zeros(1, k.shape[0], PAGE, 7, device="cuda", dtype=torch.bfloat16))), ("page_refs", dict(page_refs=refs.long())),
+                      ("a pool must be|pools must be", dict(pools=(k, v))), ("new_len", dict(new_len=n.long()))):
+        a = dict(dict(pools=(k[None], v[None]), block_table=table, kv_len=n, page_refs=refs, weights=w, keep=10), **kw)
+        with pytest.raises(ValueError, match=match):
+            lib.kv_evict(**a)
+    c.check(*c.call(lib))
