@@ -97,9 +97,11 @@ cudaError_t make_raw_map(CUtensorMap* map, const void* pool, int64_t pages, int 
 // ── which form of the kernel ──
 // Rows of a KV head: 16, 32 or 64 in a group, the fewest that hold a request's (with 64: several groups).
 int group_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
-constexpr int kMinShare = 2;
-// A cluster's parts are joined in one kernel, which is worth some tiles that shares would have spread over more blocks.
-constexpr int kClusterTiles = 12;
+constexpr int kMinShare = 2;         // tiles (one request of 2,000 entries: 12.3 us, with 1 15, with 4 13.8)
+// A cluster's parts are joined in one kernel, which is worth kClusterMore tiles that shares would have spread over more blocks (heads of 128, 16 bits): eight units, 4 tiles a block of a cluster against
+// 0.7 of a share 9.3 against 9.7 us, 8 against 1.7 13.9 against 12.3; 32 units, 16 against 13.8 27.6 against 35; 128 units, 32 against 28 45 against 54.  Beyond kClusterTiles lengths that differ,
+// which shares even out, cost more than that.  Of rows: 24 of one request's 1,000 entries 11 us in clusters against 13 in gqa_rows_kernel, 40 18 against 13.
+constexpr int kClusterMore = 5, kClusterTiles = 32, kClusterRows = 32;
 
 template <class C>
 cudaError_t run_decode(GqaArgs& a, cudaStream_t stream) {
@@ -134,12 +136,15 @@ struct Sizes {
 };
 
 // ── which kernel takes tokens that are not packed ──
-// Rows of a KV head beyond which gqa_rows_kernel takes them.
-constexpr int kRowsMore = 32, kRowsMoreE4m3 = 16;
+// Rows of a KV head beyond which gqa_rows_kernel takes them: 64 requests x 8,000 entries, heads of 128, 16 rows 322 us in gqa_decode_kernel against 336, 20 rows 359 against 339; in 8 bits 248
+// against 347 and 424 against 355.  Short 16-bit rows: 32 rows of 64 elements 246 against 265.
+constexpr int kRowsMore = 16, kRowsMore64 = 32;
 
 // ── which kernel takes a prompt ──
-// A block of tokens is 256 rows (heads of 256: 128) in gqa_prefill_kernel, and takes at least a block of the GPU to itself; the decode kernel takes 64 rows at a time and shares the entries out.
-constexpr int kPrefillMinUnits = 8, kPrefillMinRows = 64;
+// A block of tokens is 256 rows (heads of 256: 128) in gqa_prefill_kernel and has an SM to itself, where a step of 64 entries takes 1 us; the decode kernel takes 64 rows at a time, 2 us for that, and shares
+// the entries out over all SMs, for 10 us more.  Eight heads, one prompt behind a cache of 2,048 entries: 64 tokens 46 us in gqa_prefill_kernel and 33 in the other, 128 46 and 57; of 16,384:
+// 128 tokens 254 and 192, 256 260 and 355.
+constexpr int kPrefillMinUnits = 8, kPrefillStep = 10, kPrefillTile = 20, kPrefillMore = 100;      // 0.1 us
 constexpr int64_t kPrefillOwnBytes = int64_t(4) << 30;              // an 8-bit cache's pages are brought to 16 bits in a workspace of that size at most
 bool gqa_sizes(const Dsv4GqaParams* p, Sizes& s) {
     if (p == nullptr || p->B <= 0 || p->Hkv <= 0 || p->G <= 0 || p->max_pages <= 0 || p->T < 0 || p->rows < 0) return false;
@@ -156,12 +161,16 @@ bool gqa_sizes(const Dsv4GqaParams* p, Sizes& s) {
     s.blocks = int(want < resident ? want : resident);
     s.parts = 2 * int64_t(s.blocks) * s.group_rows;
     s.cluster = 0;
-    if (p->q_start == nullptr && tokens * p->G <= s.group_rows) {
-        // the widest cluster with which all units are resident at once, where no block of it can have more than kClusterTiles tiles
+    if (p->q_start == nullptr && tokens * p->G <= kClusterRows) {
+        // the widest cluster with which all units are resident at once
         const int64_t units = int64_t(p->B) * p->Hkv, most = (longest + kGqaTile - 1) / kGqaTile + 1;
-        for (int c = 8; c > 1 && s.cluster == 0; c /= 2)
-            if (units * c <= resident && most <= int64_t(c) * kClusterTiles) s.cluster = c;
-        if (s.cluster > 0) {
+        int c = 8;
+        while (c > 1 && units * c > resident) c /= 2;
+        // (with one block an SM clusters of eight do not come to lie side by side on all of them: 16 units of 256 elements 17 us, in shares 12; eight 9 against 11)
+        if (c == 8 && p->D > 128 && units * 16 > resident) c = 4;
+        const int64_t each = (most + c - 1) / c;
+        if (c > 1 && each <= kClusterTiles && each - units * most / resident <= kClusterMore - (tokens * p->G > 16)) {
+            s.cluster = c;
             s.blocks = int(units) * s.cluster;
             s.parts = 0;
         }
@@ -173,9 +182,8 @@ bool gqa_sizes(const Dsv4GqaParams* p, Sizes& s) {
     s.streams = 0;
     // (tensor maps have no axis that stays where it is)
     const bool spread = (p->Hkv * p->G == 1 || p->q_stride_h > 0) && (tokens == 1 || p->q_stride_t > 0) && (p->q_start != nullptr || p->B == 1 || p->q_stride_b > 0);
-    if (p->q_start == nullptr && p->G <= 128 && (spread || p->kv_dtype == DSV4_DTYPE_E4M3) && tokens * p->G > (p->kv_dtype == DSV4_DTYPE_E4M3 ? kRowsMoreE4m3 : kRowsMore)) {
+    if (p->q_start == nullptr && s.cluster == 0 && p->G <= 128 && (spread || p->kv_dtype == DSV4_DTYPE_E4M3) && tokens * p->G > (p->kv_dtype != DSV4_DTYPE_E4M3 && p->D == 64 ? kRowsMore64 : kRowsMore)) {
         s.streams = p->D > 128 ? 1 : 2;
-        s.cluster = 0;
         s.group_rows = (s.streams == 2 && tokens * p->G <= 64 ? 64 : 128) / p->G * p->G;
         const int64_t most = int64_t(p->B) * ((tokens * p->G + s.group_rows - 1) / s.group_rows) * p->Hkv * ((longest + kGqaTile - 1) / kGqaTile + 1);
         s.blocks = int(most < device_sms() ? most : device_sms());
@@ -186,7 +194,10 @@ bool gqa_sizes(const Dsv4GqaParams* p, Sizes& s) {
         const int64_t blocks = p->rows / block_tokens + p->B, full = (p->rows + block_tokens - 1) / block_tokens;
         const bool e4m3 = p->kv_dtype == DSV4_DTYPE_E4M3;
         const int64_t own = e4m3 ? int64_t(p->B) * p->max_pages * kGqaTile : 0;
-        s.prefill = full * p->Hkv >= kPrefillMinUnits && p->rows * p->G >= int64_t(p->B) * kPrefillMinRows && own * p->Hkv * p->D * 4 <= kPrefillOwnBytes && own < 0x7FFFFF00;
+        const int64_t steps = (longest + kGqaTile - 1) / kGqaTile, all = (full + p->B) * p->Hkv, units = all > device_sms() ? all : device_sms();
+        const int64_t groups = (p->rows * p->G + 63) / 64 * p->Hkv, tile = int64_t(kPrefillTile) * (p->D > 128 ? 2 : 1);
+        const bool quicker = steps * (units * kPrefillStep - groups * tile) <= int64_t(kPrefillMore) * device_sms();
+        s.prefill = quicker && full * p->Hkv >= kPrefillMinUnits && own * p->Hkv * p->D * 4 <= kPrefillOwnBytes && own < 0x7FFFFF00;
         if (s.prefill) {
             s.plan_words = 4 + 2 * blocks;
             s.own_rows = own;
@@ -328,12 +339,12 @@ static int gqa_fwd(const Dsv4GqaParams* p, void* stream_) {
     if (!gqa_sizes(p, s)) return int(cudaErrorInvalidValue);
     const bool e4m3 = p->kv_dtype == DSV4_DTYPE_E4M3;
     if ((p->q_dtype != DSV4_DTYPE_BF16 && p->q_dtype != DSV4_DTYPE_F16) || (!e4m3 && p->kv_dtype != p->q_dtype)) return int(cudaErrorInvalidValue);
-    if (p->num_pages <= 0 || p->num_pages * kGqaTile > 0x7FFFFFFF - kGqaTile || p->window < 0 || p->first < 0 || !(p->sm_scale > 0.f) || !(p->sm_scale < INFINITY)) return int(cudaErrorInvalidValue);
+    if (p->num_pages <= 0 || p->num_pages >= 0x7FFFFFFF / kGqaTile || p->window < 0 || p->first < 0 || !(p->sm_scale > 0.f) || !(p->sm_scale < INFINITY)) return int(cudaErrorInvalidValue);
     if (!p->q || !p->k_pool || !p->v_pool || !p->block_table || !p->kv_len || !p->out || (e4m3 && (!p->k_scale || !p->v_scale))) return int(cudaErrorInvalidValue);
     if (p->q_start == nullptr && p->rows != int64_t(p->B) * p->T) return int(cudaErrorInvalidValue);
     if (!aligned(p->q, 16) || !aligned(p->k_pool, 16) || !aligned(p->v_pool, 16) || !aligned(p->out, 16)) return int(cudaErrorInvalidValue);
     if (p->q_stride_b % 8 || p->q_stride_t % 8 || p->q_stride_h % 8) return int(cudaErrorInvalidValue);
-    if (p->weights != nullptr && (p->q_start != nullptr || p->weight_stride < s.logit_stride)) return int(cudaErrorInvalidValue);
+    if (p->weights != nullptr && (p->q_start != nullptr || p->B > 65535 || p->weight_stride < s.logit_stride)) return int(cudaErrorInvalidValue);
     if (p->workspace == nullptr || !aligned(p->workspace, 128) || p->workspace_bytes < dsv4_gqa_workspace_bytes(p)) return int(cudaErrorInvalidValue);
     const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     const HostState state = host_state();
@@ -375,7 +386,11 @@ static int gqa_fwd(const Dsv4GqaParams* p, void* stream_) {
         e = p->D == 64 ? run_decode<64>(a, p->kv_dtype, stream) : p->D == 128 ? run_decode<128>(a, p->kv_dtype, stream) : run_decode<256>(a, p->kv_dtype, stream);
     }
     if (e != cudaSuccess) return int(e);
-    const int64_t merge_rows = p->rows * p->Hkv * p->G, merge_blocks = (merge_rows + kGqaMergeRows - 1) / kGqaMergeRows;
+    // a row has as many warps as stay within 32 for every SM
+    const int64_t merge_rows = p->rows * p->Hkv * p->G;
+    a.merge_warps = kGqaMergeWarps;
+    while (a.merge_warps > 1 && merge_rows * a.merge_warps > int64_t(device_sms()) * 32) a.merge_warps /= 2;
+    const int64_t block_rows = kGqaMergeWarps / a.merge_warps, merge_blocks = (merge_rows + block_rows - 1) / block_rows;
     if (s.cluster == 0 && (s.blocks > 1 || s.streams > 0)) {
         const dim3 grid{unsigned(merge_blocks)};
         e = p->D == 64 ? launch(gqa_merge_kernel<64>, grid, kGqaMergeThreads, 0, stream, a)
@@ -434,7 +449,7 @@ extern "C" int dsv4_gqa_insert(const Dsv4GqaInsertParams* p, void* stream) {
 extern "C" int dsv4_kv_evict(const Dsv4KvEvictParams* p, void* stream_) {
     if (p == nullptr || p->B <= 0 || p->B > 65535 || p->max_pages <= 0 || p->num_pages <= 0 || p->layers <= 0 || p->pools < 0 || p->pools > DSV4_EVICT_POOLS) return int(cudaErrorInvalidValue);
     const int64_t cap = int64_t(p->max_pages) * 64;
-    if (p->num_pages * 64 > 0x7FFFFFFF || cap > 0x7FFFFFFF - kEvictPlanThreads * kEvictEach || p->first < 0 || p->recent < 0 || (p->keep_each == nullptr && p->keep < 0))
+    if (p->num_pages > 0x7FFFFFFF / 64 || cap > 0x7FFFFFFF - kEvictPlanThreads * kEvictEach || p->first < 0 || p->recent < 0 || (p->keep_each == nullptr && p->keep < 0))
         return int(cudaErrorInvalidValue);
     if (!p->block_table || !p->kv_len || !p->refs || !p->weights || !p->new_table || !p->new_len || !p->new_refs || !p->new_weights || !p->kept || !p->scratch)
         return int(cudaErrorInvalidValue);

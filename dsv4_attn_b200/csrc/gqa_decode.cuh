@@ -4,18 +4,21 @@
 // p - j < window or j < first only, and
 //     out = sum_j exp(x_j - m) v_j / (sum_j exp(x_j - m) + exp(sink - m)),   x_j = sm_scale q . k_j,   lse = m + log sum_j exp(x_j - m)
 //
-// Layout of the work.  The rows of a KV head are its (token, query head) pairs, in groups of R = 16 to 64; a unit is (request, KV head, row group), its tiles the
+// Layout of the work.  The rows of a KV head are its (token, query head) pairs, in groups of R = 16, 32 or 64; a unit is (request, KV head, row group), its tiles the
 // pages of 64 entries that some row of the group sees.  All units' tiles lie behind one another on one axis, which is cut into equal shares, one per resident block: every
 // block streams the same number of tiles whatever the lengths are.  Each block finds its place on the axis by a scan over the
-// lengths (no planner, nothing read back).  A unit inside one share writes its output; one that a cut runs through leaves FP32 partials, which gqa_merge_kernel joins.
+// lengths (no planner, nothing read back).  A unit inside one share writes its output; one that a cut runs through leaves FP32 partials, which gqa_merge_kernel joins.  Of small calls a cluster
+// has each unit to itself and joins its blocks' parts through distributed shared memory.
 //
-// What bounds it: the bytes of K and V, each read once.  A producer warp keeps a ring of K and V tiles filled by TMA (128-byte swizzle) across the
-// block's units; four warps take 16 entries of a tile each (with more rows: fewer entries, more rows), S = Q K^T and O += P V by mma.sync m16n8k16 with FP32
-// accumulators, the running maximum and sum in registers.  A tile of 64 entries x 128 in 16 bits is 128 instructions of 16 rows: a fifth of the time
+// What bounds it: the bytes of K and V, each read once.  A producer warp keeps a ring of K and V tiles filled by TMA (swizzled) across the
+// block's units; four warps take 16 entries of a tile each, or 32 of two pages where pages are small (with more rows: fewer entries, more rows), S = Q K^T and O += P V by mma.sync m16n8k16 with
+// FP32 accumulators, the running maximum and sum in registers.  A tile of 64 entries x 128 in 16 bits is 128 instructions of 16 rows, 2.2 cycles each: a fifth of the time
 // that its 32 KB take from memory, so that tcgen05's M = 128 would multiply padding and its way through tensor memory would only lengthen
-// the chain; prompts, which do have 128 rows, take gqa_prefill_kernel.
+// the chain; more rows take gqa_rows_kernel and prompts gqa_prefill_kernel.
+// 64 requests x 8,000 entries, 8 heads: of 128 in BF16 314-322 us (6.5 TB/s), in e4m3 232 (4.5: a page of 16 KB takes its warps 1,080 cycles); of 64 193 (5.4); of 256 611 (6.9, the copy
+// that 6.4 is measured by writes too).  One request of 1,000 entries 8.3 us, of 16,000 24, of 130,000 92 (5.8 TB/s).
 //
-// Rounding: P is rounded to the type of V (BF16: 2^-9, FP16: 2^-12 of a weight, at most, and at random), everything else is FP32.  An e4m3 cache is read as
+// Rounding: P is rounded to the type of V, off by half a step at most (BF16 2^-8, FP16 2^-11 of a weight) and at random; everything else is FP32.  An e4m3 cache is read as
 // FP16, which holds its values exactly; BF16 queries then go through FP16 after each row has been brought near 1 by a power of two, which is exact but for elements
 // below 2^-14 of the row's largest (off by 2^-25 of that).
 #pragma once
@@ -58,6 +61,7 @@ struct GqaArgs {
     int cluster;                     // blocks of a cluster that has a unit to itself, or 0: shares
     int one_group;                   // not packed, and a request's rows of a KV head fit a group
     int min_share;                   // tiles of a block, at least
+    int merge_warps;                 // of gqa_merge_kernel for a row: 1, 2, 4 or 8
     int streams;                     // parts that a block leaves of a piece (gqa_rows_kernel; and a place more), or 0: one
     // weights of the entries
     float* logits;                   // [B][Hkv * T * G][logit_stride], log2 units; null: not wanted
@@ -106,7 +110,7 @@ struct GqaSpan {
     __device__ __forceinline__ int slot(int k) const { return k < head ? k : k + skip; }
 };
 // (Rows and tokens of a request are below 2^29: 32-bit divisions, which take a twentieth of the time of 64-bit ones.  With those, and one more for every group, a call for one
-// request took 18 us instead of 10.)
+// request took 18.2 us instead of 12.8.)
 __device__ __forceinline__ GqaSpan gqa_span(const GqaArgs& a, const GqaRequest& r, int rg) {
     GqaSpan s;
     if (a.one_group) {
@@ -344,8 +348,8 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
         ptx::prefetch_tensormap(&a.k_map);
         ptx::prefetch_tensormap(&a.v_map);
     }
-    ptx::pdl_trigger();
     ptx::pdl_wait();
+    ptx::pdl_trigger();              // (behind the wait: the kernels that follow read lengths and offsets before theirs)
 
     GqaWalk w;
     uint32_t rank = 0;
@@ -819,17 +823,17 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
 }
 
 // ── parts of units that a cut ran through ──
-// A warp takes a row and finds out, from the same scan as above, which blocks had a part of its unit.
-constexpr int kGqaMergeRows = kGqaMergeThreads / 32;
+// A warp takes a row, or with few rows some of a row's parts, and finds out, from the same scan as above, which blocks had a part of its unit.  Bound by latency: a warp has four parts on
+// their way at once (one request of 16,000 entries in 296 parts: the call 26 us instead of 35), and reads lengths before the attention kernel's end (3 us).
+constexpr int kGqaMergeWarps = kGqaMergeThreads / 32;
 template <int D>
 __global__ void __launch_bounds__(kGqaMergeThreads) gqa_merge_kernel(const __grid_constant__ GqaArgs a) {
-    constexpr int kWarps = kGqaMergeThreads / 32;
+    constexpr int kWarps = kGqaMergeWarps;
     __shared__ int64_t sums[2][kWarps];
     __shared__ int request;
-    ptx::pdl_trigger();
-    ptx::pdl_wait();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, H = a.Hkv * a.G;
-    const int64_t row0 = int64_t(blockIdx.x) * kGqaMergeRows, token0 = quotient(row0, H);
+    __shared__ __align__(16) float slices[kWarps][D + 4];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, H = a.Hkv * a.G, row_warps = a.merge_warps, slice = warp & (row_warps - 1);
+    const int64_t row0 = int64_t(blockIdx.x) * (kWarps / row_warps), token0 = quotient(row0, H);
     // the request of the block's first row
     int first_b = a.B;
     if (a.q_start == nullptr) {
@@ -868,7 +872,7 @@ __global__ void __launch_bounds__(kGqaMergeThreads) gqa_merge_kernel(const __gri
         ahead += sums[1][i];
     }
     // this warp's row
-    const int64_t row = row0 + warp, token = token0 + int(uint32_t(row - token0 * H) / uint32_t(H));
+    const int64_t row = row0 + warp / row_warps, token = token0 + int(uint32_t(row - token0 * H) / uint32_t(H));
     GqaRequest req{};
     int b = first_b;
     for (; b < a.B; ++b) {
@@ -876,66 +880,103 @@ __global__ void __launch_bounds__(kGqaMergeThreads) gqa_merge_kernel(const __gri
         if (token < req.row0 + req.tokens && req.tokens > 0) break;
         ahead += gqa_head_tiles(a, req) * a.Hkv;
     }
-    if (b >= a.B || token < req.row0) return;
-    const int rows = req.tokens * a.G, head = int(row - token * H), h = int(uint32_t(head) / uint32_t(a.G));
-    const int at = int(token - req.row0) * a.G + head - h * a.G;               // row of the KV head
-    const int rg = a.one_group ? 0 : int(uint32_t(at) / uint32_t(a.group_rows)), r = at - rg * a.group_rows;
-    int64_t unit = ahead + h * gqa_head_tiles(a, req);
-    for (int i = 0; i < rg; ++i) unit += gqa_span(a, req, i).count;
-    const int64_t share = gqa_share(a, total);
-    const int c0 = int(quotient(unit, share)), c1 = int(quotient(unit + gqa_span(a, req, rg).count - 1, share));
-    if (c0 == c1) return;
-    const int later = unit != c0 * share;                                      // (every later block begins with its part)
-    const int streams = max(a.streams, 1), places = 2 * streams + (a.streams > 0), parts = (c1 - c0 + 1) * streams;
-    auto part = [&](int i) {
-        const int block = streams == 2 ? i >> 1 : i;
-        return (int64_t(c0 + block) * places + (block == 0 ? later * streams : 0) + (i - block * streams)) * a.group_rows + r;
-    };
-    float top = -INFINITY;
-    for (int i = lane; i < parts; i += 32) top = fmaxf(top, a.part_lse[part(i)]);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-    constexpr int kVecs = D > 128 ? D / 128 : 1;
+    bool mine = b < a.B && token >= req.row0;
+    int head = 0, h = 0, at = 0, r = 0, c0 = 0, parts = 0, later = 0;
+    const int streams = max(a.streams, 1), places = 2 * streams + (a.streams > 0);
+    if (mine) {
+        head = int(row - token * H);
+        h = int(uint32_t(head) / uint32_t(a.G));
+        at = int(token - req.row0) * a.G + head - h * a.G;                     // row of the KV head
+        const int rg = a.one_group ? 0 : int(uint32_t(at) / uint32_t(a.group_rows));
+        r = at - rg * a.group_rows;
+        int64_t unit = ahead + h * gqa_head_tiles(a, req);
+        for (int i = 0; i < rg; ++i) unit += gqa_span(a, req, i).count;
+        const int64_t share = gqa_share(a, total);
+        c0 = int(quotient(unit, share));
+        const int c1 = int(quotient(unit + gqa_span(a, req, rg).count - 1, share));
+        later = unit != c0 * share;                                            // (every later block begins with its part)
+        parts = (c1 - c0 + 1) * streams;
+        mine = c0 != c1;
+    }
+    constexpr int kVecs = D > 128 ? D / 128 : 1, kAtOnce = 4;
     float4 v[kVecs];
 #pragma unroll
     for (int x = 0; x < kVecs; ++x) v[x] = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
+    float top = -INFINITY, sum = 0.f;
     const bool in_row = 4 * lane < D;
-    for (int i0 = 0; i0 < parts; i0 += 32) {
-        float weight = 0.f;
-        if (i0 + lane < parts) {
-            const float p = a.part_lse[part(i0 + lane)];
-            weight = p == -INFINITY ? 0.f : ptx::ex2(p - (top == -INFINITY ? 0.f : top));
-        }
-#pragma unroll 4
-        for (int i = 0; i < min(32, parts - i0); ++i) {
-            const float by = __shfl_sync(0xFFFFFFFFu, weight, i);
-            sum += by;
-            if (in_row) {
-                const float* const from = a.part_o + part(i0 + i) * D + 4 * lane;
+    // (until here only what was there before the attention kernel's own wait had ended)
+    ptx::pdl_wait();
+    ptx::pdl_trigger();
+    if (mine) {
+        auto part = [&](int i) {
+            const int block = streams == 2 ? i >> 1 : i;
+            return (int64_t(c0 + block) * places + (block == 0 ? later * streams : 0) + (i - block * streams)) * a.group_rows + r;
+        };
+        for (int i = lane; i < parts; i += 32) top = fmaxf(top, a.part_lse[part(i)]);
 #pragma unroll
-                for (int x = 0; x < kVecs; ++x) {
-                    const float4 u = *reinterpret_cast<const float4*>(from + 128 * x);
-                    v[x].x = fmaf(by, u.x, v[x].x);  v[x].y = fmaf(by, u.y, v[x].y);  v[x].z = fmaf(by, u.z, v[x].z);  v[x].w = fmaf(by, u.w, v[x].w);
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+        const int each = (parts + row_warps - 1) / row_warps, end = min(parts, (slice + 1) * each);
+        for (int i0 = slice * each; i0 < end; i0 += 32) {
+            float weight = 0.f;
+            if (i0 + lane < end) {
+                const float p = a.part_lse[part(i0 + lane)];
+                weight = p == -INFINITY ? 0.f : ptx::ex2(p - (top == -INFINITY ? 0.f : top));
+            }
+            for (int i = 0; i < min(32, end - i0); i += kAtOnce) {
+                float4 u[kAtOnce][kVecs];
+#pragma unroll
+                for (int k = 0; k < kAtOnce; ++k) {
+                    const float4* const from = reinterpret_cast<const float4*>(a.part_o + part(i0 + i + k) * D + 4 * lane);
+#pragma unroll
+                    for (int x = 0; x < kVecs; ++x) u[k][x] = in_row && i0 + i + k < end ? from[32 * x] : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int k = 0; k < kAtOnce; ++k) {
+                    const float by = __shfl_sync(0xFFFFFFFFu, weight, i + k);
+                    sum += by;
+#pragma unroll
+                    for (int x = 0; x < kVecs; ++x) {
+                        v[x].x = fmaf(by, u[k][x].x, v[x].x);  v[x].y = fmaf(by, u[k][x].y, v[x].y);
+                        v[x].z = fmaf(by, u[k][x].z, v[x].z);  v[x].w = fmaf(by, u[k][x].w, v[x].w);
+                    }
                 }
             }
         }
     }
-    const float v_scale = a.v_scale != nullptr ? ptx::ld(a.v_scale + h) : 1.f;
-    if (in_row) {
+    if (row_warps > 1) {
+        // the row's first warp adds up
+        if (slice > 0) {
+            if (in_row)
 #pragma unroll
-        for (int x = 0; x < kVecs; ++x) gqa_write_row<D>(a, token, head, (int64_t(b) * a.Hkv + h) * rows + at, 128 * x + 4 * lane, v[x], top, sum, v_scale);
+                for (int x = 0; x < kVecs; ++x) *reinterpret_cast<float4*>(&slices[warp][128 * x + 4 * lane]) = v[x];
+            if (lane == 0) slices[warp][D] = sum;
+        }
+        __syncthreads();
+        if (slice > 0) return;
+        for (int i = 1; i < row_warps; ++i) {
+            sum += slices[warp + i][D];
+            if (in_row)
+#pragma unroll
+                for (int x = 0; x < kVecs; ++x) {
+                    const float4 u = *reinterpret_cast<const float4*>(&slices[warp + i][128 * x + 4 * lane]);
+                    v[x].x += u.x;  v[x].y += u.y;  v[x].z += u.z;  v[x].w += u.w;
+                }
+        }
     }
+    if (!mine || !in_row) return;
+    const float v_scale = a.v_scale != nullptr ? ptx::ld(a.v_scale + h) : 1.f;
+#pragma unroll
+    for (int x = 0; x < kVecs; ++x) gqa_write_row<D>(a, token, head, (int64_t(b) * a.Hkv + h) * (int64_t(req.tokens) * a.G) + at, 128 * x + 4 * lane, v[x], top, sum, v_scale);
 }
 
 // ── weights of the entries ──
 // weights[b][j] += sum over the tokens that see j and over the heads of exp(x_j) / denominator, from the scores that the attention kernel has left.  A thread takes an
-// entry and adds in a fixed order.
+// entry and adds in a fixed order.  Bound by the scores, read once (32 requests of up to 8,192 entries, 32 heads: 33 MB).
 __global__ void __launch_bounds__(kGqaWeightThreads) gqa_weights_kernel(const __grid_constant__ GqaArgs a) {
     ptx::pdl_trigger();
-    ptx::pdl_wait();
     const int b = blockIdx.y, p = blockIdx.x * kGqaWeightThreads + threadIdx.x;
     const GqaRequest req = gqa_request(a, b);
+    ptx::pdl_wait();                 // (lengths were there before the kernels before this one triggered it)
     if (p >= req.entries) return;
     const int rows = req.tokens * a.G;
     const int64_t base = int64_t(b) * a.Hkv * rows;
@@ -988,7 +1029,7 @@ __device__ __forceinline__ float by_scale(float x, float s, float inverse) {
 }
 
 // A block takes some consecutive tokens: a thread each finds out where they go (offset, position, page: one chain of loads for the block), then all threads copy, 16 bytes a thread
-// and load, four on the way.  Bound by that chain when small and by memory when large.
+// and load, four on the way.  Bound by that chain when small (64 tokens 3.3 us) and by memory when large (six prompts to 4,096 into e4m3 pages: 24-26 us, 4 TB/s).
 constexpr int kGqaInsertTokens = 32;
 template <bool E4M3>
 __global__ void __launch_bounds__(kGqaInsertThreads, 4) gqa_insert_kernel(const __grid_constant__ GqaInsertArgs a) {

@@ -8,7 +8,10 @@
 // too, each row brought near 1 by a power of two.
 //
 // Why not mma.sync with more rows: 64 rows x 64 entries x 128 are 512 instructions of m16n8k16, 1111 cycles at the measured 2.17 an instruction and SM, where an 8-bit page is there after
-// 700; and every warp of 16 rows converts the page for itself.
+// 700; and every warp of 16 rows converts the page for itself.  64 requests x 8,000 entries, 64 query heads for each of 8 KV heads of 128: 385 us against 670, in 8 bits 401 against 999.
+//
+// What bounds it: the shared-memory port with 8-bit pages (12 x 5 tokens of 64 heads behind 32,768 entries 289 us, of which the bytes need 125: 1,024 of a page's 1,275 cycles go to the raw page in
+// and out, the FP16 page in and out, and Q again for every page); DRAM with 16-bit ones.
 #pragma once
 
 #include "gqa_prefill.cuh"
@@ -80,8 +83,8 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_rows_kernel(const __grid_co
     __syncthreads();
     ptx::tc_fence_after_sync();
     const uint32_t tmem = *tmem_at;
-    ptx::pdl_trigger();
     ptx::pdl_wait();
+    ptx::pdl_trigger();              // (behind the wait: the merge reads lengths before its own)
 
     // where this block's share begins
     const int each = (a.B + C::Threads - 1) / C::Threads, b_from = tid * each, b_to = min(b_from + each, a.B);

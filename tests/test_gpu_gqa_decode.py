@@ -27,6 +27,24 @@ def test_lengths_around_tiles(lib, dtype, D):
     assert st.tolist() == [0, 0, 0, 0]
 
 
+@pytest.mark.parametrize("B", [1, 20, 50, 150])
+@pytest.mark.parametrize("D,G,dtype", [(64, 8, "f16"), (128, 8, "bf16"), (128, 24, "e4m3"), (256, 8, "e4m3")])
+def test_parts_joined_by_any_number_of_warps(lib, B, D, G, dtype):
+    """Few rows in many parts to many rows in few: a row of the merge has eight warps, four, two or one."""
+    c = Case([6000 // B + i * 97 % 700 for i in range(B)], 1, Hkv=4, G=G, D=D, dtype=dtype, seed=B, width=400, sink=True)
+    c.check(*c.call(lib))
+
+
+@pytest.mark.parametrize("G,T", [(4, 1), (5, 4), (32, 1)])
+@pytest.mark.parametrize("dtype,D", [("bf16", 64), ("bf16", 128), ("e4m3", 128), ("f16", 256)])
+def test_weights_after_clusters_shares_and_many_rows(lib, G, T, dtype, D):
+    for width, B in ((0, 2), (300, 2), (0, 60)):
+        c = Case([1500 // B + i * 71 % 300 + T for i in range(B)], T, Hkv=3, G=G, D=D, dtype=dtype, seed=B, width=width)
+        w = torch.zeros(B, c.table.shape[1] * PAGE, device="cuda")
+        before = w.clone()
+        c.check(*c.call(lib, weights=w), w, before)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "e4m3"])
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_lengths_in_wide_tables(lib, dtype, D):
