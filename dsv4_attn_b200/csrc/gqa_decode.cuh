@@ -1024,7 +1024,7 @@ __device__ __forceinline__ uint32_t quant_pair(float lo, float hi) {
 // x / s from the correctly rounded 1 / s: Markstein's step, which gives the correctly rounded quotient.  Quotients beyond e4m3's range are left as they are (the step would make NaN of
 // infinite ones).
 __device__ __forceinline__ float by_scale(float x, float s, float inverse) {
-    const float q = x * inverse, r = fmaf(fmaf(-q, s, x), inverse, q);
+    const float q = x * inverse, r = fmaf(fmaf(q, s, -x), -inverse, q);        // (with these signs a zero keeps its own)
     return fabsf(q) < 1024.f ? r : q;
 }
 
@@ -1088,7 +1088,7 @@ __global__ void __launch_bounds__(kGqaInsertThreads, 4) gqa_insert_kernel(const 
                 off[kv][i] = int32_t(h * a.stride_h[kv]) + 8 * (x - h * per_head);
                 if (E4M3) {
                     scale[kv][i] = ptx::ld(a.scale[kv] + h);
-                    plain &= scale[kv][i] > 1e-30f && scale[kv][i] < 1e30f;
+                    plain &= scale[kv][i] > 1e-25f && scale[kv][i] < 1e25f;
                 }
             }
         }

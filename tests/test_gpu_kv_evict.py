@@ -216,6 +216,22 @@ def test_insert(lib, dtype, packed, Hkv, D):
     assert st.tolist() == [0, 0, 0, 0]
 
 
+@pytest.mark.parametrize("src", [torch.bfloat16, torch.float16])
+def test_every_value_over_scales_of_all_sizes(lib, src):
+    x = torch.arange(65536, device="cuda", dtype=torch.int32).to(torch.int16).view(src).reshape(1, 256, 1, 256)
+    table = torch.arange(4, device="cuda", dtype=torch.int32)[None]
+    at = torch.zeros(1, device="cuda", dtype=torch.int32)
+    for s in (1.0, 0.37, 3.0, 1 / 448, 0.0123, 117.3, 6e4, 1e-7, 1e-24, 1e-26, 1e-38, 1e24, 1e30):
+        pools = [torch.zeros(4, PAGE, 1, 256, device="cuda", dtype=torch.float8_e4m3fn) for _ in "kv"]
+        scale = torch.tensor([s], device="cuda")
+        lib.gqa_insert(x, x.flip(1), *pools, table, at, k_scale=scale, v_scale=scale)
+        want = (x.float() / scale).clamp(-448, 448).to(torch.float8_e4m3fn).reshape(256, 256)
+        for p, w in zip(pools, (want, want.flip(0))):
+            p = p.reshape(256, 256)
+            nan = w.float().isnan()
+            assert torch.equal(p.float().isnan(), nan) and torch.equal(p.view(torch.uint8)[~nan], w.view(torch.uint8)[~nan])
+
+
 def test_insert_out_of_range(lib):
     pools = [torch.zeros(4, PAGE, 1, 64, device="cuda", dtype=torch.float16) for _ in "kv"]
     k = torch.ones(3, 2, 1, 64, device="cuda", dtype=torch.float16)
