@@ -27,12 +27,12 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "gqa_span.h"
 #include "ptx.cuh"
 
 namespace dsv4 {
 
 constexpr int kGqaBf16 = 0, kGqaF16 = 1, kGqaE4m3 = 2;            // types of K and V
-constexpr int kGqaTile = 64;                                      // entries of a tile: a page
 constexpr int kGqaConsumers = 128, kGqaThreads = kGqaConsumers + 32;
 constexpr int kGqaMergeThreads = 256, kGqaWeightThreads = 256;
 constexpr float kGqaLazy = 8.f;                                   // log2 of how far scores may pass a row's reference
@@ -103,36 +103,12 @@ __device__ __forceinline__ GqaRequest gqa_request(const GqaArgs& a, int b) {
 }
 
 // ── the tiles of a row group ──
-struct GqaSpan {
-    int t0, t1;                      // its tokens
-    int lo, hi, first;               // entries that some row sees: [0, first) and [lo, hi)
-    int head, skip, count;           // tiles: `head` from 0 on, the others `skip` pages further on; count >= 1 (a group that sees nothing has an empty one)
-    __device__ __forceinline__ int slot(int k) const { return k < head ? k : k + skip; }
-};
 // (Rows and tokens of a request are below 2^29: 32-bit divisions, which take a twentieth of the time of 64-bit ones.  With those, and one more for every group, a call for one
 // request took 18.2 us instead of 12.8.)
 __device__ __forceinline__ GqaSpan gqa_span(const GqaArgs& a, const GqaRequest& r, int rg) {
-    GqaSpan s;
-    if (a.one_group) {
-        s.t0 = 0;
-        s.t1 = r.tokens - 1;
-    } else {
-        const uint32_t row = uint32_t(rg) * uint32_t(a.group_rows), rows = uint32_t(r.tokens) * uint32_t(a.G);
-        s.t0 = int(row / uint32_t(a.G));
-        s.t1 = int((min(row + uint32_t(a.group_rows), rows) - 1) / uint32_t(a.G));
-    }
-    s.hi = max(min(r.place0 + s.t1 + 1, r.entries), 0);
-    s.lo = 0;
-    s.first = 0;
-    if (a.window > 0) {
-        s.lo = min(max(r.place0 + s.t0 - a.window + 1, 0), s.hi);
-        s.first = min(a.first, s.hi);
-    }
-    const int end = (s.hi + kGqaTile - 1) / kGqaTile, heads = (s.first + kGqaTile - 1) / kGqaTile, from = s.lo / kGqaTile;
-    s.head = min(heads, from);
-    s.skip = from - s.head;
-    s.count = max(end - s.skip, 1);
-    return s;
+    if (a.one_group) return gqa_token_span(r.place0, r.entries, 0, r.tokens - 1, a.window, a.first);
+    const uint32_t row = uint32_t(rg) * uint32_t(a.group_rows), rows = uint32_t(r.tokens) * uint32_t(a.G);
+    return gqa_token_span(r.place0, r.entries, int(row / uint32_t(a.G)), int((min(row + uint32_t(a.group_rows), rows) - 1) / uint32_t(a.G)), a.window, a.first);
 }
 __device__ __forceinline__ int gqa_groups(const GqaArgs& a, const GqaRequest& r) {
     if (a.one_group) return 1;
@@ -404,7 +380,7 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
             for (int k = w.k0; k < w.k1 && ok; k += 32) {
                 // the pages of the next 32 tiles, one per lane
                 int page = -1;
-                if (k + lane < w.k1 && w.span.hi > 0) {
+                if (k + lane < w.k1 && w.span.has(w.span.slot(k + lane))) {
                     page = ptx::ld(a.block_table + int64_t(w.b) * a.max_pages + w.span.slot(k + lane));
                     if (page < 0 || page >= a.num_pages) {
                         gqa_report(a.status, kGqaStatusBadIndex, 4, page);

@@ -52,25 +52,6 @@ struct PrefillCfg {
     static constexpr int ColO = 256;
 };
 
-// Entries seen by some row of tokens [t0, t1] of a request, in tiles of `tile` entries (a multiple of a page).
-__device__ __forceinline__ GqaSpan prefill_span(const GqaArgs& a, const GqaRequest& r, int t0, int t1, int tile) {
-    GqaSpan s;
-    s.t0 = t0;
-    s.t1 = t1;
-    s.hi = max(min(r.place0 + t1 + 1, r.entries), 0);
-    s.lo = 0;
-    s.first = 0;
-    if (a.window > 0) {
-        s.lo = min(max(r.place0 + t0 - a.window + 1, 0), s.hi);
-        s.first = min(a.first, s.hi);
-    }
-    const int end = (s.hi + tile - 1) / tile, heads = (s.first + tile - 1) / tile, from = s.lo / tile;
-    s.head = min(heads, from);
-    s.skip = from - s.head;
-    s.count = max(end - s.skip, 1);
-    return s;
-}
-
 // Units in the order of their steps: a counting sort.
 __global__ void __launch_bounds__(kPrefillPlanThreads) gqa_plan_kernel(const __grid_constant__ GqaPrefillArgs p) {
     __shared__ int count[kPrefillBuckets];
@@ -80,14 +61,14 @@ __global__ void __launch_bounds__(kPrefillPlanThreads) gqa_plan_kernel(const __g
     ptx::pdl_wait();
     const GqaArgs& a = p.g;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int block_tokens = a.group_rows / a.G, tile = kGqaTile;
+    const int block_tokens = a.group_rows / a.G;
     for (int i = tid; i < kPrefillBuckets; i += kPrefillPlanThreads) count[i] = 0;
     if (tid == 0) most = 0;
     __syncthreads();
     auto each = [&](auto&& f) {
         for (int b = warp; b < a.B; b += kPrefillPlanThreads / 32) {
             const GqaRequest r = gqa_request(a, b);
-            for (int i = lane; i * int64_t(block_tokens) < r.tokens; i += 32) f(b, i, prefill_span(a, r, i * block_tokens, min((i + 1) * block_tokens, r.tokens) - 1, tile).count);
+            for (int i = lane; i * int64_t(block_tokens) < r.tokens; i += 32) f(b, i, gqa_token_span(r.place0, r.entries, i * block_tokens, min((i + 1) * block_tokens, r.tokens) - 1, a.window, a.first).count);
         }
     };
     for (int b = tid; b < a.B; b += kPrefillPlanThreads)
@@ -147,7 +128,7 @@ struct PrefillWalk {
     GqaRequest req;
     GqaSpan span;
     int b;
-    __device__ __forceinline__ void take(const GqaPrefillArgs& p, int tile) {
+    __device__ __forceinline__ void take(const GqaPrefillArgs& p) {
         if (u >= total) return;
         const GqaArgs& a = p.g;
         h = u % a.Hkv;
@@ -155,17 +136,17 @@ struct PrefillWalk {
         b = ptx::ld(at);
         const int block = ptx::ld(at + 1), tokens = a.group_rows / a.G;
         req = gqa_request(a, b);
-        span = prefill_span(a, req, block * tokens, min((block + 1) * tokens, req.tokens) - 1, tile);
+        span = gqa_token_span(req.place0, req.entries, block * tokens, min((block + 1) * tokens, req.tokens) - 1, a.window, a.first);
     }
-    __device__ __forceinline__ void begin(const GqaPrefillArgs& p, int tile) {
+    __device__ __forceinline__ void begin(const GqaPrefillArgs& p) {
         total = ptx::ld(p.plan) * p.g.Hkv;
         u = blockIdx.x;
-        take(p, tile);
+        take(p);
     }
     __device__ __forceinline__ bool more() const { return u < total; }
-    __device__ __forceinline__ void next(const GqaPrefillArgs& p, int tile) {
+    __device__ __forceinline__ void next(const GqaPrefillArgs& p) {
         u += gridDim.x;
-        take(p, tile);
+        take(p);
     }
 };
 
@@ -203,7 +184,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
     ptx::pdl_trigger();
     ptx::pdl_wait();
     PrefillWalk w;
-    w.begin(p, NE);
+    w.begin(p);
     bool ok = true;
     // Two barriers at a time where a role waits for two: a look takes long while products keep the shared memory busy.
     auto wait = [&](uint32_t bar, uint32_t turn, int role, int what) {
@@ -229,7 +210,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
     if (warp == C::SoftmaxWarps) {
         // ── producer ──
         uint32_t seq = 0, unit = 0;
-        for (; w.more() && ok; w.next(p, NE), ++unit) {
+        for (; w.more() && ok; w.next(p), ++unit) {
             for (int t = 0; t < NT && ok; ++t) {
                 if (unit > 0) wait(q_empty + 8 * t, unit - 1, 0, int(unit));
                 if (ok && ptx::elect_one()) {
@@ -243,8 +224,8 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
             for (int k = 0; k < w.span.count && ok; k += 32) {
                 // the pages of the next 32 steps, one per lane
                 int page = -1;
-                const int slot = w.span.slot(k + lane), from = slot * kGqaTile;
-                if (k + lane < w.span.count && from < w.span.hi) {
+                const int slot = w.span.slot(k + lane);
+                if (k + lane < w.span.count && w.span.has(slot)) {
                     page = ptx::ld(a.block_table + int64_t(w.b) * a.max_pages + slot);
                     if (page < 0 || page >= a.num_pages) {
                         gqa_report(a.status, kGqaStatusBadIndex, 4, page);
@@ -298,7 +279,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
         constexpr uint32_t kIdesc = C::BF16 ? ptx::make_idesc_bf16(128, D, false, true) : ptx::make_idesc_f16(128, D, false, true), kDescHi = ptx::smem_desc_hi(1024);
         const uint32_t ring_lo = ptx::smem_desc_lo(ring, NE * 128);
         uint32_t at = 0;                                                      // steps of all units so far
-        for (; w.more() && ok; w.next(p, NE)) {
+        for (; w.more() && ok; w.next(p)) {
             for (int j = 0; j < w.span.count && ok; ++j, ++at) {
                 const uint32_t st = (2 * at + 1) % C::Slots, v_lo = ring_lo + st * (C::Slot >> 4);
 #pragma unroll
@@ -326,7 +307,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
         const int t = warp - C::SoftmaxWarps - 2;
         const uint32_t q_lo = ptx::smem_desc_lo(smem + t * C::QTile, 16), ring_lo = ptx::smem_desc_lo(ring, 16);
         uint32_t at = 0, unit = 0;
-        for (; w.more() && ok; w.next(p, NE), ++unit) {
+        for (; w.more() && ok; w.next(p), ++unit) {
             wait(q_full + 8 * t, unit, 1, int(unit));
             for (int j = 0; j < w.span.count; ++j, ++at) {
                 const uint32_t st = (2 * at) % C::Slots, buffer = 2 * t + (at & 1);
@@ -358,7 +339,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
         const float neg = -INFINITY;
         uint32_t step = 0, unit = 0;
         bool ahead = false;                                                   // the next step's scores are known to be there
-        for (; w.more() && ok; w.next(p, NE), ++unit) {
+        for (; w.more() && ok; w.next(p), ++unit) {
             const int token = w.span.t0 + t * p.tile_tokens + tok, place = w.req.place0 + token;
             const int first_place = w.req.place0 + w.span.t0 + t * p.tile_tokens, last_place = first_place + p.tile_tokens - 1;
             const float scale = a.scale_log2 * (a.k_scale != nullptr ? ptx::ld(a.k_scale + w.h) : 1.f);

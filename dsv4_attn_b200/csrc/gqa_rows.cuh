@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_rows_kernel(const __grid_co
             for (int k = w.k0; k < w.k1 && ok; k += 32) {
                 // the pages of the next 32 tiles, one per lane
                 int page = -1;
-                if (k + lane < w.k1 && w.span.hi > 0) {
+                if (k + lane < w.k1 && w.span.has(w.span.slot(k + lane))) {
                     page = ptx::ld(a.block_table + int64_t(w.b) * a.max_pages + w.span.slot(k + lane));
                     if (page < 0 || page >= a.num_pages) {
                         gqa_report(a.status, kGqaStatusBadIndex, 4, page);
