@@ -867,7 +867,7 @@ def _gqa(what, q, q_start, k_pool, v_pool, block_table, kv_len, sm_scale, window
 def gqa_decode(q, k_pool, v_pool, block_table, kv_len, sm_scale, *, window=0, first=0, k_scale=None, v_scale=None, attn_sink=None, weights=None, max_len=None,
                out=None, lse=None, status=None):
     """Attention of T new tokens per request over pages of K and V heads.  q bf16 or f16 [B, T, H, D] (strided rows of a fused projection will do), D 64, 128 or 256; k_pool, v_pool
-    [P, 64, Hkv, D] of q's type, or float8_e4m3fn with k_scale, v_scale f32 [Hkv]; H a multiple of Hkv; block_table int32 [B, max_pages]; kv_len int32 [B]: entries of a
+    [P, 64, Hkv, D] of q's type, or float8_e4m3fn with k_scale, v_scale f32 [Hkv] (any finite ones); H a multiple of Hkv; block_table int32 [B, max_pages]; kv_len int32 [B]: entries of a
     request, the new tokens' own (`gqa_insert`) among them.  Token t stands at place kv_len - T + t and sees the entries up to its own, with `window` > 0 those of
     the last `window` places and the `first` ones only.  Returns (out [B, T, H, D], lse f32 [B, T, H]); a token that sees nothing gives 0 and -inf.
 

@@ -198,6 +198,12 @@ __device__ __forceinline__ float gqa_near_one(uint4& v) {
     v.w = ptx::pack_f16x2(f[6] * down, f[7] * down);
     return __uint_as_float(uint32_t(127 + e) << 23);
 }
+// For kernels that set what a row does not see to -inf before they scale its scores, which takes a factor above 0: a head's negative scale stands in its products' signs (the kernels turn Q or K
+// round), and a factor of 0 (a scale of 0, or a product too small) is the smallest number, by which scores are 0 as well and -inf remains what it is.
+__device__ __forceinline__ float gqa_positive(float scale) {
+    const float s = fabsf(scale);
+    return s == 0.f ? __uint_as_float(1u) : s;
+}
 __host__ __device__ constexpr int gqa_blocks_per_sm(int D) { return D > 128 ? 1 : 2; }
 
 // D: head dimension; KVT: type of K and V; WM: warps side by side over the rows, 16 each

@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
         for (; w.more() && ok; w.next(p), ++unit) {
             const int token = w.span.t0 + t * p.tile_tokens + tok, place = w.req.place0 + token;
             const int first_place = w.req.place0 + w.span.t0 + t * p.tile_tokens, last_place = first_place + p.tile_tokens - 1;
-            const float scale = a.scale_log2 * (a.k_scale != nullptr ? ptx::ld(a.k_scale + w.h) : 1.f);
+            const float scale = a.k_scale != nullptr ? gqa_positive(a.scale_log2 * ptx::ld(a.k_scale + w.h)) : a.scale_log2;
             float ref = neg, l = 0.f;
             for (int j = 0; j < w.span.count; ++j, ++step) {
                 const int i = 2 * t + int(step & 1);
@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
 }
 
 // ── an 8-bit cache's pages in 16 bits ──
-// e4m3 values (exact in BF16 and FP16; the scales go into scores and outputs) of every page that some token sees, to pages of the call's own: [B * max_pages][64][Hkv][D].
+// e4m3 values (exact in BF16 and FP16; the scales go into scores and outputs, but for the sign of K's, which is put in here) of every page that some token sees, to pages of the call's own: [B * max_pages][64][Hkv][D].
 constexpr int kGqaUnpackThreads = 256;
 struct GqaUnpackArgs {
     GqaArgs g;
@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(kGqaUnpackThreads) gqa_unpack_kernel(const __g
     ptx::pdl_trigger();
     ptx::pdl_wait();
     const GqaArgs& a = u.g;
-    const int vecs = u.entry * kGqaTile / 16;                                 // of a page
+    const int vecs = u.entry * kGqaTile / 16, head = u.entry / a.Hkv / 16;    // of a page, of a head's row
     const int64_t pages = int64_t(a.B) * a.max_pages;
     for (int64_t at = blockIdx.x; at < pages; at += gridDim.x) {
         const int b = int(at / a.max_pages), slot = int(at - int64_t(b) * a.max_pages);
@@ -551,6 +551,7 @@ __global__ void __launch_bounds__(kGqaUnpackThreads) gqa_unpack_kernel(const __g
 #pragma unroll 4
             for (int i = threadIdx.x; i < vecs; i += kGqaUnpackThreads) {
                 const uint4 v = ptx::ldg_stream_v4(src + i);
+                const uint32_t turn = kv == 0 && ptx::ld(a.k_scale + uint32_t(i) / uint32_t(head) % uint32_t(a.Hkv)) < 0.f ? 0x80008000u : 0u;
                 const uint32_t x[4] = {v.x, v.y, v.z, v.w};
                 uint32_t o[8];
 #pragma unroll
@@ -562,6 +563,8 @@ __global__ void __launch_bounds__(kGqaUnpackThreads) gqa_unpack_kernel(const __g
                             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&o[2 * j + q]));
                             o[2 * j + q] = ptx::pack_bf16x2(f.x, f.y);
                         }
+                    o[2 * j] ^= turn;
+                    o[2 * j + 1] ^= turn;
                 }
                 ptx::stg_v8(dst + 2 * i, make_uint4(o[0], o[1], o[2], o[3]), make_uint4(o[4], o[5], o[6], o[7]));
             }

@@ -259,6 +259,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_rows_kernel(const __grid_co
             if (!ok) break;
             {
                 constexpr int kLanes = D / 8, kRows = 32 / kLanes;            // lanes of a row, 16 bytes each; rows of a load
+                const uint32_t turn = ptx::ld(a.k_scale + w.h) < 0.f ? 0x80008000u : 0u;
                 const int l = lane % kLanes, rows = w.req.tokens * a.G, first = w.rg * a.group_rows;
 #pragma unroll 4
                 for (int i = 0; i < 32 / kRows; ++i) {
@@ -270,6 +271,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_rows_kernel(const __grid_co
                     }
                     const float factor = a.q_bf16 ? gqa_near_one<kLanes>(v) : 1.f;
                     if (l == 0) row_factor[r] = factor;
+                    v.x ^= turn;  v.y ^= turn;  v.z ^= turn;  v.w ^= turn;
                     ptx::sts_v4(smem + (l / 8) * (128 * 128) + r * 128 + (((l % 8) ^ (r & 7)) << 4), v);
                 }
             }
@@ -335,7 +337,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_rows_kernel(const __grid_co
             // (without the wait a stream that has no tile of a piece would arrive for the next one too early)
             wait(q_full, piece, 2, int(piece));
             if (!ok) break;
-            if (C::E4M3) scale *= row_factor[at_row];
+            if (C::E4M3) scale = gqa_positive(scale * row_factor[at_row]);
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(q_empty);                         // (its factors have been read)
             float* const logits = a.logits != nullptr && real ? a.logits + ((int64_t(w.b) * a.Hkv + w.h) * rows + row) * a.logit_stride : nullptr;

@@ -5,7 +5,7 @@
  * The conventions are those of dsv4_attn.h: raw device pointers of the caller, nothing allocated, work enqueued on `stream`, 0 or a
  * cudaError_t value returned, an optional `status` array of DSV4_STATUS_WORDS int32.
  *
- * Pools.  K and V of one layer are [num_pages][64][Hkv][D] each, in BF16, FP16 or e4m3 (then value = e4m3 * scale[head]).  A block table
+ * Pools.  K and V of one layer are [num_pages][64][Hkv][D] each, in BF16, FP16 or e4m3 (then value = e4m3 * scale[head], for any finite scale).  A block table
  * int32 [B][max_pages] maps a request's pages to pool pages; entry j of request b lies in page block_table[b][j / 64] at j % 64.  The page tables and
  * counts are those of dsv4_speculative.h: dsv4_kv_pages_free works on them as they are.  A page outside the pool, an entry outside the table: left out, not read, and
  * reported (DSV4_STATUS_BAD_INDEX).
