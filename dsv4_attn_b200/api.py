@@ -887,7 +887,7 @@ def gqa_prefill(q, q_start, k_pool, v_pool, block_table, kv_len, sm_scale, *, wi
 def gqa_insert(k, v, k_pool, v_pool, block_table, insert_pos, *, q_start=None, n_rows=None, k_scale=None, v_scale=None, status=None) -> None:
     """New rows of K and V, bf16 or f16 [B, T, Hkv, D], into the pages: row t of request b becomes its entry insert_pos[b] + t (int32 [B]; of the first n_rows[b] rows only
     where that is given).  With q_start int32 [B + 1] the rows are packed, [rows, Hkv, D], as for `gqa_prefill`.  Pools as for `gqa_decode`; into float8_e4m3fn ones go
-    value / scale[head], rounded to the nearest.  A place outside the table or the pool is left out; status then says 16."""
+    value / scale[head], rounded to the nearest (0 / 0: 0).  A place outside the table or the pool is left out; status then says 16."""
     r = _host.gqa_insert(k, v, k_pool, v_pool, block_table, insert_pos, q_start, n_rows, k_scale, v_scale, status)
     if r is not None:
         return None if r == 0 else _rc(r, "dsv4_gqa_insert")

@@ -1010,6 +1010,9 @@ __device__ __forceinline__ float by_scale(float x, float s, float inverse) {
     return fabsf(q) < 1024.f ? r : q;
 }
 
+// The quotient over any scale; over 0 zeros stay zeros (as which a head of zeros is read back, whose largest value, 0, made the scale).
+__device__ __forceinline__ float over_scale(float x, float s) { return s == 0.f && x == 0.f ? x : __fdiv_rn(x, s); }
+
 // A block takes some consecutive tokens: a thread each finds out where they go (offset, position, page: one chain of loads for the block), then all threads copy, 16 bytes a thread
 // and load, four on the way.  Bound by that chain when small (64 tokens 3.3 us) and by memory when large (six prompts to 4,096 into e4m3 pages: 24-26 us, 4 TB/s).
 constexpr int kGqaInsertTokens = 32;
@@ -1107,7 +1110,7 @@ __global__ void __launch_bounds__(kGqaInsertThreads, 4) gqa_insert_kernel(const 
                                 hi = f.y;
                             }
                             o[j] = plain ? quant_pair(by_scale(lo, scale[kv][i], inverse), by_scale(hi, scale[kv][i], inverse))
-                                         : quant_pair(__fdiv_rn(lo, scale[kv][i]), __fdiv_rn(hi, scale[kv][i]));
+                                         : quant_pair(over_scale(lo, scale[kv][i]), over_scale(hi, scale[kv][i]));
                         }
                         *reinterpret_cast<uint2*>(dst + 256 * i) = make_uint2(o[0] | (o[1] << 16), o[2] | (o[3] << 16));
                     } else {

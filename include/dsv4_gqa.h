@@ -80,7 +80,7 @@ int dsv4_gqa_prefill_fwd(const Dsv4GqaParams* p, void* stream);
 
 /*
  * New rows of K and V, BF16 or FP16, into the pages: row t of request b becomes entry insert_pos[b] + t; rows as [B][T] (of which n_rows[b] are taken where that
- * is given) or packed by q_start.  Into e4m3 pools a value is divided by its head's scale and rounded to the nearest e4m3 (beyond 448: 448).
+ * is given) or packed by q_start.  Into e4m3 pools a value is divided by its head's scale and rounded to the nearest e4m3 (beyond 448: 448; 0 / 0: 0).
  * A place outside the table or the pool is left out and reported (code 16).
  */
 typedef struct Dsv4GqaInsertParams {

@@ -46,3 +46,24 @@ def test_a_row_of_zeros_beside_rows_far_outside_fp16(lib, call):
     c.q[0].zero_()
     c.scale = 1e-31
     c.check(*c.call(lib))
+
+
+def test_zeros_over_a_scale_of_zero(lib):
+    for src in (torch.bfloat16, torch.float16):
+        k = torch.zeros(2, 3, 3, 64, device="cuda", dtype=src)
+        k[:, :, 1] = torch.randn(2, 3, 64, device="cuda").to(src)
+        k[0, 0, 2, 5], k[0, 0, 2, 6], k[0, 0, 2, 7] = 3.0, -3.0, -0.0
+        pools = [torch.full((2, PAGE, 3, 64), 7.0, device="cuda").to(torch.float8_e4m3fn) for _ in "kv"]
+        scale = torch.tensor([0.0, 0.05, 0.0], device="cuda")
+        table, at = torch.tensor([[1], [0]], device="cuda", dtype=torch.int32), torch.tensor([0, 5], device="cuda", dtype=torch.int32)
+        lib.gqa_insert(k, k, *pools, table, at, k_scale=scale, v_scale=scale)
+        for p in pools:
+            got = torch.stack([p[1, :3], p[0, 5:8]]).float()
+            want = (k.float() / scale[:, None]).nan_to_num(0.0, 1e9, -1e9).clamp(-448, 448).to(torch.float8_e4m3fn).float()
+            assert torch.equal(got, want) and (got[..., 0, :] == 0).all()
+            assert (got * scale[:, None])[:, :, [0, 2]].abs().max() == 0
+        # and such a cache is read as zeros
+        q = torch.randn(2, 1, 6, 64, device="cuda").to(src)
+        out, lse = lib.gqa_decode(q, *pools, table[:, :1], at + 3, 0.125, k_scale=scale, v_scale=scale, window=3)
+        assert out.isfinite().all() and (out[:, :, [0, 1, 4, 5]] == 0).all()
+        assert torch.allclose(lse[:, 0, [0, 1]], torch.full((2, 2), 3.0, device="cuda").log())
