@@ -18,7 +18,9 @@
 // 64 requests x 8,000 entries, 8 heads: of 128 in BF16 314-322 us (6.5 TB/s), in e4m3 232 (4.5: a page of 16 KB takes its warps 1,080 cycles); of 64 193 (5.4); of 256 611 (6.9, the copy
 // that 6.4 is measured by writes too).  One request of 1,000 entries 8.3 us, of 16,000 24, of 130,000 92 (5.8 TB/s).
 //
-// Rounding: P is rounded to the type of V, off by half a step at most (BF16 2^-8, FP16 2^-11 of a weight) and at random; everything else is FP32.  An e4m3 cache is read as
+// Rounding: P is rounded to the type of V, off by half a step at most (BF16 2^-8, FP16 2^-11 of a weight); everything else is FP32.  Weights in FP16 are taken 2^7 larger, so that with scores that pass
+// a row's reference by 2^8 they reach 2^15 of its 2^16, and have all their bits down to 2^-21 of the reference (with a reference at 1 they had them to 2^-14: 3,000 entries of 10.45 * 2^-24 beside one
+// that outweighs them came out 4 % low); what is below 2^-32 of it vanishes.  An e4m3 cache is read as
 // FP16, which holds its values exactly; BF16 queries then go through FP16 after each row has been brought near 1 by a power of two, which is exact but for elements
 // below 2^-14 of the row's largest (off by 2^-25 of that).
 #pragma once
@@ -36,6 +38,7 @@ constexpr int kGqaBf16 = 0, kGqaF16 = 1, kGqaE4m3 = 2;            // types of K 
 constexpr int kGqaConsumers = 128, kGqaThreads = kGqaConsumers + 32;
 constexpr int kGqaMergeThreads = 256, kGqaWeightThreads = 256;
 constexpr float kGqaLazy = 8.f;                                   // log2 of how far scores may pass a row's reference
+constexpr float kGqaUp = 7.f;                                     // log2 of how far weights in FP16 are raised
 constexpr int kGqaStatusBadIndex = 7, kGqaStatusWait = 1;
 
 struct GqaArgs {
@@ -502,7 +505,8 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
             place[hh] = row_first + r < rows ? w.req.place0 + int(uint32_t(row_first + r) / uint32_t(a.G)) : -1;
             scale[hh] = kE4m3 ? head_scale * row_factor[r] : head_scale;
         }
-        // m: reference of a row's weights, in log2 units: a maximum that the row's later ones have not passed by 2^8
+        // m: reference of a row's weights, in log2 units: a maximum that the row's later ones have not passed by 2^8, for weights in FP16 less kGqaUp
+        constexpr float kUp = kBf16 ? 0.f : kGqaUp, kLazy = kGqaLazy + kUp;
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[D / 8][4];
 #pragma unroll
         for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
@@ -609,16 +613,16 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
 #pragma unroll
                     for (int i = 1; i < 2 * Sub; ++i) top[hh] = ptx::max3(top[hh], s[i][2 * hh], s[i][2 * hh + 1]);
                 }
-                if (__any_sync(0xFFFFFFFFu, (m[0] == -INFINITY ? top[0] > m[0] : top[0] - m[0] > kGqaLazy) || (m[1] == -INFINITY ? top[1] > m[1] : top[1] - m[1] > kGqaLazy))) {
+                if (__any_sync(0xFFFFFFFFu, (m[0] == -INFINITY ? top[0] > m[0] : top[0] - m[0] > kLazy) || (m[1] == -INFINITY ? top[1] > m[1] : top[1] - m[1] > kLazy))) {
 #pragma unroll
                     for (int hh = 0; hh < 2; ++hh) {
                         float t = fmaxf(top[hh], m[hh]);
                         t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 1));
                         t = fmaxf(t, __shfl_xor_sync(0xFFFFFFFFu, t, 2));
                         // (a row goes by its own scores only)
-                        const bool first = m[hh] == -INFINITY, moves = first ? t > m[hh] : t - m[hh] > kGqaLazy;
-                        const float by = moves && !first ? ptx::ex2(m[hh] - t) : 1.f;
-                        if (moves) m[hh] = t;
+                        const bool first = m[hh] == -INFINITY, moves = first ? t > m[hh] : t - m[hh] > kLazy;
+                        const float to = t - kUp, by = moves && !first ? ptx::ex2(m[hh] - to) : 1.f;
+                        if (moves) m[hh] = to;
                         l[hh] *= by;
 #pragma unroll
                         for (int j = 0; j < D / 8; ++j) {

@@ -337,6 +337,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
         const int H = a.Hkv * a.G;
         const bool real = r < p.tile_tokens * a.G;                            // (rows behind hold what the memory held)
         const float neg = -INFINITY;
+        constexpr float kUp = C::BF16 ? 0.f : kGqaUp;                         // (P in FP16, taken 2^7 larger)
         uint32_t step = 0, unit = 0;
         bool ahead = false;                                                   // the next step's scores are known to be there
         for (; w.more() && ok; w.next(p), ++unit) {
@@ -395,7 +396,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
 #pragma unroll
                             for (int q = 0; q < 4; ++q) top[q] = ptx::max3(top[q], __uint_as_float(v[c][x + 2 * q]), __uint_as_float(v[c][x + 2 * q + 1]));
                     refer(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
-                    const float sub = ref == neg ? 0.f : -ref * scale;
+                    const float sub = ref == neg ? kUp : fmaf(-ref, scale, kUp);
                     // (where scores are so large that the rounding of this product would tell, the other way)
                     done = !__any_sync(0xFFFFFFFFu, fabsf(sub) >= 16777216.f);
                     if (done) {
@@ -455,7 +456,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
                         load(v, c);
 #pragma unroll
                         for (int x = 0; x < 32; x += 2) {
-                            const float x0 = ptx::ex2((__uint_as_float(v[x]) - sub) * scale), x1 = ptx::ex2((__uint_as_float(v[x + 1]) - sub) * scale);
+                            const float x0 = ptx::ex2(fmaf(__uint_as_float(v[x]) - sub, scale, kUp)), x1 = ptx::ex2(fmaf(__uint_as_float(v[x + 1]) - sub, scale, kUp));
                             l += x0 + x1;
                             pk[x / 2] = C::BF16 ? ptx::pack_bf16x2(x0, x1) : ptx::pack_f16x2(x0, x1);
                         }
@@ -481,7 +482,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
             const bool none = l == 0.f;
             float all = l, by = 1.f;
             if (mine && a.sink != nullptr && !none) {
-                const float s = ptx::ld(a.sink + head) * 1.4426950408889634f, top = ref * scale, m2 = fmaxf(top, s);
+                const float s = ptx::ld(a.sink + head) * 1.4426950408889634f, top = fmaf(ref, scale, -kUp), m2 = fmaxf(top, s);
                 by = ptx::ex2(top - m2);
                 all = l * by + ptx::ex2(s - m2);
             }
@@ -503,7 +504,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
                     for (int x = 0; x < 4; ++x) *reinterpret_cast<uint4*>(to + 64 * c + 16 * x) = make_uint4(o[4 * x], o[4 * x + 1], o[4 * x + 2], o[4 * x + 3]);
                 }
             }
-            if (mine && a.lse != nullptr) a.lse[row] = none ? neg : (ref * scale + log2f(l)) * 0.6931471805599453f;
+            if (mine && a.lse != nullptr) a.lse[row] = none ? neg : (fmaf(ref, scale, -kUp) + log2f(l)) * 0.6931471805599453f;
             ptx::tc_fence_before_sync();
         }
     }

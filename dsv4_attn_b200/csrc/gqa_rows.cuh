@@ -326,6 +326,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_rows_kernel(const __grid_co
         const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
         const int at_row = (warp & 3) * 32 + lane, r = at_row - (t == 1 ? p.second : 0);      // row of the tile, and of the group
         const float neg = -INFINITY;
+        constexpr float kUp = C::BF16 ? 0.f : kGqaUp;
         uint32_t joined = 0;                                                  // units that both streams have joined
         for (; w.left > 0 && ok; w.next(a), ++piece) {
             const int rows = w.req.tokens * a.G, row = w.rg * a.group_rows + r;
@@ -415,7 +416,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_rows_kernel(const __grid_co
                     }
                     // Differences are taken before they are scaled: at the maximum 0, however large it is.
                     const float sub = ref == neg ? 0.f : -ref;
-                    const uint64_t sub2 = ptx::pack_f32x2(sub, sub), scale2 = ptx::pack_f32x2(scale, scale);
+                    const uint64_t sub2 = ptx::pack_f32x2(sub, sub), scale2 = ptx::pack_f32x2(scale, scale), up2 = ptx::pack_f32x2(kUp, kUp);
                     uint64_t s0 = ptx::pack_f32x2(l, 0.f), s1 = ptx::pack_f32x2(0.f, 0.f);
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
@@ -423,7 +424,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_rows_kernel(const __grid_co
 #pragma unroll
                         for (int x = 0; x < 32; x += 2) {
                             float x0, x1;
-                            ptx::unpack_f32x2(ptx::mul_f32x2(ptx::add_f32x2(ptx::pack_f32x2(__uint_as_float(v[c][x]), __uint_as_float(v[c][x + 1])), sub2), scale2), x0, x1);
+                            ptx::unpack_f32x2(ptx::fma_f32x2(ptx::add_f32x2(ptx::pack_f32x2(__uint_as_float(v[c][x]), __uint_as_float(v[c][x + 1])), sub2), scale2, up2), x0, x1);
                             x0 = ptx::ex2(x0);
                             x1 = ptx::ex2(x1);
                             if (x & 2) s1 = ptx::add_f32x2(s1, ptx::pack_f32x2(x0, x1));
@@ -451,7 +452,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_rows_kernel(const __grid_co
                 if (!ok) break;
                 ptx::tc_fence_after_sync();
             }
-            ref = ref == neg ? neg : ref * scale;                             // (in log2 units from here on)
+            ref = ref == neg ? neg : fmaf(ref, scale, -kUp);                  // (in log2 units from here on, as the weights were taken)
             const bool complete = w.k0 == 0 && w.k1 == w.span.count, mine = complete && t == 0;
             // the block's places: two pieces that a cut runs through, and the second stream's part of a unit that none does
             const int64_t part = int64_t(blockIdx.x) * (2 * NT + 1) + (complete ? 2 * NT : (w.nth > 0) * NT + t);
