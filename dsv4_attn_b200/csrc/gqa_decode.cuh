@@ -635,12 +635,14 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
 #pragma unroll
                 for (int hh = 0; hh < 2; ++hh) {
                     const float ref = m[hh] == -INFINITY ? 0.f : m[hh];
+                    float sum = 0.f;                                          // (of the visit: one rounding of the row's sum for all of its entries)
 #pragma unroll
                     for (int i = 0; i < 2 * Sub; ++i) {
                         const float e_lo = ptx::ex2(s[i][2 * hh] - ref), e_hi = ptx::ex2(s[i][2 * hh + 1] - ref);
-                        l[hh] += e_lo + e_hi;
+                        sum += e_lo + e_hi;
                         pf[i / 2][2 * (i % 2) + hh] = kBf16 ? ptx::pack_bf16x2(e_lo, e_hi) : ptx::pack_f16x2(e_lo, e_hi);
                     }
+                    l[hh] += sum;
                 }
                 if (sl + WN * Sub >= 4) {
                     __syncwarp();

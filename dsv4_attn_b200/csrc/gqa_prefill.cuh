@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
                     done = !__any_sync(0xFFFFFFFFu, fabsf(sub) >= 16777216.f);
                     if (done) {
                         const uint64_t sub2 = ptx::pack_f32x2(sub, sub), scale2 = ptx::pack_f32x2(scale, scale);
-                        uint64_t s0 = ptx::pack_f32x2(l, 0.f), s1 = ptx::pack_f32x2(0.f, 0.f);
+                        uint64_t s0 = ptx::pack_f32x2(0.f, 0.f), s1 = s0;                     // (the step's own sum: the row's is rounded once for its 64 entries)
 #pragma unroll
                         for (int c = 0; c < NE / 32; ++c) {
                             uint32_t pk[16];
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
                         }
                         float a0, a1;
                         ptx::unpack_f32x2(ptx::add_f32x2(s0, s1), a0, a1);
-                        l = a0 + a1;
+                        l += a0 + a1;
                     }
                 }
                 if (!done) {
@@ -449,6 +449,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
                     }
                     refer(fmaxf(t0, t1));
                     const float sub = ref == neg ? 0.f : ref;
+                    float sum = 0.f;
                     // (P of 32 entries takes the place of scores that have been read)
 #pragma unroll 1
                     for (int c = 0; c < NE / 32; ++c) {
@@ -457,11 +458,12 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
 #pragma unroll
                         for (int x = 0; x < 32; x += 2) {
                             const float x0 = ptx::ex2(fmaf(__uint_as_float(v[x]) - sub, scale, kUp)), x1 = ptx::ex2(fmaf(__uint_as_float(v[x + 1]) - sub, scale, kUp));
-                            l += x0 + x1;
+                            sum += x0 + x1;
                             pk[x / 2] = C::BF16 ? ptx::pack_bf16x2(x0, x1) : ptx::pack_f16x2(x0, x1);
                         }
                         tmem_st16(s_at + 16 * c, pk);
                     }
+                    l += sum;
                 }
                 // a look at the next step's scores, whose answer comes while P is on its way
                 ahead = ptx::mbar_try_wait(s_full + 8 * (2 * t + int((step + 1) & 1)), ((step + 1) >> 1) & 1u);

@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_rows_kernel(const __grid_co
                     // Differences are taken before they are scaled: at the maximum 0, however large it is.
                     const float sub = ref == neg ? 0.f : -ref;
                     const uint64_t sub2 = ptx::pack_f32x2(sub, sub), scale2 = ptx::pack_f32x2(scale, scale), up2 = ptx::pack_f32x2(kUp, kUp);
-                    uint64_t s0 = ptx::pack_f32x2(l, 0.f), s1 = ptx::pack_f32x2(0.f, 0.f);
+                    uint64_t s0 = ptx::pack_f32x2(0.f, 0.f), s1 = s0;                         // (the step's own sum: the row's is rounded once for its 64 entries)
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         uint32_t pk[16];
@@ -435,7 +435,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_rows_kernel(const __grid_co
                     }
                     float a0, a1;
                     ptx::unpack_f32x2(ptx::add_f32x2(s0, s1), a0, a1);
-                    l = a0 + a1;
+                    l += a0 + a1;
                     ptx::tmem_wait_st();
                 }
                 // (a warp of rows that are none leaves whatever stands there: those rows of O are not read)
