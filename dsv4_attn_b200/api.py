@@ -877,11 +877,15 @@ def gqa_decode(q, k_pool, v_pool, block_table, kv_len, sm_scale, *, window=0, fi
     return _gqa("dsv4_gqa_decode_fwd", q, None, k_pool, v_pool, block_table, kv_len, sm_scale, window, first, k_scale, v_scale, attn_sink, weights, max_len, out, lse, status)
 
 
-def gqa_prefill(q, q_start, k_pool, v_pool, block_table, kv_len, sm_scale, *, window=0, first=0, k_scale=None, v_scale=None, attn_sink=None, out=None, lse=None, status=None):
+def gqa_prefill(q, q_start, k_pool, v_pool, block_table, kv_len, sm_scale, *, window=0, first=0, k_scale=None, v_scale=None, attn_sink=None, max_len=None, out=None, lse=None,
+                status=None):
     """The same for prompts, or pieces of them: q [rows, H, D] holds the tokens of all requests one behind the other, those of request b in rows q_start[b] to
-    q_start[b + 1] - 1 (int32 [B + 1]); the last of them stands at place kv_len[b] - 1.  Returns (out [rows, H, D], lse f32 [rows, H]); rows of no request are left as they are."""
+    q_start[b + 1] - 1 (int32 [B + 1]); the last of them stands at place kv_len[b] - 1.  Returns (out [rows, H, D], lse f32 [rows, H]); rows of no request are left as they are.
+
+    Over an 8-bit cache prompts work on 16-bit copies of the pages, in a workspace for B * max_pages * 64 entries of all heads, up to 4 GiB (beyond that, some requests at a time).  Where tables
+    are wider than the requests are long, max_len, which no kv_len may pass (entries beyond it can be left out; status then says 7), keeps it small."""
     _check(q_start is not None, "q_start must be a tensor")
-    return _gqa("dsv4_gqa_prefill_fwd", q, q_start, k_pool, v_pool, block_table, kv_len, sm_scale, window, first, k_scale, v_scale, attn_sink, None, None, out, lse, status)
+    return _gqa("dsv4_gqa_prefill_fwd", q, q_start, k_pool, v_pool, block_table, kv_len, sm_scale, window, first, k_scale, v_scale, attn_sink, None, max_len, out, lse, status)
 
 
 def gqa_insert(k, v, k_pool, v_pool, block_table, insert_pos, *, q_start=None, n_rows=None, k_scale=None, v_scale=None, status=None) -> None:

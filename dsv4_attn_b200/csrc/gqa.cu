@@ -132,7 +132,10 @@ struct Sizes {
     int streams;                     // gqa_rows_kernel, if not 0
     int cluster;                     // blocks of a cluster that has a unit, or 0: shares
     int64_t plan_words;
-    int64_t own_rows;                // entries of the call's own 16-bit pages
+    int own_pages;                   // of a request, 16-bit copies of an 8-bit cache's, or 0
+    int round_b, round_h;            // requests and KV heads that a launch of gqa_prefill_kernel takes
+    int64_t own_bytes() const { return int64_t(round_b) * own_pages * kGqaTile * round_h * D * 2; }      // of K's copies, and of V's
+    int D;
 };
 
 // ── which kernel takes tokens that are not packed ──
@@ -145,7 +148,9 @@ constexpr int kRowsMore = 16, kRowsMore64 = 32;
 // the entries out over all SMs, for 10 us more.  Eight heads, one prompt behind a cache of 2,048 entries: 64 tokens 46 us in gqa_prefill_kernel and 33 in the other, 128 46 and 57; of 16,384:
 // 128 tokens 254 and 192, 256 260 and 355.
 constexpr int kPrefillMinUnits = 8, kPrefillStep = 10, kPrefillTile = 20, kPrefillMore = 100;      // 0.1 us
-constexpr int64_t kPrefillOwnBytes = int64_t(4) << 30;              // an 8-bit cache's pages are brought to 16 bits in a workspace of that size at most
+// An 8-bit cache's pages are brought to 16 bits in a workspace of that size at most, by the lengths that there can be: a call with room for more is gone through in rounds, some requests at a time, or
+// some heads of one.
+constexpr int64_t kPrefillOwnBytes = int64_t(4) << 30;
 bool gqa_sizes(const Dsv4GqaParams* p, Sizes& s) {
     if (p == nullptr || p->B <= 0 || p->Hkv <= 0 || p->G <= 0 || p->max_pages <= 0 || p->T < 0 || p->rows < 0) return false;
     if (p->D != 64 && p->D != 128 && p->D != 256) return false;
@@ -178,7 +183,9 @@ bool gqa_sizes(const Dsv4GqaParams* p, Sizes& s) {
     s.logit_rows = p->weights != nullptr ? int64_t(p->B) * p->Hkv * p->T * p->G : 0;
     s.logit_stride = entries;
     s.prefill = false;
-    s.plan_words = s.own_rows = 0;
+    s.plan_words = 0;
+    s.own_pages = s.round_b = s.round_h = 0;
+    s.D = p->D;
     s.streams = 0;
     // (tensor maps have no axis that stays where it is)
     const bool spread = (p->Hkv * p->G == 1 || p->q_stride_h > 0) && (tokens == 1 || p->q_stride_t > 0) && (p->q_start != nullptr || p->B == 1 || p->q_stride_b > 0);
@@ -193,15 +200,32 @@ bool gqa_sizes(const Dsv4GqaParams* p, Sizes& s) {
         const int tile_tokens = 128 / p->G, block_tokens = tile_tokens * (p->D > 128 ? 1 : 2);
         const int64_t blocks = p->rows / block_tokens + p->B, full = (p->rows + block_tokens - 1) / block_tokens;
         const bool e4m3 = p->kv_dtype == DSV4_DTYPE_E4M3;
-        const int64_t own = e4m3 ? int64_t(p->B) * p->max_pages * kGqaTile : 0;
-        const int64_t steps = (longest + kGqaTile - 1) / kGqaTile, all = (full + p->B) * p->Hkv, units = all > device_sms() ? all : device_sms();
+        int64_t own_pages = 0, round_b = p->B, round_h = p->Hkv, rounds = 1;
+        if (e4m3) {
+            own_pages = p->max_len > 0 && p->max_len < entries ? (p->max_len + kGqaTile - 1) / kGqaTile : p->max_pages;
+            const int64_t head_bytes = own_pages * kGqaTile * p->D * 4, most_b = kPrefillOwnBytes / (head_bytes * p->Hkv), most_h = kPrefillOwnBytes / head_bytes;
+            if (most_b < p->B) {
+                const int64_t n = most_b > 0 ? (p->B + most_b - 1) / most_b : p->B;
+                round_b = (p->B + n - 1) / n;                                 // (rounds alike)
+                rounds = (p->B + round_b - 1) / round_b;
+            }
+            if (most_b == 0 && most_h > 0) {
+                const int64_t n = (p->Hkv + most_h - 1) / most_h;
+                round_h = (p->Hkv + n - 1) / n;
+                rounds *= (p->Hkv + round_h - 1) / round_h;
+            }
+            if (most_h == 0) rounds = 0;                                      // (a head of one request has more: 8 million entries of 128)
+        }
+        const int64_t steps = (longest + kGqaTile - 1) / kGqaTile, all = (full + p->B) * p->Hkv, least = rounds * device_sms(), units = all > least ? all : least;
         const int64_t groups = (p->rows * p->G + 63) / 64 * p->Hkv, tile = int64_t(kPrefillTile) * (p->D > 128 ? 2 : 1);
         const bool quicker = steps * (units * kPrefillStep - groups * tile) <= int64_t(kPrefillMore) * device_sms();
-        s.prefill = quicker && full * p->Hkv >= kPrefillMinUnits && own * p->Hkv * p->D * 4 <= kPrefillOwnBytes && own < 0x7FFFFF00;
+        s.prefill = quicker && full * p->Hkv >= kPrefillMinUnits && rounds > 0 && round_b * own_pages * kGqaTile < 0x7FFFFF00;
         if (s.prefill) {
             s.plan_words = 4 + 2 * blocks;
-            s.own_rows = own;
-            const int64_t most = blocks * p->Hkv;
+            s.own_pages = int(own_pages);
+            s.round_b = int(round_b);
+            s.round_h = int(round_h);
+            const int64_t most = blocks * round_h;
             s.blocks = int(most < device_sms() ? most : device_sms());
             s.group_rows = block_tokens * p->G;
             s.parts = 0;
@@ -283,8 +307,17 @@ cudaError_t make_rows_map(CUtensorMap* map, const Dsv4GqaParams* p, int tile_tok
     return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
-cudaError_t prefill(GqaArgs& g, const Dsv4GqaParams* p, const Sizes& s, uint8_t* ws, cudaStream_t stream) {
+// Requests b0 .. of a call, heads h0 .. of them
+cudaError_t prefill_round(const GqaArgs& g, const Dsv4GqaParams* p, const Sizes& s, uint8_t* ws, int b0, int h0, cudaStream_t stream) {
     GqaPrefillArgs a{};
+    a.g = g;
+    a.g.B = p->B - b0 < s.round_b ? p->B - b0 : s.round_b;
+    a.g.q_start += b0;
+    a.g.kv_len += b0;
+    a.g.block_table += int64_t(b0) * p->max_pages;
+    a.b0 = b0;
+    a.h0 = h0;
+    a.heads = p->Hkv - h0 < s.round_h ? p->Hkv - h0 : s.round_h;
     a.plan = reinterpret_cast<int32_t*>(ws);
     a.plan_units = int((s.plan_words - 4) / 2);
     ws += up(s.plan_words * 4);
@@ -292,35 +325,44 @@ cudaError_t prefill(GqaArgs& g, const Dsv4GqaParams* p, const Sizes& s, uint8_t*
     int64_t pages = p->num_pages;
     a.tile_tokens = 128 / p->G;
     cudaError_t e = cudaSuccess;
-    if (s.own_rows > 0) {
+    if (s.own_pages > 0) {
         GqaUnpackArgs u{};
-        u.g = g;
-        u.entry = p->Hkv * p->D;
+        u.g = a.g;
+        u.own_pages = a.own_pages = s.own_pages;
+        u.h0 = h0;  u.heads = a.heads;  u.D = p->D;
         for (int i = 0; i < 2; ++i) {
             u.pool[i] = static_cast<const uint8_t*>(i ? v : k);
             u.rows[i] = ws;
-            ws += up(s.own_rows * p->Hkv * p->D * 2);
+            ws += up(s.own_bytes());
         }
         k = u.rows[0];
         v = u.rows[1];
-        pages = s.own_rows / kGqaTile;
-        a.own_pages = 1;
-        const int64_t most = int64_t(device_sms()) * 8;
-        e = launch(g.q_bf16 ? gqa_unpack_kernel<true> : gqa_unpack_kernel<false>, dim3(unsigned(pages < most ? pages : most)), kGqaUnpackThreads, 0, stream, u);
+        pages = int64_t(a.g.B) * s.own_pages;
+        // eight blocks an SM over all requests
+        const int64_t each = (int64_t(device_sms()) * 8 + a.g.B - 1) / a.g.B;
+        u.blocks = int(each < s.own_pages ? each : s.own_pages);
+        e = launch(g.q_bf16 ? gqa_unpack_kernel<true> : gqa_unpack_kernel<false>, dim3(unsigned(a.g.B) * unsigned(u.blocks)), kGqaUnpackThreads, 0, stream, u);
         if (e != cudaSuccess) return e;
     }
-    a.g = g;
     a.pool_rows = pages * kGqaTile;
-    e = make_pool_map(&a.g.k_map, k, pages, p->Hkv, p->D, p->q_dtype);
-    if (e == cudaSuccess) e = make_pool_map(&a.g.v_map, v, pages, p->Hkv, p->D, p->q_dtype);
-    if (e == cudaSuccess) e = make_pool_map(&a.v8_map, v, pages, p->Hkv, p->D, p->q_dtype, 8);
-    if (e == cudaSuccess) e = make_pool_map(&a.v1_map, v, pages, p->Hkv, p->D, p->q_dtype, 1);
+    const int pool_heads = s.own_pages > 0 ? a.heads : p->Hkv;
+    e = make_pool_map(&a.g.k_map, k, pages, pool_heads, p->D, p->q_dtype);
+    if (e == cudaSuccess) e = make_pool_map(&a.g.v_map, v, pages, pool_heads, p->D, p->q_dtype);
+    if (e == cudaSuccess) e = make_pool_map(&a.v8_map, v, pages, pool_heads, p->D, p->q_dtype, 8);
+    if (e == cudaSuccess) e = make_pool_map(&a.v1_map, v, pages, pool_heads, p->D, p->q_dtype, 1);
     if (e == cudaSuccess) e = make_rows_map(&a.q_map, p, a.tile_tokens);
     if (e == cudaSuccess) e = launch(gqa_plan_kernel, dim3(1), kPrefillPlanThreads, 0, stream, a);
     if (e != cudaSuccess) return e;
     if (p->D == 64) return g.q_bf16 ? run_prefill<64, true>(a, stream) : run_prefill<64, false>(a, stream);
     if (p->D == 128) return g.q_bf16 ? run_prefill<128, true>(a, stream) : run_prefill<128, false>(a, stream);
     return g.q_bf16 ? run_prefill<256, true>(a, stream) : run_prefill<256, false>(a, stream);
+}
+
+cudaError_t prefill(const GqaArgs& g, const Dsv4GqaParams* p, const Sizes& s, uint8_t* ws, cudaStream_t stream) {
+    cudaError_t e = cudaSuccess;
+    for (int64_t b = 0; b < p->B && e == cudaSuccess; b += s.round_b)
+        for (int64_t h = 0; h < p->Hkv && e == cudaSuccess; h += s.round_h) e = prefill_round(g, p, s, ws, int(b), int(h), stream);
+    return e;
 }
 
 }  // namespace
@@ -331,7 +373,7 @@ using namespace dsv4;
 extern "C" int64_t dsv4_gqa_workspace_bytes(const Dsv4GqaParams* p) {
     Sizes s;
     if (!gqa_sizes(p, s)) return -1;
-    return 128 + up(s.parts * p->D * 4) + up(s.parts * 4) + up(s.logit_rows * s.logit_stride * 4) + up(s.logit_rows * 4) + up(s.plan_words * 4) + 2 * up(s.own_rows * p->Hkv * p->D * 2);
+    return 128 + up(s.parts * p->D * 4) + up(s.parts * 4) + up(s.logit_rows * s.logit_stride * 4) + up(s.logit_rows * 4) + up(s.plan_words * 4) + 2 * up(s.own_bytes());
 }
 
 static int gqa_fwd(const Dsv4GqaParams* p, void* stream_) {

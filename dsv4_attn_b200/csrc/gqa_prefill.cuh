@@ -33,7 +33,9 @@ struct GqaPrefillArgs {
     int32_t* plan;                   // [0] units of one KV head; from [4] on (request, block) pairs
     int plan_units;                  // room for them
     int tile_tokens;                 // floor(128 / G)
-    int own_pages;                   // the pools are the call's copies: slot s of request b is page b * max_pages + s
+    int own_pages;                   // if not 0, the pools are the call's copies: slot s of request b is page b * own_pages + s, the first head h0
+    int h0, heads;                   // KV heads of this launch
+    int b0;                          // its first request, for reports
     int64_t pool_rows;               // entries of the pools: the first row behind them
 };
 
@@ -72,7 +74,7 @@ __global__ void __launch_bounds__(kPrefillPlanThreads) gqa_plan_kernel(const __g
         }
     };
     for (int b = tid; b < a.B; b += kPrefillPlanThreads)
-        if (gqa_request(a, b).bad) gqa_report(a.status, kGqaStatusBadIndex, 4, b);
+        if (gqa_request(a, b).bad) gqa_report(a.status, kGqaStatusBadIndex, 4, p.b0 + b);
     int top = 0;
     each([&](int, int, int steps) { top = max(top, steps); });
     atomicMax(&most, top);
@@ -131,15 +133,16 @@ struct PrefillWalk {
     __device__ __forceinline__ void take(const GqaPrefillArgs& p) {
         if (u >= total) return;
         const GqaArgs& a = p.g;
-        h = u % a.Hkv;
-        const int32_t* const at = p.plan + 4 + 2 * (u / a.Hkv);
+        const int nth = u / p.heads;
+        h = p.h0 + u - nth * p.heads;
+        const int32_t* const at = p.plan + 4 + 2 * nth;
         b = ptx::ld(at);
         const int block = ptx::ld(at + 1), tokens = a.group_rows / a.G;
         req = gqa_request(a, b);
         span = gqa_token_span(req.place0, req.entries, block * tokens, min((block + 1) * tokens, req.tokens) - 1, a.window, a.first);
     }
     __device__ __forceinline__ void begin(const GqaPrefillArgs& p) {
-        total = ptx::ld(p.plan) * p.g.Hkv;
+        total = ptx::ld(p.plan) * p.heads;
         u = blockIdx.x;
         take(p);
     }
@@ -227,11 +230,11 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
                 const int slot = w.span.slot(k + lane);
                 if (k + lane < w.span.count && w.span.has(slot)) {
                     page = ptx::ld(a.block_table + int64_t(w.b) * a.max_pages + slot);
-                    if (page < 0 || page >= a.num_pages) {
+                    if (page < 0 || page >= a.num_pages || (p.own_pages > 0 && slot >= p.own_pages)) {
                         gqa_report(a.status, kGqaStatusBadIndex, 4, page);
                         page = -1;
-                    } else if (p.own_pages) {
-                        page = w.b * a.max_pages + slot;
+                    } else if (p.own_pages > 0) {
+                        page = w.b * p.own_pages + slot;
                     }
                 }
                 const int n = min(32, w.span.count - k);
@@ -250,7 +253,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
                             const int row = pg >= 0 ? pg * kGqaTile : int(p.pool_rows);
                             if (kv == 0 || pg < 0 || (e0 + NE <= w.span.hi && (e0 >= w.span.lo || e0 + NE <= w.span.first))) {
 #pragma unroll
-                                for (int x = 0; x < D / 64; ++x) ptx::tma_load_3d(at + x * (NE * 128), kv ? &a.v_map : &a.k_map, 64 * x, w.h, row, full);
+                                for (int x = 0; x < D / 64; ++x) ptx::tma_load_3d(at + x * (NE * 128), kv ? &a.v_map : &a.k_map, 64 * x, w.h - p.h0, row, full);
                             } else {
                                 auto seen = [&](int i) { return i < w.span.hi && (i >= w.span.lo || i < w.span.first); };
                                 for (int r8 = 0; r8 < NE; r8 += 8) {
@@ -259,10 +262,10 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
                                     for (int x = 0; x < D / 64; ++x) {
                                         const uint32_t to = at + x * (NE * 128) + r8 * 128;
                                         if (bits == 0u || bits == 255u) {
-                                            ptx::tma_load_3d(to, &p.v8_map, 64 * x, w.h, bits ? row + r8 : int(p.pool_rows), full);
+                                            ptx::tma_load_3d(to, &p.v8_map, 64 * x, w.h - p.h0, bits ? row + r8 : int(p.pool_rows), full);
                                         } else {
                                             for (int r = 0; r < 8; ++r)
-                                                ptx::tma_load_3d(to + r * 128, &p.v1_map, 64 * x, w.h, (bits >> r) & 1u ? row + r8 + r : int(p.pool_rows), full);
+                                                ptx::tma_load_3d(to + r * 128, &p.v1_map, 64 * x, w.h - p.h0, (bits >> r) & 1u ? row + r8 + r : int(p.pool_rows), full);
                                         }
                                     }
                                 }
@@ -526,37 +529,40 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
 }
 
 // ── an 8-bit cache's pages in 16 bits ──
-// e4m3 values (exact in BF16 and FP16; the scales go into scores and outputs, but for the sign of K's, which is put in here) of every page that some token sees, to pages of the call's own: [B * max_pages][64][Hkv][D].
+// e4m3 values (exact in BF16 and FP16; the scales go into scores and outputs, but for the sign of K's, which is put in here) of every page that some token sees, to pages of the call's own:
+// [requests * own_pages][64][heads][D].  A request has some blocks, which go through the pages that it holds.
 constexpr int kGqaUnpackThreads = 256;
 struct GqaUnpackArgs {
-    GqaArgs g;
+    GqaArgs g;                       // the launch's requests
     const uint8_t* pool[2];
     uint8_t* rows[2];
-    int entry;                       // Hkv * D
+    int own_pages, blocks;           // pages and blocks of a request
+    int h0, heads, D;
 };
 template <bool BF16>
 __global__ void __launch_bounds__(kGqaUnpackThreads) gqa_unpack_kernel(const __grid_constant__ GqaUnpackArgs u) {
     ptx::pdl_trigger();
     ptx::pdl_wait();
     const GqaArgs& a = u.g;
-    const int vecs = u.entry * kGqaTile / 16, head = u.entry / a.Hkv / 16;    // of a page, of a head's row
-    const int64_t pages = int64_t(a.B) * a.max_pages;
-    for (int64_t at = blockIdx.x; at < pages; at += gridDim.x) {
-        const int b = int(at / a.max_pages), slot = int(at - int64_t(b) * a.max_pages);
-        const GqaRequest r = gqa_request(a, b);
-        if (r.tokens == 0) continue;
-        const int from = slot * kGqaTile, lo = a.window > 0 ? max(r.place0 - a.window + 1, 0) : 0;
-        if (from >= r.entries || (from + kGqaTile <= lo && from >= a.first)) continue;
-        const int page = ptx::ld(a.block_table + at);
+    const int b = int(blockIdx.x / uint32_t(u.blocks));
+    const GqaRequest r = gqa_request(a, b);
+    if (r.tokens == 0) return;
+    const uint32_t head = uint32_t(u.D) / 16, vecs = head * kGqaTile * uint32_t(u.heads);       // 16-byte pieces of a head's row, and of a page's heads
+    const int lo = a.window > 0 ? max(r.place0 - a.window + 1, 0) : 0, pages = min((r.entries + kGqaTile - 1) / kGqaTile, u.own_pages);
+    for (int slot = int(blockIdx.x) - b * u.blocks; slot < pages; slot += u.blocks) {
+        const int from = slot * kGqaTile;
+        if (from + kGqaTile <= lo && from >= a.first) continue;
+        const int page = ptx::ld(a.block_table + int64_t(b) * a.max_pages + slot);
         if (page < 0 || page >= a.num_pages) continue;
 #pragma unroll 1
         for (int kv = 0; kv < 2; ++kv) {
-            const uint4* const src = reinterpret_cast<const uint4*>(u.pool[kv]) + int64_t(page) * vecs;
-            uint4* const dst = reinterpret_cast<uint4*>(u.rows[kv]) + at * vecs * 2;
+            const uint4* const src = reinterpret_cast<const uint4*>(u.pool[kv]) + (int64_t(page) * kGqaTile * a.Hkv + u.h0) * head;
+            uint4* const dst = reinterpret_cast<uint4*>(u.rows[kv]) + (int64_t(b) * u.own_pages + slot) * vecs * 2;
 #pragma unroll 4
-            for (int i = threadIdx.x; i < vecs; i += kGqaUnpackThreads) {
-                const uint4 v = ptx::ldg_stream_v4(src + i);
-                const uint32_t turn = kv == 0 && ptx::ld(a.k_scale + uint32_t(i) / uint32_t(head) % uint32_t(a.Hkv)) < 0.f ? 0x80008000u : 0u;
+            for (uint32_t i = threadIdx.x; i < vecs; i += kGqaUnpackThreads) {
+                const uint32_t row = i / head, e = row / uint32_t(u.heads), h = row - e * uint32_t(u.heads);
+                const uint4 v = ptx::ldg_stream_v4(src + (int64_t(e) * a.Hkv + h) * head + (i - row * head));
+                const uint32_t turn = kv == 0 && ptx::ld(a.k_scale + u.h0 + h) < 0.f ? 0x80008000u : 0u;
                 const uint32_t x[4] = {v.x, v.y, v.z, v.w};
                 uint32_t o[8];
 #pragma unroll

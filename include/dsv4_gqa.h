@@ -45,7 +45,8 @@ typedef struct Dsv4GqaParams {
     int32_t q_dtype;            /* DSV4_DTYPE_BF16 or _F16: q and out */
     int32_t kv_dtype;           /* the same, or DSV4_DTYPE_E4M3 */
     float   sm_scale;           /* > 0 */
-    int32_t max_len;            /* optional: no kv_len is larger (steers the launch only; with weights, entries beyond it get none) */
+    int32_t max_len;            /* optional: no kv_len is larger (steers the launch and the workspace; with weights, entries beyond it get none; packed tokens over e4m3 pages may
+                                   not see entries beyond it, which are reported) */
     int64_t rows;               /* rows of q: B * T, or packed */
     int64_t num_pages;
     int64_t q_stride_b;         /* elements, multiples of 8 */
@@ -75,7 +76,10 @@ int64_t dsv4_gqa_workspace_bytes(const Dsv4GqaParams* p);
 /* T tokens per request, q_start null: a decoding step, and the verification of a few drafted tokens. */
 int dsv4_gqa_decode_fwd(const Dsv4GqaParams* p, void* stream);
 
-/* Packed tokens, q_start given: prompts, or pieces of them behind what is cached. */
+/*
+ * Packed tokens, q_start given: prompts, or pieces of them behind what is cached.  Of e4m3 pages a prompt's kernel has 16-bit copies in the workspace, which has room for B * max_pages * 64
+ * entries, or B * max_len, up to 4 GiB: beyond that the call takes some requests at a time.
+ */
 int dsv4_gqa_prefill_fwd(const Dsv4GqaParams* p, void* stream);
 
 /*
