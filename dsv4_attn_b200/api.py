@@ -872,7 +872,8 @@ def gqa_decode(q, k_pool, v_pool, block_table, kv_len, sm_scale, *, window=0, fi
     the last `window` places and the `first` ones only.  Returns (out [B, T, H, D], lse f32 [B, T, H]); a token that sees nothing gives 0 and -inf.
 
     attn_sink f32 [H]: a logit per head in the denominator.  weights f32 [B, >= max_pages * 64]: to every entry is added what it got of the softmax weights of the call's tokens and
-    heads (what `kv_evict` goes by).  max_len: no kv_len is larger; it steers the launch only, but for `weights`, which entries beyond it do not get.
+    heads (what `kv_evict` goes by).  max_len: no kv_len is larger; it steers the launch, and with `weights`, which entries beyond it do not get, a workspace
+    of 4 bytes for every row of q and entry (of max_len, or of the whole table).
     Entries that no token of the call sees may hold anything; the others must be finite."""
     return _gqa("dsv4_gqa_decode_fwd", q, None, k_pool, v_pool, block_table, kv_len, sm_scale, window, first, k_scale, v_scale, attn_sink, weights, max_len, out, lse, status)
 

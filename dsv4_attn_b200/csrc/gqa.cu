@@ -181,7 +181,7 @@ bool gqa_sizes(const Dsv4GqaParams* p, Sizes& s) {
         }
     }
     s.logit_rows = p->weights != nullptr ? int64_t(p->B) * p->Hkv * p->T * p->G : 0;
-    s.logit_stride = entries;
+    s.logit_stride = p->max_len > 0 && p->max_len < entries ? (int64_t(p->max_len) + kGqaTile - 1) / kGqaTile * kGqaTile : entries;
     s.prefill = false;
     s.plan_words = 0;
     s.own_pages = s.round_b = s.round_h = 0;
@@ -386,7 +386,7 @@ static int gqa_fwd(const Dsv4GqaParams* p, void* stream_) {
     if (p->q_start == nullptr && p->rows != int64_t(p->B) * p->T) return int(cudaErrorInvalidValue);
     if (!aligned(p->q, 16) || !aligned(p->k_pool, 16) || !aligned(p->v_pool, 16) || !aligned(p->out, 16)) return int(cudaErrorInvalidValue);
     if (p->q_stride_b % 8 || p->q_stride_t % 8 || p->q_stride_h % 8) return int(cudaErrorInvalidValue);
-    if (p->weights != nullptr && (p->q_start != nullptr || p->B > 65535 || p->weight_stride < s.logit_stride)) return int(cudaErrorInvalidValue);
+    if (p->weights != nullptr && (p->q_start != nullptr || p->B > 65535 || p->weight_stride < int64_t(p->max_pages) * kGqaTile)) return int(cudaErrorInvalidValue);
     if (p->workspace == nullptr || !aligned(p->workspace, 128) || p->workspace_bytes < dsv4_gqa_workspace_bytes(p)) return int(cudaErrorInvalidValue);
     const cudaStream_t stream = static_cast<cudaStream_t>(stream_);
     const HostState state = host_state();
@@ -410,6 +410,8 @@ static int gqa_fwd(const Dsv4GqaParams* p, void* stream_) {
         a.logits = reinterpret_cast<float*>(ws);  ws += up(s.logit_rows * s.logit_stride * 4);
         a.total = reinterpret_cast<float*>(ws);
         a.logit_stride = s.logit_stride;
+        a.logit_end = int(s.logit_stride);
+        a.weight_len = p->max_len > 0 && p->max_len < s.logit_stride ? p->max_len : a.logit_end;
         a.weights = p->weights;  a.weight_stride = p->weight_stride;
     }
     a.wait_ns = uint32_t(state.wait_ns < 4000000000ull ? state.wait_ns : 4000000000ull);
@@ -440,8 +442,7 @@ static int gqa_fwd(const Dsv4GqaParams* p, void* stream_) {
         if (e != cudaSuccess) return int(e);
     }
     if (p->weights != nullptr) {
-        const int64_t longest = p->max_len > 0 && p->max_len < s.logit_stride ? p->max_len : s.logit_stride;
-        e = launch(gqa_weights_kernel, dim3(unsigned((longest + kGqaWeightThreads - 1) / kGqaWeightThreads), unsigned(p->B)), kGqaWeightThreads, 0, stream, a);
+        e = launch(gqa_weights_kernel, dim3(unsigned((a.weight_len + kGqaWeightThreads - 1) / kGqaWeightThreads), unsigned(p->B)), kGqaWeightThreads, 0, stream, a);
     }
     return int(e);
 }

@@ -68,7 +68,9 @@ struct GqaArgs {
     int streams;                     // parts that a block leaves of a piece (gqa_rows_kernel; and a place more), or 0: one
     // weights of the entries
     float* logits;                   // [B][Hkv * T * G][logit_stride], log2 units; null: not wanted
-    int64_t logit_stride;
+    int64_t logit_stride;            // whole tiles
+    int logit_end;                   // the same, or 0 without weights: scores of entries behind it are not kept
+    int weight_len;                  // entries that can get weights
     float* total;                    // [B][Hkv * T * G]: log2 of the denominators
     float* weights;                  // [B][weight_stride], added to
     int64_t weight_stride;
@@ -587,7 +589,7 @@ __global__ void __launch_bounds__(kGqaThreads, C::BlocksPerSm) gqa_decode_kernel
                             if (!(there && p <= at && p < w.req.entries && (a.window == 0 || p > at - a.window || p < a.first))) s[i][q] = -INFINITY;
                         }
                 }
-                if (a.logits != nullptr) {
+                if (p0 < a.logit_end) {
 #pragma unroll
                     for (int hh = 0; hh < 2; ++hh) {
                         const int r = row_first + wm * 16 + g + 8 * hh;
@@ -965,7 +967,7 @@ __global__ void __launch_bounds__(kGqaWeightThreads) gqa_weights_kernel(const __
     const int b = blockIdx.y, p = blockIdx.x * kGqaWeightThreads + threadIdx.x;
     const GqaRequest req = gqa_request(a, b);
     ptx::pdl_wait();                 // (lengths were there before the kernels before this one triggered it)
-    if (p >= req.entries) return;
+    if (p >= min(req.entries, a.weight_len)) return;
     const int rows = req.tokens * a.G;
     const int64_t base = int64_t(b) * a.Hkv * rows;
     float sum = 0.f;

@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_rows_kernel(const __grid_co
 #pragma unroll
                             for (int q = 0; q < 4; ++q) tops[q] = ptx::max3(tops[q], __uint_as_float(v[c][x + 2 * q]), __uint_as_float(v[c][x + 2 * q + 1]));
                     const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-                    if (logits != nullptr) {
+                    if (logits != nullptr && e0 < a.logit_end) {
 #pragma unroll
                         for (int c = 0; c < 2; ++c)
 #pragma unroll

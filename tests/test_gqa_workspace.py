@@ -34,3 +34,12 @@ def test_copies_for_prompts_over_8_bits(lib):
     for B in (1, 16, 64):
         assert 0 <= size(lib, **PROMPT, B=B, max_len=2000) - B * 2048 * 8 * 128 * 4 < 16 << 20
     assert size(lib, **PROMPT, max_len=1 << 20) == size(lib, **PROMPT)
+
+
+def test_scores_for_weights(lib):
+    # a score for every row and entry, and a denominator a row
+    rows, room = 8 * 32, 2048 * 64
+    kw = dict(weights=4096, weight_stride=room)
+    assert size(lib, **kw) - size(lib) == rows * room * 4 + rows * 4
+    for n, entries in ((64, 64), (1000, 1024), (room - 1, room), (room, room), (1 << 30, room)):
+        assert size(lib, **kw, max_len=n) - size(lib, max_len=n) == rows * entries * 4 + rows * 4
