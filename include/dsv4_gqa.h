@@ -70,7 +70,10 @@ typedef struct Dsv4GqaParams {
     int32_t*       status;
 } Dsv4GqaParams;
 
-/* Follows from the sizes, window, first, max_len, q_start and weights being given, and the number of SMs. -1: not such sizes. */
+/*
+ * Follows from the sizes, kv_dtype, window, first, max_len, q's strides (whether they are 0: heads, tokens or requests that share their rows take other kernels), q_start and weights being
+ * given, and the number of SMs; of pointers nothing else is looked at. -1: not such sizes.
+ */
 int64_t dsv4_gqa_workspace_bytes(const Dsv4GqaParams* p);
 
 /* T tokens per request, q_start null: a decoding step, and the verification of a few drafted tokens. */

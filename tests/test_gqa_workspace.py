@@ -43,3 +43,24 @@ def test_scores_for_weights(lib):
     assert size(lib, **kw) - size(lib) == rows * room * 4 + rows * 4
     for n, entries in ((64, 64), (1000, 1024), (room - 1, room), (room, room), (1 << 30, room)):
         assert size(lib, **kw, max_len=n) - size(lib, max_len=n) == rows * entries * 4 + rows * 4
+
+
+@pytest.mark.parametrize("call", [dict(), dict(T=5, G=16, rows=40), dict(T=5, G=16, rows=40, kv_dtype=E4M3), PROMPT, dict(PROMPT, kv_dtype=BF16), dict(weights=4096, weight_stride=1 << 20)])
+def test_nothing_else(lib, call):
+    """What the header names, and no other field: buffers, scales, sink, factor, pool and status may follow later."""
+    n = size(lib, **call)
+    assert n > 0
+    later = dict(q=4096, k_pool=4096, v_pool=4096, block_table=4096, kv_len=4096, k_scale=4096, v_scale=4096, attn_sink=4096, out=4096, lse=4096, workspace=4096, workspace_bytes=1, status=4096,
+                 sm_scale=3.0, num_pages=1000, q_dtype=2, q_stride_t=8192, q_stride_h=256, q_stride_b=1 << 20)
+    for k, v in later.items():
+        assert size(lib, **{**call, k: v}) == n, k
+
+
+def test_types_and_strides_of_zero(lib):
+    assert size(lib, **PROMPT) > size(lib, **{**PROMPT, "kv_dtype": BF16})
+    # rows that are shared: other kernels, whose parts need room
+    prompt = {**PROMPT, "kv_dtype": BF16}
+    assert size(lib, **prompt, q_stride_t=0) > size(lib, **prompt) and size(lib, **prompt, q_stride_h=0) > size(lib, **prompt)
+    many = dict(T=5, G=16, rows=40)
+    assert len({size(lib, **many), size(lib, **many, q_stride_b=0)}) == 2
+    assert size(lib, **many, kv_dtype=E4M3) == size(lib, **many, kv_dtype=E4M3, q_stride_b=0)
