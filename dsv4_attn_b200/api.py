@@ -935,6 +935,8 @@ def kv_evict(pools, block_table, kv_len, page_refs, weights, keep, *, first=0, r
         _check(isinstance(t, torch.Tensor) and t.is_cuda and t.is_contiguous() and t.dim() >= 4 and t.numel() > 0, "a pool must be a contiguous cuda tensor [layers, pages, 64, ...]")
         _check(t.shape[1] == P and t.shape[2] == PAGE_ENTRIES and t.shape[0] == pools[0].shape[0], f"pools must be [layers, {P}, {PAGE_ENTRIES}, ...] with the same layers")
         _check(t[0, 0, 0].numel() * t.element_size() % 16 == 0, "the entries of a pool must be a multiple of 16 bytes")
+    at = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in pools)
+    _check(all(a[1] <= b[0] for a, b in zip(at, at[1:])), "pools must not overlap")
     _cuda_contig(weights, "weights", torch.float32, 2)
     _check(weights.shape[0] == B and weights.shape[1] >= cap, f"weights must be [B, >= max_pages * {PAGE_ENTRIES}]")
     if isinstance(keep, torch.Tensor):

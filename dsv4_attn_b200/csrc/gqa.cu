@@ -511,6 +511,12 @@ extern "C" int dsv4_kv_evict(const Dsv4KvEvictParams* p, void* stream_) {
         a.pool[i] = static_cast<uint4*>(p->pool[i]);
         a.vecs[i] = int(p->entry_bytes[i] / 16);
         vecs_of_all += p->layers * a.vecs[i];
+        // (a pool that is given twice would be moved twice, by blocks that do not know of one another)
+        const int64_t entries = p->layers * p->num_pages * 64;
+        for (int j = 0; j < i; ++j) {
+            const uint8_t *x = static_cast<const uint8_t*>(p->pool[i]), *y = static_cast<const uint8_t*>(p->pool[j]);
+            if (x < y + entries * p->entry_bytes[j] && y < x + entries * p->entry_bytes[i]) return int(cudaErrorInvalidValue);
+        }
     }
     // as wide columns as leave four blocks for every SM, from 512 bytes down to a sector; half of one where that leaves not even a block for each (one request, two layers: one step of loads
     // instead of two, 17.2 -> 14.7 us with the plan's)

@@ -837,6 +837,11 @@ PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
         p.pool[i] = ptr(t);
         p.entry_bytes[i] = int64_t(t->nbytes()) / (t->size(0) * t->size(1) * kPage);
         if (p.entry_bytes[i] % 16 != 0) return none();
+        for (int j = 0; j < i; ++j) {                             // (pools that overlap)
+            const auto *x = static_cast<const uint8_t*>(p.pool[i]), *y = static_cast<const uint8_t*>(p.pool[j]);
+            const int64_t entries = p.layers * refs->size(0) * kPage;
+            if (x < y + entries * p.entry_bytes[j] && y < x + entries * p.entry_bytes[i]) return none();
+        }
     }
     int64_t keep = 0, first, recent;
     if (PyLong_Check(a[5]) ? !integer(a[5], &keep) || keep < 0 || !fits32(keep) : (each = tensor(a[5], at::kInt, 1)) == nullptr || !has_shape(each, {B})) return none();

@@ -129,7 +129,7 @@ int dsv4_gqa_insert(const Dsv4GqaInsertParams* p, void* stream);
  * kept[b][i] is the old place of entry i, -1 behind the last; new_weights[b] the weights of the kept entries, 0 behind them; the other new_ arrays are
  * the old ones afterwards, and may be them.  Requests with keep entries or fewer stay as they are, and so do, reported, those with a page that would be written and is shared
  * (more than one reference: DSV4_STATUS_SHARED_PAGE) or one that is not in the pool.
- * Pools are [layers][num_pages][64][entry_bytes], entry_bytes a multiple of 16: K and V pages, and the latent cache's as well.  scratch: 4 * B + B * max_pages * 64 int32.
+ * Pools are [layers][num_pages][64][entry_bytes], entry_bytes a multiple of 16: K and V pages, and the latent cache's as well; no two of them may overlap.  scratch: 4 * B + B * max_pages * 64 int32.
  */
 #define DSV4_STATUS_SHARED_PAGE 12
 #define DSV4_EVICT_POOLS 4
