@@ -289,6 +289,8 @@ __device__ __forceinline__ float4 gqa_cluster_v4(uint32_t caddr) {
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(caddr) : "memory");
     return v;
 }
+// A sink's part of the denominator, in units of 2^ref, ref >= s: one that 32 bits hold as infinite leaves nothing to the entries.
+__device__ __forceinline__ float gqa_sink(float s, float ref) { return s == ref ? 1.f : ptx::ex2(s - ref); }
 // Four columns, from x on, of a complete row: v = sum of exp2(x_j - top) v_j, sum = sum of exp2(x_j - top).
 template <int D>
 __device__ __forceinline__ void gqa_write_row(const GqaArgs& a, int64_t token, int head, int64_t weight_row, int x, const float4& v, float top, float sum, float v_scale) {
@@ -299,7 +301,7 @@ __device__ __forceinline__ void gqa_write_row(const GqaArgs& a, int64_t token, i
         const float s = ptx::ld(a.sink + head) * 1.4426950408889634f;
         ref = fmaxf(top, s);
         by = ptx::ex2(top - ref);
-        all = sum * by + ptx::ex2(s - ref);
+        all = sum * by + gqa_sink(s, ref);
     }
     const float per = none ? 0.f : by * v_scale / all;
     const float o[4] = {v.x * per, v.y * per, v.z * per, v.w * per};

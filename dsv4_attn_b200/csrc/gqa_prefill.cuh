@@ -491,7 +491,7 @@ __global__ void __launch_bounds__(C::Threads, 1) gqa_prefill_kernel(const __grid
             if (mine && a.sink != nullptr && !none) {
                 const float s = ptx::ld(a.sink + head) * 1.4426950408889634f, top = fmaf(ref, scale, -kUp), m2 = fmaxf(top, s);
                 by = ptx::ex2(top - m2);
-                all = l * by + ptx::ex2(s - m2);
+                all = l * by + gqa_sink(s, m2);
             }
             const float per = none ? 0.f : by * (a.v_scale != nullptr ? ptx::ld(a.v_scale + w.h) : 1.f) / all;
             uint8_t* const to = static_cast<uint8_t*>(a.out) + row * (D * 2);
