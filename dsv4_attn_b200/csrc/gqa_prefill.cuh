@@ -547,7 +547,10 @@ __global__ void __launch_bounds__(kGqaUnpackThreads) gqa_unpack_kernel(const __g
     const int b = int(blockIdx.x / uint32_t(u.blocks));
     const GqaRequest r = gqa_request(a, b);
     if (r.tokens == 0) return;
-    const uint32_t head = uint32_t(u.D) / 16, vecs = head * kGqaTile * uint32_t(u.heads);       // 16-byte pieces of a head's row, and of a page's heads
+    // 16-byte pieces: 2^head_log2 of a head's row, `entry` of an entry's heads, of which a thread's next one is `entries` entries and `rest` pieces on
+    const uint32_t head_log2 = 31 - __clz(uint32_t(u.D) / 16), entry = uint32_t(u.heads) << head_log2, vecs = entry * kGqaTile, entries = kGqaUnpackThreads / entry, rest = kGqaUnpackThreads - entries * entry;
+    const uint32_t e0 = threadIdx.x / entry, at0 = threadIdx.x - e0 * entry;
+    const int64_t pool_entry = int64_t(a.Hkv) << head_log2;
     const int lo = a.window > 0 ? max(r.place0 - a.window + 1, 0) : 0, pages = min((r.entries + kGqaTile - 1) / kGqaTile, u.own_pages);
     for (int slot = int(blockIdx.x) - b * u.blocks; slot < pages; slot += u.blocks) {
         const int from = slot * kGqaTile;
@@ -556,13 +559,19 @@ __global__ void __launch_bounds__(kGqaUnpackThreads) gqa_unpack_kernel(const __g
         if (page < 0 || page >= a.num_pages) continue;
 #pragma unroll 1
         for (int kv = 0; kv < 2; ++kv) {
-            const uint4* const src = reinterpret_cast<const uint4*>(u.pool[kv]) + (int64_t(page) * kGqaTile * a.Hkv + u.h0) * head;
+            const uint4* const src = reinterpret_cast<const uint4*>(u.pool[kv]) + int64_t(page) * kGqaTile * pool_entry + (u.h0 << head_log2);
             uint4* const dst = reinterpret_cast<uint4*>(u.rows[kv]) + (int64_t(b) * u.own_pages + slot) * vecs * 2;
+            uint32_t e = e0, at = at0;
 #pragma unroll 4
             for (uint32_t i = threadIdx.x; i < vecs; i += kGqaUnpackThreads) {
-                const uint32_t row = i / head, e = row / uint32_t(u.heads), h = row - e * uint32_t(u.heads);
-                const uint4 v = ptx::ldg_stream_v4(src + (int64_t(e) * a.Hkv + h) * head + (i - row * head));
-                const uint32_t turn = kv == 0 && ptx::ld(a.k_scale + u.h0 + h) < 0.f ? 0x80008000u : 0u;
+                const uint4 v = ptx::ldg_stream_v4(src + e * pool_entry + at);
+                const uint32_t turn = kv == 0 && ptx::ld(a.k_scale + u.h0 + (at >> head_log2)) < 0.f ? 0x80008000u : 0u;
+                e += entries;
+                at += rest;
+                if (at >= entry) {
+                    at -= entry;
+                    ++e;
+                }
                 const uint32_t x[4] = {v.x, v.y, v.z, v.w};
                 uint32_t o[8];
 #pragma unroll
