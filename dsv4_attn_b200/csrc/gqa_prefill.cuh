@@ -3,7 +3,7 @@
 // A unit is (request, block of tokens, KV head): 128 rows a tile, row = (token, query head of the group), floor(128 / G) tokens each; two tiles a block (heads of 256: one).
 // It goes through the pages that some row sees, 64 entries a step:
 //     S = Q K^T               tcgen05.mma, M = 128, both operands in shared memory, S in tensor memory (two buffers a tile)
-//     P = exp2(c (S - ref))   in the softmax warps, a thread a row; back to tensor memory over S, in 16 bits
+//     P = exp2(c (S - ref))   in the softmax warps, a thread a row; back to tensor memory over S, in the queries' 16-bit type (FP16: times 2^7)
 //     O += P V                A = P from tensor memory, V as it lies in the cache (MN-major)
 // The scores of a step are computed while the softmax warps have those of the step before, and the two tiles take turns.  The reference of a row moves only when its maximum has
 // passed it by 2^8; then O is rescaled in tensor memory by the row's thread.  Units are listed by gqa_plan_kernel, those with most steps first, and dealt out to resident
@@ -11,7 +11,7 @@
 //
 // What bounds it, per step of two tiles with D = 128, in cycles of an SM: the tensor pipe 1280 (scores 48 an instruction, bound by their operands' way out of shared memory, outputs 64),
 // the 16,384 exponentials 1024.  A step takes 1800, of which a softmax warp spends 1100 in exponentials, two warps a scheduler; and from some 20 ms on the power limit holds the clock:
-// 4,096 tokens behind 12,288 in 0.91 ms for the first calls after a pause, 0.99 under load, 0.97 PFLOP/s (the library's products: 1.42).  Measured and taken back: steps of 128 entries with
+// 4,096 tokens behind 12,288 in 0.91 ms for the first calls after a pause, 0.99-1.02 under load, 0.94-0.97 PFLOP/s (the library's products: 1.42).  Measured and taken back: steps of 128 entries with
 // one score buffer a tile, where scores, softmax and outputs of a tile follow one another (1.06 ms; a window of 1,024: 320 us against 275); one warp for all products (1.12: a look at a
 // barrier takes 130 to 210 cycles while products keep the shared memory busy); a quarter to a half of the exponentials as polynomials on the multiply-add pipe (0.995 to 1.03).
 //

@@ -5,12 +5,12 @@
 // share the first stream joins both parts and writes the output; of one that a cut runs through each stream leaves an FP32 part, and gqa_merge_kernel joins those of all blocks.
 //
 // An 8-bit cache's pages come into a ring of raw tiles; four warps bring them to FP16 (exact) in the operands' layout, zeros for V of entries that no row sees.  Q then is FP16
-// too, each row brought near 1 by a power of two.
+// too, each row brought near 1 by a power of two, and turned round where the head's scale is negative.
 //
 // Why not mma.sync with more rows: 64 rows x 64 entries x 128 are 512 instructions of m16n8k16, 1111 cycles at the measured 2.17 an instruction and SM, where an 8-bit page is there after
 // 700; and every warp of 16 rows converts the page for itself.  64 requests x 8,000 entries, 64 query heads for each of 8 KV heads of 128: 385 us against 670, in 8 bits 401 against 999.
 //
-// What bounds it: the shared-memory port with 8-bit pages (12 x 5 tokens of 64 heads behind 32,768 entries 289 us, of which the bytes need 125: 1,024 of a page's 1,275 cycles go to the raw page in
+// What bounds it: the shared-memory port with 8-bit pages (12 x 5 tokens of 64 heads behind 32,768 entries 277-291 us, of which the bytes need 125: 1,024 of a page's 1,275 cycles go to the raw page in
 // and out, the FP16 page in and out, and Q again for every page); DRAM with 16-bit ones.
 #pragma once
 

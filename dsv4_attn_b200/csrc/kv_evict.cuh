@@ -8,7 +8,8 @@
 //                       everything that later steps read, so that one barrier between a step's loads and its stores is all it takes.
 //
 // Bound by the bytes that move, each read and written once; the order of entries is worth that to a cache whose masks go by places.  Columns are as wide as
-// leaves four blocks for every SM, 32 bytes (a sector) at least.  24 requests of 4,608 entries to 4,096, eight layers: 680-800 us, 5.1-5.9 TB/s; one of 2,176 to 2,048, two layers: 15 us, the
+// leaves four blocks for every SM, 32 bytes (a sector) at least; 16 where that leaves not even one block for each (a sector is then fetched by two blocks, and a request's places take one step of
+// loads instead of two).  24 requests of 4,608 entries to 4,096, eight layers: 680-840 us, 4.8-5.9 TB/s; one of 2,176 to 2,048, two layers: 15 us, the
 // plan's chain 8 of them.
 #pragma once
 

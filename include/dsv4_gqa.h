@@ -28,6 +28,7 @@ extern "C" {
  * token stands at kv_len[b] - 1.  Query head n reads KV head n / G.  A token sees the entries j <= p, with window > 0 only those with p - j < window or
  * j < first.  out = softmax(sm_scale q.k [, sink]) v; the sink, a logit per head, adds to the denominator.  A token that sees nothing gives 0 and an lse of -inf (natural
  * logarithm, without the sink).  Entries that no token of the request sees may hold anything; those that some token of the call sees must be finite.
+ * Softmax weights are rounded to the type of V before they are multiplied (over e4m3 pages to FP16; in the prompts' kernel, which sizes choose, to q's type), all else is FP32.
  * Rows of q outside q_start[0] .. q_start[B] are left as they are in out and lse; offsets outside [0, rows] or that fall are clamped and reported.
  *
  * weights (tokens not packed): float [B][weight_stride], weight_stride >= max_pages * 64: to entry j of request b is added what it got from the call's tokens and heads,
